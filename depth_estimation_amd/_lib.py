@@ -75,6 +75,15 @@ _SIGNATURES = {
     "ds_depth_metrics": (_i, [_fp, _fp, _i, _i, _i, _fp, _fp, _fp, _sz, _fp]),
     "ds_depth_metrics_eps": (_i, [_fp, _fp, _i, _i, _i, _f32, _fp, _fp, _fp, _sz, _fp]),
     "ds_depth_metrics_noalloc": (_i, [_fp, _fp, _i, _i, _i, _fp, _fp, _fp]),
+    "ds_head_saved_bytes": (_sz, [_ll]),
+    "ds_linear_ce_workspace_bytes": (_sz, [_i, _ll, _i, _i, _ll, _i]),
+    "ds_linear_ce_fwd": (_i, [_fp, _ll, _fp, _fp, _i, _ll, _i, _i, _ll, _i, _fp, _fp, _fp, _sz, _fp]),
+    "ds_linear_ce_bwd": (_i, [_fp, _ll, _fp, _fp, _fp, _i, _ll, _i, _i, _ll, _i, _fp, _fp, _fp, _fp, _sz, _fp]),
+    "ds_bin_expect_workspace_bytes": (_sz, [_i, _ll, _i, _i, _ll, _i]),
+    "ds_bin_expect_fwd": (_i, [_fp, _ll, _fp, _fp, _i, _ll, _i, _i, _fp, _fp, _fp, _sz, _fp]),
+    "ds_bin_expect_bwd": (_i, [_fp, _ll, _fp, _fp, _fp, _i, _ll, _i, _i, _fp, _fp, _fp, _fp, _sz, _fp]),
+    "ds_orthogonalize_workspace_bytes": (_sz, [_i, _i, _i]),
+    "ds_orthogonalize": (_i, [_fp, _i, _i, _i, _i, _i, C.POINTER(C.c_double), C.c_double, _fp, _fp, _sz, _fp]),
 }
 
 EXPORTS = tuple(_SIGNATURES)
@@ -124,6 +133,21 @@ def dev_f32(t: torch.Tensor, name: str) -> torch.Tensor:
     if t.dtype != torch.float32:
         raise RuntimeError(f"{name}: expected float32, got {t.dtype}")
     return t.contiguous()
+
+
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # DS_F32, DS_F16, DS_BF16
+
+
+def dev_float(t: torch.Tensor, name: str) -> torch.Tensor:
+    """Validate a tensor for the kernels that take float32, float16 and bfloat16 (any strides)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name}: expected a tensor on the GPU (got device {t.device}); "
+                           "depth_estimation_amd has no CPU path")
+    if t.dtype not in DTYPES:
+        raise RuntimeError(f"{name}: expected float32, float16 or bfloat16, got {t.dtype}")
+    return t
 
 
 def same_device(*ts: torch.Tensor) -> None:

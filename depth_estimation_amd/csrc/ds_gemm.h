@@ -1,0 +1,230 @@
+// ds_gemm.h -- the matrix core shared by the classification head (ds_head.hip) and the matrix update (ds_ortho.hip).
+//
+// One workgroup forms a BM x BN tile of C[m][n] = sum_k A(m,k) B(n,k) with v_mfma_f32_16x16x32.  Either operand may be
+// stored with k contiguous (kK: row m of A holds its k values) or with m contiguous (kM: row k holds all m, i.e. the
+// transposed matrix), so that none of the products here needs a transposed copy: W serves logits = H W^T as kK and
+// dH = dL W as kM.  A kM tile lies in LDS as it lies in memory, and ds_read_b64_tr_b16 hands every lane the four k values of
+// its m (measured layout: lane 4r+c of a 16-lane group reads four values of row r, lane i receives rows 0..3 of column i).
+//
+// Numbers wider than 16 bits go through as two fp16 planes x = hi + lo (22 bits, after an exact power-of-two scale that the
+// caller keeps): SPLIT = 3 adds lo*hi + hi*lo + hi*hi into the same fp32 accumulators.  What is dropped, lo*lo, is 2^-22 of
+// the product.  Three 16-bit products cost a third of the 16-bit rate, still above the rate of fp32 matrix instructions
+// (1/16 of it).
+//
+// Rows and columns beyond an operand's bounds read as zero (buffer loads whose offset is out of range), so every size works
+// without padded copies; only the contiguous extent must be a multiple of 8 elements and 16-byte aligned.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include "ds_common.h"
+
+namespace ds {
+
+typedef _Float16 f16;
+typedef __bf16 bf16;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+__host__ __device__ constexpr int cdiv(int a, int b) { return (int)(((unsigned)a + (unsigned)b - 1) / (unsigned)b); }
+inline int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
+inline int cdiv(long long a, int b) { return cdiv(a, (long long)b); }
+inline int pad8(int x) { return (x + 7) & ~7; }
+inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+enum Lay { kK = 0, kM = 1 };   // which index of the operand is contiguous
+
+struct Operand {
+    const void* p;      // 16-bit elements, 16-byte aligned
+    long long ld;       // elements between stored rows, a multiple of 8
+    long long lo;       // elements from the hi plane to the lo plane (SPLIT = 3)
+    int outer;          // stored rows that exist
+    int inner;          // elements of a row that may be read, a multiple of 8 (what lies beyond the matrix must be zero)
+};
+
+__device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c, f16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c, bf16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+constexpr int kBK = 64;                 // k per step: 128 bytes of a kK row = 8 chunks of 16 bytes
+constexpr unsigned kOut = 0xfffffff0u;  // an offset beyond every descriptor: the load returns zero
+
+// a workgroup's shape: BM x BN outputs, WM x WN waves
+template <int BM_, int BN_, int WM_, int WN_>
+struct Shape {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, T = 64 * WM_ * WN_;
+    static constexpr int FM = BM_ / WM_ / 16, FN = BN_ / WN_ / 16;   // 16x16 fragments of a wave
+    static constexpr int kLds = 2 * (BM_ + BN_) * kBK * 2;           // two buffers
+};
+
+// byte offset of 16-byte chunk c of row r in an LDS tile.  kK: the eight chunks of a row trade places by the row's low bits,
+// so that the 16 rows of a ds_read_b128 spread over all banks.  kM: 32-byte granules trade places by those bits of k in which
+// the rows of one transposing read differ.
+template <Lay L, int R>
+__device__ __forceinline__ int lds_chunk(int r, int c) {
+    if (L == kK) return r * (kBK * 2) + ((c ^ (r & 7)) << 4);
+    const int swz = ((r & 3) | ((r >> 1) & 4)) & (R / 16 - 1);
+    return r * (R * 2) + (((((c >> 1) ^ swz) << 1) | (c & 1)) << 4);
+}
+
+// One operand's tile on its way from memory to LDS: R x 64 elements, N16 16-byte chunks per thread, staged in registers.
+template <Lay L, int R, int T>
+struct Stager {
+    static constexpr int N16 = R * kBK * 2 / 16 / T;
+    static constexpr int CPR = (L == kK ? kBK : R) / 8;              // chunks per stored row
+    i32x4 v[N16];
+
+    __device__ __forceinline__ void load(const Operand& o, int r0, int k0, bool lo, int tid) {
+        // descriptor at the tile's corner: 32-bit offsets stay small however large the matrix is
+        const long long corner = L == kK ? (long long)r0 * o.ld + k0 : (long long)k0 * o.ld + r0;
+        const rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<char*>(static_cast<const char*>(o.p) + 2 * (corner + (lo ? o.lo : 0))), 0, 0x7fffffff, 0x00020000);
+        const int outer0 = L == kK ? r0 : k0, inner0 = L == kK ? k0 : r0;
+#pragma unroll
+        for (int i = 0; i < N16; ++i) {
+            const int c = tid + i * T, r = c / CPR, cc = c % CPR;
+            const bool in = outer0 + r < o.outer && inner0 + cc * 8 < o.inner;
+            const unsigned off = in ? (unsigned)(r * (int)o.ld + cc * 8) * 2u : kOut;
+            v[i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0));
+        }
+    }
+    __device__ __forceinline__ void store(char* lds, int tid) const {
+#pragma unroll
+        for (int i = 0; i < N16; ++i) {
+            const int c = tid + i * T;
+            *reinterpret_cast<i32x4*>(lds + lds_chunk<L, R>(c / CPR, c % CPR)) = v[i];
+        }
+    }
+};
+
+// the fragment of 16 rows m0..m0+15 and 32 k (sub-step kk of the tile's two): lane l holds row l%16, k = 8*(l/16)..+7
+template <Lay L, int R>
+__device__ __forceinline__ s16x8 fragment(const char* lds, int m0, int kk, int lane) {
+    if (L == kK) return *reinterpret_cast<const s16x8*>(lds + lds_chunk<L, R>(m0 + (lane & 15), kk * 4 + (lane >> 4)));
+    const int k = kk * 32 + (lane >> 4) * 8 + ((lane >> 2) & 3);
+    typedef __attribute__((address_space(3))) s16x4* lp;
+    const char* a0 = lds + lds_chunk<L, R>(k, m0 / 8 + ((lane >> 1) & 1)) + (lane & 1) * 8;
+    const char* a1 = lds + lds_chunk<L, R>(k + 4, m0 / 8 + ((lane >> 1) & 1)) + (lane & 1) * 8;
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(a0));
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(a1));
+    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// acc[i][j][e]: C at m = m0 + wave's row + 16 i + 4 (lane / 16) + e, n = n0 + wave's column + 16 j + lane % 16, over k in
+// [kbeg, kend) (kbeg a multiple of 64).  `lds`: S::kLds bytes.  Ends behind a barrier: the caller may reuse `lds`.
+template <class T, class S, Lay LA, Lay LB, int SPLIT>
+__device__ __forceinline__ void gemm_tile(const Operand& A, const Operand& B, int m0, int n0, int kbeg, int kend, char* lds,
+                                          f32x4 (&acc)[S::FM][S::FN]) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wm = (wave / S::WN) * S::FM * 16, wn = (wave % S::WN) * S::FN * 16;
+    constexpr int kA = S::BM * kBK * 2, kBuf = (S::BM + S::BN) * kBK * 2;
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    Stager<LA, S::BM, S::T> sa;
+    Stager<LB, S::BN, S::T> sb;
+    const int steps = (kend - kbeg + kBK - 1) / kBK * SPLIT;
+    auto load = [&](int s) {
+        const int k0 = kbeg + s / SPLIT * kBK, ph = s % SPLIT;
+        sa.load(A, m0, k0, SPLIT == 3 && ph == 0, tid);
+        sb.load(B, n0, k0, SPLIT == 3 && ph == 1, tid);
+    };
+    if (steps > 0) {
+        load(0);
+        sa.store(lds, tid);
+        sb.store(lds + kA, tid);
+    }
+    __syncthreads();
+    for (int s = 0; s < steps; ++s) {
+        const char* buf = lds + (s & 1) * kBuf;
+        char* nxt = lds + ((s + 1) & 1) * kBuf;
+        const bool more = s + 1 < steps;
+        if (more) load(s + 1);
+#pragma unroll
+        for (int kk = 0; kk < kBK / 32; ++kk) {
+            s16x8 a[S::FM], b[S::FN];
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i) a[i] = fragment<LA, S::BM>(buf, wm + 16 * i, kk, lane);
+#pragma unroll
+            for (int j = 0; j < S::FN; ++j) b[j] = fragment<LB, S::BN>(buf + kA, wn + 16 * j, kk, lane);
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+                for (int j = 0; j < S::FN; ++j) acc[i][j] = mfma(a[i], b[j], acc[i][j], T());
+        }
+        if (more) {
+            sa.store(nxt, tid);
+            sb.store(nxt + kA, tid);
+        }
+        __syncthreads();
+    }
+}
+
+// x as two fp16 numbers: hi = x to 11 bits, lo = the rest to 11 bits.  Where hi is not finite lo is 0, so that an infinity
+// stays one instead of becoming inf - inf.
+__device__ __forceinline__ void split16(float x, f16& hi, f16& lo) {
+    hi = (f16)x;
+    const float h = (float)hi;
+    lo = __builtin_isfinite(h) ? (f16)(x - h) : (f16)0.f;
+}
+
+// four consecutive values to 16-bit storage, one or two planes
+template <int SPLIT>
+__device__ __forceinline__ void put4(f16* p, long long lo, const float (&v)[4]) {
+    f16x4 h, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (SPLIT == 3) {
+            f16 a, b;
+            split16(v[e], a, b);
+            h[e] = a;
+            l[e] = b;
+        } else {
+            h[e] = (f16)v[e];
+        }
+    }
+    *reinterpret_cast<f16x4*>(p) = h;
+    if (SPLIT == 3) *reinterpret_cast<f16x4*>(p + lo) = l;
+}
+template <int SPLIT>
+__device__ __forceinline__ void put4(bf16* p, long long, const float (&v)[4]) {
+    bf16x4 h;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = (bf16)v[e];
+    *reinterpret_cast<bf16x4*>(p) = h;
+}
+
+// up to four consecutive outputs of a row of `n` elements, at element c of the row; rows need no alignment
+template <class O>
+__device__ __forceinline__ void put_row4(O* row, int c, int n, const float (&v)[4], bool aligned) {
+    if (aligned && c + 4 <= n) {
+        typedef O o4 __attribute__((ext_vector_type(4)));
+        o4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = (O)v[e];
+        *reinterpret_cast<o4*>(row + c) = w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < n) row[c + e] = (O)v[e];
+    }
+}
+
+// the power of two that brings a largest magnitude `amax` into [2^14, 2^15): fp16 keeps a factor of two of headroom
+__device__ __forceinline__ float scale_for(float amax) {
+    if (!(amax > 0.f) || !__builtin_isfinite(amax)) return 1.f;
+    int e = 14 - ilogbf(amax);
+    e = e > 60 ? 60 : (e < -110 ? -110 : e);
+    return ldexpf(1.f, e);
+}
+
+}  // namespace ds

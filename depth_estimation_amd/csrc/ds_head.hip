@@ -1,0 +1,894 @@
+// ds_head.hip -- a linear classification head over V classes (depth bins, a large vocabulary), without keeping its logits:
+// softmax cross entropy with its gradient (ds_linear_ce_*) and the expected bin centre under the softmax with its gradient
+// (ds_bin_expect_*).
+//
+//   l = H W^T (rows x classes)        lse_r = log sum_v exp l_rv
+//   cross entropy   loss_r = lse_r - l[r,t_r]      dl_rv = g_r (p_rv - [v = t_r])
+//   expectation     E_r = sum_v p_rv c_v           dl_rv = g_r p_rv (c_v - E_r)
+//   dH = dl W,  dW = dl^T H
+//
+// Forward: a workgroup forms a tile of l in registers and leaves three numbers per row and class tile (maximum, sum of
+// exponentials, sum of exponentials times centres); a second launch joins the tiles of a row.  Backward: per piece of the
+// classes, the tile is formed again, turned into dl with the saved maximum and sum and written once in 16 bits (two planes for fp32
+// inputs); the two products read it in place, one as kK, one as kM operand.
+//
+// Rows whose target is ignore_index take no part: the kept rows are listed first (in order, so results do not depend on
+// scheduling), everything after works on that list, and how long it is stays on the device.
+#include "ds_gemm.h"
+#include "ds_internal.h"
+#include "../../include/depthsynth.h"
+#include <type_traits>
+
+namespace ds {
+namespace {
+
+enum Mode { kCE = 0, kExpect = 1 };
+
+// What the forward leaves for the backward besides the softmax statistics: opaque to the caller.
+struct HeadState {
+    int count;           // rows kept
+    unsigned amax_h;     // bits of max |hidden| over kept rows, max |weight|: the scales of the fp16 planes (fp32 inputs)
+    unsigned amax_w;
+    int pad[13];
+};
+struct BackState {
+    unsigned gmax;       // bits of max |upstream| over kept rows
+    unsigned cmax;       // bits of max |centre|
+    int pad[14];
+};
+
+
+__device__ __forceinline__ float from_bits(unsigned u) { return __builtin_bit_cast(float, u); }
+
+// max over finite magnitudes: an infinity or a NaN in one place must not take the scale from all others
+__device__ __forceinline__ float finite_abs(float x) { return __builtin_isfinite(x) ? fabsf(x) : 0.f; }
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
+// ------------------------------------------------------------------------------------------------ kept rows, in order
+constexpr int kListT = 1024, kListPer = 16, kListBlock = kListT * kListPer;
+
+__global__ void head_init_kernel(HeadState* st, int rows) {
+    st->count = rows;
+    st->amax_h = 0;
+    st->amax_w = 0;
+}
+
+// rows kept per 16384 (only launched where one workgroup does not cover them all)
+__global__ __launch_bounds__(kListT) void count_rows_kernel(const long long* __restrict__ target, int n, long long ignore,
+                                                            int* __restrict__ counts) {
+    __shared__ int s[kListT / 64];
+    int c = 0;
+    for (int i = 0; i < kListPer; ++i) {
+        const long long r = (long long)blockIdx.x * kListBlock + i * kListT + threadIdx.x;
+        c += __popcll(__ballot(r < n && target[r < n ? r : 0] != ignore));
+    }
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = c;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int t = 0;
+        for (int i = 0; i < kListT / 64; ++i) t += s[i];
+        counts[blockIdx.x] = t;
+    }
+}
+
+// rows[j] = j-th kept row, tgt[j] = its class (-1 where it is none of 0..V-1: its loss is NaN); each_loss (may be NULL) of
+// the others is 0
+__global__ __launch_bounds__(kListT) void list_rows_kernel(const long long* __restrict__ target, int n, int V, long long ignore,
+                                                           const int* __restrict__ counts, HeadState* __restrict__ st,
+                                                           int* __restrict__ rows, int* __restrict__ tgt,
+                                                           float* __restrict__ each_loss) {
+    constexpr int kW = kListT / 64;
+    __shared__ int s[kListPer * kW + 1];
+    __shared__ int before;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (threadIdx.x == 0) before = 0;
+    __syncthreads();
+    if (blockIdx.x > 0) {   // integer sums: any order gives the same
+        int c = 0;
+        for (int i = threadIdx.x; i < (int)blockIdx.x; i += kListT) c += counts[i];
+        if (c) atomicAdd(&before, c);
+    }
+    const long long base = (long long)blockIdx.x * kListBlock;
+    long long t[kListPer];
+    unsigned long long m[kListPer];
+#pragma unroll
+    for (int i = 0; i < kListPer; ++i) {
+        const long long r = base + i * kListT + threadIdx.x;
+        t[i] = r < n ? target[r] : ignore;
+        m[i] = __ballot(t[i] != ignore);
+        if (lane == 0) s[i * kW + wave] = __popcll(m[i]);
+    }
+    __syncthreads();
+    if (wave == 0) {   // exclusive prefix over the 256 counts, four a lane
+        int v[4], sum = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] = s[lane * 4 + e];
+            sum += v[e];
+        }
+        int inc = sum;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(inc, o, 64);
+            if (lane >= o) inc += u;
+        }
+        int ex = inc - sum;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            s[lane * 4 + e] = ex;
+            ex += v[e];
+        }
+        if (lane == 63) s[kListPer * kW] = ex;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kListPer; ++i) {
+        const long long r = base + i * kListT + threadIdx.x;
+        if (t[i] != ignore) {
+            const int j = before + s[i * kW + wave] + __popcll(m[i] & ((1ull << lane) - 1));
+            rows[j] = (int)r;
+            tgt[j] = t[i] >= 0 && t[i] < V ? (int)t[i] : -1;
+        } else if (r < n && each_loss) {
+            each_loss[r] = 0.f;
+        }
+    }
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
+        st->count = before + s[kListPer * kW];
+        st->amax_h = 0;
+        st->amax_w = 0;
+    }
+}
+static_assert(kListPer * kListT / 64 == 256, "the prefix handles four counts a lane");
+
+// --------------------------------------------------------------------------------------------------- staged operands
+// max |x| over `cnt` rows (listed in `rows` if given); order-independent, so repeatable
+template <class IT>
+__global__ __launch_bounds__(256) void amax_kernel(const IT* __restrict__ x, long long ld, const int* __restrict__ rows,
+                                                   const int* __restrict__ cnt, int n, int D, unsigned* __restrict__ out) {
+    const int c = cnt ? *cnt : n;
+    float m = 0.f;
+    const int lane = threadIdx.x & 63;
+    for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < c; r += gridDim.x * 4) {
+        const IT* p = x + (rows ? rows[r] : r) * ld;
+        for (int d = lane; d < D; d += 64) m = fmaxf(m, finite_abs((float)p[d]));
+    }
+    m = wave_max(m);
+    if (lane == 0 && m > 0.f) atomicMax(out, __builtin_bit_cast(unsigned, m));
+}
+
+// rows of x (listed in `rows` if given) packed with a row pitch of Dp elements, zero behind D; fp32 as two scaled fp16 planes
+template <class IT, class T, int SPLIT>
+__global__ __launch_bounds__(256) void stage_kernel(const IT* __restrict__ x, long long ld, const int* __restrict__ rows,
+                                                    const int* __restrict__ cnt, int n, int D, int Dp,
+                                                    const unsigned* __restrict__ amax, T* __restrict__ y, long long lo) {
+    const int c = cnt ? *cnt : n;
+    const int lane = threadIdx.x & 63;
+    const float scale = SPLIT == 3 ? scale_for(from_bits(*amax)) : 1.f;
+    for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < c; r += gridDim.x * 4) {
+        const IT* p = x + (rows ? rows[r] : r) * ld;
+        T* q = y + (long long)r * Dp;
+        for (int d = lane; d < Dp; d += 64) {
+            if constexpr (SPLIT == 3) {
+                f16 h, l;
+                split16(d < D ? (float)p[d] * scale : 0.f, h, l);
+                q[d] = h;
+                q[d + lo] = l;
+            } else {
+                q[d] = d < D ? p[d] : (IT)0.f;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------ forward
+template <int SPLIT>
+__device__ __forceinline__ float logit_of(float acc, float ih, float iw) {
+    return SPLIT == 3 ? acc * ih * iw : acc;
+}
+
+// One tile of l^T: classes along m, rows along n, so that a lane holds 4 FM classes of FN rows and most of the softmax stays
+// inside it.  part: three planes [class tile][row].
+template <class T, class S, int SPLIT>
+__global__ __launch_bounds__(S::T) void head_stats_kernel(Operand W, Operand H, const HeadState* __restrict__ st, int V, int D,
+                                                          int mode, const int* __restrict__ tgt,
+                                                          const float* __restrict__ centers, float* __restrict__ tlogit,
+                                                          float* __restrict__ part, long long plane, int ld_part) {
+    __shared__ __align__(16) char lds[S::kLds];
+    const int vt = cdiv(V, S::BM);
+    const int m0 = (int)(blockIdx.x % vt) * S::BM, n0 = (int)(blockIdx.x / vt) * S::BN;
+    const int cnt = st->count;
+    if (n0 >= cnt) return;
+    H.outer = cnt;
+    f32x4 acc[S::FM][S::FN];
+    gemm_tile<T, S, kK, kK, SPLIT>(W, H, m0, n0, 0, D, lds, acc);
+    const float ih = SPLIT == 3 ? 1.f / scale_for(from_bits(st->amax_h)) : 1.f;
+    const float iw = SPLIT == 3 ? 1.f / scale_for(from_bits(st->amax_w)) : 1.f;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wm = wave / S::WN, wn = wave % S::WN;
+    float* red = reinterpret_cast<float*>(lds);   // [WM][BN][3]
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) {
+        const int nl = (wn * S::FN + j) * 16 + (lane & 15), n = n0 + nl;
+        const int t = mode == kCE && n < cnt ? tgt[n] : -1;
+        float mx = -INFINITY, s = 0.f, sc = 0.f;
+#pragma unroll
+        for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int v = m0 + (wm * S::FM + i) * 16 + (lane >> 4) * 4 + e;
+                const float l = logit_of<SPLIT>(acc[i][j][e], ih, iw);
+                if (v == t) tlogit[n] = l;
+                // a comparison, not fmaxf: a NaN has to reach the row's sum
+                if (v < V && !(l <= mx)) mx = l;
+                acc[i][j][e] = l;
+            }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+#pragma unroll
+        for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int v = m0 + (wm * S::FM + i) * 16 + (lane >> 4) * 4 + e;
+                const float x = v < V ? __expf(acc[i][j][e] - (mx == -INFINITY ? 0.f : mx)) : 0.f;
+                s += x;
+                if (mode == kExpect && v < V) sc = fmaf(x, centers[v], sc);
+            }
+        s += __shfl_xor(s, 16, 64);
+        s += __shfl_xor(s, 32, 64);
+        sc += __shfl_xor(sc, 16, 64);
+        sc += __shfl_xor(sc, 32, 64);
+        if (lane < 16) {
+            float* q = red + (wm * S::BN + nl) * 3;
+            q[0] = mx;
+            q[1] = s;
+            q[2] = sc;
+        }
+    }
+    __syncthreads();
+    for (int nl = threadIdx.x; nl < S::BN; nl += S::T) {
+        if (n0 + nl >= cnt) break;
+        float mx = -INFINITY, s = 0.f, sc = 0.f;
+#pragma unroll
+        for (int w = 0; w < S::WM; ++w) mx = fmaxf(mx, red[(w * S::BN + nl) * 3]);
+        const float ref = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+        for (int w = 0; w < S::WM; ++w) {
+            const float* q = red + (w * S::BN + nl) * 3;
+            const float f = __expf(q[0] - ref);
+            s += q[1] * f;
+            sc += q[2] * f;
+        }
+        float* q = part + (long long)(m0 / S::BM) * ld_part + n0 + nl;
+        q[0] = mx;
+        q[plane] = s;
+        if (mode == kExpect) q[2 * plane] = sc;
+    }
+}
+
+// joins the class tiles of a row: 32 rows x 8 lanes over the tiles
+__global__ __launch_bounds__(256) void head_join_kernel(const float* __restrict__ part, long long plane, int ld_part, int tiles,
+                                                        const HeadState* __restrict__ st, int mode,
+                                                        const int* __restrict__ rows, const int* __restrict__ tgt,
+                                                        const float* __restrict__ tlogit, float* __restrict__ top,
+                                                        float* __restrict__ inv_sum, float* __restrict__ mean,
+                                                        float* __restrict__ out, double* __restrict__ sums) {
+    __shared__ float red[8][32][3];
+    __shared__ double tot[32];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5, n = blockIdx.x * 32 + x;
+    const int cnt = st->count;
+    float mx = -INFINITY, s = 0.f, sc = 0.f;
+    if (n < cnt)
+        for (int t = y; t < tiles; t += 8) {
+            const float* q = part + (long long)t * ld_part + n;
+            const float m = q[0], nm = fmaxf(mx, m), ref = nm == -INFINITY ? 0.f : nm;
+            const float f0 = __expf(mx - ref), f1 = __expf(m - ref);
+            s = s * f0 + q[plane] * f1;
+            if (mode == kExpect) sc = sc * f0 + q[2 * plane] * f1;
+            mx = nm;
+        }
+    red[y][x][0] = mx;
+    red[y][x][1] = s;
+    red[y][x][2] = sc;
+    __syncthreads();
+    if (y == 0) {
+        double loss = 0.0;
+        if (n < cnt) {
+            mx = red[0][x][0];
+            for (int i = 1; i < 8; ++i) mx = fmaxf(mx, red[i][x][0]);
+            const float ref = mx == -INFINITY ? 0.f : mx;
+            s = sc = 0.f;
+            for (int i = 0; i < 8; ++i) {
+                const float f = __expf(red[i][x][0] - ref);
+                s += red[i][x][1] * f;
+                sc += red[i][x][2] * f;
+            }
+            top[n] = ref;
+            inv_sum[n] = 1.f / s;
+            if (mode == kExpect) {
+                out[n] = mean[n] = sc / s;
+            } else {
+                const float each = tgt[n] < 0 ? __builtin_nanf("") : (ref - tlogit[n]) + logf(s);
+                if (sums)
+                    loss = each;
+                else
+                    out[rows[n]] = each;
+            }
+        }
+        tot[x] = loss;
+    }
+    if (!sums) return;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double a = 0.0;
+        for (int i = 0; i < 32; ++i) a += tot[i];
+        sums[blockIdx.x] = a;
+    }
+}
+
+// the sum (mean) of the rows' losses, in a fixed order
+__global__ __launch_bounds__(256) void loss_total_kernel(const double* __restrict__ sums, const HeadState* __restrict__ st,
+                                                         int mean, float* __restrict__ out) {
+    __shared__ double s[256];
+    const int cnt = st->count, nb = (cnt + 31) / 32;
+    double a = 0.0;
+    for (int i = threadIdx.x; i < nb; i += 256) a += sums[i];
+    s[threadIdx.x] = a;
+    __syncthreads();
+    for (int o = 128; o > 0; o >>= 1) {
+        if ((int)threadIdx.x < o) s[threadIdx.x] += s[threadIdx.x + o];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) out[0] = (float)(mean ? s[0] / cnt : s[0]);
+}
+
+// ----------------------------------------------------------------------------------------------------------- backward
+// How dl is scaled: fp16 storage wants values of a fixed size, so dl is kept as dl / |g|max (a power of two >= the largest
+// upstream value, times 2 |c|max for the expectation) * 2^14; bf16 has fp32's range and takes the same with 2^0.
+template <class T> struct Store;
+template <> struct Store<f16> { static constexpr float k = 16384.f; };
+template <> struct Store<bf16> { static constexpr float k = 1.f; };
+
+__device__ __forceinline__ float pow2_above(float x) {
+    if (!(x > 0.f) || !__builtin_isfinite(x)) return 1.f;
+    int e = ilogbf(x) + 1;
+    e = e > 120 ? 120 : (e < -120 ? -120 : e);
+    return ldexpf(1.f, e);
+}
+struct Upstream {
+    const float* g;      // one value, or one per row of the caller
+    int each, mean;
+    const int* rows;     // caller's row of a kept row (NULL: the same)
+};
+__device__ __forceinline__ float upstream(const Upstream& u, int n, int cnt) {
+    if (u.each) return u.g[u.rows ? u.rows[n] : n];
+    return u.mean ? u.g[0] / cnt : u.g[0];
+}
+__device__ __forceinline__ float dl_norm(const BackState* bs, int mode) {
+    const float g = pow2_above(from_bits(bs->gmax));
+    return mode == kExpect ? g * pow2_above(2.f * from_bits(bs->cmax)) : g;
+}
+
+// largest |upstream| and |centre|; *bs zeroed by back_init_kernel before
+__global__ void back_init_kernel(BackState* bs) { bs->gmax = bs->cmax = 0; }
+__global__ __launch_bounds__(256) void back_scale_kernel(Upstream u, const HeadState* __restrict__ st,
+                                                         const float* __restrict__ centers, int V, BackState* __restrict__ bs) {
+    const int cnt = st->count, step = gridDim.x * 256, i0 = blockIdx.x * 256 + threadIdx.x;
+    float g = 0.f, c = 0.f;
+    for (int n = i0; n < (u.each ? cnt : min(cnt, 1)); n += step) g = fmaxf(g, finite_abs(upstream(u, n, cnt)));
+    if (centers)
+        for (int v = i0; v < V; v += step) c = fmaxf(c, finite_abs(centers[v]));
+    g = wave_max(g);
+    c = wave_max(c);
+    if ((threadIdx.x & 63) == 0) {
+        if (g > 0.f) atomicMax(&bs->gmax, __builtin_bit_cast(unsigned, g));
+        if (c > 0.f) atomicMax(&bs->cmax, __builtin_bit_cast(unsigned, c));
+    }
+}
+
+// dl of classes [v0, v0 + cols) in 16 bits: [row][class - v0], pitch ld (cols rounded up to 8; zeros behind the last class).
+// The rounding to 16 bits is the products' operand rounding: half a step of the gradients' own type for 16-bit inputs, 2^-22
+// with the two planes of fp32 inputs; p - 1 and c - E are formed in fp32 before it.
+template <class T, class S, int SPLIT>
+__global__ __launch_bounds__(S::T) void head_dl_kernel(Operand W, Operand H, const HeadState* __restrict__ st,
+                                                       const BackState* __restrict__ bs, int V, int D, int v0, int cols, int mode,
+                                                       const int* __restrict__ tgt, const float* __restrict__ centers,
+                                                       const float* __restrict__ top, const float* __restrict__ inv_sum,
+                                                       const float* __restrict__ mean, Upstream up, T* __restrict__ dl, int ld, long long lo) {
+    __shared__ __align__(16) char lds[S::kLds];
+    const int vt = cdiv(cols, S::BM);
+    const int m0 = (int)(blockIdx.x % vt) * S::BM, n0 = (int)(blockIdx.x / vt) * S::BN;
+    const int cnt = st->count;
+    if (n0 >= cnt) return;
+    H.outer = cnt;
+    f32x4 acc[S::FM][S::FN];
+    gemm_tile<T, S, kK, kK, SPLIT>(W, H, v0 + m0, n0, 0, D, lds, acc);
+    const float ih = SPLIT == 3 ? 1.f / scale_for(from_bits(st->amax_h)) : 1.f;
+    const float iw = SPLIT == 3 ? 1.f / scale_for(from_bits(st->amax_w)) : 1.f;
+    const float norm = Store<T>::k / dl_norm(bs, mode);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wm = wave / S::WN, wn = wave % S::WN;
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) {
+        const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
+        if (n >= cnt) continue;
+        const float tp = top[n], rs = inv_sum[n];
+        const int t = mode == kCE ? tgt[n] : -1;
+        float g = upstream(up, n, cnt) * norm;
+        if (mode == kCE && t < 0) g = __builtin_nanf("");
+        const float e0 = mode == kExpect ? mean[n] : 0.f;
+#pragma unroll
+        for (int i = 0; i < S::FM; ++i) {
+            const int c = m0 + (wm * S::FM + i) * 16 + (lane >> 4) * 4;
+            if (c >= ld) continue;
+            float d[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int v = v0 + c + e;
+                const float p = __expf(logit_of<SPLIT>(acc[i][j][e], ih, iw) - tp) * rs;
+                const float q = mode == kExpect ? p * (v < V ? centers[v] - e0 : 0.f) : p - (v == t ? 1.f : 0.f);
+                d[e] = v < V && c + e < cols ? q * g : 0.f;
+            }
+            put4<SPLIT>(dl + (long long)n * ld + c, lo, d);
+        }
+    }
+}
+
+// dH = dl W: features along m (W as kM operand, classes are k), rows along n.  ACC: fp32 partials [split][row][Dp4], added to
+// what earlier pieces of the classes left; otherwise straight into the caller's rows.
+template <class T, class S, int SPLIT, class O, bool ACC>
+__global__ __launch_bounds__(S::T) void head_dh_kernel(Operand W, Operand G, const HeadState* __restrict__ st,
+                                                       const BackState* __restrict__ bs, int D, int kcols, int splits, int mode,
+                                                       const int* __restrict__ rows, O* __restrict__ out, float* __restrict__ part,
+                                                       long long part_split, int first) {
+    __shared__ __align__(16) char lds[S::kLds];
+    const int mt = cdiv(D, S::BM);
+    const int b = (int)(blockIdx.x / splits), sp = (int)(blockIdx.x % splits);
+    const int m0 = b % mt * S::BM, n0 = b / mt * S::BN;
+    const int cnt = st->count;
+    if (n0 >= cnt) return;
+    G.outer = cnt;
+    const int per = cdiv(cdiv(kcols, kBK), splits) * kBK, k0 = min(sp * per, kcols), k1 = min(k0 + per, kcols);
+    f32x4 acc[S::FM][S::FN];
+    gemm_tile<T, S, kM, kK, SPLIT>(W, G, m0, n0, k0, k1, lds, acc);
+    const float f0 = dl_norm(bs, mode) / Store<T>::k;
+    const float iw = SPLIT == 3 ? 1.f / scale_for(from_bits(st->amax_w)) : 1.f;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wm = wave / S::WN, wn = wave % S::WN, Dp = (D + 3) & ~3;
+    const bool aligned = (D & 3) == 0;
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) {
+        const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
+        if (n >= cnt) continue;
+        const long long row = ACC ? n : (rows ? rows[n] : n);
+#pragma unroll
+        for (int i = 0; i < S::FM; ++i) {
+            const int d = m0 + (wm * S::FM + i) * 16 + (lane >> 4) * 4;
+            if (d >= D) continue;
+            if (ACC) {
+                f32x4* q = reinterpret_cast<f32x4*>(part + sp * part_split + row * Dp + d);
+                f32x4 v = acc[i][j];
+                if (!first) v += *q;
+                *q = v;
+            } else {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * f0 * iw;
+                put_row4(out + row * D, d, D, v, aligned);
+            }
+        }
+    }
+}
+
+// dW of one piece = dl^T H: features along m, classes along n, k = rows (both kM operands)
+template <class T, class S, int SPLIT, class O, bool ACC>
+__global__ __launch_bounds__(S::T) void head_dw_kernel(Operand H, Operand G, const HeadState* __restrict__ st,
+                                                       const BackState* __restrict__ bs, int D, int cols, int splits, int mode,
+                                                       O* __restrict__ out, float* __restrict__ part, long long part_split) {
+    __shared__ __align__(16) char lds[S::kLds];
+    const int mt = cdiv(D, S::BM);
+    const int b = (int)(blockIdx.x / splits), sp = (int)(blockIdx.x % splits);
+    const int m0 = b % mt * S::BM, n0 = b / mt * S::BN;
+    const int cnt = st->count;
+    H.outer = G.outer = cnt;
+    const int per = cdiv(cdiv(cnt, kBK), splits) * kBK, k0 = min(sp * per, cnt), k1 = min(k0 + per, cnt);
+    f32x4 acc[S::FM][S::FN];
+    gemm_tile<T, S, kM, kM, SPLIT>(H, G, m0, n0, k0, k1, lds, acc);
+    const float f0 = dl_norm(bs, mode) / Store<T>::k;
+    const float ih = SPLIT == 3 ? 1.f / scale_for(from_bits(st->amax_h)) : 1.f;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wm = wave / S::WN, wn = wave % S::WN, Dp = (D + 3) & ~3;
+    const bool aligned = (D & 3) == 0;
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) {
+        const int c = n0 + (wn * S::FN + j) * 16 + (lane & 15);
+        if (c >= cols) continue;
+#pragma unroll
+        for (int i = 0; i < S::FM; ++i) {
+            const int d = m0 + (wm * S::FM + i) * 16 + (lane >> 4) * 4;
+            if (d >= D) continue;
+            if (ACC) {
+                *reinterpret_cast<f32x4*>(part + sp * part_split + (long long)c * Dp + d) = acc[i][j];
+            } else {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * f0 * ih;
+                put_row4(out + (long long)c * D, d, D, v, aligned);
+            }
+        }
+    }
+}
+
+// sums the splits of a product in order, scales, and writes rows of the caller.  which: 0 = dH, 1 = dW
+template <class T, int SPLIT, class O>
+__global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__ part, long long part_split, int splits,
+                                                       const HeadState* __restrict__ st, const BackState* __restrict__ bs, int n,
+                                                       int D, int mode, int which, const int* __restrict__ rows,
+                                                       O* __restrict__ out) {
+    const int cnt = which == 0 ? st->count : n, Dp = (D + 3) & ~3, q = Dp / 4;
+    const float f0 = dl_norm(bs, mode) / Store<T>::k;
+    const float is = SPLIT == 3 ? 1.f / scale_for(from_bits(which == 0 ? st->amax_w : st->amax_h)) : 1.f;
+    const bool aligned = (D & 3) == 0;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < (long long)cnt * q; i += gridDim.x * 256ll) {
+        const long long r = i / q;
+        const int d = (int)(i % q) * 4;
+        f32x4 a = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < splits; ++s) a += *reinterpret_cast<const f32x4*>(part + s * part_split + r * Dp + d);
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = a[e] * f0 * is;
+        put_row4(out + (rows && which == 0 ? (long long)rows[r] : r) * D, d, D, v, aligned);
+    }
+}
+
+// rows that were left out have no gradient
+template <class O>
+__global__ __launch_bounds__(256) void zero_ignored_kernel(const long long* __restrict__ target, int n, long long ignore, int D,
+                                                           const HeadState* __restrict__ st, O* __restrict__ out) {
+    if (st->count == n) return;
+    const int lane = threadIdx.x & 63;
+    for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < n; r += gridDim.x * 4)
+        if (target[r] == ignore)
+            for (int d = lane; d < D; d += 64) out[(long long)r * D + d] = (O)0.f;
+}
+
+// ------------------------------------------------------------------------------------------------------------- host
+// Shapes: 128x128 outputs a workgroup, four waves of 64x64; 64 features or 32 rows have shapes of their own, whose idle
+// half would otherwise be computed and dropped.
+typedef Shape<128, 128, 2, 2> Sq;
+typedef Shape<64, 128, 1, 4> Flat;    // 64 along m
+typedef Shape<128, 32, 4, 1> Thin;    // 32 along n
+
+struct Saved {
+    HeadState* st;
+    float* top;        // a kept row's largest logit and 1 / sum exp(l - top): more exact than their join lse, whose last
+    float* inv_sum;    // bit is worth |lse| 2^-24 in every probability of the row
+    float* mean;
+    int* rows;
+    int* tgt;
+};
+size_t saved_bytes(long long N) { return align256(sizeof(HeadState)) + 5 * align256((size_t)N * 4); }
+Saved saved_of(void* p, long long N) {
+    char* c = static_cast<char*>(p);
+    Saved s;
+    s.st = reinterpret_cast<HeadState*>(c);
+    c += align256(sizeof(HeadState));
+    const size_t a = align256((size_t)N * 4);
+    s.top = reinterpret_cast<float*>(c);
+    s.inv_sum = reinterpret_cast<float*>(c + a);
+    s.mean = reinterpret_cast<float*>(c + 2 * a);
+    s.rows = reinterpret_cast<int*>(c + 3 * a);
+    s.tgt = reinterpret_cast<int*>(c + 4 * a);
+    return s;
+}
+
+struct Plan {
+    int dtype, planes, Dp, vt_fwd, piece, piece_ld, dh_splits, dw_splits;
+    bool stage_w, stage_h, dh_part;
+    bool thin, flat;
+    size_t staged_h, staged_w, counts, tlogit, part, sums, fwd_total;      // offsets of the forward's workspace
+    size_t bh, bw, bs, dl, dhp, dwp, bwd_total;                            // offsets of the backward's
+};
+
+int splits_for(long long tiles, long long steps) {
+    // enough workgroups for two a CU, no split shorter than four steps of 64
+    const long long want = cdiv(2ll * cu_count(), tiles > 0 ? tiles : 1), most = steps / 4;
+    long long s = want < most ? want : most;
+    return (int)(s < 1 ? 1 : (s > 256 ? 256 : s));
+}
+
+Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
+    Plan p;
+    p.dtype = dtype;
+    p.planes = dtype == DS_F32 ? 2 : 1;
+    p.Dp = pad8(D);
+    p.stage_w = dtype == DS_F32 || D % 8 != 0;
+    p.stage_h = mode == kCE || dtype == DS_F32 || D % 8 != 0 || ldh % 8 != 0;
+    p.thin = N <= 32;
+    p.flat = D <= 64;
+    const size_t el = 2 * p.planes;
+    const size_t h = p.stage_h ? align256((size_t)N * p.Dp * el) : 0, w = p.stage_w ? align256((size_t)V * p.Dp * el) : 0;
+    p.vt_fwd = cdiv(V, 128);
+    size_t o = 0;
+    p.staged_h = o; o += h;
+    p.staged_w = o; o += w;
+    p.counts = o; o += align256((size_t)cdiv(N, kListBlock) * 4);
+    p.tlogit = o; o += align256((size_t)N * 4);
+    p.part = o; o += 3 * align256((size_t)p.vt_fwd * N * 4);
+    p.sums = o; o += align256((size_t)cdiv(N, 32) * 8);
+    p.fwd_total = o;
+    // a piece of the classes: what fits 256 MB of dl, at least 1024 classes, a multiple of 128
+    const long long fit = (256ll << 20) / ((long long)el * N) / 128 * 128;
+    const long long piece = fit < 1024 ? 1024 : fit;
+    p.piece = piece >= V ? V : (int)piece;
+    p.piece_ld = pad8(p.piece);
+    const int bm = p.flat ? 64 : 128, bn = p.thin ? 32 : 128;
+    p.dh_splits = splits_for((long long)cdiv(D, bm) * cdiv(N, bn), cdiv(p.piece, kBK));
+    p.dw_splits = splits_for((long long)cdiv(D, bm) * cdiv(p.piece, 128), cdiv(N, kBK));
+    p.dh_part = p.dh_splits > 1 || p.piece < V;
+    const size_t D4 = (D + 3) & ~3;
+    o = 0;
+    p.bh = o; o += h;
+    p.bw = o; o += w;
+    p.bs = o; o += 256;
+    p.dl = o; o += align256((size_t)N * p.piece_ld * el);
+    p.dhp = o; o += p.dh_part ? align256((size_t)p.dh_splits * N * D4 * 4) : 0;
+    p.dwp = o; o += p.dw_splits > 1 ? align256((size_t)p.dw_splits * p.piece * D4 * 4) : 0;
+    p.bwd_total = o;
+    return p;
+}
+
+int check_sizes(int dtype, long long N, int D, int V, long long ldh) {
+    if (N <= 0 || D <= 0 || V <= 0 || ldh < D) return DS_ERR_INVALID_ARG;
+    if (dtype != DS_F32 && dtype != DS_F16 && dtype != DS_BF16) return DS_ERR_UNSUPPORTED;
+    if ((long long)cdiv(V, 128) * cdiv(N, 32) > (1ll << 30)) return DS_ERR_UNSUPPORTED;   // workgroups of one launch
+    if (N > DS_HEAD_MAX_ROWS || D > DS_HEAD_MAX_FEATURES || V > DS_HEAD_MAX_CLASSES) return DS_ERR_UNSUPPORTED;
+    return DS_OK;
+}
+
+int launched() {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? DS_OK : (int)e;
+}
+
+// inputs as matrix operands: in place, or staged into `ws`
+template <class IT, class T, int SPLIT>
+void operands(const Plan& p, const IT* hidden, long long ldh, const IT* weight, long long N, int D, int V, const Saved& s,
+              const int* rows, bool need_amax, char* wh, char* ww, Operand& H, Operand& W, hipStream_t q) {
+    const int gh = cdiv(N, 4) < 4096 ? cdiv(N, 4) : 4096, gw = cdiv(V, 4) < 4096 ? cdiv(V, 4) : 4096;
+    if (SPLIT == 3 && need_amax) {
+        amax_kernel<IT><<<gh < 1024 ? gh : 1024, 256, 0, q>>>(hidden, ldh, rows, &s.st->count, (int)N, D, &s.st->amax_h);
+        amax_kernel<IT><<<gw < 1024 ? gw : 1024, 256, 0, q>>>(weight, D, nullptr, nullptr, V, D, &s.st->amax_w);
+    }
+    H = Operand{hidden, ldh, 0, (int)N, D};
+    W = Operand{weight, D, 0, V, D};
+    if (p.stage_h) {
+        const long long lo = N * p.Dp;
+        stage_kernel<IT, T, SPLIT><<<gh, 256, 0, q>>>(hidden, ldh, rows, &s.st->count, (int)N, D, p.Dp, &s.st->amax_h,
+                                                      reinterpret_cast<T*>(wh), lo);
+        H = Operand{wh, p.Dp, lo, (int)N, p.Dp};
+    }
+    if (p.stage_w) {
+        const long long lo = (long long)V * p.Dp;
+        stage_kernel<IT, T, SPLIT><<<gw, 256, 0, q>>>(weight, D, nullptr, nullptr, V, D, p.Dp, &s.st->amax_w,
+                                                      reinterpret_cast<T*>(ww), lo);
+        W = Operand{ww, p.Dp, lo, V, p.Dp};
+    }
+}
+
+template <class IT, class T, int SPLIT>
+int head_fwd(int mode, const IT* hidden, long long ldh, const IT* weight, const long long* target, const float* centers,
+             long long N, int D, int V, long long ignore, int reduction, float* out, void* saved, char* ws, hipStream_t q) {
+    const Plan p = plan_of(mode, std::is_same<IT, float>::value ? DS_F32 : DS_F16, N, D, V, ldh);
+    const Saved s = saved_of(saved, N);
+    const int* rows = nullptr;
+    if (mode == kCE) {
+        const int nb = cdiv(N, kListBlock);
+        int* counts = reinterpret_cast<int*>(ws + p.counts);
+        if (nb > 1) count_rows_kernel<<<nb, kListT, 0, q>>>(target, (int)N, ignore, counts);
+        list_rows_kernel<<<nb, kListT, 0, q>>>(target, (int)N, V, ignore, counts, s.st, s.rows, s.tgt,
+                                               reduction == DS_REDUCE_NONE ? out : nullptr);
+        rows = s.rows;
+    } else {
+        head_init_kernel<<<1, 1, 0, q>>>(s.st, (int)N);
+    }
+    Operand H, W;
+    operands<IT, T, SPLIT>(p, hidden, ldh, weight, N, D, V, s, rows, true, ws + p.staged_h, ws + p.staged_w, H, W, q);
+    float* part = reinterpret_cast<float*>(ws + p.part);
+    float* tlogit = reinterpret_cast<float*>(ws + p.tlogit);
+    const long long plane = (long long)(align256((size_t)p.vt_fwd * N * 4) / 4);
+    if (p.thin)
+        head_stats_kernel<T, Thin, SPLIT><<<p.vt_fwd * cdiv(N, 32), Thin::T, 0, q>>>(W, H, s.st, V, D, mode, s.tgt, centers, tlogit,
+                                                                                part, plane, (int)N);
+    else
+        head_stats_kernel<T, Sq, SPLIT><<<p.vt_fwd * cdiv(N, 128), Sq::T, 0, q>>>(W, H, s.st, V, D, mode, s.tgt, centers, tlogit,
+                                                                             part, plane, (int)N);
+    double* sums = mode == kCE && reduction != DS_REDUCE_NONE ? reinterpret_cast<double*>(ws + p.sums) : nullptr;
+    head_join_kernel<<<cdiv(N, 32), 256, 0, q>>>(part, plane, (int)N, p.vt_fwd, s.st, mode, s.rows, s.tgt, tlogit, s.top,
+                                                 s.inv_sum, s.mean, out, sums);
+    if (sums) loss_total_kernel<<<1, 256, 0, q>>>(sums, s.st, reduction == DS_REDUCE_MEAN, out);
+    return launched();
+}
+
+template <class IT, class T, class S, int SPLIT>
+void dh_launch(const Plan& p, const Operand& W, const Operand& G, const Saved& s, const BackState* bs, long long N, int D,
+               int kcols, int mode, const int* rows, IT* out, float* part, int first, hipStream_t q) {
+    const int grid = cdiv(D, S::BM) * cdiv(N, S::BN) * p.dh_splits;
+    const long long ps = N * ((D + 3) & ~3);
+    if (p.dh_part)
+        head_dh_kernel<T, S, SPLIT, IT, true><<<grid, S::T, 0, q>>>(W, G, s.st, bs, D, kcols, p.dh_splits, mode, rows, out, part,
+                                                                    ps, first);
+    else
+        head_dh_kernel<T, S, SPLIT, IT, false><<<grid, S::T, 0, q>>>(W, G, s.st, bs, D, kcols, 1, mode, rows, out, part, ps, first);
+}
+template <class IT, class T, class S, int SPLIT>
+void dw_launch(const Plan& p, const Operand& H, const Operand& G, const Saved& s, const BackState* bs, int D, int cols, int mode,
+               IT* out, float* part, hipStream_t q) {
+    const int grid = cdiv(D, S::BM) * cdiv(cols, S::BN) * p.dw_splits;
+    const long long ps = (long long)p.piece * ((D + 3) & ~3);
+    if (p.dw_splits > 1)
+        head_dw_kernel<T, S, SPLIT, IT, true><<<grid, S::T, 0, q>>>(H, G, s.st, bs, D, cols, p.dw_splits, mode, out, part, ps);
+    else
+        head_dw_kernel<T, S, SPLIT, IT, false><<<grid, S::T, 0, q>>>(H, G, s.st, bs, D, cols, 1, mode, out, part, ps);
+}
+
+template <class IT, class T, int SPLIT>
+int head_bwd(int mode, const IT* hidden, long long ldh, const IT* weight, const long long* target, const float* centers,
+             const float* g, long long N, int D, int V, long long ignore, int reduction, void* saved, IT* g_hidden,
+             IT* g_weight, char* ws, hipStream_t q) {
+    const Plan p = plan_of(mode, std::is_same<IT, float>::value ? DS_F32 : DS_F16, N, D, V, ldh);
+    const Saved s = saved_of(saved, N);
+    const int* rows = mode == kCE ? s.rows : nullptr;
+    BackState* bs = reinterpret_cast<BackState*>(ws + p.bs);
+    Upstream up{g, reduction == DS_REDUCE_NONE, reduction == DS_REDUCE_MEAN, rows};
+    back_init_kernel<<<1, 1, 0, q>>>(bs);
+    const long long most = (up.each && N > V) ? N : V;
+    back_scale_kernel<<<cdiv(most, 2048) < 256 ? cdiv(most, 2048) : 256, 256, 0, q>>>(up, s.st, centers, V, bs);
+    Operand H, W;
+    operands<IT, T, SPLIT>(p, hidden, ldh, weight, N, D, V, s, rows, false, ws + p.bh, ws + p.bw, H, W, q);
+    if (mode == kCE && g_hidden)
+        zero_ignored_kernel<IT><<<cdiv(N, 4) < 8192 ? cdiv(N, 4) : 8192, 256, 0, q>>>(target, (int)N, ignore, D, s.st, g_hidden);
+    T* dl = reinterpret_cast<T*>(ws + p.dl);
+    float* dhp = reinterpret_cast<float*>(ws + p.dhp);
+    float* dwp = reinterpret_cast<float*>(ws + p.dwp);
+    const long long lo = N * p.piece_ld;
+    const int D4 = (D + 3) & ~3;
+    for (int v0 = 0; v0 < V; v0 += p.piece) {
+        const int cols = V - v0 < p.piece ? V - v0 : p.piece, ld = pad8(cols);
+        if (p.thin)
+            head_dl_kernel<T, Thin, SPLIT><<<cdiv(cols, 128) * cdiv(N, 32), Thin::T, 0, q>>>(
+                W, H, s.st, bs, V, D, v0, cols, mode, s.tgt, centers, s.top, s.inv_sum, s.mean, up, dl, ld, lo);
+        else
+            head_dl_kernel<T, Sq, SPLIT><<<cdiv(cols, 128) * cdiv(N, 128), Sq::T, 0, q>>>(
+                W, H, s.st, bs, V, D, v0, cols, mode, s.tgt, centers, s.top, s.inv_sum, s.mean, up, dl, ld, lo);
+        const Operand G{dl, ld, lo, (int)N, ld};
+        if (g_hidden) {
+            Operand Wp = W;   // classes [v0, v0 + cols) as stored rows
+            Wp.p = static_cast<const T*>(W.p) + (long long)v0 * W.ld;
+            Wp.outer = cols;
+            if (p.thin)
+                dh_launch<IT, T, Thin, SPLIT>(p, Wp, G, s, bs, N, D, cols, mode, rows, g_hidden, dhp, v0 == 0, q);
+            else if (p.flat)
+                dh_launch<IT, T, Flat, SPLIT>(p, Wp, G, s, bs, N, D, cols, mode, rows, g_hidden, dhp, v0 == 0, q);
+            else
+                dh_launch<IT, T, Sq, SPLIT>(p, Wp, G, s, bs, N, D, cols, mode, rows, g_hidden, dhp, v0 == 0, q);
+        }
+        if (g_weight) {
+            IT* gw = g_weight + (long long)v0 * D;
+            if (p.flat)
+                dw_launch<IT, T, Flat, SPLIT>(p, H, G, s, bs, D, cols, mode, gw, dwp, q);
+            else
+                dw_launch<IT, T, Sq, SPLIT>(p, H, G, s, bs, D, cols, mode, gw, dwp, q);
+            if (p.dw_splits > 1)
+                head_sum_kernel<T, SPLIT, IT><<<cdiv((long long)cols * D4 / 4, 256), 256, 0, q>>>(
+                    dwp, (long long)p.piece * D4, p.dw_splits, s.st, bs, cols, D, mode, 1, nullptr, gw);
+        }
+    }
+    if (g_hidden && p.dh_part) {
+        const int blocks = cdiv(N * (D4 / 4), 256);
+        head_sum_kernel<T, SPLIT, IT><<<blocks < 16384 ? blocks : 16384, 256, 0, q>>>(dhp, N * D4, p.dh_splits, s.st, bs, (int)N, D,
+                                                                                      mode, 0, rows, g_hidden);
+    }
+    return launched();
+}
+
+bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+
+template <class F32, class F16, class BF16>
+int by_type(int dtype, F32 f32, F16 h, BF16 b) {
+    return dtype == DS_F32 ? f32() : dtype == DS_F16 ? h() : b();
+}
+
+int fwd_any(int mode, const void* hidden, long long ldh, const void* weight, const long long* target, const float* centers,
+            int dtype, long long N, int D, int V, long long ignore, int reduction, float* out, void* saved, void* ws,
+            size_t bytes, void* stream) {
+    if (!hidden || !weight || !saved || !out) return DS_ERR_INVALID_ARG;
+    const int rc = check_sizes(dtype, N, D, V, ldh);
+    if (rc) return rc;
+    const Plan p = plan_of(mode, dtype, N, D, V, ldh);
+    if (!ws || bytes < p.fwd_total || misaligned(ws) || misaligned(saved)) return DS_ERR_WORKSPACE;
+    if ((!p.stage_w && misaligned(weight)) || (!p.stage_h && misaligned(hidden))) return DS_ERR_INVALID_ARG;
+    char* w = static_cast<char*>(ws);
+    hipStream_t q = static_cast<hipStream_t>(stream);
+#define DS_GO(IT, T, SP)                                                                                                     \
+    [&] {                                                                                                                    \
+        return head_fwd<IT, T, SP>(mode, static_cast<const IT*>(hidden), ldh, static_cast<const IT*>(weight), target, centers, \
+                                   N, D, V, ignore, reduction, out, saved, w, q);                                            \
+    }
+    return by_type(dtype, DS_GO(float, f16, 3), DS_GO(f16, f16, 1), DS_GO(bf16, bf16, 1));
+#undef DS_GO
+}
+
+int bwd_any(int mode, const void* hidden, long long ldh, const void* weight, const long long* target, const float* centers,
+            const float* g, int dtype, long long N, int D, int V, long long ignore, int reduction, void* saved, void* g_hidden,
+            void* g_weight, void* ws, size_t bytes, void* stream) {
+    if (!hidden || !weight || !saved || !g || (!g_hidden && !g_weight)) return DS_ERR_INVALID_ARG;
+    const int rc = check_sizes(dtype, N, D, V, ldh);
+    if (rc) return rc;
+    const Plan p = plan_of(mode, dtype, N, D, V, ldh);
+    if (!ws || bytes < p.bwd_total || misaligned(ws) || misaligned(saved)) return DS_ERR_WORKSPACE;
+    if ((!p.stage_w && misaligned(weight)) || (!p.stage_h && misaligned(hidden)) || misaligned(g_hidden) || misaligned(g_weight))
+        return DS_ERR_INVALID_ARG;
+    char* w = static_cast<char*>(ws);
+    hipStream_t q = static_cast<hipStream_t>(stream);
+#define DS_GO(IT, T, SP)                                                                                                       \
+    [&] {                                                                                                                      \
+        return head_bwd<IT, T, SP>(mode, static_cast<const IT*>(hidden), ldh, static_cast<const IT*>(weight), target, centers, \
+                                   g, N, D, V, ignore, reduction, saved, static_cast<IT*>(g_hidden),                           \
+                                   static_cast<IT*>(g_weight), w, q);                                                          \
+    }
+    return by_type(dtype, DS_GO(float, f16, 3), DS_GO(f16, f16, 1), DS_GO(bf16, bf16, 1));
+#undef DS_GO
+}
+
+}  // namespace
+}  // namespace ds
+
+extern "C" {
+
+size_t ds_head_saved_bytes(long long N) { return N > 0 ? ds::saved_bytes(N) : 0; }
+
+size_t ds_linear_ce_workspace_bytes(int dtype, long long N, int D, int V, long long ldh, int backward) {
+    if (ds::check_sizes(dtype, N, D, V, ldh)) return 0;
+    const ds::Plan p = ds::plan_of(ds::kCE, dtype, N, D, V, ldh);
+    return backward ? p.bwd_total : p.fwd_total;
+}
+int ds_linear_ce_fwd(const void* hidden, long long ldh, const void* weight, const long long* target, int dtype, long long N,
+                     int D, int V, long long ignore_index, int reduction, float* loss, void* saved, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+    if (!target || reduction < DS_REDUCE_NONE || reduction > DS_REDUCE_MEAN) return DS_ERR_INVALID_ARG;
+    return ds::fwd_any(ds::kCE, hidden, ldh, weight, target, nullptr, dtype, N, D, V, ignore_index, reduction, loss, saved,
+                       workspace, workspace_bytes, stream);
+}
+int ds_linear_ce_bwd(const void* hidden, long long ldh, const void* weight, const long long* target, const float* g_loss,
+                     int dtype, long long N, int D, int V, long long ignore_index, int reduction, const void* saved,
+                     void* g_hidden, void* g_weight, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!target || reduction < DS_REDUCE_NONE || reduction > DS_REDUCE_MEAN) return DS_ERR_INVALID_ARG;
+    return ds::bwd_any(ds::kCE, hidden, ldh, weight, target, nullptr, g_loss, dtype, N, D, V, ignore_index, reduction,
+                       const_cast<void*>(saved), g_hidden, g_weight, workspace, workspace_bytes, stream);
+}
+
+size_t ds_bin_expect_workspace_bytes(int dtype, long long N, int D, int V, long long ldh, int backward) {
+    if (ds::check_sizes(dtype, N, D, V, ldh)) return 0;
+    const ds::Plan p = ds::plan_of(ds::kExpect, dtype, N, D, V, ldh);
+    return backward ? p.bwd_total : p.fwd_total;
+}
+int ds_bin_expect_fwd(const void* hidden, long long ldh, const void* weight, const float* centers, int dtype, long long N, int D,
+                      int V, float* out, void* saved, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!centers) return DS_ERR_INVALID_ARG;
+    return ds::fwd_any(ds::kExpect, hidden, ldh, weight, nullptr, centers, dtype, N, D, V, 0, DS_REDUCE_NONE, out, saved,
+                       workspace, workspace_bytes, stream);
+}
+int ds_bin_expect_bwd(const void* hidden, long long ldh, const void* weight, const float* centers, const float* g_out, int dtype,
+                      long long N, int D, int V, const void* saved, void* g_hidden, void* g_weight, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+    if (!centers) return DS_ERR_INVALID_ARG;
+    return ds::bwd_any(ds::kExpect, hidden, ldh, weight, nullptr, centers, g_out, dtype, N, D, V, 0, DS_REDUCE_NONE,
+                       const_cast<void*>(saved), g_hidden, g_weight, workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

@@ -55,6 +55,17 @@ def reprojection_loss(preds: torch.Tensor, targets: torch.Tensor, shared_target:
     return out.reshape(1, 1, h, w)
 
 
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100,
+                         reduction: str = "mean") -> torch.Tensor:
+    """Softmax cross entropy of a linear head whose classes are depth bins (or any vocabulary): logits = hidden weight^T with
+    hidden (...,D) and weight (V,D) of one dtype (float32, float16, bfloat16), targets (...) integers in [0,V).  Rows with
+    target == ignore_index -- pixels without a measured depth -- take no part, and their features are not read.  reduction
+    "mean" (over the rows that take part; NaN if there is none), "sum" or "none"; the loss is float32.  A target outside
+    [0,V) that is not ignore_index makes the loss NaN.  Differentiable (once) w.r.t. hidden and weight; the logits are never
+    kept: the backward forms them again in pieces of the classes.  Not in the reference."""
+    return ops.linear_cross_entropy(hidden, weight, targets, ignore_index, reduction)
+
+
 def regularization_term(depths: torch.Tensor, target_imgs: torch.Tensor) -> torch.Tensor:
     """metrics.py:75-97 -- edge-aware smoothness: mean of |d_x D| exp(-|d_x I|) + |d_y D| exp(-|d_y I|)."""
     return ops.smoothness(depths, target_imgs)

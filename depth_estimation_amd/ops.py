@@ -630,3 +630,169 @@ def resize_bilinear(x: torch.Tensor, size) -> torch.Tensor:
 def resize_bicubic(x: torch.Tensor, size) -> torch.Tensor:
     """functional.interpolate(x, size=size, mode="bicubic") (train.py:60); x (...,H,W), no gradient."""
     return _resize("ds_resize_bicubic", x, size)
+
+
+# ----------------------------------------------------------------------------------------------------
+# classification head: cross entropy and expected bin centre, logits not kept
+# ----------------------------------------------------------------------------------------------------
+# Scratch memory of these calls is allocated per call instead of taken from L.workspace: it can be large, and a buffer
+# allocated during a graph capture belongs to that graph alone (two captured graphs that shared one would race on replay).
+def _scratch(nbytes: int, device) -> torch.Tensor:
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+
+
+def _aligned(t):
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _head_args(hidden, weight):
+    """-> hidden as (N,D) with unit column stride (a view where the strides allow it), its row pitch, weight contiguous."""
+    hidden, weight = L.dev_float(hidden, "hidden"), L.dev_float(weight, "weight")
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise RuntimeError(f"expected hidden (...,D) and weight (V,D); got {tuple(hidden.shape)}, {tuple(weight.shape)}")
+    if hidden.dtype != weight.dtype:
+        raise RuntimeError(f"hidden and weight must have one dtype, got {hidden.dtype} and {weight.dtype}")
+    L.same_device(hidden, weight)
+    d = weight.shape[1]
+    h = hidden.reshape(-1, d)
+    if h.shape[0] > 1 and (h.stride(0) < d or (d > 1 and h.stride(1) != 1)) or (d > 1 and h.stride(1) != 1):
+        h = h.contiguous()
+    h = _aligned(h)
+    return h, (h.stride(0) if h.shape[0] > 1 else d), _aligned(weight.contiguous())
+
+
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+
+
+class _LinearCE(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, ignore_index, reduction):
+        h, ldh, w = _head_args(hidden, weight)
+        if not isinstance(targets, torch.Tensor) or targets.dtype.is_floating_point or targets.dtype.is_complex or \
+                targets.dtype == torch.bool:
+            raise RuntimeError("targets must be a tensor of integers")
+        if targets.shape != hidden.shape[:-1]:
+            raise RuntimeError(f"targets must be {tuple(hidden.shape[:-1])}, got {tuple(targets.shape)}")
+        L.same_device(h, targets)
+        t = targets.to(torch.int64).contiguous()
+        (n, d), v, lib = h.shape, w.shape[0], L.lib()
+        dev, code, red = h.device, L.DTYPES[h.dtype], _REDUCTIONS[reduction]
+        out = torch.empty(targets.shape if red == 0 else (), dtype=torch.float32, device=dev)
+        saved = _scratch(lib.ds_head_saved_bytes(n), dev)
+        if n == 0:
+            if red:
+                out.fill_(0.0 if red == 1 else float("nan"))
+        else:
+            nb = lib.ds_linear_ce_workspace_bytes(code, n, d, v, ldh, 0)
+            ws = _scratch(nb, dev)
+            L.check(lib.ds_linear_ce_fwd(h.data_ptr(), ldh, w.data_ptr(), t.data_ptr(), code, n, d, v, ignore_index, red,
+                                         out.data_ptr(), saved.data_ptr(), ws.data_ptr(), nb, L.stream()), "ds_linear_ce_fwd")
+        ctx.save_for_backward(h, w, t, saved)
+        ctx.args = ldh, ignore_index, red, hidden.shape
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        h, w, t, saved = ctx.saved_tensors
+        ldh, ignore_index, red, shape = ctx.args
+        (n, d), v, lib = h.shape, w.shape[0], L.lib()
+        code = L.DTYPES[h.dtype]
+        g = L.dev_f32(g, "grad")
+        gh = torch.empty(n, d, dtype=h.dtype, device=h.device) if ctx.needs_input_grad[0] else None
+        gw = torch.empty(v, d, dtype=h.dtype, device=h.device) if ctx.needs_input_grad[1] else None
+        if n == 0:
+            gw = None if gw is None else gw.zero_()
+        elif gh is not None or gw is not None:
+            L.same_device(h, w, g)
+            nb = lib.ds_linear_ce_workspace_bytes(code, n, d, v, ldh, 1)
+            ws = _scratch(nb, h.device)
+            L.check(lib.ds_linear_ce_bwd(h.data_ptr(), ldh, w.data_ptr(), t.data_ptr(), g.data_ptr(), code, n, d, v,
+                                         ignore_index, red, saved.data_ptr(), L.ptr(gh), L.ptr(gw), ws.data_ptr(), nb,
+                                         L.stream()), "ds_linear_ce_bwd")
+        return None if gh is None else gh.reshape(shape), gw, None, None, None
+
+
+def linear_cross_entropy(hidden, weight, targets, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+    """hidden (...,D), weight (V,D), targets (...) integers -> float32 loss (...) or scalar; differentiable w.r.t. hidden and
+    weight.  Neither the logits nor their gradient exist as a whole."""
+    if reduction not in _REDUCTIONS:
+        raise RuntimeError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
+    return _LinearCE.apply(hidden, weight, targets, int(ignore_index), reduction)
+
+
+class _BinExpect(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, centers):
+        h, ldh, w = _head_args(hidden, weight)
+        c = L.dev_f32(centers, "centers")
+        (n, d), v, lib = h.shape, w.shape[0], L.lib()
+        if c.shape != (v,):
+            raise RuntimeError(f"centers must be ({v},), got {tuple(c.shape)}")
+        L.same_device(h, c)
+        dev, code = h.device, L.DTYPES[h.dtype]
+        out = torch.empty(hidden.shape[:-1], dtype=torch.float32, device=dev)
+        saved = _scratch(lib.ds_head_saved_bytes(n), dev)
+        if n:
+            nb = lib.ds_bin_expect_workspace_bytes(code, n, d, v, ldh, 0)
+            ws = _scratch(nb, dev)
+            L.check(lib.ds_bin_expect_fwd(h.data_ptr(), ldh, w.data_ptr(), c.data_ptr(), code, n, d, v, out.data_ptr(),
+                                          saved.data_ptr(), ws.data_ptr(), nb, L.stream()), "ds_bin_expect_fwd")
+        ctx.save_for_backward(h, w, c, saved)
+        ctx.args = ldh, hidden.shape
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        h, w, c, saved = ctx.saved_tensors
+        ldh, shape = ctx.args
+        (n, d), v, lib = h.shape, w.shape[0], L.lib()
+        code = L.DTYPES[h.dtype]
+        g = L.dev_f32(g, "grad")
+        gh = torch.empty(n, d, dtype=h.dtype, device=h.device) if ctx.needs_input_grad[0] else None
+        gw = torch.empty(v, d, dtype=h.dtype, device=h.device) if ctx.needs_input_grad[1] else None
+        if n == 0:
+            gw = None if gw is None else gw.zero_()
+        elif gh is not None or gw is not None:
+            L.same_device(h, w, g)
+            nb = lib.ds_bin_expect_workspace_bytes(code, n, d, v, ldh, 1)
+            ws = _scratch(nb, h.device)
+            L.check(lib.ds_bin_expect_bwd(h.data_ptr(), ldh, w.data_ptr(), c.data_ptr(), g.data_ptr(), code, n, d, v,
+                                          saved.data_ptr(), L.ptr(gh), L.ptr(gw), ws.data_ptr(), nb, L.stream()),
+                    "ds_bin_expect_bwd")
+        return None if gh is None else gh.reshape(shape), gw, None
+
+
+def bin_expectation(hidden, weight, centers) -> torch.Tensor:
+    """hidden (...,D), weight (V,D), centers (V) float32 -> (...) float32: sum_v softmax(hidden weight^T)_v centers_v;
+    differentiable w.r.t. hidden and weight."""
+    if isinstance(centers, torch.Tensor) and centers.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("bin_expectation: gradient w.r.t. centers is not implemented (detach them)")
+    return _BinExpect.apply(hidden, weight, centers)
+
+
+# ----------------------------------------------------------------------------------------------------
+# an update matrix orthogonalised by Newton-Schulz products
+# ----------------------------------------------------------------------------------------------------
+def orthogonalize(update, steps: int, coefficients, eps: float) -> torch.Tensor:
+    """update (...,m,n) -> the same shape and dtype; no gradient flows."""
+    u = L.dev_float(update.detach() if isinstance(update, torch.Tensor) else update, "update").contiguous()
+    if u.dim() < 2:
+        raise RuntimeError(f"update must be (...,m,n), got {tuple(u.shape)}")
+    co = [float(x) for x in coefficients]
+    if len(co) != 3:
+        raise RuntimeError(f"coefficients must be three numbers (a, b, c), got {len(co)}")
+    if not all(np.isfinite(co)) or not 0 <= float(eps) < float("inf"):
+        raise RuntimeError(f"coefficients must be finite and eps >= 0, got {co}, {eps}")
+    L.same_device(u)
+    out = torch.empty_like(u)
+    m, n = u.shape[-2:]
+    if u.numel() == 0:
+        return out
+    b, lib = u.numel() // (m * n), L.lib()
+    nb = lib.ds_orthogonalize_workspace_bytes(b, m, n)
+    ws = _scratch(nb, u.device)
+    L.check(lib.ds_orthogonalize(u.data_ptr(), L.DTYPES[u.dtype], b, m, n, int(steps), (C.c_double * 3)(*co), float(eps),
+                                 out.data_ptr(), ws.data_ptr(), nb, L.stream()), "ds_orthogonalize")
+    return out

@@ -71,3 +71,11 @@ def depth_from_costs(cost_volumes: torch.Tensor, num_channels: int = 80, sid: bo
     if cost_volumes.dim() != 4 or cost_volumes.shape[1] != num_channels:
         raise RuntimeError(f"cost_volumes must be (N,{num_channels},H,W), got {tuple(cost_volumes.shape)}")
     return ops.depth_from_costs(cost_volumes, sid)
+
+
+def depth_from_bins(hidden: torch.Tensor, weight: torch.Tensor, centers: torch.Tensor) -> torch.Tensor:
+    """Depth from a linear head over depth bins: sum_v softmax(hidden weight^T)_v centers_v, float32, without keeping the
+    logits.  hidden (...,D) and weight (V,D) of one dtype (float32, float16, bfloat16), centers (V) float32 -> (...).
+    Differentiable (once) w.r.t. hidden and weight, so that a photometric loss on the depth trains the head; one row (one
+    pixel) up to whole batches of maps.  Not in the reference, whose only such head is depth_from_costs."""
+    return ops.bin_expectation(hidden, weight, centers)

@@ -284,6 +284,59 @@ int ds_ingest_resize_u8(const uint8_t* frames, int N, int Hin, int Win, int Hout
  * and torchvision is absent here: parity unpinned, checked against the direct statement value / 65536. */
 int ds_ingest_depth_u16(const uint16_t* depth, int N, int H, int W, float* out, void* stream);
 
+/* ---- classification head and matrix update (no counterpart in the reference) ------------------------------------- */
+
+#define DS_F32 0   /* element type of a head's features and weights, and of an update */
+#define DS_F16 1
+#define DS_BF16 2
+#define DS_REDUCE_NONE 0
+#define DS_REDUCE_SUM 1
+#define DS_REDUCE_MEAN 2
+#define DS_HEAD_MAX_ROWS (1 << 24)
+#define DS_HEAD_MAX_FEATURES (1 << 16)
+#define DS_HEAD_MAX_CLASSES (1 << 22)
+#define DS_ORTHO_MAX_SIDE (1 << 16)
+#define DS_ORTHO_MAX_STEPS 32
+
+/* A linear head: features hidden (N,D) with ldh elements between rows, weight (V,D) contiguous, both of type `dtype`;
+ * logits l = hidden weight^T, which never reach memory as a whole.
+ *
+ * Softmax cross entropy with classes target (N) int64: loss_r = log sum_v exp l_rv - l[r,target_r].  Rows whose target is
+ * ignore_index take no part (loss 0, gradient 0; their features are not read); a target that is neither ignore_index nor in
+ * [0,V) makes its row's loss NaN, and the gradients it takes part in.  reduction: DS_REDUCE_NONE -> loss (N) and g_loss (N);
+ * SUM / MEAN (over the rows that take part; NaN if none does) -> one value each.  All sums in fp32 or more, loss fp32.
+ *
+ * Expected bin centre: out (N) fp32 = sum_v softmax(l)_rv centers[v], centers (V) fp32; g_out (N).
+ *
+ * The forward fills `saved` (ds_head_saved_bytes(N)), which the backward reads.  g_hidden (N,D) and g_weight (V,D),
+ * contiguous, of type `dtype`; either may be NULL.  fp32 inputs: every product in three fp16 products of two planes (22
+ * bits).  Results do not depend on scheduling: the same inputs give the same bits.
+ * workspace (16-byte aligned) from ds_*_workspace_bytes(..., backward); 0 = sizes outside the limits above.
+ * With D a multiple of 8 and 16-bit types, weight (and for ds_bin_expect_*, with ldh a multiple of 8, hidden) must be
+ * 16-byte aligned; g_hidden and g_weight always. */
+size_t ds_head_saved_bytes(long long N);
+size_t ds_linear_ce_workspace_bytes(int dtype, long long N, int D, int V, long long ldh, int backward);
+int ds_linear_ce_fwd(const void* hidden, long long ldh, const void* weight, const long long* target, int dtype, long long N,
+                     int D, int V, long long ignore_index, int reduction, float* loss, void* saved, void* workspace,
+                     size_t workspace_bytes, void* stream);
+int ds_linear_ce_bwd(const void* hidden, long long ldh, const void* weight, const long long* target, const float* g_loss,
+                     int dtype, long long N, int D, int V, long long ignore_index, int reduction, const void* saved,
+                     void* g_hidden, void* g_weight, void* workspace, size_t workspace_bytes, void* stream);
+size_t ds_bin_expect_workspace_bytes(int dtype, long long N, int D, int V, long long ldh, int backward);
+int ds_bin_expect_fwd(const void* hidden, long long ldh, const void* weight, const float* centers, int dtype, long long N, int D,
+                      int V, float* out, void* saved, void* workspace, size_t workspace_bytes, void* stream);
+int ds_bin_expect_bwd(const void* hidden, long long ldh, const void* weight, const float* centers, const float* g_out, int dtype,
+                      long long N, int D, int V, const void* saved, void* g_hidden, void* g_weight, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* An update orthogonalised by Newton-Schulz products: X = G / (|G|_F + eps); `steps` times, on the smaller side,
+ * A = X X^T, X = (a + b A + c A A) X.  update and out: batch matrices (m,n), contiguous, of type `dtype`; out = update is
+ * allowed.  coefficients: HOST double[3] a, b, c.  Products as for fp32 heads (22-bit operands, fp32 sums) for every dtype,
+ * one rounding at the end.  workspace (16-byte aligned) from ds_orthogonalize_workspace_bytes. */
+size_t ds_orthogonalize_workspace_bytes(int batch, int m, int n);
+int ds_orthogonalize(const void* update, int dtype, int batch, int m, int n, int steps, const double* coefficients, double eps,
+                     void* out, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

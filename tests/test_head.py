@@ -1,0 +1,471 @@
+"""metrics.linear_cross_entropy and synthesis.depth_from_bins against their formulas in float64.
+
+Tolerances, element by element, from the arithmetic (u: half a step of a type, 2^-8 bfloat16, 2^-11 float16, 2^-24 float32):
+  * logits: operands exact (16-bit types) or 22 bits with the product of the two low parts dropped (float32: 2^-21 per
+    product, plus 2^-40 of the largest operand where a small one's low part runs out of fp16's range); fp32 sums of D terms:
+    |dl| <= (2^-21 [float32] + (D + 4) 2^-24) sum_d |h||w| =: e_l;
+  * a probability: relative error <= 2 (max_v e_l) (its own logit and the normaliser) + (V + 32) 2^-24 (sum, exponentials whose
+    argument carries |l - max| 2^-24 with |l - max| <= 24 where p matters, divisions) =: e_p;
+  * dl is rounded to u of the operand type (2^-21 for float32's planes) before the products and summed in fp32:
+    |d out| <= sum |dl||x| (u + e_p' + terms 2^-24) + u |out|.
+"""
+import math
+import os
+
+import pytest
+import torch
+
+from conftest import ROOT  # noqa: F401
+
+DEV = "cuda:0"
+U = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def _data(n, d, v, dtype, seed, keep=1.0, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randn(v, d, generator=g) / math.sqrt(d)
+    t = torch.randint(0, v, (n,), generator=g)
+    h = spread * torch.randn(n, d, generator=g) + 2.0 * w[t]
+    drop = torch.rand(n, generator=g) >= keep
+    up = torch.rand(n, generator=g) + 0.5
+    c = torch.sort(80 * torch.rand(v, generator=g) + 0.1).values
+    return h.to(dtype).to(DEV), w.to(dtype).to(DEV), torch.where(drop, torch.full_like(t, -100), t).to(DEV), up.to(DEV), c.to(DEV)
+
+
+def _oracle(h, w, t=None, c=None, up=None, ignore=-100):
+    """float64: (per-row output, g_hidden, g_weight, and the tolerances of the three) for upstream `up` per row"""
+    dt = h.dtype
+    n, d = h.shape
+    v = w.shape[0]
+    H, W, up = h.double(), w.double(), up.double()
+    ok = torch.ones(n, dtype=torch.bool, device=h.device) if t is None else t != ignore
+    H = torch.where(ok[:, None], H, 0.0)
+    l = H @ W.T
+    split = 2.0 ** -21 if dt == torch.float32 else 0.0
+    # 2^-40 of the largest operand per term, where the low plane underflows
+    floor = 2.0 ** -40 * (H.abs().max() if n else 0.0) * W.abs().max() * 2 * d if dt == torch.float32 else 0.0
+    el = (split + (d + 4) * 2.0 ** -24) * (H.abs() @ W.abs().T) + floor
+    top = el.max(dim=1, keepdim=True).values
+    p = torch.softmax(l, dim=1)
+    ep = 2 * top + (v + 32) * 2.0 ** -24
+    if t is not None:
+        tc = t.clamp(min=0)
+        one = torch.nn.functional.one_hot(tc, v).double()
+        out = torch.where(ok, torch.logsumexp(l, 1) - l.gather(1, tc[:, None])[:, 0], 0.0)
+        tol = 2 * top[:, 0] + (v + 32) * 2.0 ** -24 + 4 * 2.0 ** -24 * (l.abs().max(dim=1).values + out.abs() + 1)
+        dl = (p - one) * (up * ok)[:, None]
+        mag = (p * ep + one * 2.0 ** -24) * (up.abs() * ok)[:, None]      # a bound: the upstream's size, not its sign
+    else:
+        cd = c.double()
+        out = p @ cd
+        tol = (ep * (p @ cd.abs())[:, None])[:, 0] + 4 * 2.0 ** -24 * out.abs()
+        dl = p * (cd[None] - out[:, None]) * up[:, None]
+        mag = p * (ep * (cd[None] - out[:, None]).abs() + tol[:, None] + 2.0 ** -23 * cd.abs()[None]) * up.abs()[:, None]
+    ur = 2.0 ** -21 if dt == torch.float32 else U[dt]
+    # what dl is stored to: ur of it, or where that is below fp16's normal numbers half a subnormal step, 2^-25.  dl is stored
+    # as 2^14 dl / s with s at most twice the largest upstream value (times four times the largest centre): the half step is
+    # 2^-25 2^-14 2 = 2^-38 of the largest upstream value -- not of the largest dl, which is smaller where every row is sure
+    # of its class
+    unit = (up * ok).abs().max() * (1.0 if t is not None else 4 * c.abs().max().double()) if n else 0.0
+    err = mag + ur * (dl.abs() + mag) + (0.0 if dt == torch.bfloat16 else 2.0 ** -38 * unit)
+    gh, gw = dl @ W, dl.T @ H
+    th = (err + (v + 8) * 2.0 ** -24 * dl.abs()) @ W.abs() + U[dt] * gh.abs() + split * (dl.abs() @ W.abs())
+    tw = (err + (n + 8) * 2.0 ** -24 * dl.abs()).T @ H.abs() + U[dt] * gw.abs() + split * (dl.abs().T @ H.abs())
+    # results below the smallest normal number of the type are rounded to its subnormal steps
+    sub = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -24, torch.bfloat16: 2.0 ** -133}[dt]
+    return out, gh, gw, tol, th * 1.01 + sub, tw * 1.01 + sub
+
+
+def _close(got, want, tol, what):
+    got = got.double()
+    assert got.shape == want.shape, what
+    bad = (got - want).abs() - tol
+    assert bool((bad <= 0).all()), f"{what}: off by {(got - want).abs().max():.3g}, over its bound by {bad.max():.3g}"
+
+
+def _ce(h, w, t, reduction="none", up=None, ignore=-100):
+    from depth_estimation_amd import metrics
+    h, w = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    out = metrics.linear_cross_entropy(h, w, t, ignore_index=ignore, reduction=reduction)
+    gh, gw = torch.autograd.grad(out, (h, w), up)
+    return out.detach(), gh, gw
+
+
+def _ex(h, w, c, up):
+    from depth_estimation_amd import synthesis
+    h, w = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    out = synthesis.depth_from_bins(h, w, c)
+    gh, gw = torch.autograd.grad(out, (h, w), up)
+    return out.detach(), gh, gw
+
+
+# rows, features, classes: one of each; odd everything; tile edges and one beyond; long reductions on either side; few rows
+# against many classes and the reverse
+SIZES = [(1, 1, 1), (1, 8, 2), (3, 5, 7), (1, 64, 1000), (2, 40, 129), (9, 24, 300), (31, 72, 257), (33, 64, 128),
+         (127, 65, 127), (128, 128, 128), (129, 136, 129), (300, 771, 501), (1000, 64, 80), (5000, 48, 17), (64, 96, 9001),
+         (700, 1030, 333), (257, 192, 1024)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,d,v", SIZES)
+def test_cross_entropy_and_gradients(n, d, v, dtype):
+    h, w, t, up, _ = _data(n, d, v, dtype, seed=n * 7 + d * 3 + v, keep=0.8 if n > 2 else 1.0)
+    out, gh, gw, tol, th, tw = _oracle(h, w, t=t, up=up)
+    got = _ce(h, w, t, "none", up)
+    _close(got[0], out, tol, "loss")
+    _close(got[1], gh, th, "g_hidden")
+    _close(got[2], gw, tw, "g_weight")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,d,v", SIZES)
+def test_expected_center_and_gradients(n, d, v, dtype):
+    h, w, _, up, c = _data(n, d, v, dtype, seed=n * 5 + d + v)
+    out, gh, gw, tol, th, tw = _oracle(h, w, c=c, up=up)
+    got = _ex(h, w, c, up)
+    _close(got[0], out, tol, "depth")
+    _close(got[1], gh, th, "g_hidden")
+    _close(got[2], gw, tw, "g_weight")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+@pytest.mark.parametrize("keep", [1.0, 0.5, 0.02])
+def test_reductions(reduction, keep):
+    n, d, v = 20000, 32, 50          # more rows than one listing workgroup takes
+    h, w, t, _, _ = _data(n, d, v, torch.float32, seed=11, keep=keep)
+    cnt = int((t != -100).sum())
+    f = 1.0 / cnt if reduction == "mean" else 1.0
+    up = torch.full((n,), f * 0.7, dtype=torch.float64, device=DEV)
+    out, gh, gw, tol, th, tw = _oracle(h, w, t=t, up=up)
+    got = _ce(h, w, t, reduction, torch.tensor(0.7, device=DEV))
+    want = out.sum() * f
+    _close(got[0], want, tol.sum() * f + 2.0 ** -23 * want.abs(), "loss")
+    _close(got[1], gh, th + 2.0 ** -23 * gh.abs(), "g_hidden")      # the upstream value itself is 0.7 / count in float32
+    _close(got[2], gw, tw + 2.0 ** -22 * gw.abs(), "g_weight")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_ignored_rows_are_not_read(dtype):
+    """Features of ignored rows may be anything: NaN, infinities, the type's lowest value."""
+    n, d, v = 300, 40, 70
+    h, w, t, up, _ = _data(n, d, v, dtype, seed=3, keep=0.6)
+    clean = _ce(h, w, t, "none", up)
+    dirty = h.clone()
+    ignored = (t == -100).nonzero()[:, 0]
+    dirty[ignored[0::3]] = float("nan")
+    dirty[ignored[1::3]] = float("inf")
+    dirty[ignored[2::3]] = torch.finfo(dtype).min
+    for a, b in zip(clean, _ce(dirty, w, t, "none", up)):
+        assert torch.equal(a, b)
+    assert torch.equal(clean[0][ignored], torch.zeros_like(clean[0][ignored]))
+    assert torch.equal(clean[1][ignored], torch.zeros_like(clean[1][ignored]))
+
+
+@pytest.mark.gpu
+def test_nothing_left_and_bad_targets():
+    h, w, t, up, _ = _data(40, 16, 10, torch.float32, seed=4)
+    none = torch.full_like(t, -100)
+    out, gh, gw = _ce(h, w, none, "mean")
+    assert math.isnan(float(out)) and not gh.any() and not gw.any()
+    out, gh, gw = _ce(h, w, none, "sum")
+    assert float(out) == 0 and not gh.any() and not gw.any()
+    out, gh, gw = _ce(h, w, none, "none", up)
+    assert not out.any() and not gh.any() and not gw.any()
+    bad = t.clone()
+    bad[3], bad[7] = 10, -1                                     # classes are 0..9
+    out, gh, gw = _ce(h, w, bad, "none", up)
+    assert torch.isnan(out).nonzero()[:, 0].tolist() == [3, 7]
+    assert torch.isnan(gh).any(1).nonzero()[:, 0].tolist() == [3, 7] and torch.isnan(gw).all()
+    out, _, _ = _ce(h, w, t.where(t != 5, torch.full_like(t, 5)), "none", up, ignore=5)   # a real class may be the ignored one
+    assert not out[t == 5].any() and (out[t != 5] > 0).all()
+
+
+@pytest.mark.gpu
+def test_no_rows():
+    from depth_estimation_amd import metrics, synthesis
+    w = torch.randn(6, 8, device=DEV, requires_grad=True)
+    h = torch.randn(0, 8, device=DEV, requires_grad=True)
+    t = torch.empty(0, dtype=torch.int64, device=DEV)
+    assert math.isnan(float(metrics.linear_cross_entropy(h, w, t)))
+    assert float(metrics.linear_cross_entropy(h, w, t, reduction="sum")) == 0
+    out = metrics.linear_cross_entropy(h, w, t, reduction="none")
+    assert out.shape == (0,)
+    gh, gw = torch.autograd.grad(out.sum(), (h, w))
+    assert gh.shape == (0, 8) and not gw.any()
+    assert synthesis.depth_from_bins(h, w, torch.ones(6, device=DEV)).shape == (0,)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_layouts(dtype):
+    """Strided, shifted, transposed, expanded and many-dimensional features give the bits of the plain layout."""
+    from depth_estimation_amd import metrics, synthesis
+    n, d, v = 60, 48, 30
+    h, w, t, up, c = _data(n, d, v, dtype, seed=8, keep=0.9)
+    base, exp = _ce(h, w, t, "none", up), _ex(h, w, c, up)
+    wide = torch.zeros(n, d + 16, dtype=dtype, device=DEV)
+    wide[:, 8:8 + d] = h
+    shifted = torch.zeros(n * d + 1, dtype=dtype, device=DEV)
+    shifted[1:] = h.reshape(-1)
+    wsh = torch.zeros(v * d + 3, dtype=dtype, device=DEV)
+    wsh[3:] = w.reshape(-1)
+    odd = torch.zeros(n, d + 3, dtype=dtype, device=DEV)
+    odd[:, 3:] = h
+    forms = [(wide[:, 8:8 + d], w), (shifted[1:].view(n, d), wsh[3:].view(v, d)), (odd[:, 3:], w),
+             (h.t().contiguous().t(), w.t().contiguous().t())]
+    for hh, ww in forms:
+        for a, b in zip(base, _ce(hh, ww, t, "none", up)):
+            assert torch.equal(a, b)
+        for a, b in zip(exp, _ex(hh, ww, c, up)):
+            assert torch.equal(a, b)
+    maps = h.view(3, 4, 5, d).permute(0, 3, 1, 2).contiguous().requires_grad_(True)     # (B,D,H,W) features of a network
+    out = metrics.linear_cross_entropy(maps.permute(0, 2, 3, 1), w, t.view(3, 4, 5), reduction="none")
+    assert torch.equal(out.detach().reshape(-1), base[0])
+    (g,) = torch.autograd.grad(out, maps, up.view(3, 4, 5))
+    assert torch.equal(g.permute(0, 2, 3, 1).reshape(n, d), base[1])
+    one = h[:1].expand(n, d).requires_grad_(True)
+    assert torch.equal(synthesis.depth_from_bins(one, w, c), exp[0][:1].expand(n))
+    assert synthesis.depth_from_bins(h[0], w, c).shape == ()
+    assert torch.equal(metrics.linear_cross_entropy(h, w, t.to(torch.int32), reduction="none"), base[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale_h,scale_w", [(1e-6, 1e6), (1e15, 1e-15), (1e-20, 1.0), (1e4, 1e-3)])
+def test_float32_of_any_size(scale_h, scale_w):
+    """The planes' scale follows the data: features and weights far from one lose nothing."""
+    h, w, t, up, _ = _data(50, 33, 40, torch.float32, seed=9)
+    h, w = h * scale_h, w * scale_w
+    out, gh, gw, tol, th, tw = _oracle(h, w, t=t, up=up)
+    got = _ce(h, w, t, "none", up)
+    _close(got[0], out, tol, "loss")
+    _close(got[1], gh, th, "g_hidden")
+    _close(got[2], gw, tw, "g_weight")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_large_logits_and_upstreams(dtype):
+    """Logits of +-100s, upstream values from 1e-6 to 1e6 and zero in one call."""
+    h, w, t, up, _ = _data(200, 32, 60, dtype, seed=10, spread=60.0)
+    up = up * (10.0 ** torch.linspace(-6, 6, 200, device=DEV))
+    up[17] = 0
+    out, gh, gw, tol, th, tw = _oracle(h, w, t=t, up=up)
+    fit = torch.finfo(dtype).max
+    got = _ce(h, w, t, "none", up)
+    _close(got[0], out, tol, "loss")
+    for a, b, tol_ in ((got[1], gh, th), (got[2], gw, tw)):
+        inside = b.abs() < fit / 2
+        _close(a[inside], b[inside], tol_[inside], "gradient")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_confident_rows(dtype):
+    """Rows that are all but certain of their class: p - 1 keeps its digits, nothing overflows."""
+    n, d, v = 64, 64, 64
+    w = torch.eye(v, d, device=DEV).to(dtype)
+    h = (40 * torch.eye(n, d, device=DEV)).to(dtype)
+    t = torch.arange(n, device=DEV)
+    up = torch.ones(n, device=DEV)
+    out, gh, gw, tol, th, tw = _oracle(h, w, t=t, up=up)
+    got = _ce(h, w, t, "none", up)
+    _close(got[0], out, tol, "loss")
+    _close(got[1], gh, th, "g_hidden")
+    _close(got[2], gw, tw, "g_weight")
+
+
+@pytest.mark.gpu
+def test_pieces_of_the_classes_join():
+    """More rows times classes than one piece of dl holds: the gradient of the features adds up over pieces."""
+    n, d, v = 40000, 24, 5000          # 2 bytes x 40000 rows: 3328 classes a piece
+    h, w, t, up, _ = _data(n, d, v, torch.bfloat16, seed=12, keep=0.9)
+    got = _ce(h, w, t, "none", up)
+    pick = torch.arange(0, n, 997, device=DEV)
+    out, gh, _, tol, th, _ = _oracle(h[pick], w, t=t[pick], up=up[pick])
+    _close(got[0][pick], out, tol, "loss")
+    _close(got[1][pick], gh, th, "g_hidden")
+    gw = torch.zeros(v, d, dtype=torch.float64, device=DEV)
+    tw = torch.zeros_like(gw)
+    for lo in range(0, n, 4000):
+        s = slice(lo, lo + 4000)
+        _, _, g, _, _, tt = _oracle(h[s], w, t=t[s], up=up[s])
+        gw, tw = gw + g, tw + tt
+    _close(got[2], gw, tw + n * 2.0 ** -24 * tw + U[torch.bfloat16] * gw.abs(), "g_weight")
+
+
+@pytest.mark.gpu
+def test_gradient_is_the_difference_quotient():
+    n, d, v = 6, 10, 9
+    h, w, t, up, c = _data(n, d, v, torch.float32, seed=13)
+    from depth_estimation_amd import metrics, synthesis
+    g = torch.Generator().manual_seed(1)
+    dh, dw = torch.randn(n, d, generator=g).to(DEV), torch.randn(v, d, generator=g).to(DEV)
+    for f, (_, gh, gw) in ((lambda a, b: metrics.linear_cross_entropy(a, b, t, reduction="none"), _ce(h, w, t, "none", up)),
+                           (lambda a, b: synthesis.depth_from_bins(a, b, c), _ex(h, w, c, up))):
+        e = 2.0 ** -7
+        quotient = ((f(h + e * dh, w + e * dw) - f(h - e * dh, w - e * dw)).double() * up.double()).sum() / (2 * e)
+        slope = (gh.double() * dh).sum() + (gw.double() * dw).sum()
+        # third derivatives of order 100 times e^2 / 6, and float32 outputs of size 80 over 2 e
+        assert abs(float(quotient - slope)) <= 0.02 * abs(float(slope)) + 0.02
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_same_bits_every_time(dtype):
+    h, w, t, up, c = _data(3000, 64, 700, dtype, seed=14, keep=0.7)
+    a, b = _ce(h, w, t, "mean"), _ce(h, w, t, "mean")
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    a, b = _ex(h, w, c, up), _ex(h, w, c, up)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.gpu
+def test_one_gradient_alone_and_frozen_inputs():
+    from depth_estimation_amd import metrics
+    h, w, t, up, _ = _data(70, 32, 20, torch.bfloat16, seed=15)
+    _, gh, gw = _ce(h, w, t, "none", up)
+    h1 = h.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(metrics.linear_cross_entropy(h1, w, t, reduction="none"), h1, up)[0], gh)
+    w1 = w.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(metrics.linear_cross_entropy(h, w1, t, reduction="none"), w1, up)[0], gw)
+    assert not metrics.linear_cross_entropy(h, w, t).requires_grad
+    out = metrics.linear_cross_entropy(h1, w1, t)
+    (g,) = torch.autograd.grad(out, h1, create_graph=True, retain_graph=True)
+    with pytest.raises(RuntimeError):
+        g.float().sum().backward()
+
+
+@pytest.mark.gpu
+def test_streams_and_captured_graphs():
+    """Another stream; two graphs captured one after the other and replayed in turn with eager calls between."""
+    from depth_estimation_amd import metrics, synthesis
+    h, w, t, up, c = _data(500, 64, 200, torch.bfloat16, seed=16, keep=0.8)
+    want, wexp = _ce(h, w, t, "mean"), _ex(h, w, c, up)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = _ce(h, w, t, "mean")
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+    def capture(f):
+        with torch.cuda.stream(s):
+            f()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            out = f()
+        return g, out
+
+    h2, t2 = h.clone(), t.clone()
+    g1, o1 = capture(lambda: _ce(h2, w, t2, "mean"))
+    g2, o2 = capture(lambda: _ex(h2, w, c, up))
+    other, _, tother, _, _ = _data(500, 64, 200, torch.bfloat16, seed=17, keep=0.5)
+    for k in range(4):
+        src, ts = (h, t) if k % 2 == 0 else (other, tother)
+        h2.copy_(src)
+        t2.copy_(ts)
+        torch.cuda.synchronize()
+        g1.replay()
+        g2.replay()
+        torch.cuda.synchronize()
+        e1, e2 = _ce(src, w, ts, "mean"), _ex(src, w, c, up)
+        assert all(torch.equal(a, b) for a, b in zip(o1, e1))
+        assert all(torch.equal(a, b) for a, b in zip(o2, e2))
+    assert all(torch.equal(a, b) for a, b in zip(_ex(h, w, c, up), wexp))
+    del g1, g2, o1, o2
+    assert torch.isfinite(metrics.linear_cross_entropy(h, w, t)) and torch.isfinite(synthesis.depth_from_bins(h, w, c)).all()
+
+
+@pytest.mark.gpu
+def test_head_into_the_photometric_loss():
+    """The operators together, as a trainer uses them: features -> expected depth -> warp and photometric loss, plus the cross
+    entropy of the same head where a depth was measured; one backward, one orthogonalised step.  Checked: the head's gradient
+    equals the chain of its parts."""
+    import depth_estimation_amd as de
+    B, S, H, W, D, V = 1, 2, 24, 80, 32, 40
+    g = torch.Generator().manual_seed(2)
+    feats = torch.randn(B, S, H, W, D, generator=g).to(DEV).requires_grad_(True)
+    weight = (0.3 * torch.randn(V, D, generator=g)).to(DEV).requires_grad_(True)
+    centers = torch.logspace(0, 1.9, V, device=DEV)
+    src, tgt = torch.rand(B, S, 3, H, W, generator=g).to(DEV), torch.rand(B, 3, H, W, generator=g).to(DEV)
+    K, Kinv = de.fused.intrinsics(W, H, DEV)
+    pose = de.synthesis.construct_pose_batch(0.01 * torch.randn(B * S, 6, generator=g).to(DEV)).reshape(B, S, 3, 4)
+    measured = torch.randint(0, V, (B, S, H, W), generator=g)
+    measured[torch.rand(B, S, H, W, generator=g) < 0.9] = -100
+    measured = measured.to(DEV)
+    depth = de.synthesis.depth_from_bins(feats, weight, centers)
+    photo = de.fused.train_step_loss(src, tgt, depth.unsqueeze(2), pose, K, Kinv)["total"]
+    ce = de.metrics.linear_cross_entropy(feats, weight, measured)
+    gf, gw = torch.autograd.grad(photo + 0.1 * ce, (feats, weight))
+    d = depth.detach().requires_grad_(True)
+    (gd,) = torch.autograd.grad(de.fused.train_step_loss(src, tgt, d.unsqueeze(2), pose, K, Kinv)["total"], d)
+    flat = feats.detach().reshape(-1, D)
+    _, eh, ew, _, teh, tew = _oracle(flat, weight.detach(), c=centers, up=gd.reshape(-1))
+    cnt = int((measured != -100).sum())
+    t = measured.reshape(-1)
+    _, ch, cw, _, tch, tcw = _oracle(flat, weight.detach(), t=t, up=torch.full((len(t),), 0.1 / cnt, device=DEV,
+                                                                              dtype=torch.float64))
+    _close(gf.reshape(-1, D), eh + ch, teh + tch + 2.0 ** -22 * (eh.abs() + ch.abs()), "g_hidden")
+    _close(gw, ew + cw, tew + tcw + 2.0 ** -22 * (ew.abs() + cw.abs()), "g_weight")
+    before = weight.detach().clone()
+    weight.grad = gw
+    de.optim.Muon([weight], lr=0.1, momentum=0.9).step()
+    step = (before - weight.detach()) / 0.1 / max(1.0, V / D) ** 0.5
+    assert torch.allclose(step, de.optim.orthogonalize(gw * 1.9), rtol=0, atol=1e-4)
+
+
+# ------------------------------------------------------------------------------------------------------- refusals
+def test_refusals_on_the_host():
+    """CPU tensors, and every wrong argument of the C entries, before any launch."""
+    from depth_estimation_amd import _lib as L, metrics, synthesis
+    with pytest.raises(RuntimeError, match="GPU"):
+        metrics.linear_cross_entropy(torch.zeros(2, 4), torch.zeros(3, 4), torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="GPU"):
+        synthesis.depth_from_bins(torch.zeros(2, 4), torch.zeros(3, 4), torch.zeros(3))
+    with pytest.raises(RuntimeError, match="reduction"):
+        metrics.linear_cross_entropy(torch.zeros(2, 4), torch.zeros(3, 4), torch.zeros(2, dtype=torch.int64), reduction="avg")
+    if not os.path.exists(L.LIB_PATH):
+        pytest.skip("libdepthsynth.so not built (run __graft_entry__.build())")
+    lib, fake = L.lib(), 0x1000
+    big = 1 << 40
+
+    def fwd(h=fake, ldh=64, w=fake, t=fake, dt=2, n=8, d=64, v=16, red=2, out=fake, saved=fake, ws=fake, nb=big):
+        return lib.ds_linear_ce_fwd(h, ldh, w, t, dt, n, d, v, -100, red, out, saved, ws, nb, None)
+
+    def bwd(g=fake, gh=fake, gw=fake, ws=fake, nb=big, w=fake, dt=2, ldh=64):
+        return lib.ds_linear_ce_bwd(fake, ldh, w, fake, g, dt, 8, 64, 16, -100, 2, fake, gh, gw, ws, nb, None)
+
+    for rc, want in [(fwd(h=None), -1), (fwd(w=None), -1), (fwd(t=None), -1), (fwd(out=None), -1), (fwd(saved=None), -1),
+                     (fwd(n=0), -1), (fwd(d=0), -1), (fwd(v=0), -1), (fwd(n=-5), -1), (fwd(ldh=63), -1), (fwd(red=3), -1),
+                     (fwd(red=-1), -1), (fwd(dt=3), -2), (fwd(dt=-1), -2), (fwd(n=(1 << 24) + 1), -2),
+                     (fwd(d=(1 << 16) + 8, ldh=1 << 20), -2), (fwd(v=(1 << 22) + 1), -2), (fwd(n=1 << 24, v=1 << 22), -2),
+                     (fwd(ws=None), -3), (fwd(nb=64), -3), (fwd(ws=fake + 4), -3), (fwd(w=fake + 2), -1),
+                     (bwd(g=None), -1), (bwd(gh=None, gw=None), -1), (bwd(gh=fake + 4), -1), (bwd(gw=fake + 4), -1),
+                     (bwd(nb=64), -3), (bwd(dt=7), -2), (bwd(ldh=8), -1), (bwd(w=fake + 2), -1)]:
+        assert rc == want
+    assert lib.ds_linear_ce_workspace_bytes(2, 0, 64, 16, 64, 0) == 0
+    assert lib.ds_linear_ce_workspace_bytes(9, 8, 64, 16, 64, 0) == 0
+    assert lib.ds_bin_expect_fwd(fake, 64, fake, None, 2, 8, 64, 16, fake, fake, fake, big, None) == -1
+    assert lib.ds_bin_expect_bwd(fake, 64, fake, None, fake, 2, 8, 64, 16, fake, fake, fake, fake, big, None) == -1
+    assert lib.ds_bin_expect_fwd(fake + 2, 64, fake, fake, 2, 8, 64, 16, fake, fake, fake, big, None) == -1
+
+
+@pytest.mark.gpu
+def test_refusals_of_tensors():
+    from depth_estimation_amd import metrics, synthesis
+    h, w = torch.zeros(4, 8, device=DEV), torch.zeros(5, 8, device=DEV)
+    t, c = torch.zeros(4, dtype=torch.int64, device=DEV), torch.zeros(5, device=DEV)
+    for args in [(h.bfloat16(), w, t), (h.double(), w.double(), t), (h[:, :7], w, t), (h, w[0], t), (h, w, t[:3]),
+                 (h, w, t.float()), (h, w, t.bool()), (h, w, t.cpu()), (h, w.cpu(), t), (h, w[:0], t),
+                 (h[:, :0], w[:, :0], t)]:
+        with pytest.raises(RuntimeError):
+            metrics.linear_cross_entropy(*args)
+    for args in [(h, w, c[:4]), (h, w, c.double()), (h, w, c.cpu()), (h.half(), w, c), (h, w, c.clone().requires_grad_(True))]:
+        with pytest.raises(RuntimeError):
+            synthesis.depth_from_bins(*args)

@@ -1,0 +1,210 @@
+"""optim.orthogonalize and optim.Muon against the formulas in float64.
+
+Tolerance of a step: operands in 22 bits with the product of the low parts dropped (2^-21 a product), float32 sums.  An error
+made in one step is carried by the derivative of the polynomial, at most a = 3.4445 per step where singular values are small
+and below 4 elsewhere, so five steps carry the first one's by at most 4^5; all of them together by 4^5 * 4/3.  Each step's
+own error, in the Frobenius norm of X, is at most 8 * 2^-21 sqrt(terms) (three products, coefficients of size 5): the bound is
+4^5 * 4/3 * 8 * 2^-21 = 5.2e-3 of the input's norm, which is 1 after the division -- against results whose norm is sqrt(rank).
+Measured errors are far smaller because small singular directions are lost relative to themselves, not to the norm; what the
+tests allow is 2e-5 of the result's norm per singular-value decade of spread plus half a step of the type."""
+import math
+import os
+
+import pytest
+import torch
+
+from conftest import ROOT  # noqa: F401
+
+DEV = "cuda:0"
+CO = (3.4445, -4.7750, 2.0315)
+U = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+
+
+def _oracle(g, steps=5, co=CO, eps=1e-7):
+    x = g.double().cpu()
+    x = x / (x.square().sum(dim=(-2, -1), keepdim=True).sqrt() + eps)
+    for _ in range(steps):
+        if x.shape[-2] <= x.shape[-1]:
+            a = x @ x.mT
+            x = co[0] * x + (co[1] * a + co[2] * (a @ a)) @ x
+        else:
+            a = x.mT @ x
+            x = co[0] * x + x @ (co[1] * a + co[2] * (a @ a))
+    return x
+
+
+def _error(got, want):
+    return float((got.double().cpu() - want).norm() / max(float(want.norm()), 1e-300))
+
+
+def _update(shape, dtype, seed, kind="gauss"):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(*shape, generator=g)
+    if kind == "decay":                      # a spectrum of three decades
+        u, s, v = torch.linalg.svd(x.double(), full_matrices=False)
+        k = s.shape[-1]
+        x = ((u * torch.logspace(0, -3, k, dtype=torch.float64)) @ v).float()
+    elif kind == "few":                      # a few strong directions over noise
+        m, n = shape[-2:]
+        x = 0.01 * x + torch.randn(*shape[:-2], m, 3, generator=g) @ torch.randn(*shape[:-2], 3, n, generator=g)
+    return x.to(dtype).to(DEV)
+
+
+SHAPES = [(1, 1), (1, 7), (7, 1), (2, 2), (5, 3), (3, 5), (16, 16), (64, 147), (65, 64), (64, 64), (63, 130), (128, 128),
+          (129, 257), (257, 129), (200, 1000), (1000, 200), (2, 33, 17), (3, 1, 40, 72), (384, 384)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_against_float64(shape, dtype):
+    from depth_estimation_amd import optim
+    for kind in ("gauss", "decay", "few"):
+        g = _update(shape, dtype, seed=sum(shape), kind=kind)
+        out = optim.orthogonalize(g)
+        assert out.shape == g.shape and out.dtype == dtype
+        assert _error(out, _oracle(g)) <= 2e-5 * (4 if kind == "decay" else 2) + U[dtype], kind
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(700, 700), (1100, 300), (300, 2049)], ids=str)
+def test_larger_tiles(shape):
+    from depth_estimation_amd import optim
+    g = _update((20,) + shape if shape[0] < 600 else shape, torch.float32, seed=1)
+    assert _error(optim.orthogonalize(g), _oracle(g)) <= 4e-5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("steps", [0, 1, 2, 7])
+def test_steps_coefficients_and_eps(steps):
+    from depth_estimation_amd import optim
+    for shape in ((20, 50), (50, 20)):
+        g = _update(shape, torch.float32, seed=steps)
+        for co, eps in ((CO, 1e-7), ((1.875, -1.25, 0.375), 0.5), ((1.5, -0.5, 0.0), 0.0)):
+            assert _error(optim.orthogonalize(g, steps=steps, coefficients=co, eps=eps), _oracle(g, steps, co, eps)) <= 8e-5
+
+
+@pytest.mark.gpu
+def test_singular_values_end_near_one():
+    from depth_estimation_amd import optim
+    s = torch.linalg.svdvals(optim.orthogonalize(_update((100, 300), torch.float32, 3)).cpu().double())
+    assert 0.6 < float(s.min()) and float(s.max()) < 1.3
+
+
+@pytest.mark.gpu
+def test_zeros_scales_layouts_and_non_finite():
+    from depth_estimation_amd import optim
+    z = torch.zeros(30, 40, device=DEV)
+    assert not optim.orthogonalize(z).any()
+    g = _update((48, 80), torch.float32, 4)
+    base = optim.orthogonalize(g, eps=0.0)
+    for f in (2.0 ** 60, 2.0 ** -60, 2.0 ** -100):      # the norm is taken in float64: no size is lost
+        assert torch.equal(optim.orthogonalize(g * f, eps=0.0), base)
+    wide = torch.zeros(48, 99, device=DEV)
+    wide[:, 3:83] = g
+    assert torch.equal(optim.orthogonalize(wide[:, 3:83], eps=0.0), base)
+    assert torch.equal(optim.orthogonalize(g.t().contiguous().t(), eps=0.0), base)
+    shifted = torch.zeros(48 * 80 + 1, device=DEV)
+    shifted[1:] = g.reshape(-1)
+    assert torch.equal(optim.orthogonalize(shifted[1:].view(48, 80), eps=0.0), base)
+    both = torch.stack([g, 3 * z[0].new_ones(48, 80)])
+    assert torch.equal(optim.orthogonalize(both, eps=0.0)[0], base)      # a batch's matrices do not see each other
+    g[5, 5] = float("nan")
+    both = torch.stack([g, wide[:, 3:83]])
+    out = optim.orthogonalize(both, eps=0.0)
+    assert torch.isnan(out[0]).all() and torch.equal(out[1], base)
+    assert optim.orthogonalize(torch.zeros(0, 4, 5, device=DEV)).shape == (0, 4, 5)
+    assert optim.orthogonalize(torch.zeros(3, 0, device=DEV)).shape == (3, 0)
+
+
+@pytest.mark.gpu
+def test_streams_and_captured_graphs():
+    from depth_estimation_amd import optim
+    a, b = _update((64, 147), torch.float32, 5), _update((300, 100), torch.bfloat16, 6)
+    want = optim.orthogonalize(a), optim.orthogonalize(b)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graphs = []
+    for x in (a, b):
+        with torch.cuda.stream(s):
+            optim.orthogonalize(x)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            out = optim.orthogonalize(x)
+        graphs.append((g, out))
+    for _ in range(3):
+        for g, out in graphs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for g, _ in graphs:
+            g.replay()
+        eager = optim.orthogonalize(a), optim.orthogonalize(b)
+        torch.cuda.synchronize()
+        for (g, out), w, e in zip(graphs, want, eager):
+            assert torch.equal(out, w) and torch.equal(e, w)
+
+
+@pytest.mark.gpu
+def test_muon_steps():
+    """Three steps of a small set of parameters (two of one shape, a convolution, one without a gradient) against the formula."""
+    from depth_estimation_amd import optim
+    gen = torch.Generator().manual_seed(7)
+    shapes = [(30, 20), (30, 20), (16, 3, 7, 7), (8, 8)]
+    ps = [torch.nn.Parameter(torch.randn(*s, generator=gen).to(DEV)) for s in shapes]
+    lr, mom, wd = 0.05, 0.9, 0.1
+    opt = optim.Muon(ps, lr=lr, momentum=mom, weight_decay=wd)
+    ref = [p.detach().double().cpu() for p in ps]
+    bufs = [torch.zeros_like(r) for r in ref]
+    for _ in range(3):
+        for i, p in enumerate(ps):
+            p.grad = None if i == 3 else torch.randn(p.shape, generator=gen).to(DEV)
+        opt.step()
+        for i, p in enumerate(ps[:3]):
+            g = p.grad.double().cpu()
+            bufs[i] = mom * bufs[i] + g
+            u = (g + mom * bufs[i]).flatten(1)
+            o = _oracle(u.float()).view(p.shape)
+            ref[i] = ref[i] * (1 - lr * wd) - lr * max(1.0, u.shape[0] / u.shape[1]) ** 0.5 * o
+    for i, p in enumerate(ps):
+        assert _error(p.detach(), ref[i]) <= 1e-4
+    state = opt.state_dict()
+    other = optim.Muon(ps, lr=lr)
+    other.load_state_dict(state)
+    assert torch.equal(other.state[ps[0]]["momentum_buffer"], opt.state[ps[0]]["momentum_buffer"])
+
+
+def test_refusals_on_the_host():
+    from depth_estimation_amd import _lib as L, optim
+    with pytest.raises(RuntimeError, match="GPU"):
+        optim.orthogonalize(torch.zeros(4, 4))
+    with pytest.raises(ValueError):
+        optim.Muon([torch.nn.Parameter(torch.zeros(4))])
+    for bad in (dict(lr=-1.0), dict(momentum=1.0), dict(weight_decay=-0.1)):
+        with pytest.raises(ValueError):
+            optim.Muon([torch.nn.Parameter(torch.zeros(4, 4))], **bad)
+    if not os.path.exists(L.LIB_PATH):
+        pytest.skip("libdepthsynth.so not built (run __graft_entry__.build())")
+    import ctypes as C
+    lib, fake, co = L.lib(), 0x1000, (C.c_double * 3)(*CO)
+
+    def call(u=fake, dt=0, b=1, m=8, n=8, steps=5, c=co, eps=1e-7, out=fake, ws=fake, nb=1 << 40):
+        return lib.ds_orthogonalize(u, dt, b, m, n, steps, c, eps, out, ws, nb, None)
+
+    for rc, want in [(call(u=None), -1), (call(out=None), -1), (call(c=None), -1), (call(steps=-1), -1), (call(eps=-1.0), -1),
+                     (call(eps=math.nan), -1), (call(b=0), -1), (call(m=0), -1), (call(n=-3), -1), (call(dt=3), -2),
+                     (call(steps=33), -2), (call(m=1 << 17), -2), (call(m=40000, n=40000), -2), (call(b=70000), -2),
+                     (call(ws=None), -3), (call(nb=16), -3), (call(ws=fake + 8), -3), (call(out=fake + 4), -1)]:
+        assert rc == want
+    assert lib.ds_orthogonalize_workspace_bytes(1, 0, 4) == 0
+
+
+@pytest.mark.gpu
+def test_refusals_of_tensors():
+    from depth_estimation_amd import optim
+    g = torch.zeros(4, 4, device=DEV)
+    for args, kw in [((g[0],), {}), ((g.double(),), {}), ((g.int(),), {}), ((g,), dict(steps=-1)), ((g,), dict(steps=40)),
+                     ((g,), dict(coefficients=(1.0, 2.0))), ((g,), dict(coefficients=(1.0, 2.0, math.inf))),
+                     ((g,), dict(eps=-1.0)), ((g,), dict(eps=math.nan))]:
+        with pytest.raises(RuntimeError):
+            optim.orthogonalize(*args, **kw)
