@@ -105,18 +105,27 @@ struct Stager {
     }
 };
 
-// the fragment of 16 rows m0..m0+15 and 32 k (sub-step kk of the tile's two): lane l holds row l%16, k = 8*(l/16)..+7
+// Fragments of 16 rows and 32 k out of an LDS tile: lane l holds row l % 16, k = 8 (l / 16) .. + 7.  Fragment i of a wave whose
+// rows begin at m0 (a multiple of 16 times the power of two above i), sub-step kk of the tile's two: what depends on the lane
+// is one number, the rest constants and exclusive-ors of constants.
 template <Lay L, int R>
-__device__ __forceinline__ s16x8 fragment(const char* lds, int m0, int kk, int lane) {
-    if (L == kK) return *reinterpret_cast<const s16x8*>(lds + lds_chunk<L, R>(m0 + (lane & 15), kk * 4 + (lane >> 4)));
-    const int k = kk * 32 + (lane >> 4) * 8 + ((lane >> 2) & 3);
-    typedef __attribute__((address_space(3))) s16x4* lp;
-    const char* a0 = lds + lds_chunk<L, R>(k, m0 / 8 + ((lane >> 1) & 1)) + (lane & 1) * 8;
-    const char* a1 = lds + lds_chunk<L, R>(k + 4, m0 / 8 + ((lane >> 1) & 1)) + (lane & 1) * 8;
-    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(a0));
-    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(a1));
-    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-}
+struct Fragments {
+    int base;
+    __device__ __forceinline__ Fragments(int m0, int lane) {
+        if (L == kK)
+            base = lds_chunk<L, R>(m0 + (lane & 15), lane >> 4);
+        else
+            base = lds_chunk<L, R>((lane >> 4) * 8 + ((lane >> 2) & 3), m0 / 8 + ((lane >> 1) & 1)) + (lane & 1) * 8;
+    }
+    __device__ __forceinline__ s16x8 get(const char* tile, int i, int kk) const {
+        if (L == kK) return *reinterpret_cast<const s16x8*>(tile + (base ^ (kk << 6)) + i * 16 * (kBK * 2));
+        typedef __attribute__((address_space(3))) s16x4* lp;
+        const char* p = tile + (base ^ (i << 5)) + kk * 32 * (R * 2);
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p));
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 4 * (R * 2)));
+        return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
 
 // acc[i][j][e]: C at m = m0 + wave's row + 16 i + 4 (lane / 16) + e, n = n0 + wave's column + 16 j + lane % 16, over k in
 // [kbeg, kend) (kbeg a multiple of 64).  `lds`: S::kLds bytes.  Ends behind a barrier: the caller may reuse `lds`.
@@ -130,6 +139,8 @@ __device__ __forceinline__ void gemm_tile(const Operand& A, const Operand& B, in
     for (int i = 0; i < S::FM; ++i)
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const Fragments<LA, S::BM> fa(wm, lane);
+    const Fragments<LB, S::BN> fb(wn, lane);
     Stager<LA, S::BM, S::T> sa;
     Stager<LB, S::BN, S::T> sb;
     const int steps = (kend - kbeg + kBK - 1) / kBK * SPLIT;
@@ -153,9 +164,9 @@ __device__ __forceinline__ void gemm_tile(const Operand& A, const Operand& B, in
         for (int kk = 0; kk < kBK / 32; ++kk) {
             s16x8 a[S::FM], b[S::FN];
 #pragma unroll
-            for (int i = 0; i < S::FM; ++i) a[i] = fragment<LA, S::BM>(buf, wm + 16 * i, kk, lane);
+            for (int i = 0; i < S::FM; ++i) a[i] = fa.get(buf, i, kk);
 #pragma unroll
-            for (int j = 0; j < S::FN; ++j) b[j] = fragment<LB, S::BN>(buf + kA, wn + 16 * j, kk, lane);
+            for (int j = 0; j < S::FN; ++j) b[j] = fb.get(buf + kA, j, kk);
 #pragma unroll
             for (int i = 0; i < S::FM; ++i)
 #pragma unroll
@@ -167,6 +178,194 @@ __device__ __forceinline__ void gemm_tile(const Operand& A, const Operand& B, in
         }
         __syncthreads();
     }
+}
+
+// ---- the large shape: 256 x 256, eight waves in two groups that take turns ---------------------------------------------
+//
+// At this size a step (64 k) is 2048 cycles of matrix instructions and 1536 cycles of LDS reads, which only run side by side
+// if different waves do them: every SIMD holds one wave of each group, and while one group multiplies, the other fetches its
+// operands of the next 32 k; an s_barrier ends each turn.  Tiles come to LDS by DMA (buffer_load ... lds: no registers, no
+// LDS store instructions), the next step's under way during the whole current one, and the next tile's first step during the
+// last one of the tile before, so that a workgroup that goes through several tiles waits for memory once.
+//   4096 x 4096 x 4096 bf16: 109 us = 1266 TFLOP/s (register-staged 128 x 128 tiles: 166 us; the same 256 x 256 tile with
+//   all waves in step: 142 us); a library product of that size reaches 1436 TFLOP/s here.
+
+// 16 bytes per lane from a buffer to LDS at `lds` + 16 * lane; out-of-range lanes write zeros.  In assembly because the
+// compiler, which cannot tell the two buffers apart, would wait for every such load before the next LDS read; wait_dma()
+// before a barrier is the wait.  The instruction has no destination register.  (m0 holds the LDS address; the compiler warns
+// that it reserves the register for itself, and sets it anew before each use of its own.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void dma16(unsigned lds, unsigned off, rsrc_t r) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(lds), "v"(off), "s"(r)
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
+__device__ __forceinline__ void wait_dma() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void turn() {   // end of a turn; nothing moves across it
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// a wave's share of one operand's tile: N16 DMA instructions, offsets kept per lane
+template <Lay L, int R, int T>
+struct Mover {
+    static constexpr int N16 = R * kBK * 2 / 16 / T;
+    static constexpr int CPR = (L == kK ? kBK : R) / 8;
+    unsigned off[N16];
+    // LDS slot p holds row r = p / CPR and, of that row, the chunk c that lds_chunk() puts there (its permutations are
+    // their own inverse)
+    static __device__ __forceinline__ void at(int i, int tid, int& r, int& c) {
+        const int p = i * T + tid, x = p % CPR;
+        r = p / CPR;
+        if (L == kK) {
+            c = x ^ (r & 7);
+        } else {
+            const int swz = ((r & 3) | ((r >> 1) & 4)) & (R / 16 - 1);
+            c = (((x >> 1) ^ swz) << 1) | (x & 1);
+        }
+    }
+    __device__ __forceinline__ void init(const Operand& o, int r0, int tid) {
+#pragma unroll
+        for (int i = 0; i < N16; ++i) {
+            int r, c;
+            at(i, tid, r, c);
+            const bool in = L == kK ? r0 + r < o.outer : r0 + c * 8 < o.inner;
+            off[i] = in ? (unsigned)(r * (int)o.ld + c * 8) * 2u : kOut;
+        }
+    }
+    __device__ __forceinline__ void move(const Operand& o, int r0, int k0, bool lo, unsigned lds, int tid) const {
+        const long long corner = L == kK ? (long long)r0 * o.ld + k0 : (long long)k0 * o.ld + r0;
+        const rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<char*>(static_cast<const char*>(o.p) + 2 * (corner + (lo ? o.lo : 0))), 0, 0x7fffffff, 0x00020000);
+        const unsigned base = __builtin_amdgcn_readfirstlane(lds + (tid >> 6) * 1024);
+        const int left = (L == kK ? o.inner : o.outer) - k0;
+        if (left >= kBK) {
+#pragma unroll
+            for (int i = 0; i < N16; ++i) dma16(base + i * T * 16, off[i], rs);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N16; ++i) {
+                int r, c;
+                at(i, tid, r, c);
+                dma16(base + i * T * 16, (L == kK ? c * 8 : r) < left ? off[i] : kOut, rs);
+            }
+        }
+    }
+};
+
+typedef Shape<256, 256, 2, 4> Big;
+
+// What a workgroup multiplies next.  A tile of no steps is given one step of zeros.
+struct Job {
+    Operand A, B;
+    int m0, n0, kbeg, kend;
+};
+
+template <class T, Lay LA, Lay LB, int SPLIT>
+struct TileStream {
+    using S = Big;
+    Mover<LA, S::BM, S::T> ma;
+    Mover<LB, S::BN, S::T> mb;
+    Job job;
+    int steps, parity, tid;
+    char* lds;       // S::kLds bytes that nothing else uses
+
+    __device__ __forceinline__ void move(int s) {
+        const int k0 = job.kbeg + s / SPLIT * kBK, ph = s % SPLIT;
+        const unsigned buf = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds +
+                             ((s + parity) & 1) * ((S::BM + S::BN) * kBK * 2);
+        ma.move(job.A, job.m0, k0, SPLIT == 3 && ph == 0, buf, tid);
+        mb.move(job.B, job.n0, k0, SPLIT == 3 && ph == 1, buf + S::BM * kBK * 2, tid);
+    }
+    // takes up a job and sets its first step under way
+    __device__ __forceinline__ void start(const Job& j) {
+        job = j;
+        const int n = (j.kend - j.kbeg + kBK - 1) / kBK * SPLIT;
+        steps = n > 0 ? n : 1;
+        ma.init(j.A, j.m0, tid);
+        mb.init(j.B, j.n0, tid);
+        move(0);
+    }
+    __device__ __forceinline__ TileStream(char* lds_, const Job& j) : parity(0), tid(threadIdx.x), lds(lds_) { start(j); }
+
+    // Multiplies the job that start() took up.  next(Job&) -> bool names the one after it, whose first step is then under way
+    // on return.  All waves leave together; acc as in gemm_tile.
+    template <class Next>
+    __device__ __forceinline__ void multiply(f32x4 (&acc)[S::FM][S::FN], Next next) {
+        const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = wave / S::WN;
+        const int wm = group * S::FM * 16, wn = (wave % S::WN) * S::FN * 16;
+        constexpr int kA = S::BM * kBK * 2, kBuf = (S::BM + S::BN) * kBK * 2;
+        const Fragments<LA, S::BM> fa(wm, lane);
+        const Fragments<LB, S::BN> fb(wn, lane);
+#pragma unroll
+        for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+            for (int j = 0; j < S::FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        wait_dma();
+        turn();
+        if (group == 1) turn();       // half a step behind the other group from here on
+        const int n = steps;
+        for (int s = 0; s < n; ++s) {
+            const char* buf = lds + ((s + parity) & 1) * kBuf;
+            s16x8 a[S::FM], b[S::FN];
+#pragma unroll
+            for (int j = 0; j < S::FN; ++j) b[j] = fb.get(buf + kA, j, 0);
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i) a[i] = fa.get(buf, i, 0);
+            // the other buffer was read for the last time in the turn before this one (group 1's second half of step s - 1)
+            if (s + 1 < n) {
+                move(s + 1);
+            } else {
+                Job j;
+                if (next(j)) {
+                    parity = (parity + n) & 1;
+                    start(j);
+                }
+            }
+            wait_lds();
+            turn();
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+                for (int j = 0; j < S::FN; ++j) acc[i][j] = mfma(a[i], b[j], acc[i][j], T());
+            __builtin_amdgcn_s_setprio(0);
+            turn();
+#pragma unroll
+            for (int j = 0; j < S::FN; ++j) b[j] = fb.get(buf + kA, j, 1);
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i) a[i] = fa.get(buf, i, 1);
+            wait_lds();
+            // both groups' shares of the next step have arrived when the turn ends in which group 1 reads this step's last
+            if (group == 1 && s + 1 < n) wait_dma();
+            turn();
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+                for (int j = 0; j < S::FN; ++j) acc[i][j] = mfma(a[i], b[j], acc[i][j], T());
+            __builtin_amdgcn_s_setprio(0);
+            if (group == 0 && s + 1 < n) wait_dma();
+            turn();
+        }
+        if (group == 0) turn();
+    }
+};
+
+// Tile t of mt x nt in the order in which they are taken: workgroup b runs on XCD b % 8, each with an L2 of its own, so every
+// XCD gets a contiguous share, and inside it bands of four tile columns are gone through row by row: the tiles in flight on an
+// XCD share a few rows and columns.
+__device__ __forceinline__ void tile_of(int t, int tiles, int mt, int nt, int& m, int& n) {
+    const int q = tiles >> 3, r = tiles & 7, x = t & 7;
+    const int u = x * q + (x < r ? x : r) + (t >> 3);
+    const int band = u / (4 * mt), in = u - band * 4 * mt, w = nt - band * 4 < 4 ? nt - band * 4 : 4;
+    n = band * 4 + in % w;
+    m = in / w;
 }
 
 // x as two fp16 numbers: hi = x to 11 bits, lo = the rest to 11 bits.  Where hi is not finite lo is 0, so that an infinity

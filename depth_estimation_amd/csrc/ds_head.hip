@@ -43,6 +43,8 @@ __device__ __forceinline__ float from_bits(unsigned u) { return __builtin_bit_ca
 // max over finite magnitudes: an infinity or a NaN in one place must not take the scale from all others
 __device__ __forceinline__ float finite_abs(float x) { return __builtin_isfinite(x) ? fabsf(x) : 0.f; }
 
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
+
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
@@ -186,57 +188,68 @@ __global__ __launch_bounds__(256) void stage_kernel(const IT* __restrict__ x, lo
 }
 
 // ------------------------------------------------------------------------------------------------------------ forward
-template <int SPLIT>
-__device__ __forceinline__ float logit_of(float acc, float ih, float iw) {
-    return SPLIT == 3 ? acc * ih * iw : acc;
-}
-
-// One tile of l^T: classes along m, rows along n, so that a lane holds 4 FM classes of FN rows and most of the softmax stays
-// inside it.  part: three planes [class tile][row].
-template <class T, class S, int SPLIT>
-__global__ __launch_bounds__(S::T) void head_stats_kernel(Operand W, Operand H, const HeadState* __restrict__ st, int V, int D,
-                                                          int mode, const int* __restrict__ tgt,
-                                                          const float* __restrict__ centers, float* __restrict__ tlogit,
-                                                          float* __restrict__ part, long long plane, int ld_part) {
-    __shared__ __align__(16) char lds[S::kLds];
-    const int vt = cdiv(V, S::BM);
-    const int m0 = (int)(blockIdx.x % vt) * S::BM, n0 = (int)(blockIdx.x / vt) * S::BN;
-    const int cnt = st->count;
-    if (n0 >= cnt) return;
-    H.outer = cnt;
-    f32x4 acc[S::FM][S::FN];
-    gemm_tile<T, S, kK, kK, SPLIT>(W, H, m0, n0, 0, D, lds, acc);
-    const float ih = SPLIT == 3 ? 1.f / scale_for(from_bits(st->amax_h)) : 1.f;
-    const float iw = SPLIT == 3 ? 1.f / scale_for(from_bits(st->amax_w)) : 1.f;
+// Statistics of one tile of l^T: classes along m, rows along n, so that a lane holds 4 FM classes of FN rows and most of the
+// softmax stays inside it.  part: three planes [class tile][row].  red: [WM][BN][3] floats in LDS; behind a barrier on entry
+// and on return.
+struct StatsArgs {
+    int V;
+    const int* tgt;
+    const float* centers;
+    float* tlogit;
+    float* part;
+    long long plane;
+    int ld_part;
+};
+template <class S, int SPLIT, int MODE>
+__device__ __forceinline__ void stats_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int cnt, const HeadState* st,
+                                              const StatsArgs& a, float* red) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = wave / S::WN, wn = wave % S::WN;
-    float* red = reinterpret_cast<float*>(lds);   // [WM][BN][3]
+    const int wm = wave / S::WN, wn = wave % S::WN, v0 = m0 + wm * S::FM * 16 + (lane >> 4) * 4;
+    if (SPLIT == 3) {
+        const float ih = 1.f / scale_for(from_bits(st->amax_h)), iw = 1.f / scale_for(from_bits(st->amax_w));
+#pragma unroll
+        for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+            for (int j = 0; j < S::FN; ++j) acc[i][j] = acc[i][j] * ih * iw;
+    }
+    const bool edge = m0 + S::BM > a.V;      // only the last class tile has classes that do not exist
 #pragma unroll
     for (int j = 0; j < S::FN; ++j) {
         const int nl = (wn * S::FN + j) * 16 + (lane & 15), n = n0 + nl;
-        const int t = mode == kCE && n < cnt ? tgt[n] : -1;
+        if (edge) {
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (v0 + i * 16 + e >= a.V) acc[i][j][e] = -INFINITY;
+        }
+        if (MODE == kCE) {
+            const int t = n < cnt ? a.tgt[n] - v0 : -1;     // the row's class, counted from this lane's first one
+            if (t >= 0 && t < S::FM * 16 && (t & 15) < 4) {
+                float l = 0.f;
+#pragma unroll
+                for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (t == i * 16 + e) l = acc[i][j][e];
+                a.tlogit[n] = l;
+            }
+        }
         float mx = -INFINITY, s = 0.f, sc = 0.f;
 #pragma unroll
         for (int i = 0; i < S::FM; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int v = m0 + (wm * S::FM + i) * 16 + (lane >> 4) * 4 + e;
-                const float l = logit_of<SPLIT>(acc[i][j][e], ih, iw);
-                if (v == t) tlogit[n] = l;
-                // a comparison, not fmaxf: a NaN has to reach the row's sum
-                if (v < V && !(l <= mx)) mx = l;
-                acc[i][j][e] = l;
-            }
+            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, acc[i][j][e]);     // passes over NaN, which reaches the sum below
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float ref = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
         for (int i = 0; i < S::FM; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int v = m0 + (wm * S::FM + i) * 16 + (lane >> 4) * 4 + e;
-                const float x = v < V ? __expf(acc[i][j][e] - (mx == -INFINITY ? 0.f : mx)) : 0.f;
+                const float x = exp_of(acc[i][j][e] - ref);
                 s += x;
-                if (mode == kExpect && v < V) sc = fmaf(x, centers[v], sc);
+                if (MODE == kExpect) sc = fmaf(x, edge && v0 + i * 16 + e >= a.V ? 0.f : a.centers[v0 + i * 16 + e], sc);
             }
         s += __shfl_xor(s, 16, 64);
         s += __shfl_xor(s, 32, 64);
@@ -259,14 +272,57 @@ __global__ __launch_bounds__(S::T) void head_stats_kernel(Operand W, Operand H, 
 #pragma unroll
         for (int w = 0; w < S::WM; ++w) {
             const float* q = red + (w * S::BN + nl) * 3;
-            const float f = __expf(q[0] - ref);
+            const float f = exp_of(q[0] - ref);
             s += q[1] * f;
             sc += q[2] * f;
         }
-        float* q = part + (long long)(m0 / S::BM) * ld_part + n0 + nl;
+        float* q = a.part + (long long)(m0 / S::BM) * a.ld_part + n0 + nl;
         q[0] = mx;
-        q[plane] = s;
-        if (mode == kExpect) q[2 * plane] = sc;
+        q[a.plane] = s;
+        if (MODE == kExpect) q[2 * a.plane] = sc;
+    }
+    __syncthreads();
+}
+
+template <class T, class S, int SPLIT, int MODE>
+__global__ __launch_bounds__(S::T) void head_stats_kernel(Operand W, Operand H, const HeadState* __restrict__ st, int D,
+                                                          StatsArgs a) {
+    __shared__ __align__(16) char lds[S::kLds];
+    const int vt = cdiv(a.V, S::BM);
+    const int m0 = (int)(blockIdx.x % vt) * S::BM, n0 = (int)(blockIdx.x / vt) * S::BN;
+    const int cnt = st->count;
+    if (n0 >= cnt) return;
+    H.outer = cnt;
+    f32x4 acc[S::FM][S::FN];
+    gemm_tile<T, S, kK, kK, SPLIT>(W, H, m0, n0, 0, D, lds, acc);
+    stats_of_tile<S, SPLIT, MODE>(acc, m0, n0, cnt, st, a, reinterpret_cast<float*>(lds));
+}
+
+// the same in tiles of 256 x 256, a workgroup going through several
+template <class T, int SPLIT, int MODE>
+__global__ __launch_bounds__(Big::T) void head_stats_big_kernel(Operand W, Operand H, const HeadState* __restrict__ st, int D,
+                                                                StatsArgs a) {
+    __shared__ __align__(16) char lds[Big::kLds];
+    __shared__ float red[Big::WM * Big::BN * 3];
+    const int cnt = st->count, mt = cdiv(a.V, Big::BM), nt = cdiv(cnt, Big::BN), tiles = mt * nt;
+    int t = blockIdx.x;
+    if (t >= tiles) return;
+    H.outer = cnt;
+    auto job = [&](int u) {
+        int m, n;
+        tile_of(u, tiles, mt, nt, m, n);
+        return Job{W, H, m * Big::BM, n * Big::BN, 0, D};
+    };
+    TileStream<T, kK, kK, SPLIT> stream(lds, job(t));
+    for (; t < tiles; t += gridDim.x) {
+        const int m0 = stream.job.m0, n0 = stream.job.n0;
+        f32x4 acc[Big::FM][Big::FN];
+        stream.multiply(acc, [&](Job& j) {
+            const int u = t + gridDim.x;
+            if (u < tiles) j = job(u);
+            return u < tiles;
+        });
+        stats_of_tile<Big, SPLIT, MODE>(acc, m0, n0, cnt, st, a, red);
     }
 }
 
@@ -286,7 +342,7 @@ __global__ __launch_bounds__(256) void head_join_kernel(const float* __restrict_
         for (int t = y; t < tiles; t += 8) {
             const float* q = part + (long long)t * ld_part + n;
             const float m = q[0], nm = fmaxf(mx, m), ref = nm == -INFINITY ? 0.f : nm;
-            const float f0 = __expf(mx - ref), f1 = __expf(m - ref);
+            const float f0 = exp_of(mx - ref), f1 = exp_of(m - ref);
             s = s * f0 + q[plane] * f1;
             if (mode == kExpect) sc = sc * f0 + q[2 * plane] * f1;
             mx = nm;
@@ -303,7 +359,7 @@ __global__ __launch_bounds__(256) void head_join_kernel(const float* __restrict_
             const float ref = mx == -INFINITY ? 0.f : mx;
             s = sc = 0.f;
             for (int i = 0; i < 8; ++i) {
-                const float f = __expf(red[i][x][0] - ref);
+                const float f = exp_of(red[i][x][0] - ref);
                 s += red[i][x][1] * f;
                 sc += red[i][x][2] * f;
             }
@@ -393,133 +449,192 @@ __global__ __launch_bounds__(256) void back_scale_kernel(Upstream u, const HeadS
 // dl of classes [v0, v0 + cols) in 16 bits: [row][class - v0], pitch ld (cols rounded up to 8; zeros behind the last class).
 // The rounding to 16 bits is the products' operand rounding: half a step of the gradients' own type for 16-bit inputs, 2^-22
 // with the two planes of fp32 inputs; p - 1 and c - E are formed in fp32 before it.
-template <class T, class S, int SPLIT>
+struct DlArgs {
+    int v0, cols;
+    const int* tgt;
+    const float* centers;
+    const float* top;
+    const float* inv_sum;
+    const float* mean;
+    Upstream up;
+    void* dl;
+    int ld;
+    long long lo;
+};
+template <class T, class S, int SPLIT, int MODE>
+__device__ __forceinline__ void dl_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int cnt, const HeadState* st,
+                                           const BackState* bs, const DlArgs& a) {
+    const float il = SPLIT == 3 ? 1.f / scale_for(from_bits(st->amax_h)) : 1.f;
+    const float iw = SPLIT == 3 ? 1.f / scale_for(from_bits(st->amax_w)) : 1.f;
+    const float norm = Store<T>::k / dl_norm(bs, MODE);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wm = wave / S::WN, wn = wave % S::WN, c0 = m0 + wm * S::FM * 16 + (lane >> 4) * 4;
+    T* dl = static_cast<T*>(a.dl);
+    const bool edge = m0 + S::BM > a.cols;
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) {
+        const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
+        if (n >= cnt) continue;
+        const float tp = a.top[n], rs = a.inv_sum[n];
+        float g = upstream(a.up, n, cnt) * norm;
+        if (MODE == kCE) {
+            const int t = a.tgt[n] - a.v0 - c0;
+            if (a.tgt[n] < 0) g = __builtin_nanf("");
+            const float gr = g * rs;
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float l = SPLIT == 3 ? acc[i][j][e] * il * iw : acc[i][j][e];
+                    const float x = exp_of(l - tp);
+                    acc[i][j][e] = t == i * 16 + e ? (x * rs - 1.f) * g : x * gr;
+                }
+        } else {
+            const float e0 = a.mean[n], gr = g * rs;
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int c = c0 + i * 16 + e;
+                    const float l = SPLIT == 3 ? acc[i][j][e] * il * iw : acc[i][j][e];
+                    acc[i][j][e] = exp_of(l - tp) * gr * ((edge && c >= a.cols ? 0.f : a.centers[a.v0 + c]) - e0);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < S::FM; ++i) {
+            const int c = c0 + i * 16;
+            if (edge && c >= a.ld) continue;
+            float d[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[e] = edge && c + e >= a.cols ? 0.f : acc[i][j][e];
+            put4<SPLIT>(dl + (long long)n * a.ld + c, a.lo, d);
+        }
+    }
+}
+template <class T, class S, int SPLIT, int MODE>
 __global__ __launch_bounds__(S::T) void head_dl_kernel(Operand W, Operand H, const HeadState* __restrict__ st,
-                                                       const BackState* __restrict__ bs, int V, int D, int v0, int cols, int mode,
-                                                       const int* __restrict__ tgt, const float* __restrict__ centers,
-                                                       const float* __restrict__ top, const float* __restrict__ inv_sum,
-                                                       const float* __restrict__ mean, Upstream up, T* __restrict__ dl, int ld, long long lo) {
+                                                       const BackState* __restrict__ bs, int D, DlArgs a) {
     __shared__ __align__(16) char lds[S::kLds];
-    const int vt = cdiv(cols, S::BM);
+    const int vt = cdiv(a.cols, S::BM);
     const int m0 = (int)(blockIdx.x % vt) * S::BM, n0 = (int)(blockIdx.x / vt) * S::BN;
     const int cnt = st->count;
     if (n0 >= cnt) return;
     H.outer = cnt;
     f32x4 acc[S::FM][S::FN];
-    gemm_tile<T, S, kK, kK, SPLIT>(W, H, v0 + m0, n0, 0, D, lds, acc);
-    const float ih = SPLIT == 3 ? 1.f / scale_for(from_bits(st->amax_h)) : 1.f;
-    const float iw = SPLIT == 3 ? 1.f / scale_for(from_bits(st->amax_w)) : 1.f;
-    const float norm = Store<T>::k / dl_norm(bs, mode);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = wave / S::WN, wn = wave % S::WN;
-#pragma unroll
-    for (int j = 0; j < S::FN; ++j) {
-        const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
-        if (n >= cnt) continue;
-        const float tp = top[n], rs = inv_sum[n];
-        const int t = mode == kCE ? tgt[n] : -1;
-        float g = upstream(up, n, cnt) * norm;
-        if (mode == kCE && t < 0) g = __builtin_nanf("");
-        const float e0 = mode == kExpect ? mean[n] : 0.f;
-#pragma unroll
-        for (int i = 0; i < S::FM; ++i) {
-            const int c = m0 + (wm * S::FM + i) * 16 + (lane >> 4) * 4;
-            if (c >= ld) continue;
-            float d[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int v = v0 + c + e;
-                const float p = __expf(logit_of<SPLIT>(acc[i][j][e], ih, iw) - tp) * rs;
-                const float q = mode == kExpect ? p * (v < V ? centers[v] - e0 : 0.f) : p - (v == t ? 1.f : 0.f);
-                d[e] = v < V && c + e < cols ? q * g : 0.f;
-            }
-            put4<SPLIT>(dl + (long long)n * ld + c, lo, d);
-        }
+    gemm_tile<T, S, kK, kK, SPLIT>(W, H, m0, n0, 0, D, lds, acc);
+    dl_of_tile<T, S, SPLIT, MODE>(acc, m0, n0, cnt, st, bs, a);
+}
+template <class T, int SPLIT, int MODE>
+__global__ __launch_bounds__(Big::T) void head_dl_big_kernel(Operand W, Operand H, const HeadState* __restrict__ st,
+                                                             const BackState* __restrict__ bs, int D, DlArgs a) {
+    __shared__ __align__(16) char lds[Big::kLds];
+    const int cnt = st->count, mt = cdiv(a.cols, Big::BM), nt = cdiv(cnt, Big::BN), tiles = mt * nt;
+    int t = blockIdx.x;
+    if (t >= tiles) return;
+    H.outer = cnt;
+    auto job = [&](int u) {
+        int m, n;
+        tile_of(u, tiles, mt, nt, m, n);
+        return Job{W, H, m * Big::BM, n * Big::BN, 0, D};
+    };
+    TileStream<T, kK, kK, SPLIT> stream(lds, job(t));
+    for (; t < tiles; t += gridDim.x) {
+        const int m0 = stream.job.m0, n0 = stream.job.n0;
+        f32x4 acc[Big::FM][Big::FN];
+        stream.multiply(acc, [&](Job& j) {
+            const int u = t + gridDim.x;
+            if (u < tiles) j = job(u);
+            return u < tiles;
+        });
+        dl_of_tile<T, Big, SPLIT, MODE>(acc, m0, n0, cnt, st, bs, a);
     }
 }
 
 // dH = dl W: features along m (W as kM operand, classes are k), rows along n.  ACC: fp32 partials [split][row][Dp4], added to
 // what earlier pieces of the classes left; otherwise straight into the caller's rows.
-template <class T, class S, int SPLIT, class O, bool ACC>
-__global__ __launch_bounds__(S::T) void head_dh_kernel(Operand W, Operand G, const HeadState* __restrict__ st,
-                                                       const BackState* __restrict__ bs, int D, int kcols, int splits, int mode,
-                                                       const int* __restrict__ rows, O* __restrict__ out, float* __restrict__ part,
-                                                       long long part_split, int first) {
-    __shared__ __align__(16) char lds[S::kLds];
-    const int mt = cdiv(D, S::BM);
-    const int b = (int)(blockIdx.x / splits), sp = (int)(blockIdx.x % splits);
-    const int m0 = b % mt * S::BM, n0 = b / mt * S::BN;
-    const int cnt = st->count;
-    if (n0 >= cnt) return;
-    G.outer = cnt;
-    const int per = cdiv(cdiv(kcols, kBK), splits) * kBK, k0 = min(sp * per, kcols), k1 = min(k0 + per, kcols);
-    f32x4 acc[S::FM][S::FN];
-    gemm_tile<T, S, kM, kK, SPLIT>(W, G, m0, n0, k0, k1, lds, acc);
-    const float f0 = dl_norm(bs, mode) / Store<T>::k;
-    const float iw = SPLIT == 3 ? 1.f / scale_for(from_bits(st->amax_w)) : 1.f;
+// dW of one piece = dl^T H: features along m, classes along n, k = rows (both kM operands).
+struct GradArgs {
+    int D, k, splits, mode;      // k: classes of the piece (dH); cols: classes of the piece (dW, whose k is the row count)
+    int cols, first;
+    const int* rows;
+    void* out;
+    float* part;
+    long long part_split;
+};
+// which: 0 = dH, 1 = dW.  Writes the tile of row / class n and features m.
+template <class T, class S, int SPLIT, class O, bool ACC, int WHICH>
+__device__ __forceinline__ void grad_of_tile(const f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int sp, int bound,
+                                             const HeadState* st, const BackState* bs, const GradArgs& a) {
+    const float f0 = dl_norm(bs, a.mode) / Store<T>::k;
+    const float is = SPLIT == 3 ? 1.f / scale_for(from_bits(WHICH == 0 ? st->amax_w : st->amax_h)) : 1.f;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = wave / S::WN, wn = wave % S::WN, Dp = (D + 3) & ~3;
-    const bool aligned = (D & 3) == 0;
+    const int wm = wave / S::WN, wn = wave % S::WN, Dp = (a.D + 3) & ~3;
+    const bool aligned = (a.D & 3) == 0;
 #pragma unroll
     for (int j = 0; j < S::FN; ++j) {
         const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
-        if (n >= cnt) continue;
-        const long long row = ACC ? n : (rows ? rows[n] : n);
+        if (n >= bound) continue;
+        const long long row = !ACC && WHICH == 0 && a.rows ? a.rows[n] : n;
 #pragma unroll
         for (int i = 0; i < S::FM; ++i) {
             const int d = m0 + (wm * S::FM + i) * 16 + (lane >> 4) * 4;
-            if (d >= D) continue;
+            if (d >= a.D) continue;
             if (ACC) {
-                f32x4* q = reinterpret_cast<f32x4*>(part + sp * part_split + row * Dp + d);
+                f32x4* q = reinterpret_cast<f32x4*>(a.part + sp * a.part_split + row * Dp + d);
                 f32x4 v = acc[i][j];
-                if (!first) v += *q;
+                if (WHICH == 0 && !a.first) v += *q;
                 *q = v;
             } else {
                 float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * f0 * iw;
-                put_row4(out + row * D, d, D, v, aligned);
+                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * f0 * is;
+                put_row4(static_cast<O*>(a.out) + row * a.D, d, a.D, v, aligned);
             }
         }
     }
 }
-
-// dW of one piece = dl^T H: features along m, classes along n, k = rows (both kM operands)
-template <class T, class S, int SPLIT, class O, bool ACC>
-__global__ __launch_bounds__(S::T) void head_dw_kernel(Operand H, Operand G, const HeadState* __restrict__ st,
-                                                       const BackState* __restrict__ bs, int D, int cols, int splits, int mode,
-                                                       O* __restrict__ out, float* __restrict__ part, long long part_split) {
+// A: W (dH) or H (dW), B: dl.  Workgroups: tiles x splits, the splits of a tile next to each other.
+template <class T, class S, int SPLIT, class O, bool ACC, int WHICH>
+__global__ __launch_bounds__(S::T) void head_grad_kernel(Operand A, Operand B, const HeadState* __restrict__ st,
+                                                         const BackState* __restrict__ bs, GradArgs a) {
     __shared__ __align__(16) char lds[S::kLds];
-    const int mt = cdiv(D, S::BM);
-    const int b = (int)(blockIdx.x / splits), sp = (int)(blockIdx.x % splits);
-    const int m0 = b % mt * S::BM, n0 = b / mt * S::BN;
-    const int cnt = st->count;
-    H.outer = G.outer = cnt;
-    const int per = cdiv(cdiv(cnt, kBK), splits) * kBK, k0 = min(sp * per, cnt), k1 = min(k0 + per, cnt);
-    f32x4 acc[S::FM][S::FN];
-    gemm_tile<T, S, kM, kM, SPLIT>(H, G, m0, n0, k0, k1, lds, acc);
-    const float f0 = dl_norm(bs, mode) / Store<T>::k;
-    const float ih = SPLIT == 3 ? 1.f / scale_for(from_bits(st->amax_h)) : 1.f;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = wave / S::WN, wn = wave % S::WN, Dp = (D + 3) & ~3;
-    const bool aligned = (D & 3) == 0;
-#pragma unroll
-    for (int j = 0; j < S::FN; ++j) {
-        const int c = n0 + (wn * S::FN + j) * 16 + (lane & 15);
-        if (c >= cols) continue;
-#pragma unroll
-        for (int i = 0; i < S::FM; ++i) {
-            const int d = m0 + (wm * S::FM + i) * 16 + (lane >> 4) * 4;
-            if (d >= D) continue;
-            if (ACC) {
-                *reinterpret_cast<f32x4*>(part + sp * part_split + (long long)c * Dp + d) = acc[i][j];
-            } else {
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * f0 * ih;
-                put_row4(out + (long long)c * D, d, D, v, aligned);
-            }
+    const int cnt = st->count, mt = cdiv(a.D, S::BM), bound = WHICH == 0 ? cnt : a.cols;
+    const int k = WHICH == 0 ? a.k : cnt, per = cdiv(cdiv(k, kBK), a.splits) * kBK;
+    B.outer = cnt;
+    if (WHICH == 1) A.outer = cnt;
+    constexpr Lay LB = WHICH == 0 ? kK : kM;
+    if constexpr (std::is_same<S, Big>::value) {
+        const int nt = cdiv(bound, S::BN), units = mt * nt * a.splits;
+        int t = blockIdx.x;
+        if (t >= units) return;
+        auto job = [&](int u, int& sp) {
+            int x, n;
+            tile_of(u, units, mt * a.splits, nt, x, n);
+            sp = x % a.splits;
+            const int k0 = min(sp * per, k);
+            return Job{A, B, x / a.splits * S::BM, n * S::BN, k0, min(k0 + per, k)};
+        };
+        int sp, next_sp = 0;
+        TileStream<T, kM, LB, SPLIT> stream(lds, job(t, sp));
+        for (; t < units; t += gridDim.x) {
+            const int m0 = stream.job.m0, n0 = stream.job.n0;
+            f32x4 acc[S::FM][S::FN];
+            stream.multiply(acc, [&](Job& j) {
+                const int u = t + gridDim.x;
+                if (u < units) j = job(u, next_sp);
+                return u < units;
+            });
+            grad_of_tile<T, S, SPLIT, O, ACC, WHICH>(acc, m0, n0, sp, bound, st, bs, a);
+            sp = next_sp;
         }
+    } else {
+        const int b = (int)(blockIdx.x / a.splits), sp = (int)(blockIdx.x % a.splits);
+        const int m0 = b % mt * S::BM, n0 = b / mt * S::BN;
+        if (n0 >= bound) return;
+        const int k0 = min(sp * per, k);
+        f32x4 acc[S::FM][S::FN];
+        gemm_tile<T, S, kM, LB, SPLIT>(A, B, m0, n0, k0, min(k0 + per, k), lds, acc);
+        grad_of_tile<T, S, SPLIT, O, ACC, WHICH>(acc, m0, n0, sp, bound, st, bs, a);
     }
 }
 
@@ -557,11 +672,39 @@ __global__ __launch_bounds__(256) void zero_ignored_kernel(const long long* __re
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
-// Shapes: 128x128 outputs a workgroup, four waves of 64x64; 64 features or 32 rows have shapes of their own, whose idle
-// half would otherwise be computed and dropped.
+// Shapes: 256x256 outputs a workgroup (TileStream) for large products; 128x128, four waves of 64x64, below that; 64 features or
+// 32 rows have shapes of their own, whose idle half would otherwise be computed and dropped.
 typedef Shape<128, 128, 2, 2> Sq;
 typedef Shape<64, 128, 1, 4> Flat;    // 64 along m
 typedef Shape<128, 32, 4, 1> Thin;    // 32 along n
+enum ShapeId { kSq, kFlat, kThin, kBig };
+
+// Which shape a product takes and over how many workgroups its sum is split.  Times in us, measured for bf16: a step of 64
+// k costs a 256x256 tile 1.55 and its start and end 4.2 (4096^2 tiles at k = 256 .. 16384); two 128x128 tiles share a CU and
+// take 1.36 and 3 each.  A split sum is written and read once more, at 4 bytes an element and 4 TB/s.
+struct Cut {
+    ShapeId shape;
+    int splits;
+};
+Cut cut_of(long long M, long long N, long long K, int planes, bool may_split) {
+    const long long cu = cu_count(), steps = (K + kBK - 1) / kBK;
+    Cut best{kSq, 1};
+    double least = 1e300;
+    for (int big = 0; big < 2; ++big) {
+        const long long b = big ? 256 : 128, tiles = ((M + b - 1) / b) * ((N + b - 1) / b), slots = big ? cu : 2 * cu;
+        const long long most = may_split ? (steps / 4 < 256 ? steps / 4 : 256) : 1;
+        for (long long s = 1; s <= (most > 1 ? most : 1); s += s < 16 ? 1 : s / 8) {
+            const double per = (double)((steps + s - 1) / s) * (planes == 2 ? 3 : 1);
+            const double t = (double)((tiles * s + slots - 1) / slots) * (big ? 1.55 * per + 4.2 : 1.36 * per + 3.0) +
+                             (s > 1 ? 3.0 + 8e-6 * (double)s * M * N / 4.0 : 0.0);
+            if (t < least) {
+                least = t;
+                best = Cut{big ? kBig : kSq, (int)s};
+            }
+        }
+    }
+    return best;
+}
 
 struct Saved {
     HeadState* st;
@@ -589,7 +732,7 @@ Saved saved_of(void* p, long long N) {
 struct Plan {
     int dtype, planes, Dp, vt_fwd, piece, piece_ld, dh_splits, dw_splits;
     bool stage_w, stage_h, dh_part;
-    bool thin, flat;
+    ShapeId fwd, dl_shape, dh, dw;
     size_t staged_h, staged_w, counts, tlogit, part, sums, fwd_total;      // offsets of the forward's workspace
     size_t bh, bw, bs, dl, dhp, dwp, bwd_total;                            // offsets of the backward's
 };
@@ -608,11 +751,11 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     p.Dp = pad8(D);
     p.stage_w = dtype == DS_F32 || D % 8 != 0;
     p.stage_h = mode == kCE || dtype == DS_F32 || D % 8 != 0 || ldh % 8 != 0;
-    p.thin = N <= 32;
-    p.flat = D <= 64;
     const size_t el = 2 * p.planes;
     const size_t h = p.stage_h ? align256((size_t)N * p.Dp * el) : 0, w = p.stage_w ? align256((size_t)V * p.Dp * el) : 0;
-    p.vt_fwd = cdiv(V, 128);
+    const bool thin = N <= 32, flat = D <= 64;
+    p.fwd = thin ? kThin : cut_of(V, N, D, p.planes, false).shape;
+    p.vt_fwd = cdiv(V, p.fwd == kBig ? Big::BM : Sq::BM);
     size_t o = 0;
     p.staged_h = o; o += h;
     p.staged_w = o; o += w;
@@ -621,14 +764,19 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     p.part = o; o += 3 * align256((size_t)p.vt_fwd * N * 4);
     p.sums = o; o += align256((size_t)cdiv(N, 32) * 8);
     p.fwd_total = o;
-    // a piece of the classes: what fits 256 MB of dl, at least 1024 classes, a multiple of 128
-    const long long fit = (256ll << 20) / ((long long)el * N) / 128 * 128;
+    // a piece of the classes: what fits 256 MB of dl, at least 1024 classes, a multiple of 256
+    const long long fit = (256ll << 20) / ((long long)el * N) / 256 * 256;
     const long long piece = fit < 1024 ? 1024 : fit;
     p.piece = piece >= V ? V : (int)piece;
     p.piece_ld = pad8(p.piece);
-    const int bm = p.flat ? 64 : 128, bn = p.thin ? 32 : 128;
-    p.dh_splits = splits_for((long long)cdiv(D, bm) * cdiv(N, bn), cdiv(p.piece, kBK));
-    p.dw_splits = splits_for((long long)cdiv(D, bm) * cdiv(p.piece, 128), cdiv(N, kBK));
+    p.dl_shape = thin ? kThin : cut_of(p.piece, N, D, p.planes, false).shape;
+    const Cut dh = cut_of(D, N, p.piece, p.planes, true), dw = cut_of(D, p.piece, N, p.planes, true);
+    p.dh = thin ? kThin : flat ? kFlat : dh.shape;
+    p.dh_splits = p.dh == dh.shape ? dh.splits
+                                   : splits_for((long long)cdiv(D, flat && !thin ? 64 : 128) * cdiv(N, thin ? 32 : 128),
+                                                cdiv(p.piece, kBK));
+    p.dw = flat ? kFlat : dw.shape;
+    p.dw_splits = p.dw == dw.shape ? dw.splits : splits_for((long long)cdiv(D, 64) * cdiv(p.piece, 128), cdiv(N, kBK));
     p.dh_part = p.dh_splits > 1 || p.piece < V;
     const size_t D4 = (D + 3) & ~3;
     o = 0;
@@ -680,6 +828,18 @@ void operands(const Plan& p, const IT* hidden, long long ldh, const IT* weight, 
     }
 }
 
+template <class T, int SPLIT, int MODE>
+void stats_launch(const Plan& p, const Operand& W, const Operand& H, const Saved& s, long long N, int D, const StatsArgs& a,
+                  hipStream_t q) {
+    const int tiles = p.vt_fwd * cdiv(N, p.fwd == kThin ? 32 : p.fwd == kBig ? Big::BN : 128);
+    if (p.fwd == kThin)
+        head_stats_kernel<T, Thin, SPLIT, MODE><<<tiles, Thin::T, 0, q>>>(W, H, s.st, D, a);
+    else if (p.fwd == kBig)
+        head_stats_big_kernel<T, SPLIT, MODE><<<tiles < cu_count() ? tiles : cu_count(), Big::T, 0, q>>>(W, H, s.st, D, a);
+    else
+        head_stats_kernel<T, Sq, SPLIT, MODE><<<tiles, Sq::T, 0, q>>>(W, H, s.st, D, a);
+}
+
 template <class IT, class T, int SPLIT>
 int head_fwd(int mode, const IT* hidden, long long ldh, const IT* weight, const long long* target, const float* centers,
              long long N, int D, int V, long long ignore, int reduction, float* out, void* saved, char* ws, hipStream_t q) {
@@ -700,40 +860,51 @@ int head_fwd(int mode, const IT* hidden, long long ldh, const IT* weight, const 
     operands<IT, T, SPLIT>(p, hidden, ldh, weight, N, D, V, s, rows, true, ws + p.staged_h, ws + p.staged_w, H, W, q);
     float* part = reinterpret_cast<float*>(ws + p.part);
     float* tlogit = reinterpret_cast<float*>(ws + p.tlogit);
-    const long long plane = (long long)(align256((size_t)p.vt_fwd * N * 4) / 4);
-    if (p.thin)
-        head_stats_kernel<T, Thin, SPLIT><<<p.vt_fwd * cdiv(N, 32), Thin::T, 0, q>>>(W, H, s.st, V, D, mode, s.tgt, centers, tlogit,
-                                                                                part, plane, (int)N);
+    const StatsArgs sa{V, s.tgt, centers, tlogit, part, (long long)(align256((size_t)p.vt_fwd * N * 4) / 4), (int)N};
+    if (mode == kCE)
+        stats_launch<T, SPLIT, kCE>(p, W, H, s, N, D, sa, q);
     else
-        head_stats_kernel<T, Sq, SPLIT><<<p.vt_fwd * cdiv(N, 128), Sq::T, 0, q>>>(W, H, s.st, V, D, mode, s.tgt, centers, tlogit,
-                                                                             part, plane, (int)N);
+        stats_launch<T, SPLIT, kExpect>(p, W, H, s, N, D, sa, q);
     double* sums = mode == kCE && reduction != DS_REDUCE_NONE ? reinterpret_cast<double*>(ws + p.sums) : nullptr;
-    head_join_kernel<<<cdiv(N, 32), 256, 0, q>>>(part, plane, (int)N, p.vt_fwd, s.st, mode, s.rows, s.tgt, tlogit, s.top,
+    head_join_kernel<<<cdiv(N, 32), 256, 0, q>>>(part, sa.plane, (int)N, p.vt_fwd, s.st, mode, s.rows, s.tgt, tlogit, s.top,
                                                  s.inv_sum, s.mean, out, sums);
     if (sums) loss_total_kernel<<<1, 256, 0, q>>>(sums, s.st, reduction == DS_REDUCE_MEAN, out);
     return launched();
 }
 
-template <class IT, class T, class S, int SPLIT>
-void dh_launch(const Plan& p, const Operand& W, const Operand& G, const Saved& s, const BackState* bs, long long N, int D,
-               int kcols, int mode, const int* rows, IT* out, float* part, int first, hipStream_t q) {
-    const int grid = cdiv(D, S::BM) * cdiv(N, S::BN) * p.dh_splits;
-    const long long ps = N * ((D + 3) & ~3);
-    if (p.dh_part)
-        head_dh_kernel<T, S, SPLIT, IT, true><<<grid, S::T, 0, q>>>(W, G, s.st, bs, D, kcols, p.dh_splits, mode, rows, out, part,
-                                                                    ps, first);
+template <class T, int SPLIT, int MODE>
+void dl_launch(const Plan& p, const Operand& W, const Operand& H, const Saved& s, const BackState* bs, long long N, int D,
+               const DlArgs& a, hipStream_t q) {
+    const int b = p.dl_shape == kBig ? Big::BM : 128;
+    const int tiles = cdiv(a.cols, b) * cdiv(N, p.dl_shape == kThin ? 32 : b);
+    if (p.dl_shape == kThin)
+        head_dl_kernel<T, Thin, SPLIT, MODE><<<tiles, Thin::T, 0, q>>>(W, H, s.st, bs, D, a);
+    else if (p.dl_shape == kBig)
+        head_dl_big_kernel<T, SPLIT, MODE><<<tiles < cu_count() ? tiles : cu_count(), Big::T, 0, q>>>(W, H, s.st, bs, D, a);
     else
-        head_dh_kernel<T, S, SPLIT, IT, false><<<grid, S::T, 0, q>>>(W, G, s.st, bs, D, kcols, 1, mode, rows, out, part, ps, first);
+        head_dl_kernel<T, Sq, SPLIT, MODE><<<tiles, Sq::T, 0, q>>>(W, H, s.st, bs, D, a);
 }
-template <class IT, class T, class S, int SPLIT>
-void dw_launch(const Plan& p, const Operand& H, const Operand& G, const Saved& s, const BackState* bs, int D, int cols, int mode,
-               IT* out, float* part, hipStream_t q) {
-    const int grid = cdiv(D, S::BM) * cdiv(cols, S::BN) * p.dw_splits;
-    const long long ps = (long long)p.piece * ((D + 3) & ~3);
-    if (p.dw_splits > 1)
-        head_dw_kernel<T, S, SPLIT, IT, true><<<grid, S::T, 0, q>>>(H, G, s.st, bs, D, cols, p.dw_splits, mode, out, part, ps);
+template <class IT, class T, class S, int SPLIT, int WHICH>
+void grad_shape(bool acc, const Operand& A, const Operand& B, const Saved& s, const BackState* bs, long long n,
+                const GradArgs& a, hipStream_t q) {
+    int grid = cdiv(a.D, S::BM) * cdiv(n, S::BN) * a.splits;
+    if (std::is_same<S, Big>::value && grid > cu_count()) grid = cu_count();
+    if (acc)
+        head_grad_kernel<T, S, SPLIT, IT, true, WHICH><<<grid, S::T, 0, q>>>(A, B, s.st, bs, a);
     else
-        head_dw_kernel<T, S, SPLIT, IT, false><<<grid, S::T, 0, q>>>(H, G, s.st, bs, D, cols, 1, mode, out, part, ps);
+        head_grad_kernel<T, S, SPLIT, IT, false, WHICH><<<grid, S::T, 0, q>>>(A, B, s.st, bs, a);
+}
+template <class IT, class T, int SPLIT, int WHICH>
+void grad_launch(ShapeId shape, bool acc, const Operand& A, const Operand& B, const Saved& s, const BackState* bs, long long n,
+                 const GradArgs& a, hipStream_t q) {
+    if (WHICH == 0 && shape == kThin)
+        grad_shape<IT, T, Thin, SPLIT, 0>(acc, A, B, s, bs, n, a, q);
+    else if (shape == kFlat)
+        grad_shape<IT, T, Flat, SPLIT, WHICH>(acc, A, B, s, bs, n, a, q);
+    else if (shape == kBig)
+        grad_shape<IT, T, Big, SPLIT, WHICH>(acc, A, B, s, bs, n, a, q);
+    else
+        grad_shape<IT, T, Sq, SPLIT, WHICH>(acc, A, B, s, bs, n, a, q);
 }
 
 template <class IT, class T, int SPLIT>
@@ -759,30 +930,23 @@ int head_bwd(int mode, const IT* hidden, long long ldh, const IT* weight, const 
     const int D4 = (D + 3) & ~3;
     for (int v0 = 0; v0 < V; v0 += p.piece) {
         const int cols = V - v0 < p.piece ? V - v0 : p.piece, ld = pad8(cols);
-        if (p.thin)
-            head_dl_kernel<T, Thin, SPLIT><<<cdiv(cols, 128) * cdiv(N, 32), Thin::T, 0, q>>>(
-                W, H, s.st, bs, V, D, v0, cols, mode, s.tgt, centers, s.top, s.inv_sum, s.mean, up, dl, ld, lo);
+        Operand Wp = W;   // classes [v0, v0 + cols)
+        Wp.p = static_cast<const T*>(W.p) + (long long)v0 * W.ld;
+        Wp.outer = cols;
+        const DlArgs da{v0, cols, s.tgt, centers, s.top, s.inv_sum, s.mean, up, dl, ld, lo};
+        if (mode == kCE)
+            dl_launch<T, SPLIT, kCE>(p, Wp, H, s, bs, N, D, da, q);
         else
-            head_dl_kernel<T, Sq, SPLIT><<<cdiv(cols, 128) * cdiv(N, 128), Sq::T, 0, q>>>(
-                W, H, s.st, bs, V, D, v0, cols, mode, s.tgt, centers, s.top, s.inv_sum, s.mean, up, dl, ld, lo);
+            dl_launch<T, SPLIT, kExpect>(p, Wp, H, s, bs, N, D, da, q);
         const Operand G{dl, ld, lo, (int)N, ld};
         if (g_hidden) {
-            Operand Wp = W;   // classes [v0, v0 + cols) as stored rows
-            Wp.p = static_cast<const T*>(W.p) + (long long)v0 * W.ld;
-            Wp.outer = cols;
-            if (p.thin)
-                dh_launch<IT, T, Thin, SPLIT>(p, Wp, G, s, bs, N, D, cols, mode, rows, g_hidden, dhp, v0 == 0, q);
-            else if (p.flat)
-                dh_launch<IT, T, Flat, SPLIT>(p, Wp, G, s, bs, N, D, cols, mode, rows, g_hidden, dhp, v0 == 0, q);
-            else
-                dh_launch<IT, T, Sq, SPLIT>(p, Wp, G, s, bs, N, D, cols, mode, rows, g_hidden, dhp, v0 == 0, q);
+            const GradArgs ga{D, cols, p.dh_splits, mode, cols, v0 == 0, rows, g_hidden, dhp, N * D4};
+            grad_launch<IT, T, SPLIT, 0>(p.dh, p.dh_part, Wp, G, s, bs, N, ga, q);
         }
         if (g_weight) {
             IT* gw = g_weight + (long long)v0 * D;
-            if (p.flat)
-                dw_launch<IT, T, Flat, SPLIT>(p, H, G, s, bs, D, cols, mode, gw, dwp, q);
-            else
-                dw_launch<IT, T, Sq, SPLIT>(p, H, G, s, bs, D, cols, mode, gw, dwp, q);
+            const GradArgs ga{D, cols, p.dw_splits, mode, cols, 1, nullptr, gw, dwp, (long long)p.piece * D4};
+            grad_launch<IT, T, SPLIT, 1>(p.dw, p.dw_splits > 1, H, G, s, bs, cols, ga, q);
             if (p.dw_splits > 1)
                 head_sum_kernel<T, SPLIT, IT><<<cdiv((long long)cols * D4 / 4, 256), 256, 0, q>>>(
                     dwp, (long long)p.piece * D4, p.dw_splits, s.st, bs, cols, D, mode, 1, nullptr, gw);
