@@ -62,7 +62,7 @@ template <int BM_, int BN_, int WM_, int WN_>
 struct Shape {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, T = 64 * WM_ * WN_;
     static constexpr int FM = BM_ / WM_ / 16, FN = BN_ / WN_ / 16;   // 16x16 fragments of a wave
-    static constexpr int kLds = 2 * (BM_ + BN_) * kBK * 2;           // two buffers
+    static constexpr int kLds = 2 * (BM_ + BN_) * kBK * 2;           // two steps of one plane
 };
 
 // byte offset of 16-byte chunk c of row r in an LDS tile.  kK: the eight chunks of a row trade places by the row's low bits,
@@ -128,36 +128,52 @@ struct Fragments {
 };
 
 // acc[i][j][e]: C at m = m0 + wave's row + 16 i + 4 (lane / 16) + e, n = n0 + wave's column + 16 j + lane % 16, over k in
-// [kbeg, kend) (kbeg a multiple of 64).  `lds`: S::kLds bytes.  Ends behind a barrier: the caller may reuse `lds`.
+// [kbeg, kend) (kbeg a multiple of 64).  `lds`: lds_bytes<S, SPLIT>() bytes.  Ends behind a barrier: the caller may reuse
+// `lds`.  SPLIT = 3: a step brings both planes of both operands and adds its three products from them, so that each plane is
+// moved once and a step's latency is covered by three products.  128 x 128 tiles then keep one step in LDS (the next one
+// waits in registers), which leaves room for two workgroups a CU.
+template <class S, int SPLIT>
+constexpr int lds_buffers() { return SPLIT == 3 && S::BM * S::BN > 64 * 128 ? 1 : 2; }
+template <class S, int SPLIT>
+constexpr int lds_bytes() { return lds_buffers<S, SPLIT>() * (SPLIT == 3 ? 2 : 1) * (S::BM + S::BN) * kBK * 2; }
+
 template <class T, class S, Lay LA, Lay LB, int SPLIT>
 __device__ __forceinline__ void gemm_tile(const Operand& A, const Operand& B, int m0, int n0, int kbeg, int kend, char* lds,
                                           f32x4 (&acc)[S::FM][S::FN]) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = (wave / S::WN) * S::FM * 16, wn = (wave % S::WN) * S::FN * 16;
-    constexpr int kA = S::BM * kBK * 2, kBuf = (S::BM + S::BN) * kBK * 2;
+    constexpr int P = SPLIT == 3 ? 2 : 1, kA = S::BM * kBK * 2, kB = S::BN * kBK * 2, kBuf = P * (kA + kB);
+    constexpr int NB = lds_buffers<S, SPLIT>();
 #pragma unroll
     for (int i = 0; i < S::FM; ++i)
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     const Fragments<LA, S::BM> fa(wm, lane);
     const Fragments<LB, S::BN> fb(wn, lane);
-    Stager<LA, S::BM, S::T> sa;
-    Stager<LB, S::BN, S::T> sb;
-    const int steps = (kend - kbeg + kBK - 1) / kBK * SPLIT;
+    Stager<LA, S::BM, S::T> sa[P];
+    Stager<LB, S::BN, S::T> sb[P];
+    const int steps = (kend - kbeg + kBK - 1) / kBK;
     auto load = [&](int s) {
-        const int k0 = kbeg + s / SPLIT * kBK, ph = s % SPLIT;
-        sa.load(A, m0, k0, SPLIT == 3 && ph == 0, tid);
-        sb.load(B, n0, k0, SPLIT == 3 && ph == 1, tid);
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            sa[p].load(A, m0, kbeg + s * kBK, p == 1, tid);
+            sb[p].load(B, n0, kbeg + s * kBK, p == 1, tid);
+        }
+    };
+    auto store = [&](char* buf) {   // hi A, hi B, lo A, lo B
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            sa[p].store(buf + p * (kA + kB), tid);
+            sb[p].store(buf + p * (kA + kB) + kA, tid);
+        }
     };
     if (steps > 0) {
         load(0);
-        sa.store(lds, tid);
-        sb.store(lds + kA, tid);
+        store(lds);
     }
     __syncthreads();
     for (int s = 0; s < steps; ++s) {
-        const char* buf = lds + (s & 1) * kBuf;
-        char* nxt = lds + ((s + 1) & 1) * kBuf;
+        const char* buf = lds + (NB == 2 ? (s & 1) * kBuf : 0);
         const bool more = s + 1 < steps;
         if (more) load(s + 1);
 #pragma unroll
@@ -167,15 +183,28 @@ __device__ __forceinline__ void gemm_tile(const Operand& A, const Operand& B, in
             for (int i = 0; i < S::FM; ++i) a[i] = fa.get(buf, i, kk);
 #pragma unroll
             for (int j = 0; j < S::FN; ++j) b[j] = fb.get(buf + kA, j, kk);
+            if (SPLIT == 3) {
+                s16x8 c[S::FM], d[S::FN];
+#pragma unroll
+                for (int i = 0; i < S::FM; ++i) c[i] = fa.get(buf + kA + kB, i, kk);
+#pragma unroll
+                for (int j = 0; j < S::FN; ++j) d[j] = fb.get(buf + kA + kB + kA, j, kk);
+#pragma unroll
+                for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+                    for (int j = 0; j < S::FN; ++j) acc[i][j] = mfma(c[i], b[j], acc[i][j], T());
+#pragma unroll
+                for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+                    for (int j = 0; j < S::FN; ++j) acc[i][j] = mfma(a[i], d[j], acc[i][j], T());
+            }
 #pragma unroll
             for (int i = 0; i < S::FM; ++i)
 #pragma unroll
                 for (int j = 0; j < S::FN; ++j) acc[i][j] = mfma(a[i], b[j], acc[i][j], T());
         }
-        if (more) {
-            sa.store(nxt, tid);
-            sb.store(nxt + kA, tid);
-        }
+        if (NB == 1) __syncthreads();
+        if (more) store(lds + (NB == 2 ? ((s + 1) & 1) * kBuf : 0));
         __syncthreads();
     }
 }
@@ -424,6 +453,53 @@ __device__ __forceinline__ float scale_for(float amax) {
     int e = 14 - ilogbf(amax);
     e = e > 60 ? 60 : (e < -110 ? -110 : e);
     return ldexpf(1.f, e);
+}
+
+// ---- which shape a product takes, and over how many workgroups its sum is split (host) -----------------------------------
+enum ShapeId { kSq, kFlat, kThin, kBig, kSmall };
+typedef Shape<128, 128, 2, 2> Sq;
+typedef Shape<64, 64, 2, 2> Small;
+
+struct Cut {
+    ShapeId shape;
+    int splits;
+};
+// tiles(b): tiles of b x b; area: outputs; planes 2: three products a step.
+template <class Tiles>
+inline Cut cut_of(Tiles tiles, double area, long long K, int planes, bool may_split, bool small_too, int cus) {
+    // us a step of 64 k: `step` of a CU's time with `at_once` workgroups on it, `alone` at least; `ends`: start and end of a
+    // tile.  Measured at k = 512 and 2048 with half a workgroup to sixteen a CU; in TFLOP/s of 16-bit products with the chip
+    // full: 256 x 256 tiles 1330, 128 x 128 870, 64 x 64 660; with two planes 1365, 1160, 780.
+    struct Cost {
+        ShapeId id;
+        int b, at_once;
+        double step, alone, ends;
+    };
+    static const Cost one[3] = {{kBig, 256, 1, 1.5, 1.35, 4.5}, {kSq, 128, 2, 0.60, 0.78, 3.0}, {kSmall, 64, 4, 0.21, 0.57, 2.0}};
+    static const Cost two[3] = {{kBig, 256, 1, 4.5, 4.1, 5.0}, {kSq, 128, 2, 1.40, 1.85, 3.0}, {kSmall, 64, 2, 0.53, 0.68, 2.5}};
+    const long long steps = (K + kBK - 1) / kBK, most = may_split ? (steps < 256 ? steps : 256) : 1;
+    Cut best{kSq, 1};
+    double least = 1e300;
+    for (int c = 0; c < (small_too ? 3 : 2); ++c) {
+        const Cost& q = planes == 2 ? two[c] : one[c];
+        const long long t = tiles(q.b);
+        for (long long s = 1; s <= most; s += s < 16 ? 1 : s / 8) {
+            const double per = (double)((steps + s - 1) / s);
+            const long long n = (t * s + cus - 1) / cus, full = n / q.at_once, rest = n % q.at_once;
+            auto round = [&](long long k) {
+                const double shared = q.step * (double)k;
+                return (shared > q.alone ? shared : q.alone) * per + q.ends;
+            };
+            // a split sum is written and read once more, 4 bytes an element at 4 TB/s, and takes one more launch
+            const double time = (double)full * round(q.at_once) + (rest ? round(rest) : 0.0) +
+                                (s > 1 ? 4.0 + 8e-6 * (double)s * area / 4.0 : 0.0);
+            if (time < least) {
+                least = time;
+                best = Cut{q.id, (int)s};
+            }
+        }
+    }
+    return best;
 }
 
 }  // namespace ds

@@ -287,7 +287,7 @@ __device__ __forceinline__ void stats_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0
 template <class T, class S, int SPLIT, int MODE>
 __global__ __launch_bounds__(S::T) void head_stats_kernel(Operand W, Operand H, const HeadState* __restrict__ st, int D,
                                                           StatsArgs a) {
-    __shared__ __align__(16) char lds[S::kLds];
+    __shared__ __align__(16) char lds[lds_bytes<S, SPLIT>()];
     const int vt = cdiv(a.V, S::BM);
     const int m0 = (int)(blockIdx.x % vt) * S::BM, n0 = (int)(blockIdx.x / vt) * S::BN;
     const int cnt = st->count;
@@ -514,7 +514,7 @@ __device__ __forceinline__ void dl_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, i
 template <class T, class S, int SPLIT, int MODE>
 __global__ __launch_bounds__(S::T) void head_dl_kernel(Operand W, Operand H, const HeadState* __restrict__ st,
                                                        const BackState* __restrict__ bs, int D, DlArgs a) {
-    __shared__ __align__(16) char lds[S::kLds];
+    __shared__ __align__(16) char lds[lds_bytes<S, SPLIT>()];
     const int vt = cdiv(a.cols, S::BM);
     const int m0 = (int)(blockIdx.x % vt) * S::BM, n0 = (int)(blockIdx.x / vt) * S::BN;
     const int cnt = st->count;
@@ -597,7 +597,7 @@ __device__ __forceinline__ void grad_of_tile(const f32x4 (&acc)[S::FM][S::FN], i
 template <class T, class S, int SPLIT, class O, bool ACC, int WHICH>
 __global__ __launch_bounds__(S::T) void head_grad_kernel(Operand A, Operand B, const HeadState* __restrict__ st,
                                                          const BackState* __restrict__ bs, GradArgs a) {
-    __shared__ __align__(16) char lds[S::kLds];
+    __shared__ __align__(16) char lds[std::is_same<S, Big>::value ? Big::kLds : lds_bytes<S, SPLIT>()];
     const int cnt = st->count, mt = cdiv(a.D, S::BM), bound = WHICH == 0 ? cnt : a.cols;
     const int k = WHICH == 0 ? a.k : cnt, per = cdiv(cdiv(k, kBK), a.splits) * kBK;
     B.outer = cnt;
@@ -674,36 +674,11 @@ __global__ __launch_bounds__(256) void zero_ignored_kernel(const long long* __re
 // ------------------------------------------------------------------------------------------------------------- host
 // Shapes: 256x256 outputs a workgroup (TileStream) for large products; 128x128, four waves of 64x64, below that; 64 features or
 // 32 rows have shapes of their own, whose idle half would otherwise be computed and dropped.
-typedef Shape<128, 128, 2, 2> Sq;
 typedef Shape<64, 128, 1, 4> Flat;    // 64 along m
 typedef Shape<128, 32, 4, 1> Thin;    // 32 along n
-enum ShapeId { kSq, kFlat, kThin, kBig };
-
-// Which shape a product takes and over how many workgroups its sum is split.  Times in us, measured for bf16: a step of 64
-// k costs a 256x256 tile 1.55 and its start and end 4.2 (4096^2 tiles at k = 256 .. 16384); two 128x128 tiles share a CU and
-// take 1.36 and 3 each.  A split sum is written and read once more, at 4 bytes an element and 4 TB/s.
-struct Cut {
-    ShapeId shape;
-    int splits;
-};
 Cut cut_of(long long M, long long N, long long K, int planes, bool may_split) {
-    const long long cu = cu_count(), steps = (K + kBK - 1) / kBK;
-    Cut best{kSq, 1};
-    double least = 1e300;
-    for (int big = 0; big < 2; ++big) {
-        const long long b = big ? 256 : 128, tiles = ((M + b - 1) / b) * ((N + b - 1) / b), slots = big ? cu : 2 * cu;
-        const long long most = may_split ? (steps / 4 < 256 ? steps / 4 : 256) : 1;
-        for (long long s = 1; s <= (most > 1 ? most : 1); s += s < 16 ? 1 : s / 8) {
-            const double per = (double)((steps + s - 1) / s) * (planes == 2 ? 3 : 1);
-            const double t = (double)((tiles * s + slots - 1) / slots) * (big ? 1.55 * per + 4.2 : 1.36 * per + 3.0) +
-                             (s > 1 ? 3.0 + 8e-6 * (double)s * M * N / 4.0 : 0.0);
-            if (t < least) {
-                least = t;
-                best = Cut{big ? kBig : kSq, (int)s};
-            }
-        }
-    }
-    return best;
+    return ds::cut_of([&](long long b) { return ((M + b - 1) / b) * ((N + b - 1) / b); }, (double)M * N, K, planes, may_split,
+                      false, cu_count());
 }
 
 struct Saved {

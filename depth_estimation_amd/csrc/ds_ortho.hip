@@ -17,51 +17,74 @@ namespace ds {
 namespace {
 
 constexpr float kXs = 8192.f;    // stored X = 2^13 X, stored A = 2^13 A: 8x headroom in fp16
-constexpr int kNormBlocks = 64;  // partial sums of squares per matrix
-
-
-__global__ __launch_bounds__(256) void ortho_norm_kernel(const void* __restrict__ g, int dtype, long long mn,
-                                                         double* __restrict__ part) {
-    __shared__ double s[4];
-    const long long base = blockIdx.y * mn;
-    double a = 0.0;
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < mn; i += kNormBlocks * 256ll) {
-        const float x = dtype == DS_F32   ? static_cast<const float*>(g)[base + i]
-                        : dtype == DS_F16 ? (float)static_cast<const f16*>(g)[base + i]
-                                          : (float)static_cast<const bf16*>(g)[base + i];
-        a += (double)x * x;
-    }
+// blocks that sum squares of one matrix: 4096 elements each, at most 512
+__host__ __device__ inline int norm_blocks(long long mn) {
+    const long long n = (mn + 4095) / 4096;
+    return n < 512 ? (int)n : 512;
+}
+__device__ __forceinline__ float element(const void* g, int dtype, long long i) {
+    return dtype == DS_F32   ? static_cast<const float*>(g)[i]
+           : dtype == DS_F16 ? (float)static_cast<const f16*>(g)[i]
+                             : (float)static_cast<const bf16*>(g)[i];
+}
+// sum over a workgroup of T threads, the same in every thread
+template <int T>
+__device__ __forceinline__ double sum_all(double a, double* s) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) a += __shfl_xor(a, o, 64);
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = a;
     __syncthreads();
-    if (threadIdx.x == 0) part[blockIdx.y * kNormBlocks + blockIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
+    a = 0.0;
+    for (int i = 0; i < T / 64; ++i) a += s[i];
+    __syncthreads();
+    return a;
+}
+
+__global__ __launch_bounds__(256) void ortho_norm_kernel(const void* __restrict__ g, int dtype, long long mn,
+                                                         double* __restrict__ part) {
+    __shared__ double s[4];
+    const long long base = blockIdx.y * mn, step = gridDim.x * 256ll;
+    double a0 = 0.0, a1 = 0.0, a2 = 0.0, a3 = 0.0;
+    long long i = blockIdx.x * 256ll + threadIdx.x;
+    for (; i + 3 * step < mn; i += 4 * step) {
+        const float x0 = element(g, dtype, base + i), x1 = element(g, dtype, base + i + step);
+        const float x2 = element(g, dtype, base + i + 2 * step), x3 = element(g, dtype, base + i + 3 * step);
+        a0 += (double)x0 * x0;
+        a1 += (double)x1 * x1;
+        a2 += (double)x2 * x2;
+        a3 += (double)x3 * x3;
+    }
+    for (; i < mn; i += step) {
+        const float x = element(g, dtype, base + i);
+        a0 += (double)x * x;
+    }
+    const double a = sum_all<256>((a0 + a1) + (a2 + a3), s);
+    if (threadIdx.x == 0) part[blockIdx.y * gridDim.x + blockIdx.x] = a;
+}
+__device__ __forceinline__ double inverse_norm(const double* part, int blocks, double eps, double* s) {
+    double t = 0.0;
+    for (int i = threadIdx.x; i < blocks; i += 256) t += part[i];
+    return 1.0 / (sqrt(sum_all<256>(t, s)) + eps);
 }
 
 // G / (|G| + eps) as two planes, rows padded with zeros to np
 __global__ __launch_bounds__(256) void ortho_load_kernel(const void* __restrict__ g, int dtype, int m, int n, int np, double eps,
-                                                         const double* __restrict__ part, f16* __restrict__ x, long long lo,
-                                                         long long per) {
-    double t = 0.0;
-    for (int i = 0; i < kNormBlocks; ++i) t += part[blockIdx.y * kNormBlocks + i];
-    const double inv = 1.0 / (sqrt(t) + eps);
+                                                         const double* __restrict__ part, int blocks, f16* __restrict__ x,
+                                                         long long lo, long long per) {
+    __shared__ double s[4];
+    const double inv = inverse_norm(part + (long long)blockIdx.y * blocks, blocks, eps, s) * kXs;
     const long long base = (long long)blockIdx.y * m * n;
     f16* y = x + blockIdx.y * per;
-    const int lane = threadIdx.x & 63;
-    for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < m; r += gridDim.x * 4)
-        for (int c = lane; c < np; c += 64) {
-            float v = 0.f;
-            if (c < n) {
-                const long long i = base + (long long)r * n + c;
-                v = dtype == DS_F32   ? static_cast<const float*>(g)[i]
-                    : dtype == DS_F16 ? (float)static_cast<const f16*>(g)[i]
-                                      : (float)static_cast<const bf16*>(g)[i];
-            }
-            f16 h, l;
-            split16((float)(v * inv * kXs), h, l);   // scaled in double: a tiny or huge norm keeps its bits
-            y[(long long)r * np + c] = h;
-            y[(long long)r * np + c + lo] = l;
-        }
+    const unsigned q = np / 4;
+    const long long all = (long long)m * q;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
+        const int r = all < (1ll << 31) ? (int)((unsigned)i / q) : (int)(i / q), c = (int)(i - (long long)r * q) * 4;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)   // scaled in double: a tiny or huge norm keeps its bits
+            v[e] = c + e < n ? (float)(element(g, dtype, base + (long long)r * n + c + e) * inv) : 0.f;
+        put4<3>(y + (long long)r * np + c, lo, v);
+    }
 }
 
 // tile pair (i >= j) of a triangular index
@@ -72,122 +95,407 @@ __device__ __forceinline__ void triangle(int t, int& i, int& j) {
     j = t - i * (i + 1) / 2;
 }
 
-// One symmetric product of s x s: POLY false: A = X X^T (L = kK) or X^T X (L = kM);  true: B = a I + b A + c A A.
-// Tiles with m0 >= n0; the element (m, n) is written at [n][m] (four consecutive m per lane) and, off the diagonal, at [m][n].
-template <class S, Lay L, bool POLY>
-__global__ __launch_bounds__(S::T) void ortho_sym_kernel(Operand X, long long per_x, int s, int k, f16* __restrict__ out, int ld,
-                                                         long long lo, long long per_out, float ca, float cb, float cc,
-                                                         float factor) {
-    __shared__ __align__(16) char lds[S::kLds];
-    int ti, tj;
-    triangle(blockIdx.x, ti, tj);
-    const int m0 = ti * S::BM, n0 = tj * S::BN;
-    X.p = static_cast<const f16*>(X.p) + blockIdx.y * per_x;
-    out += blockIdx.y * per_out;
-    f32x4 acc[S::FM][S::FN];
-    gemm_tile<f16, S, L, L, 3>(X, X, m0, n0, 0, k, lds, acc);
+// What becomes of a product's tile.  kGram: A = X X^T;  kPoly: B = a I + b A + c A A;  both symmetric: tiles with m0 >= n0, the
+// element (m, n) written at [n][m] (four consecutive m per lane) and, off the diagonal, at [m][n].  kNext: the next X, row n,
+// columns along m.  kLast: the result in the caller's type.
+enum Use { kGram, kPoly, kNext, kLast };
+struct UseArgs {
+    int rows, cols;          // of the result; columns beyond `cols` up to ld are written as zeros
+    void* out;
+    int ld;
+    long long lo, per_out;   // planes apart, matrices apart
+    const f16* a;            // kPoly: A again
+    long long per_a;
+    float ca, cb, cc;        // kPoly's coefficients, scaled; else ca: the factor
+};
+// fragment row i of a tile
+template <class S, Use U, class O>
+__device__ __forceinline__ void use_row(const f32x4 (&acc)[S::FN], int i, int m0, int n0, int batch, const UseArgs& u) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / S::WN, wn = wave % S::WN;
-    const f16* a = static_cast<const f16*>(X.p);
+    const int m = m0 + (wm * S::FM + i) * 16 + (lane >> 4) * 4;
+    if (m >= u.ld) return;
+    {
 #pragma unroll
-    for (int j = 0; j < S::FN; ++j) {
-        const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
-        if (n >= s) continue;
-#pragma unroll
-        for (int i = 0; i < S::FM; ++i) {
-            const int m = m0 + (wm * S::FM + i) * 16 + (lane >> 4) * 4;
-            if (m >= ld) continue;
+        for (int j = 0; j < S::FN; ++j) {
+            const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
+            if (n >= u.rows) continue;
             float v[4];
-            if (POLY) {
-                const f16x4 h = *reinterpret_cast<const f16x4*>(a + (long long)n * X.ld + m);
-                const f16x4 l = *reinterpret_cast<const f16x4*>(a + (long long)n * X.ld + m + X.lo);
+            if (U == kPoly) {
+                const f16* a = u.a + batch * u.per_a + (long long)n * u.ld + m;
+                const f16x4 h = *reinterpret_cast<const f16x4*>(a), l = *reinterpret_cast<const f16x4*>(a + u.lo);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    v[e] = m + e < s ? fmaf(cc, acc[i][j][e], cb * ((float)h[e] + (float)l[e])) + (m + e == n ? ca : 0.f) : 0.f;
+                    v[e] = fmaf(u.cc, acc[j][e], u.cb * ((float)h[e] + (float)l[e])) + (m + e == n ? u.ca : 0.f);
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * factor;
+                for (int e = 0; e < 4; ++e) v[e] = acc[j][e] * u.ca;
             }
-            put4<3>(out + (long long)n * ld + m, lo, v);
-            if (ti != tj) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (m + e < s) {
-                        f16 h, l;
-                        split16(v[e], h, l);
-                        out[(long long)(m + e) * ld + n] = h;
-                        out[(long long)(m + e) * ld + n + lo] = l;
-                    }
+            for (int e = 0; e < 4; ++e)
+                if (m + e >= u.cols) v[e] = 0.f;
+            if (U == kLast) {
+                put_row4(static_cast<O*>(u.out) + batch * u.per_out + (long long)n * u.cols, m, u.cols, v, (u.cols & 3) == 0);
+            } else {
+                f16* out = static_cast<f16*>(u.out) + batch * u.per_out;
+                put4<3>(out + (long long)n * u.ld + m, u.lo, v);
+                if ((U == kGram || U == kPoly) && m0 != n0) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (m + e < u.cols) {
+                            f16 h, l;
+                            split16(v[e], h, l);
+                            out[(long long)(m + e) * u.ld + n] = h;
+                            out[(long long)(m + e) * u.ld + n + u.lo] = l;
+                        }
+                }
             }
         }
     }
 }
+template <class S, Use U, class O>
+__device__ __forceinline__ void use_tile(const f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int batch, const UseArgs& u) {
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i) use_row<S, U, O>(acc[i], i, m0, n0, batch, u);
+}
 
-// X' = B X (LA = kM on X, rows of B along n) or X B (LA = kK on B, rows of X along n): row r, columns along m.
-// O = void: the next X (two planes); else the result in the caller's type, row pitch `cols`.
-template <class S, Lay LA, class O>
-__global__ __launch_bounds__(S::T) void ortho_apply_kernel(Operand A, Operand B, long long per_a, long long per_b, int rows,
-                                                           int cols, int k, float factor, void* __restrict__ out, int ld,
-                                                           long long lo, long long per_out) {
-    __shared__ __align__(16) char lds[S::kLds];
-    const int mt = cdiv(cols, S::BM);
-    const int m0 = (int)(blockIdx.x % mt) * S::BM, n0 = (int)(blockIdx.x / mt) * S::BN;
-    A.p = static_cast<const f16*>(A.p) + blockIdx.y * per_a;
-    B.p = static_cast<const f16*>(B.p) + blockIdx.y * per_b;
+// C = A B over k.  tri: only tiles with m0 >= n0.  Units: matrices x tiles x splits; part (may be NULL: no splits): the tiles'
+// sums, a thread's fragments 16 bytes next to its neighbour's, for ortho_finish_kernel.
+struct ProductArgs {
+    Operand A, B;
+    long long per_a, per_b;
+    int mt, nt, tri, k, splits, batch;
+    float* part;
+};
+template <class S>
+__device__ __forceinline__ void unit_of(const ProductArgs& p, int u, int units, int& batch, int& m0, int& n0, int& sp, int& tile) {
+    const int per = units / p.batch, tiles = per / p.splits;
+    batch = u / per;
+    const int in = u % per;
+    sp = in % p.splits;
+    int m, n;
+    if (p.tri) {
+        triangle(in / p.splits, m, n);
+    } else {
+        tile_of(in / p.splits, tiles, p.mt, p.nt, m, n);
+    }
+    tile = batch * tiles + in / p.splits;
+    m0 = m * S::BM;
+    n0 = n * S::BN;
+}
+template <class S>
+__device__ __forceinline__ void keep_part(const f32x4 (&acc)[S::FM][S::FN], const ProductArgs& p, int tile, int sp) {
+    f32x4* q = reinterpret_cast<f32x4*>(p.part) + ((long long)tile * p.splits + sp) * (S::BM * S::BN / 4) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) q[(i * S::FN + j) * S::T] = acc[i][j];
+}
+template <class S, Lay LA, Lay LB, Use U, class O, bool PART>
+__global__ __launch_bounds__(S::T) void ortho_product_kernel(ProductArgs p, UseArgs u, int units) {
+    __shared__ __align__(16) char lds[std::is_same<S, Big>::value ? Big::kLds : lds_bytes<S, 3>()];
+    const int per = cdiv(cdiv(p.k, kBK), p.splits) * kBK;
+    auto job = [&](int x) {
+        int batch, m0, n0, sp, tile;
+        unit_of<S>(p, x, units, batch, m0, n0, sp, tile);
+        Job j{p.A, p.B, m0, n0, min(sp * per, p.k), min(sp * per + per, p.k)};
+        j.A.p = static_cast<const f16*>(j.A.p) + batch * p.per_a;
+        j.B.p = static_cast<const f16*>(j.B.p) + batch * p.per_b;
+        return j;
+    };
+    auto done = [&](int x, const f32x4 (&acc)[S::FM][S::FN]) {
+        int batch, m0, n0, sp, tile;
+        unit_of<S>(p, x, units, batch, m0, n0, sp, tile);
+        if (PART)
+            keep_part<S>(acc, p, tile, sp);
+        else
+            use_tile<S, U, O>(acc, m0, n0, batch, u);
+    };
+    int t = blockIdx.x;
     f32x4 acc[S::FM][S::FN];
-    gemm_tile<f16, S, LA, kK, 3>(A, B, m0, n0, 0, k, lds, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = wave / S::WN, wn = wave % S::WN;
+    if constexpr (std::is_same<S, Big>::value) {
+        TileStream<f16, LA, LB, 3> stream(lds, job(t));
+        for (; t < units; t += gridDim.x) {
+            stream.multiply(acc, [&](Job& j) {
+                const int x = t + gridDim.x;
+                if (x < units) j = job(x);
+                return x < units;
+            });
+            done(t, acc);
+        }
+    } else {
+        const Job j = job(t);
+        gemm_tile<f16, S, LA, LB, 3>(j.A, j.B, j.m0, j.n0, j.kbeg, j.kend, lds, acc);
+        done(t, acc);
+    }
+}
+// adds a tile's splits in order; a workgroup for every fragment row, because there are few tiles where there are splits
+template <class S, Use U, class O>
+__global__ __launch_bounds__(S::T) void ortho_finish_kernel(ProductArgs p, UseArgs u) {
+    int batch, m0, n0, sp, tile;
+    unit_of<S>(p, blockIdx.x * p.splits, gridDim.x * p.splits, batch, m0, n0, sp, tile);
+    const int i = blockIdx.y;
+    const f32x4* q = reinterpret_cast<const f32x4*>(p.part) + (long long)tile * p.splits * (S::BM * S::BN / 4) + threadIdx.x +
+                     i * S::FN * S::T;
+    f32x4 acc[S::FN];
 #pragma unroll
-    for (int j = 0; j < S::FN; ++j) {
-        const int r = n0 + (wn * S::FN + j) * 16 + (lane & 15);
-        if (r >= rows) continue;
+    for (int j = 0; j < S::FN; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < p.splits; ++s)
 #pragma unroll
-        for (int i = 0; i < S::FM; ++i) {
-            const int c = m0 + (wm * S::FM + i) * 16 + (lane >> 4) * 4;
-            float v[4];
+        for (int j = 0; j < S::FN; ++j) acc[j] += q[(long long)s * (S::BM * S::BN / 4) + j * S::T];
+    use_row<S, U, O>(acc, i, m0, n0, batch, u);
+}
+
+// ---- small matrices: all steps in one workgroup ------------------------------------------------------------------------
+//
+// X (small side s first, so a tall matrix is held transposed) and A, later B in its place, stay in LDS as two planes each;
+// rows are padded to a multiple of 32 with zeros and by 8 elements more, which spreads the fragment reads over the banks.
+// A wave forms fragments (16 x 16) of the products in registers; a result replaces its operand behind a barrier.  What bounds
+// it is the latency of the chain norm -> 3 products a step -> store: 64 x 147 in 5 steps 81 us as 17 launches.
+constexpr int kSmallT = 512;
+
+struct SmallPlan {
+    int sp, lp, px, pa;      // sides padded to 32; row pitches of X and A
+    int bytes;
+};
+__host__ __device__ inline SmallPlan small_plan(int s, int l) {
+    SmallPlan p;
+    p.sp = (s + 31) & ~31;
+    p.lp = (l + 31) & ~31;
+    p.px = p.lp + 8;
+    p.pa = p.sp + 8;
+    p.bytes = 4 * p.sp * (p.px + p.pa);
+    return p;
+}
+// fits LDS, and every wave's fragments its registers
+inline bool small_fits(int s, int l) {
+    if (s > 128 || l > 4096) return false;
+    const SmallPlan p = small_plan(s, l);
+    return p.bytes <= 152 * 1024 && cdiv(p.lp / 16, kSmallT / 64 / (p.sp / 16)) <= (s > 64 ? 8 : 10);
+}
+
+struct Planes {
+    f16* hi;
+    f16* lo;
+    int pitch;
+};
+__device__ __forceinline__ s16x8 rows_frag(const f16* p, int pitch, int r0, int k0, int lane) {
+    return *reinterpret_cast<const s16x8*>(p + (r0 + (lane & 15)) * pitch + k0 + (lane >> 4) * 8);
+}
+// the same fragment of the transposed matrix: 16 columns from c0, k along the rows
+__device__ __forceinline__ s16x8 cols_frag(const f16* p, int pitch, int c0, int k0, int lane) {
+    typedef __attribute__((address_space(3))) s16x4* lp;
+    const f16* q = p + (k0 + (lane >> 4) * 8 + ((lane >> 2) & 3)) * pitch + c0 + (lane & 3) * 4;
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q));
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q + 4 * pitch));
+    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// A wave's fragments of a product: row block w % nr, column blocks w / nr, + G, .. (G waves share a row block; of nr = 6 row
+// blocks two waves have none).  The result's row runs along the lanes (operand R), four columns per lane (operand C).  Blocks
+// beyond the last repeat it, so that no branch keeps the loads of one k apart.
+struct Share {
+    int row, col, step, cols;    // this wave's row block, first column block and stride, column blocks there are
+    bool has;
+    __device__ __forceinline__ Share(int wave, int nr, int nc) {
+        const int g = kSmallT / 64 / nr;
+        row = wave % nr;
+        col = wave / nr;
+        step = g;
+        cols = nc;
+        has = col < g;
+    }
+    __device__ __forceinline__ int c0(int i) const {
+        const int c = col + i * step;
+        return (c < cols ? c : cols - 1) * 16;
+    }
+    __device__ __forceinline__ bool mine(int i) const { return has && col + i * step < cols; }
+};
+template <bool TRANS, int NF>
+__device__ __forceinline__ void small_product(const Planes& R, const Planes& C, const Share& sh, int k, int lane,
+                                              f32x4 (&acc)[NF]) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = c + e < cols ? acc[i][j][e] * factor : 0.f;
-            if constexpr (std::is_same<O, void>::value) {
-                if (c < ld) put4<3>(static_cast<f16*>(out) + blockIdx.y * per_out + (long long)r * ld + c, lo, v);
+    for (int i = 0; i < NF; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (!sh.has) return;
+    for (int k0 = 0; k0 < k; k0 += 32) {
+        const s16x8 rh = rows_frag(R.hi, R.pitch, sh.row * 16, k0, lane), rl = rows_frag(R.lo, R.pitch, sh.row * 16, k0, lane);
+#pragma unroll
+        for (int i = 0; i < NF; ++i) {
+            s16x8 ch, cl;
+            if (TRANS) {
+                ch = cols_frag(C.hi, C.pitch, sh.c0(i), k0, lane);
+                cl = cols_frag(C.lo, C.pitch, sh.c0(i), k0, lane);
             } else {
-                if (c < cols)
-                    put_row4(static_cast<O*>(out) + blockIdx.y * per_out + (long long)r * cols, c, cols, v,
-                             (cols & 3) == 0);
+                ch = rows_frag(C.hi, C.pitch, sh.c0(i), k0, lane);
+                cl = rows_frag(C.lo, C.pitch, sh.c0(i), k0, lane);
+            }
+            acc[i] = mfma(cl, rh, acc[i], f16());
+            acc[i] = mfma(ch, rl, acc[i], f16());
+            acc[i] = mfma(ch, rh, acc[i], f16());
+        }
+    }
+}
+struct SmallArgs {
+    int m, n, steps;
+    double eps;
+    float ca, cb, cc, bs;     // as UseArgs of kPoly; B's scale
+};
+// NA, NX: fragments a wave holds of the square products and of X
+template <class O, int NA, int NX>
+__global__ __launch_bounds__(kSmallT) void ortho_small_kernel(const O* __restrict__ g, O* __restrict__ out, SmallArgs a) {
+    extern __shared__ __align__(16) char lds[];
+    __shared__ double red[kSmallT / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const bool wide = a.m <= a.n;
+    const int s = wide ? a.m : a.n, l = wide ? a.n : a.m, mn = a.m * a.n;
+    const SmallPlan p = small_plan(s, l);
+    Planes X{reinterpret_cast<f16*>(lds), reinterpret_cast<f16*>(lds) + p.sp * p.px, p.px};
+    Planes A{X.lo + p.sp * p.px, X.lo + p.sp * (p.px + p.pa), p.pa};
+    const O* gm = g + (long long)blockIdx.x * mn;
+    O* om = out + (long long)blockIdx.x * mn;
+    for (int i = tid; i < p.sp * p.px / 2; i += kSmallT) reinterpret_cast<int*>(X.hi)[i] = reinterpret_cast<int*>(X.lo)[i] = 0;
+    // eight loads under way at a time, in both passes over the matrix
+    double t = 0.0;
+    for (int i0 = tid; i0 < mn; i0 += 8 * kSmallT) {
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = i0 + u * kSmallT < mn ? (float)gm[i0 + u * kSmallT] : 0.f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) t += (double)x[u] * x[u];
+    }
+    const double inv = 1.0 / (sqrt(sum_all<kSmallT>(t, red)) + a.eps) * kXs;
+    const int dr = kSmallT / a.n, dc = kSmallT - dr * a.n;      // from one element of a thread to its next
+    int r0 = tid / a.n, c0 = tid - r0 * a.n;
+    for (int i0 = tid; i0 < mn; i0 += 8 * kSmallT) {
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = i0 + u * kSmallT < mn ? (float)gm[i0 + u * kSmallT] : 0.f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int at = wide ? r0 * p.px + c0 : c0 * p.px + r0;
+            f16 h, w;
+            split16((float)(x[u] * inv), h, w);
+            if (i0 + u * kSmallT < mn) {
+                X.hi[at] = h;
+                X.lo[at] = w;
+            }
+            r0 += dr;
+            c0 += dc;
+            if (c0 >= a.n) {
+                c0 -= a.n;
+                ++r0;
             }
         }
+    }
+    __syncthreads();
+    const int ns = p.sp / 16, nl = p.lp / 16;
+    const Share sq(wave, ns, ns), sx(wave, ns, nl);
+    const int r = sq.row * 16 + (lane & 15), q = (lane >> 4) * 4;
+    for (int step = 0; step < a.steps; ++step) {
+        f32x4 b[NA];
+        small_product<false, NA>(X, X, sq, p.lp, lane, b);
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (sq.mine(i)) {
+                const float v[4] = {b[i][0] * (1.f / kXs), b[i][1] * (1.f / kXs), b[i][2] * (1.f / kXs), b[i][3] * (1.f / kXs)};
+                put4<3>(A.hi + r * p.pa + sq.c0(i) + q, A.lo - A.hi, v);
+            }
+        __syncthreads();
+        small_product<false, NA>(A, A, sq, p.sp, lane, b);
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (sq.mine(i)) {
+                const int c = sq.c0(i) + q;
+                const f16x4 h = *reinterpret_cast<const f16x4*>(A.hi + r * p.pa + c);
+                const f16x4 w = *reinterpret_cast<const f16x4*>(A.lo + r * p.pa + c);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    b[i][e] = fmaf(a.cc, b[i][e], a.cb * ((float)h[e] + (float)w[e])) + (c + e == r && r < s ? a.ca : 0.f);
+            }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (sq.mine(i)) {
+                const float v[4] = {b[i][0], b[i][1], b[i][2], b[i][3]};
+                put4<3>(A.hi + r * p.pa + sq.c0(i) + q, A.lo - A.hi, v);
+            }
+        __syncthreads();
+        f32x4 x[NX];
+        small_product<true, NX>(A, X, sx, p.sp, lane, x);
+        const bool last = step + 1 == a.steps;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NX; ++i)
+            if (sx.mine(i)) {
+                const int c = sx.c0(i) + q;
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = x[i][e] * (last ? 1.f / (a.bs * kXs) : 1.f / a.bs);
+                if (!last) {
+                    put4<3>(X.hi + r * p.px + c, X.lo - X.hi, v);
+                } else if (r < s) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (c + e < l) om[wide ? r * a.n + c + e : (c + e) * a.n + r] = (O)v[e];
+                }
+            }
+        __syncthreads();
     }
 }
 
 template <class O>
 __global__ __launch_bounds__(256) void ortho_only_scale_kernel(const void* __restrict__ g, double eps,
-                                                               const double* __restrict__ part, long long mn,
+                                                               const double* __restrict__ part, int blocks, long long mn,
                                                                void* __restrict__ out) {
-    double t = 0.0;
-    for (int i = 0; i < kNormBlocks; ++i) t += part[blockIdx.y * kNormBlocks + i];
-    const double inv = 1.0 / (sqrt(t) + eps);
+    __shared__ double s[4];
+    const double inv = inverse_norm(part + (long long)blockIdx.y * blocks, blocks, eps, s);
     const long long base = blockIdx.y * mn;
     for (long long i = blockIdx.x * 256ll + threadIdx.x; i < mn; i += gridDim.x * 256ll)
         static_cast<O*>(out)[base + i] = (O)(float)((float)static_cast<const O*>(g)[base + i] * inv);
 }
 
 struct OrthoPlan {
-    int s, l, sp, np;      // smaller and larger side; row pitch of A and of X
-    size_t part, x0, x1, a, b, total;
+    int s, l, sp, np, blocks;                 // smaller and larger side; row pitch of A and of X
+    Cut gram, poly, apply;
+    size_t norm, x0, x1, a, b, part, total;
 };
+int tiles_of(ShapeId id, int M, int N, bool tri) {
+    const int b = id == kBig ? 256 : id == kSq ? 128 : 64, m = cdiv(M, b), n = cdiv(N, b);
+    return tri ? m * (m + 1) / 2 : m * n;
+}
+size_t part_bytes(const Cut& c, int M, int N, bool tri, int batch) {
+    const size_t b = c.shape == kBig ? 256 : c.shape == kSq ? 128 : 64;
+    return c.splits > 1 ? (size_t)batch * tiles_of(c.shape, M, N, tri) * c.splits * b * b * 4 : 0;
+}
 OrthoPlan ortho_plan(int batch, int m, int n) {
     OrthoPlan p;
     p.s = m < n ? m : n;
     p.l = m < n ? n : m;
     p.sp = pad8(p.s);
     p.np = pad8(n);
+    p.blocks = norm_blocks((long long)m * n);
+    auto cut = [&](int M, int N, int K, bool tri) {
+        return cut_of(
+            [&](long long b) {
+                const long long x = (M + b - 1) / b, y = (N + b - 1) / b;
+                return batch * (tri ? x * (x + 1) / 2 : x * y);
+            },
+            (double)M * N * batch * (tri ? 0.5 : 1.0), K, 2, true, true, cu_count());
+    };
+    p.gram = cut(p.s, p.s, p.l, true);
+    p.poly = cut(p.s, p.s, p.s, true);
+    p.apply = cut(n, m, p.s, false);
     const size_t x = align256((size_t)batch * m * p.np * 4), a = align256((size_t)batch * p.s * p.sp * 4);
+    size_t part = part_bytes(p.gram, p.s, p.s, true, batch), q = part_bytes(p.poly, p.s, p.s, true, batch);
+    if (q > part) part = q;
+    q = part_bytes(p.apply, n, m, false, batch);
+    if (q > part) part = q;
     size_t o = 0;
-    p.part = o; o += align256((size_t)batch * kNormBlocks * 8);
+    p.norm = o; o += align256((size_t)batch * p.blocks * 8);
     p.x0 = o; o += x;
     p.x1 = o; o += x;
     p.a = o; o += a;
     p.b = o; o += a;
+    p.part = o; o += align256(part);
     p.total = o;
     return p;
 }
@@ -199,40 +507,71 @@ int check_ortho(int batch, int m, int n) {
     return DS_OK;
 }
 
-template <class S, class O>
+template <class S, Lay LA, Lay LB, Use U, class O>
+void product_shape(ProductArgs p, const UseArgs& u, int tiles, hipStream_t q) {
+    const int units = tiles * p.splits;
+    const int grid = std::is_same<S, Big>::value && units > cu_count() ? cu_count() : units;
+    if (p.splits > 1) {
+        ortho_product_kernel<S, LA, LB, kGram, float, true><<<grid, S::T, 0, q>>>(p, u, units);
+        ortho_finish_kernel<S, U, O><<<dim3(tiles, S::FM), S::T, 0, q>>>(p, u);
+    } else {
+        ortho_product_kernel<S, LA, LB, U, O, false><<<grid, S::T, 0, q>>>(p, u, units);
+    }
+}
+template <Lay LA, Lay LB, Use U, class O>
+void product(const Cut& c, ProductArgs p, const UseArgs& u, int M, int N, hipStream_t q) {
+    p.splits = c.splits;
+    const int b = c.shape == kBig ? 256 : c.shape == kSq ? 128 : 64, tiles = tiles_of(c.shape, M, N, p.tri) * p.batch;
+    p.mt = cdiv(M, b);
+    p.nt = cdiv(N, b);
+    if (c.shape == kBig)
+        product_shape<Big, LA, LB, U, O>(p, u, tiles, q);
+    else if (c.shape == kSq)
+        product_shape<Sq, LA, LB, U, O>(p, u, tiles, q);
+    else
+        product_shape<Small, LA, LB, U, O>(p, u, tiles, q);
+}
+
+// stored B = 2^e B with |B| <= |a| + 2 |b| + 4 |c| below 2^15
+float b_scale(const double* co) {
+    const double bound = fabs(co[0]) + 2 * fabs(co[1]) + 4 * fabs(co[2]);
+    return (float)(bound > 0 ? exp2(floor(log2(32768.0 / bound))) : 1.0);
+}
+
+template <class O>
 void ortho_steps(const OrthoPlan& p, int batch, int m, int n, int steps, const double* co, char* ws, void* out, hipStream_t q) {
     f16 *x = reinterpret_cast<f16*>(ws + p.x0), *y = reinterpret_cast<f16*>(ws + p.x1);
     f16 *a = reinterpret_cast<f16*>(ws + p.a), *b = reinterpret_cast<f16*>(ws + p.b);
+    float* part = reinterpret_cast<float*>(ws + p.part);
     const long long px = 2ll * m * p.np, lox = (long long)m * p.np, pa = 2ll * p.s * p.sp, loa = (long long)p.s * p.sp;
-    // stored B = 2^e B with |B| <= |a| + 2 |b| + 4 |c| below 2^15
-    const double bound = fabs(co[0]) + 2 * fabs(co[1]) + 4 * fabs(co[2]);
-    const float bs = (float)(bound > 0 ? exp2(floor(log2(32768.0 / bound))) : 1.0);
+    const float bs = b_scale(co);
     const bool wide = m <= n;
-    const int t = cdiv(p.s, S::BM), tiles = t * (t + 1) / 2;
     for (int i = 0; i < steps; ++i) {
         const Operand X{x, p.np, lox, m, p.np}, A{a, p.sp, loa, p.s, p.sp}, B{b, p.sp, loa, p.s, p.sp};
-        const dim3 gs(tiles, batch);
+        const ProductArgs pg{X, X, px, px, 0, 0, 1, p.l, 1, batch, part};
+        const UseArgs ug{p.s, p.s, a, p.sp, loa, pa, nullptr, 0, 1.f / kXs, 0.f, 0.f};
         if (wide)
-            ortho_sym_kernel<S, kK, false><<<gs, S::T, 0, q>>>(X, px, p.s, n, a, p.sp, loa, pa, 0, 0, 0, 1.f / kXs);
+            product<kK, kK, kGram, float>(p.gram, pg, ug, p.s, p.s, q);
         else
-            ortho_sym_kernel<S, kM, false><<<gs, S::T, 0, q>>>(X, px, p.s, m, a, p.sp, loa, pa, 0, 0, 0, 1.f / kXs);
-        ortho_sym_kernel<S, kK, true><<<gs, S::T, 0, q>>>(A, pa, p.s, p.s, b, p.sp, loa, pa, (float)(co[0] * bs),
-                                                          (float)(co[1] * bs / kXs), (float)(co[2] * bs / (kXs * kXs)), 0.f);
-        const dim3 ga(cdiv(n, S::BM) * cdiv(m, S::BN), batch);
+            product<kM, kM, kGram, float>(p.gram, pg, ug, p.s, p.s, q);
+        const ProductArgs pp{A, A, pa, pa, 0, 0, 1, p.s, 1, batch, part};
+        const UseArgs up{p.s, p.s, b, p.sp, loa, pa, a, pa, (float)(co[0] * bs), (float)(co[1] * bs / kXs),
+                         (float)(co[2] * bs / (kXs * kXs))};
+        product<kK, kK, kPoly, float>(p.poly, pp, up, p.s, p.s, q);
         const bool last = i + 1 == steps;
-        const float f = last ? 1.f / (bs * kXs) : 1.f / bs;
-        void* to = last ? out : y;
-        const long long po = last ? (long long)m * n : px;
+        const UseArgs ua{m, n, last ? out : y, p.np, lox, last ? (long long)m * n : px, nullptr, 0,
+                         last ? 1.f / (bs * kXs) : 1.f / bs, 0.f, 0.f};
+        const ProductArgs pw{wide ? X : B, wide ? B : X, wide ? px : pa, wide ? pa : px, 0, 0, 0, p.s, 1, batch, part};
         if (wide) {
             if (last)
-                ortho_apply_kernel<S, kM, O><<<ga, S::T, 0, q>>>(X, B, px, pa, m, n, p.s, f, to, p.np, lox, po);
+                product<kM, kK, kLast, O>(p.apply, pw, ua, n, m, q);
             else
-                ortho_apply_kernel<S, kM, void><<<ga, S::T, 0, q>>>(X, B, px, pa, m, n, p.s, f, to, p.np, lox, po);
+                product<kM, kK, kNext, float>(p.apply, pw, ua, n, m, q);
         } else {
             if (last)
-                ortho_apply_kernel<S, kK, O><<<ga, S::T, 0, q>>>(B, X, pa, px, m, n, p.s, f, to, p.np, lox, po);
+                product<kK, kK, kLast, O>(p.apply, pw, ua, n, m, q);
             else
-                ortho_apply_kernel<S, kK, void><<<ga, S::T, 0, q>>>(B, X, pa, px, m, n, p.s, f, to, p.np, lox, po);
+                product<kK, kK, kNext, float>(p.apply, pw, ua, n, m, q);
         }
         f16* z = x;
         x = y;
@@ -240,25 +579,43 @@ void ortho_steps(const OrthoPlan& p, int batch, int m, int n, int steps, const d
     }
 }
 
+template <class O, int NA, int NX>
+int small_launch(const void* g, void* out, int batch, const SmallArgs& a, int bytes, hipStream_t q) {
+    if (bytes > 64 * 1024) {   // what a kernel may ask for without saying so
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&ortho_small_kernel<O, NA, NX>),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != hipSuccess) return (int)e;
+    }
+    ortho_small_kernel<O, NA, NX><<<batch, kSmallT, bytes, q>>>(static_cast<const O*>(g), static_cast<O*>(out), a);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? DS_OK : (int)e;
+}
+
 template <class O>
 int ortho_any(const OrthoPlan& p, const void* g, int dtype, int batch, int m, int n, int steps, const double* co, double eps,
               void* out, char* ws, hipStream_t q) {
-    double* part = reinterpret_cast<double*>(ws + p.part);
+    if (steps > 0 && small_fits(p.s, p.l)) {
+        const float bs = b_scale(co);
+        const SmallArgs a{m, n, steps, eps, (float)(co[0] * bs), (float)(co[1] * bs / kXs), (float)(co[2] * bs / (kXs * kXs)), bs};
+        const SmallPlan sp = small_plan(p.s, p.l);
+        const int nx = cdiv(sp.lp / 16, kSmallT / 64 / (sp.sp / 16));      // fragments of X a wave holds
+        if (sp.sp > 64) return small_launch<O, 8, 8>(g, out, batch, a, sp.bytes, q);
+        return nx <= 2   ? small_launch<O, 2, 2>(g, out, batch, a, sp.bytes, q)
+               : nx <= 5 ? small_launch<O, 2, 5>(g, out, batch, a, sp.bytes, q)
+                         : small_launch<O, 2, 10>(g, out, batch, a, sp.bytes, q);
+    }
+    double* part = reinterpret_cast<double*>(ws + p.norm);
     const long long mn = (long long)m * n;
-    ortho_norm_kernel<<<dim3(kNormBlocks, batch), 256, 0, q>>>(g, dtype, mn, part);
+    ortho_norm_kernel<<<dim3(p.blocks, batch), 256, 0, q>>>(g, dtype, mn, part);
     if (steps == 0) {
         const int nb = cdiv(mn, 1024) < 4096 ? cdiv(mn, 1024) : 4096;
-        ortho_only_scale_kernel<O><<<dim3(nb, batch), 256, 0, q>>>(g, eps, part, mn, out);
+        ortho_only_scale_kernel<O><<<dim3(nb, batch), 256, 0, q>>>(g, eps, part, p.blocks, mn, out);
     } else {
-        const int nb = cdiv(m, 4) < 2048 ? cdiv(m, 4) : 2048;
-        ortho_load_kernel<<<dim3(nb, batch), 256, 0, q>>>(g, dtype, m, n, p.np, eps, part, reinterpret_cast<f16*>(ws + p.x0),
-                                                          (long long)m * p.np, 2ll * m * p.np);
-        // 64x64 tiles where 128x128 ones would leave most of the chip idle
-        const int t = cdiv(p.s, 128);
-        if ((long long)t * (t + 1) / 2 * batch < cu_count())
-            ortho_steps<Shape<64, 64, 2, 2>, O>(p, batch, m, n, steps, co, ws, out, q);
-        else
-            ortho_steps<Shape<128, 128, 2, 2>, O>(p, batch, m, n, steps, co, ws, out, q);
+        const int nb = cdiv((long long)m * p.np, 4096) < 2048 ? cdiv((long long)m * p.np, 4096) : 2048;
+        ortho_load_kernel<<<dim3(nb, batch), 256, 0, q>>>(g, dtype, m, n, p.np, eps, part, p.blocks,
+                                                          reinterpret_cast<f16*>(ws + p.x0), (long long)m * p.np,
+                                                          2ll * m * p.np);
+        ortho_steps<O>(p, batch, m, n, steps, co, ws, out, q);
     }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? DS_OK : (int)e;
