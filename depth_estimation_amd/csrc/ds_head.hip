@@ -148,43 +148,112 @@ __global__ __launch_bounds__(kListT) void list_rows_kernel(const long long* __re
 static_assert(kListPer * kListT / 64 == 256, "the prefix handles four counts a lane");
 
 // --------------------------------------------------------------------------------------------------- staged operands
-// max |x| over `cnt` rows (listed in `rows` if given); order-independent, so repeatable
+// Row-wise passes over a matrix: a wave takes 64 / L rows at once, L lanes a row, VEC elements (16 bytes) a lane where rows are
+// aligned, one where not; L is the power of two that a row of D elements needs, at most 64.
+inline int lanes_for(int vectors) {
+    int l = 1;
+    while (l < vectors && l < 64) l <<= 1;
+    return l;
+}
+template <class IT, int VEC>
+struct Vec {
+    typedef IT type __attribute__((ext_vector_type(VEC)));
+};
 template <class IT>
-__global__ __launch_bounds__(256) void amax_kernel(const IT* __restrict__ x, long long ld, const int* __restrict__ rows,
-                                                   const int* __restrict__ cnt, int n, int D, unsigned* __restrict__ out) {
-    const int c = cnt ? *cnt : n;
-    float m = 0.f;
-    const int lane = threadIdx.x & 63;
-    for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < c; r += gridDim.x * 4) {
-        const IT* p = x + (rows ? rows[r] : r) * ld;
-        for (int d = lane; d < D; d += 64) m = fmaxf(m, finite_abs((float)p[d]));
+struct Vec<IT, 1> {
+    typedef IT type;
+};
+template <class IT, int VEC>
+__device__ __forceinline__ void load_vec(const IT* p, IT (&x)[VEC]) {
+    if constexpr (VEC == 1) {
+        x[0] = *p;
+    } else {
+        const typename Vec<IT, VEC>::type v = *reinterpret_cast<const typename Vec<IT, VEC>::type*>(p);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[e] = v[e];
     }
+}
+
+// max |x| over the rows of two matrices (one launch): `cnt` of the first one's, listed in `rows` if given, all n1 of the
+// second's; order-independent, so repeatable
+template <class IT, int VEC>
+__global__ __launch_bounds__(256) void amax_kernel(const IT* __restrict__ x, long long ld, const int* __restrict__ rows,
+                                                   HeadState* __restrict__ st, const IT* __restrict__ w, int V, int D, int L,
+                                                   int blocks_x) {
+    const bool second = (int)blockIdx.x >= blocks_x;
+    const int c = second ? V : st->count, b = second ? blockIdx.x - blocks_x : blockIdx.x;
+    const int nb = second ? gridDim.x - blocks_x : blocks_x;
+    const IT* src = second ? w : x;
+    const long long pitch = second ? D : ld;
+    const int lane = threadIdx.x & 63, sub = lane & (L - 1), R = 64 / L;
+    float m = 0.f;
+    constexpr int U = 4;        // rows under way at a time
+    for (int r0 = (b * 4 + (threadIdx.x >> 6)) * R + lane / L; r0 < c; r0 += nb * 4 * R * U)
+        for (int d = sub * VEC; d < D; d += L * VEC) {
+            IT v[U][VEC];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = min(r0 + u * nb * 4 * R, c - 1);
+                load_vec<IT, VEC>(src + (rows && !second ? rows[r] : r) * pitch + d, v[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) m = fmaxf(m, finite_abs((float)v[u][e]));
+        }
     m = wave_max(m);
-    if (lane == 0 && m > 0.f) atomicMax(out, __builtin_bit_cast(unsigned, m));
+    if (lane == 0 && m > 0.f) atomicMax(second ? &st->amax_w : &st->amax_h, __builtin_bit_cast(unsigned, m));
 }
 
 // rows of x (listed in `rows` if given) packed with a row pitch of Dp elements, zero behind D; fp32 as two scaled fp16 planes
-template <class IT, class T, int SPLIT>
+template <class IT, class T, int SPLIT, int VEC>
 __global__ __launch_bounds__(256) void stage_kernel(const IT* __restrict__ x, long long ld, const int* __restrict__ rows,
-                                                    const int* __restrict__ cnt, int n, int D, int Dp,
+                                                    const int* __restrict__ cnt, int n, int D, int Dp, int L,
                                                     const unsigned* __restrict__ amax, T* __restrict__ y, long long lo) {
     const int c = cnt ? *cnt : n;
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, sub = lane & (L - 1), R = 64 / L;
     const float scale = SPLIT == 3 ? scale_for(from_bits(*amax)) : 1.f;
-    for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < c; r += gridDim.x * 4) {
-        const IT* p = x + (rows ? rows[r] : r) * ld;
-        T* q = y + (long long)r * Dp;
-        for (int d = lane; d < Dp; d += 64) {
-            if constexpr (SPLIT == 3) {
-                f16 h, l;
-                split16(d < D ? (float)p[d] * scale : 0.f, h, l);
-                q[d] = h;
-                q[d + lo] = l;
-            } else {
-                q[d] = d < D ? p[d] : (IT)0.f;
+    constexpr int U = 4;
+    const int hop = gridDim.x * 4 * R;
+    for (int r0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * R + lane / L; r0 < c; r0 += hop * U)
+        for (int d = sub * VEC; d < Dp; d += L * VEC) {
+            IT v[U][VEC];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = min(r0 + u * hop, c - 1);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[u][e] = (IT)0.f;
+                if (d < D) load_vec<IT, VEC>(x + (rows ? rows[r] : r) * ld + d, v[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = r0 + u * hop;
+                if (r >= c) break;
+                T* q = y + (long long)r * Dp + d;
+                typename Vec<T, VEC>::type h, l;
+                if constexpr (VEC == 1) {
+                    if constexpr (SPLIT == 3) {
+                        split16((float)v[u][0] * scale, h, l);
+                    } else {
+                        h = v[u][0];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        if constexpr (SPLIT == 3) {
+                            f16 a, b;
+                            split16((float)v[u][e] * scale, a, b);
+                            h[e] = a;
+                            l[e] = b;
+                        } else {
+                            h[e] = v[u][e];
+                        }
+                    }
+                }
+                *reinterpret_cast<typename Vec<T, VEC>::type*>(q) = h;
+                if (SPLIT == 3) *reinterpret_cast<typename Vec<T, VEC>::type*>(q + lo) = l;
             }
         }
-    }
 }
 
 // ------------------------------------------------------------------------------------------------------------ forward
@@ -388,9 +457,9 @@ __global__ __launch_bounds__(256) void head_join_kernel(const float* __restrict_
 
 // the sum (mean) of the rows' losses, in a fixed order
 __global__ __launch_bounds__(256) void loss_total_kernel(const double* __restrict__ sums, const HeadState* __restrict__ st,
-                                                         int mean, float* __restrict__ out) {
+                                                         int mean, int entries, float* __restrict__ out) {
     __shared__ double s[256];
-    const int cnt = st->count, nb = (cnt + 31) / 32;
+    const int cnt = st->count, nb = entries > 0 ? entries : (cnt + 31) / 32;
     double a = 0.0;
     for (int i = threadIdx.x; i < nb; i += 256) a += sums[i];
     s[threadIdx.x] = a;
@@ -424,12 +493,16 @@ __device__ __forceinline__ float upstream(const Upstream& u, int n, int cnt) {
     if (u.each) return u.g[u.rows ? u.rows[n] : n];
     return u.mean ? u.g[0] / cnt : u.g[0];
 }
-__device__ __forceinline__ float dl_norm(const BackState* bs, int mode) {
+// the power of two dl is divided by, before Store<T>::k
+template <class T>
+__device__ __forceinline__ float dl_norm(const BackState* bs, const Upstream& u, int mode, int cnt) {
+    if (std::is_same<T, bf16>::value) return 1.f;
+    if (mode == kCE && !u.each) return pow2_above(finite_abs(upstream(u, 0, cnt)));
     const float g = pow2_above(from_bits(bs->gmax));
     return mode == kExpect ? g * pow2_above(2.f * from_bits(bs->cmax)) : g;
 }
 
-// largest |upstream| and |centre|; *bs zeroed by back_init_kernel before
+// largest |upstream| and |centre|, where dl_norm asks for them; *bs zeroed by back_init_kernel before
 __global__ void back_init_kernel(BackState* bs) { bs->gmax = bs->cmax = 0; }
 __global__ __launch_bounds__(256) void back_scale_kernel(Upstream u, const HeadState* __restrict__ st,
                                                          const float* __restrict__ centers, int V, BackState* __restrict__ bs) {
@@ -466,7 +539,7 @@ __device__ __forceinline__ void dl_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, i
                                            const BackState* bs, const DlArgs& a) {
     const float il = SPLIT == 3 ? 1.f / scale_for(from_bits(st->amax_h)) : 1.f;
     const float iw = SPLIT == 3 ? 1.f / scale_for(from_bits(st->amax_w)) : 1.f;
-    const float norm = Store<T>::k / dl_norm(bs, MODE);
+    const float norm = Store<T>::k / dl_norm<T>(bs, a.up, MODE, cnt);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / S::WN, wn = wave % S::WN, c0 = m0 + wm * S::FM * 16 + (lane >> 4) * 4;
     T* dl = static_cast<T*>(a.dl);
@@ -560,12 +633,13 @@ struct GradArgs {
     void* out;
     float* part;
     long long part_split;
+    Upstream up;
 };
 // which: 0 = dH, 1 = dW.  Writes the tile of row / class n and features m.
 template <class T, class S, int SPLIT, class O, bool ACC, int WHICH>
 __device__ __forceinline__ void grad_of_tile(const f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int sp, int bound,
                                              const HeadState* st, const BackState* bs, const GradArgs& a) {
-    const float f0 = dl_norm(bs, a.mode) / Store<T>::k;
+    const float f0 = dl_norm<T>(bs, a.up, a.mode, st->count) / Store<T>::k;
     const float is = SPLIT == 3 ? 1.f / scale_for(from_bits(WHICH == 0 ? st->amax_w : st->amax_h)) : 1.f;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / S::WN, wn = wave % S::WN, Dp = (a.D + 3) & ~3;
@@ -638,37 +712,504 @@ __global__ __launch_bounds__(S::T) void head_grad_kernel(Operand A, Operand B, c
     }
 }
 
-// sums the splits of a product in order, scales, and writes rows of the caller.  which: 0 = dH, 1 = dW
-template <class T, int SPLIT, class O>
+// sums the splits of a product in order, scales, and writes rows of the caller.  which: 0 = dH, 1 = dW.  PAR lanes share the
+// splits of an output (each a contiguous share, joined in order), for products of few outputs and many splits.
+template <class T, int SPLIT, class O, int PAR>
 __global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__ part, long long part_split, int splits,
                                                        const HeadState* __restrict__ st, const BackState* __restrict__ bs, int n,
-                                                       int D, int mode, int which, const int* __restrict__ rows,
+                                                       int D, int mode, int which, Upstream up, const int* __restrict__ rows,
                                                        O* __restrict__ out) {
+    constexpr int kOuts = 256 / PAR;
+    __shared__ f32x4 red[PAR][kOuts + 1];
     const int cnt = which == 0 ? st->count : n, Dp = (D + 3) & ~3, q = Dp / 4;
-    const float f0 = dl_norm(bs, mode) / Store<T>::k;
+    const float f0 = dl_norm<T>(bs, up, mode, st->count) / Store<T>::k;
     const float is = SPLIT == 3 ? 1.f / scale_for(from_bits(which == 0 ? st->amax_w : st->amax_h)) : 1.f;
     const bool aligned = (D & 3) == 0;
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < (long long)cnt * q; i += gridDim.x * 256ll) {
-        const long long r = i / q;
-        const int d = (int)(i % q) * 4;
+    const long long all = (long long)cnt * q;
+    const int x = threadIdx.x % kOuts, y = threadIdx.x / kOuts, per = (splits + PAR - 1) / PAR;
+    for (long long i0 = (long long)blockIdx.x * kOuts; i0 < all; i0 += (long long)gridDim.x * kOuts) {
+        const long long i = i0 + x;
         f32x4 a = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < splits; ++s) a += *reinterpret_cast<const f32x4*>(part + s * part_split + r * Dp + d);
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = a[e] * f0 * is;
-        put_row4(out + (rows && which == 0 ? (long long)rows[r] : r) * D, d, D, v, aligned);
+        if (i < all) {
+            const float* p = part + i * 4;
+            const int s1 = min(splits, (y + 1) * per);
+#pragma unroll 4
+            for (int s = y * per; s < s1; ++s) a += *reinterpret_cast<const f32x4*>(p + s * part_split);
+        }
+        if (PAR > 1) {
+            red[y][x] = a;
+            __syncthreads();
+            a = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (y == 0)
+                for (int s = 0; s < PAR; ++s) a += red[s][x];
+            __syncthreads();
+        }
+        if (i < all && y == 0) {
+            const long long r = i / q;
+            const int d = (int)(i - r * q) * 4;
+            const float v[4] = {a[0] * f0 * is, a[1] * f0 * is, a[2] * f0 * is, a[3] * f0 * is};
+            put_row4(out + (rows && which == 0 ? (long long)rows[r] : r) * D, d, D, v, aligned);
+        }
     }
 }
 
 // rows that were left out have no gradient
-template <class O>
+template <class O, int VEC>
 __global__ __launch_bounds__(256) void zero_ignored_kernel(const long long* __restrict__ target, int n, long long ignore, int D,
-                                                           const HeadState* __restrict__ st, O* __restrict__ out) {
+                                                           int L, const HeadState* __restrict__ st, O* __restrict__ out) {
     if (st->count == n) return;
-    const int lane = threadIdx.x & 63;
-    for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < n; r += gridDim.x * 4)
-        if (target[r] == ignore)
-            for (int d = lane; d < D; d += 64) out[(long long)r * D + d] = (O)0.f;
+    const int lane = threadIdx.x & 63, sub = lane & (L - 1), R = 64 / L, hop = gridDim.x * 4 * R;
+    constexpr int U = 4;
+    for (int r0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * R + lane / L; r0 < n; r0 += hop * U) {
+        long long t[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) t[u] = target[min(r0 + u * hop, n - 1)];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (r0 + u * hop < n && t[u] == ignore)
+                for (int d = sub * VEC; d < D; d += L * VEC) {
+                    typename Vec<O, VEC>::type z;
+                    if constexpr (VEC == 1) {
+                        z = (O)0.f;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) z[e] = (O)0.f;
+                    }
+                    *reinterpret_cast<typename Vec<O, VEC>::type*>(out + (long long)(r0 + u * hop) * D + d) = z;
+                }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------ small heads
+//
+// A head whose weight fits LDS (depth bins) is bound by the features' bytes, not by its products: a wave takes 16 rows, keeps
+// their features in registers, meets all classes in LDS and has the whole softmax of its rows to itself -- no partial
+// statistics, no barrier.  Backward the same: dl of 32 classes, as the matrix instruction leaves it, is the operand of
+// dH = dl W as it stands (its lanes hold rows, its registers classes, taken as k in the order 4 q + e of two fragments; the
+// transposing LDS reads of W follow that order), so dH needs no second pass; dl itself is written once for dW.
+//   12 x 96 x 320 rows, 64 features, 80 bins, bf16, forward: 48 -> SLIMF us (47 MB of features)
+constexpr int kSlimT = 512;
+struct SlimArgs {
+    const void* h;             // features: the caller's rows, or staged ones
+    long long ldh, lo_h;
+    const int* gather;         // where the features of a kept row are (NULL: in order)
+    const int* rows;           // the caller's row of a kept row (NULL: the same)
+    HeadState* st;             // count of kept rows and scales; set_count: n rows, and st->count is written
+    int set_count;
+    int n, D, V, Vp;           // Vp: V rounded up to 32
+    Operand W;
+    int planes_scaled;         // two planes: divide by the scales
+    const int* tgt;
+    const float* centers;
+    float *top, *inv_sum, *mean;
+};
+struct SlimFwd {
+    float* out;                // CE: per caller's row (NULL: only sums), expectation: per row
+    double* sums;              // CE: a workgroup's sum of losses (NULL: none)
+};
+struct SlimBwd {
+    const BackState* bs;
+    Upstream up;
+    void* g_hidden;            // NULL: not wanted
+    void* dl;                  // NULL: dW not wanted
+    int ld;
+    long long lo;
+    void* packed;              // kept rows' features written densely for dW (NULL: they lie so already), pitch Dp
+    int Dp;
+};
+
+// W to LDS: per plane, blocks of 64 columns, each [Vp][64] in lds_chunk's order
+template <int P, int ND>
+__device__ __forceinline__ void slim_load_w(const SlimArgs& a, char* lds) {
+    constexpr int kChunks = ND * 4;
+    for (int i = threadIdx.x; i < a.Vp * kChunks; i += kSlimT) {
+        const int v = i / kChunks, c = i % kChunks;
+        const bool in = v < a.V && c * 8 < a.W.inner;
+        const char* src = static_cast<const char*>(a.W.p) + 2 * ((long long)v * a.W.ld + c * 8);
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            i32x4 x = {0, 0, 0, 0};
+            if (in) x = *reinterpret_cast<const i32x4*>(src + 2 * p * a.W.lo);
+            *reinterpret_cast<i32x4*>(lds + p * a.Vp * ND * 64 + (c >> 3) * a.Vp * 128 + lds_chunk<kK, 16>(v, c & 7)) = x;
+        }
+    }
+    __syncthreads();
+}
+template <int P, int ND>
+struct SlimRows {
+    s16x8 h[P][ND];
+    __device__ __forceinline__ void load(const SlimArgs& a, int n, int cnt, int lane) {
+        const int m = n < cnt ? n : cnt - 1;
+        const long long row = a.gather ? a.gather[m] : m;
+        const char* p = static_cast<const char*>(a.h) + 2 * (row * a.ldh + (lane >> 4) * 8);
+#pragma unroll
+        for (int k = 0; k < ND; ++k)
+#pragma unroll
+            for (int q = 0; q < P; ++q) {
+                s16x8 x = {0, 0, 0, 0, 0, 0, 0, 0};
+                if (k * 32 + (lane >> 4) * 8 < a.D) x = *reinterpret_cast<const s16x8*>(p + 2 * (k * 32 + q * a.lo_h));
+                h[q][k] = x;
+            }
+    }
+};
+// logits of the 16 classes of fragment f for the wave's rows: lane holds row lane % 16, classes 16 f + 4 (lane / 16) + e
+template <class T, int P, int ND>
+__device__ __forceinline__ f32x4 slim_logits(const SlimRows<P, ND>& r, const char* lds, int base, int f, int Vp, float scale) {
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < ND; ++k) {
+        const char* p = lds + (k >> 1) * Vp * 128 + f * 16 * 128 + (base ^ ((k & 1) << 6));
+        const s16x8 w = *reinterpret_cast<const s16x8*>(p);
+        if (P == 2) {
+            const s16x8 wl = *reinterpret_cast<const s16x8*>(p + Vp * ND * 64);
+            acc = mfma(wl, r.h[0][k], acc, T());
+            acc = mfma(w, r.h[P - 1][k], acc, T());
+        }
+        acc = mfma(w, r.h[0][k], acc, T());
+    }
+    return P == 2 ? acc * scale : acc;
+}
+__device__ __forceinline__ void join_softmax(float& mx, float& s, float& sc, float m2, float s2, float c2) {
+    const float nm = fmaxf(mx, m2), ref = nm == -INFINITY ? 0.f : nm;
+    const float f1 = exp_of(mx - ref), f2 = exp_of(m2 - ref);
+    s = s * f1 + s2 * f2;
+    sc = sc * f1 + c2 * f2;
+    mx = nm;
+}
+__device__ __forceinline__ float slim_scale(const SlimArgs& a) {
+    return a.planes_scaled ? 1.f / scale_for(from_bits(a.st->amax_h)) * (1.f / scale_for(from_bits(a.st->amax_w))) : 1.f;
+}
+
+template <class T, int P, int ND, int MODE>
+__global__ __launch_bounds__(kSlimT) void slim_fwd_kernel(SlimArgs a, SlimFwd o) {
+    extern __shared__ __align__(16) char lds[];
+    __shared__ double wsum[kSlimT / 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int cnt = a.set_count ? a.n : a.st->count, blocks = (cnt + 15) / 16, step = gridDim.x * (kSlimT / 64);
+    int b = blockIdx.x * (kSlimT / 64) + wave;
+    if (a.set_count && blockIdx.x == 0 && threadIdx.x == 0) a.st->count = a.n;
+    SlimRows<P, ND> next;
+    if (b < blocks) next.load(a, b * 16 + (lane & 15), cnt, lane);
+    slim_load_w<P, ND>(a, lds);
+    const float scale = slim_scale(a);
+    const int base = lds_chunk<kK, 16>(lane & 15, lane >> 4), frags = a.Vp / 16;
+    double total = 0.0;
+    for (; b < blocks; b += step) {
+        const SlimRows<P, ND> r = next;
+        const int n = b * 16 + (lane & 15);
+        if (b + step < blocks) next.load(a, (b + step) * 16 + (lane & 15), cnt, lane);
+        const int t = MODE == kCE ? a.tgt[n < cnt ? n : cnt - 1] : -1;
+        float mx = -INFINITY, s = 0.f, sc = 0.f, tl = 0.f;
+        for (int f = 0; f < frags; f += 2) {
+            f32x4 l[2];
+            float m = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                l[u] = slim_logits<T, P, ND>(r, lds, base, f + u, a.Vp, scale);
+                const int v = (f + u) * 16 + (lane >> 4) * 4;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (v + e >= a.V) l[u][e] = -INFINITY;
+                    if (MODE == kCE && v + e == t) tl = l[u][e];
+                    m = fmaxf(m, l[u][e]);      // passes over NaN, which reaches the sum
+                }
+            }
+            const float nm = fmaxf(mx, m), ref = nm == -INFINITY ? 0.f : nm, f1 = exp_of(mx - ref);
+            s *= f1;
+            sc *= f1;
+            mx = nm;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int v = (f + u) * 16 + (lane >> 4) * 4;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = exp_of(l[u][e] - ref);
+                    s += x;
+                    if (MODE == kExpect) sc = fmaf(x, a.centers[v + e < a.V ? v + e : a.V - 1], sc);
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 16; d < 64; d <<= 1) {
+            join_softmax(mx, s, sc, __shfl_xor(mx, d, 64), __shfl_xor(s, d, 64), __shfl_xor(sc, d, 64));
+            if (MODE == kCE) tl += __shfl_xor(tl, d, 64);     // three of the four are zero
+        }
+        if (lane < 16 && n < cnt) {
+            const float ref = mx == -INFINITY ? 0.f : mx;
+            a.top[n] = ref;
+            a.inv_sum[n] = 1.f / s;
+            if (MODE == kExpect) {
+                o.out[n] = a.mean[n] = sc / s;
+            } else {
+                const float each = t < 0 ? __builtin_nanf("") : (ref - tl) + logf(s);
+                if (o.out) o.out[a.rows ? a.rows[n] : n] = each;
+                total += each;
+            }
+        }
+    }
+    if (MODE == kCE && o.sums) {
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) total += __shfl_xor(total, d, 64);
+        if (lane == 0) wsum[wave] = total;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            double x = 0.0;
+            for (int i = 0; i < kSlimT / 64; ++i) x += wsum[i];
+            o.sums[blockIdx.x] = x;
+        }
+    }
+}
+
+template <class T, int P, int ND, int MODE, class O>
+__global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o) {
+    extern __shared__ __align__(16) char lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int cnt = a.st->count, blocks = (cnt + 15) / 16, step = gridDim.x * (kSlimT / 64);
+    int b = blockIdx.x * (kSlimT / 64) + wave;
+    SlimRows<P, ND> next;
+    if (b < blocks) next.load(a, b * 16 + (lane & 15), cnt, lane);
+    slim_load_w<P, ND>(a, lds);
+    const float scale = slim_scale(a), norm = Store<T>::k / dl_norm<T>(o.bs, o.up, MODE, cnt);
+    const float back = dl_norm<T>(o.bs, o.up, MODE, cnt) / Store<T>::k *
+                       (a.planes_scaled ? 1.f / scale_for(from_bits(a.st->amax_w)) : 1.f);
+    const int base = lds_chunk<kK, 16>(lane & 15, lane >> 4), frags = a.Vp / 16;
+    // transposing reads: lane i of a 16-lane group q starts at class 4 q + i / 4, feature 4 (i % 4)
+    const int tr = (lane >> 4) * 4 + ((lane >> 2) & 3);
+    const int tbase = lds_chunk<kK, 16>(tr, (lane >> 1) & 1) + (lane & 1) * 8;
+    typedef __attribute__((address_space(3))) s16x4* lp;
+    T* dl = static_cast<T*>(o.dl);
+    for (; b < blocks; b += step) {
+        const SlimRows<P, ND> r = next;
+        const int n = b * 16 + (lane & 15), m = n < cnt ? n : cnt - 1;
+        if (b + step < blocks) next.load(a, (b + step) * 16 + (lane & 15), cnt, lane);
+        const float tp = a.top[m], rs = a.inv_sum[m], e0 = MODE == kExpect ? a.mean[m] : 0.f;
+        const int t = MODE == kCE ? a.tgt[m] : -1;
+        float g = upstream(o.up, m, cnt) * norm;
+        if (MODE == kCE && t < 0) g = __builtin_nanf("");
+        const float gr = g * rs;
+        f32x4 acc[2 * ND];
+#pragma unroll
+        for (int i = 0; i < 2 * ND; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int f = 0; f < frags; f += 2) {
+            f32x4 d[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const f32x4 l = slim_logits<T, P, ND>(r, lds, base, f + u, a.Vp, scale);
+                const int v = (f + u) * 16 + (lane >> 4) * 4;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = exp_of(l[e] - tp);
+                    float y;
+                    if (MODE == kExpect)
+                        y = x * gr * (a.centers[v + e < a.V ? v + e : a.V - 1] - e0);
+                    else
+                        y = v + e == t ? (x * rs - 1.f) * g : x * gr;
+                    d[u][e] = v + e < a.V ? y : 0.f;
+                }
+                if (dl && n < cnt && v < o.ld) {
+                    const float y[4] = {d[u][0], d[u][1], d[u][2], d[u][3]};
+                    put4<P == 2 ? 3 : 1>(dl + (long long)n * o.ld + v, o.lo, y);
+                }
+            }
+            if (o.g_hidden) {
+                typedef T t8 __attribute__((ext_vector_type(8)));
+                t8 hi, lw;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float y = d[e >> 2][e & 3];
+                    if constexpr (P == 2) {
+                        f16 p, q;
+                        split16(y, p, q);
+                        hi[e] = p;
+                        lw[e] = q;
+                    } else {
+                        hi[e] = (T)y;
+                    }
+                }
+                const s16x8 bh = __builtin_bit_cast(s16x8, hi);
+#pragma unroll
+                for (int i = 0; i < 2 * ND; ++i) {
+                    const char* p = lds + (i >> 2) * a.Vp * 128 + f * 16 * 128 + (tbase ^ ((i & 3) << 5));
+                    auto get = [&](const char* q) {
+                        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q));
+                        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q + 16 * 128));
+                        return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+                    };
+                    const s16x8 w = get(p);
+                    if constexpr (P == 2) {
+                        acc[i] = mfma(get(p + a.Vp * ND * 64), bh, acc[i], T());
+                        acc[i] = mfma(w, __builtin_bit_cast(s16x8, lw), acc[i], T());
+                    }
+                    acc[i] = mfma(w, bh, acc[i], T());
+                }
+            }
+        }
+        if (n < cnt) {
+            if (o.g_hidden) {
+                O* row = static_cast<O*>(o.g_hidden) + (long long)(a.rows ? a.rows[n] : n) * a.D;
+#pragma unroll
+                for (int i = 0; i < 2 * ND; ++i) {
+                    const int c = i * 16 + (lane >> 4) * 4;
+                    const float y[4] = {acc[i][0] * back, acc[i][1] * back, acc[i][2] * back, acc[i][3] * back};
+                    if (c < a.D) put_row4(row, c, a.D, y, (a.D & 3) == 0);
+                }
+            }
+            if (o.packed) {
+#pragma unroll
+                for (int k = 0; k < ND; ++k) {
+                    const int c = k * 32 + (lane >> 4) * 8;
+                    if (c < o.Dp) *reinterpret_cast<s16x8*>(static_cast<T*>(o.packed) + (long long)n * o.Dp + c) = r.h[0][k];
+                }
+            }
+        }
+    }
+}
+
+// ----------------------------------------------------------------------------------------------------------- few rows
+//
+// Up to eight rows (a single position answered) read the weight once and are bound by that: every class row goes straight from
+// memory to registers, as it is (fp32 too: no planes), and meets the rows' features out of LDS in fp32.  L lanes share a
+// class, four classes a group are under way at a time.
+constexpr int kFewT = 512, kFewMax = 8;
+struct FewArgs {
+    const int* rows;
+    HeadState* st;
+    int set_count, n, D, V, L;
+    const int* tgt;
+    const float* centers;
+    float* part;               // [workgroup][row][4]: maximum, sum, sum of centres, logit of the target
+};
+template <class IT, int VEC, int NR>
+__global__ __launch_bounds__(kFewT) void few_kernel(const IT* __restrict__ h, long long ldh, const IT* __restrict__ w, FewArgs a) {
+    extern __shared__ __align__(16) char lds_[];
+    float* hs = reinterpret_cast<float*>(lds_);            // [NR][Dq]
+    __shared__ float red[kFewT / 64][NR][4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, Dq = (a.D + 7) & ~7;
+    if (a.set_count && blockIdx.x == 0 && threadIdx.x == 0) a.st->count = a.n;
+    const int cnt = a.set_count ? a.n : a.st->count;
+    for (int r = 0; r < NR; ++r)
+        for (int d = threadIdx.x; d < Dq; d += kFewT)
+            hs[r * Dq + d] = r < cnt && d < a.D ? (float)h[(a.rows ? a.rows[r] : r) * ldh + d] : 0.f;
+    __syncthreads();
+    const int L = a.L, sub = lane & (L - 1), G = 64 / L;
+    const int groups = gridDim.x * (kFewT / 64) * G, g = (blockIdx.x * (kFewT / 64) + wave) * G + lane / L;
+    constexpr int U = 4;
+    float mx[NR], s[NR], sc[NR], tl[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+        mx[r] = -INFINITY;
+        s[r] = sc[r] = tl[r] = 0.f;
+    }
+    for (int v0 = g; v0 < a.V; v0 += groups * U) {
+        float acc[U][NR];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < NR; ++r) acc[u][r] = 0.f;
+        for (int d = sub * VEC; d < a.D; d += L * VEC) {
+            IT x[U][VEC];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int v = min(v0 + u * groups, a.V - 1);
+                load_vec<IT, VEC>(w + (long long)v * a.D + d, x[u]);
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    const float y = hs[r * Dq + d + e];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) acc[u][r] = fmaf((float)x[u][e], y, acc[u][r]);
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int v = v0 + u * groups;
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                float l = acc[u][r];
+                for (int o = 1; o < L; o <<= 1) l += __shfl_xor(l, o, 64);
+                if (v < a.V) {
+                    if (a.tgt && v == a.tgt[r < cnt ? r : 0]) tl[r] = l;
+                    join_softmax(mx[r], s[r], sc[r], l, 1.f, a.centers ? a.centers[v] : 0.f);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+        for (int o = L; o < 64; o <<= 1) {
+            join_softmax(mx[r], s[r], sc[r], __shfl_xor(mx[r], o, 64), __shfl_xor(s[r], o, 64), __shfl_xor(sc[r], o, 64));
+            tl[r] += __shfl_xor(tl[r], o, 64);          // one group met the target
+        }
+        if (lane == 0) {
+            red[wave][r][0] = mx[r];
+            red[wave][r][1] = s[r];
+            red[wave][r][2] = sc[r];
+            red[wave][r][3] = tl[r];
+        }
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < NR) {
+        const int r = threadIdx.x;
+        float m = -INFINITY, t = 0.f, c = 0.f, l = 0.f;
+        for (int i = 0; i < kFewT / 64; ++i) {
+            join_softmax(m, t, c, red[i][r][0], red[i][r][1], red[i][r][2]);
+            l += red[i][r][3];
+        }
+        float* q = a.part + ((long long)blockIdx.x * NR + r) * 4;
+        q[0] = m;
+        q[1] = t;
+        q[2] = c;
+        q[3] = l;
+    }
+}
+// joins the workgroups of few_kernel (or the class tiles of the thin shape): one workgroup, a wave per row at a time
+struct JoinArgs {
+    const float *mx, *s, *sc, *tl;      // entry i of row r at [i * step + r * pitch]; tl: per row where tl_step is 0
+    long long step, pitch, tl_step;
+    int entries, mode;
+    const HeadState* st;
+    const int* rows;
+    const int* tgt;
+    float *top, *inv_sum, *mean, *out;
+    int total;                          // CE: 0 each row, 1 sum, 2 mean
+};
+__global__ __launch_bounds__(1024) void join_few_kernel(JoinArgs a) {
+    __shared__ float each[32];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cnt = a.st->count;
+    for (int r = wave; r < cnt; r += 16) {
+        float mx = -INFINITY, s = 0.f, sc = 0.f, tl = 0.f;
+        for (int i = lane; i < a.entries; i += 64) {
+            const long long at = i * a.step + r * a.pitch;
+            join_softmax(mx, s, sc, a.mx[at], a.s[at], a.mode == kExpect ? a.sc[at] : 0.f);
+            if (a.mode == kCE && a.tl_step) tl += a.tl[at];
+        }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            join_softmax(mx, s, sc, __shfl_xor(mx, o, 64), __shfl_xor(s, o, 64), __shfl_xor(sc, o, 64));
+            tl += __shfl_xor(tl, o, 64);
+        }
+        if (lane == 0) {
+            const float ref = mx == -INFINITY ? 0.f : mx;
+            a.top[r] = ref;
+            a.inv_sum[r] = 1.f / s;
+            if (a.mode == kExpect) {
+                a.out[r] = a.mean[r] = sc / s;
+            } else {
+                if (!a.tl_step) tl = a.tl[r];
+                each[r] = a.tgt[r] < 0 ? __builtin_nanf("") : (ref - tl) + logf(s);
+                if (!a.total) a.out[a.rows[r]] = each[r];
+            }
+        }
+    }
+    if (a.mode == kExpect || !a.total) return;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = 0.0;
+        for (int r = 0; r < cnt; ++r) t += each[r];
+        a.out[0] = (float)(a.total == DS_REDUCE_MEAN ? t / cnt : t);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
@@ -680,6 +1221,8 @@ Cut cut_of(long long M, long long N, long long K, int planes, bool may_split) {
     return ds::cut_of([&](long long b) { return ((M + b - 1) / b) * ((N + b - 1) / b); }, (double)M * N, K, planes, may_split,
                       false, cu_count());
 }
+
+bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
 struct Saved {
     HeadState* st;
@@ -708,6 +1251,9 @@ struct Plan {
     int dtype, planes, Dp, vt_fwd, piece, piece_ld, dh_splits, dw_splits;
     bool stage_w, stage_h, dh_part;
     ShapeId fwd, dl_shape, dh, dw;
+    int few, few_grid;                 // forward of few rows: rows a workgroup holds (0: not that path)
+    int slim, slim_bytes, slim_grid;   // small head: k steps of 32 a row (0: not that path); backward: slim_back
+    bool slim_back, pack;
     size_t staged_h, staged_w, counts, tlogit, part, sums, fwd_total;      // offsets of the forward's workspace
     size_t bh, bw, bs, dl, dhp, dwp, bwd_total;                            // offsets of the backward's
 };
@@ -725,10 +1271,25 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     p.planes = dtype == DS_F32 ? 2 : 1;
     p.Dp = pad8(D);
     p.stage_w = dtype == DS_F32 || D % 8 != 0;
-    p.stage_h = mode == kCE || dtype == DS_F32 || D % 8 != 0 || ldh % 8 != 0;
     const size_t el = 2 * p.planes;
-    const size_t h = p.stage_h ? align256((size_t)N * p.Dp * el) : 0, w = p.stage_w ? align256((size_t)V * p.Dp * el) : 0;
     const bool thin = N <= 32, flat = D <= 64;
+    // few rows: their features have to fit LDS in fp32 beside three more workgroups
+    p.few = N > kFewMax ? 0 : N <= 1 ? 1 : N <= 2 ? 2 : N <= 4 ? 4 : 8;
+    if (p.few && (size_t)p.few * pad8(D) * 4 > 40 * 1024) p.few = 0;
+    const int vec = dtype == DS_F32 ? 4 : 8, lanes = lanes_for(cdiv(D, D % vec == 0 ? vec : 1));
+    p.few_grid = cdiv(V, kFewT / lanes * 4) < 2 * cu_count() ? cdiv(V, kFewT / lanes * 4) : 2 * cu_count();
+    // small head: the weight in LDS, two workgroups a CU
+    const int Vp = (V + 31) & ~31;
+    p.slim = D <= 64 ? 2 : D <= 128 ? 4 : D <= 256 ? 8 : 0;
+    const long long bytes = (long long)Vp * p.slim * 64 * p.planes;
+    if (bytes > 78 * 1024) p.slim = 0;
+    p.slim_bytes = (int)bytes;
+    p.slim_grid = cdiv(N, 16 * (kSlimT / 64)) < 2 * cu_count() ? cdiv(N, 16 * (kSlimT / 64)) : 2 * cu_count();
+    p.slim_back = p.slim && (long long)N * pad8(V) * (long long)el <= (1ll << 30);
+    const bool whole = D % 8 == 0 && ldh % 8 == 0 && dtype != DS_F32;     // rows of the caller's can be read as they are
+    p.stage_h = !whole || (mode == kCE && !p.slim_back);
+    p.pack = whole && mode == kCE && p.slim_back;
+    const size_t h = p.stage_h || p.pack ? align256((size_t)N * p.Dp * el) : 0, w = p.stage_w ? align256((size_t)V * p.Dp * el) : 0;
     p.fwd = thin ? kThin : cut_of(V, N, D, p.planes, false).shape;
     p.vt_fwd = cdiv(V, p.fwd == kBig ? Big::BM : Sq::BM);
     size_t o = 0;
@@ -736,12 +1297,12 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     p.staged_w = o; o += w;
     p.counts = o; o += align256((size_t)cdiv(N, kListBlock) * 4);
     p.tlogit = o; o += align256((size_t)N * 4);
-    p.part = o; o += 3 * align256((size_t)p.vt_fwd * N * 4);
-    p.sums = o; o += align256((size_t)cdiv(N, 32) * 8);
+    p.part = o; o += p.few ? align256((size_t)p.few_grid * p.few * 16) : p.slim ? 0 : 3 * align256((size_t)p.vt_fwd * N * 4);
+    p.sums = o; o += align256((size_t)(cdiv(N, 32) > p.slim_grid ? cdiv(N, 32) : p.slim_grid) * 8);
     p.fwd_total = o;
     // a piece of the classes: what fits 256 MB of dl, at least 1024 classes, a multiple of 256
     const long long fit = (256ll << 20) / ((long long)el * N) / 256 * 256;
-    const long long piece = fit < 1024 ? 1024 : fit;
+    const long long piece = p.slim_back ? V : fit < 1024 ? 1024 : fit;
     p.piece = piece >= V ? V : (int)piece;
     p.piece_ld = pad8(p.piece);
     p.dl_shape = thin ? kThin : cut_of(p.piece, N, D, p.planes, false).shape;
@@ -778,29 +1339,98 @@ int launched() {
     return e == hipSuccess ? DS_OK : (int)e;
 }
 
+template <class IT, class T, int SPLIT>
+void stage(const IT* x, long long ld, const int* rows, const int* cnt, long long n, int D, int Dp, const unsigned* amax, T* y,
+           long long lo, hipStream_t q) {
+    constexpr int VEC = 16 / sizeof(IT);
+    const bool v = D % VEC == 0 && ld % VEC == 0 && !misaligned(x);
+    const int L = lanes_for(v ? Dp / VEC : Dp), blocks = cdiv(n, 4 * 64 / L * 2), grid = blocks < 4096 ? blocks : 4096;
+    if (v)
+        stage_kernel<IT, T, SPLIT, VEC><<<grid, 256, 0, q>>>(x, ld, rows, cnt, (int)n, D, Dp, L, amax, y, lo);
+    else
+        stage_kernel<IT, T, SPLIT, 1><<<grid, 256, 0, q>>>(x, ld, rows, cnt, (int)n, D, Dp, L, amax, y, lo);
+}
+// scales of fp32 inputs (st->amax_h, amax_w; zeroed before)
+template <class IT>
+void scales(const IT* hidden, long long ldh, const int* rows, const IT* weight, long long N, int D, int V, HeadState* st,
+            hipStream_t q) {
+    constexpr int VEC = 16 / sizeof(IT);
+    const bool v = D % VEC == 0 && ldh % VEC == 0 && !misaligned(hidden) && !misaligned(weight);
+    const int L = lanes_for(v ? D / VEC : D), per = 4 * 64 / L * 4;
+    const int bx = cdiv(N, per) < 1024 ? cdiv(N, per) : 1024, bw = cdiv(V, per) < 1024 ? cdiv(V, per) : 1024;
+    if (v)
+        amax_kernel<IT, VEC><<<bx + bw, 256, 0, q>>>(hidden, ldh, rows, st, weight, V, D, L, bx);
+    else
+        amax_kernel<IT, 1><<<bx + bw, 256, 0, q>>>(hidden, ldh, rows, st, weight, V, D, L, bx);
+}
 // inputs as matrix operands: in place, or staged into `ws`
 template <class IT, class T, int SPLIT>
 void operands(const Plan& p, const IT* hidden, long long ldh, const IT* weight, long long N, int D, int V, const Saved& s,
-              const int* rows, bool need_amax, char* wh, char* ww, Operand& H, Operand& W, hipStream_t q) {
-    const int gh = cdiv(N, 4) < 4096 ? cdiv(N, 4) : 4096, gw = cdiv(V, 4) < 4096 ? cdiv(V, 4) : 4096;
-    if (SPLIT == 3 && need_amax) {
-        amax_kernel<IT><<<gh < 1024 ? gh : 1024, 256, 0, q>>>(hidden, ldh, rows, &s.st->count, (int)N, D, &s.st->amax_h);
-        amax_kernel<IT><<<gw < 1024 ? gw : 1024, 256, 0, q>>>(weight, D, nullptr, nullptr, V, D, &s.st->amax_w);
-    }
+              const int* rows, bool need_scales, char* wh, char* ww, Operand& H, Operand& W, hipStream_t q) {
+    if constexpr (SPLIT == 3)
+        if (need_scales) scales(hidden, ldh, rows, weight, N, D, V, s.st, q);
     H = Operand{hidden, ldh, 0, (int)N, D};
     W = Operand{weight, D, 0, V, D};
     if (p.stage_h) {
         const long long lo = N * p.Dp;
-        stage_kernel<IT, T, SPLIT><<<gh, 256, 0, q>>>(hidden, ldh, rows, &s.st->count, (int)N, D, p.Dp, &s.st->amax_h,
-                                                      reinterpret_cast<T*>(wh), lo);
+        stage<IT, T, SPLIT>(hidden, ldh, rows, &s.st->count, N, D, p.Dp, &s.st->amax_h, reinterpret_cast<T*>(wh), lo, q);
         H = Operand{wh, p.Dp, lo, (int)N, p.Dp};
     }
     if (p.stage_w) {
         const long long lo = (long long)V * p.Dp;
-        stage_kernel<IT, T, SPLIT><<<gw, 256, 0, q>>>(weight, D, nullptr, nullptr, V, D, p.Dp, &s.st->amax_w,
-                                                      reinterpret_cast<T*>(ww), lo);
+        stage<IT, T, SPLIT>(weight, D, nullptr, nullptr, V, D, p.Dp, &s.st->amax_w, reinterpret_cast<T*>(ww), lo, q);
         W = Operand{ww, p.Dp, lo, V, p.Dp};
     }
+}
+
+template <class K>
+int with_lds(K kernel, int bytes) {    // what a kernel may use beyond 64 KB it has to ask for
+    return bytes <= 64 * 1024 ? 0
+                              : (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                         hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+SlimArgs slim_args(const Plan& p, const Operand& H, const Operand& W, const Saved& s, const int* rows, long long N, int D, int V,
+                   const float* centers) {
+    return SlimArgs{H.p, H.ld, H.lo, p.stage_h ? nullptr : rows, rows, s.st, 0, (int)N, D, V, (V + 31) & ~31, W, p.planes == 2,
+                    s.tgt, centers, s.top, s.inv_sum, s.mean};
+}
+template <class T, int P, int ND, int MODE>
+int slim_fwd_launch(const Plan& p, const SlimArgs& a, const SlimFwd& o, hipStream_t q) {
+    const int rc = with_lds(&slim_fwd_kernel<T, P, ND, MODE>, p.slim_bytes);
+    if (rc) return rc;
+    slim_fwd_kernel<T, P, ND, MODE><<<p.slim_grid, kSlimT, p.slim_bytes, q>>>(a, o);
+    return 0;
+}
+template <class T, int P, int ND, int MODE, class O>
+int slim_bwd_launch(const Plan& p, const SlimArgs& a, const SlimBwd& o, hipStream_t q) {
+    const int rc = with_lds(&slim_bwd_kernel<T, P, ND, MODE, O>, p.slim_bytes);
+    if (rc) return rc;
+    slim_bwd_kernel<T, P, ND, MODE, O><<<p.slim_grid, kSlimT, p.slim_bytes, q>>>(a, o);
+    return 0;
+}
+template <class T, int P, int MODE>
+int slim_fwd(const Plan& p, const SlimArgs& a, const SlimFwd& o, hipStream_t q) {
+    return p.slim == 2   ? slim_fwd_launch<T, P, 2, MODE>(p, a, o, q)
+           : p.slim == 4 ? slim_fwd_launch<T, P, 4, MODE>(p, a, o, q)
+                         : slim_fwd_launch<T, P, 8, MODE>(p, a, o, q);
+}
+template <class T, int P, int MODE, class O>
+int slim_bwd(const Plan& p, const SlimArgs& a, const SlimBwd& o, hipStream_t q) {
+    return p.slim == 2   ? slim_bwd_launch<T, P, 2, MODE, O>(p, a, o, q)
+           : p.slim == 4 ? slim_bwd_launch<T, P, 4, MODE, O>(p, a, o, q)
+                         : slim_bwd_launch<T, P, 8, MODE, O>(p, a, o, q);
+}
+
+template <class IT, int NR>
+void few_launch(const Plan& p, const IT* h, long long ldh, const IT* w, FewArgs a, hipStream_t q) {
+    constexpr int VEC = 16 / sizeof(IT);
+    const bool v = a.D % VEC == 0 && !misaligned(w);
+    a.L = lanes_for(v ? a.D / VEC : a.D);
+    const int bytes = NR * pad8(a.D) * 4;
+    if (v)
+        few_kernel<IT, VEC, NR><<<p.few_grid, kFewT, bytes, q>>>(h, ldh, w, a);
+    else
+        few_kernel<IT, 1, NR><<<p.few_grid, kFewT, bytes, q>>>(h, ldh, w, a);
 }
 
 template <class T, int SPLIT, int MODE>
@@ -828,22 +1458,69 @@ int head_fwd(int mode, const IT* hidden, long long ldh, const IT* weight, const 
         list_rows_kernel<<<nb, kListT, 0, q>>>(target, (int)N, V, ignore, counts, s.st, s.rows, s.tgt,
                                                reduction == DS_REDUCE_NONE ? out : nullptr);
         rows = s.rows;
-    } else {
-        head_init_kernel<<<1, 1, 0, q>>>(s.st, (int)N);
+    }
+    // expectation: all rows; the count is written by the first kernel that runs
+    const bool set_count = mode == kExpect && (p.few || (p.slim && !p.stage_h));
+    if (mode == kExpect && !set_count) head_init_kernel<<<1, 1, 0, q>>>(s.st, (int)N);
+    float* part = reinterpret_cast<float*>(ws + p.part);
+    float* tlogit = reinterpret_cast<float*>(ws + p.tlogit);
+    JoinArgs ja{};
+    ja.mode = mode;
+    ja.st = s.st;
+    ja.rows = s.rows;
+    ja.tgt = s.tgt;
+    ja.top = s.top;
+    ja.inv_sum = s.inv_sum;
+    ja.mean = s.mean;
+    ja.out = out;
+    ja.total = mode == kCE ? reduction : 0;
+    if (p.few) {
+        const FewArgs fa{rows, s.st, set_count, (int)N, D, V, 0, mode == kCE ? s.tgt : nullptr, centers, part};
+        p.few == 1   ? few_launch<IT, 1>(p, hidden, ldh, weight, fa, q)
+        : p.few == 2 ? few_launch<IT, 2>(p, hidden, ldh, weight, fa, q)
+        : p.few == 4 ? few_launch<IT, 4>(p, hidden, ldh, weight, fa, q)
+                     : few_launch<IT, 8>(p, hidden, ldh, weight, fa, q);
+        ja.mx = part;
+        ja.s = part + 1;
+        ja.sc = part + 2;
+        ja.tl = part + 3;
+        ja.step = ja.tl_step = p.few * 4;
+        ja.pitch = 4;
+        ja.entries = p.few_grid;
+        join_few_kernel<<<1, 1024, 0, q>>>(ja);
+        return launched();
     }
     Operand H, W;
     operands<IT, T, SPLIT>(p, hidden, ldh, weight, N, D, V, s, rows, true, ws + p.staged_h, ws + p.staged_w, H, W, q);
-    float* part = reinterpret_cast<float*>(ws + p.part);
-    float* tlogit = reinterpret_cast<float*>(ws + p.tlogit);
+    double* sums = mode == kCE && reduction != DS_REDUCE_NONE ? reinterpret_cast<double*>(ws + p.sums) : nullptr;
+    if (p.slim) {
+        SlimArgs a = slim_args(p, H, W, s, rows, N, D, V, centers);
+        a.set_count = set_count;
+        const SlimFwd o{sums ? nullptr : out, sums};
+        const int rc = mode == kCE ? slim_fwd<T, SPLIT == 3 ? 2 : 1, kCE>(p, a, o, q) : slim_fwd<T, SPLIT == 3 ? 2 : 1, kExpect>(p, a, o, q);
+        if (rc) return rc;
+        if (sums) loss_total_kernel<<<1, 256, 0, q>>>(sums, s.st, reduction == DS_REDUCE_MEAN, p.slim_grid, out);
+        return launched();
+    }
     const StatsArgs sa{V, s.tgt, centers, tlogit, part, (long long)(align256((size_t)p.vt_fwd * N * 4) / 4), (int)N};
     if (mode == kCE)
         stats_launch<T, SPLIT, kCE>(p, W, H, s, N, D, sa, q);
     else
         stats_launch<T, SPLIT, kExpect>(p, W, H, s, N, D, sa, q);
-    double* sums = mode == kCE && reduction != DS_REDUCE_NONE ? reinterpret_cast<double*>(ws + p.sums) : nullptr;
+    if (N <= 32) {
+        ja.mx = part;
+        ja.s = part + sa.plane;
+        ja.sc = part + 2 * sa.plane;
+        ja.tl = tlogit;
+        ja.step = N;
+        ja.pitch = 1;
+        ja.entries = p.vt_fwd;
+        join_few_kernel<<<1, 1024, 0, q>>>(ja);
+        return launched();
+    }
     head_join_kernel<<<cdiv(N, 32), 256, 0, q>>>(part, sa.plane, (int)N, p.vt_fwd, s.st, mode, s.rows, s.tgt, tlogit, s.top,
                                                  s.inv_sum, s.mean, out, sums);
-    if (sums) loss_total_kernel<<<1, 256, 0, q>>>(sums, s.st, reduction == DS_REDUCE_MEAN, out);
+    if (sums) loss_total_kernel<<<1, 256, 0, q>>>(sums, s.st, reduction == DS_REDUCE_MEAN, 0, out);
     return launched();
 }
 
@@ -891,13 +1568,25 @@ int head_bwd(int mode, const IT* hidden, long long ldh, const IT* weight, const 
     const int* rows = mode == kCE ? s.rows : nullptr;
     BackState* bs = reinterpret_cast<BackState*>(ws + p.bs);
     Upstream up{g, reduction == DS_REDUCE_NONE, reduction == DS_REDUCE_MEAN, rows};
-    back_init_kernel<<<1, 1, 0, q>>>(bs);
-    const long long most = (up.each && N > V) ? N : V;
-    back_scale_kernel<<<cdiv(most, 2048) < 256 ? cdiv(most, 2048) : 256, 256, 0, q>>>(up, s.st, centers, V, bs);
+    if (!std::is_same<T, bf16>::value && (up.each || mode == kExpect)) {    // where dl_norm reads it
+        back_init_kernel<<<1, 1, 0, q>>>(bs);
+        const long long most = up.each && N > V ? N : V;
+        back_scale_kernel<<<cdiv(most, 2048) < 256 ? cdiv(most, 2048) : 256, 256, 0, q>>>(up, s.st, centers, V, bs);
+    }
+    // the forward of few rows needs no scales and leaves none
+    const bool need_scales = SPLIT == 3 && p.few;
+    if (need_scales && mode == kExpect) head_init_kernel<<<1, 1, 0, q>>>(s.st, (int)N);
     Operand H, W;
-    operands<IT, T, SPLIT>(p, hidden, ldh, weight, N, D, V, s, rows, false, ws + p.bh, ws + p.bw, H, W, q);
-    if (mode == kCE && g_hidden)
-        zero_ignored_kernel<IT><<<cdiv(N, 4) < 8192 ? cdiv(N, 4) : 8192, 256, 0, q>>>(target, (int)N, ignore, D, s.st, g_hidden);
+    operands<IT, T, SPLIT>(p, hidden, ldh, weight, N, D, V, s, rows, need_scales, ws + p.bh, ws + p.bw, H, W, q);
+    if (mode == kCE && g_hidden) {
+        constexpr int VEC = 16 / sizeof(IT);
+        const bool v = D % VEC == 0;
+        const int L = lanes_for(v ? D / VEC : D), blocks = cdiv(N, 4 * 64 / L * 4), grid = blocks < 4096 ? blocks : 4096;
+        if (v)
+            zero_ignored_kernel<IT, VEC><<<grid, 256, 0, q>>>(target, (int)N, ignore, D, L, s.st, g_hidden);
+        else
+            zero_ignored_kernel<IT, 1><<<grid, 256, 0, q>>>(target, (int)N, ignore, D, L, s.st, g_hidden);
+    }
     T* dl = reinterpret_cast<T*>(ws + p.dl);
     float* dhp = reinterpret_cast<float*>(ws + p.dhp);
     float* dwp = reinterpret_cast<float*>(ws + p.dwp);
@@ -908,34 +1597,49 @@ int head_bwd(int mode, const IT* hidden, long long ldh, const IT* weight, const 
         Operand Wp = W;   // classes [v0, v0 + cols)
         Wp.p = static_cast<const T*>(W.p) + (long long)v0 * W.ld;
         Wp.outer = cols;
-        const DlArgs da{v0, cols, s.tgt, centers, s.top, s.inv_sum, s.mean, up, dl, ld, lo};
-        if (mode == kCE)
-            dl_launch<T, SPLIT, kCE>(p, Wp, H, s, bs, N, D, da, q);
-        else
-            dl_launch<T, SPLIT, kExpect>(p, Wp, H, s, bs, N, D, da, q);
+        if (p.slim_back) {
+            const SlimArgs a = slim_args(p, H, W, s, rows, N, D, V, centers);
+            const SlimBwd o{bs, up, g_hidden, g_weight ? dl : nullptr, ld, lo, g_weight && p.pack ? ws + p.bh : nullptr, p.Dp};
+            const int rc = mode == kCE ? slim_bwd<T, SPLIT == 3 ? 2 : 1, kCE, IT>(p, a, o, q)
+                                       : slim_bwd<T, SPLIT == 3 ? 2 : 1, kExpect, IT>(p, a, o, q);
+            if (rc) return rc;
+            if (p.pack) H = Operand{ws + p.bh, p.Dp, 0, (int)N, p.Dp};
+        } else {
+            const DlArgs da{v0, cols, s.tgt, centers, s.top, s.inv_sum, s.mean, up, dl, ld, lo};
+            if (mode == kCE)
+                dl_launch<T, SPLIT, kCE>(p, Wp, H, s, bs, N, D, da, q);
+            else
+                dl_launch<T, SPLIT, kExpect>(p, Wp, H, s, bs, N, D, da, q);
+        }
         const Operand G{dl, ld, lo, (int)N, ld};
-        if (g_hidden) {
-            const GradArgs ga{D, cols, p.dh_splits, mode, cols, v0 == 0, rows, g_hidden, dhp, N * D4};
+        if (g_hidden && !p.slim_back) {
+            const GradArgs ga{D, cols, p.dh_splits, mode, cols, v0 == 0, rows, g_hidden, dhp, N * D4, up};
             grad_launch<IT, T, SPLIT, 0>(p.dh, p.dh_part, Wp, G, s, bs, N, ga, q);
         }
         if (g_weight) {
             IT* gw = g_weight + (long long)v0 * D;
-            const GradArgs ga{D, cols, p.dw_splits, mode, cols, 1, nullptr, gw, dwp, (long long)p.piece * D4};
+            const GradArgs ga{D, cols, p.dw_splits, mode, cols, 1, nullptr, gw, dwp, (long long)p.piece * D4, up};
             grad_launch<IT, T, SPLIT, 1>(p.dw, p.dw_splits > 1, H, G, s, bs, cols, ga, q);
-            if (p.dw_splits > 1)
-                head_sum_kernel<T, SPLIT, IT><<<cdiv((long long)cols * D4 / 4, 256), 256, 0, q>>>(
-                    dwp, (long long)p.piece * D4, p.dw_splits, s.st, bs, cols, D, mode, 1, nullptr, gw);
+            if (p.dw_splits > 8)
+                head_sum_kernel<T, SPLIT, IT, 16><<<cdiv((long long)cols * D4 / 4, 16), 256, 0, q>>>(
+                    dwp, (long long)p.piece * D4, p.dw_splits, s.st, bs, cols, D, mode, 1, up, nullptr, gw);
+            else if (p.dw_splits > 1)
+                head_sum_kernel<T, SPLIT, IT, 1><<<cdiv((long long)cols * D4 / 4, 256), 256, 0, q>>>(
+                    dwp, (long long)p.piece * D4, p.dw_splits, s.st, bs, cols, D, mode, 1, up, nullptr, gw);
         }
     }
-    if (g_hidden && p.dh_part) {
-        const int blocks = cdiv(N * (D4 / 4), 256);
-        head_sum_kernel<T, SPLIT, IT><<<blocks < 16384 ? blocks : 16384, 256, 0, q>>>(dhp, N * D4, p.dh_splits, s.st, bs, (int)N, D,
-                                                                                      mode, 0, rows, g_hidden);
+    if (g_hidden && p.dh_part && !p.slim_back) {
+        const bool many = p.dh_splits > 8;
+        const int blocks = cdiv(N * (D4 / 4), many ? 16 : 256), grid = blocks < 16384 ? blocks : 16384;
+        if (many)
+            head_sum_kernel<T, SPLIT, IT, 16><<<grid, 256, 0, q>>>(dhp, N * D4, p.dh_splits, s.st, bs, (int)N, D, mode, 0, up, rows,
+                                                                   g_hidden);
+        else
+            head_sum_kernel<T, SPLIT, IT, 1><<<grid, 256, 0, q>>>(dhp, N * D4, p.dh_splits, s.st, bs, (int)N, D, mode, 0, up, rows,
+                                                                  g_hidden);
     }
     return launched();
 }
-
-bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
 template <class F32, class F16, class BF16>
 int by_type(int dtype, F32 f32, F16 h, BF16 b) {
