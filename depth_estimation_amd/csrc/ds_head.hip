@@ -65,10 +65,14 @@ __global__ __launch_bounds__(kListT) void count_rows_kernel(const long long* __r
                                                             int* __restrict__ counts) {
     __shared__ int s[kListT / 64];
     int c = 0;
+    long long t[kListPer];
+#pragma unroll
     for (int i = 0; i < kListPer; ++i) {
         const long long r = (long long)blockIdx.x * kListBlock + i * kListT + threadIdx.x;
-        c += __popcll(__ballot(r < n && target[r < n ? r : 0] != ignore));
+        t[i] = r < n ? target[r] : ignore;
     }
+#pragma unroll
+    for (int i = 0; i < kListPer; ++i) c += __popcll(__ballot(t[i] != ignore));
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = c;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -148,8 +152,7 @@ __global__ __launch_bounds__(kListT) void list_rows_kernel(const long long* __re
 static_assert(kListPer * kListT / 64 == 256, "the prefix handles four counts a lane");
 
 // --------------------------------------------------------------------------------------------------- staged operands
-// Row-wise passes over a matrix: a wave takes 64 / L rows at once, L lanes a row, VEC elements (16 bytes) a lane where rows are
-// aligned, one where not; L is the power of two that a row of D elements needs, at most 64.
+// Row-wise passes over a matrix: a wave takes 64 / L rows at once, L lanes a row, VEC elements (16 bytes) a lane; L is the power of two that a row of D elements needs, at most 64.
 inline int lanes_for(int vectors) {
     int l = 1;
     while (l < vectors && l < 64) l <<= 1;
@@ -159,18 +162,18 @@ template <class IT, int VEC>
 struct Vec {
     typedef IT type __attribute__((ext_vector_type(VEC)));
 };
-template <class IT>
-struct Vec<IT, 1> {
-    typedef IT type;
-};
+// VEC elements of a row from element d on, zero behind its last; rows need only their type's alignment (gfx950 loads 16 bytes
+// from any address)
 template <class IT, int VEC>
-__device__ __forceinline__ void load_vec(const IT* p, IT (&x)[VEC]) {
-    if constexpr (VEC == 1) {
-        x[0] = *p;
-    } else {
-        const typename Vec<IT, VEC>::type v = *reinterpret_cast<const typename Vec<IT, VEC>::type*>(p);
+__device__ __forceinline__ void load_vec(const IT* row, int d, int D, IT (&x)[VEC]) {
+    typedef typename Vec<IT, VEC>::type loose __attribute__((aligned(sizeof(IT))));
+    if (d + VEC <= D) {
+        const loose v = *reinterpret_cast<const loose*>(row + d);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) x[e] = v[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[e] = d + e < D ? row[d + e] : (IT)0.f;
     }
 }
 
@@ -194,7 +197,7 @@ __global__ __launch_bounds__(256) void amax_kernel(const IT* __restrict__ x, lon
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int r = min(r0 + u * nb * 4 * R, c - 1);
-                load_vec<IT, VEC>(src + (rows && !second ? rows[r] : r) * pitch + d, v[u]);
+                load_vec<IT, VEC>(src + (rows && !second ? rows[r] : r) * pitch, d, D, v[u]);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -202,7 +205,14 @@ __global__ __launch_bounds__(256) void amax_kernel(const IT* __restrict__ x, lon
                 for (int e = 0; e < VEC; ++e) m = fmaxf(m, finite_abs((float)v[u][e]));
         }
     m = wave_max(m);
-    if (lane == 0 && m > 0.f) atomicMax(second ? &st->amax_w : &st->amax_h, __builtin_bit_cast(unsigned, m));
+    __shared__ float s[4];
+    if (lane == 0) s[threadIdx.x >> 6] = m;
+    __syncthreads();
+    // one atomic a workgroup: they all meet in one place, 20 ns each
+    if (threadIdx.x == 0) {
+        m = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+        if (m > 0.f) atomicMax(second ? &st->amax_w : &st->amax_h, __builtin_bit_cast(unsigned, m));
+    }
 }
 
 // rows of x (listed in `rows` if given) packed with a row pitch of Dp elements, zero behind D; fp32 as two scaled fp16 planes
@@ -221,9 +231,7 @@ __global__ __launch_bounds__(256) void stage_kernel(const IT* __restrict__ x, lo
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int r = min(r0 + u * hop, c - 1);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) v[u][e] = (IT)0.f;
-                if (d < D) load_vec<IT, VEC>(x + (rows ? rows[r] : r) * ld + d, v[u]);
+                load_vec<IT, VEC>(x + (rows ? rows[r] : r) * ld, d, D, v[u]);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -231,23 +239,15 @@ __global__ __launch_bounds__(256) void stage_kernel(const IT* __restrict__ x, lo
                 if (r >= c) break;
                 T* q = y + (long long)r * Dp + d;
                 typename Vec<T, VEC>::type h, l;
-                if constexpr (VEC == 1) {
-                    if constexpr (SPLIT == 3) {
-                        split16((float)v[u][0] * scale, h, l);
-                    } else {
-                        h = v[u][0];
-                    }
-                } else {
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        if constexpr (SPLIT == 3) {
-                            f16 a, b;
-                            split16((float)v[u][e] * scale, a, b);
-                            h[e] = a;
-                            l[e] = b;
-                        } else {
-                            h[e] = v[u][e];
-                        }
+                for (int e = 0; e < VEC; ++e) {
+                    if constexpr (SPLIT == 3) {
+                        f16 a, b;
+                        split16((float)v[u][e] * scale, a, b);
+                        h[e] = a;
+                        l[e] = b;
+                    } else {
+                        h[e] = v[u][e];
                     }
                 }
                 *reinterpret_cast<typename Vec<T, VEC>::type*>(q) = h;
@@ -768,14 +768,15 @@ __global__ __launch_bounds__(256) void zero_ignored_kernel(const long long* __re
         for (int u = 0; u < U; ++u)
             if (r0 + u * hop < n && t[u] == ignore)
                 for (int d = sub * VEC; d < D; d += L * VEC) {
-                    typename Vec<O, VEC>::type z;
+                    O* q = out + (long long)(r0 + u * hop) * D + d;
                     if constexpr (VEC == 1) {
-                        z = (O)0.f;
+                        *q = (O)0.f;
                     } else {
+                        typename Vec<O, VEC>::type z;
 #pragma unroll
                         for (int e = 0; e < VEC; ++e) z[e] = (O)0.f;
+                        *reinterpret_cast<typename Vec<O, VEC>::type*>(q) = z;
                     }
-                    *reinterpret_cast<typename Vec<O, VEC>::type*>(out + (long long)(r0 + u * hop) * D + d) = z;
                 }
     }
 }
@@ -821,16 +822,27 @@ struct SlimBwd {
 // W to LDS: per plane, blocks of 64 columns, each [Vp][64] in lds_chunk's order
 template <int P, int ND>
 __device__ __forceinline__ void slim_load_w(const SlimArgs& a, char* lds) {
-    constexpr int kChunks = ND * 4;
-    for (int i = threadIdx.x; i < a.Vp * kChunks; i += kSlimT) {
-        const int v = i / kChunks, c = i % kChunks;
-        const bool in = v < a.V && c * 8 < a.W.inner;
-        const char* src = static_cast<const char*>(a.W.p) + 2 * ((long long)v * a.W.ld + c * 8);
+    constexpr int kChunks = ND * 4, U = 4;       // chunks of a row; loads under way at a time
+    for (int i0 = threadIdx.x; i0 < a.Vp * kChunks; i0 += U * kSlimT) {
+        i32x4 x[U][P];
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            i32x4 x = {0, 0, 0, 0};
-            if (in) x = *reinterpret_cast<const i32x4*>(src + 2 * p * a.W.lo);
-            *reinterpret_cast<i32x4*>(lds + p * a.Vp * ND * 64 + (c >> 3) * a.Vp * 128 + lds_chunk<kK, 16>(v, c & 7)) = x;
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * kSlimT, v = i / kChunks, c = i % kChunks;
+            const bool in = v < a.V && c * 8 < a.W.inner;
+            const char* src = static_cast<const char*>(a.W.p) + 2 * ((long long)v * a.W.ld + c * 8);
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                x[u][p] = i32x4{0, 0, 0, 0};
+                if (in) x[u][p] = *reinterpret_cast<const i32x4*>(src + 2 * p * a.W.lo);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * kSlimT, v = i / kChunks, c = i % kChunks;
+            if (v >= a.Vp) break;
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+                *reinterpret_cast<i32x4*>(lds + p * a.Vp * ND * 64 + (c >> 3) * a.Vp * 128 + lds_chunk<kK, 16>(v, c & 7)) = x[u][p];
         }
     }
     __syncthreads();
@@ -1111,7 +1123,7 @@ __global__ __launch_bounds__(kFewT) void few_kernel(const IT* __restrict__ h, lo
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int v = min(v0 + u * groups, a.V - 1);
-                load_vec<IT, VEC>(w + (long long)v * a.D + d, x[u]);
+                load_vec<IT, VEC>(w + (long long)v * a.D, d, a.D, x[u]);
             }
 #pragma unroll
             for (int e = 0; e < VEC; ++e)
@@ -1276,7 +1288,7 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     // few rows: their features have to fit LDS in fp32 beside three more workgroups
     p.few = N > kFewMax ? 0 : N <= 1 ? 1 : N <= 2 ? 2 : N <= 4 ? 4 : 8;
     if (p.few && (size_t)p.few * pad8(D) * 4 > 40 * 1024) p.few = 0;
-    const int vec = dtype == DS_F32 ? 4 : 8, lanes = lanes_for(cdiv(D, D % vec == 0 ? vec : 1));
+    const int vec = dtype == DS_F32 ? 4 : 8, lanes = lanes_for(cdiv(D, vec));
     p.few_grid = cdiv(V, kFewT / lanes * 4) < 2 * cu_count() ? cdiv(V, kFewT / lanes * 4) : 2 * cu_count();
     // small head: the weight in LDS, two workgroups a CU
     const int Vp = (V + 31) & ~31;
@@ -1343,25 +1355,17 @@ template <class IT, class T, int SPLIT>
 void stage(const IT* x, long long ld, const int* rows, const int* cnt, long long n, int D, int Dp, const unsigned* amax, T* y,
            long long lo, hipStream_t q) {
     constexpr int VEC = 16 / sizeof(IT);
-    const bool v = D % VEC == 0 && ld % VEC == 0 && !misaligned(x);
-    const int L = lanes_for(v ? Dp / VEC : Dp), blocks = cdiv(n, 4 * 64 / L * 2), grid = blocks < 4096 ? blocks : 4096;
-    if (v)
-        stage_kernel<IT, T, SPLIT, VEC><<<grid, 256, 0, q>>>(x, ld, rows, cnt, (int)n, D, Dp, L, amax, y, lo);
-    else
-        stage_kernel<IT, T, SPLIT, 1><<<grid, 256, 0, q>>>(x, ld, rows, cnt, (int)n, D, Dp, L, amax, y, lo);
+    const int L = lanes_for(cdiv(Dp, VEC)), blocks = cdiv(n, 4 * 64 / L * 2), grid = blocks < 4096 ? blocks : 4096;
+    stage_kernel<IT, T, SPLIT, VEC><<<grid, 256, 0, q>>>(x, ld, rows, cnt, (int)n, D, Dp, L, amax, y, lo);
 }
 // scales of fp32 inputs (st->amax_h, amax_w; zeroed before)
 template <class IT>
 void scales(const IT* hidden, long long ldh, const int* rows, const IT* weight, long long N, int D, int V, HeadState* st,
             hipStream_t q) {
     constexpr int VEC = 16 / sizeof(IT);
-    const bool v = D % VEC == 0 && ldh % VEC == 0 && !misaligned(hidden) && !misaligned(weight);
-    const int L = lanes_for(v ? D / VEC : D), per = 4 * 64 / L * 4;
-    const int bx = cdiv(N, per) < 1024 ? cdiv(N, per) : 1024, bw = cdiv(V, per) < 1024 ? cdiv(V, per) : 1024;
-    if (v)
-        amax_kernel<IT, VEC><<<bx + bw, 256, 0, q>>>(hidden, ldh, rows, st, weight, V, D, L, bx);
-    else
-        amax_kernel<IT, 1><<<bx + bw, 256, 0, q>>>(hidden, ldh, rows, st, weight, V, D, L, bx);
+    const int L = lanes_for(cdiv(D, VEC)), per = 4 * 64 / L * 4;
+    const int bx = cdiv(N, per) < 512 ? cdiv(N, per) : 512, bw = cdiv(V, per) < 512 ? cdiv(V, per) : 512;
+    amax_kernel<IT, VEC><<<bx + bw, 256, 0, q>>>(hidden, ldh, rows, st, weight, V, D, L, bx);
 }
 // inputs as matrix operands: in place, or staged into `ws`
 template <class IT, class T, int SPLIT>
@@ -1424,13 +1428,8 @@ int slim_bwd(const Plan& p, const SlimArgs& a, const SlimBwd& o, hipStream_t q) 
 template <class IT, int NR>
 void few_launch(const Plan& p, const IT* h, long long ldh, const IT* w, FewArgs a, hipStream_t q) {
     constexpr int VEC = 16 / sizeof(IT);
-    const bool v = a.D % VEC == 0 && !misaligned(w);
-    a.L = lanes_for(v ? a.D / VEC : a.D);
-    const int bytes = NR * pad8(a.D) * 4;
-    if (v)
-        few_kernel<IT, VEC, NR><<<p.few_grid, kFewT, bytes, q>>>(h, ldh, w, a);
-    else
-        few_kernel<IT, 1, NR><<<p.few_grid, kFewT, bytes, q>>>(h, ldh, w, a);
+    a.L = lanes_for(cdiv(a.D, VEC));
+    few_kernel<IT, VEC, NR><<<p.few_grid, kFewT, NR * pad8(a.D) * 4, q>>>(h, ldh, w, a);
 }
 
 template <class T, int SPLIT, int MODE>
