@@ -7,8 +7,8 @@
 // its m (measured layout: lane 4r+c of a 16-lane group reads four values of row r, lane i receives rows 0..3 of column i).
 //
 // Numbers wider than 16 bits go through as two fp16 planes x = hi + lo (22 bits, after an exact power-of-two scale that the
-// caller keeps): SPLIT = 3 adds lo*hi + hi*lo + hi*hi into the same fp32 accumulators.  What is dropped, lo*lo, is 2^-22 of
-// the product.  Three 16-bit products cost a third of the 16-bit rate, still above the rate of fp32 matrix instructions
+// caller keeps): lo*hi + hi*lo + hi*hi go into the same fp32 accumulators.  What is dropped, lo*lo, is 2^-22 of the product.
+// PA and PB say how many planes A and B have.  Three 16-bit products cost a third of the 16-bit rate, still above the rate of fp32 matrix instructions
 // (1/16 of it).
 //
 // Rows and columns beyond an operand's bounds read as zero (buffer loads whose offset is out of range), so every size works
@@ -42,7 +42,7 @@ enum Lay { kK = 0, kM = 1 };   // which index of the operand is contiguous
 struct Operand {
     const void* p;      // 16-bit elements, 16-byte aligned
     long long ld;       // elements between stored rows, a multiple of 8
-    long long lo;       // elements from the hi plane to the lo plane (SPLIT = 3)
+    long long lo;       // elements from the hi plane to the lo plane (two planes)
     int outer;          // stored rows that exist
     int inner;          // elements of a row that may be read, a multiple of 8 (what lies beyond the matrix must be zero)
 };
@@ -128,44 +128,42 @@ struct Fragments {
 };
 
 // acc[i][j][e]: C at m = m0 + wave's row + 16 i + 4 (lane / 16) + e, n = n0 + wave's column + 16 j + lane % 16, over k in
-// [kbeg, kend) (kbeg a multiple of 64).  `lds`: lds_bytes<S, SPLIT>() bytes.  Ends behind a barrier: the caller may reuse
-// `lds`.  SPLIT = 3: a step brings both planes of both operands and adds its three products from them, so that each plane is
-// moved once and a step's latency is covered by three products.  128 x 128 tiles then keep one step in LDS (the next one
+// [kbeg, kend) (kbeg a multiple of 64).  `lds`: lds_bytes<S, PA, PB>() bytes.  Ends behind a barrier: the caller may reuse
+// `lds`.  A step brings all planes of both operands and adds its products from them, so that each plane is moved once and a
+// step's latency is covered by up to three products.  128 x 128 tiles then keep one step in LDS (the next one
 // waits in registers), which leaves room for two workgroups a CU.
-template <class S, int SPLIT>
-constexpr int lds_buffers() { return SPLIT == 3 && S::BM * S::BN > 64 * 128 ? 1 : 2; }
-template <class S, int SPLIT>
-constexpr int lds_bytes() { return lds_buffers<S, SPLIT>() * (SPLIT == 3 ? 2 : 1) * (S::BM + S::BN) * kBK * 2; }
+template <class S, int PA, int PB>
+constexpr int lds_buffers() { return PA + PB > 2 && S::BM * S::BN > 64 * 128 ? 1 : 2; }
+template <class S, int PA, int PB>
+constexpr int lds_bytes() { return lds_buffers<S, PA, PB>() * (PA * S::BM + PB * S::BN) * kBK * 2; }
 
-template <class T, class S, Lay LA, Lay LB, int SPLIT>
+template <class T, class S, Lay LA, Lay LB, int PA, int PB>
 __device__ __forceinline__ void gemm_tile(const Operand& A, const Operand& B, int m0, int n0, int kbeg, int kend, char* lds,
                                           f32x4 (&acc)[S::FM][S::FN]) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = (wave / S::WN) * S::FM * 16, wn = (wave % S::WN) * S::FN * 16;
-    constexpr int P = SPLIT == 3 ? 2 : 1, kA = S::BM * kBK * 2, kB = S::BN * kBK * 2, kBuf = P * (kA + kB);
-    constexpr int NB = lds_buffers<S, SPLIT>();
+    constexpr int kA = S::BM * kBK * 2, kB = S::BN * kBK * 2, kBuf = PA * kA + PB * kB;
+    constexpr int NB = lds_buffers<S, PA, PB>();
 #pragma unroll
     for (int i = 0; i < S::FM; ++i)
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     const Fragments<LA, S::BM> fa(wm, lane);
     const Fragments<LB, S::BN> fb(wn, lane);
-    Stager<LA, S::BM, S::T> sa[P];
-    Stager<LB, S::BN, S::T> sb[P];
+    Stager<LA, S::BM, S::T> sa[PA];
+    Stager<LB, S::BN, S::T> sb[PB];
     const int steps = (kend - kbeg + kBK - 1) / kBK;
     auto load = [&](int s) {
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            sa[p].load(A, m0, kbeg + s * kBK, p == 1, tid);
-            sb[p].load(B, n0, kbeg + s * kBK, p == 1, tid);
-        }
-    };
-    auto store = [&](char* buf) {   // hi A, hi B, lo A, lo B
+        for (int p = 0; p < PA; ++p) sa[p].load(A, m0, kbeg + s * kBK, p == 1, tid);
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            sa[p].store(buf + p * (kA + kB), tid);
-            sb[p].store(buf + p * (kA + kB) + kA, tid);
-        }
+        for (int p = 0; p < PB; ++p) sb[p].load(B, n0, kbeg + s * kBK, p == 1, tid);
+    };
+    auto store = [&](char* buf) {
+#pragma unroll
+        for (int p = 0; p < PA; ++p) sa[p].store(buf + p * kA, tid);
+#pragma unroll
+        for (int p = 0; p < PB; ++p) sb[p].store(buf + PA * kA + p * kB, tid);
     };
     if (steps > 0) {
         load(0);
@@ -178,30 +176,23 @@ __device__ __forceinline__ void gemm_tile(const Operand& A, const Operand& B, in
         if (more) load(s + 1);
 #pragma unroll
         for (int kk = 0; kk < kBK / 32; ++kk) {
-            s16x8 a[S::FM], b[S::FN];
+            s16x8 a[PA][S::FM], b[PB][S::FN];
 #pragma unroll
-            for (int i = 0; i < S::FM; ++i) a[i] = fa.get(buf, i, kk);
+            for (int p = 0; p < PA; ++p)
 #pragma unroll
-            for (int j = 0; j < S::FN; ++j) b[j] = fb.get(buf + kA, j, kk);
-            if (SPLIT == 3) {
-                s16x8 c[S::FM], d[S::FN];
+                for (int i = 0; i < S::FM; ++i) a[p][i] = fa.get(buf + p * kA, i, kk);
 #pragma unroll
-                for (int i = 0; i < S::FM; ++i) c[i] = fa.get(buf + kA + kB, i, kk);
+            for (int p = 0; p < PB; ++p)
 #pragma unroll
-                for (int j = 0; j < S::FN; ++j) d[j] = fb.get(buf + kA + kB + kA, j, kk);
+                for (int j = 0; j < S::FN; ++j) b[p][j] = fb.get(buf + PA * kA + p * kB, j, kk);
 #pragma unroll
-                for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-                    for (int j = 0; j < S::FN; ++j) acc[i][j] = mfma(c[i], b[j], acc[i][j], T());
+            for (int pair = PA + PB - 2; pair >= 0; --pair) {      // (lo, hi) and (hi, lo), as far as there are any, then (hi, hi)
+                const int p = pair > 0 && PA == 2 && pair == PA + PB - 2 ? 1 : 0, q = pair > 0 && !p ? 1 : 0;
 #pragma unroll
                 for (int i = 0; i < S::FM; ++i)
 #pragma unroll
-                    for (int j = 0; j < S::FN; ++j) acc[i][j] = mfma(a[i], d[j], acc[i][j], T());
+                    for (int j = 0; j < S::FN; ++j) acc[i][j] = mfma(a[PA == 2 ? p : 0][i], b[PB == 2 ? q : 0][j], acc[i][j], T());
             }
-#pragma unroll
-            for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-                for (int j = 0; j < S::FN; ++j) acc[i][j] = mfma(a[i], b[j], acc[i][j], T());
         }
         if (NB == 1) __syncthreads();
         if (more) store(lds + (NB == 2 ? ((s + 1) & 1) * kBuf : 0));
@@ -295,9 +286,11 @@ struct Job {
     int m0, n0, kbeg, kend;
 };
 
-template <class T, Lay LA, Lay LB, int SPLIT>
+// Planes are taken one pair after the other, a step of the same k each.
+template <class T, Lay LA, Lay LB, int PA, int PB>
 struct TileStream {
     using S = Big;
+    static constexpr int kPairs = PA + PB - 1;     // (lo, hi) and (hi, lo), as far as there are any, and (hi, hi)
     Mover<LA, S::BM, S::T> ma;
     Mover<LB, S::BN, S::T> mb;
     Job job;
@@ -305,16 +298,16 @@ struct TileStream {
     char* lds;       // S::kLds bytes that nothing else uses
 
     __device__ __forceinline__ void move(int s) {
-        const int k0 = job.kbeg + s / SPLIT * kBK, ph = s % SPLIT;
+        const int k0 = job.kbeg + s / kPairs * kBK, ph = s % kPairs;
         const unsigned buf = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds +
                              ((s + parity) & 1) * ((S::BM + S::BN) * kBK * 2);
-        ma.move(job.A, job.m0, k0, SPLIT == 3 && ph == 0, buf, tid);
-        mb.move(job.B, job.n0, k0, SPLIT == 3 && ph == 1, buf + S::BM * kBK * 2, tid);
+        ma.move(job.A, job.m0, k0, PA == 2 && ph == 0, buf, tid);
+        mb.move(job.B, job.n0, k0, PB == 2 && ph == PA - 1, buf + S::BM * kBK * 2, tid);
     }
     // takes up a job and sets its first step under way
     __device__ __forceinline__ void start(const Job& j) {
         job = j;
-        const int n = (j.kend - j.kbeg + kBK - 1) / kBK * SPLIT;
+        const int n = (j.kend - j.kbeg + kBK - 1) / kBK * kPairs;
         steps = n > 0 ? n : 1;
         ma.init(j.A, j.m0, tid);
         mb.init(j.B, j.n0, tid);
@@ -464,24 +457,25 @@ struct Cut {
     ShapeId shape;
     int splits;
 };
-// tiles(b): tiles of b x b; area: outputs; planes 2: three products a step.
+// tiles(b): tiles of b x b; area: outputs; pairs: products a step (three of two planes each, two of two planes and one).
 template <class Tiles>
-inline Cut cut_of(Tiles tiles, double area, long long K, int planes, bool may_split, bool small_too, int cus) {
+inline Cut cut_of(Tiles tiles, double area, long long K, int pairs, bool may_split, bool small_too, int cus) {
     // us a step of 64 k: `step` of a CU's time with `at_once` workgroups on it, `alone` at least; `ends`: start and end of a
     // tile.  Measured at k = 512 and 2048 with half a workgroup to sixteen a CU; in TFLOP/s of 16-bit products with the chip
-    // full: 256 x 256 tiles 1330, 128 x 128 870, 64 x 64 660; with two planes 1365, 1160, 780.
+    // full: 256 x 256 tiles 1330, 128 x 128 870, 64 x 64 660; three products a step 1365, 1160, 780 (two: between).
     struct Cost {
         ShapeId id;
         int b, at_once;
         double step, alone, ends;
     };
     static const Cost one[3] = {{kBig, 256, 1, 1.5, 1.35, 4.5}, {kSq, 128, 2, 0.60, 0.78, 3.0}, {kSmall, 64, 4, 0.21, 0.57, 2.0}};
-    static const Cost two[3] = {{kBig, 256, 1, 4.5, 4.1, 5.0}, {kSq, 128, 2, 1.40, 1.85, 3.0}, {kSmall, 64, 2, 0.53, 0.68, 2.5}};
+    static const Cost two[3] = {{kBig, 256, 1, 3.0, 2.7, 5.0}, {kSq, 128, 2, 1.00, 1.30, 3.0}, {kSmall, 64, 3, 0.37, 0.62, 2.5}};
+    static const Cost three[3] = {{kBig, 256, 1, 4.5, 4.1, 5.0}, {kSq, 128, 2, 1.40, 1.85, 3.0}, {kSmall, 64, 2, 0.53, 0.68, 2.5}};
     const long long steps = (K + kBK - 1) / kBK, most = may_split ? (steps < 256 ? steps : 256) : 1;
     Cut best{kSq, 1};
     double least = 1e300;
     for (int c = 0; c < (small_too ? 3 : 2); ++c) {
-        const Cost& q = planes == 2 ? two[c] : one[c];
+        const Cost& q = pairs == 1 ? one[c] : pairs == 2 ? two[c] : three[c];
         const long long t = tiles(q.b);
         for (long long s = 1; s <= most; s += s < 16 ? 1 : s / 8) {
             const double per = (double)((steps + s - 1) / s);

@@ -22,6 +22,10 @@
 namespace ds {
 namespace {
 
+// planes of an operand; SPLIT: products a step, 1 (16-bit inputs) or 3 (fp32)
+template <int SPLIT>
+constexpr int kP = SPLIT == 3 ? 2 : 1;
+
 enum Mode { kCE = 0, kExpect = 1 };
 
 // What the forward leaves for the backward besides the softmax statistics: opaque to the caller.
@@ -356,14 +360,14 @@ __device__ __forceinline__ void stats_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0
 template <class T, class S, int SPLIT, int MODE>
 __global__ __launch_bounds__(S::T) void head_stats_kernel(Operand W, Operand H, const HeadState* __restrict__ st, int D,
                                                           StatsArgs a) {
-    __shared__ __align__(16) char lds[lds_bytes<S, SPLIT>()];
+    __shared__ __align__(16) char lds[lds_bytes<S, kP<SPLIT>, kP<SPLIT>>()];
     const int vt = cdiv(a.V, S::BM);
     const int m0 = (int)(blockIdx.x % vt) * S::BM, n0 = (int)(blockIdx.x / vt) * S::BN;
     const int cnt = st->count;
     if (n0 >= cnt) return;
     H.outer = cnt;
     f32x4 acc[S::FM][S::FN];
-    gemm_tile<T, S, kK, kK, SPLIT>(W, H, m0, n0, 0, D, lds, acc);
+    gemm_tile<T, S, kK, kK, kP<SPLIT>, kP<SPLIT>>(W, H, m0, n0, 0, D, lds, acc);
     stats_of_tile<S, SPLIT, MODE>(acc, m0, n0, cnt, st, a, reinterpret_cast<float*>(lds));
 }
 
@@ -382,7 +386,7 @@ __global__ __launch_bounds__(Big::T) void head_stats_big_kernel(Operand W, Opera
         tile_of(u, tiles, mt, nt, m, n);
         return Job{W, H, m * Big::BM, n * Big::BN, 0, D};
     };
-    TileStream<T, kK, kK, SPLIT> stream(lds, job(t));
+    TileStream<T, kK, kK, kP<SPLIT>, kP<SPLIT>> stream(lds, job(t));
     for (; t < tiles; t += gridDim.x) {
         const int m0 = stream.job.m0, n0 = stream.job.n0;
         f32x4 acc[Big::FM][Big::FN];
@@ -587,14 +591,14 @@ __device__ __forceinline__ void dl_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, i
 template <class T, class S, int SPLIT, int MODE>
 __global__ __launch_bounds__(S::T) void head_dl_kernel(Operand W, Operand H, const HeadState* __restrict__ st,
                                                        const BackState* __restrict__ bs, int D, DlArgs a) {
-    __shared__ __align__(16) char lds[lds_bytes<S, SPLIT>()];
+    __shared__ __align__(16) char lds[lds_bytes<S, kP<SPLIT>, kP<SPLIT>>()];
     const int vt = cdiv(a.cols, S::BM);
     const int m0 = (int)(blockIdx.x % vt) * S::BM, n0 = (int)(blockIdx.x / vt) * S::BN;
     const int cnt = st->count;
     if (n0 >= cnt) return;
     H.outer = cnt;
     f32x4 acc[S::FM][S::FN];
-    gemm_tile<T, S, kK, kK, SPLIT>(W, H, m0, n0, 0, D, lds, acc);
+    gemm_tile<T, S, kK, kK, kP<SPLIT>, kP<SPLIT>>(W, H, m0, n0, 0, D, lds, acc);
     dl_of_tile<T, S, SPLIT, MODE>(acc, m0, n0, cnt, st, bs, a);
 }
 template <class T, int SPLIT, int MODE>
@@ -610,7 +614,7 @@ __global__ __launch_bounds__(Big::T) void head_dl_big_kernel(Operand W, Operand 
         tile_of(u, tiles, mt, nt, m, n);
         return Job{W, H, m * Big::BM, n * Big::BN, 0, D};
     };
-    TileStream<T, kK, kK, SPLIT> stream(lds, job(t));
+    TileStream<T, kK, kK, kP<SPLIT>, kP<SPLIT>> stream(lds, job(t));
     for (; t < tiles; t += gridDim.x) {
         const int m0 = stream.job.m0, n0 = stream.job.n0;
         f32x4 acc[Big::FM][Big::FN];
@@ -671,7 +675,7 @@ __device__ __forceinline__ void grad_of_tile(const f32x4 (&acc)[S::FM][S::FN], i
 template <class T, class S, int SPLIT, class O, bool ACC, int WHICH>
 __global__ __launch_bounds__(S::T) void head_grad_kernel(Operand A, Operand B, const HeadState* __restrict__ st,
                                                          const BackState* __restrict__ bs, GradArgs a) {
-    __shared__ __align__(16) char lds[std::is_same<S, Big>::value ? Big::kLds : lds_bytes<S, SPLIT>()];
+    __shared__ __align__(16) char lds[std::is_same<S, Big>::value ? Big::kLds : lds_bytes<S, kP<SPLIT>, kP<SPLIT>>()];
     const int cnt = st->count, mt = cdiv(a.D, S::BM), bound = WHICH == 0 ? cnt : a.cols;
     const int k = WHICH == 0 ? a.k : cnt, per = cdiv(cdiv(k, kBK), a.splits) * kBK;
     B.outer = cnt;
@@ -689,7 +693,7 @@ __global__ __launch_bounds__(S::T) void head_grad_kernel(Operand A, Operand B, c
             return Job{A, B, x / a.splits * S::BM, n * S::BN, k0, min(k0 + per, k)};
         };
         int sp, next_sp = 0;
-        TileStream<T, kM, LB, SPLIT> stream(lds, job(t, sp));
+        TileStream<T, kM, LB, kP<SPLIT>, kP<SPLIT>> stream(lds, job(t, sp));
         for (; t < units; t += gridDim.x) {
             const int m0 = stream.job.m0, n0 = stream.job.n0;
             f32x4 acc[S::FM][S::FN];
@@ -707,7 +711,7 @@ __global__ __launch_bounds__(S::T) void head_grad_kernel(Operand A, Operand B, c
         if (n0 >= bound) return;
         const int k0 = min(sp * per, k);
         f32x4 acc[S::FM][S::FN];
-        gemm_tile<T, S, kM, LB, SPLIT>(A, B, m0, n0, k0, min(k0 + per, k), lds, acc);
+        gemm_tile<T, S, kM, LB, kP<SPLIT>, kP<SPLIT>>(A, B, m0, n0, k0, min(k0 + per, k), lds, acc);
         grad_of_tile<T, S, SPLIT, O, ACC, WHICH>(acc, m0, n0, sp, bound, st, bs, a);
     }
 }
@@ -1230,7 +1234,7 @@ __global__ __launch_bounds__(1024) void join_few_kernel(JoinArgs a) {
 typedef Shape<64, 128, 1, 4> Flat;    // 64 along m
 typedef Shape<128, 32, 4, 1> Thin;    // 32 along n
 Cut cut_of(long long M, long long N, long long K, int planes, bool may_split) {
-    return ds::cut_of([&](long long b) { return ((M + b - 1) / b) * ((N + b - 1) / b); }, (double)M * N, K, planes, may_split,
+    return ds::cut_of([&](long long b) { return ((M + b - 1) / b) * ((N + b - 1) / b); }, (double)M * N, K, planes == 2 ? 3 : 1, may_split,
                       false, cu_count());
 }
 

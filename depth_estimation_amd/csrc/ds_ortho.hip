@@ -7,6 +7,11 @@
 // lost: with X, A and B rounded to bf16 the result is off by 1e-2 .. 6e-2, to fp16 by up to 8e-3 (matrices with a spectrum of
 // three decades; measured against 64 bits), so all three are kept as two fp16 planes (22 bits; 1e-6) under fixed powers of
 // two: entries of X and A are at most about 1.3, B's bound follows from the coefficients.
+//
+// bf16 results of larger matrices need less, and take half the products (Light): A and B keep one plane (11 bits) off the
+// diagonal, where their entries are small, and their diagonals, which carry most of X, in fp32 beside it; X keeps two planes
+// where it is multiplied by B.  What that costs is 2e-4 .. 9e-4 of the result's norm (sides of 64 and more; Gaussian, decaying
+// and nearly low-rank matrices), under the 1.7e-3 that rounding the result to bf16 costs.
 #include "ds_gemm.h"
 #include "ds_internal.h"
 #include "../../include/depthsynth.h"
@@ -99,64 +104,91 @@ __device__ __forceinline__ void triangle(int t, int& i, int& j) {
 // element (m, n) written at [n][m] (four consecutive m per lane) and, off the diagonal, at [m][n].  kNext: the next X, row n,
 // columns along m.  kLast: the result in the caller's type.
 enum Use { kGram, kPoly, kNext, kLast };
+template <Use U_, bool LIGHT_>
+struct How {
+    static constexpr Use U = U_;
+    static constexpr bool LIGHT = LIGHT_;
+};
 struct UseArgs {
     int rows, cols;          // of the result; columns beyond `cols` up to ld are written as zeros
     void* out;
     int ld;
     long long lo, per_out;   // planes apart, matrices apart
-    const f16* a;            // kPoly: A again
+    const f16* a;            // kPoly: A again; light kNext and kLast: X again
     long long per_a;
     float ca, cb, cc;        // kPoly's coefficients, scaled; else ca: the factor
+    float *da, *db;          // light: diagonals of A and of B, scaled as their matrices, `side` a matrix
+    int side, wide;
 };
 // fragment row i of a tile
-template <class S, Use U, class O>
+template <class S, class H, class O>
 __device__ __forceinline__ void use_row(const f32x4 (&acc)[S::FN], int i, int m0, int n0, int batch, const UseArgs& u) {
+    constexpr Use U = H::U;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / S::WN, wn = wave % S::WN;
     const int m = m0 + (wm * S::FM + i) * 16 + (lane >> 4) * 4;
     if (m >= u.ld) return;
-    {
+    const float* da = H::LIGHT ? u.da + (long long)batch * u.side : nullptr;
+    const float* db = H::LIGHT ? u.db + (long long)batch * u.side : nullptr;
 #pragma unroll
-        for (int j = 0; j < S::FN; ++j) {
-            const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
-            if (n >= u.rows) continue;
-            float v[4];
-            if (U == kPoly) {
-                const f16* a = u.a + batch * u.per_a + (long long)n * u.ld + m;
-                const f16x4 h = *reinterpret_cast<const f16x4*>(a), l = *reinterpret_cast<const f16x4*>(a + u.lo);
+    for (int j = 0; j < S::FN; ++j) {
+        const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
+        if (n >= u.rows) continue;
+        float v[4], old[4];
+        if (U == kPoly || (H::LIGHT && U != kGram)) {      // A or X at the same place
+            const f16* a = u.a + batch * u.per_a + (long long)n * u.ld + m;
+            const f16x4 h = *reinterpret_cast<const f16x4*>(a);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) old[e] = (float)h[e];
+            if (!(H::LIGHT && U == kPoly)) {
+                const f16x4 l = *reinterpret_cast<const f16x4*>(a + u.lo);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) old[e] += (float)l[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool in = m + e < u.cols, diagonal = m + e == n;
+            if (U == kPoly && !H::LIGHT) {
+                v[e] = fmaf(u.cc, acc[j][e], u.cb * old[e]) + (diagonal ? u.ca : 0.f);
+            } else if (U == kPoly) {
+                const float dn = da[n], dm = in ? da[m + e] : 0.f;
+                // (O + D)(O + D) = O O + O D + D O + D D
+                v[e] = diagonal ? 0.f : fmaf(u.cc, fmaf(dn + dm, old[e], acc[j][e]), u.cb * old[e]);
+                if (diagonal) u.db[(long long)batch * u.side + n] = fmaf(u.cc, fmaf(dn, dn, acc[j][e]), fmaf(u.cb, dn, u.ca));
+            } else if (H::LIGHT && U == kGram) {
+                v[e] = diagonal ? 0.f : acc[j][e] * u.ca;
+                if (diagonal) u.da[(long long)batch * u.side + n] = acc[j][e] * u.ca;
+            } else if (H::LIGHT) {
+                v[e] = in ? fmaf(db[u.wide ? n : m + e], old[e], acc[j][e]) * u.ca : 0.f;
+            } else {
+                v[e] = acc[j][e] * u.ca;
+            }
+            if (!in) v[e] = 0.f;
+        }
+        if (U == kLast) {
+            put_row4(static_cast<O*>(u.out) + batch * u.per_out + (long long)n * u.cols, m, u.cols, v, (u.cols & 3) == 0);
+        } else {
+            constexpr int kPut = H::LIGHT && U != kNext ? 1 : 3;
+            f16* out = static_cast<f16*>(u.out) + batch * u.per_out;
+            put4<kPut>(out + (long long)n * u.ld + m, u.lo, v);
+            if ((U == kGram || U == kPoly) && m0 != n0) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    v[e] = fmaf(u.cc, acc[j][e], u.cb * ((float)h[e] + (float)l[e])) + (m + e == n ? u.ca : 0.f);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[j][e] * u.ca;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (m + e >= u.cols) v[e] = 0.f;
-            if (U == kLast) {
-                put_row4(static_cast<O*>(u.out) + batch * u.per_out + (long long)n * u.cols, m, u.cols, v, (u.cols & 3) == 0);
-            } else {
-                f16* out = static_cast<f16*>(u.out) + batch * u.per_out;
-                put4<3>(out + (long long)n * u.ld + m, u.lo, v);
-                if ((U == kGram || U == kPoly) && m0 != n0) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (m + e < u.cols) {
-                            f16 h, l;
-                            split16(v[e], h, l);
-                            out[(long long)(m + e) * u.ld + n] = h;
-                            out[(long long)(m + e) * u.ld + n + u.lo] = l;
-                        }
-                }
+                    if (m + e < u.cols) {
+                        f16 h, l;
+                        split16(v[e], h, l);
+                        out[(long long)(m + e) * u.ld + n] = h;
+                        if (kPut == 3) out[(long long)(m + e) * u.ld + n + u.lo] = l;
+                    }
             }
         }
     }
 }
-template <class S, Use U, class O>
+template <class S, class H, class O>
 __device__ __forceinline__ void use_tile(const f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int batch, const UseArgs& u) {
 #pragma unroll
-    for (int i = 0; i < S::FM; ++i) use_row<S, U, O>(acc[i], i, m0, n0, batch, u);
+    for (int i = 0; i < S::FM; ++i) use_row<S, H, O>(acc[i], i, m0, n0, batch, u);
 }
 
 // C = A B over k.  tri: only tiles with m0 >= n0.  Units: matrices x tiles x splits; part (may be NULL: no splits): the tiles'
@@ -191,9 +223,9 @@ __device__ __forceinline__ void keep_part(const f32x4 (&acc)[S::FM][S::FN], cons
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) q[(i * S::FN + j) * S::T] = acc[i][j];
 }
-template <class S, Lay LA, Lay LB, Use U, class O, bool PART>
+template <class S, Lay LA, Lay LB, int PA, int PB, class H, class O, bool PART>
 __global__ __launch_bounds__(S::T) void ortho_product_kernel(ProductArgs p, UseArgs u, int units) {
-    __shared__ __align__(16) char lds[std::is_same<S, Big>::value ? Big::kLds : lds_bytes<S, 3>()];
+    __shared__ __align__(16) char lds[std::is_same<S, Big>::value ? Big::kLds : lds_bytes<S, PA, PB>()];
     const int per = cdiv(cdiv(p.k, kBK), p.splits) * kBK;
     auto job = [&](int x) {
         int batch, m0, n0, sp, tile;
@@ -209,12 +241,12 @@ __global__ __launch_bounds__(S::T) void ortho_product_kernel(ProductArgs p, UseA
         if (PART)
             keep_part<S>(acc, p, tile, sp);
         else
-            use_tile<S, U, O>(acc, m0, n0, batch, u);
+            use_tile<S, H, O>(acc, m0, n0, batch, u);
     };
     int t = blockIdx.x;
     f32x4 acc[S::FM][S::FN];
     if constexpr (std::is_same<S, Big>::value) {
-        TileStream<f16, LA, LB, 3> stream(lds, job(t));
+        TileStream<f16, LA, LB, PA, PB> stream(lds, job(t));
         for (; t < units; t += gridDim.x) {
             stream.multiply(acc, [&](Job& j) {
                 const int x = t + gridDim.x;
@@ -225,12 +257,12 @@ __global__ __launch_bounds__(S::T) void ortho_product_kernel(ProductArgs p, UseA
         }
     } else {
         const Job j = job(t);
-        gemm_tile<f16, S, LA, LB, 3>(j.A, j.B, j.m0, j.n0, j.kbeg, j.kend, lds, acc);
+        gemm_tile<f16, S, LA, LB, PA, PB>(j.A, j.B, j.m0, j.n0, j.kbeg, j.kend, lds, acc);
         done(t, acc);
     }
 }
 // adds a tile's splits in order; a workgroup for every fragment row, because there are few tiles where there are splits
-template <class S, Use U, class O>
+template <class S, class H, class O>
 __global__ __launch_bounds__(S::T) void ortho_finish_kernel(ProductArgs p, UseArgs u) {
     int batch, m0, n0, sp, tile;
     unit_of<S>(p, blockIdx.x * p.splits, gridDim.x * p.splits, batch, m0, n0, sp, tile);
@@ -243,7 +275,7 @@ __global__ __launch_bounds__(S::T) void ortho_finish_kernel(ProductArgs p, UseAr
     for (int s = 0; s < p.splits; ++s)
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) acc[j] += q[(long long)s * (S::BM * S::BN / 4) + j * S::T];
-    use_row<S, U, O>(acc, i, m0, n0, batch, u);
+    use_row<S, H, O>(acc, i, m0, n0, batch, u);
 }
 
 // ---- small matrices: all steps in one workgroup ------------------------------------------------------------------------
@@ -456,7 +488,8 @@ __global__ __launch_bounds__(256) void ortho_only_scale_kernel(const void* __res
 struct OrthoPlan {
     int s, l, sp, np, blocks;                 // smaller and larger side; row pitch of A and of X
     Cut gram, poly, apply;
-    size_t norm, x0, x1, a, b, part, total;
+    bool light;
+    size_t norm, x0, x1, a, b, da, part, total;
 };
 int tiles_of(ShapeId id, int M, int N, bool tri) {
     const int b = id == kBig ? 256 : id == kSq ? 128 : 64, m = cdiv(M, b), n = cdiv(N, b);
@@ -466,24 +499,26 @@ size_t part_bytes(const Cut& c, int M, int N, bool tri, int batch) {
     const size_t b = c.shape == kBig ? 256 : c.shape == kSq ? 128 : 64;
     return c.splits > 1 ? (size_t)batch * tiles_of(c.shape, M, N, tri) * c.splits * b * b * 4 : 0;
 }
-OrthoPlan ortho_plan(int batch, int m, int n) {
+OrthoPlan ortho_plan(int dtype, int batch, int m, int n) {
     OrthoPlan p;
     p.s = m < n ? m : n;
     p.l = m < n ? n : m;
     p.sp = pad8(p.s);
     p.np = pad8(n);
     p.blocks = norm_blocks((long long)m * n);
-    auto cut = [&](int M, int N, int K, bool tri) {
+    // below a side of 256 launches and latency are what a step takes, not products
+    p.light = dtype == DS_BF16 && p.s >= 256;
+    auto cut = [&](int M, int N, int K, int pairs, bool tri) {
         return cut_of(
             [&](long long b) {
                 const long long x = (M + b - 1) / b, y = (N + b - 1) / b;
                 return batch * (tri ? x * (x + 1) / 2 : x * y);
             },
-            (double)M * N * batch * (tri ? 0.5 : 1.0), K, 2, true, true, cu_count());
+            (double)M * N * batch * (tri ? 0.5 : 1.0), K, pairs, true, true, cu_count());
     };
-    p.gram = cut(p.s, p.s, p.l, true);
-    p.poly = cut(p.s, p.s, p.s, true);
-    p.apply = cut(n, m, p.s, false);
+    p.gram = cut(p.s, p.s, p.l, p.light ? 1 : 3, true);
+    p.poly = cut(p.s, p.s, p.s, p.light ? 1 : 3, true);
+    p.apply = cut(n, m, p.s, p.light ? 2 : 3, false);
     const size_t x = align256((size_t)batch * m * p.np * 4), a = align256((size_t)batch * p.s * p.sp * 4);
     size_t part = part_bytes(p.gram, p.s, p.s, true, batch), q = part_bytes(p.poly, p.s, p.s, true, batch);
     if (q > part) part = q;
@@ -495,6 +530,7 @@ OrthoPlan ortho_plan(int batch, int m, int n) {
     p.x1 = o; o += x;
     p.a = o; o += a;
     p.b = o; o += a;
+    p.da = o; o += align256((size_t)batch * p.s * 8);
     p.part = o; o += align256(part);
     p.total = o;
     return p;
@@ -507,29 +543,29 @@ int check_ortho(int batch, int m, int n) {
     return DS_OK;
 }
 
-template <class S, Lay LA, Lay LB, Use U, class O>
+template <class S, Lay LA, Lay LB, int PA, int PB, class H, class O>
 void product_shape(ProductArgs p, const UseArgs& u, int tiles, hipStream_t q) {
     const int units = tiles * p.splits;
     const int grid = std::is_same<S, Big>::value && units > cu_count() ? cu_count() : units;
     if (p.splits > 1) {
-        ortho_product_kernel<S, LA, LB, kGram, float, true><<<grid, S::T, 0, q>>>(p, u, units);
-        ortho_finish_kernel<S, U, O><<<dim3(tiles, S::FM), S::T, 0, q>>>(p, u);
+        ortho_product_kernel<S, LA, LB, PA, PB, How<kGram, false>, float, true><<<grid, S::T, 0, q>>>(p, u, units);
+        ortho_finish_kernel<S, H, O><<<dim3(tiles, S::FM), S::T, 0, q>>>(p, u);
     } else {
-        ortho_product_kernel<S, LA, LB, U, O, false><<<grid, S::T, 0, q>>>(p, u, units);
+        ortho_product_kernel<S, LA, LB, PA, PB, H, O, false><<<grid, S::T, 0, q>>>(p, u, units);
     }
 }
-template <Lay LA, Lay LB, Use U, class O>
+template <Lay LA, Lay LB, int PA, int PB, class H, class O>
 void product(const Cut& c, ProductArgs p, const UseArgs& u, int M, int N, hipStream_t q) {
     p.splits = c.splits;
     const int b = c.shape == kBig ? 256 : c.shape == kSq ? 128 : 64, tiles = tiles_of(c.shape, M, N, p.tri) * p.batch;
     p.mt = cdiv(M, b);
     p.nt = cdiv(N, b);
     if (c.shape == kBig)
-        product_shape<Big, LA, LB, U, O>(p, u, tiles, q);
+        product_shape<Big, LA, LB, PA, PB, H, O>(p, u, tiles, q);
     else if (c.shape == kSq)
-        product_shape<Sq, LA, LB, U, O>(p, u, tiles, q);
+        product_shape<Sq, LA, LB, PA, PB, H, O>(p, u, tiles, q);
     else
-        product_shape<Small, LA, LB, U, O>(p, u, tiles, q);
+        product_shape<Small, LA, LB, PA, PB, H, O>(p, u, tiles, q);
 }
 
 // stored B = 2^e B with |B| <= |a| + 2 |b| + 4 |c| below 2^15
@@ -538,40 +574,41 @@ float b_scale(const double* co) {
     return (float)(bound > 0 ? exp2(floor(log2(32768.0 / bound))) : 1.0);
 }
 
-template <class O>
+template <class O, bool LIGHT>
 void ortho_steps(const OrthoPlan& p, int batch, int m, int n, int steps, const double* co, char* ws, void* out, hipStream_t q) {
     f16 *x = reinterpret_cast<f16*>(ws + p.x0), *y = reinterpret_cast<f16*>(ws + p.x1);
     f16 *a = reinterpret_cast<f16*>(ws + p.a), *b = reinterpret_cast<f16*>(ws + p.b);
-    float* part = reinterpret_cast<float*>(ws + p.part);
+    float *part = reinterpret_cast<float*>(ws + p.part), *da = reinterpret_cast<float*>(ws + p.da), *db = da + (long long)batch * p.s;
     const long long px = 2ll * m * p.np, lox = (long long)m * p.np, pa = 2ll * p.s * p.sp, loa = (long long)p.s * p.sp;
     const float bs = b_scale(co);
     const bool wide = m <= n;
+    constexpr int P = LIGHT ? 1 : 2;      // planes of A, of B, and of X in A = X X^T
     for (int i = 0; i < steps; ++i) {
         const Operand X{x, p.np, lox, m, p.np}, A{a, p.sp, loa, p.s, p.sp}, B{b, p.sp, loa, p.s, p.sp};
         const ProductArgs pg{X, X, px, px, 0, 0, 1, p.l, 1, batch, part};
-        const UseArgs ug{p.s, p.s, a, p.sp, loa, pa, nullptr, 0, 1.f / kXs, 0.f, 0.f};
+        const UseArgs ug{p.s, p.s, a, p.sp, loa, pa, nullptr, 0, 1.f / kXs, 0.f, 0.f, da, db, p.s, wide};
         if (wide)
-            product<kK, kK, kGram, float>(p.gram, pg, ug, p.s, p.s, q);
+            product<kK, kK, P, P, How<kGram, LIGHT>, float>(p.gram, pg, ug, p.s, p.s, q);
         else
-            product<kM, kM, kGram, float>(p.gram, pg, ug, p.s, p.s, q);
+            product<kM, kM, P, P, How<kGram, LIGHT>, float>(p.gram, pg, ug, p.s, p.s, q);
         const ProductArgs pp{A, A, pa, pa, 0, 0, 1, p.s, 1, batch, part};
         const UseArgs up{p.s, p.s, b, p.sp, loa, pa, a, pa, (float)(co[0] * bs), (float)(co[1] * bs / kXs),
-                         (float)(co[2] * bs / (kXs * kXs))};
-        product<kK, kK, kPoly, float>(p.poly, pp, up, p.s, p.s, q);
+                         (float)(co[2] * bs / (kXs * kXs)), da, db, p.s, wide};
+        product<kK, kK, P, P, How<kPoly, LIGHT>, float>(p.poly, pp, up, p.s, p.s, q);
         const bool last = i + 1 == steps;
-        const UseArgs ua{m, n, last ? out : y, p.np, lox, last ? (long long)m * n : px, nullptr, 0,
-                         last ? 1.f / (bs * kXs) : 1.f / bs, 0.f, 0.f};
+        const UseArgs ua{m, n, last ? out : y, p.np, lox, last ? (long long)m * n : px, x, px,
+                         last ? 1.f / (bs * kXs) : 1.f / bs, 0.f, 0.f, da, db, p.s, wide};
         const ProductArgs pw{wide ? X : B, wide ? B : X, wide ? px : pa, wide ? pa : px, 0, 0, 0, p.s, 1, batch, part};
         if (wide) {
             if (last)
-                product<kM, kK, kLast, O>(p.apply, pw, ua, n, m, q);
+                product<kM, kK, 2, P, How<kLast, LIGHT>, O>(p.apply, pw, ua, n, m, q);
             else
-                product<kM, kK, kNext, float>(p.apply, pw, ua, n, m, q);
+                product<kM, kK, 2, P, How<kNext, LIGHT>, float>(p.apply, pw, ua, n, m, q);
         } else {
             if (last)
-                product<kK, kK, kLast, O>(p.apply, pw, ua, n, m, q);
+                product<kK, kK, P, 2, How<kLast, LIGHT>, O>(p.apply, pw, ua, n, m, q);
             else
-                product<kK, kK, kNext, float>(p.apply, pw, ua, n, m, q);
+                product<kK, kK, P, 2, How<kNext, LIGHT>, float>(p.apply, pw, ua, n, m, q);
         }
         f16* z = x;
         x = y;
@@ -615,7 +652,10 @@ int ortho_any(const OrthoPlan& p, const void* g, int dtype, int batch, int m, in
         ortho_load_kernel<<<dim3(nb, batch), 256, 0, q>>>(g, dtype, m, n, p.np, eps, part, p.blocks,
                                                           reinterpret_cast<f16*>(ws + p.x0), (long long)m * p.np,
                                                           2ll * m * p.np);
-        ortho_steps<O>(p, batch, m, n, steps, co, ws, out, q);
+        if constexpr (std::is_same<O, bf16>::value) {
+            if (p.light) ortho_steps<O, true>(p, batch, m, n, steps, co, ws, out, q);
+        }
+        if (!p.light) ortho_steps<O, false>(p, batch, m, n, steps, co, ws, out, q);
     }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? DS_OK : (int)e;
@@ -626,8 +666,8 @@ int ortho_any(const OrthoPlan& p, const void* g, int dtype, int batch, int m, in
 
 extern "C" {
 
-size_t ds_orthogonalize_workspace_bytes(int batch, int m, int n) {
-    return ds::check_ortho(batch, m, n) ? 0 : ds::ortho_plan(batch, m, n).total;
+size_t ds_orthogonalize_workspace_bytes(int dtype, int batch, int m, int n) {
+    return ds::check_ortho(batch, m, n) ? 0 : ds::ortho_plan(dtype, batch, m, n).total;
 }
 
 int ds_orthogonalize(const void* update, int dtype, int batch, int m, int n, int steps, const double* coefficients, double eps,
@@ -637,7 +677,7 @@ int ds_orthogonalize(const void* update, int dtype, int batch, int m, int n, int
     if (rc) return rc;
     if (steps > DS_ORTHO_MAX_STEPS || (dtype != DS_F32 && dtype != DS_F16 && dtype != DS_BF16)) return DS_ERR_UNSUPPORTED;
     if (((uintptr_t)out & 15) != 0) return DS_ERR_INVALID_ARG;
-    const ds::OrthoPlan p = ds::ortho_plan(batch, m, n);
+    const ds::OrthoPlan p = ds::ortho_plan(dtype, batch, m, n);
     if (!workspace || workspace_bytes < p.total || ((uintptr_t)workspace & 15) != 0) return DS_ERR_WORKSPACE;
     char* ws = static_cast<char*>(workspace);
     hipStream_t q = static_cast<hipStream_t>(stream);

@@ -791,7 +791,7 @@ def orthogonalize(update, steps: int, coefficients, eps: float) -> torch.Tensor:
     if u.numel() == 0:
         return out
     b, lib = u.numel() // (m * n), L.lib()
-    nb = lib.ds_orthogonalize_workspace_bytes(b, m, n)
+    nb = lib.ds_orthogonalize_workspace_bytes(L.DTYPES[u.dtype], b, m, n)
     ws = _scratch(nb, u.device)
     L.check(lib.ds_orthogonalize(u.data_ptr(), L.DTYPES[u.dtype], b, m, n, int(steps), (C.c_double * 3)(*co), float(eps),
                                  out.data_ptr(), ws.data_ptr(), nb, L.stream()), "ds_orthogonalize")

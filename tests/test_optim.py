@@ -75,6 +75,21 @@ def test_larger_tiles(shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["gauss", "decay", "few"])
+@pytest.mark.parametrize("shape", [(256, 256), (256, 1000), (1001, 259), (2, 300, 530), (700, 700), (2300, 2100)], ids=str)
+def test_bfloat16_with_fewer_products(shape, kind):
+    """Sides of 256 and more: 11-bit operands.  Rounding the result alone is off by 2^-8 / sqrt(3) at most in norm (1.7e-3 for
+    numbers spread evenly between powers of two), the operands' rounding by less (9e-4 was the most over these spectra when
+    the arithmetic was written out in float64): together at most sqrt(1.7^2 + 1.1^2) 1e-3 = 2.0e-3 with some room, against
+    half a step of bfloat16, 3.9e-3."""
+    from depth_estimation_amd import optim
+    if shape[-1] > 2000 and kind == "decay":
+        pytest.skip("a float64 decomposition of this size takes too long")
+    g = _update(shape, torch.bfloat16, seed=sum(shape), kind=kind)
+    assert _error(optim.orthogonalize(g), _oracle(g)) <= 2.3e-3
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("steps", [0, 1, 2, 7])
 def test_steps_coefficients_and_eps(steps):
     from depth_estimation_amd import optim
@@ -196,7 +211,7 @@ def test_refusals_on_the_host():
                      (call(steps=33), -2), (call(m=1 << 17), -2), (call(m=40000, n=40000), -2), (call(b=70000), -2),
                      (call(ws=None), -3), (call(nb=16), -3), (call(ws=fake + 8), -3), (call(out=fake + 4), -1)]:
         assert rc == want
-    assert lib.ds_orthogonalize_workspace_bytes(1, 0, 4) == 0
+    assert lib.ds_orthogonalize_workspace_bytes(0, 1, 0, 4) == 0
 
 
 @pytest.mark.gpu
