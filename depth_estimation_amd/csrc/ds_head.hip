@@ -647,7 +647,6 @@ __device__ __forceinline__ void grad_of_tile(const f32x4 (&acc)[S::FM][S::FN], i
     const float is = SPLIT == 3 ? 1.f / scale_for(from_bits(WHICH == 0 ? st->amax_w : st->amax_h)) : 1.f;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / S::WN, wn = wave % S::WN, Dp = (a.D + 3) & ~3;
-    const bool aligned = (a.D & 3) == 0;
 #pragma unroll
     for (int j = 0; j < S::FN; ++j) {
         const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
@@ -666,7 +665,7 @@ __device__ __forceinline__ void grad_of_tile(const f32x4 (&acc)[S::FM][S::FN], i
                 float v[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * f0 * is;
-                put_row4(static_cast<O*>(a.out) + row * a.D, d, a.D, v, aligned);
+                put_row4(static_cast<O*>(a.out) + row * a.D, d, a.D, v);
             }
         }
     }
@@ -728,7 +727,6 @@ __global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__
     const int cnt = which == 0 ? st->count : n, Dp = (D + 3) & ~3, q = Dp / 4;
     const float f0 = dl_norm<T>(bs, up, mode, st->count) / Store<T>::k;
     const float is = SPLIT == 3 ? 1.f / scale_for(from_bits(which == 0 ? st->amax_w : st->amax_h)) : 1.f;
-    const bool aligned = (D & 3) == 0;
     const long long all = (long long)cnt * q;
     const int x = threadIdx.x % kOuts, y = threadIdx.x / kOuts, per = (splits + PAR - 1) / PAR;
     for (long long i0 = (long long)blockIdx.x * kOuts; i0 < all; i0 += (long long)gridDim.x * kOuts) {
@@ -752,7 +750,7 @@ __global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__
             const long long r = i / q;
             const int d = (int)(i - r * q) * 4;
             const float v[4] = {a[0] * f0 * is, a[1] * f0 * is, a[2] * f0 * is, a[3] * f0 * is};
-            put_row4(out + (rows && which == 0 ? (long long)rows[r] : r) * D, d, D, v, aligned);
+            put_row4(out + (rows && which == 0 ? (long long)rows[r] : r) * D, d, D, v);
         }
     }
 }
@@ -1067,7 +1065,7 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
                 for (int i = 0; i < 2 * ND; ++i) {
                     const int c = i * 16 + (lane >> 4) * 4;
                     const float y[4] = {acc[i][0] * back, acc[i][1] * back, acc[i][2] * back, acc[i][3] * back};
-                    if (c < a.D) put_row4(row, c, a.D, y, (a.D & 3) == 0);
+                    if (c < a.D) put_row4(row, c, a.D, y);
                 }
             }
             if (o.packed) {
@@ -1316,8 +1314,9 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     p.part = o; o += p.few ? align256((size_t)p.few_grid * p.few * 16) : p.slim ? 0 : 3 * align256((size_t)p.vt_fwd * N * 4);
     p.sums = o; o += align256((size_t)(cdiv(N, 32) > p.slim_grid ? cdiv(N, 32) : p.slim_grid) * 8);
     p.fwd_total = o;
-    // a piece of the classes: what fits 256 MB of dl, at least 1024 classes, a multiple of 256
-    const long long fit = (256ll << 20) / ((long long)el * N) / 256 * 256;
+    // a piece of the classes: what fits 256 MB of dl (64 MB: 16 % slower at 8192 x 65536 x 1024, 128 MB: 4 %, 512 MB: the
+    // same), at least 1024 classes, a multiple of 256
+        const long long fit = (256ll << 20) / ((long long)el * N) / 256 * 256;
     const long long piece = p.slim_back ? V : fit < 1024 ? 1024 : fit;
     p.piece = piece >= V ? V : (int)piece;
     p.piece_ld = pad8(p.piece);

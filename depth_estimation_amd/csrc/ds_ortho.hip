@@ -45,25 +45,32 @@ __device__ __forceinline__ double sum_all(double a, double* s) {
     return a;
 }
 
-__global__ __launch_bounds__(256) void ortho_norm_kernel(const void* __restrict__ g, int dtype, long long mn,
-                                                         double* __restrict__ part) {
+// 16 bytes a lane, four such loads under way; the elements behind the last whole vector by the first block
+template <class O>
+__global__ __launch_bounds__(256) void ortho_norm_kernel(const O* __restrict__ g, long long mn, double* __restrict__ part) {
+    constexpr int VEC = 16 / sizeof(O), U = 4;
+    typedef O vec __attribute__((ext_vector_type(VEC)));
+    typedef vec loose __attribute__((aligned(sizeof(O))));
     __shared__ double s[4];
-    const long long base = blockIdx.y * mn, step = gridDim.x * 256ll;
-    double a0 = 0.0, a1 = 0.0, a2 = 0.0, a3 = 0.0;
-    long long i = blockIdx.x * 256ll + threadIdx.x;
-    for (; i + 3 * step < mn; i += 4 * step) {
-        const float x0 = element(g, dtype, base + i), x1 = element(g, dtype, base + i + step);
-        const float x2 = element(g, dtype, base + i + 2 * step), x3 = element(g, dtype, base + i + 3 * step);
-        a0 += (double)x0 * x0;
-        a1 += (double)x1 * x1;
-        a2 += (double)x2 * x2;
-        a3 += (double)x3 * x3;
+    const O* x = g + blockIdx.y * mn;
+    const long long nv = mn / VEC, step = gridDim.x * 256ll;
+    double a = 0.0;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < nv; i += U * step) {
+        vec v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            v[u] = *reinterpret_cast<const loose*>(x + (i + u * step < nv ? i + u * step : i) * VEC);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i + u * step < nv)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) a = fma((double)(float)v[u][e], (double)(float)v[u][e], a);
     }
-    for (; i < mn; i += step) {
-        const float x = element(g, dtype, base + i);
-        a0 += (double)x * x;
+    if (blockIdx.x == 0 && nv * VEC + threadIdx.x < mn) {
+        const double y = (float)x[nv * VEC + threadIdx.x];
+        a = fma(y, y, a);
     }
-    const double a = sum_all<256>((a0 + a1) + (a2 + a3), s);
+    a = sum_all<256>(a, s);
     if (threadIdx.x == 0) part[blockIdx.y * gridDim.x + blockIdx.x] = a;
 }
 __device__ __forceinline__ double inverse_norm(const double* part, int blocks, double eps, double* s) {
@@ -167,7 +174,7 @@ __device__ __forceinline__ void use_row(const f32x4 (&acc)[S::FN], int i, int m0
             if (!in) v[e] = 0.f;
         }
         if (U == kLast) {
-            put_row4(static_cast<O*>(u.out) + batch * u.per_out + (long long)n * u.cols, m, u.cols, v, (u.cols & 3) == 0);
+            put_row4(static_cast<O*>(u.out) + batch * u.per_out + (long long)n * u.cols, m, u.cols, v);
         } else {
             constexpr int kPut = H::LIGHT && U != kNext ? 1 : 3;
             f16* out = static_cast<f16*>(u.out) + batch * u.per_out;
@@ -643,7 +650,7 @@ int ortho_any(const OrthoPlan& p, const void* g, int dtype, int batch, int m, in
     }
     double* part = reinterpret_cast<double*>(ws + p.norm);
     const long long mn = (long long)m * n;
-    ortho_norm_kernel<<<dim3(p.blocks, batch), 256, 0, q>>>(g, dtype, mn, part);
+    ortho_norm_kernel<O><<<dim3(p.blocks, batch), 256, 0, q>>>(static_cast<const O*>(g), mn, part);
     if (steps == 0) {
         const int nb = cdiv(mn, 1024) < 4096 ? cdiv(mn, 1024) : 4096;
         ortho_only_scale_kernel<O><<<dim3(nb, batch), 256, 0, q>>>(g, eps, part, p.blocks, mn, out);
