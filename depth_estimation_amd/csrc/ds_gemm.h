@@ -295,6 +295,7 @@ struct TileStream {
     Mover<LB, S::BN, S::T> mb;
     Job job;
     int steps, parity, tid;
+    bool edge;       // the lane offsets are those of a tile that lies across an edge (or of none)
     char* lds;       // S::kLds bytes that nothing else uses
 
     __device__ __forceinline__ void move(int s) {
@@ -309,11 +310,62 @@ struct TileStream {
         job = j;
         const int n = (j.kend - j.kbeg + kBK - 1) / kBK * kPairs;
         steps = n > 0 ? n : 1;
-        ma.init(j.A, j.m0, tid);
-        mb.init(j.B, j.n0, tid);
+        // lane offsets differ from the tile before only where one of the two lies across an edge
+        const bool e = j.m0 + S::BM > (LA == kK ? j.A.outer : j.A.inner) || j.n0 + S::BN > (LB == kK ? j.B.outer : j.B.inner);
+        if (e || edge) {
+            ma.init(j.A, j.m0, tid);
+            mb.init(j.B, j.n0, tid);
+        }
+        edge = e;
         move(0);
     }
-    __device__ __forceinline__ TileStream(char* lds_, const Job& j) : parity(0), tid(threadIdx.x), lds(lds_) { start(j); }
+    __device__ __forceinline__ TileStream(char* lds_, const Job& j) : parity(0), tid(threadIdx.x), edge(true), lds(lds_) { start(j); }
+
+    __device__ __forceinline__ void fetch(const char* buf, int kk, const Fragments<LA, S::BM>& fa, const Fragments<LB, S::BN>& fb,
+                                          s16x8 (&a)[S::FM], s16x8 (&b)[S::FN]) const {
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) b[j] = fb.get(buf + S::BM * kBK * 2, j, kk);
+#pragma unroll
+        for (int i = 0; i < S::FM; ++i) a[i] = fa.get(buf, i, kk);
+    }
+    template <bool ZERO>      // ZERO: the sums begin here
+    __device__ __forceinline__ void add(const s16x8 (&a)[S::FM], const s16x8 (&b)[S::FN], f32x4 (&acc)[S::FM][S::FN]) const {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+            for (int j = 0; j < S::FN; ++j) acc[i][j] = mfma(a[i], b[j], ZERO ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[i][j], T());
+        __builtin_amdgcn_s_setprio(0);
+    }
+    template <bool FIRST, class Next>
+    __device__ __forceinline__ void step(int s, int n, int group, const Fragments<LA, S::BM>& fa, const Fragments<LB, S::BN>& fb,
+                                         f32x4 (&acc)[S::FM][S::FN], Next& next) {
+        const char* buf = lds + ((s + parity) & 1) * ((S::BM + S::BN) * kBK * 2);
+        s16x8 a[S::FM], b[S::FN];
+        fetch(buf, 0, fa, fb, a, b);
+        // the other buffer was read for the last time in the turn before this one (group 1's second half of step s - 1)
+        if (s + 1 < n) {
+            move(s + 1);
+        } else {
+            Job j;
+            if (next(j)) {
+                parity = (parity + n) & 1;
+                start(j);
+            }
+        }
+        wait_lds();
+        turn();
+        add<FIRST>(a, b, acc);
+        turn();
+        fetch(buf, 1, fa, fb, a, b);
+        wait_lds();
+        // both groups' shares of the next step have arrived when the turn ends in which group 1 reads this step's last
+        if (group == 1 && s + 1 < n) wait_dma();
+        turn();
+        add<false>(a, b, acc);
+        if (group == 0 && s + 1 < n) wait_dma();
+        turn();
+    }
 
     // Multiplies the job that start() took up.  next(Job&) -> bool names the one after it, whose first step is then under way
     // on return (waiting for it here, so that the caller's stores need not be waited for with it, cost 4 %: 4.09 against
@@ -322,74 +374,45 @@ struct TileStream {
     __device__ __forceinline__ void multiply(f32x4 (&acc)[S::FM][S::FN], Next next) {
         const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = wave / S::WN;
         const int wm = group * S::FM * 16, wn = (wave % S::WN) * S::FN * 16;
-        constexpr int kA = S::BM * kBK * 2, kBuf = (S::BM + S::BN) * kBK * 2;
         const Fragments<LA, S::BM> fa(wm, lane);
         const Fragments<LB, S::BN> fb(wn, lane);
-#pragma unroll
-        for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-            for (int j = 0; j < S::FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         wait_dma();
         turn();
         if (group == 1) turn();       // half a step behind the other group from here on
         const int n = steps;
-        for (int s = 0; s < n; ++s) {
-            const char* buf = lds + ((s + parity) & 1) * kBuf;
-            s16x8 a[S::FM], b[S::FN];
-#pragma unroll
-            for (int j = 0; j < S::FN; ++j) b[j] = fb.get(buf + kA, j, 0);
-#pragma unroll
-            for (int i = 0; i < S::FM; ++i) a[i] = fa.get(buf, i, 0);
-            // the other buffer was read for the last time in the turn before this one (group 1's second half of step s - 1)
-            if (s + 1 < n) {
-                move(s + 1);
-            } else {
-                Job j;
-                if (next(j)) {
-                    parity = (parity + n) & 1;
-                    start(j);
-                }
-            }
-            wait_lds();
-            turn();
-            __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-            for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-                for (int j = 0; j < S::FN; ++j) acc[i][j] = mfma(a[i], b[j], acc[i][j], T());
-            __builtin_amdgcn_s_setprio(0);
-            turn();
-#pragma unroll
-            for (int j = 0; j < S::FN; ++j) b[j] = fb.get(buf + kA, j, 1);
-#pragma unroll
-            for (int i = 0; i < S::FM; ++i) a[i] = fa.get(buf, i, 1);
-            wait_lds();
-            // both groups' shares of the next step have arrived when the turn ends in which group 1 reads this step's last
-            if (group == 1 && s + 1 < n) wait_dma();
-            turn();
-            __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-            for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-                for (int j = 0; j < S::FN; ++j) acc[i][j] = mfma(a[i], b[j], acc[i][j], T());
-            __builtin_amdgcn_s_setprio(0);
-            if (group == 0 && s + 1 < n) wait_dma();
-            turn();
-        }
+        step<true>(0, n, group, fa, fb, acc, next);
+        // not unrolled, nor its last step peeled: the compiler would move all sums between two sets of registers
+#pragma clang loop unroll(disable)
+        for (int s = 1; s < n; ++s) step<false>(s, n, group, fa, fb, acc, next);
         if (group == 0) turn();
     }
 };
 
 // Tile t of mt x nt in the order in which they are taken: workgroup b runs on XCD b % 8, each with an L2 of its own, so every
 // XCD gets a contiguous share, and inside it bands of four tile columns are gone through row by row: the tiles in flight on an
-// XCD share a few rows and columns.
-__device__ __forceinline__ void tile_of(int t, int tiles, int mt, int nt, int& m, int& n) {
-    const int q = tiles >> 3, r = tiles & 7, x = t & 7;
-    const int u = x * q + (x < r ? x : r) + (t >> 3);
-    const int band = u / (4 * mt), in = u - band * 4 * mt, w = nt - band * 4 < 4 ? nt - band * 4 : 4;
-    n = band * 4 + in % w;
-    m = in / w;
-}
+// XCD share a few rows and columns.  (No division but by the few columns of a last, narrower band: the next tile is looked up
+// while a turn waits for it.)
+struct Order {
+    int tiles, mt, nt, q, r;
+    float inv;       // 1 / (4 mt)
+    __device__ __forceinline__ Order(int tiles_, int mt_, int nt_) : tiles(tiles_), mt(mt_), nt(nt_), q(tiles_ >> 3), r(tiles_ & 7) {
+        inv = 1.f / (4.f * mt_);
+    }
+    __device__ __forceinline__ void operator()(int t, int& m, int& n) const {
+        const int x = t & 7, u = x * q + (x < r ? x : r) + (t >> 3);
+        int band = __builtin_amdgcn_readfirstlane((int)((float)u * inv));      // off by one at most, or a little more far out
+        while (band * 4 * mt > u) --band;
+        while ((band + 1) * 4 * mt <= u) ++band;
+        const int in = u - band * 4 * mt, w = nt - band * 4;
+        if (w >= 4) {
+            n = band * 4 + (in & 3);
+            m = in >> 2;
+        } else {
+            n = band * 4 + in % w;
+            m = in / w;
+        }
+    }
+};
 
 // x as two fp16 numbers: hi = x to 11 bits, lo = the rest to 11 bits.  Where hi is not finite lo is 0, so that an infinity
 // stays one instead of becoming inf - inf.

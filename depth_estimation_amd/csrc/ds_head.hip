@@ -381,9 +381,10 @@ __global__ __launch_bounds__(Big::T) void head_stats_big_kernel(Operand W, Opera
     int t = blockIdx.x;
     if (t >= tiles) return;
     H.outer = cnt;
+    const Order order(tiles, mt, nt);
     auto job = [&](int u) {
         int m, n;
-        tile_of(u, tiles, mt, nt, m, n);
+        order(u, m, n);
         return Job{W, H, m * Big::BM, n * Big::BN, 0, D};
     };
     TileStream<T, kK, kK, kP<SPLIT>, kP<SPLIT>> stream(lds, job(t));
@@ -609,9 +610,10 @@ __global__ __launch_bounds__(Big::T) void head_dl_big_kernel(Operand W, Operand 
     int t = blockIdx.x;
     if (t >= tiles) return;
     H.outer = cnt;
+    const Order order(tiles, mt, nt);
     auto job = [&](int u) {
         int m, n;
-        tile_of(u, tiles, mt, nt, m, n);
+        order(u, m, n);
         return Job{W, H, m * Big::BM, n * Big::BN, 0, D};
     };
     TileStream<T, kK, kK, kP<SPLIT>, kP<SPLIT>> stream(lds, job(t));
@@ -684,12 +686,14 @@ __global__ __launch_bounds__(S::T) void head_grad_kernel(Operand A, Operand B, c
         const int nt = cdiv(bound, S::BN), units = mt * nt * a.splits;
         int t = blockIdx.x;
         if (t >= units) return;
+        const Order order(units, mt * a.splits, nt);
         auto job = [&](int u, int& sp) {
             int x, n;
-            tile_of(u, units, mt * a.splits, nt, x, n);
-            sp = x % a.splits;
+            order(u, x, n);
+            const int m = x / a.splits;
+            sp = x - m * a.splits;
             const int k0 = min(sp * per, k);
-            return Job{A, B, x / a.splits * S::BM, n * S::BN, k0, min(k0 + per, k)};
+            return Job{A, B, m * S::BM, n * S::BN, k0, min(k0 + per, k)};
         };
         int sp, next_sp = 0;
         TileStream<T, kM, LB, kP<SPLIT>, kP<SPLIT>> stream(lds, job(t, sp));

@@ -216,7 +216,7 @@ __device__ __forceinline__ void unit_of(const ProductArgs& p, int u, int units, 
     if (p.tri) {
         triangle(in / p.splits, m, n);
     } else {
-        tile_of(in / p.splits, tiles, p.mt, p.nt, m, n);
+        Order(tiles, p.mt, p.nt)(in / p.splits, m, n);
     }
     tile = batch * tiles + in / p.splits;
     m0 = m * S::BM;
