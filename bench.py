@@ -508,6 +508,8 @@ def main():
     ap.add_argument("--steps", type=int, default=200)
     ap.add_argument("--warmup", type=int, default=20)
     ap.add_argument("--workload", default="b12_s2_192x640_fwdbwd", choices=sorted(WORKLOADS))
+    ap.add_argument("--optimizer", default="adam", choices=("adam", "muon"),
+                    help="full_step: torch's Adam, or depth_estimation_amd.optim.Muon for the weight matrices")
     ap.add_argument("--image-grad", action="store_true", help="also scatter the source-image gradient")
     ap.add_argument("--no-cpu", action="store_true", help="skip the cpu_baseline leg")
     ap.add_argument("--cold-steps", type=int, default=20, help="single steps timed after a cache flush (0 = skip)")

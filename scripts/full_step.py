@@ -1,6 +1,6 @@
 """the whole train.py step, batch-sharded over the ranks, with the gradient all-reduce.
 
-    python bench.py --workload full_step [--gpus N] [--steps K] [--warmup W]
+    python bench.py --workload full_step [--gpus N] [--steps K] [--warmup W] [--optimizer muon]
 
 What a step does (reference: train.py:39-109; optimizer set train.py:140; frozen encoder depth_encoder.py:28):
 
@@ -122,6 +122,28 @@ def trainable(nets):
     return [p for m in (nets.pose, nets.decoder, nets.convgru) for p in m.parameters()]
 
 
+class MatrixAndVectorOptimizer:
+    """depth_estimation_amd.optim.Muon for the weight matrices (two or more dimensions), torch.optim.Adam for the rest: the
+    two calls of an optimizer that train_step makes."""
+
+    def __init__(self, params):
+        from depth_estimation_amd.optim import Muon
+        self.parts = [Muon([p for p in params if p.dim() >= 2]), torch.optim.Adam([p for p in params if p.dim() < 2])]
+
+    def zero_grad(self, set_to_none: bool = True):
+        for opt in self.parts:
+            opt.zero_grad(set_to_none=set_to_none)
+
+    def step(self):
+        for opt in self.parts:
+            opt.step()
+
+
+def build_optimizer(params, name: str = "adam"):
+    """"adam": the reference's (train.py:140); "muon": orthogonalised steps for the matrices (GPU only)."""
+    return torch.optim.Adam(params) if name == "adam" else MatrixAndVectorOptimizer(params)
+
+
 def train_step(nets, opt, buckets, imgs, path, max_depth=MAX_DEPTH):
     """One optimisation step on this rank's samples imgs (B, S+1, 3, H, W); the last frame of a sample is the target
     (train.py:42).  `path` supplies the hot-path functions (HIP in bench.py, torch stand-ins in the CPU test):
@@ -185,7 +207,10 @@ def main(args, rank, local_rank, world, dry=False):
     """dry: the same harness on the CPU over gloo -- launcher, rendezvous, bucketed all-reduce from the backward hooks,
     clipping, Adam -- with torch stand-ins for the hot path, tiny networks and images; no kernels, `value` 0."""
     import torch.distributed as dist
+    optimizer = getattr(args, "optimizer", "adam")
     if dry:
+        if optimizer != "adam":
+            raise SystemExit("--optimizer muon runs HIP kernels and has no CPU form: not with --dry")
         dev = torch.device("cpu")
         torch.set_num_threads(1)
         if world > 1:
@@ -211,7 +236,7 @@ def main(args, rank, local_rank, world, dry=False):
     nets = build_networks(dev, counts)
     params = trainable(nets)
     n_params = sum(p.numel() for p in params)
-    opt = torch.optim.Adam(params)                                               # train.py:140
+    opt = build_optimizer(params, optimizer)                                     # train.py:140
     buckets = GradBuckets(params, bucket_bytes=bucket_bytes, average=False)
     buckets.attach()
     g = torch.Generator().manual_seed(100 + rank)
@@ -276,6 +301,7 @@ def main(args, rank, local_rank, world, dry=False):
             "scaling": "weak", "vs_baseline": None, "dtype": "f32", "data": "synthetic",
             "config": {"workload": "full_step", "samples_per_gpu": B, "sources_per_target": S, "height": H, "width": W,
                        "networks": "stand-ins with the reference's trainable parameter counts", "params": n_params,
+                       "optimizer": optimizer,
                        "parallelism": f"batch-sharded x{world}, gradient all-reduce (RCCL), SUM over ranks"},
             "samples_per_s": round(world * B * args.steps / elapsed, 2),
             "world_size": dist.get_world_size() if world > 1 else 1, "ranks_summed": ranks_summed,

@@ -189,6 +189,31 @@ def test_muon_steps():
     assert torch.equal(other.state[ps[0]]["momentum_buffer"], opt.state[ps[0]]["momentum_buffer"])
 
 
+@pytest.mark.gpu
+def test_whole_training_step_with_matrix_updates():
+    """scripts/full_step.train_step with --optimizer muon: every matrix moves by its orthogonalised first momentum, the vectors
+    by Adam."""
+    import depth_estimation_amd as de
+    from scripts import full_step as fs
+    dev, H, W = torch.device(DEV), 48, 160
+    nets = fs.build_networks(dev, dict(pose=20_000, decoder=1_000, convgru=500), seed=3)
+    params = fs.trainable(nets)
+    before = [p.detach().clone() for p in params]
+    opt = fs.build_optimizer(params, "muon")
+    imgs = torch.rand(1, 3, 3, H, W, generator=torch.Generator().manual_seed(9)).to(dev)
+    loss = fs.train_step(nets, opt, None, imgs, fs.hip_path(de, H, W, dev))
+    assert bool(torch.isfinite(loss))
+    for p, old in zip(params, before):
+        if p.dim() < 2:
+            assert float((p - old).abs().max()) <= 1.01e-3                      # Adam's first step: at most its learning rate
+            continue
+        g = p.grad.flatten(1)
+        want = _oracle(1.95 * g).view(p.shape).to(dev) * 0.02 * max(1.0, g.shape[0] / g.shape[1]) ** 0.5
+        # the orthogonalised matrix is exact to 2e-4 of its norm (the gradients' spectra are wide); a step of size 0.02 on
+        # weights of size one is read back with 2^-24
+        assert float(((old - p.detach()).double() - want).norm()) <= 1e-3 * float(want.norm()) + 2.0 ** -24 * p.numel() ** 0.5
+
+
 def test_refusals_on_the_host():
     from depth_estimation_amd import _lib as L, optim
     with pytest.raises(RuntimeError, match="GPU"):
