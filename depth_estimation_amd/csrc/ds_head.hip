@@ -565,7 +565,7 @@ __device__ __forceinline__ void dl_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, i
                 for (int e = 0; e < 4; ++e) {
                     const float l = SPLIT == 3 ? acc[i][j][e] * il * iw : acc[i][j][e];
                     const float x = exp_of(l - tp);
-                    acc[i][j][e] = t == i * 16 + e ? (x * rs - 1.f) * g : x * gr;
+                    acc[i][j][e] = fmaf(x, gr, t == i * 16 + e ? -g : 0.f);
                 }
         } else {
             const float e0 = a.mean[n], gr = g * rs;
@@ -851,6 +851,10 @@ __device__ __forceinline__ void slim_load_w(const SlimArgs& a, char* lds) {
                 *reinterpret_cast<i32x4*>(lds + p * a.Vp * ND * 64 + (c >> 3) * a.Vp * 128 + lds_chunk<kK, 16>(v, c & 7)) = x[u][p];
         }
     }
+    if (a.centers) {      // behind the weight; zero where there is no class
+        float* c = reinterpret_cast<float*>(lds + P * a.Vp * ND * 64);
+        for (int v = threadIdx.x; v < a.Vp; v += kSlimT) c[v] = v < a.V ? a.centers[v] : 0.f;
+    }
     __syncthreads();
 }
 template <int P, int ND>
@@ -910,40 +914,48 @@ __global__ __launch_bounds__(kSlimT) void slim_fwd_kernel(SlimArgs a, SlimFwd o)
     if (b < blocks) next.load(a, b * 16 + (lane & 15), cnt, lane);
     slim_load_w<P, ND>(a, lds);
     const float scale = slim_scale(a);
-    const int base = lds_chunk<kK, 16>(lane & 15, lane >> 4), frags = a.Vp / 16;
+    const int base = lds_chunk<kK, 16>(lane & 15, lane >> 4), frags = a.Vp / 16, q4 = (lane >> 4) * 4;
+    const float* centers = reinterpret_cast<const float*>(lds + P * a.Vp * ND * 64);
     double total = 0.0;
     for (; b < blocks; b += step) {
         const SlimRows<P, ND> r = next;
         const int n = b * 16 + (lane & 15);
         if (b + step < blocks) next.load(a, (b + step) * 16 + (lane & 15), cnt, lane);
-        const int t = MODE == kCE ? a.tgt[n < cnt ? n : cnt - 1] : -1;
+        const int target = MODE == kCE ? a.tgt[n < cnt ? n : cnt - 1] : -1, t = target - q4;      // t: from the lane's first class
         float mx = -INFINITY, s = 0.f, sc = 0.f, tl = 0.f;
         for (int f = 0; f < frags; f += 2) {
             f32x4 l[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) l[u] = slim_logits<T, P, ND>(r, lds, base, f + u, a.Vp, scale);
+            if (f * 16 + 32 > a.V) {       // classes that do not exist
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if ((f + u) * 16 + q4 + e >= a.V) l[u][e] = -INFINITY;
+            }
             float m = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                l[u] = slim_logits<T, P, ND>(r, lds, base, f + u, a.Vp, scale);
-                const int v = (f + u) * 16 + (lane >> 4) * 4;
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if (v + e >= a.V) l[u][e] = -INFINITY;
-                    if (MODE == kCE && v + e == t) tl = l[u][e];
+                    if (MODE == kCE && (f + u) * 16 + e == t) tl = l[u][e];
                     m = fmaxf(m, l[u][e]);      // passes over NaN, which reaches the sum
                 }
-            }
+            // the running maximum moves only where it must: its factor is exp(0) = 1 otherwise
             const float nm = fmaxf(mx, m), ref = nm == -INFINITY ? 0.f : nm, f1 = exp_of(mx - ref);
             s *= f1;
             sc *= f1;
             mx = nm;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const int v = (f + u) * 16 + (lane >> 4) * 4;
+                f32x4 c = {0.f, 0.f, 0.f, 0.f};
+                if (MODE == kExpect) c = *reinterpret_cast<const f32x4*>(centers + (f + u) * 16 + q4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float x = exp_of(l[u][e] - ref);
                     s += x;
-                    if (MODE == kExpect) sc = fmaf(x, a.centers[v + e < a.V ? v + e : a.V - 1], sc);
+                    if (MODE == kExpect) sc = fmaf(x, c[e], sc);
                 }
             }
         }
@@ -959,7 +971,7 @@ __global__ __launch_bounds__(kSlimT) void slim_fwd_kernel(SlimArgs a, SlimFwd o)
             if (MODE == kExpect) {
                 o.out[n] = a.mean[n] = sc / s;
             } else {
-                const float each = t < 0 ? __builtin_nanf("") : (ref - tl) + logf(s);
+                const float each = target < 0 ? __builtin_nanf("") : (ref - tl) + logf(s);
                 if (o.out) o.out[a.rows ? a.rows[n] : n] = each;
                 total += each;
             }
@@ -990,7 +1002,8 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
     const float scale = slim_scale(a), norm = Store<T>::k / dl_norm<T>(o.bs, o.up, MODE, cnt);
     const float back = dl_norm<T>(o.bs, o.up, MODE, cnt) / Store<T>::k *
                        (a.planes_scaled ? 1.f / scale_for(from_bits(a.st->amax_w)) : 1.f);
-    const int base = lds_chunk<kK, 16>(lane & 15, lane >> 4), frags = a.Vp / 16;
+    const int base = lds_chunk<kK, 16>(lane & 15, lane >> 4), frags = a.Vp / 16, q4 = (lane >> 4) * 4;
+    const float* centers = reinterpret_cast<const float*>(lds + P * a.Vp * ND * 64);
     // transposing reads: lane i of a 16-lane group q starts at class 4 q + i / 4, feature 4 (i % 4)
     const int tr = (lane >> 4) * 4 + ((lane >> 2) & 3);
     const int tbase = lds_chunk<kK, 16>(tr, (lane >> 1) & 1) + (lane & 1) * 8;
@@ -1001,9 +1014,9 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
         const int n = b * 16 + (lane & 15), m = n < cnt ? n : cnt - 1;
         if (b + step < blocks) next.load(a, (b + step) * 16 + (lane & 15), cnt, lane);
         const float tp = a.top[m], rs = a.inv_sum[m], e0 = MODE == kExpect ? a.mean[m] : 0.f;
-        const int t = MODE == kCE ? a.tgt[m] : -1;
+        const int target = MODE == kCE ? a.tgt[m] : -1, t = target - q4;
         float g = upstream(o.up, m, cnt) * norm;
-        if (MODE == kCE && t < 0) g = __builtin_nanf("");
+        if (MODE == kCE && target < 0) g = __builtin_nanf("");
         const float gr = g * rs;
         f32x4 acc[2 * ND];
 #pragma unroll
@@ -1013,16 +1026,21 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const f32x4 l = slim_logits<T, P, ND>(r, lds, base, f + u, a.Vp, scale);
-                const int v = (f + u) * 16 + (lane >> 4) * 4;
+                const int v = (f + u) * 16 + q4;
+                f32x4 c = {0.f, 0.f, 0.f, 0.f};
+                if (MODE == kExpect) c = *reinterpret_cast<const f32x4*>(centers + v);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float x = exp_of(l[e] - tp);
-                    float y;
                     if (MODE == kExpect)
-                        y = x * gr * (a.centers[v + e < a.V ? v + e : a.V - 1] - e0);
+                        d[u][e] = x * gr * (c[e] - e0);
                     else
-                        y = v + e == t ? (x * rs - 1.f) * g : x * gr;
-                    d[u][e] = v + e < a.V ? y : 0.f;
+                        d[u][e] = fmaf(x, gr, (f + u) * 16 + e == t ? -g : 0.f);
+                }
+                if (f * 16 + 32 > a.V) {      // classes that do not exist
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (v + e >= a.V) d[u][e] = 0.f;
                 }
                 if (dl && n < cnt && v < o.ld) {
                     const float y[4] = {d[u][0], d[u][1], d[u][2], d[u][3]};
@@ -1300,8 +1318,8 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     const int Vp = (V + 31) & ~31;
     p.slim = D <= 64 ? 2 : D <= 128 ? 4 : D <= 256 ? 8 : 0;
     const long long bytes = (long long)Vp * p.slim * 64 * p.planes;
-    if (bytes > 78 * 1024) p.slim = 0;
-    p.slim_bytes = (int)bytes;
+    if (bytes + Vp * 4 > 78 * 1024) p.slim = 0;
+    p.slim_bytes = (int)bytes + Vp * 4;
     p.slim_grid = cdiv(N, 16 * (kSlimT / 64)) < 2 * cu_count() ? cdiv(N, 16 * (kSlimT / 64)) : 2 * cu_count();
     p.slim_back = p.slim && (long long)N * pad8(V) * (long long)el <= (1ll << 30);
     const bool whole = D % 8 == 0 && ldh % 8 == 0 && dtype != DS_F32;     // rows of the caller's can be read as they are

@@ -73,10 +73,11 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(const O* __restrict__ g
     a = sum_all<256>(a, s);
     if (threadIdx.x == 0) part[blockIdx.y * gridDim.x + blockIdx.x] = a;
 }
+template <int T>
 __device__ __forceinline__ double inverse_norm(const double* part, int blocks, double eps, double* s) {
     double t = 0.0;
-    for (int i = threadIdx.x; i < blocks; i += 256) t += part[i];
-    return 1.0 / (sqrt(sum_all<256>(t, s)) + eps);
+    for (int i = threadIdx.x; i < blocks; i += T) t += part[i];
+    return 1.0 / (sqrt(sum_all<T>(t, s)) + eps);
 }
 
 // G / (|G| + eps) as two planes, rows padded with zeros to np
@@ -84,7 +85,7 @@ __global__ __launch_bounds__(256) void ortho_load_kernel(const void* __restrict_
                                                          const double* __restrict__ part, int blocks, f16* __restrict__ x,
                                                          long long lo, long long per) {
     __shared__ double s[4];
-    const double inv = inverse_norm(part + (long long)blockIdx.y * blocks, blocks, eps, s) * kXs;
+    const double inv = inverse_norm<256>(part + (long long)blockIdx.y * blocks, blocks, eps, s) * kXs;
     const long long base = (long long)blockIdx.y * m * n;
     f16* y = x + blockIdx.y * per;
     const unsigned q = np / 4;
@@ -378,6 +379,39 @@ struct SmallArgs {
     double eps;
     float ca, cb, cc, bs;     // as UseArgs of kPoly; B's scale
 };
+// b: this wave's fragments of X X^T (2^26 of it); leaves the polynomial B in A's place
+template <int NA>
+__device__ __forceinline__ void gram_to_poly(const Planes& A, const Share& sq, int s, int sp, int lane, const SmallArgs& a,
+                                             f32x4 (&b)[NA]) {
+    const int r = sq.row * 16 + (lane & 15), q = (lane >> 4) * 4;
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+        if (sq.mine(i)) {
+            const float v[4] = {b[i][0] * (1.f / kXs), b[i][1] * (1.f / kXs), b[i][2] * (1.f / kXs), b[i][3] * (1.f / kXs)};
+            put4<3>(A.hi + r * A.pitch + sq.c0(i) + q, A.lo - A.hi, v);
+        }
+    __syncthreads();
+    small_product<false, NA>(A, A, sq, sp, lane, b);
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+        if (sq.mine(i)) {
+            const int c = sq.c0(i) + q;
+            const f16x4 h = *reinterpret_cast<const f16x4*>(A.hi + r * A.pitch + c);
+            const f16x4 w = *reinterpret_cast<const f16x4*>(A.lo + r * A.pitch + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                b[i][e] = fmaf(a.cc, b[i][e], a.cb * ((float)h[e] + (float)w[e])) + (c + e == r && r < s ? a.ca : 0.f);
+        }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+        if (sq.mine(i)) {
+            const float v[4] = {b[i][0], b[i][1], b[i][2], b[i][3]};
+            put4<3>(A.hi + r * A.pitch + sq.c0(i) + q, A.lo - A.hi, v);
+        }
+    __syncthreads();
+}
+
 // NA, NX: fragments a wave holds of the square products and of X
 template <class O, int NA, int NX>
 __global__ __launch_bounds__(kSmallT) void ortho_small_kernel(const O* __restrict__ g, O* __restrict__ out, SmallArgs a) {
@@ -432,32 +466,7 @@ __global__ __launch_bounds__(kSmallT) void ortho_small_kernel(const O* __restric
     for (int step = 0; step < a.steps; ++step) {
         f32x4 b[NA];
         small_product<false, NA>(X, X, sq, p.lp, lane, b);
-#pragma unroll
-        for (int i = 0; i < NA; ++i)
-            if (sq.mine(i)) {
-                const float v[4] = {b[i][0] * (1.f / kXs), b[i][1] * (1.f / kXs), b[i][2] * (1.f / kXs), b[i][3] * (1.f / kXs)};
-                put4<3>(A.hi + r * p.pa + sq.c0(i) + q, A.lo - A.hi, v);
-            }
-        __syncthreads();
-        small_product<false, NA>(A, A, sq, p.sp, lane, b);
-#pragma unroll
-        for (int i = 0; i < NA; ++i)
-            if (sq.mine(i)) {
-                const int c = sq.c0(i) + q;
-                const f16x4 h = *reinterpret_cast<const f16x4*>(A.hi + r * p.pa + c);
-                const f16x4 w = *reinterpret_cast<const f16x4*>(A.lo + r * p.pa + c);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    b[i][e] = fmaf(a.cc, b[i][e], a.cb * ((float)h[e] + (float)w[e])) + (c + e == r && r < s ? a.ca : 0.f);
-            }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < NA; ++i)
-            if (sq.mine(i)) {
-                const float v[4] = {b[i][0], b[i][1], b[i][2], b[i][3]};
-                put4<3>(A.hi + r * p.pa + sq.c0(i) + q, A.lo - A.hi, v);
-            }
-        __syncthreads();
+        gram_to_poly<NA>(A, sq, s, p.sp, lane, a, b);
         f32x4 x[NX];
         small_product<true, NX>(A, X, sx, p.sp, lane, x);
         const bool last = step + 1 == a.steps;
@@ -481,12 +490,111 @@ __global__ __launch_bounds__(kSmallT) void ortho_small_kernel(const O* __restric
     }
 }
 
+// ---- a small side of up to 64 and a longer other one: a launch a step ---------------------------------------------------
+//
+// A workgroup owns a slab of X's columns.  A launch adds all slabs' parts of A = X X^T (every workgroup for itself: 16 KB a slab
+// at s = 64), forms B from it, multiplies its slab and leaves the slab's part of the next A.  What bounds a step is its chain
+// of latencies, 9 us, once instead of the 3 to 5 times of separate products: 64 x 576 in 5 steps 98 -> 56 us.
+struct SlabArgs {
+    SmallArgs a;
+    int w, slabs, first, last;      // columns of a slab, a multiple of 32
+    const double* norm;
+    int blocks;
+    f16* x;                         // [matrix][slab][plane][sp][w]
+    const f32x4* old;               // parts of A: [matrix][slab][fragment of a wave][thread]
+    f32x4* part;
+};
+template <class O, int NA, int NX>
+__global__ __launch_bounds__(kSmallT) void ortho_slab_kernel(const O* __restrict__ g, O* __restrict__ out, SlabArgs p) {
+    extern __shared__ __align__(16) char lds[];
+    __shared__ double red[kSmallT / 64];
+    const SmallArgs& a = p.a;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const bool wide = a.m <= a.n;
+    const int s = wide ? a.m : a.n, l = wide ? a.n : a.m, sp = (s + 31) & ~31, px = p.w + 8, pa = sp + 8;
+    const int c_beg = blockIdx.x * p.w, wc = min(p.w, l - c_beg), slab = blockIdx.y * p.slabs + blockIdx.x;
+    Planes X{reinterpret_cast<f16*>(lds), reinterpret_cast<f16*>(lds) + sp * px, px};
+    Planes A{X.lo + sp * px, X.lo + sp * (px + pa), pa};
+    f16* keep = p.x + (long long)slab * 2 * sp * p.w;
+    const O* gm = g + (long long)blockIdx.y * a.m * a.n;
+    O* om = out + (long long)blockIdx.y * a.m * a.n;
+    const int ns = sp / 16, nl = p.w / 16;
+    const Share sq(wave, ns, ns), sx(wave, ns, nl);
+    const int r = sq.row * 16 + (lane & 15), q = (lane >> 4) * 4;
+    f32x4 b[NA];
+    if (p.first) {
+        for (int i = tid; i < sp * px / 2; i += kSmallT) reinterpret_cast<int*>(X.hi)[i] = reinterpret_cast<int*>(X.lo)[i] = 0;
+        const double inv = inverse_norm<kSmallT>(p.norm + (long long)blockIdx.y * p.blocks, p.blocks, a.eps, red) * kXs;
+        // the matrix's own rows along the lanes
+        const int rows = wide ? s : wc, cols = wide ? wc : s;
+        const O* src = gm + (wide ? (long long)c_beg : (long long)c_beg * a.n);
+        for (int y = wave; y < rows; y += kSmallT / 64)
+#pragma unroll 4
+            for (int x = lane; x < cols; x += 64) {
+                f16 h, w;
+                split16((float)((float)src[(long long)y * a.n + x] * inv), h, w);
+                const int at = wide ? y * px + x : x * px + y;
+                X.hi[at] = h;
+                X.lo[at] = w;
+            }
+    } else {
+        for (int i = tid; i < sp * p.w / 4; i += kSmallT) {      // chunks of 8, both planes
+            const int plane = i >= sp * p.w / 8, k = i - (plane ? sp * p.w / 8 : 0), y = k / (p.w / 8), x = k % (p.w / 8) * 8;
+            *reinterpret_cast<i32x4*>((plane ? X.lo : X.hi) + y * px + x) =
+                *reinterpret_cast<const i32x4*>(keep + (plane ? sp * p.w : 0) + y * p.w + x);
+        }
+#pragma unroll
+        for (int i = 0; i < NA; ++i) b[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const f32x4* old = p.old + (long long)blockIdx.y * p.slabs * NA * kSmallT + tid;
+#pragma unroll 2
+        for (int j = 0; j < p.slabs; ++j)
+#pragma unroll
+            for (int i = 0; i < NA; ++i) b[i] += old[(j * NA + i) * kSmallT];
+        gram_to_poly<NA>(A, sq, s, sp, lane, a, b);
+        f32x4 x[NX];
+        small_product<true, NX>(A, X, sx, sp, lane, x);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NX; ++i)
+            if (sx.mine(i)) {
+                const int c = sx.c0(i) + q;
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = x[i][e] * (p.last ? 1.f / (a.bs * kXs) : 1.f / a.bs);
+                if (!p.last) {
+                    put4<3>(X.hi + r * px + c, X.lo - X.hi, v);
+                    put4<3>(keep + r * p.w + c, sp * p.w, v);
+                } else if (r < s) {
+                    if (wide) {
+                        put_row4(om + (long long)r * a.n + c_beg, c, wc, v);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (c + e < wc) om[(long long)(c_beg + c + e) * a.n + r] = (O)v[e];
+                    }
+                }
+            }
+        if (p.last) return;
+    }
+    __syncthreads();
+    if (p.first)
+        for (int i = tid; i < sp * p.w / 4; i += kSmallT) {
+            const int plane = i >= sp * p.w / 8, k = i - (plane ? sp * p.w / 8 : 0), y = k / (p.w / 8), x = k % (p.w / 8) * 8;
+            *reinterpret_cast<i32x4*>(keep + (plane ? sp * p.w : 0) + y * p.w + x) =
+                *reinterpret_cast<const i32x4*>((plane ? X.lo : X.hi) + y * px + x);
+        }
+    small_product<false, NA>(X, X, sq, p.w, lane, b);
+    f32x4* to = p.part + (long long)slab * NA * kSmallT + tid;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) to[i * kSmallT] = b[i];
+}
+
 template <class O>
 __global__ __launch_bounds__(256) void ortho_only_scale_kernel(const void* __restrict__ g, double eps,
                                                                const double* __restrict__ part, int blocks, long long mn,
                                                                void* __restrict__ out) {
     __shared__ double s[4];
-    const double inv = inverse_norm(part + (long long)blockIdx.y * blocks, blocks, eps, s);
+    const double inv = inverse_norm<256>(part + (long long)blockIdx.y * blocks, blocks, eps, s);
     const long long base = blockIdx.y * mn;
     for (long long i = blockIdx.x * 256ll + threadIdx.x; i < mn; i += gridDim.x * 256ll)
         static_cast<O*>(out)[base + i] = (O)(float)((float)static_cast<const O*>(g)[base + i] * inv);
@@ -495,7 +603,8 @@ __global__ __launch_bounds__(256) void ortho_only_scale_kernel(const void* __res
 struct OrthoPlan {
     int s, l, sp, np, blocks;                 // smaller and larger side; row pitch of A and of X
     Cut gram, poly, apply;
-    bool light;
+    bool light, small;
+    int slab, slabs;                          // columns of a slab (0: not that path), slabs
     size_t norm, x0, x1, a, b, da, part, total;
 };
 int tiles_of(ShapeId id, int M, int N, bool tri) {
@@ -531,8 +640,22 @@ OrthoPlan ortho_plan(int dtype, int batch, int m, int n) {
     if (q > part) part = q;
     q = part_bytes(p.apply, n, m, false, batch);
     if (q > part) part = q;
+    p.small = small_fits(p.s, p.l);
+    const int s32 = (p.s + 31) & ~31;
+    // (at s = 128 the parts are 64 KB a slab and the products of a slab 8 us: no gain over separate launches)
+    p.slab = p.small || s32 > 64 ? 0 : p.l > 4096 ? 256 : 128;
+    p.slabs = p.slab ? cdiv(p.l, p.slab) : 0;
+    if ((size_t)p.slabs * s32 * s32 * 4 > (1u << 20)) p.slab = 0;       // parts that every workgroup reads
     size_t o = 0;
     p.norm = o; o += align256((size_t)batch * p.blocks * 8);
+    if (p.small || p.slab) {
+        p.x0 = o; o += align256((size_t)batch * p.slabs * s32 * p.slab * 4);
+        const size_t parts = align256((size_t)batch * p.slabs * 2 * kSmallT * 16);
+        p.a = o; o += parts;
+        p.b = o; o += parts;
+        p.x1 = p.da = p.part = p.total = o;
+        return p;
+    }
     p.x0 = o; o += x;
     p.x1 = o; o += x;
     p.a = o; o += a;
@@ -635,13 +758,39 @@ int small_launch(const void* g, void* out, int batch, const SmallArgs& a, int by
     return e == hipSuccess ? DS_OK : (int)e;
 }
 
+template <class O, int NA, int NX>
+int slab_launch(const OrthoPlan& p, const void* g, void* out, int batch, const SmallArgs& a, char* ws, hipStream_t q) {
+    const int s32 = (p.s + 31) & ~31, bytes = 4 * s32 * (p.slab + 8 + s32 + 8);
+    if (bytes > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&ortho_slab_kernel<O, NA, NX>),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != hipSuccess) return (int)e;
+    }
+    f32x4* parts[2] = {reinterpret_cast<f32x4*>(ws + p.a), reinterpret_cast<f32x4*>(ws + p.b)};
+    double* norm = reinterpret_cast<double*>(ws + p.norm);
+    ortho_norm_kernel<O><<<dim3(p.blocks, batch), 256, 0, q>>>(static_cast<const O*>(g), (long long)a.m * a.n, norm);
+    for (int i = 0; i <= a.steps; ++i) {
+        const SlabArgs b{a, p.slab, p.slabs, i == 0, i == a.steps, norm, p.blocks, reinterpret_cast<f16*>(ws + p.x0),
+                         parts[(i + 1) & 1], parts[i & 1]};
+        ortho_slab_kernel<O, NA, NX><<<dim3(p.slabs, batch), kSmallT, bytes, q>>>(static_cast<const O*>(g), static_cast<O*>(out), b);
+    }
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? DS_OK : (int)e;
+}
+
 template <class O>
 int ortho_any(const OrthoPlan& p, const void* g, int dtype, int batch, int m, int n, int steps, const double* co, double eps,
               void* out, char* ws, hipStream_t q) {
-    if (steps > 0 && small_fits(p.s, p.l)) {
+    if (steps > 0 && (p.small || p.slab)) {
         const float bs = b_scale(co);
         const SmallArgs a{m, n, steps, eps, (float)(co[0] * bs), (float)(co[1] * bs / kXs), (float)(co[2] * bs / (kXs * kXs)), bs};
         const SmallPlan sp = small_plan(p.s, p.l);
+        if (p.slab) {
+            const int nx = cdiv(p.slab / 16, kSmallT / 64 / (sp.sp / 16));
+            return nx <= 2   ? slab_launch<O, 2, 2>(p, g, out, batch, a, ws, q)
+                   : nx <= 5 ? slab_launch<O, 2, 5>(p, g, out, batch, a, ws, q)
+                             : slab_launch<O, 2, 10>(p, g, out, batch, a, ws, q);
+        }
         const int nx = cdiv(sp.lp / 16, kSmallT / 64 / (sp.sp / 16));      // fragments of X a wave holds
         if (sp.sp > 64) return small_launch<O, 8, 8>(g, out, batch, a, sp.bytes, q);
         return nx <= 2   ? small_launch<O, 2, 2>(g, out, batch, a, sp.bytes, q)
