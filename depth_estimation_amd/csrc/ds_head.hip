@@ -219,29 +219,42 @@ __global__ __launch_bounds__(256) void amax_kernel(const IT* __restrict__ x, lon
     }
 }
 
-// rows of x (listed in `rows` if given) packed with a row pitch of Dp elements, zero behind D; fp32 as two scaled fp16 planes
+// Rows of one or two matrices (one launch) packed with a row pitch of Dp elements, zero behind D; fp32 as two scaled fp16
+// planes.  Workgroups [first, first + blocks) take a source.
+struct Source {
+    const void* x;
+    long long ld;
+    const int* rows;           // listed rows (NULL: in order)
+    const int* cnt;            // how many, on the device (NULL: n)
+    int n;
+    const unsigned* amax;
+    void* y;
+    long long lo;
+    int first, blocks;         // blocks 0: not there
+};
 template <class IT, class T, int SPLIT, int VEC>
-__global__ __launch_bounds__(256) void stage_kernel(const IT* __restrict__ x, long long ld, const int* __restrict__ rows,
-                                                    const int* __restrict__ cnt, int n, int D, int Dp, int L,
-                                                    const unsigned* __restrict__ amax, T* __restrict__ y, long long lo) {
-    const int c = cnt ? *cnt : n;
+__global__ __launch_bounds__(256) void stage_kernel(Source s0, Source s1, int D, int Dp, int L) {
+    const bool second = s1.blocks > 0 && (int)blockIdx.x >= s1.first;
+    const Source& s = second ? s1 : s0;
+    const IT* x = static_cast<const IT*>(s.x);
+    const int c = s.cnt ? *s.cnt : s.n;
     const int lane = threadIdx.x & 63, sub = lane & (L - 1), R = 64 / L;
-    const float scale = SPLIT == 3 ? scale_for(from_bits(*amax)) : 1.f;
+    const float scale = SPLIT == 3 ? scale_for(from_bits(*s.amax)) : 1.f;
     constexpr int U = 4;
-    const int hop = gridDim.x * 4 * R;
-    for (int r0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * R + lane / L; r0 < c; r0 += hop * U)
+    const int hop = s.blocks * 4 * R;
+    for (int r0 = (((int)blockIdx.x - s.first) * 4 + (threadIdx.x >> 6)) * R + lane / L; r0 < c; r0 += hop * U)
         for (int d = sub * VEC; d < Dp; d += L * VEC) {
             IT v[U][VEC];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int r = min(r0 + u * hop, c - 1);
-                load_vec<IT, VEC>(x + (rows ? rows[r] : r) * ld, d, D, v[u]);
+                load_vec<IT, VEC>(x + (s.rows ? s.rows[r] : r) * s.ld, d, D, v[u]);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int r = r0 + u * hop;
                 if (r >= c) break;
-                T* q = y + (long long)r * Dp + d;
+                T* q = static_cast<T*>(s.y) + (long long)r * Dp + d;
                 typename Vec<T, VEC>::type h, l;
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
@@ -255,7 +268,7 @@ __global__ __launch_bounds__(256) void stage_kernel(const IT* __restrict__ x, lo
                     }
                 }
                 *reinterpret_cast<typename Vec<T, VEC>::type*>(q) = h;
-                if (SPLIT == 3) *reinterpret_cast<typename Vec<T, VEC>::type*>(q + lo) = l;
+                if (SPLIT == 3) *reinterpret_cast<typename Vec<T, VEC>::type*>(q + s.lo) = l;
             }
         }
 }
@@ -759,32 +772,40 @@ __global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__
     }
 }
 
-// rows that were left out have no gradient
-template <class O, int VEC>
-__global__ __launch_bounds__(256) void zero_ignored_kernel(const long long* __restrict__ target, int n, long long ignore, int D,
-                                                           int L, const HeadState* __restrict__ st, O* __restrict__ out) {
-    if (st->count == n) return;
-    const int lane = threadIdx.x & 63, sub = lane & (L - 1), R = 64 / L, hop = gridDim.x * 4 * R;
-    constexpr int U = 4;
-    for (int r0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * R + lane / L; r0 < n; r0 += hop * U) {
+// Rows that were left out have no gradient.  Waves w, w + waves, .. of a launch.
+struct Ignored {
+    const long long* target;     // NULL: nothing to do
+    int n, L, vec;
+    long long ignore;
+};
+template <class O>
+__device__ __forceinline__ void zero_ignored(const Ignored& g, int D, const HeadState* st, O* out, int w, int waves) {
+    if (!g.target || st->count == g.n) return;
+    constexpr int VEC = 16 / sizeof(O), U = 4;
+    const int lane = threadIdx.x & 63, sub = lane & (g.L - 1), R = 64 / g.L, hop = waves * R;
+    for (int r0 = w * R + lane / g.L; r0 < g.n; r0 += hop * U) {
         long long t[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) t[u] = target[min(r0 + u * hop, n - 1)];
+        for (int u = 0; u < U; ++u) t[u] = g.target[min(r0 + u * hop, g.n - 1)];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (r0 + u * hop < n && t[u] == ignore)
-                for (int d = sub * VEC; d < D; d += L * VEC) {
-                    O* q = out + (long long)(r0 + u * hop) * D + d;
-                    if constexpr (VEC == 1) {
-                        *q = (O)0.f;
-                    } else {
-                        typename Vec<O, VEC>::type z;
+            if (r0 + u * hop < g.n && t[u] == g.ignore) {
+                O* q = out + (long long)(r0 + u * hop) * D;
+                if (g.vec) {
+                    typename Vec<O, VEC>::type z;
 #pragma unroll
-                        for (int e = 0; e < VEC; ++e) z[e] = (O)0.f;
-                        *reinterpret_cast<typename Vec<O, VEC>::type*>(q) = z;
-                    }
+                    for (int e = 0; e < VEC; ++e) z[e] = (O)0.f;
+                    for (int d = sub * VEC; d < D; d += g.L * VEC) *reinterpret_cast<typename Vec<O, VEC>::type*>(q + d) = z;
+                } else {
+                    for (int d = sub; d < D; d += g.L) q[d] = (O)0.f;
                 }
+            }
     }
+}
+template <class O>
+__global__ __launch_bounds__(256) void zero_ignored_kernel(Ignored g, int D, const HeadState* __restrict__ st,
+                                                           O* __restrict__ out) {
+    zero_ignored(g, D, st, out, blockIdx.x * 4 + (threadIdx.x >> 6), gridDim.x * 4);
 }
 
 // ------------------------------------------------------------------------------------------------------ small heads
@@ -821,6 +842,7 @@ struct SlimBwd {
     void* dl;                  // NULL: dW not wanted
     int ld;
     long long lo;
+    Ignored ignored;           // the caller's rows that were left out (with g_hidden)
     void* packed;              // kept rows' features written densely for dW (NULL: they lie so already), pitch Dp
     int Dp;
 };
@@ -1099,6 +1121,8 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
             }
         }
     }
+    if (o.g_hidden)
+        zero_ignored(o.ignored, a.D, a.st, static_cast<O*>(o.g_hidden), blockIdx.x * (kSlimT / 64) + wave, gridDim.x * (kSlimT / 64));
 }
 
 // ----------------------------------------------------------------------------------------------------------- few rows
@@ -1376,13 +1400,6 @@ int launched() {
     return e == hipSuccess ? DS_OK : (int)e;
 }
 
-template <class IT, class T, int SPLIT>
-void stage(const IT* x, long long ld, const int* rows, const int* cnt, long long n, int D, int Dp, const unsigned* amax, T* y,
-           long long lo, hipStream_t q) {
-    constexpr int VEC = 16 / sizeof(IT);
-    const int L = lanes_for(cdiv(Dp, VEC)), blocks = cdiv(n, 4 * 64 / L * 2), grid = blocks < 4096 ? blocks : 4096;
-    stage_kernel<IT, T, SPLIT, VEC><<<grid, 256, 0, q>>>(x, ld, rows, cnt, (int)n, D, Dp, L, amax, y, lo);
-}
 // scales of fp32 inputs (st->amax_h, amax_w; zeroed before)
 template <class IT>
 void scales(const IT* hidden, long long ldh, const int* rows, const IT* weight, long long N, int D, int V, HeadState* st,
@@ -1400,16 +1417,25 @@ void operands(const Plan& p, const IT* hidden, long long ldh, const IT* weight, 
         if (need_scales) scales(hidden, ldh, rows, weight, N, D, V, s.st, q);
     H = Operand{hidden, ldh, 0, (int)N, D};
     W = Operand{weight, D, 0, V, D};
+    constexpr int VEC = 16 / sizeof(IT);
+    const int L = lanes_for(cdiv(p.Dp, VEC));
+    auto blocks = [&](long long n) {
+        const int b = cdiv(n, 4 * 64 / L * 2);
+        return b < 4096 ? b : 4096;
+    };
+    Source a{}, b{};
     if (p.stage_h) {
         const long long lo = N * p.Dp;
-        stage<IT, T, SPLIT>(hidden, ldh, rows, &s.st->count, N, D, p.Dp, &s.st->amax_h, reinterpret_cast<T*>(wh), lo, q);
+        a = Source{hidden, ldh, rows, &s.st->count, (int)N, &s.st->amax_h, wh, lo, 0, blocks(N)};
         H = Operand{wh, p.Dp, lo, (int)N, p.Dp};
     }
     if (p.stage_w) {
         const long long lo = (long long)V * p.Dp;
-        stage<IT, T, SPLIT>(weight, D, nullptr, nullptr, V, D, p.Dp, &s.st->amax_w, reinterpret_cast<T*>(ww), lo, q);
+        b = Source{weight, D, nullptr, nullptr, V, &s.st->amax_w, ww, lo, a.blocks, blocks(V)};
         W = Operand{ww, p.Dp, lo, V, p.Dp};
     }
+    if (a.blocks + b.blocks > 0)
+        stage_kernel<IT, T, SPLIT, VEC><<<a.blocks + b.blocks, 256, 0, q>>>(a.blocks ? a : b, a.blocks ? b : Source{}, D, p.Dp, L);
 }
 
 template <class K>
@@ -1602,14 +1628,14 @@ int head_bwd(int mode, const IT* hidden, long long ldh, const IT* weight, const 
     if (need_scales && mode == kExpect) head_init_kernel<<<1, 1, 0, q>>>(s.st, (int)N);
     Operand H, W;
     operands<IT, T, SPLIT>(p, hidden, ldh, weight, N, D, V, s, rows, need_scales, ws + p.bh, ws + p.bw, H, W, q);
+    Ignored ignored{};
     if (mode == kCE && g_hidden) {
         constexpr int VEC = 16 / sizeof(IT);
-        const bool v = D % VEC == 0;
-        const int L = lanes_for(v ? D / VEC : D), blocks = cdiv(N, 4 * 64 / L * 4), grid = blocks < 4096 ? blocks : 4096;
-        if (v)
-            zero_ignored_kernel<IT, VEC><<<grid, 256, 0, q>>>(target, (int)N, ignore, D, L, s.st, g_hidden);
-        else
-            zero_ignored_kernel<IT, 1><<<grid, 256, 0, q>>>(target, (int)N, ignore, D, L, s.st, g_hidden);
+        ignored = Ignored{target, (int)N, lanes_for(D % VEC == 0 ? D / VEC : D), D % VEC == 0, ignore};
+        if (!p.slim_back) {
+            const int blocks = cdiv(N, 4 * 64 / ignored.L * 4);
+            zero_ignored_kernel<IT><<<blocks < 4096 ? blocks : 4096, 256, 0, q>>>(ignored, D, s.st, g_hidden);
+        }
     }
     T* dl = reinterpret_cast<T*>(ws + p.dl);
     float* dhp = reinterpret_cast<float*>(ws + p.dhp);
@@ -1623,7 +1649,7 @@ int head_bwd(int mode, const IT* hidden, long long ldh, const IT* weight, const 
         Wp.outer = cols;
         if (p.slim_back) {
             const SlimArgs a = slim_args(p, H, W, s, rows, N, D, V, centers);
-            const SlimBwd o{bs, up, g_hidden, g_weight ? dl : nullptr, ld, lo, g_weight && p.pack ? ws + p.bh : nullptr, p.Dp};
+            const SlimBwd o{bs, up, g_hidden, g_weight ? dl : nullptr, ld, lo, ignored, g_weight && p.pack ? ws + p.bh : nullptr, p.Dp};
             const int rc = mode == kCE ? slim_bwd<T, SPLIT == 3 ? 2 : 1, kCE, IT>(p, a, o, q)
                                        : slim_bwd<T, SPLIT == 3 ? 2 : 1, kExpect, IT>(p, a, o, q);
             if (rc) return rc;

@@ -654,7 +654,7 @@ def _head_args(hidden, weight):
         raise RuntimeError(f"hidden and weight must have one dtype, got {hidden.dtype} and {weight.dtype}")
     L.same_device(hidden, weight)
     d = weight.shape[1]
-    h = hidden.reshape(-1, d)
+    h = hidden if hidden.dim() == 2 else hidden.reshape(-1, d)
     if h.shape[0] > 1 and (h.stride(0) < d or (d > 1 and h.stride(1) != 1)) or (d > 1 and h.stride(1) != 1):
         h = h.contiguous()
     h = _aligned(h)
