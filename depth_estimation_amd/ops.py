@@ -7,9 +7,11 @@ Outputs and workspaces are torch tensors allocated here; the kernels never alloc
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 
@@ -638,7 +640,18 @@ def resize_bicubic(x: torch.Tensor, size) -> torch.Tensor:
 # Scratch memory of these calls is allocated per call instead of taken from L.workspace: it can be large, and a buffer
 # allocated during a graph capture belongs to that graph alone (two captured graphs that shared one would race on replay).
 def _scratch(nbytes: int, device) -> torch.Tensor:
-    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+    return torch.empty(nbytes if nbytes > 16 else 16, dtype=torch.uint8, device=device)
+
+
+# what a call needs depends on sizes alone; asked for once per size (a small training step is bound by the host)
+@functools.lru_cache(maxsize=1024)
+def _head_bytes(which: str, code: int, n: int, d: int, v: int, ldh: int, backward: int) -> int:
+    return int(getattr(L.lib(), which)(code, n, d, v, ldh, backward))
+
+
+@functools.lru_cache(maxsize=1024)
+def _saved_bytes(n: int) -> int:
+    return int(L.lib().ds_head_saved_bytes(n))
 
 
 def _aligned(t):
@@ -648,42 +661,52 @@ def _aligned(t):
 def _head_args(hidden, weight):
     """-> hidden as (N,D) with unit column stride (a view where the strides allow it), its row pitch, weight contiguous."""
     hidden, weight = L.dev_float(hidden, "hidden"), L.dev_float(weight, "weight")
-    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or 0 in weight.shape:
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or weight.numel() == 0:
         raise RuntimeError(f"expected hidden (...,D) and weight (V,D); got {tuple(hidden.shape)}, {tuple(weight.shape)}")
     if hidden.dtype != weight.dtype:
         raise RuntimeError(f"hidden and weight must have one dtype, got {hidden.dtype} and {weight.dtype}")
     L.same_device(hidden, weight)
-    d = weight.shape[1]
-    h = hidden if hidden.dim() == 2 else hidden.reshape(-1, d)
-    if h.shape[0] > 1 and (h.stride(0) < d or (d > 1 and h.stride(1) != 1)) or (d > 1 and h.stride(1) != 1):
+    h = hidden if hidden.dim() == 2 else hidden.reshape(-1, weight.shape[1])
+    n, d = h.shape
+    if not h.is_contiguous() and ((d > 1 and h.stride(1) != 1) or (n > 1 and h.stride(0) < d)):
         h = h.contiguous()
     h = _aligned(h)
-    return h, (h.stride(0) if h.shape[0] > 1 else d), _aligned(weight.contiguous())
+    return h, n, d, (h.stride(0) if n > 1 else d), _aligned(weight.contiguous())
+
+
+def _head_grads(ctx, h, w):
+    """uninitialised gradients of the inputs that need one; zero for the weight where there are no rows"""
+    gh = torch.empty(h.shape, dtype=h.dtype, device=h.device) if ctx.needs_input_grad[0] else None
+    gw = None
+    if ctx.needs_input_grad[1]:
+        gw = torch.empty_like(w) if h.shape[0] else torch.zeros_like(w)
+    return gh, gw
 
 
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+_INTEGERS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 
 
 class _LinearCE(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, ignore_index, reduction):
-        h, ldh, w = _head_args(hidden, weight)
-        if not isinstance(targets, torch.Tensor) or targets.dtype.is_floating_point or targets.dtype.is_complex or \
-                targets.dtype == torch.bool:
+        h, n, d, ldh, w = _head_args(hidden, weight)
+        if not isinstance(targets, torch.Tensor) or targets.dtype not in _INTEGERS:
             raise RuntimeError("targets must be a tensor of integers")
         if targets.shape != hidden.shape[:-1]:
             raise RuntimeError(f"targets must be {tuple(hidden.shape[:-1])}, got {tuple(targets.shape)}")
         L.same_device(h, targets)
-        t = targets.to(torch.int64).contiguous()
-        (n, d), v, lib = h.shape, w.shape[0], L.lib()
-        dev, code, red = h.device, L.DTYPES[h.dtype], _REDUCTIONS[reduction]
+        t = targets if targets.dtype == torch.int64 else targets.to(torch.int64)
+        t = t.contiguous()
+        v, lib, dev = w.shape[0], L.lib(), h.device
+        code, red = L.DTYPES[h.dtype], _REDUCTIONS[reduction]
         out = torch.empty(targets.shape if red == 0 else (), dtype=torch.float32, device=dev)
-        saved = _scratch(lib.ds_head_saved_bytes(n), dev)
+        saved = _scratch(_saved_bytes(n), dev)
         if n == 0:
             if red:
                 out.fill_(0.0 if red == 1 else float("nan"))
         else:
-            nb = lib.ds_linear_ce_workspace_bytes(code, n, d, v, ldh, 0)
+            nb = _head_bytes("ds_linear_ce_workspace_bytes", code, n, d, v, ldh, 0)
             ws = _scratch(nb, dev)
             L.check(lib.ds_linear_ce_fwd(h.data_ptr(), ldh, w.data_ptr(), t.data_ptr(), code, n, d, v, ignore_index, red,
                                          out.data_ptr(), saved.data_ptr(), ws.data_ptr(), nb, L.stream()), "ds_linear_ce_fwd")
@@ -692,25 +715,21 @@ class _LinearCE(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, g):
         h, w, t, saved = ctx.saved_tensors
         ldh, ignore_index, red, shape = ctx.args
-        (n, d), v, lib = h.shape, w.shape[0], L.lib()
-        code = L.DTYPES[h.dtype]
-        g = L.dev_f32(g, "grad")
-        gh = torch.empty(n, d, dtype=h.dtype, device=h.device) if ctx.needs_input_grad[0] else None
-        gw = torch.empty(v, d, dtype=h.dtype, device=h.device) if ctx.needs_input_grad[1] else None
-        if n == 0:
-            gw = None if gw is None else gw.zero_()
-        elif gh is not None or gw is not None:
-            L.same_device(h, w, g)
-            nb = lib.ds_linear_ce_workspace_bytes(code, n, d, v, ldh, 1)
+        (n, d), v = h.shape, w.shape[0]
+        gh, gw = _head_grads(ctx, h, w)
+        if n and (gh is not None or gw is not None):
+            code, lib, g = L.DTYPES[h.dtype], L.lib(), L.dev_f32(g, "grad")
+            L.same_device(h, g)
+            nb = _head_bytes("ds_linear_ce_workspace_bytes", code, n, d, v, ldh, 1)
             ws = _scratch(nb, h.device)
             L.check(lib.ds_linear_ce_bwd(h.data_ptr(), ldh, w.data_ptr(), t.data_ptr(), g.data_ptr(), code, n, d, v,
                                          ignore_index, red, saved.data_ptr(), L.ptr(gh), L.ptr(gw), ws.data_ptr(), nb,
                                          L.stream()), "ds_linear_ce_bwd")
-        return None if gh is None else gh.reshape(shape), gw, None, None, None
+        return gh if gh is None or len(shape) == 2 else gh.reshape(shape), gw, None, None, None
 
 
 def linear_cross_entropy(hidden, weight, targets, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
@@ -724,17 +743,16 @@ def linear_cross_entropy(hidden, weight, targets, ignore_index: int = -100, redu
 class _BinExpect(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, centers):
-        h, ldh, w = _head_args(hidden, weight)
+        h, n, d, ldh, w = _head_args(hidden, weight)
         c = L.dev_f32(centers, "centers")
-        (n, d), v, lib = h.shape, w.shape[0], L.lib()
+        v, lib, dev, code = w.shape[0], L.lib(), h.device, L.DTYPES[h.dtype]
         if c.shape != (v,):
             raise RuntimeError(f"centers must be ({v},), got {tuple(c.shape)}")
         L.same_device(h, c)
-        dev, code = h.device, L.DTYPES[h.dtype]
         out = torch.empty(hidden.shape[:-1], dtype=torch.float32, device=dev)
-        saved = _scratch(lib.ds_head_saved_bytes(n), dev)
+        saved = _scratch(_saved_bytes(n), dev)
         if n:
-            nb = lib.ds_bin_expect_workspace_bytes(code, n, d, v, ldh, 0)
+            nb = _head_bytes("ds_bin_expect_workspace_bytes", code, n, d, v, ldh, 0)
             ws = _scratch(nb, dev)
             L.check(lib.ds_bin_expect_fwd(h.data_ptr(), ldh, w.data_ptr(), c.data_ptr(), code, n, d, v, out.data_ptr(),
                                           saved.data_ptr(), ws.data_ptr(), nb, L.stream()), "ds_bin_expect_fwd")
@@ -743,25 +761,21 @@ class _BinExpect(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, g):
         h, w, c, saved = ctx.saved_tensors
         ldh, shape = ctx.args
-        (n, d), v, lib = h.shape, w.shape[0], L.lib()
-        code = L.DTYPES[h.dtype]
-        g = L.dev_f32(g, "grad")
-        gh = torch.empty(n, d, dtype=h.dtype, device=h.device) if ctx.needs_input_grad[0] else None
-        gw = torch.empty(v, d, dtype=h.dtype, device=h.device) if ctx.needs_input_grad[1] else None
-        if n == 0:
-            gw = None if gw is None else gw.zero_()
-        elif gh is not None or gw is not None:
-            L.same_device(h, w, g)
-            nb = lib.ds_bin_expect_workspace_bytes(code, n, d, v, ldh, 1)
+        (n, d), v = h.shape, w.shape[0]
+        gh, gw = _head_grads(ctx, h, w)
+        if n and (gh is not None or gw is not None):
+            code, lib, g = L.DTYPES[h.dtype], L.lib(), L.dev_f32(g, "grad")
+            L.same_device(h, g)
+            nb = _head_bytes("ds_bin_expect_workspace_bytes", code, n, d, v, ldh, 1)
             ws = _scratch(nb, h.device)
             L.check(lib.ds_bin_expect_bwd(h.data_ptr(), ldh, w.data_ptr(), c.data_ptr(), g.data_ptr(), code, n, d, v,
                                           saved.data_ptr(), L.ptr(gh), L.ptr(gw), ws.data_ptr(), nb, L.stream()),
                     "ds_bin_expect_bwd")
-        return None if gh is None else gh.reshape(shape), gw, None
+        return gh if gh is None or len(shape) == 2 else gh.reshape(shape), gw, None
 
 
 def bin_expectation(hidden, weight, centers) -> torch.Tensor:
