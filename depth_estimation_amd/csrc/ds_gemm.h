@@ -280,6 +280,10 @@ struct Mover {
 
 typedef Shape<256, 256, 2, 4> Big;
 
+// Where split sp of a sum over k begins, `per` (a multiple of 64) each.  A split behind the last step begins at the next multiple
+// of 64, where every operand ends: from k itself a row's padding would run into the row after it.
+__device__ __forceinline__ int split_start(int sp, int per, int k) { return min(sp * per, (k + kBK - 1) / kBK * kBK); }
+
 // What a workgroup multiplies next.  A tile of no steps is given one step of zeros.
 struct Job {
     Operand A, B;

@@ -705,7 +705,7 @@ __global__ __launch_bounds__(S::T) void head_grad_kernel(Operand A, Operand B, c
             order(u, x, n);
             const int m = x / a.splits;
             sp = x - m * a.splits;
-            const int k0 = min(sp * per, k);
+            const int k0 = split_start(sp, per, k);
             return Job{A, B, m * S::BM, n * S::BN, k0, min(k0 + per, k)};
         };
         int sp, next_sp = 0;
@@ -725,7 +725,7 @@ __global__ __launch_bounds__(S::T) void head_grad_kernel(Operand A, Operand B, c
         const int b = (int)(blockIdx.x / a.splits), sp = (int)(blockIdx.x % a.splits);
         const int m0 = b % mt * S::BM, n0 = b / mt * S::BN;
         if (n0 >= bound) return;
-        const int k0 = min(sp * per, k);
+        const int k0 = split_start(sp, per, k);
         f32x4 acc[S::FM][S::FN];
         gemm_tile<T, S, kM, LB, kP<SPLIT>, kP<SPLIT>>(A, B, m0, n0, k0, min(k0 + per, k), lds, acc);
         grad_of_tile<T, S, SPLIT, O, ACC, WHICH>(acc, m0, n0, sp, bound, st, bs, a);
@@ -1145,7 +1145,10 @@ __global__ __launch_bounds__(kFewT) void few_kernel(const IT* __restrict__ h, lo
     float* hs = reinterpret_cast<float*>(lds_);            // [NR][Dq]
     __shared__ float red[kFewT / 64][NR][4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, Dq = (a.D + 7) & ~7;
-    if (a.set_count && blockIdx.x == 0 && threadIdx.x == 0) a.st->count = a.n;
+    if (a.set_count && blockIdx.x == 0 && threadIdx.x == 0) {
+        a.st->count = a.n;
+        a.st->amax_h = a.st->amax_w = 0;
+    }
     const int cnt = a.set_count ? a.n : a.st->count;
     for (int r = 0; r < NR; ++r)
         for (int d = threadIdx.x; d < Dq; d += kFewT)
@@ -1308,7 +1311,7 @@ Saved saved_of(void* p, long long N) {
 }
 
 struct Plan {
-    int dtype, planes, Dp, vt_fwd, piece, piece_ld, dh_splits, dw_splits;
+    int planes, Dp, vt_fwd, piece, piece_ld, dh_splits, dw_splits;
     bool stage_w, stage_h, dh_part;
     ShapeId fwd, dl_shape, dh, dw;
     int few, few_grid;                 // forward of few rows: rows a workgroup holds (0: not that path)
@@ -1327,7 +1330,6 @@ int splits_for(long long tiles, long long steps) {
 
 Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     Plan p;
-    p.dtype = dtype;
     p.planes = dtype == DS_F32 ? 2 : 1;
     p.Dp = pad8(D);
     p.stage_w = dtype == DS_F32 || D % 8 != 0;
@@ -1346,7 +1348,8 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     p.slim_bytes = (int)bytes + Vp * 4;
     p.slim_grid = cdiv(N, 16 * (kSlimT / 64)) < 2 * cu_count() ? cdiv(N, 16 * (kSlimT / 64)) : 2 * cu_count();
     p.slim_back = p.slim && (long long)N * pad8(V) * (long long)el <= (1ll << 30);
-    const bool whole = D % 8 == 0 && ldh % 8 == 0 && dtype != DS_F32;     // rows of the caller's can be read as they are
+    // rows of the caller's can be read as they are (a tile's byte offsets have 31 bits: 256 rows)
+    const bool whole = D % 8 == 0 && ldh % 8 == 0 && dtype != DS_F32 && ldh <= (1 << 21);
     p.stage_h = !whole || (mode == kCE && !p.slim_back);
     p.pack = whole && mode == kCE && p.slim_back;
     const size_t h = p.stage_h || p.pack ? align256((size_t)N * p.Dp * el) : 0, w = p.stage_w ? align256((size_t)V * p.Dp * el) : 0;
@@ -1362,7 +1365,7 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     p.fwd_total = o;
     // a piece of the classes: what fits 256 MB of dl (64 MB: 16 % slower at 8192 x 65536 x 1024, 128 MB: 4 %, 512 MB: the
     // same), at least 1024 classes, a multiple of 256
-        const long long fit = (256ll << 20) / ((long long)el * N) / 256 * 256;
+    const long long fit = (256ll << 20) / ((long long)el * N) / 256 * 256;
     const long long piece = p.slim_back ? V : fit < 1024 ? 1024 : fit;
     p.piece = piece >= V ? V : (int)piece;
     p.piece_ld = pad8(p.piece);
@@ -1496,9 +1499,8 @@ void stats_launch(const Plan& p, const Operand& W, const Operand& H, const Saved
 }
 
 template <class IT, class T, int SPLIT>
-int head_fwd(int mode, const IT* hidden, long long ldh, const IT* weight, const long long* target, const float* centers,
+int head_fwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT* weight, const long long* target, const float* centers,
              long long N, int D, int V, long long ignore, int reduction, float* out, void* saved, char* ws, hipStream_t q) {
-    const Plan p = plan_of(mode, std::is_same<IT, float>::value ? DS_F32 : DS_F16, N, D, V, ldh);
     const Saved s = saved_of(saved, N);
     const int* rows = nullptr;
     if (mode == kCE) {
@@ -1610,10 +1612,9 @@ void grad_launch(ShapeId shape, bool acc, const Operand& A, const Operand& B, co
 }
 
 template <class IT, class T, int SPLIT>
-int head_bwd(int mode, const IT* hidden, long long ldh, const IT* weight, const long long* target, const float* centers,
+int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT* weight, const long long* target, const float* centers,
              const float* g, long long N, int D, int V, long long ignore, int reduction, void* saved, IT* g_hidden,
              IT* g_weight, char* ws, hipStream_t q) {
-    const Plan p = plan_of(mode, std::is_same<IT, float>::value ? DS_F32 : DS_F16, N, D, V, ldh);
     const Saved s = saved_of(saved, N);
     const int* rows = mode == kCE ? s.rows : nullptr;
     BackState* bs = reinterpret_cast<BackState*>(ws + p.bs);
@@ -1623,9 +1624,9 @@ int head_bwd(int mode, const IT* hidden, long long ldh, const IT* weight, const 
         const long long most = up.each && N > V ? N : V;
         back_scale_kernel<<<cdiv(most, 2048) < 256 ? cdiv(most, 2048) : 256, 256, 0, q>>>(up, s.st, centers, V, bs);
     }
-    // the forward of few rows needs no scales and leaves none
+    // the forward of few rows needs no scales and leaves zeros; the maximum that a second backward of the same forward, maybe
+    // at the same time, finds there is the one that it forms itself
     const bool need_scales = SPLIT == 3 && p.few;
-    if (need_scales && mode == kExpect) head_init_kernel<<<1, 1, 0, q>>>(s.st, (int)N);
     Operand H, W;
     operands<IT, T, SPLIT>(p, hidden, ldh, weight, N, D, V, s, rows, need_scales, ws + p.bh, ws + p.bw, H, W, q);
     Ignored ignored{};
@@ -1709,7 +1710,7 @@ int fwd_any(int mode, const void* hidden, long long ldh, const void* weight, con
     hipStream_t q = static_cast<hipStream_t>(stream);
 #define DS_GO(IT, T, SP)                                                                                                     \
     [&] {                                                                                                                    \
-        return head_fwd<IT, T, SP>(mode, static_cast<const IT*>(hidden), ldh, static_cast<const IT*>(weight), target, centers, \
+        return head_fwd<IT, T, SP>(p, mode, static_cast<const IT*>(hidden), ldh, static_cast<const IT*>(weight), target, centers, \
                                    N, D, V, ignore, reduction, out, saved, w, q);                                            \
     }
     return by_type(dtype, DS_GO(float, f16, 3), DS_GO(f16, f16, 1), DS_GO(bf16, bf16, 1));
@@ -1730,7 +1731,7 @@ int bwd_any(int mode, const void* hidden, long long ldh, const void* weight, con
     hipStream_t q = static_cast<hipStream_t>(stream);
 #define DS_GO(IT, T, SP)                                                                                                       \
     [&] {                                                                                                                      \
-        return head_bwd<IT, T, SP>(mode, static_cast<const IT*>(hidden), ldh, static_cast<const IT*>(weight), target, centers, \
+        return head_bwd<IT, T, SP>(p, mode, static_cast<const IT*>(hidden), ldh, static_cast<const IT*>(weight), target, centers, \
                                    g, N, D, V, ignore, reduction, saved, static_cast<IT*>(g_hidden),                           \
                                    static_cast<IT*>(g_weight), w, q);                                                          \
     }

@@ -238,7 +238,8 @@ __global__ __launch_bounds__(S::T) void ortho_product_kernel(ProductArgs p, UseA
     auto job = [&](int x) {
         int batch, m0, n0, sp, tile;
         unit_of<S>(p, x, units, batch, m0, n0, sp, tile);
-        Job j{p.A, p.B, m0, n0, min(sp * per, p.k), min(sp * per + per, p.k)};
+        const int k0 = split_start(sp, per, p.k);
+        Job j{p.A, p.B, m0, n0, k0, min(k0 + per, p.k)};
         j.A.p = static_cast<const f16*>(j.A.p) + batch * p.per_a;
         j.B.p = static_cast<const f16*>(j.B.p) + batch * p.per_b;
         return j;

@@ -654,6 +654,9 @@ def _saved_bytes(n: int) -> int:
     return int(L.lib().ds_head_saved_bytes(n))
 
 
+_INT = 2 ** 31 - 1      # sizes and counts cross the C interface as int
+
+
 def _aligned(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
@@ -665,6 +668,8 @@ def _head_args(hidden, weight):
         raise RuntimeError(f"expected hidden (...,D) and weight (V,D); got {tuple(hidden.shape)}, {tuple(weight.shape)}")
     if hidden.dtype != weight.dtype:
         raise RuntimeError(f"hidden and weight must have one dtype, got {hidden.dtype} and {weight.dtype}")
+    if weight.shape[0] > _INT or weight.shape[1] > _INT:
+        raise RuntimeError(f"weight {tuple(weight.shape)} is too large")
     L.same_device(hidden, weight)
     h = hidden if hidden.dim() == 2 else hidden.reshape(-1, weight.shape[1])
     n, d = h.shape
@@ -737,6 +742,8 @@ def linear_cross_entropy(hidden, weight, targets, ignore_index: int = -100, redu
     weight.  Neither the logits nor their gradient exist as a whole."""
     if reduction not in _REDUCTIONS:
         raise RuntimeError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
+    if not -2 ** 63 <= int(ignore_index) < 2 ** 63:
+        raise RuntimeError(f"ignore_index must be a 64-bit integer, got {ignore_index}")
     return _LinearCE.apply(hidden, weight, targets, int(ignore_index), reduction)
 
 
@@ -805,6 +812,8 @@ def orthogonalize(update, steps: int, coefficients, eps: float) -> torch.Tensor:
     if u.numel() == 0:
         return out
     b, lib = u.numel() // (m * n), L.lib()
+    if max(b, m, n) > _INT or not 0 <= int(steps) <= 32:
+        raise RuntimeError(f"orthogonalize: {steps} steps of {tuple(u.shape)} are not supported")
     nb = lib.ds_orthogonalize_workspace_bytes(L.DTYPES[u.dtype], b, m, n)
     ws = _scratch(nb, u.device)
     L.check(lib.ds_orthogonalize(u.data_ptr(), L.DTYPES[u.dtype], b, m, n, int(steps), (C.c_double * 3)(*co), float(eps),

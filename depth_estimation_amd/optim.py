@@ -36,10 +36,13 @@ class Muon(torch.optim.Optimizer):
             raise ValueError(f"bad lr, momentum or weight_decay: {lr}, {momentum}, {weight_decay}")
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
                                       coefficients=tuple(coefficients), eps=eps))
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.dim() < 2:
-                    raise ValueError(f"Muon steps matrices; a parameter of shape {tuple(p.shape)} belongs to another optimiser")
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() < 2:
+                self.param_groups.pop()
+                raise ValueError(f"Muon steps matrices; a parameter of shape {tuple(p.shape)} belongs to another optimiser")
 
     @torch.no_grad()
     def step(self, closure=None):

@@ -162,6 +162,48 @@ def test_streams_and_captured_graphs():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("shape", [(1000, 40003), (20003, 1500), (1500, 20003), (300, 65531), (500, 65531), (64, 65531)], ids=str)
+def test_long_sides(shape, dtype):
+    """Sums over a long side split over many workgroups, with a last split that is short or empty.  The tolerances of
+    test_against_float64 and test_bfloat16_with_fewer_products."""
+    from depth_estimation_amd import optim
+    g = torch.randn(*shape, generator=torch.Generator(device=DEV).manual_seed(sum(shape)), device=DEV).to(dtype)
+    x = g.double()
+    x /= x.norm() + 1e-7
+    for _ in range(5):
+        a = x @ x.mT if shape[0] <= shape[1] else x.mT @ x
+        b = CO[1] * a + CO[2] * (a @ a)
+        x = CO[0] * x + (b @ x if shape[0] <= shape[1] else x @ b)
+    out = optim.orthogonalize(g).double()
+    assert float((out - x).norm() / x.norm()) <= (4e-5 if dtype == torch.float32 else 2.3e-3 if min(shape) >= 256 else 4e-5 + U[dtype])
+
+
+@pytest.mark.gpu
+def test_captured_graphs_of_every_form():
+    """One workgroup's memory above its default, slabs, split sums: replayed with eager calls between."""
+    from depth_estimation_amd import optim
+    s = torch.cuda.Stream()
+    for shape, dtype in (((128, 128), torch.float32), ((64, 1500), torch.bfloat16), ((2, 300, 700), torch.float32),
+                         ((700, 700), torch.bfloat16)):
+        x, y = _update(shape, dtype, 7), _update(shape, dtype, 8)
+        buf = x.clone()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            optim.orthogonalize(buf)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            out = optim.orthogonalize(buf)
+        for src in (x, y, x):
+            buf.copy_(src)
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, optim.orthogonalize(src))
+
+
+@pytest.mark.gpu
 def test_muon_steps():
     """Three steps of a small set of parameters (two of one shape, a convolution, one without a gradient) against the formula."""
     from depth_estimation_amd import optim
@@ -221,6 +263,10 @@ def test_refusals_on_the_host():
         optim.orthogonalize(torch.zeros(4, 4))
     with pytest.raises(ValueError):
         optim.Muon([torch.nn.Parameter(torch.zeros(4))])
+    muon = optim.Muon([torch.nn.Parameter(torch.zeros(4, 4))])
+    with pytest.raises(ValueError):
+        muon.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(4))]))
+    assert len(muon.param_groups) == 1
     for bad in (dict(lr=-1.0), dict(momentum=1.0), dict(weight_decay=-0.1)):
         with pytest.raises(ValueError):
             optim.Muon([torch.nn.Parameter(torch.zeros(4, 4))], **bad)
@@ -244,7 +290,7 @@ def test_refusals_on_the_host():
 def test_refusals_of_tensors():
     from depth_estimation_amd import optim
     g = torch.zeros(4, 4, device=DEV)
-    for args, kw in [((g[0],), {}), ((g.double(),), {}), ((g.int(),), {}), ((g,), dict(steps=-1)), ((g,), dict(steps=40)),
+    for args, kw in [((g[0],), {}), ((g.double(),), {}), ((g.int(),), {}), ((g,), dict(steps=-1)), ((g,), dict(steps=40)), ((g,), dict(steps=2 ** 32 + 5)),
                      ((g,), dict(coefficients=(1.0, 2.0))), ((g,), dict(coefficients=(1.0, 2.0, math.inf))),
                      ((g,), dict(eps=-1.0)), ((g,), dict(eps=math.nan))]:
         with pytest.raises(RuntimeError):
