@@ -393,8 +393,9 @@ struct TileStream {
 };
 
 // Tile t of mt x nt in the order in which they are taken: workgroup b runs on XCD b % 8, each with an L2 of its own, so every
-// XCD gets a contiguous share, and inside it bands of four tile columns are gone through row by row: the tiles in flight on an
-// XCD share a few rows and columns.  (No division but by the few columns of a last, narrower band: the next tile is looked up
+// XCD gets a contiguous share (turn_of), and inside it bands of four tile columns are gone through row by row (at): the tiles in
+// flight on an XCD share a few rows and columns.  Split sums count their splits as tile rows, split by split, so that an XCD
+// works on few ranges of k at a time.  (No division but by the few columns of a last, narrower band: the next tile is looked up
 // while a turn waits for it.)
 struct Order {
     int tiles, mt, nt, q, r;
@@ -402,8 +403,12 @@ struct Order {
     __device__ __forceinline__ Order(int tiles_, int mt_, int nt_) : tiles(tiles_), mt(mt_), nt(nt_), q(tiles_ >> 3), r(tiles_ & 7) {
         inv = 1.f / (4.f * mt_);
     }
-    __device__ __forceinline__ void operator()(int t, int& m, int& n) const {
-        const int x = t & 7, u = x * q + (x < r ? x : r) + (t >> 3);
+    __device__ __forceinline__ int turn_of(int t) const {
+        const int x = t & 7;
+        return x * q + (x < r ? x : r) + (t >> 3);
+    }
+    __device__ __forceinline__ void operator()(int t, int& m, int& n) const { at(turn_of(t), m, n); }
+    __device__ __forceinline__ void at(int u, int& m, int& n) const {
         int band = __builtin_amdgcn_readfirstlane((int)((float)u * inv));      // off by one at most, or a little more far out
         while (band * 4 * mt > u) --band;
         while ((band + 1) * 4 * mt <= u) ++band;
@@ -479,7 +484,7 @@ __device__ __forceinline__ float scale_for(float amax) {
 
 // ---- which shape a product takes, and over how many workgroups its sum is split (host) -----------------------------------
 enum ShapeId { kSq, kFlat, kThin, kBig, kSmall };
-typedef Shape<128, 128, 2, 2> Sq;
+typedef Shape<128, 128, 4, 2> Sq;
 typedef Shape<64, 64, 2, 2> Small;
 
 struct Cut {
@@ -497,9 +502,9 @@ inline Cut cut_of(Tiles tiles, double area, long long K, int pairs, bool may_spl
         int b, at_once;
         double step, alone, ends;
     };
-    static const Cost one[3] = {{kBig, 256, 1, 1.5, 1.35, 4.5}, {kSq, 128, 2, 0.60, 0.78, 3.0}, {kSmall, 64, 4, 0.21, 0.57, 2.0}};
-    static const Cost two[3] = {{kBig, 256, 1, 3.0, 2.7, 5.0}, {kSq, 128, 2, 1.00, 1.30, 3.0}, {kSmall, 64, 3, 0.37, 0.62, 2.5}};
-    static const Cost three[3] = {{kBig, 256, 1, 4.5, 4.1, 5.0}, {kSq, 128, 2, 1.40, 1.85, 3.0}, {kSmall, 64, 2, 0.53, 0.68, 2.5}};
+    static const Cost one[3] = {{kBig, 256, 1, 1.5, 1.35, 4.5}, {kSq, 128, 2, 0.58, 0.66, 3.0}, {kSmall, 64, 4, 0.21, 0.57, 2.0}};
+    static const Cost two[3] = {{kBig, 256, 1, 3.0, 2.7, 5.0}, {kSq, 128, 2, 0.94, 1.08, 3.0}, {kSmall, 64, 3, 0.37, 0.62, 2.5}};
+    static const Cost three[3] = {{kBig, 256, 1, 4.5, 4.1, 5.0}, {kSq, 128, 2, 1.33, 1.50, 3.0}, {kSmall, 64, 2, 0.53, 0.68, 2.5}};
     const long long steps = (K + kBK - 1) / kBK, most = may_split ? (steps < 256 ? steps : 256) : 1;
     Cut best{kSq, 1};
     double least = 1e300;

@@ -685,7 +685,7 @@ __device__ __forceinline__ void grad_of_tile(const f32x4 (&acc)[S::FM][S::FN], i
         }
     }
 }
-// A: W (dH) or H (dW), B: dl.  Workgroups: tiles x splits, the splits of a tile next to each other.
+// A: W (dH) or H (dW), B: dl.  Workgroups: tiles x splits in Order.
 template <class T, class S, int SPLIT, class O, bool ACC, int WHICH>
 __global__ __launch_bounds__(S::T) void head_grad_kernel(Operand A, Operand B, const HeadState* __restrict__ st,
                                                          const BackState* __restrict__ bs, GradArgs a) {
@@ -695,20 +695,20 @@ __global__ __launch_bounds__(S::T) void head_grad_kernel(Operand A, Operand B, c
     B.outer = cnt;
     if (WHICH == 1) A.outer = cnt;
     constexpr Lay LB = WHICH == 0 ? kK : kM;
+    const int nt = cdiv(bound, S::BN), units = mt * nt * a.splits;
+    int t = blockIdx.x;
+    if (t >= units) return;
+    const Order order(units, mt * a.splits, nt);
+    auto job = [&](int u, int& sp) {
+        int x, n;
+        order(u, x, n);
+        sp = x / mt;
+        const int k0 = split_start(sp, per, k);
+        return Job{A, B, (x - sp * mt) * S::BM, n * S::BN, k0, min(k0 + per, k)};
+    };
+    int sp;
     if constexpr (std::is_same<S, Big>::value) {
-        const int nt = cdiv(bound, S::BN), units = mt * nt * a.splits;
-        int t = blockIdx.x;
-        if (t >= units) return;
-        const Order order(units, mt * a.splits, nt);
-        auto job = [&](int u, int& sp) {
-            int x, n;
-            order(u, x, n);
-            const int m = x / a.splits;
-            sp = x - m * a.splits;
-            const int k0 = split_start(sp, per, k);
-            return Job{A, B, m * S::BM, n * S::BN, k0, min(k0 + per, k)};
-        };
-        int sp, next_sp = 0;
+        int next_sp = 0;
         TileStream<T, kM, LB, kP<SPLIT>, kP<SPLIT>> stream(lds, job(t, sp));
         for (; t < units; t += gridDim.x) {
             const int m0 = stream.job.m0, n0 = stream.job.n0;
@@ -722,13 +722,10 @@ __global__ __launch_bounds__(S::T) void head_grad_kernel(Operand A, Operand B, c
             sp = next_sp;
         }
     } else {
-        const int b = (int)(blockIdx.x / a.splits), sp = (int)(blockIdx.x % a.splits);
-        const int m0 = b % mt * S::BM, n0 = b / mt * S::BN;
-        if (n0 >= bound) return;
-        const int k0 = split_start(sp, per, k);
+        const Job j = job(t, sp);
         f32x4 acc[S::FM][S::FN];
-        gemm_tile<T, S, kM, LB, kP<SPLIT>, kP<SPLIT>>(A, B, m0, n0, k0, min(k0 + per, k), lds, acc);
-        grad_of_tile<T, S, SPLIT, O, ACC, WHICH>(acc, m0, n0, sp, bound, st, bs, a);
+        gemm_tile<T, S, kM, LB, kP<SPLIT>, kP<SPLIT>>(A, B, j.m0, j.n0, j.kbeg, j.kend, lds, acc);
+        grad_of_tile<T, S, SPLIT, O, ACC, WHICH>(acc, j.m0, j.n0, sp, bound, st, bs, a);
     }
 }
 

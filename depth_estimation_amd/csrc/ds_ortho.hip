@@ -207,21 +207,26 @@ struct ProductArgs {
     int mt, nt, tri, k, splits, batch;
     float* part;
 };
+// a tile's matrix and place; tiles: of a matrix
 template <class S>
-__device__ __forceinline__ void unit_of(const ProductArgs& p, int u, int units, int& batch, int& m0, int& n0, int& sp, int& tile) {
-    const int per = units / p.batch, tiles = per / p.splits;
-    batch = u / per;
-    const int in = u % per;
-    sp = in % p.splits;
+__device__ __forceinline__ void tile_of(const ProductArgs& p, int tile, int tiles, int& batch, int& m0, int& n0) {
+    batch = tile / tiles;
     int m, n;
-    if (p.tri) {
-        triangle(in / p.splits, m, n);
-    } else {
-        Order(tiles, p.mt, p.nt)(in / p.splits, m, n);
-    }
-    tile = batch * tiles + in / p.splits;
+    if (p.tri)
+        triangle(tile - batch * tiles, m, n);
+    else
+        Order(tiles, p.mt, p.nt).at(tile - batch * tiles, m, n);
     m0 = m * S::BM;
     n0 = n * S::BN;
+}
+// matrix by matrix, split by split: an XCD works on few ranges of k at a time
+template <class S>
+__device__ __forceinline__ void unit_of(const ProductArgs& p, int u, int units, int& batch, int& m0, int& n0, int& sp, int& tile) {
+    const int v = Order(units, p.mt, p.nt).turn_of(u), per = units / p.batch, tiles = per / p.splits;
+    batch = v / per;
+    sp = (v - batch * per) / tiles;
+    tile = v - sp * tiles - batch * (per - tiles);
+    tile_of<S>(p, tile, tiles, batch, m0, n0);
 }
 template <class S>
 __device__ __forceinline__ void keep_part(const f32x4 (&acc)[S::FM][S::FN], const ProductArgs& p, int tile, int sp) {
@@ -273,9 +278,9 @@ __global__ __launch_bounds__(S::T) void ortho_product_kernel(ProductArgs p, UseA
 // adds a tile's splits in order; a workgroup for every fragment row, because there are few tiles where there are splits
 template <class S, class H, class O>
 __global__ __launch_bounds__(S::T) void ortho_finish_kernel(ProductArgs p, UseArgs u) {
-    int batch, m0, n0, sp, tile;
-    unit_of<S>(p, blockIdx.x * p.splits, gridDim.x * p.splits, batch, m0, n0, sp, tile);
-    const int i = blockIdx.y;
+    int batch, m0, n0;
+    const int tile = blockIdx.x, i = blockIdx.y;
+    tile_of<S>(p, tile, gridDim.x / p.batch, batch, m0, n0);
     const f32x4* q = reinterpret_cast<const f32x4*>(p.part) + (long long)tile * p.splits * (S::BM * S::BN / 4) + threadIdx.x +
                      i * S::FN * S::T;
     f32x4 acc[S::FN];
