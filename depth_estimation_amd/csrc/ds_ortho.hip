@@ -27,11 +27,6 @@ __host__ __device__ inline int norm_blocks(long long mn) {
     const long long n = (mn + 4095) / 4096;
     return n < 512 ? (int)n : 512;
 }
-__device__ __forceinline__ float element(const void* g, int dtype, long long i) {
-    return dtype == DS_F32   ? static_cast<const float*>(g)[i]
-           : dtype == DS_F16 ? (float)static_cast<const f16*>(g)[i]
-                             : (float)static_cast<const bf16*>(g)[i];
-}
 // sum over a workgroup of T threads, the same in every thread
 template <int T>
 __device__ __forceinline__ double sum_all(double a, double* s) {
@@ -80,23 +75,47 @@ __device__ __forceinline__ double inverse_norm(const double* part, int blocks, d
     return 1.0 / (sqrt(sum_all<T>(t, s)) + eps);
 }
 
-// G / (|G| + eps) as two planes, rows padded with zeros to np
-__global__ __launch_bounds__(256) void ortho_load_kernel(const void* __restrict__ g, int dtype, int m, int n, int np, double eps,
+// G / (|G| + eps) as two planes, rows padded with zeros to np.  Four elements a lane, four such loads under way (one at a time:
+// 11 us at 512 x 4608 float32)
+template <class O>
+__global__ __launch_bounds__(256) void ortho_load_kernel(const O* __restrict__ g, int m, int n, int np, double eps,
                                                          const double* __restrict__ part, int blocks, f16* __restrict__ x,
                                                          long long lo, long long per) {
+    constexpr int U = 4;
+    typedef O o4 __attribute__((ext_vector_type(4)));
+    typedef o4 loose __attribute__((aligned(sizeof(O))));
     __shared__ double s[4];
-    const double inv = inverse_norm<256>(part + (long long)blockIdx.y * blocks, blocks, eps, s) * kXs;
-    const long long base = (long long)blockIdx.y * m * n;
+    const O* src = g + (long long)blockIdx.y * m * n;
     f16* y = x + blockIdx.y * per;
     const unsigned q = np / 4;
-    const long long all = (long long)m * q;
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
+    const long long all = (long long)m * q, step = gridDim.x * 256ll;
+    auto load = [&](long long i, o4& v) {
         const int r = all < (1ll << 31) ? (int)((unsigned)i / q) : (int)(i / q), c = (int)(i - (long long)r * q) * 4;
-        float v[4];
+        const O* p = src + (long long)r * n + c;
+        if (c + 4 <= n) {
+            v = *reinterpret_cast<const loose*>(p);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)   // scaled in double: a tiny or huge norm keeps its bits
-            v[e] = c + e < n ? (float)(element(g, dtype, base + (long long)r * n + c + e) * inv) : 0.f;
-        put4<3>(y + (long long)r * np + c, lo, v);
+            for (int e = 0; e < 4; ++e) v[e] = c + e < n ? p[e] : (O)0.f;
+        }
+    };
+    const long long i0 = blockIdx.x * 256ll + threadIdx.x;
+    o4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (i0 + u * step < all) load(i0 + u * step, v[u]);
+    const double inv = inverse_norm<256>(part + (long long)blockIdx.y * blocks, blocks, eps, s) * kXs;
+    for (long long i = i0; i < all; i += U * step) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long at = i + u * step;
+            if (at >= all) break;
+            if (i != i0) load(at, v[u]);
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = (float)((float)v[u][e] * inv);   // scaled in double: a tiny or huge norm keeps its bits
+            put4<3>(y + at * 4, lo, w);
+        }
     }
 }
 
@@ -811,7 +830,7 @@ int ortho_any(const OrthoPlan& p, const void* g, int dtype, int batch, int m, in
         ortho_only_scale_kernel<O><<<dim3(nb, batch), 256, 0, q>>>(g, eps, part, p.blocks, mn, out);
     } else {
         const int nb = cdiv((long long)m * p.np, 4096) < 2048 ? cdiv((long long)m * p.np, 4096) : 2048;
-        ortho_load_kernel<<<dim3(nb, batch), 256, 0, q>>>(g, dtype, m, n, p.np, eps, part, p.blocks,
+        ortho_load_kernel<O><<<dim3(nb, batch), 256, 0, q>>>(static_cast<const O*>(g), m, n, p.np, eps, part, p.blocks,
                                                           reinterpret_cast<f16*>(ws + p.x0), (long long)m * p.np,
                                                           2ll * m * p.np);
         if constexpr (std::is_same<O, bf16>::value) {
