@@ -75,10 +75,11 @@ _SIGNATURES = {
     "ds_depth_metrics": (_i, [_fp, _fp, _i, _i, _i, _fp, _fp, _fp, _sz, _fp]),
     "ds_depth_metrics_eps": (_i, [_fp, _fp, _i, _i, _i, _f32, _fp, _fp, _fp, _sz, _fp]),
     "ds_depth_metrics_noalloc": (_i, [_fp, _fp, _i, _i, _i, _fp, _fp, _fp]),
-    "ds_head_saved_bytes": (_sz, [_ll]),
+    "ds_linear_ce_saved_bytes": (_sz, [_i, _ll, _i, _i, _ll]),
     "ds_linear_ce_workspace_bytes": (_sz, [_i, _ll, _i, _i, _ll, _i]),
     "ds_linear_ce_fwd": (_i, [_fp, _ll, _fp, _fp, _i, _ll, _i, _i, _ll, _i, _fp, _fp, _fp, _sz, _fp]),
     "ds_linear_ce_bwd": (_i, [_fp, _ll, _fp, _fp, _fp, _i, _ll, _i, _i, _ll, _i, _fp, _fp, _fp, _fp, _sz, _fp]),
+    "ds_bin_expect_saved_bytes": (_sz, [_i, _ll, _i, _i, _ll]),
     "ds_bin_expect_workspace_bytes": (_sz, [_i, _ll, _i, _i, _ll, _i]),
     "ds_bin_expect_fwd": (_i, [_fp, _ll, _fp, _fp, _i, _ll, _i, _i, _fp, _fp, _fp, _sz, _fp]),
     "ds_bin_expect_bwd": (_i, [_fp, _ll, _fp, _fp, _fp, _i, _ll, _i, _i, _fp, _fp, _fp, _fp, _sz, _fp]),

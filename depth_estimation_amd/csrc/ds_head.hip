@@ -1314,7 +1314,8 @@ struct Plan {
     int few, few_grid;                 // forward of few rows: rows a workgroup holds (0: not that path)
     int slim, slim_bytes, slim_grid;   // small head: k steps of 32 a row (0: not that path); backward: slim_back
     bool slim_back, pack;
-    size_t staged_h, staged_w, counts, tlogit, part, sums, fwd_total;      // offsets of the forward's workspace
+    size_t sh, sw, saved_total;                                            // staged operands behind Saved (not of few rows)
+    size_t counts, tlogit, part, sums, fwd_total;                          // offsets of the forward's workspace
     size_t bh, bw, bs, dl, dhp, dwp, bwd_total;                            // offsets of the backward's
 };
 
@@ -1349,12 +1350,16 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     const bool whole = D % 8 == 0 && ldh % 8 == 0 && dtype != DS_F32 && ldh <= (1 << 21);
     p.stage_h = !whole || (mode == kCE && !p.slim_back);
     p.pack = whole && mode == kCE && p.slim_back;
-    const size_t h = p.stage_h || p.pack ? align256((size_t)N * p.Dp * el) : 0, w = p.stage_w ? align256((size_t)V * p.Dp * el) : 0;
+    const size_t h = align256((size_t)N * p.Dp * el), w = p.stage_w ? align256((size_t)V * p.Dp * el) : 0;
+    // what the forward stages is kept for the backward (staging 50021 classes of 771 features once more: 35 of 490 us); few
+    // rows are read as they are
     p.fwd = thin ? kThin : cut_of(V, N, D, p.planes, false).shape;
     p.vt_fwd = cdiv(V, p.fwd == kBig ? Big::BM : Sq::BM);
-    size_t o = 0;
-    p.staged_h = o; o += h;
-    p.staged_w = o; o += w;
+    size_t o = saved_bytes(N);
+    p.sh = o; o += p.stage_h && !p.few ? h : 0;
+    p.sw = o; o += p.few ? 0 : w;
+    p.saved_total = o;
+    o = 0;
     p.counts = o; o += align256((size_t)cdiv(N, kListBlock) * 4);
     p.tlogit = o; o += align256((size_t)N * 4);
     p.part = o; o += p.few ? align256((size_t)p.few_grid * p.few * 16) : p.slim ? 0 : 3 * align256((size_t)p.vt_fwd * N * 4);
@@ -1377,8 +1382,8 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     p.dh_part = p.dh_splits > 1 || p.piece < V;
     const size_t D4 = (D + 3) & ~3;
     o = 0;
-    p.bh = o; o += h;
-    p.bw = o; o += w;
+    p.bh = o; o += (p.stage_h && p.few) || p.pack ? h : 0;
+    p.bw = o; o += p.few ? w : 0;
     p.bs = o; o += 256;
     p.dl = o; o += align256((size_t)N * p.piece_ld * el);
     p.dhp = o; o += p.dh_part ? align256((size_t)p.dh_splits * N * D4 * 4) : 0;
@@ -1409,12 +1414,12 @@ void scales(const IT* hidden, long long ldh, const int* rows, const IT* weight, 
     const int bx = cdiv(N, per) < 512 ? cdiv(N, per) : 512, bw = cdiv(V, per) < 512 ? cdiv(V, per) : 512;
     amax_kernel<IT, VEC><<<bx + bw, 256, 0, q>>>(hidden, ldh, rows, st, weight, V, D, L, bx);
 }
-// inputs as matrix operands: in place, or staged into `ws`
+// inputs as matrix operands: in place, or staged at wh and ww (stage: now)
 template <class IT, class T, int SPLIT>
 void operands(const Plan& p, const IT* hidden, long long ldh, const IT* weight, long long N, int D, int V, const Saved& s,
-              const int* rows, bool need_scales, char* wh, char* ww, Operand& H, Operand& W, hipStream_t q) {
+              const int* rows, bool stage, char* wh, char* ww, Operand& H, Operand& W, hipStream_t q) {
     if constexpr (SPLIT == 3)
-        if (need_scales) scales(hidden, ldh, rows, weight, N, D, V, s.st, q);
+        if (stage) scales(hidden, ldh, rows, weight, N, D, V, s.st, q);
     H = Operand{hidden, ldh, 0, (int)N, D};
     W = Operand{weight, D, 0, V, D};
     constexpr int VEC = 16 / sizeof(IT);
@@ -1434,7 +1439,7 @@ void operands(const Plan& p, const IT* hidden, long long ldh, const IT* weight, 
         b = Source{weight, D, nullptr, nullptr, V, &s.st->amax_w, ww, lo, a.blocks, blocks(V)};
         W = Operand{ww, p.Dp, lo, V, p.Dp};
     }
-    if (a.blocks + b.blocks > 0)
+    if (stage && a.blocks + b.blocks > 0)
         stage_kernel<IT, T, SPLIT, VEC><<<a.blocks + b.blocks, 256, 0, q>>>(a.blocks ? a : b, a.blocks ? b : Source{}, D, p.Dp, L);
 }
 
@@ -1540,7 +1545,8 @@ int head_fwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
         return launched();
     }
     Operand H, W;
-    operands<IT, T, SPLIT>(p, hidden, ldh, weight, N, D, V, s, rows, true, ws + p.staged_h, ws + p.staged_w, H, W, q);
+    char* keep = static_cast<char*>(saved);
+    operands<IT, T, SPLIT>(p, hidden, ldh, weight, N, D, V, s, rows, true, keep + p.sh, keep + p.sw, H, W, q);
     double* sums = mode == kCE && reduction != DS_REDUCE_NONE ? reinterpret_cast<double*>(ws + p.sums) : nullptr;
     if (p.slim) {
         SlimArgs a = slim_args(p, H, W, s, rows, N, D, V, centers);
@@ -1621,11 +1627,12 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
         const long long most = up.each && N > V ? N : V;
         back_scale_kernel<<<cdiv(most, 2048) < 256 ? cdiv(most, 2048) : 256, 256, 0, q>>>(up, s.st, centers, V, bs);
     }
-    // the forward of few rows needs no scales and leaves zeros; the maximum that a second backward of the same forward, maybe
-    // at the same time, finds there is the one that it forms itself
-    const bool need_scales = SPLIT == 3 && p.few;
+    // the forward of few rows stages nothing and leaves zero scales; the maximum that a second backward of the same forward,
+    // maybe at the same time, finds there is the one that it forms itself
     Operand H, W;
-    operands<IT, T, SPLIT>(p, hidden, ldh, weight, N, D, V, s, rows, need_scales, ws + p.bh, ws + p.bw, H, W, q);
+    char* staged = p.few ? ws : static_cast<char*>(saved);
+    operands<IT, T, SPLIT>(p, hidden, ldh, weight, N, D, V, s, rows, p.few != 0, staged + (p.few ? p.bh : p.sh),
+                           staged + (p.few ? p.bw : p.sw), H, W, q);
     Ignored ignored{};
     if (mode == kCE && g_hidden) {
         constexpr int VEC = 16 / sizeof(IT);
@@ -1741,8 +1748,9 @@ int bwd_any(int mode, const void* hidden, long long ldh, const void* weight, con
 
 extern "C" {
 
-size_t ds_head_saved_bytes(long long N) { return N > 0 ? ds::saved_bytes(N) : 0; }
-
+size_t ds_linear_ce_saved_bytes(int dtype, long long N, int D, int V, long long ldh) {
+    return ds::check_sizes(dtype, N, D, V, ldh) ? 0 : ds::plan_of(ds::kCE, dtype, N, D, V, ldh).saved_total;
+}
 size_t ds_linear_ce_workspace_bytes(int dtype, long long N, int D, int V, long long ldh, int backward) {
     if (ds::check_sizes(dtype, N, D, V, ldh)) return 0;
     const ds::Plan p = ds::plan_of(ds::kCE, dtype, N, D, V, ldh);
@@ -1763,6 +1771,9 @@ int ds_linear_ce_bwd(const void* hidden, long long ldh, const void* weight, cons
                        const_cast<void*>(saved), g_hidden, g_weight, workspace, workspace_bytes, stream);
 }
 
+size_t ds_bin_expect_saved_bytes(int dtype, long long N, int D, int V, long long ldh) {
+    return ds::check_sizes(dtype, N, D, V, ldh) ? 0 : ds::plan_of(ds::kExpect, dtype, N, D, V, ldh).saved_total;
+}
 size_t ds_bin_expect_workspace_bytes(int dtype, long long N, int D, int V, long long ldh, int backward) {
     if (ds::check_sizes(dtype, N, D, V, ldh)) return 0;
     const ds::Plan p = ds::plan_of(ds::kExpect, dtype, N, D, V, ldh);

@@ -645,13 +645,10 @@ def _scratch(nbytes: int, device) -> torch.Tensor:
 
 # what a call needs depends on sizes alone; asked for once per size (a small training step is bound by the host)
 @functools.lru_cache(maxsize=1024)
-def _head_bytes(which: str, code: int, n: int, d: int, v: int, ldh: int, backward: int) -> int:
-    return int(getattr(L.lib(), which)(code, n, d, v, ldh, backward))
-
-
-@functools.lru_cache(maxsize=1024)
-def _saved_bytes(n: int) -> int:
-    return int(L.lib().ds_head_saved_bytes(n))
+def _head_bytes(op: str, code: int, n: int, d: int, v: int, ldh: int):
+    """bytes to save, of the forward's workspace and of the backward's"""
+    saved, ws = getattr(L.lib(), f"ds_{op}_saved_bytes"), getattr(L.lib(), f"ds_{op}_workspace_bytes")
+    return int(saved(code, n, d, v, ldh)), int(ws(code, n, d, v, ldh, 0)), int(ws(code, n, d, v, ldh, 1))
 
 
 _INT = 2 ** 31 - 1      # sizes and counts cross the C interface as int
@@ -688,6 +685,11 @@ def _head_grads(ctx, h, w):
     return gh, gw
 
 
+def _once(gradients, ctx, g):
+    """once_differentiable where a second derivative could be asked for; without its cost where none can (grad mode is off)"""
+    return once_differentiable(gradients)(ctx, g) if torch.is_grad_enabled() else gradients(ctx, g)
+
+
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 _INTEGERS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 
@@ -706,12 +708,12 @@ class _LinearCE(torch.autograd.Function):
         v, lib, dev = w.shape[0], L.lib(), h.device
         code, red = L.DTYPES[h.dtype], _REDUCTIONS[reduction]
         out = torch.empty(targets.shape if red == 0 else (), dtype=torch.float32, device=dev)
-        saved = _scratch(_saved_bytes(n), dev)
+        keep, nb, _ = _head_bytes("linear_ce", code, n, d, v, ldh)
+        saved = _scratch(keep, dev)
         if n == 0:
             if red:
                 out.fill_(0.0 if red == 1 else float("nan"))
         else:
-            nb = _head_bytes("ds_linear_ce_workspace_bytes", code, n, d, v, ldh, 0)
             ws = _scratch(nb, dev)
             L.check(lib.ds_linear_ce_fwd(h.data_ptr(), ldh, w.data_ptr(), t.data_ptr(), code, n, d, v, ignore_index, red,
                                          out.data_ptr(), saved.data_ptr(), ws.data_ptr(), nb, L.stream()), "ds_linear_ce_fwd")
@@ -720,8 +722,11 @@ class _LinearCE(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
+        return _once(_LinearCE._gradients, ctx, g)
+
+    @staticmethod
+    def _gradients(ctx, g):
         h, w, t, saved = ctx.saved_tensors
         ldh, ignore_index, red, shape = ctx.args
         (n, d), v = h.shape, w.shape[0]
@@ -729,7 +734,7 @@ class _LinearCE(torch.autograd.Function):
         if n and (gh is not None or gw is not None):
             code, lib, g = L.DTYPES[h.dtype], L.lib(), L.dev_f32(g, "grad")
             L.same_device(h, g)
-            nb = _head_bytes("ds_linear_ce_workspace_bytes", code, n, d, v, ldh, 1)
+            nb = _head_bytes("linear_ce", code, n, d, v, ldh)[2]
             ws = _scratch(nb, h.device)
             L.check(lib.ds_linear_ce_bwd(h.data_ptr(), ldh, w.data_ptr(), t.data_ptr(), g.data_ptr(), code, n, d, v,
                                          ignore_index, red, saved.data_ptr(), L.ptr(gh), L.ptr(gw), ws.data_ptr(), nb,
@@ -757,9 +762,9 @@ class _BinExpect(torch.autograd.Function):
             raise RuntimeError(f"centers must be ({v},), got {tuple(c.shape)}")
         L.same_device(h, c)
         out = torch.empty(hidden.shape[:-1], dtype=torch.float32, device=dev)
-        saved = _scratch(_saved_bytes(n), dev)
+        keep, nb, _ = _head_bytes("bin_expect", code, n, d, v, ldh)
+        saved = _scratch(keep, dev)
         if n:
-            nb = _head_bytes("ds_bin_expect_workspace_bytes", code, n, d, v, ldh, 0)
             ws = _scratch(nb, dev)
             L.check(lib.ds_bin_expect_fwd(h.data_ptr(), ldh, w.data_ptr(), c.data_ptr(), code, n, d, v, out.data_ptr(),
                                           saved.data_ptr(), ws.data_ptr(), nb, L.stream()), "ds_bin_expect_fwd")
@@ -768,8 +773,11 @@ class _BinExpect(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
+        return _once(_BinExpect._gradients, ctx, g)
+
+    @staticmethod
+    def _gradients(ctx, g):
         h, w, c, saved = ctx.saved_tensors
         ldh, shape = ctx.args
         (n, d), v = h.shape, w.shape[0]
@@ -777,7 +785,7 @@ class _BinExpect(torch.autograd.Function):
         if n and (gh is not None or gw is not None):
             code, lib, g = L.DTYPES[h.dtype], L.lib(), L.dev_f32(g, "grad")
             L.same_device(h, g)
-            nb = _head_bytes("ds_bin_expect_workspace_bytes", code, n, d, v, ldh, 1)
+            nb = _head_bytes("bin_expect", code, n, d, v, ldh)[2]
             ws = _scratch(nb, h.device)
             L.check(lib.ds_bin_expect_bwd(h.data_ptr(), ldh, w.data_ptr(), c.data_ptr(), g.data_ptr(), code, n, d, v,
                                           saved.data_ptr(), L.ptr(gh), L.ptr(gw), ws.data_ptr(), nb, L.stream()),
