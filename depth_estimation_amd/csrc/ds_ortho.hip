@@ -8,10 +8,12 @@
 // three decades; measured against 64 bits), so all three are kept as two fp16 planes (22 bits; 1e-6) under fixed powers of
 // two: entries of X and A are at most about 1.3, B's bound follows from the coefficients.
 //
-// bf16 results of larger matrices need less, and take half the products (Light): A and B keep one plane (11 bits) off the
-// diagonal, where their entries are small, and their diagonals, which carry most of X, in fp32 beside it; X keeps two planes
-// where it is multiplied by B.  What that costs is 2e-4 .. 9e-4 of the result's norm (sides of 64 and more; Gaussian, decaying
-// and nearly low-rank matrices), under the 1.7e-3 that rounding the result to bf16 costs.
+// bf16 results of larger matrices need less, and take half the products (Light): A keeps one plane (11 bits) off the diagonal,
+// where its entries are small, and its diagonal in fp32 beside it.  B keeps one plane; what its diagonal, which carries most of
+// X, lost by that is made up for as a factor of the result's row: diag(d) X (1 + rounding) off the diagonal is the smaller part.
+// X keeps two planes where it is multiplied by B.  What that costs is 4e-4 .. 9e-4 of the result's norm (sides of 256 and more;
+// Gaussian, decaying and nearly low-rank matrices, written out in float64), under the 1.7e-3 that rounding the result to bf16
+// costs; without the factors 6e-4 .. 1.2e-3.
 #include "ds_gemm.h"
 #include "ds_internal.h"
 #include "../../include/depthsynth.h"
@@ -141,10 +143,10 @@ struct UseArgs {
     void* out;
     int ld;
     long long lo, per_out;   // planes apart, matrices apart
-    const f16* a;            // kPoly: A again; light kNext and kLast: X again
+    const f16* a;            // kPoly: A again
     long long per_a;
     float ca, cb, cc;        // kPoly's coefficients, scaled; else ca: the factor
-    float *da, *db;          // light: diagonals of A and of B, scaled as their matrices, `side` a matrix
+    float *da, *db;          // light: A's diagonal, scaled as A, and B's as it is over what its plane holds; `side` a matrix
     int side, wide;
 };
 // fragment row i of a tile
@@ -162,12 +164,12 @@ __device__ __forceinline__ void use_row(const f32x4 (&acc)[S::FN], int i, int m0
         const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
         if (n >= u.rows) continue;
         float v[4], old[4];
-        if (U == kPoly || (H::LIGHT && U != kGram)) {      // A or X at the same place
+        if (U == kPoly) {      // A at the same place
             const f16* a = u.a + batch * u.per_a + (long long)n * u.ld + m;
             const f16x4 h = *reinterpret_cast<const f16x4*>(a);
 #pragma unroll
             for (int e = 0; e < 4; ++e) old[e] = (float)h[e];
-            if (!(H::LIGHT && U == kPoly)) {
+            if (!H::LIGHT) {
                 const f16x4 l = *reinterpret_cast<const f16x4*>(a + u.lo);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) old[e] += (float)l[e];
@@ -181,13 +183,17 @@ __device__ __forceinline__ void use_row(const f32x4 (&acc)[S::FN], int i, int m0
             } else if (U == kPoly) {
                 const float dn = da[n], dm = in ? da[m + e] : 0.f;
                 // (O + D)(O + D) = O O + O D + D O + D D
-                v[e] = diagonal ? 0.f : fmaf(u.cc, fmaf(dn + dm, old[e], acc[j][e]), u.cb * old[e]);
-                if (diagonal) u.db[(long long)batch * u.side + n] = fmaf(u.cc, fmaf(dn, dn, acc[j][e]), fmaf(u.cb, dn, u.ca));
+                v[e] = diagonal ? fmaf(u.cc, fmaf(dn, dn, acc[j][e]), fmaf(u.cb, dn, u.ca))
+                                : fmaf(u.cc, fmaf(dn + dm, old[e], acc[j][e]), u.cb * old[e]);
+                if (diagonal) {      // (below fp16's normal numbers nothing is lost that matters beside B's other entries)
+                    const float h = (float)(f16)v[e];
+                    u.db[(long long)batch * u.side + n] = fabsf(h) >= 6.1035156e-5f ? v[e] / h : 1.f;
+                }
             } else if (H::LIGHT && U == kGram) {
                 v[e] = diagonal ? 0.f : acc[j][e] * u.ca;
                 if (diagonal) u.da[(long long)batch * u.side + n] = acc[j][e] * u.ca;
             } else if (H::LIGHT) {
-                v[e] = in ? fmaf(db[u.wide ? n : m + e], old[e], acc[j][e]) * u.ca : 0.f;
+                v[e] = in ? acc[j][e] * (db[u.wide ? n : m + e] * u.ca) : 0.f;
             } else {
                 v[e] = acc[j][e] * u.ca;
             }
@@ -751,7 +757,7 @@ void ortho_steps(const OrthoPlan& p, int batch, int m, int n, int steps, const d
                          (float)(co[2] * bs / (kXs * kXs)), da, db, p.s, wide};
         product<kK, kK, P, P, How<kPoly, LIGHT>, float>(p.poly, pp, up, p.s, p.s, q);
         const bool last = i + 1 == steps;
-        const UseArgs ua{m, n, last ? out : y, p.np, lox, last ? (long long)m * n : px, x, px,
+        const UseArgs ua{m, n, last ? out : y, p.np, lox, last ? (long long)m * n : px, nullptr, 0,
                          last ? 1.f / (bs * kXs) : 1.f / bs, 0.f, 0.f, da, db, p.s, wide};
         const ProductArgs pw{wide ? X : B, wide ? B : X, wide ? px : pa, wide ? pa : px, 0, 0, 0, p.s, 1, batch, part};
         if (wide) {
