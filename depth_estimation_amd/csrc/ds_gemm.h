@@ -457,6 +457,44 @@ __device__ __forceinline__ void put4(bf16* p, long long, const float (&v)[4]) {
     *reinterpret_cast<bf16x4*>(p) = h;
 }
 
+// Fragments i and i + 1 of a row in 16 bits: lane group q holds four elements from 4 q of either (x, y) and gets eight
+// consecutive ones of the 32, from 8 q: stores of 16 bytes a lane, 64 a row at a time, instead of 8 and 32.
+__device__ __forceinline__ void eight_of(s16x4 x, s16x4 y, s16x8& out) {
+    typedef unsigned u2 __attribute__((ext_vector_type(2)));
+    const u2 a = __builtin_bit_cast(u2, x), b = __builtin_bit_cast(u2, y);
+    unsigned w[4];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        // groups 0 1 2 3 of a and b -> a0 a1 b0 b1 and a2 a3 b2 b3 -> a0 a2 b0 b2 and a1 a3 b1 b3
+        const auto half = __builtin_amdgcn_permlane32_swap(a[k], b[k], false, false);
+        const auto quarter = __builtin_amdgcn_permlane16_swap(half[0], half[1], false, false);
+        w[k] = quarter[0];
+        w[2 + k] = quarter[1];
+    }
+    typedef unsigned u4 __attribute__((ext_vector_type(4)));
+    out = __builtin_bit_cast(s16x8, u4{w[0], w[1], w[2], w[3]});
+}
+template <class T>
+__device__ __forceinline__ s16x4 round4(const f32x4& v) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    t4 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = (T)v[e];
+    return __builtin_bit_cast(s16x4, r);
+}
+
+// the low plane of four values
+__device__ __forceinline__ s16x4 rest4(const f32x4& v) {
+    f16x4 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        f16 h, l;
+        split16(v[e], h, l);
+        r[e] = l;
+    }
+    return __builtin_bit_cast(s16x4, r);
+}
+
 // up to four consecutive outputs of a row of `n` elements, at element c of the row; rows need only their type's alignment
 template <class O>
 __device__ __forceinline__ void put_row4(O* row, int c, int n, const float (&v)[4]) {

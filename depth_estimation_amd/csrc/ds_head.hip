@@ -591,14 +591,24 @@ __device__ __forceinline__ void dl_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, i
                     acc[i][j][e] = exp_of(l - tp) * gr * ((edge && c >= a.cols ? 0.f : a.centers[a.v0 + c]) - e0);
                 }
         }
+        if (edge) {
 #pragma unroll
-        for (int i = 0; i < S::FM; ++i) {
-            const int c = c0 + i * 16;
+            for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c0 + i * 16 + e >= a.cols) acc[i][j][e] = 0.f;
+        }
+        const int c8 = m0 + wm * S::FM * 16 + (lane >> 4) * 8;
+#pragma unroll
+        for (int i = 0; i < S::FM; i += 2) {
+            const int c = c8 + i * 16;
+            s16x8 hi, lo;
+            eight_of(round4<T>(acc[i][j]), round4<T>(acc[i + 1][j]), hi);
+            if constexpr (SPLIT == 3) eight_of(rest4(acc[i][j]), rest4(acc[i + 1][j]), lo);
             if (edge && c >= a.ld) continue;
-            float d[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) d[e] = edge && c + e >= a.cols ? 0.f : acc[i][j][e];
-            put4<SPLIT>(dl + (long long)n * a.ld + c, a.lo, d);
+            T* q = dl + (long long)n * a.ld + c;
+            *reinterpret_cast<s16x8*>(q) = hi;
+            if constexpr (SPLIT == 3) *reinterpret_cast<s16x8*>(q + a.lo) = lo;
         }
     }
 }
