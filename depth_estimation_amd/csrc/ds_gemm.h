@@ -512,6 +512,32 @@ __device__ __forceinline__ void put_row4(O* row, int c, int n, const float (&v)[
     }
 }
 
+// fragments i and i + 1 of a row of `n` elements of type O: x and y from element c + 4 (lane / 16) and 16 on, c that of the
+// fragments' first element.  All four lane groups of a row call together.
+template <class O>
+__device__ __forceinline__ void put_row8(O* row, int c, int n, int lane, const f32x4& x, const f32x4& y) {
+    if constexpr (sizeof(O) == 2) {
+        typedef O o8 __attribute__((ext_vector_type(8)));
+        typedef o8 loose __attribute__((aligned(sizeof(O))));
+        s16x8 w;
+        eight_of(round4<O>(x), round4<O>(y), w);
+        const o8 v = __builtin_bit_cast(o8, w);
+        c += (lane >> 4) * 8;
+        if (c + 8 <= n) {
+            *reinterpret_cast<loose*>(row + c) = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c + e < n) row[c + e] = v[e];
+        }
+    } else {
+        c += (lane >> 4) * 4;
+        const float v[4] = {x[0], x[1], x[2], x[3]}, w[4] = {y[0], y[1], y[2], y[3]};
+        put_row4(row, c, n, v);
+        put_row4(row, c + 16, n, w);
+    }
+}
+
 // the power of two that brings a largest magnitude `amax` into [2^14, 2^15): fp16 keeps a factor of two of headroom
 __device__ __forceinline__ float scale_for(float amax) {
     if (!(amax > 0.f) || !__builtin_isfinite(amax)) return 1.f;

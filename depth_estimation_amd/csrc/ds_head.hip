@@ -677,21 +677,21 @@ __device__ __forceinline__ void grad_of_tile(const f32x4 (&acc)[S::FM][S::FN], i
         const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
         if (n >= bound) continue;
         const long long row = !ACC && WHICH == 0 && a.rows ? a.rows[n] : n;
+        if (ACC) {
 #pragma unroll
-        for (int i = 0; i < S::FM; ++i) {
-            const int d = m0 + (wm * S::FM + i) * 16 + (lane >> 4) * 4;
-            if (d >= a.D) continue;
-            if (ACC) {
+            for (int i = 0; i < S::FM; ++i) {
+                const int d = m0 + (wm * S::FM + i) * 16 + (lane >> 4) * 4;
+                if (d >= a.D) continue;
                 f32x4* q = reinterpret_cast<f32x4*>(a.part + sp * a.part_split + row * Dp + d);
                 f32x4 v = acc[i][j];
                 if (WHICH == 0 && !a.first) v += *q;
                 *q = v;
-            } else {
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * f0 * is;
-                put_row4(static_cast<O*>(a.out) + row * a.D, d, a.D, v);
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < S::FM; i += 2)
+                put_row8(static_cast<O*>(a.out) + row * a.D, m0 + (wm * S::FM + i) * 16, a.D, lane, acc[i][j] * f0 * is,
+                         acc[i + 1][j] * f0 * is);
         }
     }
 }

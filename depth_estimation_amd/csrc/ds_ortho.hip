@@ -149,79 +149,96 @@ struct UseArgs {
     float *da, *db;          // light: A's diagonal, scaled as A, and B's as it is over what its plane holds; `side` a matrix
     int side, wide;
 };
-// fragment row i of a tile
+// fragment rows i and i + 1 of a tile
 template <class S, class H, class O>
-__device__ __forceinline__ void use_row(const f32x4 (&acc)[S::FN], int i, int m0, int n0, int batch, const UseArgs& u) {
+__device__ __forceinline__ void use_rows(const f32x4 (&x)[S::FN], const f32x4 (&y)[S::FN], int i, int m0, int n0, int batch,
+                                         const UseArgs& u) {
     constexpr Use U = H::U;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / S::WN, wn = wave % S::WN;
-    const int m = m0 + (wm * S::FM + i) * 16 + (lane >> 4) * 4;
-    if (m >= u.ld) return;
+    const int mi = m0 + (wm * S::FM + i) * 16;
     const float* da = H::LIGHT ? u.da + (long long)batch * u.side : nullptr;
     const float* db = H::LIGHT ? u.db + (long long)batch * u.side : nullptr;
 #pragma unroll
     for (int j = 0; j < S::FN; ++j) {
         const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
         if (n >= u.rows) continue;
-        float v[4], old[4];
-        if (U == kPoly) {      // A at the same place
-            const f16* a = u.a + batch * u.per_a + (long long)n * u.ld + m;
-            const f16x4 h = *reinterpret_cast<const f16x4*>(a);
+        f32x4 v[2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) old[e] = (float)h[e];
-            if (!H::LIGHT) {
-                const f16x4 l = *reinterpret_cast<const f16x4*>(a + u.lo);
+        for (int f = 0; f < 2; ++f) {
+            const f32x4 acc = f ? y[j] : x[j];
+            const int m = mi + f * 16 + (lane >> 4) * 4;
+            float old[4] = {0.f, 0.f, 0.f, 0.f};
+            if (U == kPoly && m < u.ld) {      // A at the same place
+                const f16* a = u.a + batch * u.per_a + (long long)n * u.ld + m;
+                const f16x4 h = *reinterpret_cast<const f16x4*>(a);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) old[e] += (float)l[e];
-            }
-        }
+                for (int e = 0; e < 4; ++e) old[e] = (float)h[e];
+                if (!H::LIGHT) {
+                    const f16x4 l = *reinterpret_cast<const f16x4*>(a + u.lo);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const bool in = m + e < u.cols, diagonal = m + e == n;
-            if (U == kPoly && !H::LIGHT) {
-                v[e] = fmaf(u.cc, acc[j][e], u.cb * old[e]) + (diagonal ? u.ca : 0.f);
-            } else if (U == kPoly) {
-                const float dn = da[n], dm = in ? da[m + e] : 0.f;
-                // (O + D)(O + D) = O O + O D + D O + D D
-                v[e] = diagonal ? fmaf(u.cc, fmaf(dn, dn, acc[j][e]), fmaf(u.cb, dn, u.ca))
-                                : fmaf(u.cc, fmaf(dn + dm, old[e], acc[j][e]), u.cb * old[e]);
-                if (diagonal) {      // (below fp16's normal numbers nothing is lost that matters beside B's other entries)
-                    const float h = (float)(f16)v[e];
-                    u.db[(long long)batch * u.side + n] = fabsf(h) >= 6.1035156e-5f ? v[e] / h : 1.f;
+                    for (int e = 0; e < 4; ++e) old[e] += (float)l[e];
                 }
-            } else if (H::LIGHT && U == kGram) {
-                v[e] = diagonal ? 0.f : acc[j][e] * u.ca;
-                if (diagonal) u.da[(long long)batch * u.side + n] = acc[j][e] * u.ca;
-            } else if (H::LIGHT) {
-                v[e] = in ? acc[j][e] * (db[u.wide ? n : m + e] * u.ca) : 0.f;
-            } else {
-                v[e] = acc[j][e] * u.ca;
             }
-            if (!in) v[e] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool in = m + e < u.cols, diagonal = m + e == n;
+                if (U == kPoly && !H::LIGHT) {
+                    v[f][e] = fmaf(u.cc, acc[e], u.cb * old[e]) + (diagonal ? u.ca : 0.f);
+                } else if (U == kPoly) {
+                    const float dn = da[n], dm = in ? da[m + e] : 0.f;
+                    // (O + D)(O + D) = O O + O D + D O + D D
+                    v[f][e] = diagonal ? fmaf(u.cc, fmaf(dn, dn, acc[e]), fmaf(u.cb, dn, u.ca))
+                                       : fmaf(u.cc, fmaf(dn + dm, old[e], acc[e]), u.cb * old[e]);
+                    if (diagonal) {      // (below fp16's normal numbers nothing is lost that matters beside B's other entries)
+                        const float h = (float)(f16)v[f][e];
+                        u.db[(long long)batch * u.side + n] = fabsf(h) >= 6.1035156e-5f ? v[f][e] / h : 1.f;
+                    }
+                } else if (H::LIGHT && U == kGram) {
+                    v[f][e] = diagonal ? 0.f : acc[e] * u.ca;
+                    if (diagonal) u.da[(long long)batch * u.side + n] = acc[e] * u.ca;
+                } else if (H::LIGHT) {
+                    v[f][e] = in ? acc[e] * (db[u.wide ? n : m + e] * u.ca) : 0.f;
+                } else {
+                    v[f][e] = acc[e] * u.ca;
+                }
+                if (!in) v[f][e] = 0.f;
+            }
         }
         if (U == kLast) {
-            put_row4(static_cast<O*>(u.out) + batch * u.per_out + (long long)n * u.cols, m, u.cols, v);
-        } else {
-            constexpr int kPut = H::LIGHT && U != kNext ? 1 : 3;
-            f16* out = static_cast<f16*>(u.out) + batch * u.per_out;
-            put4<kPut>(out + (long long)n * u.ld + m, u.lo, v);
-            if ((U == kGram || U == kPoly) && m0 != n0) {
+            put_row8(static_cast<O*>(u.out) + batch * u.per_out + (long long)n * u.cols, mi, u.cols, lane, v[0], v[1]);
+            continue;
+        }
+        constexpr bool kTwo = !H::LIGHT || U == kNext;      // planes of the result
+        f16* out = static_cast<f16*>(u.out) + batch * u.per_out;
+        const int m8 = mi + (lane >> 4) * 8;
+        s16x8 hi, lo;
+        eight_of(round4<f16>(v[0]), round4<f16>(v[1]), hi);
+        if constexpr (kTwo) eight_of(rest4(v[0]), rest4(v[1]), lo);
+        if (m8 < u.ld) {
+            *reinterpret_cast<s16x8*>(out + (long long)n * u.ld + m8) = hi;
+            if constexpr (kTwo) *reinterpret_cast<s16x8*>(out + (long long)n * u.ld + m8 + u.lo) = lo;
+        }
+        if ((U == kGram || U == kPoly) && m0 != n0) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (m + e < u.cols) {
+            for (int f = 0; f < 2; ++f)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int m = mi + f * 16 + (lane >> 4) * 4 + e;
+                    if (m < u.cols) {
                         f16 h, l;
-                        split16(v[e], h, l);
-                        out[(long long)(m + e) * u.ld + n] = h;
-                        if (kPut == 3) out[(long long)(m + e) * u.ld + n + u.lo] = l;
+                        split16(v[f][e], h, l);
+                        out[(long long)m * u.ld + n] = h;
+                        if (kTwo) out[(long long)m * u.ld + n + u.lo] = l;
                     }
-            }
+                }
         }
     }
 }
 template <class S, class H, class O>
 __device__ __forceinline__ void use_tile(const f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int batch, const UseArgs& u) {
 #pragma unroll
-    for (int i = 0; i < S::FM; ++i) use_row<S, H, O>(acc[i], i, m0, n0, batch, u);
+    for (int i = 0; i < S::FM; i += 2) use_rows<S, H, O>(acc[i], acc[i + 1], i, m0, n0, batch, u);
 }
 
 // C = A B over k.  tri: only tiles with m0 >= n0.  Units: matrices x tiles x splits; part (may be NULL: no splits): the tiles'
@@ -300,21 +317,21 @@ __global__ __launch_bounds__(S::T) void ortho_product_kernel(ProductArgs p, UseA
         done(t, acc);
     }
 }
-// adds a tile's splits in order; a workgroup for every fragment row, because there are few tiles where there are splits
+// adds a tile's splits in order; a workgroup for every two fragment rows, because there are few tiles where there are splits
 template <class S, class H, class O>
 __global__ __launch_bounds__(S::T) void ortho_finish_kernel(ProductArgs p, UseArgs u) {
     int batch, m0, n0;
-    const int tile = blockIdx.x, i = blockIdx.y;
+    const int tile = blockIdx.x, i = blockIdx.y * 2;
     tile_of<S>(p, tile, gridDim.x / p.batch, batch, m0, n0);
     const f32x4* q = reinterpret_cast<const f32x4*>(p.part) + (long long)tile * p.splits * (S::BM * S::BN / 4) + threadIdx.x +
                      i * S::FN * S::T;
-    f32x4 acc[S::FN];
+    f32x4 acc[2][S::FN];
 #pragma unroll
-    for (int j = 0; j < S::FN; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < 2 * S::FN; ++j) acc[j / S::FN][j % S::FN] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < p.splits; ++s)
 #pragma unroll
-        for (int j = 0; j < S::FN; ++j) acc[j] += q[(long long)s * (S::BM * S::BN / 4) + j * S::T];
-    use_row<S, H, O>(acc, i, m0, n0, batch, u);
+        for (int j = 0; j < 2 * S::FN; ++j) acc[j / S::FN][j % S::FN] += q[(long long)s * (S::BM * S::BN / 4) + j * S::T];
+    use_rows<S, H, O>(acc[0], acc[1], i, m0, n0, batch, u);
 }
 
 // ---- small matrices: all steps in one workgroup ------------------------------------------------------------------------
@@ -710,7 +727,7 @@ void product_shape(ProductArgs p, const UseArgs& u, int tiles, hipStream_t q) {
     const int grid = std::is_same<S, Big>::value && units > cu_count() ? cu_count() : units;
     if (p.splits > 1) {
         ortho_product_kernel<S, LA, LB, PA, PB, How<kGram, false>, float, true><<<grid, S::T, 0, q>>>(p, u, units);
-        ortho_finish_kernel<S, H, O><<<dim3(tiles, S::FM), S::T, 0, q>>>(p, u);
+        ortho_finish_kernel<S, H, O><<<dim3(tiles, S::FM / 2), S::T, 0, q>>>(p, u);
     } else {
         ortho_product_kernel<S, LA, LB, PA, PB, H, O, false><<<grid, S::T, 0, q>>>(p, u, units);
     }
