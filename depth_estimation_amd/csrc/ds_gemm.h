@@ -547,7 +547,7 @@ __device__ __forceinline__ float scale_for(float amax) {
 }
 
 // ---- which shape a product takes, and over how many workgroups its sum is split (host) -----------------------------------
-enum ShapeId { kSq, kFlat, kThin, kBig, kSmall };
+enum ShapeId { kSq, kThin, kBig, kSmall };
 typedef Shape<128, 128, 4, 2> Sq;
 typedef Shape<64, 64, 2, 2> Small;
 

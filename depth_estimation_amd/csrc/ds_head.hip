@@ -64,7 +64,11 @@ __global__ void head_init_kernel(HeadState* st, int rows) {
     st->amax_w = 0;
 }
 
-// rows kept per 16384 (only launched where one workgroup does not cover them all)
+// Up to four workgroups count what comes before them themselves: a launch (3 us of the host's time) less, and no slower (61440
+// rows: 13.9 us, against 7.0 and 6.4 in two launches; every further workgroup waits for 2 us more).
+constexpr int kListAlone = 4;
+
+// rows kept per 16384 (only launched for more workgroups than that)
 __global__ __launch_bounds__(kListT) void count_rows_kernel(const long long* __restrict__ target, int n, long long ignore,
                                                             int* __restrict__ counts) {
     __shared__ int s[kListT / 64];
@@ -98,13 +102,23 @@ __global__ __launch_bounds__(kListT) void list_rows_kernel(const long long* __re
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (threadIdx.x == 0) before = 0;
     __syncthreads();
+    long long t[kListPer];
     if (blockIdx.x > 0) {   // integer sums: any order gives the same
         int c = 0;
-        for (int i = threadIdx.x; i < (int)blockIdx.x; i += kListT) c += counts[i];
+        if (counts) {
+            for (int i = threadIdx.x; i < (int)blockIdx.x; i += kListT) c += counts[i];
+        } else {
+            for (int b = 0; b < (int)blockIdx.x; ++b) {      // whole blocks of rows
+#pragma unroll
+                for (int i = 0; i < kListPer; ++i) t[i] = target[b * kListBlock + i * kListT + threadIdx.x];
+#pragma unroll
+                for (int i = 0; i < kListPer; ++i) c += __popcll(__ballot(t[i] != ignore));
+            }
+            if (lane != 0) c = 0;
+        }
         if (c) atomicAdd(&before, c);
     }
     const long long base = (long long)blockIdx.x * kListBlock;
-    long long t[kListPer];
     unsigned long long m[kListPer];
 #pragma unroll
     for (int i = 0; i < kListPer; ++i) {
@@ -156,7 +170,8 @@ __global__ __launch_bounds__(kListT) void list_rows_kernel(const long long* __re
 static_assert(kListPer * kListT / 64 == 256, "the prefix handles four counts a lane");
 
 // --------------------------------------------------------------------------------------------------- staged operands
-// Row-wise passes over a matrix: a wave takes 64 / L rows at once, L lanes a row, VEC elements (16 bytes) a lane; L is the power of two that a row of D elements needs, at most 64.
+// Row-wise passes over a matrix: a wave takes 64 / L rows at once, L lanes a row, VEC elements (16 bytes) a lane; L is the power
+// of two that a row of D elements needs, at most 64.
 inline int lanes_for(int vectors) {
     int l = 1;
     while (l < vectors && l < 64) l <<= 1;
@@ -285,7 +300,12 @@ struct StatsArgs {
     float* part;
     long long plane;
     int ld_part;
+    int set_count;       // not 0: so many rows, and *st gets to know it here
 };
+__device__ __forceinline__ int rows_of(const StatsArgs& a, HeadState* st) {
+    if (a.set_count && blockIdx.x == 0 && threadIdx.x == 0) st->count = a.set_count;
+    return a.set_count ? a.set_count : st->count;
+}
 template <class S, int SPLIT, int MODE>
 __device__ __forceinline__ void stats_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int cnt, const HeadState* st,
                                               const StatsArgs& a, float* red) {
@@ -371,12 +391,12 @@ __device__ __forceinline__ void stats_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0
 }
 
 template <class T, class S, int SPLIT, int MODE>
-__global__ __launch_bounds__(S::T) void head_stats_kernel(Operand W, Operand H, const HeadState* __restrict__ st, int D,
+__global__ __launch_bounds__(S::T) void head_stats_kernel(Operand W, Operand H, HeadState* __restrict__ st, int D,
                                                           StatsArgs a) {
     __shared__ __align__(16) char lds[lds_bytes<S, kP<SPLIT>, kP<SPLIT>>()];
     const int vt = cdiv(a.V, S::BM);
     const int m0 = (int)(blockIdx.x % vt) * S::BM, n0 = (int)(blockIdx.x / vt) * S::BN;
-    const int cnt = st->count;
+    const int cnt = rows_of(a, st);
     if (n0 >= cnt) return;
     H.outer = cnt;
     f32x4 acc[S::FM][S::FN];
@@ -386,11 +406,11 @@ __global__ __launch_bounds__(S::T) void head_stats_kernel(Operand W, Operand H, 
 
 // the same in tiles of 256 x 256, a workgroup going through several
 template <class T, int SPLIT, int MODE>
-__global__ __launch_bounds__(Big::T) void head_stats_big_kernel(Operand W, Operand H, const HeadState* __restrict__ st, int D,
+__global__ __launch_bounds__(Big::T) void head_stats_big_kernel(Operand W, Operand H, HeadState* __restrict__ st, int D,
                                                                 StatsArgs a) {
     __shared__ __align__(16) char lds[Big::kLds];
     __shared__ float red[Big::WM * Big::BN * 3];
-    const int cnt = st->count, mt = cdiv(a.V, Big::BM), nt = cdiv(cnt, Big::BN), tiles = mt * nt;
+    const int cnt = rows_of(a, st), mt = cdiv(a.V, Big::BM), nt = cdiv(cnt, Big::BN), tiles = mt * nt;
     int t = blockIdx.x;
     if (t >= tiles) return;
     H.outer = cnt;
@@ -741,6 +761,9 @@ __global__ __launch_bounds__(S::T) void head_grad_kernel(Operand A, Operand B, c
 
 // sums the splits of a product in order, scales, and writes rows of the caller.  which: 0 = dH, 1 = dW.  PAR lanes share the
 // splits of an output (each a contiguous share, joined in order), for products of few outputs and many splits.
+// (16 of them: 80 x 64 outputs of 100000 rows 62 us a step against 83, 256 x 128 of 20000 56 against 61, 600 x 256 200 against
+// 196.)
+constexpr long long kShareOuts = 1 << 17;
 template <class T, int SPLIT, class O, int PAR>
 __global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__ part, long long part_split, int splits,
                                                        const HeadState* __restrict__ st, const BackState* __restrict__ bs, int n,
@@ -822,7 +845,7 @@ __global__ __launch_bounds__(256) void zero_ignored_kernel(Ignored g, int D, con
 // statistics, no barrier.  Backward the same: dl of 32 classes, as the matrix instruction leaves it, is the operand of
 // dH = dl W as it stands (its lanes hold rows, its registers classes, taken as k in the order 4 q + e of two fragments; the
 // transposing LDS reads of W follow that order), so dH needs no second pass; dl itself is written once for dW.
-//   12 x 96 x 320 rows, 64 features, 80 bins, bf16, forward: 48 -> SLIMF us (47 MB of features)
+//   12 x 96 x 320 rows, 64 features, 80 bins, bf16, forward 20 us (47 MB of features; the tiles above: 48)
 constexpr int kSlimT = 512;
 struct SlimArgs {
     const void* h;             // features: the caller's rows, or staged ones
@@ -1134,10 +1157,10 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
 
 // ----------------------------------------------------------------------------------------------------------- few rows
 //
-// Up to eight rows (a single position answered) read the weight once and are bound by that: every class row goes straight from
+// Up to four rows (a single position answered) read the weight once and are bound by that: every class row goes straight from
 // memory to registers, as it is (fp32 too: no planes), and meets the rows' features out of LDS in fp32.  L lanes share a
 // class, four classes a group are under way at a time.
-constexpr int kFewT = 512, kFewMax = 8;
+constexpr int kFewT = 512, kFewMax = 4;
 struct FewArgs {
     const int* rows;
     HeadState* st;
@@ -1283,9 +1306,9 @@ __global__ __launch_bounds__(1024) void join_few_kernel(JoinArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
-// Shapes: 256x256 outputs a workgroup (TileStream) for large products; 128x128, four waves of 64x64, below that; 64 features or
-// 32 rows have shapes of their own, whose idle half would otherwise be computed and dropped.
-typedef Shape<64, 128, 1, 4> Flat;    // 64 along m
+// Shapes: 256x256 outputs a workgroup (TileStream) for large products; 128x128 below that; up to 32 rows have a shape of their
+// own, most of whose work would otherwise be dropped (a training step of 16 rows: 65536 classes of 1024 features, bf16, 127
+// us against 142; 1000 of 256, float32, 48 against 54).
 typedef Shape<128, 32, 4, 1> Thin;    // 32 along n
 Cut cut_of(long long M, long long N, long long K, int planes, bool may_split) {
     return ds::cut_of([&](long long b) { return ((M + b - 1) / b) * ((N + b - 1) / b); }, (double)M * N, K, planes == 2 ? 3 : 1, may_split,
@@ -1342,9 +1365,12 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     p.Dp = pad8(D);
     p.stage_w = dtype == DS_F32 || D % 8 != 0;
     const size_t el = 2 * p.planes;
-    const bool thin = N <= 32, flat = D <= 64;
-    // few rows: their features have to fit LDS in fp32 beside three more workgroups
-    p.few = N > kFewMax ? 0 : N <= 1 ? 1 : N <= 2 ? 2 : N <= 4 ? 4 : 8;
+    const bool thin = N <= 32;
+    // few rows of a weight that would have to be packed first (20000 classes of 256 features, float32, 1 / 4 / 8 rows: 18 / 30
+    // / 76 us here, 39 / 39 / 40 packed and multiplied); a 16-bit weight is read as it is by the matrix instructions as well
+    // (65536 of 1024, bf16: 39 / 70 / 177 us here, 36 / 36 / 39 there).  Their features have to fit LDS in fp32 beside three
+    // more workgroups.
+    p.few = N > kFewMax || !p.stage_w ? 0 : N <= 1 ? 1 : N <= 2 ? 2 : 4;
     if (p.few && (size_t)p.few * pad8(D) * 4 > 40 * 1024) p.few = 0;
     const int vec = dtype == DS_F32 ? 4 : 8, lanes = lanes_for(cdiv(D, vec));
     p.few_grid = cdiv(V, kFewT / lanes * 4) < 2 * cu_count() ? cdiv(V, kFewT / lanes * 4) : 2 * cu_count();
@@ -1383,12 +1409,10 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     p.piece_ld = pad8(p.piece);
     p.dl_shape = thin ? kThin : cut_of(p.piece, N, D, p.planes, false).shape;
     const Cut dh = cut_of(D, N, p.piece, p.planes, true), dw = cut_of(D, p.piece, N, p.planes, true);
-    p.dh = thin ? kThin : flat ? kFlat : dh.shape;
-    p.dh_splits = p.dh == dh.shape ? dh.splits
-                                   : splits_for((long long)cdiv(D, flat && !thin ? 64 : 128) * cdiv(N, thin ? 32 : 128),
-                                                cdiv(p.piece, kBK));
-    p.dw = flat ? kFlat : dw.shape;
-    p.dw_splits = p.dw == dw.shape ? dw.splits : splits_for((long long)cdiv(D, 64) * cdiv(p.piece, 128), cdiv(N, kBK));
+    p.dh = thin ? kThin : dh.shape;
+    p.dh_splits = thin ? splits_for(cdiv(D, 128), cdiv(p.piece, kBK)) : dh.splits;
+    p.dw = dw.shape;
+    p.dw_splits = dw.splits;
     p.dh_part = p.dh_splits > 1 || p.piece < V;
     const size_t D4 = (D + 3) & ~3;
     o = 0;
@@ -1517,14 +1541,14 @@ int head_fwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
     const int* rows = nullptr;
     if (mode == kCE) {
         const int nb = cdiv(N, kListBlock);
-        int* counts = reinterpret_cast<int*>(ws + p.counts);
-        if (nb > 1) count_rows_kernel<<<nb, kListT, 0, q>>>(target, (int)N, ignore, counts);
+        int* counts = nb > kListAlone ? reinterpret_cast<int*>(ws + p.counts) : nullptr;
+        if (counts) count_rows_kernel<<<nb, kListT, 0, q>>>(target, (int)N, ignore, counts);
         list_rows_kernel<<<nb, kListT, 0, q>>>(target, (int)N, V, ignore, counts, s.st, s.rows, s.tgt,
                                                reduction == DS_REDUCE_NONE ? out : nullptr);
         rows = s.rows;
     }
     // expectation: all rows; the count is written by the first kernel that runs
-    const bool set_count = mode == kExpect && (p.few || (p.slim && !p.stage_h));
+    const bool set_count = mode == kExpect && (p.few || !p.stage_h);
     if (mode == kExpect && !set_count) head_init_kernel<<<1, 1, 0, q>>>(s.st, (int)N);
     float* part = reinterpret_cast<float*>(ws + p.part);
     float* tlogit = reinterpret_cast<float*>(ws + p.tlogit);
@@ -1542,8 +1566,7 @@ int head_fwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
         const FewArgs fa{rows, s.st, set_count, (int)N, D, V, 0, mode == kCE ? s.tgt : nullptr, centers, part};
         p.few == 1   ? few_launch<IT, 1>(p, hidden, ldh, weight, fa, q)
         : p.few == 2 ? few_launch<IT, 2>(p, hidden, ldh, weight, fa, q)
-        : p.few == 4 ? few_launch<IT, 4>(p, hidden, ldh, weight, fa, q)
-                     : few_launch<IT, 8>(p, hidden, ldh, weight, fa, q);
+                     : few_launch<IT, 4>(p, hidden, ldh, weight, fa, q);
         ja.mx = part;
         ja.s = part + 1;
         ja.sc = part + 2;
@@ -1567,7 +1590,8 @@ int head_fwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
         if (sums) loss_total_kernel<<<1, 256, 0, q>>>(sums, s.st, reduction == DS_REDUCE_MEAN, p.slim_grid, out);
         return launched();
     }
-    const StatsArgs sa{V, s.tgt, centers, tlogit, part, (long long)(align256((size_t)p.vt_fwd * N * 4) / 4), (int)N};
+    const StatsArgs sa{V, s.tgt, centers, tlogit, part, (long long)(align256((size_t)p.vt_fwd * N * 4) / 4), (int)N,
+                       set_count ? (int)N : 0};
     if (mode == kCE)
         stats_launch<T, SPLIT, kCE>(p, W, H, s, N, D, sa, q);
     else
@@ -1616,8 +1640,6 @@ void grad_launch(ShapeId shape, bool acc, const Operand& A, const Operand& B, co
                  const GradArgs& a, hipStream_t q) {
     if (WHICH == 0 && shape == kThin)
         grad_shape<IT, T, Thin, SPLIT, 0>(acc, A, B, s, bs, n, a, q);
-    else if (shape == kFlat)
-        grad_shape<IT, T, Flat, SPLIT, WHICH>(acc, A, B, s, bs, n, a, q);
     else if (shape == kBig)
         grad_shape<IT, T, Big, SPLIT, WHICH>(acc, A, B, s, bs, n, a, q);
     else
@@ -1685,7 +1707,7 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
             IT* gw = g_weight + (long long)v0 * D;
             const GradArgs ga{D, cols, p.dw_splits, mode, cols, 1, nullptr, gw, dwp, (long long)p.piece * D4, up};
             grad_launch<IT, T, SPLIT, 1>(p.dw, p.dw_splits > 1, H, G, s, bs, cols, ga, q);
-            if (p.dw_splits > 8)
+            if (p.dw_splits > 8 && (long long)cols * D4 <= kShareOuts)
                 head_sum_kernel<T, SPLIT, IT, 16><<<cdiv((long long)cols * D4 / 4, 16), 256, 0, q>>>(
                     dwp, (long long)p.piece * D4, p.dw_splits, s.st, bs, cols, D, mode, 1, up, nullptr, gw);
             else if (p.dw_splits > 1)
@@ -1694,7 +1716,7 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
         }
     }
     if (g_hidden && p.dh_part && !p.slim_back) {
-        const bool many = p.dh_splits > 8;
+        const bool many = p.dh_splits > 8 && N * D4 <= kShareOuts;
         const int blocks = cdiv(N * (D4 / 4), many ? 16 : 256), grid = blocks < 16384 ? blocks : 16384;
         if (many)
             head_sum_kernel<T, SPLIT, IT, 16><<<grid, 256, 0, q>>>(dhp, N * D4, p.dh_splits, s.st, bs, (int)N, D, mode, 0, up, rows,

@@ -670,8 +670,9 @@ OrthoPlan ortho_plan(int dtype, int batch, int m, int n) {
     p.sp = pad8(p.s);
     p.np = pad8(n);
     p.blocks = norm_blocks((long long)m * n);
-    // below a side of 256 launches and latency are what a step takes, not products
-    p.light = dtype == DS_BF16 && p.s >= 256;
+    // on smaller sides launches and latency are what a step takes, not products (five steps of 256 x 1024: 149 us so, 145
+    // with all planes; 512 x 512 150 and 166, 1024 x 1024 229 and 254, 2048 x 2048 505 and 759)
+    p.light = dtype == DS_BF16 && p.s >= 512;
     auto cut = [&](int M, int N, int K, int pairs, bool tri) {
         return cut_of(
             [&](long long b) {

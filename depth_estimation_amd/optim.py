@@ -16,7 +16,7 @@ COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # steep at zero: five steps bring sin
 def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7) -> torch.Tensor:
     """update (...,m,n) float32, float16 or bfloat16 on the GPU -> same shape and dtype: X = G / (|G|_F + eps), then `steps`
     (0..32) times X = (a I + b A + c A A) X with A = X X^T on the smaller side.  No gradient flows.  Products on 22-bit
-    operands with float32 sums, one rounding at the end; bfloat16 matrices with sides of 256 and more take 11-bit operands
+    operands with float32 sums, one rounding at the end; bfloat16 matrices with sides of 512 and more take 11-bit operands
     where that costs less than the rounding of the result does.  The coefficients must keep singular values of
     [0,1] below 4 (the default: below 1.3)."""
     return ops.orthogonalize(update, steps, coefficients, eps)

@@ -334,7 +334,7 @@ int ds_bin_expect_bwd(const void* hidden, long long ldh, const void* weight, con
 /* An update orthogonalised by Newton-Schulz products: X = G / (|G|_F + eps); `steps` times, on the smaller side,
  * A = X X^T, X = (a + b A + c A A) X.  update and out: batch matrices (m,n), contiguous, of type `dtype`; out = update is
  * allowed.  coefficients: HOST double[3] a, b, c.  Products as for fp32 heads (22-bit operands, fp32 sums) for every dtype,
- * one rounding at the end; bf16 matrices whose smaller side is 256 or more take 11-bit operands where that costs less than
+ * one rounding at the end; bf16 matrices whose smaller side is 512 or more take 11-bit operands where that costs less than
  * the rounding to bf16 does.  workspace (16-byte aligned) from ds_orthogonalize_workspace_bytes. */
 size_t ds_orthogonalize_workspace_bytes(int dtype, int batch, int m, int n);
 int ds_orthogonalize(const void* update, int dtype, int batch, int m, int n, int steps, const double* coefficients, double eps,

@@ -591,3 +591,19 @@ def test_refusals_of_tensors():
     wide = torch.empty(2 ** 32 + 5, 1, dtype=torch.float16, device=DEV)      # as a 32-bit number of classes: five
     with pytest.raises(RuntimeError, match="too large"):
         metrics.linear_cross_entropy(h[:, :1].half(), wide, t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [16384, 16385, 40000, 131072, 131073, 300000])
+def test_many_rows_are_listed_in_order(n):
+    """Rows left out here and there: every kept row's loss and gradient comes back to its own place."""
+    d, v = 8, 4
+    h, w, t, up, _ = _data(n, d, v, torch.float32, seed=n, keep=0.37)
+    out, gh, gw, tol, th, tw = _oracle(h, w, t=t, up=up)
+    got = _ce(h, w, t, "none", up)
+    _close(got[0], out, tol, "loss")
+    _close(got[1], gh, th, "g_hidden")
+    _close(got[2], gw, tw, "g_weight")
+    mean = _ce(h, w, t, "mean")[0].double()
+    kept = t != -100
+    assert abs(float(mean - out[kept].mean())) <= float(tol[kept].mean()) + 2.0 ** -23 * float(mean)

@@ -77,9 +77,9 @@ def test_larger_tiles(shape):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["gauss", "decay", "few"])
-@pytest.mark.parametrize("shape", [(256, 256), (256, 1000), (1001, 259), (2, 300, 530), (700, 700), (2300, 2100)], ids=str)
+@pytest.mark.parametrize("shape", [(256, 256), (256, 1000), (1001, 259), (2, 300, 530), (512, 512), (2, 513, 1031), (700, 700), (1500, 650), (2300, 2100)], ids=str)
 def test_bfloat16_with_fewer_products(shape, kind):
-    """Sides of 256 and more: 11-bit operands.  Rounding the result alone is off by 2^-8 / sqrt(3) at most in norm (1.7e-3 for
+    """Sides of 512 and more: 11-bit operands (22 below).  Rounding the result alone is off by 2^-8 / sqrt(3) at most in norm (1.7e-3 for
     numbers spread evenly between powers of two), the operands' rounding by less (9e-4 was the most over these spectra when
     the arithmetic was written out in float64): together at most sqrt(1.7^2 + 1.1^2) 1e-3 = 2.0e-3 with some room, against
     half a step of bfloat16, 3.9e-3."""
