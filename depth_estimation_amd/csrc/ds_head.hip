@@ -1310,9 +1310,9 @@ __global__ __launch_bounds__(1024) void join_few_kernel(JoinArgs a) {
 // own, most of whose work would otherwise be dropped (a training step of 16 rows: 65536 classes of 1024 features, bf16, 127
 // us against 142; 1000 of 256, float32, 48 against 54).
 typedef Shape<128, 32, 4, 1> Thin;    // 32 along n
-Cut cut_of(long long M, long long N, long long K, int planes, bool may_split) {
+Cut cut_of(long long M, long long N, long long K, int planes, bool may_split, bool small_too) {
     return ds::cut_of([&](long long b) { return ((M + b - 1) / b) * ((N + b - 1) / b); }, (double)M * N, K, planes == 2 ? 3 : 1, may_split,
-                      false, cu_count());
+                      small_too, cu_count());
 }
 
 bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
@@ -1389,7 +1389,7 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     const size_t h = align256((size_t)N * p.Dp * el), w = p.stage_w ? align256((size_t)V * p.Dp * el) : 0;
     // what the forward stages is kept for the backward (staging 50021 classes of 771 features once more: 35 of 490 us); few
     // rows are read as they are
-    p.fwd = thin ? kThin : cut_of(V, N, D, p.planes, false).shape;
+    p.fwd = thin ? kThin : cut_of(V, N, D, p.planes, false, false).shape;
     p.vt_fwd = cdiv(V, p.fwd == kBig ? Big::BM : Sq::BM);
     size_t o = saved_bytes(N);
     p.sh = o; o += p.stage_h && !p.few ? h : 0;
@@ -1407,8 +1407,8 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     const long long piece = p.slim_back ? V : fit < 1024 ? 1024 : fit;
     p.piece = piece >= V ? V : (int)piece;
     p.piece_ld = pad8(p.piece);
-    p.dl_shape = thin ? kThin : cut_of(p.piece, N, D, p.planes, false).shape;
-    const Cut dh = cut_of(D, N, p.piece, p.planes, true), dw = cut_of(D, p.piece, N, p.planes, true);
+    p.dl_shape = thin ? kThin : cut_of(p.piece, N, D, p.planes, false, false).shape;
+    const Cut dh = cut_of(D, N, p.piece, p.planes, true, true), dw = cut_of(D, p.piece, N, p.planes, true, true);
     p.dh = thin ? kThin : dh.shape;
     p.dh_splits = thin ? splits_for(cdiv(D, 128), cdiv(p.piece, kBK)) : dh.splits;
     p.dw = dw.shape;
@@ -1642,6 +1642,8 @@ void grad_launch(ShapeId shape, bool acc, const Operand& A, const Operand& B, co
         grad_shape<IT, T, Thin, SPLIT, 0>(acc, A, B, s, bs, n, a, q);
     else if (shape == kBig)
         grad_shape<IT, T, Big, SPLIT, WHICH>(acc, A, B, s, bs, n, a, q);
+    else if (shape == kSmall)
+        grad_shape<IT, T, Small, SPLIT, WHICH>(acc, A, B, s, bs, n, a, q);
     else
         grad_shape<IT, T, Sq, SPLIT, WHICH>(acc, A, B, s, bs, n, a, q);
 }
