@@ -551,13 +551,15 @@ enum ShapeId { kSq, kThin, kBig, kSmall };
 typedef Shape<128, 128, 4, 2> Sq;
 typedef Shape<64, 64, 2, 2> Small;
 
+inline int side_of(ShapeId s) { return s == kBig ? Big::BM : s == kSmall ? Small::BM : Sq::BM; }   // Thin: along m
+
 struct Cut {
     ShapeId shape;
     int splits;
 };
 // tiles(b): tiles of b x b; area: outputs; pairs: products a step (three of two planes each, two of two planes and one).
 template <class Tiles>
-inline Cut cut_of(Tiles tiles, double area, long long K, int pairs, bool may_split, bool small_too, int cus) {
+inline Cut cut_of(Tiles tiles, double area, long long K, int pairs, bool may_split, int cus) {
     // us a step of 64 k: `step` of a CU's time with `at_once` workgroups on it, `alone` at least; `ends`: start and end of a
     // tile.  Measured at k = 512 and 2048 with half a workgroup to sixteen a CU; in TFLOP/s of 16-bit products with the chip
     // full: 256 x 256 tiles 1330, 128 x 128 870, 64 x 64 660; three products a step 1365, 1160, 780 (two: between).
@@ -572,7 +574,7 @@ inline Cut cut_of(Tiles tiles, double area, long long K, int pairs, bool may_spl
     const long long steps = (K + kBK - 1) / kBK, most = may_split ? (steps < 256 ? steps : 256) : 1;
     Cut best{kSq, 1};
     double least = 1e300;
-    for (int c = 0; c < (small_too ? 3 : 2); ++c) {
+    for (int c = 0; c < 3; ++c) {
         const Cost& q = pairs == 1 ? one[c] : pairs == 2 ? two[c] : three[c];
         const long long t = tiles(q.b);
         for (long long s = 1; s <= most; s += s < 16 ? 1 : s / 8) {

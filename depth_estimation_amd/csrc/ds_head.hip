@@ -445,13 +445,29 @@ __global__ __launch_bounds__(256) void head_join_kernel(const float* __restrict_
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5, n = blockIdx.x * 32 + x;
     const int cnt = st->count;
     float mx = -INFINITY, s = 0.f, sc = 0.f;
+    constexpr int U = 8;        // tiles under way at a time
     if (n < cnt)
-        for (int t = y; t < tiles; t += 8) {
-            const float* q = part + (long long)t * ld_part + n;
-            const float m = q[0], nm = fmaxf(mx, m), ref = nm == -INFINITY ? 0.f : nm;
-            const float f0 = exp_of(mx - ref), f1 = exp_of(m - ref);
-            s = s * f0 + q[plane] * f1;
-            if (mode == kExpect) sc = sc * f0 + q[2 * plane] * f1;
+        for (int t0 = y; t0 < tiles; t0 += 8 * U) {
+            float m[U], a[U], c[U], nm = mx;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const bool in = t0 + u * 8 < tiles;
+                const float* q = part + (long long)(t0 + u * 8) * ld_part + n;
+                m[u] = in ? q[0] : -INFINITY;
+                a[u] = in ? q[plane] : 0.f;
+                c[u] = in && mode == kExpect ? q[2 * plane] : 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) nm = fmaxf(nm, m[u]);
+            const float ref = nm == -INFINITY ? 0.f : nm, f0 = exp_of(mx - ref);
+            s *= f0;
+            sc *= f0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float f = exp_of(m[u] - ref);
+                s = fmaf(a[u], f, s);
+                sc = fmaf(c[u], f, sc);
+            }
             mx = nm;
         }
     red[y][x][0] = mx;
@@ -1306,13 +1322,13 @@ __global__ __launch_bounds__(1024) void join_few_kernel(JoinArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
-// Shapes: 256x256 outputs a workgroup (TileStream) for large products; 128x128 below that; up to 32 rows have a shape of their
+// Shapes: 256x256 outputs a workgroup (TileStream) for large products; 128x128 and 64x64 below that; up to 32 rows have a shape of their
 // own, most of whose work would otherwise be dropped (a training step of 16 rows: 65536 classes of 1024 features, bf16, 127
 // us against 142; 1000 of 256, float32, 48 against 54).
 typedef Shape<128, 32, 4, 1> Thin;    // 32 along n
-Cut cut_of(long long M, long long N, long long K, int planes, bool may_split, bool small_too) {
+Cut cut_of(long long M, long long N, long long K, int planes, bool may_split) {
     return ds::cut_of([&](long long b) { return ((M + b - 1) / b) * ((N + b - 1) / b); }, (double)M * N, K, planes == 2 ? 3 : 1, may_split,
-                      small_too, cu_count());
+                      cu_count());
 }
 
 bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
@@ -1389,8 +1405,8 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     const size_t h = align256((size_t)N * p.Dp * el), w = p.stage_w ? align256((size_t)V * p.Dp * el) : 0;
     // what the forward stages is kept for the backward (staging 50021 classes of 771 features once more: 35 of 490 us); few
     // rows are read as they are
-    p.fwd = thin ? kThin : cut_of(V, N, D, p.planes, false, false).shape;
-    p.vt_fwd = cdiv(V, p.fwd == kBig ? Big::BM : Sq::BM);
+    p.fwd = thin ? kThin : cut_of(V, N, D, p.planes, false).shape;
+    p.vt_fwd = cdiv(V, side_of(p.fwd));
     size_t o = saved_bytes(N);
     p.sh = o; o += p.stage_h && !p.few ? h : 0;
     p.sw = o; o += p.few ? 0 : w;
@@ -1407,8 +1423,8 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     const long long piece = p.slim_back ? V : fit < 1024 ? 1024 : fit;
     p.piece = piece >= V ? V : (int)piece;
     p.piece_ld = pad8(p.piece);
-    p.dl_shape = thin ? kThin : cut_of(p.piece, N, D, p.planes, false, false).shape;
-    const Cut dh = cut_of(D, N, p.piece, p.planes, true, true), dw = cut_of(D, p.piece, N, p.planes, true, true);
+    p.dl_shape = thin ? kThin : cut_of(p.piece, N, D, p.planes, false).shape;
+    const Cut dh = cut_of(D, N, p.piece, p.planes, true), dw = cut_of(D, p.piece, N, p.planes, true);
     p.dh = thin ? kThin : dh.shape;
     p.dh_splits = thin ? splits_for(cdiv(D, 128), cdiv(p.piece, kBK)) : dh.splits;
     p.dw = dw.shape;
@@ -1525,11 +1541,13 @@ void few_launch(const Plan& p, const IT* h, long long ldh, const IT* w, FewArgs 
 template <class T, int SPLIT, int MODE>
 void stats_launch(const Plan& p, const Operand& W, const Operand& H, const Saved& s, long long N, int D, const StatsArgs& a,
                   hipStream_t q) {
-    const int tiles = p.vt_fwd * cdiv(N, p.fwd == kThin ? 32 : p.fwd == kBig ? Big::BN : 128);
+    const int tiles = p.vt_fwd * cdiv(N, p.fwd == kThin ? Thin::BN : side_of(p.fwd));
     if (p.fwd == kThin)
         head_stats_kernel<T, Thin, SPLIT, MODE><<<tiles, Thin::T, 0, q>>>(W, H, s.st, D, a);
     else if (p.fwd == kBig)
         head_stats_big_kernel<T, SPLIT, MODE><<<tiles < cu_count() ? tiles : cu_count(), Big::T, 0, q>>>(W, H, s.st, D, a);
+    else if (p.fwd == kSmall)
+        head_stats_kernel<T, Small, SPLIT, MODE><<<tiles, Small::T, 0, q>>>(W, H, s.st, D, a);
     else
         head_stats_kernel<T, Sq, SPLIT, MODE><<<tiles, Sq::T, 0, q>>>(W, H, s.st, D, a);
 }
@@ -1616,12 +1634,13 @@ int head_fwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
 template <class T, int SPLIT, int MODE>
 void dl_launch(const Plan& p, const Operand& W, const Operand& H, const Saved& s, const BackState* bs, long long N, int D,
                const DlArgs& a, hipStream_t q) {
-    const int b = p.dl_shape == kBig ? Big::BM : 128;
-    const int tiles = cdiv(a.cols, b) * cdiv(N, p.dl_shape == kThin ? 32 : b);
+    const int tiles = cdiv(a.cols, side_of(p.dl_shape)) * cdiv(N, p.dl_shape == kThin ? Thin::BN : side_of(p.dl_shape));
     if (p.dl_shape == kThin)
         head_dl_kernel<T, Thin, SPLIT, MODE><<<tiles, Thin::T, 0, q>>>(W, H, s.st, bs, D, a);
     else if (p.dl_shape == kBig)
         head_dl_big_kernel<T, SPLIT, MODE><<<tiles < cu_count() ? tiles : cu_count(), Big::T, 0, q>>>(W, H, s.st, bs, D, a);
+    else if (p.dl_shape == kSmall)
+        head_dl_kernel<T, Small, SPLIT, MODE><<<tiles, Small::T, 0, q>>>(W, H, s.st, bs, D, a);
     else
         head_dl_kernel<T, Sq, SPLIT, MODE><<<tiles, Sq::T, 0, q>>>(W, H, s.st, bs, D, a);
 }

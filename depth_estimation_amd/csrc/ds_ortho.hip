@@ -656,11 +656,11 @@ struct OrthoPlan {
     size_t norm, x0, x1, a, b, da, part, total;
 };
 int tiles_of(ShapeId id, int M, int N, bool tri) {
-    const int b = id == kBig ? 256 : id == kSq ? 128 : 64, m = cdiv(M, b), n = cdiv(N, b);
+    const int b = side_of(id), m = cdiv(M, b), n = cdiv(N, b);
     return tri ? m * (m + 1) / 2 : m * n;
 }
 size_t part_bytes(const Cut& c, int M, int N, bool tri, int batch) {
-    const size_t b = c.shape == kBig ? 256 : c.shape == kSq ? 128 : 64;
+    const size_t b = side_of(c.shape);
     return c.splits > 1 ? (size_t)batch * tiles_of(c.shape, M, N, tri) * c.splits * b * b * 4 : 0;
 }
 OrthoPlan ortho_plan(int dtype, int batch, int m, int n) {
@@ -679,7 +679,7 @@ OrthoPlan ortho_plan(int dtype, int batch, int m, int n) {
                 const long long x = (M + b - 1) / b, y = (N + b - 1) / b;
                 return batch * (tri ? x * (x + 1) / 2 : x * y);
             },
-            (double)M * N * batch * (tri ? 0.5 : 1.0), K, pairs, true, true, cu_count());
+            (double)M * N * batch * (tri ? 0.5 : 1.0), K, pairs, true, cu_count());
     };
     p.gram = cut(p.s, p.s, p.l, p.light ? 1 : 3, true);
     p.poly = cut(p.s, p.s, p.s, p.light ? 1 : 3, true);
@@ -736,7 +736,7 @@ void product_shape(ProductArgs p, const UseArgs& u, int tiles, hipStream_t q) {
 template <Lay LA, Lay LB, int PA, int PB, class H, class O>
 void product(const Cut& c, ProductArgs p, const UseArgs& u, int M, int N, hipStream_t q) {
     p.splits = c.splits;
-    const int b = c.shape == kBig ? 256 : c.shape == kSq ? 128 : 64, tiles = tiles_of(c.shape, M, N, p.tri) * p.batch;
+    const int b = side_of(c.shape), tiles = tiles_of(c.shape, M, N, p.tri) * p.batch;
     p.mt = cdiv(M, b);
     p.nt = cdiv(N, b);
     if (c.shape == kBig)
