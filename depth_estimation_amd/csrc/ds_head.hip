@@ -196,14 +196,15 @@ __device__ __forceinline__ void load_vec(const IT* row, int d, int D, IT (&x)[VE
     }
 }
 
-// max |x| over the rows of two matrices (one launch): `cnt` of the first one's, listed in `rows` if given, all n1 of the
-// second's; order-independent, so repeatable
+// max |x| over the rows of two matrices (one launch): the first one's kept rows, listed in `rows` if given, all of the second's;
+// order-independent, so repeatable.  A workgroup each (alone) writes what it finds, and the row count if set_count gives it;
+// else *st was cleared before.
 template <class IT, int VEC>
 __global__ __launch_bounds__(256) void amax_kernel(const IT* __restrict__ x, long long ld, const int* __restrict__ rows,
                                                    HeadState* __restrict__ st, const IT* __restrict__ w, int V, int D, int L,
-                                                   int blocks_x) {
-    const bool second = (int)blockIdx.x >= blocks_x;
-    const int c = second ? V : st->count, b = second ? blockIdx.x - blocks_x : blockIdx.x;
+                                                   int blocks_x, int set_count) {
+    const bool second = (int)blockIdx.x >= blocks_x, alone = gridDim.x == 2;
+    const int c = second ? V : set_count ? set_count : st->count, b = second ? blockIdx.x - blocks_x : blockIdx.x;
     const int nb = second ? gridDim.x - blocks_x : blocks_x;
     const IT* src = second ? w : x;
     const long long pitch = second ? D : ld;
@@ -230,7 +231,9 @@ __global__ __launch_bounds__(256) void amax_kernel(const IT* __restrict__ x, lon
     // one atomic a workgroup: they all meet in one place, 20 ns each
     if (threadIdx.x == 0) {
         m = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-        if (m > 0.f) atomicMax(second ? &st->amax_w : &st->amax_h, __builtin_bit_cast(unsigned, m));
+        if (alone) (second ? st->amax_w : st->amax_h) = __builtin_bit_cast(unsigned, m);
+        if (alone && set_count && !second) st->count = set_count;
+        if (!alone && m > 0.f) atomicMax(second ? &st->amax_w : &st->amax_h, __builtin_bit_cast(unsigned, m));
     }
 }
 
@@ -556,18 +559,36 @@ __device__ __forceinline__ float dl_norm(const BackState* bs, const Upstream& u,
     return mode == kExpect ? g * pow2_above(2.f * from_bits(bs->cmax)) : g;
 }
 
-// largest |upstream| and |centre|, where dl_norm asks for them; *bs zeroed by back_init_kernel before
+// largest |upstream| and |centre|, where dl_norm asks for them; *bs zeroed by back_init_kernel before, unless one workgroup
+// does it all (a launch less)
+constexpr int kScaleT = 512, kScaleAlone = 16 * kScaleT;
 __global__ void back_init_kernel(BackState* bs) { bs->gmax = bs->cmax = 0; }
-__global__ __launch_bounds__(256) void back_scale_kernel(Upstream u, const HeadState* __restrict__ st,
+__global__ __launch_bounds__(kScaleT) void back_scale_kernel(Upstream u, const HeadState* __restrict__ st,
                                                          const float* __restrict__ centers, int V, BackState* __restrict__ bs) {
-    const int cnt = st->count, step = gridDim.x * 256, i0 = blockIdx.x * 256 + threadIdx.x;
+    __shared__ float red[kScaleT / 64][2];
+    const int cnt = st->count, step = gridDim.x * kScaleT, i0 = blockIdx.x * kScaleT + threadIdx.x;
     float g = 0.f, c = 0.f;
-    for (int n = i0; n < (u.each ? cnt : min(cnt, 1)); n += step) g = fmaxf(g, finite_abs(upstream(u, n, cnt)));
+#pragma unroll 4
+    for (int n = i0; n < cnt; n += step) g = fmaxf(g, finite_abs(upstream(u, n, cnt)));
     if (centers)
+#pragma unroll 4
         for (int v = i0; v < V; v += step) c = fmaxf(c, finite_abs(centers[v]));
     g = wave_max(g);
     c = wave_max(c);
     if ((threadIdx.x & 63) == 0) {
+        red[threadIdx.x >> 6][0] = g;
+        red[threadIdx.x >> 6][1] = c;
+    }
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int i = 1; i < kScaleT / 64; ++i) {
+        g = fmaxf(g, red[i][0]);
+        c = fmaxf(c, red[i][1]);
+    }
+    if (gridDim.x == 1) {
+        bs->gmax = __builtin_bit_cast(unsigned, g);
+        bs->cmax = __builtin_bit_cast(unsigned, c);
+    } else {
         if (g > 0.f) atomicMax(&bs->gmax, __builtin_bit_cast(unsigned, g));
         if (c > 0.f) atomicMax(&bs->cmax, __builtin_bit_cast(unsigned, c));
     }
@@ -1455,21 +1476,23 @@ int launched() {
     return e == hipSuccess ? DS_OK : (int)e;
 }
 
-// scales of fp32 inputs (st->amax_h, amax_w; zeroed before)
+// scales of fp32 inputs (st->amax_h, amax_w); `clear`: all N rows, and *st is not cleared yet
 template <class IT>
 void scales(const IT* hidden, long long ldh, const int* rows, const IT* weight, long long N, int D, int V, HeadState* st,
-            hipStream_t q) {
+            bool clear, hipStream_t q) {
     constexpr int VEC = 16 / sizeof(IT);
     const int L = lanes_for(cdiv(D, VEC)), per = 4 * 64 / L * 4;
-    const int bx = cdiv(N, per) < 512 ? cdiv(N, per) : 512, bw = cdiv(V, per) < 512 ? cdiv(V, per) : 512;
-    amax_kernel<IT, VEC><<<bx + bw, 256, 0, q>>>(hidden, ldh, rows, st, weight, V, D, L, bx);
+    const bool alone = cdiv(N, per) <= 4 && cdiv(V, per) <= 4;      // a pass of loads takes less than a launch
+    const int bx = alone ? 1 : cdiv(N, per) < 512 ? cdiv(N, per) : 512, bw = alone ? 1 : cdiv(V, per) < 512 ? cdiv(V, per) : 512;
+    if (clear && bx + bw > 2) head_init_kernel<<<1, 1, 0, q>>>(st, (int)N);
+    amax_kernel<IT, VEC><<<bx + bw, 256, 0, q>>>(hidden, ldh, rows, st, weight, V, D, L, bx, clear ? (int)N : 0);
 }
-// inputs as matrix operands: in place, or staged at wh and ww (stage: now)
+// inputs as matrix operands: in place, or staged at wh and ww (stage: now; clear: *s.st is not set yet)
 template <class IT, class T, int SPLIT>
 void operands(const Plan& p, const IT* hidden, long long ldh, const IT* weight, long long N, int D, int V, const Saved& s,
-              const int* rows, bool stage, char* wh, char* ww, Operand& H, Operand& W, hipStream_t q) {
+              const int* rows, bool stage, bool clear, char* wh, char* ww, Operand& H, Operand& W, hipStream_t q) {
     if constexpr (SPLIT == 3)
-        if (stage) scales(hidden, ldh, rows, weight, N, D, V, s.st, q);
+        if (stage) scales(hidden, ldh, rows, weight, N, D, V, s.st, clear, q);
     H = Operand{hidden, ldh, 0, (int)N, D};
     W = Operand{weight, D, 0, V, D};
     constexpr int VEC = 16 / sizeof(IT);
@@ -1567,7 +1590,8 @@ int head_fwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
     }
     // expectation: all rows; the count is written by the first kernel that runs
     const bool set_count = mode == kExpect && (p.few || !p.stage_h);
-    if (mode == kExpect && !set_count) head_init_kernel<<<1, 1, 0, q>>>(s.st, (int)N);
+    const bool clear = mode == kExpect && !set_count;
+    if (clear && SPLIT != 3) head_init_kernel<<<1, 1, 0, q>>>(s.st, (int)N);
     float* part = reinterpret_cast<float*>(ws + p.part);
     float* tlogit = reinterpret_cast<float*>(ws + p.tlogit);
     JoinArgs ja{};
@@ -1597,7 +1621,7 @@ int head_fwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
     }
     Operand H, W;
     char* keep = static_cast<char*>(saved);
-    operands<IT, T, SPLIT>(p, hidden, ldh, weight, N, D, V, s, rows, true, keep + p.sh, keep + p.sw, H, W, q);
+    operands<IT, T, SPLIT>(p, hidden, ldh, weight, N, D, V, s, rows, true, clear, keep + p.sh, keep + p.sw, H, W, q);
     double* sums = mode == kCE && reduction != DS_REDUCE_NONE ? reinterpret_cast<double*>(ws + p.sums) : nullptr;
     if (p.slim) {
         SlimArgs a = slim_args(p, H, W, s, rows, N, D, V, centers);
@@ -1675,16 +1699,17 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
     const int* rows = mode == kCE ? s.rows : nullptr;
     BackState* bs = reinterpret_cast<BackState*>(ws + p.bs);
     Upstream up{g, reduction == DS_REDUCE_NONE, reduction == DS_REDUCE_MEAN, rows};
-    if (!std::is_same<T, bf16>::value && (up.each || mode == kExpect)) {    // where dl_norm reads it
-        back_init_kernel<<<1, 1, 0, q>>>(bs);
-        const long long most = up.each && N > V ? N : V;
-        back_scale_kernel<<<cdiv(most, 2048) < 256 ? cdiv(most, 2048) : 256, 256, 0, q>>>(up, s.st, centers, V, bs);
+    if (!std::is_same<T, bf16>::value && up.each) {    // where dl_norm reads it
+        const long long most = centers && V > N ? V : N;
+        const int blocks = most <= kScaleAlone ? 1 : cdiv(most, 4 * kScaleT) < 256 ? cdiv(most, 4 * kScaleT) : 256;
+        if (blocks > 1) back_init_kernel<<<1, 1, 0, q>>>(bs);
+        back_scale_kernel<<<blocks, kScaleT, 0, q>>>(up, s.st, centers, V, bs);
     }
     // the forward of few rows stages nothing and leaves zero scales; the maximum that a second backward of the same forward,
     // maybe at the same time, finds there is the one that it forms itself
     Operand H, W;
     char* staged = p.few ? ws : static_cast<char*>(saved);
-    operands<IT, T, SPLIT>(p, hidden, ldh, weight, N, D, V, s, rows, p.few != 0, staged + (p.few ? p.bh : p.sh),
+    operands<IT, T, SPLIT>(p, hidden, ldh, weight, N, D, V, s, rows, p.few != 0, false, staged + (p.few ? p.bh : p.sh),
                            staged + (p.few ? p.bw : p.sw), H, W, q);
     Ignored ignored{};
     if (mode == kCE && g_hidden) {
