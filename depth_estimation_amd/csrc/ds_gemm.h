@@ -131,7 +131,9 @@ struct Fragments {
 // [kbeg, kend) (kbeg a multiple of 64).  `lds`: lds_bytes<S, PA, PB>() bytes.  Ends behind a barrier: the caller may reuse
 // `lds`.  A step brings all planes of both operands and adds its products from them, so that each plane is moved once and a
 // step's latency is covered by up to three products.  128 x 128 tiles then keep one step in LDS (the next one
-// waits in registers), which leaves room for two workgroups a CU.
+// waits in registers), which leaves room for two workgroups a CU.  Eight waves a 128 x 128 tile, two a SIMD, so that one's
+// LDS reads run beside the other's products: 512 x 4608 x 512 of two planes 15.1 us, 17.5 with four waves; two buffers or
+// loads two steps ahead gained nothing.
 template <class S, int PA, int PB>
 constexpr int lds_buffers() { return PA + PB > 2 && S::BM * S::BN > 64 * 128 ? 1 : 2; }
 template <class S, int PA, int PB>
@@ -207,8 +209,8 @@ __device__ __forceinline__ void gemm_tile(const Operand& A, const Operand& B, in
 // operands of the next 32 k; an s_barrier ends each turn.  Tiles come to LDS by DMA (buffer_load ... lds: no registers, no
 // LDS store instructions), the next step's under way during the whole current one, and the next tile's first step during the
 // last one of the tile before, so that a workgroup that goes through several tiles waits for memory once.
-//   4096 x 4096 x 4096 bf16: 109 us = 1266 TFLOP/s (register-staged 128 x 128 tiles: 166 us; the same 256 x 256 tile with
-//   all waves in step: 142 us); a library product of that size reaches 1436 TFLOP/s here.
+//   4096 x 4096 x 4096 bf16: 103 us = 1337 TFLOP/s, 109 us with one operand kM (register-staged 128 x 128 tiles: 166 us; the
+//   same 256 x 256 tile with all waves in step: 142 us); a library product of that size reaches 1436 TFLOP/s here.
 
 // 16 bytes per lane from a buffer to LDS at `lds` + 16 * lane; out-of-range lanes write zeros.  In assembly because the
 // compiler, which cannot tell the two buffers apart, would wait for every such load before the next LDS read; wait_dma()
@@ -562,7 +564,7 @@ template <class Tiles>
 inline Cut cut_of(Tiles tiles, double area, long long K, int pairs, bool may_split, int cus) {
     // us a step of 64 k: `step` of a CU's time with `at_once` workgroups on it, `alone` at least; `ends`: start and end of a
     // tile.  Measured at k = 512 and 2048 with half a workgroup to sixteen a CU; in TFLOP/s of 16-bit products with the chip
-    // full: 256 x 256 tiles 1330, 128 x 128 870, 64 x 64 660; three products a step 1365, 1160, 780 (two: between).
+    // full: 256 x 256 tiles 1330, 128 x 128 900, 64 x 64 660; three products a step 1365, 1170, 780 (two: between).
     struct Cost {
         ShapeId id;
         int b, at_once;

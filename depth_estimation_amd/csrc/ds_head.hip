@@ -1411,7 +1411,9 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     if (p.few && (size_t)p.few * pad8(D) * 4 > 40 * 1024) p.few = 0;
     const int vec = dtype == DS_F32 ? 4 : 8, lanes = lanes_for(cdiv(D, vec));
     p.few_grid = cdiv(V, kFewT / lanes * 4) < 2 * cu_count() ? cdiv(V, kFewT / lanes * 4) : 2 * cu_count();
-    // small head: the weight in LDS, two workgroups a CU
+    // small head: the weight in LDS, two workgroups a CU (training steps of 100000 rows, here / in tiles: 80 classes of 64
+    // features, bf16, 62 / 90 us; 576 of 64 133 / 190; 256 of 128 109 / 134; 128 of 250 142 / 139, forward 49 / 51; 288 of 64,
+    // float32, 170 / 224)
     const int Vp = (V + 31) & ~31;
     p.slim = D <= 64 ? 2 : D <= 128 ? 4 : D <= 256 ? 8 : 0;
     const long long bytes = (long long)Vp * p.slim * 64 * p.planes;

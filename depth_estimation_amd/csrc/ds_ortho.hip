@@ -339,7 +339,8 @@ __global__ __launch_bounds__(S::T) void ortho_finish_kernel(ProductArgs p, UseAr
 // X (small side s first, so a tall matrix is held transposed) and A, later B in its place, stay in LDS as two planes each;
 // rows are padded to a multiple of 32 with zeros and by 8 elements more, which spreads the fragment reads over the banks.
 // A wave forms fragments (16 x 16) of the products in registers; a result replaces its operand behind a barrier.  What bounds
-// it is the latency of the chain norm -> 3 products a step -> store: 64 x 147 in 5 steps 81 us as 17 launches.
+// it is the latency of the chain norm -> 3 products a step -> store: 64 x 147 in 5 steps 32 us (81 as 17 launches), 128 x 128
+// 85 (94).
 constexpr int kSmallT = 512;
 
 struct SmallPlan {
