@@ -549,41 +549,45 @@ __device__ __forceinline__ float scale_for(float amax) {
 }
 
 // ---- which shape a product takes, and over how many workgroups its sum is split (host) -----------------------------------
-enum ShapeId { kSq, kThin, kBig, kSmall };
+enum ShapeId { kSq, kThin, kBig, kSmall, kTiny };
 typedef Shape<128, 128, 4, 2> Sq;
 typedef Shape<64, 64, 2, 2> Small;
+typedef Shape<32, 32, 2, 2> Tiny;     // where there are fewer tiles than CUs: 512 x 512 x 512 of two planes 4.8 us, Small 7.5
 
-inline int side_of(ShapeId s) { return s == kBig ? Big::BM : s == kSmall ? Small::BM : Sq::BM; }   // Thin: along m
+inline int side_of(ShapeId s) { return s == kBig ? Big::BM : s == kSmall ? Small::BM : s == kTiny ? Tiny::BM : Sq::BM; }   // Thin: along m
 
 struct Cut {
     ShapeId shape;
     int splits;
 };
 // tiles(b): tiles of b x b; area: outputs; pairs: products a step (three of two planes each, two of two planes and one).
+// strided: an operand is kM.  Its rows of 32 elements are half a cache line: 32 x 32 tiles take a quarter longer
+// where several share a CU.
 template <class Tiles>
-inline Cut cut_of(Tiles tiles, double area, long long K, int pairs, bool may_split, int cus) {
+inline Cut cut_of(Tiles tiles, double area, long long K, int pairs, bool may_split, bool strided, int cus) {
     // us a step of 64 k: `step` of a CU's time with `at_once` workgroups on it, `alone` at least; `ends`: start and end of a
     // tile.  Measured at k = 512 and 2048 with half a workgroup to sixteen a CU; in TFLOP/s of 16-bit products with the chip
-    // full: 256 x 256 tiles 1330, 128 x 128 900, 64 x 64 660; three products a step 1365, 1170, 780 (two: between).
+    // full: 256 x 256 tiles 1330, 128 x 128 900, 64 x 64 660, 32 x 32 290; three products a step 1365, 1170, 780, 510 (two:
+    // between).
     struct Cost {
         ShapeId id;
         int b, at_once;
         double step, alone, ends;
     };
-    static const Cost one[3] = {{kBig, 256, 1, 1.5, 1.35, 4.5}, {kSq, 128, 2, 0.58, 0.66, 3.0}, {kSmall, 64, 4, 0.21, 0.57, 2.0}};
-    static const Cost two[3] = {{kBig, 256, 1, 3.0, 2.7, 5.0}, {kSq, 128, 2, 0.94, 1.08, 3.0}, {kSmall, 64, 3, 0.37, 0.62, 2.5}};
-    static const Cost three[3] = {{kBig, 256, 1, 4.5, 4.1, 5.0}, {kSq, 128, 2, 1.33, 1.50, 3.0}, {kSmall, 64, 2, 0.53, 0.68, 2.5}};
+    static const Cost one[4] = {{kBig, 256, 1, 1.5, 1.35, 4.5}, {kSq, 128, 2, 0.58, 0.66, 3.0}, {kSmall, 64, 4, 0.21, 0.52, 2.0}, {kTiny, 32, 8, 0.125, 0.23, 2.2}};
+    static const Cost two[4] = {{kBig, 256, 1, 3.0, 2.7, 5.0}, {kSq, 128, 2, 0.94, 1.08, 3.0}, {kSmall, 64, 3, 0.37, 0.62, 2.5}, {kTiny, 32, 5, 0.19, 0.29, 2.2}};
+    static const Cost three[4] = {{kBig, 256, 1, 4.5, 4.1, 5.0}, {kSq, 128, 2, 1.33, 1.50, 3.0}, {kSmall, 64, 2, 0.53, 0.68, 2.5}, {kTiny, 32, 4, 0.25, 0.34, 2.2}};
     const long long steps = (K + kBK - 1) / kBK, most = may_split ? (steps < 256 ? steps : 256) : 1;
     Cut best{kSq, 1};
     double least = 1e300;
-    for (int c = 0; c < 3; ++c) {
+    for (int c = 0; c < 4; ++c) {
         const Cost& q = pairs == 1 ? one[c] : pairs == 2 ? two[c] : three[c];
         const long long t = tiles(q.b);
         for (long long s = 1; s <= most; s += s < 16 ? 1 : s / 8) {
             const double per = (double)((steps + s - 1) / s);
             const long long n = (t * s + cus - 1) / cus, full = n / q.at_once, rest = n % q.at_once;
             auto round = [&](long long k) {
-                const double shared = q.step * (double)k;
+                const double shared = (strided && q.id == kTiny ? 1.25 * q.step : q.step) * (double)k;
                 return (shared > q.alone ? shared : q.alone) * per + q.ends;
             };
             // a split sum is written and read once more, 4 bytes an element at 4 TB/s, and takes one more launch

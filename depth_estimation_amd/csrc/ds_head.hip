@@ -655,9 +655,14 @@ __device__ __forceinline__ void dl_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, i
                 for (int e = 0; e < 4; ++e)
                     if (c0 + i * 16 + e >= a.cols) acc[i][j][e] = 0.f;
         }
+        if constexpr (S::FM == 1) {
+            const float d[4] = {acc[0][j][0], acc[0][j][1], acc[0][j][2], acc[0][j][3]};
+            if (!(edge && c0 >= a.ld)) put4<SPLIT>(dl + (long long)n * a.ld + c0, a.lo, d);
+            continue;
+        }
         const int c8 = m0 + wm * S::FM * 16 + (lane >> 4) * 8;
 #pragma unroll
-        for (int i = 0; i < S::FM; i += 2) {
+        for (int i = 0; i + 1 < S::FM; i += 2) {
             const int c = c8 + i * 16;
             s16x8 hi, lo;
             eight_of(round4<T>(acc[i][j]), round4<T>(acc[i + 1][j]), hi);
@@ -744,9 +749,13 @@ __device__ __forceinline__ void grad_of_tile(const f32x4 (&acc)[S::FM][S::FN], i
                 if (WHICH == 0 && !a.first) v += *q;
                 *q = v;
             }
+        } else if (S::FM == 1) {
+            const f32x4 v = acc[0][j] * f0 * is;
+            const float w[4] = {v[0], v[1], v[2], v[3]};
+            put_row4(static_cast<O*>(a.out) + row * a.D, m0 + wm * 16 + (lane >> 4) * 4, a.D, w);
         } else {
 #pragma unroll
-            for (int i = 0; i < S::FM; i += 2)
+            for (int i = 0; i + 1 < S::FM; i += 2)
                 put_row8(static_cast<O*>(a.out) + row * a.D, m0 + (wm * S::FM + i) * 16, a.D, lane, acc[i][j] * f0 * is,
                          acc[i + 1][j] * f0 * is);
         }
@@ -1343,13 +1352,13 @@ __global__ __launch_bounds__(1024) void join_few_kernel(JoinArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
-// Shapes: 256x256 outputs a workgroup (TileStream) for large products; 128x128 and 64x64 below that; up to 32 rows have a shape of their
+// Shapes: 256x256 outputs a workgroup (TileStream) for large products; 128x128, 64x64 and 32x32 below that; up to 32 rows have a shape of their
 // own, most of whose work would otherwise be dropped (a training step of 16 rows: 65536 classes of 1024 features, bf16, 127
 // us against 142; 1000 of 256, float32, 48 against 54).
 typedef Shape<128, 32, 4, 1> Thin;    // 32 along n
-Cut cut_of(long long M, long long N, long long K, int planes, bool may_split) {
-    return ds::cut_of([&](long long b) { return ((M + b - 1) / b) * ((N + b - 1) / b); }, (double)M * N, K, planes == 2 ? 3 : 1, may_split,
-                      cu_count());
+Cut cut_of(long long M, long long N, long long K, int planes, bool grad) {      // grad: operands kM, sums may be split
+    return ds::cut_of([&](long long b) { return ((M + b - 1) / b) * ((N + b - 1) / b); }, (double)M * N, K, planes == 2 ? 3 : 1, grad,
+                      grad, cu_count());
 }
 
 bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
@@ -1573,6 +1582,8 @@ void stats_launch(const Plan& p, const Operand& W, const Operand& H, const Saved
         head_stats_big_kernel<T, SPLIT, MODE><<<tiles < cu_count() ? tiles : cu_count(), Big::T, 0, q>>>(W, H, s.st, D, a);
     else if (p.fwd == kSmall)
         head_stats_kernel<T, Small, SPLIT, MODE><<<tiles, Small::T, 0, q>>>(W, H, s.st, D, a);
+    else if (p.fwd == kTiny)
+        head_stats_kernel<T, Tiny, SPLIT, MODE><<<tiles, Tiny::T, 0, q>>>(W, H, s.st, D, a);
     else
         head_stats_kernel<T, Sq, SPLIT, MODE><<<tiles, Sq::T, 0, q>>>(W, H, s.st, D, a);
 }
@@ -1667,6 +1678,8 @@ void dl_launch(const Plan& p, const Operand& W, const Operand& H, const Saved& s
         head_dl_big_kernel<T, SPLIT, MODE><<<tiles < cu_count() ? tiles : cu_count(), Big::T, 0, q>>>(W, H, s.st, bs, D, a);
     else if (p.dl_shape == kSmall)
         head_dl_kernel<T, Small, SPLIT, MODE><<<tiles, Small::T, 0, q>>>(W, H, s.st, bs, D, a);
+    else if (p.dl_shape == kTiny)
+        head_dl_kernel<T, Tiny, SPLIT, MODE><<<tiles, Tiny::T, 0, q>>>(W, H, s.st, bs, D, a);
     else
         head_dl_kernel<T, Sq, SPLIT, MODE><<<tiles, Sq::T, 0, q>>>(W, H, s.st, bs, D, a);
 }
@@ -1689,6 +1702,8 @@ void grad_launch(ShapeId shape, bool acc, const Operand& A, const Operand& B, co
         grad_shape<IT, T, Big, SPLIT, WHICH>(acc, A, B, s, bs, n, a, q);
     else if (shape == kSmall)
         grad_shape<IT, T, Small, SPLIT, WHICH>(acc, A, B, s, bs, n, a, q);
+    else if (shape == kTiny)
+        grad_shape<IT, T, Tiny, SPLIT, WHICH>(acc, A, B, s, bs, n, a, q);
     else
         grad_shape<IT, T, Sq, SPLIT, WHICH>(acc, A, B, s, bs, n, a, q);
 }

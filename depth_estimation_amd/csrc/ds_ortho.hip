@@ -149,11 +149,12 @@ struct UseArgs {
     float *da, *db;          // light: A's diagonal, scaled as A, and B's as it is over what its plane holds; `side` a matrix
     int side, wide;
 };
-// fragment rows i and i + 1 of a tile
+// fragment rows i and i + 1 of a tile (of a shape with one: x)
 template <class S, class H, class O>
 __device__ __forceinline__ void use_rows(const f32x4 (&x)[S::FN], const f32x4 (&y)[S::FN], int i, int m0, int n0, int batch,
                                          const UseArgs& u) {
     constexpr Use U = H::U;
+    constexpr int F = S::FM == 1 ? 1 : 2;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / S::WN, wn = wave % S::WN;
     const int mi = m0 + (wm * S::FM + i) * 16;
@@ -163,9 +164,9 @@ __device__ __forceinline__ void use_rows(const f32x4 (&x)[S::FN], const f32x4 (&
     for (int j = 0; j < S::FN; ++j) {
         const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
         if (n >= u.rows) continue;
-        f32x4 v[2];
+        f32x4 v[F];
 #pragma unroll
-        for (int f = 0; f < 2; ++f) {
+        for (int f = 0; f < F; ++f) {
             const f32x4 acc = f ? y[j] : x[j];
             const int m = mi + f * 16 + (lane >> 4) * 4;
             float old[4] = {0.f, 0.f, 0.f, 0.f};
@@ -205,23 +206,32 @@ __device__ __forceinline__ void use_rows(const f32x4 (&x)[S::FN], const f32x4 (&
                 if (!in) v[f][e] = 0.f;
             }
         }
+        const float v0[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
         if (U == kLast) {
-            put_row8(static_cast<O*>(u.out) + batch * u.per_out + (long long)n * u.cols, mi, u.cols, lane, v[0], v[1]);
+            O* row = static_cast<O*>(u.out) + batch * u.per_out + (long long)n * u.cols;
+            if (F == 2)
+                put_row8(row, mi, u.cols, lane, v[0], v[F - 1]);
+            else
+                put_row4(row, mi + (lane >> 4) * 4, u.cols, v0);
             continue;
         }
         constexpr bool kTwo = !H::LIGHT || U == kNext;      // planes of the result
         f16* out = static_cast<f16*>(u.out) + batch * u.per_out;
-        const int m8 = mi + (lane >> 4) * 8;
-        s16x8 hi, lo;
-        eight_of(round4<f16>(v[0]), round4<f16>(v[1]), hi);
-        if constexpr (kTwo) eight_of(rest4(v[0]), rest4(v[1]), lo);
-        if (m8 < u.ld) {
-            *reinterpret_cast<s16x8*>(out + (long long)n * u.ld + m8) = hi;
-            if constexpr (kTwo) *reinterpret_cast<s16x8*>(out + (long long)n * u.ld + m8 + u.lo) = lo;
+        if constexpr (F == 2) {
+            const int m8 = mi + (lane >> 4) * 8;
+            s16x8 hi, lo;
+            eight_of(round4<f16>(v[0]), round4<f16>(v[1]), hi);
+            if constexpr (kTwo) eight_of(rest4(v[0]), rest4(v[1]), lo);
+            if (m8 < u.ld) {
+                *reinterpret_cast<s16x8*>(out + (long long)n * u.ld + m8) = hi;
+                if constexpr (kTwo) *reinterpret_cast<s16x8*>(out + (long long)n * u.ld + m8 + u.lo) = lo;
+            }
+        } else if (mi + (lane >> 4) * 4 < u.ld) {
+            put4<kTwo ? 3 : 1>(out + (long long)n * u.ld + mi + (lane >> 4) * 4, u.lo, v0);
         }
         if ((U == kGram || U == kPoly) && m0 != n0) {
 #pragma unroll
-            for (int f = 0; f < 2; ++f)
+            for (int f = 0; f < F; ++f)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int m = mi + f * 16 + (lane >> 4) * 4 + e;
@@ -238,7 +248,7 @@ __device__ __forceinline__ void use_rows(const f32x4 (&x)[S::FN], const f32x4 (&
 template <class S, class H, class O>
 __device__ __forceinline__ void use_tile(const f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int batch, const UseArgs& u) {
 #pragma unroll
-    for (int i = 0; i < S::FM; i += 2) use_rows<S, H, O>(acc[i], acc[i + 1], i, m0, n0, batch, u);
+    for (int i = 0; i < S::FM; i += 2) use_rows<S, H, O>(acc[i], acc[S::FM == 1 ? 0 : i + 1], i, m0, n0, batch, u);
 }
 
 // C = A B over k.  tri: only tiles with m0 >= n0.  Units: matrices x tiles x splits; part (may be NULL: no splits): the tiles'
@@ -325,13 +335,14 @@ __global__ __launch_bounds__(S::T) void ortho_finish_kernel(ProductArgs p, UseAr
     tile_of<S>(p, tile, gridDim.x / p.batch, batch, m0, n0);
     const f32x4* q = reinterpret_cast<const f32x4*>(p.part) + (long long)tile * p.splits * (S::BM * S::BN / 4) + threadIdx.x +
                      i * S::FN * S::T;
-    f32x4 acc[2][S::FN];
+    constexpr int F = S::FM == 1 ? 1 : 2;
+    f32x4 acc[F][S::FN];
 #pragma unroll
-    for (int j = 0; j < 2 * S::FN; ++j) acc[j / S::FN][j % S::FN] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < F * S::FN; ++j) acc[j / S::FN][j % S::FN] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < p.splits; ++s)
 #pragma unroll
-        for (int j = 0; j < 2 * S::FN; ++j) acc[j / S::FN][j % S::FN] += q[(long long)s * (S::BM * S::BN / 4) + j * S::T];
-    use_rows<S, H, O>(acc[0], acc[1], i, m0, n0, batch, u);
+        for (int j = 0; j < F * S::FN; ++j) acc[j / S::FN][j % S::FN] += q[(long long)s * (S::BM * S::BN / 4) + j * S::T];
+    use_rows<S, H, O>(acc[0], acc[F - 1], i, m0, n0, batch, u);
 }
 
 // ---- small matrices: all steps in one workgroup ------------------------------------------------------------------------
@@ -674,17 +685,17 @@ OrthoPlan ortho_plan(int dtype, int batch, int m, int n) {
     // on smaller sides launches and latency are what a step takes, not products (five steps of 256 x 1024: 149 us so, 145
     // with all planes; 512 x 512 150 and 166, 1024 x 1024 229 and 254, 2048 x 2048 505 and 759)
     p.light = dtype == DS_BF16 && p.s >= 512;
-    auto cut = [&](int M, int N, int K, int pairs, bool tri) {
+    auto cut = [&](int M, int N, int K, int pairs, bool tri, bool strided) {
         return cut_of(
             [&](long long b) {
                 const long long x = (M + b - 1) / b, y = (N + b - 1) / b;
                 return batch * (tri ? x * (x + 1) / 2 : x * y);
             },
-            (double)M * N * batch * (tri ? 0.5 : 1.0), K, pairs, true, cu_count());
+            (double)M * N * batch * (tri ? 0.5 : 1.0), K, pairs, true, strided, cu_count());
     };
-    p.gram = cut(p.s, p.s, p.l, p.light ? 1 : 3, true);
-    p.poly = cut(p.s, p.s, p.s, p.light ? 1 : 3, true);
-    p.apply = cut(n, m, p.s, p.light ? 2 : 3, false);
+    p.gram = cut(p.s, p.s, p.l, p.light ? 1 : 3, true, m > n);
+    p.poly = cut(p.s, p.s, p.s, p.light ? 1 : 3, true, false);
+    p.apply = cut(n, m, p.s, p.light ? 2 : 3, false, m <= n);
     const size_t x = align256((size_t)batch * m * p.np * 4), a = align256((size_t)batch * p.s * p.sp * 4);
     size_t part = part_bytes(p.gram, p.s, p.s, true, batch), q = part_bytes(p.poly, p.s, p.s, true, batch);
     if (q > part) part = q;
@@ -729,7 +740,7 @@ void product_shape(ProductArgs p, const UseArgs& u, int tiles, hipStream_t q) {
     const int grid = std::is_same<S, Big>::value && units > cu_count() ? cu_count() : units;
     if (p.splits > 1) {
         ortho_product_kernel<S, LA, LB, PA, PB, How<kGram, false>, float, true><<<grid, S::T, 0, q>>>(p, u, units);
-        ortho_finish_kernel<S, H, O><<<dim3(tiles, S::FM / 2), S::T, 0, q>>>(p, u);
+        ortho_finish_kernel<S, H, O><<<dim3(tiles, (S::FM + 1) / 2), S::T, 0, q>>>(p, u);
     } else {
         ortho_product_kernel<S, LA, LB, PA, PB, H, O, false><<<grid, S::T, 0, q>>>(p, u, units);
     }
@@ -744,8 +755,10 @@ void product(const Cut& c, ProductArgs p, const UseArgs& u, int M, int N, hipStr
         product_shape<Big, LA, LB, PA, PB, H, O>(p, u, tiles, q);
     else if (c.shape == kSq)
         product_shape<Sq, LA, LB, PA, PB, H, O>(p, u, tiles, q);
-    else
+    else if (c.shape == kSmall)
         product_shape<Small, LA, LB, PA, PB, H, O>(p, u, tiles, q);
+    else
+        product_shape<Tiny, LA, LB, PA, PB, H, O>(p, u, tiles, q);
 }
 
 // stored B = 2^e B with |B| <= |a| + 2 |b| + 4 |c| below 2^15
