@@ -350,8 +350,7 @@ __global__ __launch_bounds__(S::T) void ortho_finish_kernel(ProductArgs p, UseAr
 // X (small side s first, so a tall matrix is held transposed) and A, later B in its place, stay in LDS as two planes each;
 // rows are padded to a multiple of 32 with zeros and by 8 elements more, which spreads the fragment reads over the banks.
 // A wave forms fragments (16 x 16) of the products in registers; a result replaces its operand behind a barrier.  What bounds
-// it is the latency of the chain norm -> 3 products a step -> store: 64 x 147 in 5 steps 32 us (81 as 17 launches), 128 x 128
-// 85 (94).
+// it is the latency of the chain norm -> 3 products a step -> store: 64 x 147 in 5 steps 32 us (71 as 17 launches).
 constexpr int kSmallT = 512;
 
 struct SmallPlan {
@@ -367,9 +366,12 @@ __host__ __device__ inline SmallPlan small_plan(int s, int l) {
     p.bytes = 4 * p.sp * (p.px + p.pa);
     return p;
 }
-// fits LDS, and every wave's fragments its registers
-inline bool small_fits(int s, int l) {
-    if (s > 128 || l > 4096) return false;
+// Fits LDS, and every wave's fragments its registers, and a few matrices are not faster in slabs (32 x 600 61 us here, 46 there;
+// 16 x 400 40 and 42, 40 x 256 48 and 54) or, with more than 96 rows, in separate launches (128 x 128 85 and 72, three of 100 x
+// 120 81 and 73, 96 x 128 69 and 71).  A stack gains nothing there: 200 of 16 x 500 45 us here, 111 in slabs; 32 of 100 x 120
+// 82 and 82, 200 of them 86 and 159.
+inline bool small_fits(int batch, int s, int l) {
+    if (s > 128 || l > 4096 || (batch < 32 && (s > 96 || l > 448))) return false;
     const SmallPlan p = small_plan(s, l);
     return p.bytes <= 152 * 1024 && cdiv(p.lp / 16, kSmallT / 64 / (p.sp / 16)) <= (s > 64 ? 8 : 10);
 }
@@ -701,7 +703,7 @@ OrthoPlan ortho_plan(int dtype, int batch, int m, int n) {
     if (q > part) part = q;
     q = part_bytes(p.apply, n, m, false, batch);
     if (q > part) part = q;
-    p.small = small_fits(p.s, p.l);
+    p.small = small_fits(batch, p.s, p.l);
     const int s32 = (p.s + 31) & ~31;
     // (at s = 128 the parts are 64 KB a slab and the products of a slab 8 us: no gain over separate launches)
     p.slab = p.small || s32 > 64 ? 0 : p.l > 4096 ? 256 : 128;

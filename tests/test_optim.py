@@ -52,7 +52,8 @@ def _update(shape, dtype, seed, kind="gauss"):
 
 SHAPES = [(1, 1), (1, 7), (7, 1), (2, 2), (5, 3), (3, 5), (16, 16), (64, 147), (65, 64), (64, 64), (63, 130), (128, 128),
           (129, 257), (257, 129), (200, 1000), (1000, 200), (2, 33, 17), (3, 1, 40, 72), (384, 384), (64, 576), (576, 64), (20, 3001), (100, 129),
-          (128, 1152), (2, 1153, 127), (3, 33, 1200), (60, 4111), (4111, 60), (65, 300)]
+          (128, 1152), (2, 1153, 127), (3, 33, 1200), (60, 4111), (4111, 60), (65, 300), (96, 100), (40, 128, 97), (33, 120, 128),
+          (64, 320), (449, 31), (7, 30, 640), (40, 16, 500)]
 
 
 @pytest.mark.gpu
