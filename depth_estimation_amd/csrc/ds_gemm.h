@@ -8,8 +8,8 @@
 //
 // Numbers wider than 16 bits go through as two fp16 planes x = hi + lo (22 bits, after an exact power-of-two scale that the
 // caller keeps): lo*hi + hi*lo + hi*hi go into the same fp32 accumulators.  What is dropped, lo*lo, is 2^-22 of the product.
-// PA and PB say how many planes A and B have.  Three 16-bit products cost a third of the 16-bit rate, still above the rate of fp32 matrix instructions
-// (1/16 of it).
+// PA and PB say how many planes A and B have.  Three 16-bit products cost a third of the 16-bit rate, still above the rate of
+// fp32 matrix instructions (1/16 of it).
 //
 // Rows and columns beyond an operand's bounds read as zero (buffer loads whose offset is out of range), so every size works
 // without padded copies; only the contiguous extent must be a multiple of 8 elements and 16-byte aligned.
@@ -554,7 +554,9 @@ typedef Shape<128, 128, 4, 2> Sq;
 typedef Shape<64, 64, 2, 2> Small;
 typedef Shape<32, 32, 2, 2> Tiny;     // where there are fewer tiles than CUs: 512 x 512 x 512 of two planes 4.8 us, Small 7.5
 
-inline int side_of(ShapeId s) { return s == kBig ? Big::BM : s == kSmall ? Small::BM : s == kTiny ? Tiny::BM : Sq::BM; }   // Thin: along m
+inline int side_of(ShapeId s) {      // Thin: along m
+    return s == kBig ? Big::BM : s == kSmall ? Small::BM : s == kTiny ? Tiny::BM : Sq::BM;
+}
 
 struct Cut {
     ShapeId shape;
@@ -567,16 +569,19 @@ template <class Tiles>
 inline Cut cut_of(Tiles tiles, double area, long long K, int pairs, bool may_split, bool strided, int cus) {
     // us a step of 64 k: `step` of a CU's time with `at_once` workgroups on it, `alone` at least; `ends`: start and end of a
     // tile.  Measured at k = 512 and 2048 with half a workgroup to sixteen a CU; in TFLOP/s of 16-bit products with the chip
-    // full: 256 x 256 tiles 1330, 128 x 128 900, 64 x 64 660, 32 x 32 290; three products a step 1365, 1170, 780, 510 (two:
+    // full: 256 x 256 tiles 1330, 128 x 128 900, 64 x 64 660, 32 x 32 290; three products a step 1365, 1170, 780, 490 (two:
     // between).
     struct Cost {
         ShapeId id;
         int b, at_once;
         double step, alone, ends;
     };
-    static const Cost one[4] = {{kBig, 256, 1, 1.5, 1.35, 4.5}, {kSq, 128, 2, 0.58, 0.66, 3.0}, {kSmall, 64, 4, 0.21, 0.52, 2.0}, {kTiny, 32, 8, 0.125, 0.23, 2.2}};
-    static const Cost two[4] = {{kBig, 256, 1, 3.0, 2.7, 5.0}, {kSq, 128, 2, 0.94, 1.08, 3.0}, {kSmall, 64, 3, 0.37, 0.62, 2.5}, {kTiny, 32, 5, 0.19, 0.29, 2.2}};
-    static const Cost three[4] = {{kBig, 256, 1, 4.5, 4.1, 5.0}, {kSq, 128, 2, 1.33, 1.50, 3.0}, {kSmall, 64, 2, 0.53, 0.68, 2.5}, {kTiny, 32, 4, 0.25, 0.34, 2.2}};
+    static const Cost one[4] = {{kBig, 256, 1, 1.5, 1.35, 4.5}, {kSq, 128, 2, 0.58, 0.66, 3.0},
+                                {kSmall, 64, 4, 0.21, 0.52, 2.0}, {kTiny, 32, 8, 0.125, 0.23, 2.2}};
+    static const Cost two[4] = {{kBig, 256, 1, 3.0, 2.7, 5.0}, {kSq, 128, 2, 0.94, 1.08, 3.0},
+                                {kSmall, 64, 3, 0.37, 0.62, 2.5}, {kTiny, 32, 5, 0.19, 0.29, 2.2}};
+    static const Cost three[4] = {{kBig, 256, 1, 4.5, 4.1, 5.0}, {kSq, 128, 2, 1.33, 1.50, 3.0},
+                                  {kSmall, 64, 2, 0.53, 0.68, 2.5}, {kTiny, 32, 4, 0.25, 0.34, 2.2}};
     const long long steps = (K + kBK - 1) / kBK, most = may_split ? (steps < 256 ? steps : 256) : 1;
     Cut best{kSq, 1};
     double least = 1e300;

@@ -1357,8 +1357,8 @@ __global__ __launch_bounds__(1024) void join_few_kernel(JoinArgs a) {
 // us against 142; 1000 of 256, float32, 48 against 54).
 typedef Shape<128, 32, 4, 1> Thin;    // 32 along n
 Cut cut_of(long long M, long long N, long long K, int planes, bool grad) {      // grad: operands kM, sums may be split
-    return ds::cut_of([&](long long b) { return ((M + b - 1) / b) * ((N + b - 1) / b); }, (double)M * N, K, planes == 2 ? 3 : 1, grad,
-                      grad, cu_count());
+    return ds::cut_of([&](long long b) { return ((M + b - 1) / b) * ((N + b - 1) / b); }, (double)M * N, K,
+                      planes == 2 ? 3 : 1, grad, grad, cu_count());
 }
 
 bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }

@@ -51,7 +51,8 @@ def _update(shape, dtype, seed, kind="gauss"):
 
 
 SHAPES = [(1, 1), (1, 7), (7, 1), (2, 2), (5, 3), (3, 5), (16, 16), (64, 147), (65, 64), (64, 64), (63, 130), (128, 128),
-          (129, 257), (257, 129), (200, 1000), (1000, 200), (2, 33, 17), (3, 1, 40, 72), (384, 384), (64, 576), (576, 64), (20, 3001), (100, 129),
+          (129, 257), (257, 129), (200, 1000), (1000, 200), (2, 33, 17), (3, 1, 40, 72), (384, 384), (64, 576), (576, 64), (20, 3001),
+          (100, 129),
           (128, 1152), (2, 1153, 127), (3, 33, 1200), (60, 4111), (4111, 60), (65, 300), (96, 100), (40, 128, 97), (33, 120, 128),
           (64, 320), (449, 31), (7, 30, 640), (40, 16, 500)]
 
@@ -78,7 +79,8 @@ def test_larger_tiles(shape):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["gauss", "decay", "few"])
-@pytest.mark.parametrize("shape", [(256, 256), (256, 1000), (1001, 259), (2, 300, 530), (512, 512), (2, 513, 1031), (700, 700), (1500, 650), (2300, 2100)], ids=str)
+@pytest.mark.parametrize("shape", [(256, 256), (256, 1000), (1001, 259), (2, 300, 530), (512, 512), (2, 513, 1031), (700, 700),
+                                   (1500, 650), (2300, 2100)], ids=str)
 def test_bfloat16_with_fewer_products(shape, kind):
     """Sides of 512 and more: 11-bit operands (22 below).  Rounding the result alone is off by 2^-8 / sqrt(3) at most in norm (1.7e-3 for
     numbers spread evenly between powers of two), the operands' rounding by less (9e-4 was the most over these spectra when
