@@ -436,10 +436,9 @@ def test_large_tiles(n, d, v, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
-def test_last_piece_of_few_classes(dtype):
-    """44644 classes: the last piece has 100, most of the ten splits of the sum over classes nothing.  A row of NaN gradients
-    reaches no other row."""
-    n, d, v, bad = 3000, 500, 44644, 1501
+def test_pieces_with_a_row_of_nan(dtype):
+    """70001 classes in two pieces (three in float32), the sum over them split.  A row of NaN gradients reaches no other row."""
+    n, d, v, bad = 3000, 500, 70001, 1501
     h, w, t, up, _ = _data(n, d, v, dtype, seed=21)
     t[7] = v - 1                                   # a target in the last piece
     pick = torch.arange(bad - 40, bad + 40, device=DEV)
