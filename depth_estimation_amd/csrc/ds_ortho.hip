@@ -5,8 +5,9 @@
 // A step is three products.  The first two have symmetric results: only tiles on and below the diagonal are formed, their
 // mirror images written along.  Small singular values grow by a factor a = 3.4 per step, and with them whatever the products
 // lost: with X, A and B rounded to bf16 the result is off by 1e-2 .. 6e-2, to fp16 by up to 8e-3 (matrices with a spectrum of
-// three decades; measured against 64 bits), so all three are kept as two fp16 planes (22 bits; 1e-6) under fixed powers of
-// two: entries of X and A are at most about 1.3, B's bound follows from the coefficients.
+// three decades; measured against 64 bits), so all three are kept as two fp16 planes (22 bits; 1e-6) under powers of two that
+// follow from the coefficients alone: singular values begin in [0, 1], so how far each step can take them is known before it
+// (steps_of), and entries are at most as large as the largest singular value.
 //
 // bf16 results of larger matrices need less, and take half the products (Light): A keeps one plane (11 bits) off the diagonal,
 // where its entries are small, and its diagonal in fp32 beside it.  B keeps one plane; what its diagonal, which carries most of
@@ -23,7 +24,55 @@
 namespace ds {
 namespace {
 
-constexpr float kXs = 8192.f;    // stored X = 2^13 X, stored A = 2^13 A: 8x headroom in fp16
+constexpr float kXs = 8192.f;    // stored X = 2^13 X where singular values are at most sqrt(2), stored A = 2^13 A
+
+// Factors of one step's products, and of the result.  X is stored as 2^(13 - e) X and A as 2^(13 - 2e) A, where e, the step's
+// own, is the least with |X| <= 2^e sqrt(2) (spectral norm; 0 for coefficients that keep it near one), so that A <= 2^14 as
+// stored; B with its bound |a| + |b| A + |c| A^2 in (2^14, 2^15].
+struct Step {
+    float gram;          // accumulated X X^T -> stored A
+    float ca, cb, cc;    // accumulated A A, stored A, and the identity -> stored B
+    float next;          // accumulated B X -> the next stored X, or after the last step X itself
+};
+struct Steps {
+    Step s[DS_ORTHO_MAX_STEPS];
+};
+constexpr int kMostShift = 24;
+
+// the largest |x (a + b x^2 + c x^4)| for x in [0, m]
+double reach_of(const double* co, double m) {
+    auto at = [&](double t) { return fabs(sqrt(t) * (co[0] + t * (co[1] + t * co[2]))); };
+    double most = at(m * m);
+    // the derivative a + 3 b t + 5 c t^2, t = x^2, is zero
+    const double p = 3 * co[1], q = 5 * co[2], d = p * p - 4 * q * co[0];
+    if (d >= 0) {
+        const double r = -0.5 * (p + (p >= 0 ? sqrt(d) : -sqrt(d))), roots[2] = {q != 0 ? r / q : -1, r != 0 ? co[0] / r : -1};
+        for (double t : roots)
+            if (t > 0 && t < m * m && at(t) > most) most = at(t);
+    }
+    return most;
+}
+// false: singular values would leave the range (2^kMostShift before the last step, 2^100 after it; NaN)
+bool steps_of(const double* co, int steps, Steps& out) {
+    double m = 1;
+    auto shift = [](double x) {
+        const double e = x > 0 ? ceil(log2(x / sqrt(2.0))) : -kMostShift;
+        return e < -kMostShift ? -kMostShift : e;     // (smaller yet: bits are lost one by one, as below any type's range)
+    };
+    for (int i = 0; i < steps; ++i) {
+        const double e = shift(m), xs = exp2(13 - e), as = exp2(13 - 2 * e), top = 2 * exp2(2 * e);
+        const double bound = fabs(co[0]) + top * (fabs(co[1]) + top * fabs(co[2]));
+        if (!(e <= kMostShift) || !(bound <= exp2(100))) return false;
+        const double k = bound > 0 ? floor(log2(32768.0 / bound)) : 0, bs = exp2(k > 100 ? 100 : k);
+        m = reach_of(co, m);
+        const bool last = i + 1 == steps;
+        if (!(m <= exp2(last ? 100 : kMostShift))) return false;
+        const double next = last ? 1 : exp2(13 - shift(m));
+        out.s[i] = Step{(float)(as / (xs * xs)), (float)(co[0] * bs), (float)(co[1] * bs / as), (float)(co[2] * bs / (as * as)),
+                        (float)(next / (bs * xs))};
+    }
+    return true;
+}
 // blocks that sum squares of one matrix: 4096 elements each, at most 512
 __host__ __device__ inline int norm_blocks(long long mn) {
     const long long n = (mn + 4095) / 4096;
@@ -145,7 +194,7 @@ struct UseArgs {
     long long lo, per_out;   // planes apart, matrices apart
     const f16* a;            // kPoly: A again
     long long per_a;
-    float ca, cb, cc;        // kPoly's coefficients, scaled; else ca: the factor
+    float ca, cb, cc;        // kPoly: Step's; else ca: the factor
     float *da, *db;          // light: A's diagonal, scaled as A, and B's as it is over what its plane holds; `side` a matrix
     int side, wide;
 };
@@ -439,17 +488,16 @@ __device__ __forceinline__ void small_product(const Planes& R, const Planes& C, 
 struct SmallArgs {
     int m, n, steps;
     double eps;
-    float ca, cb, cc, bs;     // as UseArgs of kPoly; B's scale
 };
-// b: this wave's fragments of X X^T (2^26 of it); leaves the polynomial B in A's place
+// b: this wave's fragments of X X^T; leaves the polynomial B in A's place
 template <int NA>
-__device__ __forceinline__ void gram_to_poly(const Planes& A, const Share& sq, int s, int sp, int lane, const SmallArgs& a,
+__device__ __forceinline__ void gram_to_poly(const Planes& A, const Share& sq, int s, int sp, int lane, const Step& a,
                                              f32x4 (&b)[NA]) {
     const int r = sq.row * 16 + (lane & 15), q = (lane >> 4) * 4;
 #pragma unroll
     for (int i = 0; i < NA; ++i)
         if (sq.mine(i)) {
-            const float v[4] = {b[i][0] * (1.f / kXs), b[i][1] * (1.f / kXs), b[i][2] * (1.f / kXs), b[i][3] * (1.f / kXs)};
+            const float v[4] = {b[i][0] * a.gram, b[i][1] * a.gram, b[i][2] * a.gram, b[i][3] * a.gram};
             put4<3>(A.hi + r * A.pitch + sq.c0(i) + q, A.lo - A.hi, v);
         }
     __syncthreads();
@@ -476,7 +524,7 @@ __device__ __forceinline__ void gram_to_poly(const Planes& A, const Share& sq, i
 
 // NA, NX: fragments a wave holds of the square products and of X
 template <class O, int NA, int NX>
-__global__ __launch_bounds__(kSmallT) void ortho_small_kernel(const O* __restrict__ g, O* __restrict__ out, SmallArgs a) {
+__global__ __launch_bounds__(kSmallT) void ortho_small_kernel(const O* __restrict__ g, O* __restrict__ out, SmallArgs a, Steps steps) {
     extern __shared__ __align__(16) char lds[];
     __shared__ double red[kSmallT / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -528,7 +576,8 @@ __global__ __launch_bounds__(kSmallT) void ortho_small_kernel(const O* __restric
     for (int step = 0; step < a.steps; ++step) {
         f32x4 b[NA];
         small_product<false, NA>(X, X, sq, p.lp, lane, b);
-        gram_to_poly<NA>(A, sq, s, p.sp, lane, a, b);
+        const Step st = steps.s[step];
+        gram_to_poly<NA>(A, sq, s, p.sp, lane, st, b);
         f32x4 x[NX];
         small_product<true, NX>(A, X, sx, p.sp, lane, x);
         const bool last = step + 1 == a.steps;
@@ -539,7 +588,7 @@ __global__ __launch_bounds__(kSmallT) void ortho_small_kernel(const O* __restric
                 const int c = sx.c0(i) + q;
                 float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = x[i][e] * (last ? 1.f / (a.bs * kXs) : 1.f / a.bs);
+                for (int e = 0; e < 4; ++e) v[e] = x[i][e] * st.next;
                 if (!last) {
                     put4<3>(X.hi + r * p.px + c, X.lo - X.hi, v);
                 } else if (r < s) {
@@ -559,6 +608,7 @@ __global__ __launch_bounds__(kSmallT) void ortho_small_kernel(const O* __restric
 // of latencies, 9 us, once instead of the 3 to 5 times of separate products: 64 x 576 in 5 steps 98 -> 56 us.
 struct SlabArgs {
     SmallArgs a;
+    Step step;                      // not the first launch's
     int w, slabs, first, last;      // columns of a slab, a multiple of 32
     const double* norm;
     int blocks;
@@ -612,7 +662,7 @@ __global__ __launch_bounds__(kSmallT) void ortho_slab_kernel(const O* __restrict
         for (int j = 0; j < p.slabs; ++j)
 #pragma unroll
             for (int i = 0; i < NA; ++i) b[i] += old[(j * NA + i) * kSmallT];
-        gram_to_poly<NA>(A, sq, s, sp, lane, a, b);
+        gram_to_poly<NA>(A, sq, s, sp, lane, p.step, b);
         f32x4 x[NX];
         small_product<true, NX>(A, X, sx, sp, lane, x);
         __syncthreads();
@@ -622,7 +672,7 @@ __global__ __launch_bounds__(kSmallT) void ortho_slab_kernel(const O* __restrict
                 const int c = sx.c0(i) + q;
                 float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = x[i][e] * (p.last ? 1.f / (a.bs * kXs) : 1.f / a.bs);
+                for (int e = 0; e < 4; ++e) v[e] = x[i][e] * p.step.next;
                 if (!p.last) {
                     put4<3>(X.hi + r * px + c, X.lo - X.hi, v);
                     put4<3>(keep + r * p.w + c, sp * p.w, v);
@@ -763,36 +813,29 @@ void product(const Cut& c, ProductArgs p, const UseArgs& u, int M, int N, hipStr
         product_shape<Tiny, LA, LB, PA, PB, H, O>(p, u, tiles, q);
 }
 
-// stored B = 2^e B with |B| <= |a| + 2 |b| + 4 |c| below 2^15
-float b_scale(const double* co) {
-    const double bound = fabs(co[0]) + 2 * fabs(co[1]) + 4 * fabs(co[2]);
-    return (float)(bound > 0 ? exp2(floor(log2(32768.0 / bound))) : 1.0);
-}
-
 template <class O, bool LIGHT>
-void ortho_steps(const OrthoPlan& p, int batch, int m, int n, int steps, const double* co, char* ws, void* out, hipStream_t q) {
+void ortho_steps(const OrthoPlan& p, int batch, int m, int n, int steps, const Steps& st, char* ws, void* out, hipStream_t q) {
     f16 *x = reinterpret_cast<f16*>(ws + p.x0), *y = reinterpret_cast<f16*>(ws + p.x1);
     f16 *a = reinterpret_cast<f16*>(ws + p.a), *b = reinterpret_cast<f16*>(ws + p.b);
     float *part = reinterpret_cast<float*>(ws + p.part), *da = reinterpret_cast<float*>(ws + p.da), *db = da + (long long)batch * p.s;
     const long long px = 2ll * m * p.np, lox = (long long)m * p.np, pa = 2ll * p.s * p.sp, loa = (long long)p.s * p.sp;
-    const float bs = b_scale(co);
     const bool wide = m <= n;
     constexpr int P = LIGHT ? 1 : 2;      // planes of A, of B, and of X in A = X X^T
     for (int i = 0; i < steps; ++i) {
         const Operand X{x, p.np, lox, m, p.np}, A{a, p.sp, loa, p.s, p.sp}, B{b, p.sp, loa, p.s, p.sp};
+        const Step& f = st.s[i];
         const ProductArgs pg{X, X, px, px, 0, 0, 1, p.l, 1, batch, part};
-        const UseArgs ug{p.s, p.s, a, p.sp, loa, pa, nullptr, 0, 1.f / kXs, 0.f, 0.f, da, db, p.s, wide};
+        const UseArgs ug{p.s, p.s, a, p.sp, loa, pa, nullptr, 0, f.gram, 0.f, 0.f, da, db, p.s, wide};
         if (wide)
             product<kK, kK, P, P, How<kGram, LIGHT>, float>(p.gram, pg, ug, p.s, p.s, q);
         else
             product<kM, kM, P, P, How<kGram, LIGHT>, float>(p.gram, pg, ug, p.s, p.s, q);
         const ProductArgs pp{A, A, pa, pa, 0, 0, 1, p.s, 1, batch, part};
-        const UseArgs up{p.s, p.s, b, p.sp, loa, pa, a, pa, (float)(co[0] * bs), (float)(co[1] * bs / kXs),
-                         (float)(co[2] * bs / (kXs * kXs)), da, db, p.s, wide};
+        const UseArgs up{p.s, p.s, b, p.sp, loa, pa, a, pa, f.ca, f.cb, f.cc, da, db, p.s, wide};
         product<kK, kK, P, P, How<kPoly, LIGHT>, float>(p.poly, pp, up, p.s, p.s, q);
         const bool last = i + 1 == steps;
-        const UseArgs ua{m, n, last ? out : y, p.np, lox, last ? (long long)m * n : px, nullptr, 0,
-                         last ? 1.f / (bs * kXs) : 1.f / bs, 0.f, 0.f, da, db, p.s, wide};
+        const UseArgs ua{m, n, last ? out : y, p.np, lox, last ? (long long)m * n : px, nullptr, 0, f.next,
+                         0.f, 0.f, da, db, p.s, wide};
         const ProductArgs pw{wide ? X : B, wide ? B : X, wide ? px : pa, wide ? pa : px, 0, 0, 0, p.s, 1, batch, part};
         if (wide) {
             if (last)
@@ -812,19 +855,20 @@ void ortho_steps(const OrthoPlan& p, int batch, int m, int n, int steps, const d
 }
 
 template <class O, int NA, int NX>
-int small_launch(const void* g, void* out, int batch, const SmallArgs& a, int bytes, hipStream_t q) {
+int small_launch(const void* g, void* out, int batch, const SmallArgs& a, const Steps& st, int bytes, hipStream_t q) {
     if (bytes > 64 * 1024) {   // what a kernel may ask for without saying so
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&ortho_small_kernel<O, NA, NX>),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
         if (e != hipSuccess) return (int)e;
     }
-    ortho_small_kernel<O, NA, NX><<<batch, kSmallT, bytes, q>>>(static_cast<const O*>(g), static_cast<O*>(out), a);
+    ortho_small_kernel<O, NA, NX><<<batch, kSmallT, bytes, q>>>(static_cast<const O*>(g), static_cast<O*>(out), a, st);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? DS_OK : (int)e;
 }
 
 template <class O, int NA, int NX>
-int slab_launch(const OrthoPlan& p, const void* g, void* out, int batch, const SmallArgs& a, char* ws, hipStream_t q) {
+int slab_launch(const OrthoPlan& p, const void* g, void* out, int batch, const SmallArgs& a, const Steps& st, char* ws,
+                hipStream_t q) {
     const int s32 = (p.s + 31) & ~31, bytes = 4 * s32 * (p.slab + 8 + s32 + 8);
     if (bytes > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&ortho_slab_kernel<O, NA, NX>),
@@ -835,7 +879,7 @@ int slab_launch(const OrthoPlan& p, const void* g, void* out, int batch, const S
     double* norm = reinterpret_cast<double*>(ws + p.norm);
     ortho_norm_kernel<O><<<dim3(p.blocks, batch), 256, 0, q>>>(static_cast<const O*>(g), (long long)a.m * a.n, norm);
     for (int i = 0; i <= a.steps; ++i) {
-        const SlabArgs b{a, p.slab, p.slabs, i == 0, i == a.steps, norm, p.blocks, reinterpret_cast<f16*>(ws + p.x0),
+        const SlabArgs b{a, st.s[i > 0 ? i - 1 : 0], p.slab, p.slabs, i == 0, i == a.steps, norm, p.blocks, reinterpret_cast<f16*>(ws + p.x0),
                          parts[(i + 1) & 1], parts[i & 1]};
         ortho_slab_kernel<O, NA, NX><<<dim3(p.slabs, batch), kSmallT, bytes, q>>>(static_cast<const O*>(g), static_cast<O*>(out), b);
     }
@@ -844,23 +888,22 @@ int slab_launch(const OrthoPlan& p, const void* g, void* out, int batch, const S
 }
 
 template <class O>
-int ortho_any(const OrthoPlan& p, const void* g, int dtype, int batch, int m, int n, int steps, const double* co, double eps,
+int ortho_any(const OrthoPlan& p, const void* g, int dtype, int batch, int m, int n, int steps, const Steps& st, double eps,
               void* out, char* ws, hipStream_t q) {
     if (steps > 0 && (p.small || p.slab)) {
-        const float bs = b_scale(co);
-        const SmallArgs a{m, n, steps, eps, (float)(co[0] * bs), (float)(co[1] * bs / kXs), (float)(co[2] * bs / (kXs * kXs)), bs};
+        const SmallArgs a{m, n, steps, eps};
         const SmallPlan sp = small_plan(p.s, p.l);
         if (p.slab) {
             const int nx = cdiv(p.slab / 16, kSmallT / 64 / (sp.sp / 16));
-            return nx <= 2   ? slab_launch<O, 2, 2>(p, g, out, batch, a, ws, q)
-                   : nx <= 5 ? slab_launch<O, 2, 5>(p, g, out, batch, a, ws, q)
-                             : slab_launch<O, 2, 10>(p, g, out, batch, a, ws, q);
+            return nx <= 2   ? slab_launch<O, 2, 2>(p, g, out, batch, a, st, ws, q)
+                   : nx <= 5 ? slab_launch<O, 2, 5>(p, g, out, batch, a, st, ws, q)
+                             : slab_launch<O, 2, 10>(p, g, out, batch, a, st, ws, q);
         }
         const int nx = cdiv(sp.lp / 16, kSmallT / 64 / (sp.sp / 16));      // fragments of X a wave holds
-        if (sp.sp > 64) return small_launch<O, 8, 8>(g, out, batch, a, sp.bytes, q);
-        return nx <= 2   ? small_launch<O, 2, 2>(g, out, batch, a, sp.bytes, q)
-               : nx <= 5 ? small_launch<O, 2, 5>(g, out, batch, a, sp.bytes, q)
-                         : small_launch<O, 2, 10>(g, out, batch, a, sp.bytes, q);
+        if (sp.sp > 64) return small_launch<O, 8, 8>(g, out, batch, a, st, sp.bytes, q);
+        return nx <= 2   ? small_launch<O, 2, 2>(g, out, batch, a, st, sp.bytes, q)
+               : nx <= 5 ? small_launch<O, 2, 5>(g, out, batch, a, st, sp.bytes, q)
+                         : small_launch<O, 2, 10>(g, out, batch, a, st, sp.bytes, q);
     }
     double* part = reinterpret_cast<double*>(ws + p.norm);
     const long long mn = (long long)m * n;
@@ -874,9 +917,9 @@ int ortho_any(const OrthoPlan& p, const void* g, int dtype, int batch, int m, in
                                                           reinterpret_cast<f16*>(ws + p.x0), (long long)m * p.np,
                                                           2ll * m * p.np);
         if constexpr (std::is_same<O, bf16>::value) {
-            if (p.light) ortho_steps<O, true>(p, batch, m, n, steps, co, ws, out, q);
+            if (p.light) ortho_steps<O, true>(p, batch, m, n, steps, st, ws, out, q);
         }
-        if (!p.light) ortho_steps<O, false>(p, batch, m, n, steps, co, ws, out, q);
+        if (!p.light) ortho_steps<O, false>(p, batch, m, n, steps, st, ws, out, q);
     }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? DS_OK : (int)e;
@@ -897,14 +940,17 @@ int ds_orthogonalize(const void* update, int dtype, int batch, int m, int n, int
     const int rc = ds::check_ortho(batch, m, n);
     if (rc) return rc;
     if (steps > DS_ORTHO_MAX_STEPS || (dtype != DS_F32 && dtype != DS_F16 && dtype != DS_BF16)) return DS_ERR_UNSUPPORTED;
+    if (!isfinite(coefficients[0]) || !isfinite(coefficients[1]) || !isfinite(coefficients[2])) return DS_ERR_INVALID_ARG;
+    ds::Steps st;
+    if (!ds::steps_of(coefficients, steps, st)) return DS_ERR_UNSUPPORTED;
     if (((uintptr_t)out & 15) != 0) return DS_ERR_INVALID_ARG;
     const ds::OrthoPlan p = ds::ortho_plan(dtype, batch, m, n);
     if (!workspace || workspace_bytes < p.total || ((uintptr_t)workspace & 15) != 0) return DS_ERR_WORKSPACE;
     char* ws = static_cast<char*>(workspace);
     hipStream_t q = static_cast<hipStream_t>(stream);
-    if (dtype == DS_F32) return ds::ortho_any<float>(p, update, dtype, batch, m, n, steps, coefficients, eps, out, ws, q);
-    if (dtype == DS_F16) return ds::ortho_any<ds::f16>(p, update, dtype, batch, m, n, steps, coefficients, eps, out, ws, q);
-    return ds::ortho_any<ds::bf16>(p, update, dtype, batch, m, n, steps, coefficients, eps, out, ws, q);
+    if (dtype == DS_F32) return ds::ortho_any<float>(p, update, dtype, batch, m, n, steps, st, eps, out, ws, q);
+    if (dtype == DS_F16) return ds::ortho_any<ds::f16>(p, update, dtype, batch, m, n, steps, st, eps, out, ws, q);
+    return ds::ortho_any<ds::bf16>(p, update, dtype, batch, m, n, steps, st, eps, out, ws, q);
 }
 
 }  // extern "C"

@@ -289,6 +289,59 @@ def test_refusals_on_the_host():
     assert lib.ds_orthogonalize_workspace_bytes(0, 1, 0, 4) == 0
 
 
+# coefficients, steps: singular values grow to 3 and fall to 0; wander up to 3.2; double, quadruple; grow a thousandfold, and
+# by 4 and more (2^20 and beyond); shrink a thousandfold
+REACHES = [((3.375, -0.375, 0.0), 2), ((2.6, -0.25, 0.0), 5), ((2.0, 0.0, 0.0), 5), ((4.0, 0.0, 0.0), 3), ((10.0, 0.0, 0.0), 4),
+           ((1.0, 2.0, 0.5), 3), ((-3.0, -1.0, 0.0), 3), ((0.1, 0.0, 0.0), 4), ((0.0, 0.0, 1.5), 3), ((0.0, 0.0, 0.0), 2)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("co,steps", REACHES, ids=str)
+@pytest.mark.parametrize("shape", [(1, 1), (3, 5), (40, 60), (40, 700), (130, 90), (3, 200, 300)], ids=str)
+def test_coefficients_that_take_singular_values_far(co, steps, shape):
+    """In the Frobenius norm.  A step takes values of at most m to at most M = |a| m + |b| m^3 + |c| m^5 and errors to at most
+    L = |a| + 3 |b| m^2 + 5 |c| m^4 times themselves.  Its own error: three products of 22-bit operands (2^-21 each) with float32
+    sums, of matrices of norm m sqrt(k) at most whose absolute values' norms are sqrt(k) times theirs at most: 6 2^-21 k M."""
+    from depth_estimation_amd import optim
+    k = min(shape[-2:])
+    one_entry = torch.zeros(shape, device=DEV)
+    one_entry[..., 0, 0] = 1.0                       # rank one, along an axis: one entry holds the whole singular value
+    for g in (_update(shape, torch.float32, seed=3), one_entry, -one_entry):
+        want = _oracle(g, steps, co)
+        m, tol = 1.0, 0.0
+        for _ in range(steps):
+            a, b, c = (abs(x) for x in co)
+            big = a * m + b * m ** 3 + c * m ** 5
+            tol = tol * (a + 3 * b * m ** 2 + 5 * c * m ** 4) + 6 * 2.0 ** -21 * k * big
+            m = big
+        got = optim.orthogonalize(g, steps=steps, coefficients=co)
+        assert bool(torch.isfinite(got).all())
+        assert float((got.double().cpu() - want).norm()) <= tol * math.prod(shape[:-2]) ** 0.5 + 2.0 ** -24 * float(want.norm())
+
+
+@pytest.mark.gpu
+def test_coefficients_at_their_limit():
+    from depth_estimation_amd import optim
+    one = torch.ones(1, 1, device=DEV)
+    for co, steps in (((2.0 ** 24, 0.0, 0.0), 2), ((2.0, 0.0, 0.0), 25)):        # 2^24 before the last step
+        got = optim.orthogonalize(one, steps=steps, coefficients=co, eps=0.0)
+        assert abs(float(got) / co[0] ** steps - 1) <= steps * 2.0 ** -21
+    for co, steps in (((2.0 ** 24, 0.0, 0.0), 3), ((2.0, 0.0, 0.0), 26), ((2.0 ** 24 + 4, 0.0, 0.0), 2), ((0.0, 0.0, 10.0 ** 31), 1)):
+        with pytest.raises(RuntimeError):
+            optim.orthogonalize(one, steps=steps, coefficients=co, eps=0.0)
+
+
+def test_refusals_of_coefficients_on_the_host():
+    from depth_estimation_amd import _lib as L
+    if not os.path.exists(L.LIB_PATH):
+        pytest.skip("libdepthsynth.so not built (run __graft_entry__.build())")
+    import ctypes as C
+    lib, fake = L.lib(), 0x1000
+    for co, steps, want in (((3.0, 0.0, 0.0), 32, -2), ((2.0 ** 30, 0.0, 0.0), 2, -2), ((0.0, 0.0, 1e200), 1, -2),
+                            ((math.nan, 0.0, 0.0), 1, -1), ((1.0, math.inf, 0.0), 1, -1)):
+        assert lib.ds_orthogonalize(fake, 0, 1, 8, 8, steps, (C.c_double * 3)(*co), 0.0, fake, fake, 1 << 40, None) == want
+
+
 @pytest.mark.gpu
 def test_refusals_of_tensors():
     from depth_estimation_amd import optim
