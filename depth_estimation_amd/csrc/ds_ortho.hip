@@ -9,12 +9,13 @@
 // follow from the coefficients alone: singular values begin in [0, 1], so how far each step can take them is known before it
 // (steps_of), and entries are at most as large as the largest singular value.
 //
-// bf16 results of larger matrices need less, and take half the products (Light): A keeps one plane (11 bits) off the diagonal,
+// bf16 results of larger matrices after few steps need less, and take half the products (Light): A keeps one plane (11 bits) off the diagonal,
 // where its entries are small, and its diagonal in fp32 beside it.  B keeps one plane; what its diagonal, which carries most of
 // X, lost by that is made up for as a factor of the result's row: diag(d) X (1 + rounding) off the diagonal is the smaller part.
-// X keeps two planes where it is multiplied by B.  What that costs is 4e-4 .. 9e-4 of the result's norm (sides of 256 and more;
-// Gaussian, decaying and nearly low-rank matrices, written out in float64), under the 1.7e-3 that rounding the result to bf16
-// costs; without the factors 6e-4 .. 1.2e-3.
+// X keeps two planes where it is multiplied by B.  What that costs after five steps is 4e-4 .. 9e-4 of the result's norm (sides
+// of 256 and more; Gaussian, decaying and nearly low-rank matrices, written out in float64), under the 1.7e-3 that rounding the
+// result to bf16 costs; without the factors 6e-4 .. 1.2e-3.  It grows with the steps (ten: 1.8e-3), and with how steep the
+// polynomial is: small_errors() has the condition.
 #include "ds_gemm.h"
 #include "ds_internal.h"
 #include "../../include/depthsynth.h"
@@ -39,6 +40,20 @@ struct Steps {
 };
 constexpr int kMostShift = 24;
 
+// Whether one plane is enough for a bf16 result (Light): up to six steps of a polynomial p that lifts small singular values,
+// keeps all of them positive and at most sqrt(2), and has slopes of -1.7 .. 4 where it meets any.  Over 130 such polynomials
+// (written out in float64, 512 x 512 Gaussian, decaying and nearly low-rank) the result was off by 1.13e-3 of its norm at most;
+// with slopes to -3 by 1.5e-2, after ten steps of the default polynomial by 1.8e-3 and after 32 by 3.2e-3.
+bool small_errors(const double* co, int steps, double most /* the largest singular value before any step */) {
+    const double m2 = most * most;
+    auto value = [&](double t) { return co[0] + t * (co[1] + t * co[2]); };               // p(x) / x, t = x^2
+    auto slope = [&](double t) { return co[0] + t * (3 * co[1] + t * 5 * co[2]); };
+    auto steep = [&](double t) { return slope(t) > 4 || slope(t) < -1.7; };
+    if (steps > 6 || m2 > 2 || co[0] < 1 || !(value(m2) > 0) || steep(0) || steep(m2)) return false;
+    const double at = co[2] != 0 ? -co[1] / (2 * co[2]) : 0, turn = 0.6 * at;             // where the two have their extrema
+    return !(at > 0 && at < m2 && !(value(at) > 0)) && !(turn > 0 && turn < m2 && steep(turn));
+}
+
 // the largest |x (a + b x^2 + c x^4)| for x in [0, m]
 double reach_of(const double* co, double m) {
     auto at = [&](double t) { return fabs(sqrt(t) * (co[0] + t * (co[1] + t * co[2]))); };
@@ -53,8 +68,8 @@ double reach_of(const double* co, double m) {
     return most;
 }
 // false: singular values would leave the range (2^kMostShift before the last step, 2^100 after it; NaN)
-bool steps_of(const double* co, int steps, Steps& out) {
-    double m = 1;
+bool steps_of(const double* co, int steps, Steps& out, bool& light) {
+    double m = 1, most = 1;
     auto shift = [](double x) {
         const double e = x > 0 ? ceil(log2(x / sqrt(2.0))) : -kMostShift;
         return e < -kMostShift ? -kMostShift : e;     // (smaller yet: bits are lost one by one, as below any type's range)
@@ -66,11 +81,13 @@ bool steps_of(const double* co, int steps, Steps& out) {
         const double k = bound > 0 ? floor(log2(32768.0 / bound)) : 0, bs = exp2(k > 100 ? 100 : k);
         m = reach_of(co, m);
         const bool last = i + 1 == steps;
+        if (!last && m > most) most = m;
         if (!(m <= exp2(last ? 100 : kMostShift))) return false;
         const double next = last ? 1 : exp2(13 - shift(m));
         out.s[i] = Step{(float)(as / (xs * xs)), (float)(co[0] * bs), (float)(co[1] * bs / as), (float)(co[2] * bs / (as * as)),
                         (float)(next / (bs * xs))};
     }
+    light = small_errors(co, steps, most);
     return true;
 }
 // blocks that sum squares of one matrix: 4096 elements each, at most 512
@@ -727,7 +744,7 @@ size_t part_bytes(const Cut& c, int M, int N, bool tri, int batch) {
     const size_t b = side_of(c.shape);
     return c.splits > 1 ? (size_t)batch * tiles_of(c.shape, M, N, tri) * c.splits * b * b * 4 : 0;
 }
-OrthoPlan ortho_plan(int dtype, int batch, int m, int n) {
+OrthoPlan ortho_plan(int dtype, int batch, int m, int n, bool light) {      // light: where the sizes suit it
     OrthoPlan p;
     p.s = m < n ? m : n;
     p.l = m < n ? n : m;
@@ -736,7 +753,7 @@ OrthoPlan ortho_plan(int dtype, int batch, int m, int n) {
     p.blocks = norm_blocks((long long)m * n);
     // on smaller sides launches and latency are what a step takes, not products (five steps of 256 x 1024: 149 us so, 145
     // with all planes; 512 x 512 150 and 166, 1024 x 1024 229 and 254, 2048 x 2048 505 and 759)
-    p.light = dtype == DS_BF16 && p.s >= 512;
+    p.light = light && dtype == DS_BF16 && p.s >= 512;
     auto cut = [&](int M, int N, int K, int pairs, bool tri, bool strided) {
         return cut_of(
             [&](long long b) {
@@ -931,7 +948,9 @@ int ortho_any(const OrthoPlan& p, const void* g, int dtype, int batch, int m, in
 extern "C" {
 
 size_t ds_orthogonalize_workspace_bytes(int dtype, int batch, int m, int n) {
-    return ds::check_ortho(batch, m, n) ? 0 : ds::ortho_plan(dtype, batch, m, n).total;
+    if (ds::check_ortho(batch, m, n)) return 0;
+    const size_t a = ds::ortho_plan(dtype, batch, m, n, false).total, b = ds::ortho_plan(dtype, batch, m, n, true).total;
+    return a > b ? a : b;
 }
 
 int ds_orthogonalize(const void* update, int dtype, int batch, int m, int n, int steps, const double* coefficients, double eps,
@@ -942,9 +961,10 @@ int ds_orthogonalize(const void* update, int dtype, int batch, int m, int n, int
     if (steps > DS_ORTHO_MAX_STEPS || (dtype != DS_F32 && dtype != DS_F16 && dtype != DS_BF16)) return DS_ERR_UNSUPPORTED;
     if (!isfinite(coefficients[0]) || !isfinite(coefficients[1]) || !isfinite(coefficients[2])) return DS_ERR_INVALID_ARG;
     ds::Steps st;
-    if (!ds::steps_of(coefficients, steps, st)) return DS_ERR_UNSUPPORTED;
+    bool light;
+    if (!ds::steps_of(coefficients, steps, st, light)) return DS_ERR_UNSUPPORTED;
     if (((uintptr_t)out & 15) != 0) return DS_ERR_INVALID_ARG;
-    const ds::OrthoPlan p = ds::ortho_plan(dtype, batch, m, n);
+    const ds::OrthoPlan p = ds::ortho_plan(dtype, batch, m, n, light);
     if (!workspace || workspace_bytes < p.total || ((uintptr_t)workspace & 15) != 0) return DS_ERR_WORKSPACE;
     char* ws = static_cast<char*>(workspace);
     hipStream_t q = static_cast<hipStream_t>(stream);

@@ -16,8 +16,9 @@ COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # steep at zero: five steps bring sin
 def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7) -> torch.Tensor:
     """update (...,m,n) float32, float16 or bfloat16 on the GPU -> same shape and dtype: X = G / (|G|_F + eps), then `steps`
     (0..32) times X = (a I + b A + c A A) X with A = X X^T on the smaller side.  No gradient flows.  Products on 22-bit
-    operands with float32 sums, one rounding at the end; bfloat16 matrices with sides of 512 and more take 11-bit operands
-    where that costs less than the rounding of the result does.  Coefficients that would take singular values of
+    operands with float32 sums, one rounding at the end; up to six steps of bfloat16 matrices with sides of 512 and more take
+    11-bit operands where that costs less than the rounding of the result does (1.2e-3 of its norm at most, against 1.7e-3;
+    coefficients whose polynomial is steeper than the default's keep 22 bits).  Coefficients that would take singular values of
     [0,1] beyond 2^24 before the last step are refused (the default keeps them below 1.3).  Parts of X below 2^-38 are not
     kept: with a norm of G far below eps the result loses digits."""
     return ops.orthogonalize(update, steps, coefficients, eps)

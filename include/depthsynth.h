@@ -334,8 +334,9 @@ int ds_bin_expect_bwd(const void* hidden, long long ldh, const void* weight, con
 /* An update orthogonalised by Newton-Schulz products: X = G / (|G|_F + eps); `steps` times, on the smaller side,
  * A = X X^T, X = (a + b A + c A A) X.  update and out: batch matrices (m,n), contiguous, of type `dtype`; out = update is
  * allowed.  coefficients: HOST double[3] a, b, c.  Products as for fp32 heads (22-bit operands, fp32 sums) for every dtype,
- * one rounding at the end; bf16 matrices whose smaller side is 512 or more take 11-bit operands where that costs less than
- * the rounding to bf16 does.  X, A and the polynomial are held under powers of two that follow from the coefficients (singular
+ * one rounding at the end; bf16 matrices whose smaller side is 512 or more take 11-bit operands for up to six steps of a
+ * polynomial no steeper than the usual one, where that costs less (1.2e-3 of the result's norm at most) than the rounding to
+ * bf16 does.  X, A and the polynomial are held under powers of two that follow from the coefficients (singular
  * values begin in [0,1]); coefficients under which singular values could pass 2^24 before the last step are refused
  * (DS_ERR_UNSUPPORTED).  Parts of X below 2^-38 (a norm far below eps) are lost.  workspace (16-byte aligned) from
  * ds_orthogonalize_workspace_bytes. */
