@@ -84,6 +84,7 @@ _SIGNATURES = {
     "ds_bin_expect_fwd": (_i, [_fp, _ll, _fp, _fp, _i, _ll, _i, _i, _fp, _fp, _fp, _sz, _fp]),
     "ds_bin_expect_bwd": (_i, [_fp, _ll, _fp, _fp, _fp, _i, _ll, _i, _i, _fp, _fp, _fp, _fp, _sz, _fp]),
     "ds_orthogonalize_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "ds_orthogonalize_check": (_i, [_i, _i, _i, _i, _i, C.POINTER(C.c_double), C.c_double]),
     "ds_orthogonalize": (_i, [_fp, _i, _i, _i, _i, _i, C.POINTER(C.c_double), C.c_double, _fp, _fp, _sz, _fp]),
 }
 

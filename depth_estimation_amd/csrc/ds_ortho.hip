@@ -803,6 +803,15 @@ int check_ortho(int batch, int m, int n) {
     return DS_OK;
 }
 
+int check_call(int dtype, int batch, int m, int n, int steps, const double* co, double eps, Steps& st, bool& light) {
+    if (!co || steps < 0 || !(eps >= 0)) return DS_ERR_INVALID_ARG;
+    const int rc = check_ortho(batch, m, n);
+    if (rc) return rc;
+    if (steps > DS_ORTHO_MAX_STEPS || (dtype != DS_F32 && dtype != DS_F16 && dtype != DS_BF16)) return DS_ERR_UNSUPPORTED;
+    if (!isfinite(co[0]) || !isfinite(co[1]) || !isfinite(co[2])) return DS_ERR_INVALID_ARG;
+    return steps_of(co, steps, st, light) ? DS_OK : DS_ERR_UNSUPPORTED;
+}
+
 template <class S, Lay LA, Lay LB, int PA, int PB, class H, class O>
 void product_shape(ProductArgs p, const UseArgs& u, int tiles, hipStream_t q) {
     const int units = tiles * p.splits;
@@ -953,16 +962,19 @@ size_t ds_orthogonalize_workspace_bytes(int dtype, int batch, int m, int n) {
     return a > b ? a : b;
 }
 
-int ds_orthogonalize(const void* update, int dtype, int batch, int m, int n, int steps, const double* coefficients, double eps,
-                     void* out, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!update || !out || !coefficients || steps < 0 || !(eps >= 0)) return DS_ERR_INVALID_ARG;
-    const int rc = ds::check_ortho(batch, m, n);
-    if (rc) return rc;
-    if (steps > DS_ORTHO_MAX_STEPS || (dtype != DS_F32 && dtype != DS_F16 && dtype != DS_BF16)) return DS_ERR_UNSUPPORTED;
-    if (!isfinite(coefficients[0]) || !isfinite(coefficients[1]) || !isfinite(coefficients[2])) return DS_ERR_INVALID_ARG;
+int ds_orthogonalize_check(int dtype, int batch, int m, int n, int steps, const double* coefficients, double eps) {
     ds::Steps st;
     bool light;
-    if (!ds::steps_of(coefficients, steps, st, light)) return DS_ERR_UNSUPPORTED;
+    return ds::check_call(dtype, batch, m, n, steps, coefficients, eps, st, light);
+}
+
+int ds_orthogonalize(const void* update, int dtype, int batch, int m, int n, int steps, const double* coefficients, double eps,
+                     void* out, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!update || !out) return DS_ERR_INVALID_ARG;
+    ds::Steps st;
+    bool light;
+    const int rc = ds::check_call(dtype, batch, m, n, steps, coefficients, eps, st, light);
+    if (rc) return rc;
     if (((uintptr_t)out & 15) != 0) return DS_ERR_INVALID_ARG;
     const ds::OrthoPlan p = ds::ortho_plan(dtype, batch, m, n, light);
     if (!workspace || workspace_bytes < p.total || ((uintptr_t)workspace & 15) != 0) return DS_ERR_WORKSPACE;

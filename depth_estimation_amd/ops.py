@@ -804,26 +804,41 @@ def bin_expectation(hidden, weight, centers) -> torch.Tensor:
 # ----------------------------------------------------------------------------------------------------
 # an update matrix orthogonalised by Newton-Schulz products
 # ----------------------------------------------------------------------------------------------------
-def orthogonalize(update, steps: int, coefficients, eps: float) -> torch.Tensor:
-    """update (...,m,n) -> the same shape and dtype; no gradient flows."""
-    u = L.dev_float(update.detach() if isinstance(update, torch.Tensor) else update, "update").contiguous()
-    if u.dim() < 2:
-        raise RuntimeError(f"update must be (...,m,n), got {tuple(u.shape)}")
+def orthogonalize_options(steps, coefficients, eps):
+    """-> steps, coefficients (a C array) and eps, or RuntimeError where no size would make a call of them."""
     co = [float(x) for x in coefficients]
     if len(co) != 3:
         raise RuntimeError(f"coefficients must be three numbers (a, b, c), got {len(co)}")
     if not all(np.isfinite(co)) or not 0 <= float(eps) < float("inf"):
         raise RuntimeError(f"coefficients must be finite and eps >= 0, got {co}, {eps}")
+    if not 0 <= int(steps) <= 32:
+        raise RuntimeError(f"steps must be 0..32, got {steps}")
+    return int(steps), (C.c_double * 3)(*co), float(eps)
+
+
+def orthogonalize_check(dtype, b: int, m: int, n: int, steps: int, co, eps: float) -> None:
+    """RuntimeError where orthogonalize would refuse b matrices (m,n) with these options; nothing is launched."""
+    if max(b, m, n) > _INT:
+        raise RuntimeError(f"orthogonalize: {b} matrices of {m} x {n} are not supported")
+    rc = L.lib().ds_orthogonalize_check(L.DTYPES[dtype], b, m, n, steps, co, eps)
+    L.check(rc, f"orthogonalize: {steps} steps of {b} matrices of {m} x {n} with coefficients {tuple(co)}")
+
+
+def orthogonalize(update, steps: int, coefficients, eps: float) -> torch.Tensor:
+    """update (...,m,n) -> the same shape and dtype; no gradient flows."""
+    u = L.dev_float(update.detach() if isinstance(update, torch.Tensor) else update, "update").contiguous()
+    if u.dim() < 2:
+        raise RuntimeError(f"update must be (...,m,n), got {tuple(u.shape)}")
+    steps, co, eps = orthogonalize_options(steps, coefficients, eps)
     L.same_device(u)
-    out = torch.empty_like(u)
     m, n = u.shape[-2:]
     if u.numel() == 0:
-        return out
+        return torch.empty_like(u)
     b, lib = u.numel() // (m * n), L.lib()
-    if max(b, m, n) > _INT or not 0 <= int(steps) <= 32:
-        raise RuntimeError(f"orthogonalize: {steps} steps of {tuple(u.shape)} are not supported")
+    orthogonalize_check(u.dtype, b, m, n, steps, co, eps)
+    out = torch.empty_like(u)
     nb = lib.ds_orthogonalize_workspace_bytes(L.DTYPES[u.dtype], b, m, n)
     ws = _scratch(nb, u.device)
-    L.check(lib.ds_orthogonalize(u.data_ptr(), L.DTYPES[u.dtype], b, m, n, int(steps), (C.c_double * 3)(*co), float(eps),
-                                 out.data_ptr(), ws.data_ptr(), nb, L.stream()), "ds_orthogonalize")
+    L.check(lib.ds_orthogonalize(u.data_ptr(), L.DTYPES[u.dtype], b, m, n, steps, co, eps, out.data_ptr(), ws.data_ptr(), nb,
+                                 L.stream()), "ds_orthogonalize")
     return out

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import torch
 
+from . import _lib as L
 from . import ops
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # steep at zero: five steps bring singular values from 0.01 up into 0.7 .. 1.2
@@ -30,7 +31,9 @@ class Muon(torch.optim.Optimizer):
         buf = momentum buf + grad;  u = grad + momentum buf (nesterov) or buf
         p = p (1 - lr weight_decay) - lr sqrt(max(1, m/n)) orthogonalize(u)
 
-    Matrices of one shape and dtype are orthogonalised as one batch."""
+    Matrices of one shape and dtype are orthogonalised as one batch.  Parameters that no call would take (fewer than two
+    dimensions, other types, a flattened side beyond 65536 or a smaller one beyond 32768: a head of 100000 classes) are refused
+    when they are added; a step that cannot be made raises before it has changed anything."""
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
                  steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7):
@@ -41,10 +44,45 @@ class Muon(torch.optim.Optimizer):
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
-        for p in self.param_groups[-1]["params"]:
-            if p.dim() < 2:
-                self.param_groups.pop()
-                raise ValueError(f"Muon steps matrices; a parameter of shape {tuple(p.shape)} belongs to another optimiser")
+        group = self.param_groups[-1]
+        try:
+            try:
+                ops.orthogonalize_options(group["steps"], group["coefficients"], group["eps"])
+            except RuntimeError as e:
+                raise ValueError(str(e)) from None
+            for p in group["params"]:
+                self._fits(p)
+        except ValueError:
+            self.param_groups.pop()
+            raise
+
+    @staticmethod
+    def _fits(p):
+        if p.dim() < 2:
+            raise ValueError(f"Muon steps matrices; a parameter of shape {tuple(p.shape)} belongs to another optimiser")
+        if p.dtype not in L.DTYPES:
+            raise ValueError(f"Muon steps float32, float16 and bfloat16; got {p.dtype}")
+        m, n = p.size(0), p.numel() // max(p.size(0), 1)
+        if max(m, n) > 1 << 16 or min(m, n) > 1 << 15:
+            raise ValueError(f"Muon steps matrices up to 65536 x 32768; a parameter of shape {tuple(p.shape)} ({m} x {n}) belongs "
+                             "to another optimiser")
+
+    def _check(self):
+        """Whatever would make a call of orthogonalize fail, before a buffer or a parameter has changed."""
+        for group in self.param_groups:
+            steps, co, eps = ops.orthogonalize_options(group["steps"], group["coefficients"], group["eps"])
+            shapes = {}
+            for p in group["params"]:
+                if p.grad is None or p.numel() == 0:
+                    continue
+                if p.grad.layout != torch.strided:
+                    raise RuntimeError(f"Muon: dense gradients only, got {p.grad.layout}")
+                L.dev_float(p.grad, "gradient")
+                L.same_device(p.grad, p)
+                key = p.grad.dtype, p.size(0), p.numel() // p.size(0)
+                shapes[key] = shapes.get(key, 0) + 1
+            for (dtype, m, n), b in shapes.items():
+                ops.orthogonalize_check(dtype, b, m, n, steps, co, eps)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -52,6 +90,7 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        self._check()
         for group in self.param_groups:
             same = {}
             for p in group["params"]:

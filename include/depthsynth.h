@@ -341,6 +341,8 @@ int ds_bin_expect_bwd(const void* hidden, long long ldh, const void* weight, con
  * (DS_ERR_UNSUPPORTED).  Parts of X below 2^-38 (a norm far below eps) are lost.  workspace (16-byte aligned) from
  * ds_orthogonalize_workspace_bytes. */
 size_t ds_orthogonalize_workspace_bytes(int dtype, int batch, int m, int n);
+/* What ds_orthogonalize answers to these arguments before it launches anything; host only. */
+int ds_orthogonalize_check(int dtype, int batch, int m, int n, int steps, const double* coefficients, double eps);
 int ds_orthogonalize(const void* update, int dtype, int batch, int m, int n, int steps, const double* coefficients, double eps,
                      void* out, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -356,6 +356,59 @@ def test_refusals_of_coefficients_on_the_host():
         assert lib.ds_orthogonalize(fake, 0, 1, 8, 8, steps, (C.c_double * 3)(*co), 0.0, fake, fake, 1 << 40, None) == want
 
 
+def test_muon_refuses_on_the_host():
+    from depth_estimation_amd import optim
+    ok = torch.nn.Parameter(torch.zeros(4, 4))
+    meta = torch.device("meta")
+    for p in (torch.empty(100_000, 8, device=meta), torch.empty(8, 70_000, device=meta), torch.empty(40_000, 40_000, device=meta),
+              torch.empty(8, 300, 300, device=meta), torch.empty(4, 4, dtype=torch.float64),
+              torch.empty(4, 4, dtype=torch.complex64)):
+        p = torch.nn.Parameter(p)
+        with pytest.raises(ValueError):
+            optim.Muon([ok, p])
+        muon = optim.Muon([ok])
+        with pytest.raises(ValueError):
+            muon.add_param_group(dict(params=[p]))
+        assert len(muon.param_groups) == 1
+    for bad in (dict(steps=-1), dict(steps=33), dict(coefficients=(1.0, 2.0)), dict(coefficients=(1.0, math.nan, 0.0)),
+                dict(eps=-1.0)):
+        with pytest.raises(ValueError):
+            optim.Muon([ok], **bad)
+    optim.Muon([torch.nn.Parameter(torch.empty(65536, 32768, device=meta)), torch.nn.Parameter(torch.empty(0, 5))])
+
+
+def test_muon_step_that_cannot_be_made_changes_nothing():
+    """One gradient of two is on the CPU, sparse, or the options are out of range: no buffer, no parameter moves."""
+    from depth_estimation_amd import optim
+    for how in ("cpu", "sparse", "steps"):
+        ps = [torch.nn.Parameter(torch.ones(4, 4)) for _ in range(2)]
+        muon = optim.Muon(ps)
+        for p in ps:
+            p.grad = torch.ones(4, 4)
+        if how == "sparse":
+            ps[0].grad = ps[0].grad.to_sparse()
+        if how == "steps":
+            muon.param_groups[0]["steps"] = 40
+        for _ in range(2):
+            with pytest.raises(RuntimeError):
+                muon.step()
+        assert all(torch.equal(p, torch.ones(4, 4)) for p in ps) and not muon.state
+
+
+@pytest.mark.gpu
+def test_muon_second_group_refused_before_the_first_moves():
+    from depth_estimation_amd import optim
+    a, b = (torch.nn.Parameter(torch.ones(6, 5, device=DEV)) for _ in range(2))
+    muon = optim.Muon([dict(params=[a]), dict(params=[b], coefficients=(3.0, 0.0, 0.0), steps=32)])      # beyond 2^24
+    a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+    with pytest.raises(RuntimeError):
+        muon.step()
+    assert torch.equal(a, torch.ones_like(a)) and not muon.state
+    muon.param_groups[1]["steps"] = 5
+    muon.step()
+    assert not torch.equal(a, torch.ones_like(a)) and torch.equal(muon.state[a]["momentum_buffer"], a.grad)
+
+
 @pytest.mark.gpu
 def test_refusals_of_tensors():
     from depth_estimation_amd import optim
