@@ -540,12 +540,11 @@ __device__ __forceinline__ void put_row8(O* row, int c, int n, int lane, const f
     }
 }
 
-// the power of two that brings a largest magnitude `amax` into [2^14, 2^15): fp16 keeps a factor of two of headroom
-__device__ __forceinline__ float scale_for(float amax) {
-    if (!(amax > 0.f) || !__builtin_isfinite(amax)) return 1.f;
-    int e = 14 - ilogbf(amax);
-    e = e > 60 ? 60 : (e < -110 ? -110 : e);
-    return ldexpf(1.f, e);
+// the power of two that brings a largest magnitude `amax` into [2^14, 2^15): fp16 keeps a factor of two of headroom.  As an
+// exponent, for ldexpf: that of the smallest float32 is 163, whose power is none
+__device__ __forceinline__ int shift_for(float amax) { return amax > 0.f && __builtin_isfinite(amax) ? 14 - ilogbf(amax) : 0; }
+__device__ __forceinline__ f32x4 scaled(const f32x4& v, int e) {
+    return f32x4{ldexpf(v[0], e), ldexpf(v[1], e), ldexpf(v[2], e), ldexpf(v[3], e)};
 }
 
 // ---- which shape a product takes, and over how many workgroups its sum is split (host) -----------------------------------

@@ -257,7 +257,7 @@ __global__ __launch_bounds__(256) void stage_kernel(Source s0, Source s1, int D,
     const IT* x = static_cast<const IT*>(s.x);
     const int c = s.cnt ? *s.cnt : s.n;
     const int lane = threadIdx.x & 63, sub = lane & (L - 1), R = 64 / L;
-    const float scale = SPLIT == 3 ? scale_for(from_bits(*s.amax)) : 1.f;
+    const int shift = SPLIT == 3 ? shift_for(from_bits(*s.amax)) : 0;
     constexpr int U = 4;
     const int hop = s.blocks * 4 * R;
     for (int r0 = (((int)blockIdx.x - s.first) * 4 + (threadIdx.x >> 6)) * R + lane / L; r0 < c; r0 += hop * U)
@@ -278,7 +278,7 @@ __global__ __launch_bounds__(256) void stage_kernel(Source s0, Source s1, int D,
                 for (int e = 0; e < VEC; ++e) {
                     if constexpr (SPLIT == 3) {
                         f16 a, b;
-                        split16((float)v[u][e] * scale, a, b);
+                        split16(ldexpf((float)v[u][e], shift), a, b);
                         h[e] = a;
                         l[e] = b;
                     } else {
@@ -289,6 +289,11 @@ __global__ __launch_bounds__(256) void stage_kernel(Source s0, Source s1, int D,
                 if (SPLIT == 3) *reinterpret_cast<typename Vec<T, VEC>::type*>(q + s.lo) = l;
             }
         }
+}
+
+// exponent of accumulated products of planes -> logits
+__device__ __forceinline__ int logit_shift(const HeadState* st) {
+    return -shift_for(from_bits(st->amax_h)) - shift_for(from_bits(st->amax_w));
 }
 
 // ------------------------------------------------------------------------------------------------------------ forward
@@ -315,11 +320,11 @@ __device__ __forceinline__ void stats_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / S::WN, wn = wave % S::WN, v0 = m0 + wm * S::FM * 16 + (lane >> 4) * 4;
     if (SPLIT == 3) {
-        const float ih = 1.f / scale_for(from_bits(st->amax_h)), iw = 1.f / scale_for(from_bits(st->amax_w));
+        const int shift = logit_shift(st);
 #pragma unroll
         for (int i = 0; i < S::FM; ++i)
 #pragma unroll
-            for (int j = 0; j < S::FN; ++j) acc[i][j] = acc[i][j] * ih * iw;
+            for (int j = 0; j < S::FN; ++j) acc[i][j] = scaled(acc[i][j], shift);
     }
     const bool edge = m0 + S::BM > a.V;      // only the last class tile has classes that do not exist
 #pragma unroll
@@ -529,18 +534,13 @@ __global__ __launch_bounds__(256) void loss_total_kernel(const double* __restric
 }
 
 // ----------------------------------------------------------------------------------------------------------- backward
-// How dl is scaled: fp16 storage wants values of a fixed size, so dl is kept as dl / |g|max (a power of two >= the largest
-// upstream value, times 2 |c|max for the expectation) * 2^14; bf16 has fp32's range and takes the same with 2^0.
-template <class T> struct Store;
-template <> struct Store<f16> { static constexpr float k = 16384.f; };
-template <> struct Store<bf16> { static constexpr float k = 1.f; };
+// How dl is scaled: fp16 storage wants values of a fixed size, so dl is kept as 2^14 dl / 2^e, where 2^e is above the largest
+// upstream value, times the largest |c - E| for the expectation.  bf16 has fp32's range and takes dl as it is.  All powers of two
+// are exponents, for ldexpf: upstreams of 1e38 or 1e-38 are in range.
+constexpr int kDlTop = 14;
 
-__device__ __forceinline__ float pow2_above(float x) {
-    if (!(x > 0.f) || !__builtin_isfinite(x)) return 1.f;
-    int e = ilogbf(x) + 1;
-    e = e > 120 ? 120 : (e < -120 ? -120 : e);
-    return ldexpf(1.f, e);
-}
+// the least e with |x| < 2^e; 0 where there is none
+__device__ __forceinline__ int exp_above(float x) { return x > 0.f && __builtin_isfinite(x) ? ilogbf(x) + 1 : 0; }
 struct Upstream {
     const float* g;      // one value, or one per row of the caller
     int each, mean;
@@ -550,16 +550,24 @@ __device__ __forceinline__ float upstream(const Upstream& u, int n, int cnt) {
     if (u.each) return u.g[u.rows ? u.rows[n] : n];
     return u.mean ? u.g[0] / cnt : u.g[0];
 }
-// the power of two dl is divided by, before Store<T>::k
+// |c - E| < 2^e; as a factor 2^-e of the centres (in float32's normal range)
+__device__ __forceinline__ int center_exp(const BackState* bs) {
+    const int e = exp_above(from_bits(bs->cmax)) + 1;
+    return e < -125 ? -125 : (e > 126 ? 126 : e);
+}
+// exponents: the upstream value's in dl, and all of dl's
 template <class T>
-__device__ __forceinline__ float dl_norm(const BackState* bs, const Upstream& u, int mode, int cnt) {
-    if (std::is_same<T, bf16>::value) return 1.f;
-    if (mode == kCE && !u.each) return pow2_above(finite_abs(upstream(u, 0, cnt)));
-    const float g = pow2_above(from_bits(bs->gmax));
-    return mode == kExpect ? g * pow2_above(2.f * from_bits(bs->cmax)) : g;
+__device__ __forceinline__ int up_exp(const BackState* bs, const Upstream& u, int mode, int cnt) {
+    if (std::is_same<T, bf16>::value) return 0;
+    return kDlTop - (mode == kCE && !u.each ? exp_above(fabsf(upstream(u, 0, cnt))) : exp_above(from_bits(bs->gmax)));
+}
+template <class T>
+__device__ __forceinline__ int dl_exp(const BackState* bs, const Upstream& u, int mode, int cnt) {
+    if (std::is_same<T, bf16>::value) return 0;
+    return up_exp<T>(bs, u, mode, cnt) - (mode == kExpect ? center_exp(bs) : 0);
 }
 
-// largest |upstream| and |centre|, where dl_norm asks for them; *bs zeroed by back_init_kernel before, unless one workgroup
+// largest |upstream| and |centre|, where dl_exp asks for them; *bs zeroed by back_init_kernel before, unless one workgroup
 // does it all (a launch less)
 constexpr int kScaleT = 512, kScaleAlone = 16 * kScaleT;
 __global__ void back_init_kernel(BackState* bs) { bs->gmax = bs->cmax = 0; }
@@ -612,9 +620,8 @@ struct DlArgs {
 template <class T, class S, int SPLIT, int MODE>
 __device__ __forceinline__ void dl_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int cnt, const HeadState* st,
                                            const BackState* bs, const DlArgs& a) {
-    const float il = SPLIT == 3 ? 1.f / scale_for(from_bits(st->amax_h)) : 1.f;
-    const float iw = SPLIT == 3 ? 1.f / scale_for(from_bits(st->amax_w)) : 1.f;
-    const float norm = Store<T>::k / dl_norm<T>(bs, a.up, MODE, cnt);
+    const int shift = SPLIT == 3 ? logit_shift(st) : 0, ue = up_exp<T>(bs, a.up, MODE, cnt);
+    const float cs = MODE == kExpect && !std::is_same<T, bf16>::value ? ldexpf(1.f, -center_exp(bs)) : 1.f;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / S::WN, wn = wave % S::WN, c0 = m0 + wm * S::FM * 16 + (lane >> 4) * 4;
     T* dl = static_cast<T*>(a.dl);
@@ -624,7 +631,7 @@ __device__ __forceinline__ void dl_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, i
         const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
         if (n >= cnt) continue;
         const float tp = a.top[n], rs = a.inv_sum[n];
-        float g = upstream(a.up, n, cnt) * norm;
+        float g = ldexpf(upstream(a.up, n, cnt), ue);
         if (MODE == kCE) {
             const int t = a.tgt[n] - a.v0 - c0;
             if (a.tgt[n] < 0) g = __builtin_nanf("");
@@ -633,19 +640,19 @@ __device__ __forceinline__ void dl_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, i
             for (int i = 0; i < S::FM; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float l = SPLIT == 3 ? acc[i][j][e] * il * iw : acc[i][j][e];
+                    const float l = SPLIT == 3 ? ldexpf(acc[i][j][e], shift) : acc[i][j][e];
                     const float x = exp_of(l - tp);
                     acc[i][j][e] = fmaf(x, gr, t == i * 16 + e ? -g : 0.f);
                 }
         } else {
-            const float e0 = a.mean[n], gr = g * rs;
+            const float e0 = a.mean[n] * cs, gr = g * rs;      // (cs: a power of two, exact)
 #pragma unroll
             for (int i = 0; i < S::FM; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int c = c0 + i * 16 + e;
-                    const float l = SPLIT == 3 ? acc[i][j][e] * il * iw : acc[i][j][e];
-                    acc[i][j][e] = exp_of(l - tp) * gr * ((edge && c >= a.cols ? 0.f : a.centers[a.v0 + c]) - e0);
+                    const float l = SPLIT == 3 ? ldexpf(acc[i][j][e], shift) : acc[i][j][e];
+                    acc[i][j][e] = exp_of(l - tp) * gr * fmaf(edge && c >= a.cols ? 0.f : a.centers[a.v0 + c], cs, -e0);
                 }
         }
         if (edge) {
@@ -730,8 +737,8 @@ struct GradArgs {
 template <class T, class S, int SPLIT, class O, bool ACC, int WHICH>
 __device__ __forceinline__ void grad_of_tile(const f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int sp, int bound,
                                              const HeadState* st, const BackState* bs, const GradArgs& a) {
-    const float f0 = dl_norm<T>(bs, a.up, a.mode, st->count) / Store<T>::k;
-    const float is = SPLIT == 3 ? 1.f / scale_for(from_bits(WHICH == 0 ? st->amax_w : st->amax_h)) : 1.f;
+    const int back = -dl_exp<T>(bs, a.up, a.mode, st->count) -
+                     (SPLIT == 3 ? shift_for(from_bits(WHICH == 0 ? st->amax_w : st->amax_h)) : 0);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / S::WN, wn = wave % S::WN, Dp = (a.D + 3) & ~3;
 #pragma unroll
@@ -750,14 +757,14 @@ __device__ __forceinline__ void grad_of_tile(const f32x4 (&acc)[S::FM][S::FN], i
                 *q = v;
             }
         } else if (S::FM == 1) {
-            const f32x4 v = acc[0][j] * f0 * is;
+            const f32x4 v = scaled(acc[0][j], back);
             const float w[4] = {v[0], v[1], v[2], v[3]};
             put_row4(static_cast<O*>(a.out) + row * a.D, m0 + wm * 16 + (lane >> 4) * 4, a.D, w);
         } else {
 #pragma unroll
             for (int i = 0; i + 1 < S::FM; i += 2)
-                put_row8(static_cast<O*>(a.out) + row * a.D, m0 + (wm * S::FM + i) * 16, a.D, lane, acc[i][j] * f0 * is,
-                         acc[i + 1][j] * f0 * is);
+                put_row8(static_cast<O*>(a.out) + row * a.D, m0 + (wm * S::FM + i) * 16, a.D, lane, scaled(acc[i][j], back),
+                         scaled(acc[i + 1][j], back));
         }
     }
 }
@@ -818,8 +825,8 @@ __global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__
     constexpr int kOuts = 256 / PAR;
     __shared__ f32x4 red[PAR][kOuts + 1];
     const int cnt = which == 0 ? st->count : n, Dp = (D + 3) & ~3, q = Dp / 4;
-    const float f0 = dl_norm<T>(bs, up, mode, st->count) / Store<T>::k;
-    const float is = SPLIT == 3 ? 1.f / scale_for(from_bits(which == 0 ? st->amax_w : st->amax_h)) : 1.f;
+    const int back = -dl_exp<T>(bs, up, mode, st->count) -
+                     (SPLIT == 3 ? shift_for(from_bits(which == 0 ? st->amax_w : st->amax_h)) : 0);
     const long long all = (long long)cnt * q;
     const int x = threadIdx.x % kOuts, y = threadIdx.x / kOuts, per = (splits + PAR - 1) / PAR;
     for (long long i0 = (long long)blockIdx.x * kOuts; i0 < all; i0 += (long long)gridDim.x * kOuts) {
@@ -842,7 +849,8 @@ __global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__
         if (i < all && y == 0) {
             const long long r = i / q;
             const int d = (int)(i - r * q) * 4;
-            const float v[4] = {a[0] * f0 * is, a[1] * f0 * is, a[2] * f0 * is, a[3] * f0 * is};
+            a = scaled(a, back);
+            const float v[4] = {a[0], a[1], a[2], a[3]};
             put_row4(out + (rows && which == 0 ? (long long)rows[r] : r) * D, d, D, v);
         }
     }
@@ -902,7 +910,6 @@ struct SlimArgs {
     int set_count;
     int n, D, V, Vp;           // Vp: V rounded up to 32
     Operand W;
-    int planes_scaled;         // two planes: divide by the scales
     const int* tgt;
     const float* centers;
     float *top, *inv_sum, *mean;
@@ -974,7 +981,7 @@ struct SlimRows {
 };
 // logits of the 16 classes of fragment f for the wave's rows: lane holds row lane % 16, classes 16 f + 4 (lane / 16) + e
 template <class T, int P, int ND>
-__device__ __forceinline__ f32x4 slim_logits(const SlimRows<P, ND>& r, const char* lds, int base, int f, int Vp, float scale) {
+__device__ __forceinline__ f32x4 slim_logits(const SlimRows<P, ND>& r, const char* lds, int base, int f, int Vp, int shift) {
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < ND; ++k) {
@@ -987,7 +994,7 @@ __device__ __forceinline__ f32x4 slim_logits(const SlimRows<P, ND>& r, const cha
         }
         acc = mfma(w, r.h[0][k], acc, T());
     }
-    return P == 2 ? acc * scale : acc;
+    return P == 2 ? scaled(acc, shift) : acc;
 }
 __device__ __forceinline__ void join_softmax(float& mx, float& s, float& sc, float m2, float s2, float c2) {
     const float nm = fmaxf(mx, m2), ref = nm == -INFINITY ? 0.f : nm;
@@ -995,9 +1002,6 @@ __device__ __forceinline__ void join_softmax(float& mx, float& s, float& sc, flo
     s = s * f1 + s2 * f2;
     sc = sc * f1 + c2 * f2;
     mx = nm;
-}
-__device__ __forceinline__ float slim_scale(const SlimArgs& a) {
-    return a.planes_scaled ? 1.f / scale_for(from_bits(a.st->amax_h)) * (1.f / scale_for(from_bits(a.st->amax_w))) : 1.f;
 }
 
 template <class T, int P, int ND, int MODE>
@@ -1011,7 +1015,7 @@ __global__ __launch_bounds__(kSlimT) void slim_fwd_kernel(SlimArgs a, SlimFwd o)
     SlimRows<P, ND> next;
     if (b < blocks) next.load(a, b * 16 + (lane & 15), cnt, lane);
     slim_load_w<P, ND>(a, lds);
-    const float scale = slim_scale(a);
+    const int shift = P == 2 ? logit_shift(a.st) : 0;
     const int base = lds_chunk<kK, 16>(lane & 15, lane >> 4), frags = a.Vp / 16, q4 = (lane >> 4) * 4;
     const float* centers = reinterpret_cast<const float*>(lds + P * a.Vp * ND * 64);
     double total = 0.0;
@@ -1024,7 +1028,7 @@ __global__ __launch_bounds__(kSlimT) void slim_fwd_kernel(SlimArgs a, SlimFwd o)
         for (int f = 0; f < frags; f += 2) {
             f32x4 l[2];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) l[u] = slim_logits<T, P, ND>(r, lds, base, f + u, a.Vp, scale);
+            for (int u = 0; u < 2; ++u) l[u] = slim_logits<T, P, ND>(r, lds, base, f + u, a.Vp, shift);
             if (f * 16 + 32 > a.V) {       // classes that do not exist
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
@@ -1097,9 +1101,9 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
     SlimRows<P, ND> next;
     if (b < blocks) next.load(a, b * 16 + (lane & 15), cnt, lane);
     slim_load_w<P, ND>(a, lds);
-    const float scale = slim_scale(a), norm = Store<T>::k / dl_norm<T>(o.bs, o.up, MODE, cnt);
-    const float back = dl_norm<T>(o.bs, o.up, MODE, cnt) / Store<T>::k *
-                       (a.planes_scaled ? 1.f / scale_for(from_bits(a.st->amax_w)) : 1.f);
+    const int shift = P == 2 ? logit_shift(a.st) : 0, ue = up_exp<T>(o.bs, o.up, MODE, cnt);
+    const int back = -dl_exp<T>(o.bs, o.up, MODE, cnt) - (P == 2 ? shift_for(from_bits(a.st->amax_w)) : 0);
+    const float cs = MODE == kExpect && !std::is_same<T, bf16>::value ? ldexpf(1.f, -center_exp(o.bs)) : 1.f;
     const int base = lds_chunk<kK, 16>(lane & 15, lane >> 4), frags = a.Vp / 16, q4 = (lane >> 4) * 4;
     const float* centers = reinterpret_cast<const float*>(lds + P * a.Vp * ND * 64);
     // transposing reads: lane i of a 16-lane group q starts at class 4 q + i / 4, feature 4 (i % 4)
@@ -1111,9 +1115,9 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
         const SlimRows<P, ND> r = next;
         const int n = b * 16 + (lane & 15), m = n < cnt ? n : cnt - 1;
         if (b + step < blocks) next.load(a, (b + step) * 16 + (lane & 15), cnt, lane);
-        const float tp = a.top[m], rs = a.inv_sum[m], e0 = MODE == kExpect ? a.mean[m] : 0.f;
+        const float tp = a.top[m], rs = a.inv_sum[m], e0 = MODE == kExpect ? a.mean[m] * cs : 0.f;
         const int target = MODE == kCE ? a.tgt[m] : -1, t = target - q4;
-        float g = upstream(o.up, m, cnt) * norm;
+        float g = ldexpf(upstream(o.up, m, cnt), ue);
         if (MODE == kCE && target < 0) g = __builtin_nanf("");
         const float gr = g * rs;
         f32x4 acc[2 * ND];
@@ -1123,7 +1127,7 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
             f32x4 d[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const f32x4 l = slim_logits<T, P, ND>(r, lds, base, f + u, a.Vp, scale);
+                const f32x4 l = slim_logits<T, P, ND>(r, lds, base, f + u, a.Vp, shift);
                 const int v = (f + u) * 16 + q4;
                 f32x4 c = {0.f, 0.f, 0.f, 0.f};
                 if (MODE == kExpect) c = *reinterpret_cast<const f32x4*>(centers + v);
@@ -1131,7 +1135,7 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
                 for (int e = 0; e < 4; ++e) {
                     const float x = exp_of(l[e] - tp);
                     if (MODE == kExpect)
-                        d[u][e] = x * gr * (c[e] - e0);
+                        d[u][e] = x * gr * fmaf(c[e], cs, -e0);
                     else
                         d[u][e] = fmaf(x, gr, (f + u) * 16 + e == t ? -g : 0.f);
                 }
@@ -1184,7 +1188,8 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
 #pragma unroll
                 for (int i = 0; i < 2 * ND; ++i) {
                     const int c = i * 16 + (lane >> 4) * 4;
-                    const float y[4] = {acc[i][0] * back, acc[i][1] * back, acc[i][2] * back, acc[i][3] * back};
+                    const f32x4 x = scaled(acc[i], back);
+                    const float y[4] = {x[0], x[1], x[2], x[3]};
                     if (c < a.D) put_row4(row, c, a.D, y);
                 }
             }
@@ -1536,7 +1541,7 @@ int with_lds(K kernel, int bytes) {    // what a kernel may use beyond 64 KB it 
 }
 SlimArgs slim_args(const Plan& p, const Operand& H, const Operand& W, const Saved& s, const int* rows, long long N, int D, int V,
                    const float* centers) {
-    return SlimArgs{H.p, H.ld, H.lo, p.stage_h ? nullptr : rows, rows, s.st, 0, (int)N, D, V, (V + 31) & ~31, W, p.planes == 2,
+    return SlimArgs{H.p, H.ld, H.lo, p.stage_h ? nullptr : rows, rows, s.st, 0, (int)N, D, V, (V + 31) & ~31, W,
                     s.tgt, centers, s.top, s.inv_sum, s.mean};
 }
 template <class T, int P, int ND, int MODE>
@@ -1717,7 +1722,7 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
     const int* rows = mode == kCE ? s.rows : nullptr;
     BackState* bs = reinterpret_cast<BackState*>(ws + p.bs);
     Upstream up{g, reduction == DS_REDUCE_NONE, reduction == DS_REDUCE_MEAN, rows};
-    if (!std::is_same<T, bf16>::value && up.each) {    // where dl_norm reads it
+    if (!std::is_same<T, bf16>::value && up.each) {    // where up_exp reads it
         const long long most = centers && V > N ? V : N;
         const int blocks = most <= kScaleAlone ? 1 : cdiv(most, 4 * kScaleT) < 256 ? cdiv(most, 4 * kScaleT) : 256;
         if (blocks > 1) back_init_kernel<<<1, 1, 0, q>>>(bs);

@@ -248,6 +248,44 @@ def test_float32_of_any_size(scale_h, scale_w):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,d,v", [(50, 33, 40), (200, 301, 700), (3, 40, 500)])
+@pytest.mark.parametrize("scale_h,scale_w", [(1e-30, 1e30), (1e30, 1e-30), (2e37, 1e-37), (1e-36, 1e35), (1e-25, 1e-10), (1e-5, 1e-28)])
+def test_float32_to_the_ends_of_its_range(n, d, v, scale_h, scale_w):
+    """As above, to where float32's normal numbers end, in kernels for small heads, tiles and few rows."""
+    h, w, t, up, c = _data(n, d, v, torch.float32, seed=n, keep=0.9 if n > 3 else 1.0)
+    h, w = h * scale_h, w * scale_w
+    for got, (out, gh, gw, tol, th, tw) in ((_ce(h, w, t, "none", up), _oracle(h, w, t=t, up=up)),
+                                            (_ex(h, w, c, up), _oracle(h, w, c=c, up=up))):
+        _close(got[0], out, tol, "output")
+        for a, b, tol_ in ((got[1], gh, th), (got[2], gw, tw)):
+            inside = b.abs() < torch.finfo(torch.float32).max / 4
+            _close(a[inside], b[inside], tol_[inside], "gradient")
+
+
+# factors of the upstream values and of the centres; float16's gradients stay in range only where one makes up for the other
+FAR = [(torch.float32, 1e-36, 1.0), (torch.float32, 1e36, 1.0), (torch.bfloat16, 1e-28, 1.0), (torch.bfloat16, 1e36, 1.0)] + [
+    (t, a, b) for t in TYPES for a, b in ((1e-30, 1e30), (1e30, 1e-30))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,size_up,size_c", FAR, ids=str)
+@pytest.mark.parametrize("n,d,v", [(60, 40, 50), (200, 64, 900)])
+def test_upstreams_and_centers_of_any_size(n, d, v, dtype, size_up, size_c):
+    h, w, t, up, c = _data(n, d, v, dtype, seed=n, keep=0.9)
+    up, c = up * size_up, c * size_c
+    pairs = [(_ex(h, w, c, up), _oracle(h, w, c=c, up=up))]
+    if size_c == 1.0:
+        pairs.append((_ce(h, w, t, "none", up), _oracle(h, w, t=t, up=up)))
+        f = float(up[0])
+        pairs.append((_ce(h, w, t, "sum", up[0]), _oracle(h, w, t=t, up=torch.full_like(up, f))))
+    for got, (out, gh, gw, tol, th, tw) in pairs:
+        if got[0].dim():
+            _close(got[0], out, tol, "output")
+        _close(got[1], gh, th, "g_hidden")
+        _close(got[2], gw, tw, "g_weight")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_large_logits_and_upstreams(dtype):
     """Logits of +-100s, upstream values from 1e-6 to 1e6 and zero in one call."""
