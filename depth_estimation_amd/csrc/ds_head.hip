@@ -17,6 +17,7 @@
 #include "ds_gemm.h"
 #include "ds_internal.h"
 #include "../../include/depthsynth.h"
+#include <algorithm>
 #include <type_traits>
 
 namespace ds {
@@ -36,10 +37,11 @@ struct HeadState {
     int pad[13];
 };
 struct BackState {
-    unsigned gmax;       // bits of max |upstream| over kept rows
+    int most;            // the largest exponent a kept row takes part in dW with (kNone: no row does)
     unsigned cmax;       // bits of max |centre|
     int pad[14];
 };
+constexpr int kNone = -(1 << 30);
 
 
 __device__ __forceinline__ float from_bits(unsigned u) { return __builtin_bit_cast(float, u); }
@@ -534,9 +536,11 @@ __global__ __launch_bounds__(256) void loss_total_kernel(const double* __restric
 }
 
 // ----------------------------------------------------------------------------------------------------------- backward
-// How dl is scaled: fp16 storage wants values of a fixed size, so dl is kept as 2^14 dl / 2^e, where 2^e is above the largest
-// upstream value, times the largest |c - E| for the expectation.  bf16 has fp32's range and takes dl as it is.  All powers of two
-// are exponents, for ldexpf: upstreams of 1e38 or 1e-38 are in range.
+// How dl is scaled: fp16 storage wants values of a fixed size, so a row of dl is kept as 2^14 dl / 2^e, where 2^e is above the
+// row's upstream value, times the largest |c - E| for the expectation; dH's rows are scaled back one by one, so that a row keeps
+// its digits whatever the others' upstream is.  dW adds rows up, weighted with 2^e, and what is lost there is 2^-39 of the largest
+// row's part.  bf16 has fp32's range and takes dl as it is.  All powers of two are exponents, for ldexpf: upstreams of 1e38 or
+// 1e-38 are in range.
 constexpr int kDlTop = 14;
 
 // the least e with |x| < 2^e; 0 where there is none
@@ -555,50 +559,113 @@ __device__ __forceinline__ int center_exp(const BackState* bs) {
     const int e = exp_above(from_bits(bs->cmax)) + 1;
     return e < -125 ? -125 : (e > 126 ? 126 : e);
 }
-// exponents: the upstream value's in dl, and all of dl's
+// exponent e of a row's upstream value, 0 where T needs none
 template <class T>
-__device__ __forceinline__ int up_exp(const BackState* bs, const Upstream& u, int mode, int cnt) {
-    if (std::is_same<T, bf16>::value) return 0;
-    return kDlTop - (mode == kCE && !u.each ? exp_above(fabsf(upstream(u, 0, cnt))) : exp_above(from_bits(bs->gmax)));
+__device__ __forceinline__ int row_exp(float g) { return std::is_same<T, bf16>::value ? 0 : exp_above(fabsf(g)); }
+// exponent of a row of stored dl -> dl: this and the row's
+template <class T>
+__device__ __forceinline__ int dl_exp(const BackState* bs, int mode) {
+    return std::is_same<T, bf16>::value ? 0 : (mode == kExpect ? center_exp(bs) : 0) - kDlTop;
 }
+// exponent of a row's weight in dW, at most 0: rows without a gradient weigh nothing either way, and are left as they are
+__device__ __forceinline__ int weight_exp(const BackState* bs, float g) {
+    return g != 0.f && __builtin_isfinite(g) ? exp_above(fabsf(g)) - bs->most : 0;
+}
+// exponent of sums over rows -> dW, beside the inputs' own
 template <class T>
-__device__ __forceinline__ int dl_exp(const BackState* bs, const Upstream& u, int mode, int cnt) {
+__device__ __forceinline__ int dw_exp(const BackState* bs, const Upstream& u, int mode, int cnt) {
     if (std::is_same<T, bf16>::value) return 0;
-    return up_exp<T>(bs, u, mode, cnt) - (mode == kExpect ? center_exp(bs) : 0);
+    return dl_exp<T>(bs, mode) + (u.each ? bs->most == kNone ? 0 : bs->most : row_exp<T>(upstream(u, 0, cnt)));
 }
 
-// largest |upstream| and |centre|, where dl_exp asks for them; *bs zeroed by back_init_kernel before, unless one workgroup
-// does it all (a launch less)
+// bs->most (with `h`, the features of float16 rows that fold_rows_kernel will weigh: as far as they reach, too) and the largest
+// |centre|, for upstreams that differ; *bs set by back_init_kernel before, unless one workgroup does it all (a launch less)
 constexpr int kScaleT = 512, kScaleAlone = 16 * kScaleT;
-__global__ void back_init_kernel(BackState* bs) { bs->gmax = bs->cmax = 0; }
+__global__ void back_init_kernel(BackState* bs) {
+    bs->most = kNone;
+    bs->cmax = 0;
+}
+struct Features {
+    const f16* h;        // NULL: not asked for
+    long long ld;
+    const int* rows;     // listed rows (NULL: in order)
+    int D, L;
+};
 __global__ __launch_bounds__(kScaleT) void back_scale_kernel(Upstream u, const HeadState* __restrict__ st,
-                                                         const float* __restrict__ centers, int V, BackState* __restrict__ bs) {
-    __shared__ float red[kScaleT / 64][2];
+                                                             const float* __restrict__ centers, int V, Features f,
+                                                             BackState* __restrict__ bs) {
+    __shared__ float red[kScaleT / 64];
+    __shared__ int top[kScaleT / 64];
     const int cnt = st->count, step = gridDim.x * kScaleT, i0 = blockIdx.x * kScaleT + threadIdx.x;
-    float g = 0.f, c = 0.f;
+    const int lane = threadIdx.x & 63;
+    float c = 0.f;
+    int most = kNone;
+    auto take = [&](float g, int more) {
+        if (g != 0.f && __builtin_isfinite(g)) most = max(most, exp_above(fabsf(g)) + more);
+    };
+    if (f.h) {
+        const int sub = lane & (f.L - 1), R = 64 / f.L;
+        for (int n = i0 / 64 * R + lane / f.L; n < cnt; n += step / 64 * R) {
+            const f16* row = f.h + (f.rows ? f.rows[n] : n) * f.ld;
+            float m = 0.f;
+            for (int d = sub * 8; d < f.D; d += f.L * 8) {
+                f16 x[8];
+                load_vec<f16, 8>(row, d, f.D, x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_abs((float)x[e]));
+            }
+            for (int o = 1; o < f.L; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+            if (m > 0.f) take(upstream(u, n, cnt), exp_above(m));
+        }
+    } else {
 #pragma unroll 4
-    for (int n = i0; n < cnt; n += step) g = fmaxf(g, finite_abs(upstream(u, n, cnt)));
+        for (int n = i0; n < cnt; n += step) take(upstream(u, n, cnt), 0);
+    }
     if (centers)
 #pragma unroll 4
         for (int v = i0; v < V; v += step) c = fmaxf(c, finite_abs(centers[v]));
-    g = wave_max(g);
     c = wave_max(c);
-    if ((threadIdx.x & 63) == 0) {
-        red[threadIdx.x >> 6][0] = g;
-        red[threadIdx.x >> 6][1] = c;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+    if (lane == 0) {
+        red[threadIdx.x >> 6] = c;
+        top[threadIdx.x >> 6] = most;
     }
     __syncthreads();
     if (threadIdx.x != 0) return;
     for (int i = 1; i < kScaleT / 64; ++i) {
-        g = fmaxf(g, red[i][0]);
-        c = fmaxf(c, red[i][1]);
+        c = fmaxf(c, red[i]);
+        most = max(most, top[i]);
     }
     if (gridDim.x == 1) {
-        bs->gmax = __builtin_bit_cast(unsigned, g);
+        bs->most = most;
         bs->cmax = __builtin_bit_cast(unsigned, c);
     } else {
-        if (g > 0.f) atomicMax(&bs->gmax, __builtin_bit_cast(unsigned, g));
+        if (most > kNone) atomicMax(&bs->most, most);
         if (c > 0.f) atomicMax(&bs->cmax, __builtin_bit_cast(unsigned, c));
+    }
+}
+
+// The features of kept rows times 2^weight_exp, for dW (whose other operand holds every row of dl at full size): float32's
+// planes as they are scaled already; float16 to 2^14, where its rows reach at most.  Eight elements a thread.
+template <int SPLIT>
+__global__ __launch_bounds__(256) void fold_rows_kernel(Operand H, const HeadState* __restrict__ st, Upstream u,
+                                                        const BackState* __restrict__ bs, f16* __restrict__ y, int Dp,
+                                                        long long lo) {
+    const int cnt = st->count, q = Dp / 8;
+    const long long all = (long long)cnt * q;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
+        const int n = (int)(i / q), d = (int)(i - (long long)n * q) * 8;
+        const float g = upstream(u, n, cnt);
+        const bool weighs = g != 0.f && __builtin_isfinite(g) && bs->most != kNone;
+        const int e = weighs ? weight_exp(bs, g) + (SPLIT == 3 ? 0 : 14) : 0;
+#pragma unroll
+        for (int p = 0; p < (SPLIT == 3 ? 2 : 1); ++p) {
+            f16x8 x = *reinterpret_cast<const f16x8*>(static_cast<const f16*>(H.p) + n * H.ld + d + p * H.lo);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = (f16)ldexpf((float)x[k], e);
+            *reinterpret_cast<f16x8*>(y + n * (long long)Dp + d + p * lo) = x;
+        }
     }
 }
 
@@ -620,7 +687,7 @@ struct DlArgs {
 template <class T, class S, int SPLIT, int MODE>
 __device__ __forceinline__ void dl_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int cnt, const HeadState* st,
                                            const BackState* bs, const DlArgs& a) {
-    const int shift = SPLIT == 3 ? logit_shift(st) : 0, ue = up_exp<T>(bs, a.up, MODE, cnt);
+    const int shift = SPLIT == 3 ? logit_shift(st) : 0;
     const float cs = MODE == kExpect && !std::is_same<T, bf16>::value ? ldexpf(1.f, -center_exp(bs)) : 1.f;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / S::WN, wn = wave % S::WN, c0 = m0 + wm * S::FM * 16 + (lane >> 4) * 4;
@@ -631,7 +698,8 @@ __device__ __forceinline__ void dl_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, i
         const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
         if (n >= cnt) continue;
         const float tp = a.top[n], rs = a.inv_sum[n];
-        float g = ldexpf(upstream(a.up, n, cnt), ue);
+        float g = upstream(a.up, n, cnt);
+        if (!std::is_same<T, bf16>::value) g = ldexpf(g, kDlTop - row_exp<T>(g));
         if (MODE == kCE) {
             const int t = a.tgt[n] - a.v0 - c0;
             if (a.tgt[n] < 0) g = __builtin_nanf("");
@@ -732,13 +800,14 @@ struct GradArgs {
     float* part;
     long long part_split;
     Upstream up;
+    int folded;                  // dW: exponent that fold_rows_kernel gave the features
 };
 // which: 0 = dH, 1 = dW.  Writes the tile of row / class n and features m.
 template <class T, class S, int SPLIT, class O, bool ACC, int WHICH>
 __device__ __forceinline__ void grad_of_tile(const f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int sp, int bound,
                                              const HeadState* st, const BackState* bs, const GradArgs& a) {
-    const int back = -dl_exp<T>(bs, a.up, a.mode, st->count) -
-                     (SPLIT == 3 ? shift_for(from_bits(WHICH == 0 ? st->amax_w : st->amax_h)) : 0);
+    const int cnt = st->count, inputs = SPLIT == 3 ? shift_for(from_bits(WHICH == 0 ? st->amax_w : st->amax_h)) : 0;
+    const int all = (WHICH == 0 ? dl_exp<T>(bs, a.mode) : dw_exp<T>(bs, a.up, a.mode, cnt) - a.folded) - inputs;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / S::WN, wn = wave % S::WN, Dp = (a.D + 3) & ~3;
 #pragma unroll
@@ -746,6 +815,7 @@ __device__ __forceinline__ void grad_of_tile(const f32x4 (&acc)[S::FM][S::FN], i
         const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
         if (n >= bound) continue;
         const long long row = !ACC && WHICH == 0 && a.rows ? a.rows[n] : n;
+        const int back = !ACC && WHICH == 0 ? all + row_exp<T>(upstream(a.up, n, cnt)) : all;
         if (ACC) {
 #pragma unroll
             for (int i = 0; i < S::FM; ++i) {
@@ -820,13 +890,13 @@ constexpr long long kShareOuts = 1 << 17;
 template <class T, int SPLIT, class O, int PAR>
 __global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__ part, long long part_split, int splits,
                                                        const HeadState* __restrict__ st, const BackState* __restrict__ bs, int n,
-                                                       int D, int mode, int which, Upstream up, const int* __restrict__ rows,
-                                                       O* __restrict__ out) {
+                                                       int D, int mode, int which, Upstream up, int folded,
+                                                       const int* __restrict__ rows, O* __restrict__ out) {
     constexpr int kOuts = 256 / PAR;
     __shared__ f32x4 red[PAR][kOuts + 1];
     const int cnt = which == 0 ? st->count : n, Dp = (D + 3) & ~3, q = Dp / 4;
-    const int back = -dl_exp<T>(bs, up, mode, st->count) -
-                     (SPLIT == 3 ? shift_for(from_bits(which == 0 ? st->amax_w : st->amax_h)) : 0);
+    const int inputs = SPLIT == 3 ? shift_for(from_bits(which == 0 ? st->amax_w : st->amax_h)) : 0;
+    const int same = (which == 0 ? dl_exp<T>(bs, mode) : dw_exp<T>(bs, up, mode, st->count) - folded) - inputs;
     const long long all = (long long)cnt * q;
     const int x = threadIdx.x % kOuts, y = threadIdx.x / kOuts, per = (splits + PAR - 1) / PAR;
     for (long long i0 = (long long)blockIdx.x * kOuts; i0 < all; i0 += (long long)gridDim.x * kOuts) {
@@ -849,7 +919,7 @@ __global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__
         if (i < all && y == 0) {
             const long long r = i / q;
             const int d = (int)(i - r * q) * 4;
-            a = scaled(a, back);
+            a = scaled(a, which == 0 ? same + row_exp<T>(upstream(up, (int)r, cnt)) : same);
             const float v[4] = {a[0], a[1], a[2], a[3]};
             put_row4(out + (rows && which == 0 ? (long long)rows[r] : r) * D, d, D, v);
         }
@@ -1101,8 +1171,8 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
     SlimRows<P, ND> next;
     if (b < blocks) next.load(a, b * 16 + (lane & 15), cnt, lane);
     slim_load_w<P, ND>(a, lds);
-    const int shift = P == 2 ? logit_shift(a.st) : 0, ue = up_exp<T>(o.bs, o.up, MODE, cnt);
-    const int back = -dl_exp<T>(o.bs, o.up, MODE, cnt) - (P == 2 ? shift_for(from_bits(a.st->amax_w)) : 0);
+    const int shift = P == 2 ? logit_shift(a.st) : 0;
+    const int same = dl_exp<T>(o.bs, MODE) - (P == 2 ? shift_for(from_bits(a.st->amax_w)) : 0);
     const float cs = MODE == kExpect && !std::is_same<T, bf16>::value ? ldexpf(1.f, -center_exp(o.bs)) : 1.f;
     const int base = lds_chunk<kK, 16>(lane & 15, lane >> 4), frags = a.Vp / 16, q4 = (lane >> 4) * 4;
     const float* centers = reinterpret_cast<const float*>(lds + P * a.Vp * ND * 64);
@@ -1117,7 +1187,9 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
         if (b + step < blocks) next.load(a, (b + step) * 16 + (lane & 15), cnt, lane);
         const float tp = a.top[m], rs = a.inv_sum[m], e0 = MODE == kExpect ? a.mean[m] * cs : 0.f;
         const int target = MODE == kCE ? a.tgt[m] : -1, t = target - q4;
-        float g = ldexpf(upstream(o.up, m, cnt), ue);
+        float g = upstream(o.up, m, cnt);
+        const int ge = row_exp<T>(g), we = !std::is_same<T, bf16>::value && o.up.each ? weight_exp(o.bs, g) : 0;
+        g = ldexpf(g, std::is_same<T, bf16>::value ? 0 : kDlTop - ge);
         if (MODE == kCE && target < 0) g = __builtin_nanf("");
         const float gr = g * rs;
         f32x4 acc[2 * ND];
@@ -1145,7 +1217,8 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
                         if (v + e >= a.V) d[u][e] = 0.f;
                 }
                 if (dl && n < cnt && v < o.ld) {
-                    const float y[4] = {d[u][0], d[u][1], d[u][2], d[u][3]};
+                    const f32x4 w = std::is_same<T, bf16>::value ? d[u] : scaled(d[u], we);      // weighted for dW
+                    const float y[4] = {w[0], w[1], w[2], w[3]};
                     put4<P == 2 ? 3 : 1>(dl + (long long)n * o.ld + v, o.lo, y);
                 }
             }
@@ -1188,7 +1261,7 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
 #pragma unroll
                 for (int i = 0; i < 2 * ND; ++i) {
                     const int c = i * 16 + (lane >> 4) * 4;
-                    const f32x4 x = scaled(acc[i], back);
+                    const f32x4 x = scaled(acc[i], same + ge);
                     const float y[4] = {x[0], x[1], x[2], x[3]};
                     if (c < a.D) put_row4(row, c, a.D, y);
                 }
@@ -1400,7 +1473,7 @@ struct Plan {
     bool slim_back, pack;
     size_t sh, sw, saved_total;                                            // staged operands behind Saved (not of few rows)
     size_t counts, tlogit, part, sums, fwd_total;                          // offsets of the forward's workspace
-    size_t bh, bw, bs, dl, dhp, dwp, bwd_total;                            // offsets of the backward's
+    size_t bh, bw, bs, hw, dl, dhp, dwp, bwd_total;                            // offsets of the backward's
 };
 
 int splits_for(long long tiles, long long steps) {
@@ -1473,6 +1546,7 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     p.bh = o; o += (p.stage_h && p.few) || p.pack ? h : 0;
     p.bw = o; o += p.few ? w : 0;
     p.bs = o; o += 256;
+    p.hw = o; o += dtype == DS_BF16 || p.slim_back ? 0 : h;      // weighted rows for dW
     p.dl = o; o += align256((size_t)N * p.piece_ld * el);
     p.dhp = o; o += p.dh_part ? align256((size_t)p.dh_splits * N * D4 * 4) : 0;
     p.dwp = o; o += p.dw_splits > 1 ? align256((size_t)p.dw_splits * p.piece * D4 * 4) : 0;
@@ -1722,11 +1796,15 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
     const int* rows = mode == kCE ? s.rows : nullptr;
     BackState* bs = reinterpret_cast<BackState*>(ws + p.bs);
     Upstream up{g, reduction == DS_REDUCE_NONE, reduction == DS_REDUCE_MEAN, rows};
-    if (!std::is_same<T, bf16>::value && up.each) {    // where up_exp reads it
-        const long long most = centers && V > N ? V : N;
+    const bool weigh = !std::is_same<T, bf16>::value && up.each, fold = weigh && g_weight && !p.slim_back;
+    if (weigh) {
+        Features f{};
+        if constexpr (std::is_same<IT, f16>::value)
+            if (fold) f = Features{hidden, ldh, rows, D, lanes_for(cdiv(D, 8))};
+        const long long most = std::max<long long>(centers ? V : 0, f.h ? N * f.L : N);      // threads
         const int blocks = most <= kScaleAlone ? 1 : cdiv(most, 4 * kScaleT) < 256 ? cdiv(most, 4 * kScaleT) : 256;
         if (blocks > 1) back_init_kernel<<<1, 1, 0, q>>>(bs);
-        back_scale_kernel<<<blocks, kScaleT, 0, q>>>(up, s.st, centers, V, bs);
+        back_scale_kernel<<<blocks, kScaleT, 0, q>>>(up, s.st, centers, V, f, bs);
     }
     // the forward of few rows stages nothing and leaves zero scales; the maximum that a second backward of the same forward,
     // maybe at the same time, finds there is the one that it forms itself
@@ -1743,6 +1821,15 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
             zero_ignored_kernel<IT><<<blocks < 4096 ? blocks : 4096, 256, 0, q>>>(ignored, D, s.st, g_hidden);
         }
     }
+    Operand Hw = H;      // dW's features
+    if constexpr (std::is_same<T, f16>::value)
+        if (fold) {
+            Hw = Operand{ws + p.hw, p.Dp, N * p.Dp, (int)N, p.Dp};
+            const int blocks = cdiv(N * p.Dp, 8 * 256 * 2);
+            fold_rows_kernel<SPLIT><<<blocks < 4096 ? blocks : 4096, 256, 0, q>>>(H, s.st, up, bs, reinterpret_cast<f16*>(ws + p.hw),
+                                                                                  p.Dp, N * p.Dp);
+        }
+    const int folded = fold && SPLIT != 3 ? 14 : 0;
     T* dl = reinterpret_cast<T*>(ws + p.dl);
     float* dhp = reinterpret_cast<float*>(ws + p.dhp);
     float* dwp = reinterpret_cast<float*>(ws + p.dwp);
@@ -1759,7 +1846,7 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
             const int rc = mode == kCE ? slim_bwd<T, SPLIT == 3 ? 2 : 1, kCE, IT>(p, a, o, q)
                                        : slim_bwd<T, SPLIT == 3 ? 2 : 1, kExpect, IT>(p, a, o, q);
             if (rc) return rc;
-            if (p.pack) H = Operand{ws + p.bh, p.Dp, 0, (int)N, p.Dp};
+            if (p.pack) Hw = Operand{ws + p.bh, p.Dp, 0, (int)N, p.Dp};
         } else {
             const DlArgs da{v0, cols, s.tgt, centers, s.top, s.inv_sum, s.mean, up, dl, ld, lo};
             if (mode == kCE)
@@ -1769,29 +1856,29 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
         }
         const Operand G{dl, ld, lo, (int)N, ld};
         if (g_hidden && !p.slim_back) {
-            const GradArgs ga{D, cols, p.dh_splits, mode, cols, v0 == 0, rows, g_hidden, dhp, N * D4, up};
+            const GradArgs ga{D, cols, p.dh_splits, mode, cols, v0 == 0, rows, g_hidden, dhp, N * D4, up, 0};
             grad_launch<IT, T, SPLIT, 0>(p.dh, p.dh_part, Wp, G, s, bs, N, ga, q);
         }
         if (g_weight) {
             IT* gw = g_weight + (long long)v0 * D;
-            const GradArgs ga{D, cols, p.dw_splits, mode, cols, 1, nullptr, gw, dwp, (long long)p.piece * D4, up};
-            grad_launch<IT, T, SPLIT, 1>(p.dw, p.dw_splits > 1, H, G, s, bs, cols, ga, q);
+            const GradArgs ga{D, cols, p.dw_splits, mode, cols, 1, nullptr, gw, dwp, (long long)p.piece * D4, up, folded};
+            grad_launch<IT, T, SPLIT, 1>(p.dw, p.dw_splits > 1, Hw, G, s, bs, cols, ga, q);
             if (p.dw_splits > 8 && (long long)cols * D4 <= kShareOuts)
                 head_sum_kernel<T, SPLIT, IT, 16><<<cdiv((long long)cols * D4 / 4, 16), 256, 0, q>>>(
-                    dwp, (long long)p.piece * D4, p.dw_splits, s.st, bs, cols, D, mode, 1, up, nullptr, gw);
+                    dwp, (long long)p.piece * D4, p.dw_splits, s.st, bs, cols, D, mode, 1, up, folded, nullptr, gw);
             else if (p.dw_splits > 1)
                 head_sum_kernel<T, SPLIT, IT, 1><<<cdiv((long long)cols * D4 / 4, 256), 256, 0, q>>>(
-                    dwp, (long long)p.piece * D4, p.dw_splits, s.st, bs, cols, D, mode, 1, up, nullptr, gw);
+                    dwp, (long long)p.piece * D4, p.dw_splits, s.st, bs, cols, D, mode, 1, up, folded, nullptr, gw);
         }
     }
     if (g_hidden && p.dh_part && !p.slim_back) {
         const bool many = p.dh_splits > 8 && N * D4 <= kShareOuts;
         const int blocks = cdiv(N * (D4 / 4), many ? 16 : 256), grid = blocks < 16384 ? blocks : 16384;
         if (many)
-            head_sum_kernel<T, SPLIT, IT, 16><<<grid, 256, 0, q>>>(dhp, N * D4, p.dh_splits, s.st, bs, (int)N, D, mode, 0, up, rows,
+            head_sum_kernel<T, SPLIT, IT, 16><<<grid, 256, 0, q>>>(dhp, N * D4, p.dh_splits, s.st, bs, (int)N, D, mode, 0, up, 0, rows,
                                                                    g_hidden);
         else
-            head_sum_kernel<T, SPLIT, IT, 1><<<grid, 256, 0, q>>>(dhp, N * D4, p.dh_splits, s.st, bs, (int)N, D, mode, 0, up, rows,
+            head_sum_kernel<T, SPLIT, IT, 1><<<grid, 256, 0, q>>>(dhp, N * D4, p.dh_splits, s.st, bs, (int)N, D, mode, 0, up, 0, rows,
                                                                   g_hidden);
     }
     return launched();

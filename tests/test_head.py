@@ -301,6 +301,69 @@ def test_large_logits_and_upstreams(dtype):
         _close(a[inside], b[inside], tol_[inside], "gradient")
 
 
+def _row_oracle(h, w, up, t=None, c=None):
+    """g_hidden and its tolerance row by row: a row's gradient is its upstream value times what it is for 1, and so is what it may be
+    off by, whatever the other rows' upstream"""
+    one = torch.ones_like(up)
+    _, gh, _, _, th, _ = _oracle(h, w, t=t, c=c, up=one)
+    sub = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -24, torch.bfloat16: 2.0 ** -133}[h.dtype]
+    s = up.double()[:, None]
+    return gh * s, th * s.abs() + sub
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,d,v", [(3, 40, 500), (60, 40, 50), (70, 33, 50), (200, 64, 900), (9000, 24, 40), (3000, 136, 1500),
+                                   (700, 131, 2500), (6000, 256, 700), (1500, 24, 200_001)])
+def test_a_row_keeps_its_gradient_beside_larger_ones(n, d, v, dtype):
+    """Upstream values that span 2^26 (float16: as far as its results reach), 2^80 and zero: every row's own digits, and dW's as
+    far as they follow from the largest."""
+    lo, hi = (-3.0, 4.5) if dtype == torch.float16 else (-20.0, 4.0)
+    h, w, t, up, c = _data(n, d, v, dtype, seed=n + d)
+    c = c / 80
+    g = torch.Generator().manual_seed(n)
+    up = up * (10.0 ** (lo + (hi - lo) * torch.rand(n, generator=g))).to(DEV)
+    up[n // 2] = 0
+    if n > 3:
+        t[1::7] = -100
+    if v > 100_000:          # pieces of the classes, and their sums: the oracle takes every 13th row
+        pick = torch.arange(0, n, 13, device=DEV)
+    else:
+        pick = torch.arange(n, device=DEV)
+    for ce in (True, False):
+        k = dict(t=t) if ce else dict(c=c)
+        got = _ce(h, w, t, "none", up) if ce else _ex(h, w, c, up)
+        gh, th = _row_oracle(h[pick], w, up[pick], t=t[pick] if ce else None, c=None if ce else c)
+        fits = gh.abs() < torch.finfo(dtype).max / 2
+        mine = got[1][pick]
+        _close(torch.where(fits, mine.double(), 0.0), torch.where(fits, gh, 0.0), th, "g_hidden")
+        big = (gh.abs() > th) & fits
+        assert not (mine == 0)[big].any()
+        if v <= 100_000:
+            _, _, gw, _, _, tw = _oracle(h, w, up=up, **k)
+            fits = gw.abs() < torch.finfo(dtype).max / 2
+            _close(got[2][fits], gw[fits], tw[fits], "g_weight")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,d,v", [(60, 40, 50), (200, 64, 900), (500, 131, 700)])
+def test_weighted_out_rows_leave_no_trace(n, d, v, dtype):
+    """Rows of large features and zero upstream (a caller's own mask): dW is that of the other rows, as exactly."""
+    h, w, t, up, c = _data(n, d, v, dtype, seed=n + v)
+    small = h * 2.0 ** -9
+    loud = small.clone()
+    loud[::5] = h[::5] * 2.0 ** 5
+    up[::5] = 0
+    quiet = small.clone()
+    quiet[::5] = 0
+    for a, b, want in ((_ce(loud, w, t, "none", up), _ce(quiet, w, t, "none", up), _oracle(quiet, w, t=t, up=up)),
+                       (_ex(loud, w, c, up), _ex(quiet, w, c, up), _oracle(quiet, w, c=c, up=up))):
+        _close(a[2], want[2], want[5], "g_weight")
+        _close(b[2], want[2], want[5], "g_weight")
+        assert not a[1][::5].any()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_confident_rows(dtype):
