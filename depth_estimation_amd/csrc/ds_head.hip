@@ -28,20 +28,23 @@ template <int SPLIT>
 constexpr int kP = SPLIT == 3 ? 2 : 1;
 
 enum Mode { kCE = 0, kExpect = 1 };
+constexpr int kNone = -(1 << 30);   // no exponent
 
 // What the forward leaves for the backward besides the softmax statistics: opaque to the caller.
+constexpr int kReach = 16;          // places where workgroups meet, each in a cache line of its own
 struct HeadState {
-    int count;           // rows kept
-    unsigned amax_h;     // bits of max |hidden| over kept rows, max |weight|: the scales of the fp16 planes (fp32 inputs)
-    unsigned amax_w;
-    int pad[13];
+    int count;                      // rows kept
+    unsigned amax_w;                // bits of max |weight|: the scale of its fp16 planes (fp32 inputs)
+    int pad[30];
+    struct {
+        int most, pad[31];          // max over staged rows of the exponent above their largest feature (cross entropy)
+    } reach[kReach];
 };
 struct BackState {
-    int most;            // the largest exponent a kept row takes part in dW with (kNone: no row does)
+    int most;            // the largest exponent that a kept row takes part in dW with (kNone: no row does)
     unsigned cmax;       // bits of max |centre|
     int pad[14];
 };
-constexpr int kNone = -(1 << 30);
 
 
 __device__ __forceinline__ float from_bits(unsigned u) { return __builtin_bit_cast(float, u); }
@@ -62,7 +65,6 @@ constexpr int kListT = 1024, kListPer = 16, kListBlock = kListT * kListPer;
 
 __global__ void head_init_kernel(HeadState* st, int rows) {
     st->count = rows;
-    st->amax_h = 0;
     st->amax_w = 0;
 }
 
@@ -165,9 +167,9 @@ __global__ __launch_bounds__(kListT) void list_rows_kernel(const long long* __re
     }
     if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
         st->count = before + s[kListPer * kW];
-        st->amax_h = 0;
         st->amax_w = 0;
     }
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x < kReach) st->reach[threadIdx.x].most = kNone;
 }
 static_assert(kListPer * kListT / 64 == 256, "the prefix handles four counts a lane");
 
@@ -198,29 +200,21 @@ __device__ __forceinline__ void load_vec(const IT* row, int d, int D, IT (&x)[VE
     }
 }
 
-// max |x| over the rows of two matrices (one launch): the first one's kept rows, listed in `rows` if given, all of the second's;
-// order-independent, so repeatable.  A workgroup each (alone) writes what it finds, and the row count if set_count gives it;
-// else *st was cleared before.
+// max |weight|; order-independent, so repeatable.  One workgroup writes what it finds, and the row count if set_count gives it;
+// where there are more, *st was cleared before.
 template <class IT, int VEC>
-__global__ __launch_bounds__(256) void amax_kernel(const IT* __restrict__ x, long long ld, const int* __restrict__ rows,
-                                                   HeadState* __restrict__ st, const IT* __restrict__ w, int V, int D, int L,
-                                                   int blocks_x, int set_count) {
-    const bool second = (int)blockIdx.x >= blocks_x, alone = gridDim.x == 2;
-    const int c = second ? V : set_count ? set_count : st->count, b = second ? blockIdx.x - blocks_x : blockIdx.x;
-    const int nb = second ? gridDim.x - blocks_x : blocks_x;
-    const IT* src = second ? w : x;
-    const long long pitch = second ? D : ld;
+__global__ __launch_bounds__(256) void amax_kernel(const IT* __restrict__ w, HeadState* __restrict__ st, int V, int D, int L,
+                                                   int set_count) {
+    const bool alone = gridDim.x == 1;
     const int lane = threadIdx.x & 63, sub = lane & (L - 1), R = 64 / L;
     float m = 0.f;
     constexpr int U = 4;        // rows under way at a time
-    for (int r0 = (b * 4 + (threadIdx.x >> 6)) * R + lane / L; r0 < c; r0 += nb * 4 * R * U)
+    const int hop = gridDim.x * 4 * R;
+    for (int r0 = ((int)blockIdx.x * 4 + (threadIdx.x >> 6)) * R + lane / L; r0 < V; r0 += hop * U)
         for (int d = sub * VEC; d < D; d += L * VEC) {
             IT v[U][VEC];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int r = min(r0 + u * nb * 4 * R, c - 1);
-                load_vec<IT, VEC>(src + (rows && !second ? rows[r] : r) * pitch, d, D, v[u]);
-            }
+            for (int u = 0; u < U; ++u) load_vec<IT, VEC>(w + (long long)min(r0 + u * hop, V - 1) * D, d, D, v[u]);
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -233,25 +227,29 @@ __global__ __launch_bounds__(256) void amax_kernel(const IT* __restrict__ x, lon
     // one atomic a workgroup: they all meet in one place, 20 ns each
     if (threadIdx.x == 0) {
         m = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-        if (alone) (second ? st->amax_w : st->amax_h) = __builtin_bit_cast(unsigned, m);
-        if (alone && set_count && !second) st->count = set_count;
-        if (!alone && m > 0.f) atomicMax(second ? &st->amax_w : &st->amax_h, __builtin_bit_cast(unsigned, m));
+        if (alone) st->amax_w = __builtin_bit_cast(unsigned, m);
+        if (alone && set_count) st->count = set_count;
+        if (!alone && m > 0.f) atomicMax(&st->amax_w, __builtin_bit_cast(unsigned, m));
     }
 }
 
 // Rows of one or two matrices (one launch) packed with a row pitch of Dp elements, zero behind D; fp32 as two scaled fp16
-// planes.  Workgroups [first, first + blocks) take a source.
+// planes: the weight under one scale (dH sums over its rows), every row of the features under its own, so that a row's result
+// does not depend on what else is in the batch.  Workgroups [first, first + blocks) take a source.
 struct Source {
     const void* x;
     long long ld;
     const int* rows;           // listed rows (NULL: in order)
     const int* cnt;            // how many, on the device (NULL: n)
     int n;
-    const unsigned* amax;
+    const unsigned* amax;      // scale of all rows (fp32), or
+    int* shifts;               // every row's own, left here: 2^shift brings its largest element into [2^14, 2^15)
+    HeadState* reach;          // NULL: not asked for
     void* y;
     long long lo;
     int first, blocks;         // blocks 0: not there
 };
+constexpr int kZeroShift = 163;    // of a row without finite elements but zeros: it reaches nowhere
 template <class IT, class T, int SPLIT, int VEC>
 __global__ __launch_bounds__(256) void stage_kernel(Source s0, Source s1, int D, int Dp, int L) {
     const bool second = s1.blocks > 0 && (int)blockIdx.x >= s1.first;
@@ -259,17 +257,44 @@ __global__ __launch_bounds__(256) void stage_kernel(Source s0, Source s1, int D,
     const IT* x = static_cast<const IT*>(s.x);
     const int c = s.cnt ? *s.cnt : s.n;
     const int lane = threadIdx.x & 63, sub = lane & (L - 1), R = 64 / L;
-    const int shift = SPLIT == 3 ? shift_for(from_bits(*s.amax)) : 0;
     constexpr int U = 4;
+    constexpr bool kShifts = !std::is_same<T, bf16>::value;      // (fp16 rows are left as they are, but dW wants to know)
+    int shift[U], reach = kNone;
+#pragma unroll
+    for (int u = 0; u < U; ++u) shift[u] = SPLIT == 3 && s.amax ? shift_for(from_bits(*s.amax)) : 0;
     const int hop = s.blocks * 4 * R;
-    for (int r0 = (((int)blockIdx.x - s.first) * 4 + (threadIdx.x >> 6)) * R + lane / L; r0 < c; r0 += hop * U)
-        for (int d = sub * VEC; d < Dp; d += L * VEC) {
-            IT v[U][VEC];
+    for (int r0 = (((int)blockIdx.x - s.first) * 4 + (threadIdx.x >> 6)) * R + lane / L; r0 < c; r0 += hop * U) {
+        IT v[U][VEC];
+        auto load = [&](int d) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int r = min(r0 + u * hop, c - 1);
                 load_vec<IT, VEC>(x + (s.rows ? s.rows[r] : r) * s.ld, d, D, v[u]);
             }
+        };
+        const bool kept = kShifts && s.shifts && Dp <= L * VEC;      // one load brings the whole row
+        if (kShifts && s.shifts) {
+            float m[U] = {};
+            for (int d = sub * VEC; d < Dp; d += L * VEC) {
+                load(d);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) m[u] = fmaxf(m[u], finite_abs((float)v[u][e]));
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                for (int o = 1; o < L; o <<= 1) m[u] = fmaxf(m[u], __shfl_xor(m[u], o, 64));
+                const int own = m[u] > 0.f ? shift_for(m[u]) : kZeroShift;
+                if (SPLIT == 3) shift[u] = own;
+                if (sub == 0 && r0 + u * hop < c) {
+                    s.shifts[r0 + u * hop] = own;
+                    reach = max(reach, 15 - own);
+                }
+            }
+        }
+        for (int d = sub * VEC; d < Dp; d += L * VEC) {
+            if (!kept) load(d);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int r = r0 + u * hop;
@@ -280,7 +305,7 @@ __global__ __launch_bounds__(256) void stage_kernel(Source s0, Source s1, int D,
                 for (int e = 0; e < VEC; ++e) {
                     if constexpr (SPLIT == 3) {
                         f16 a, b;
-                        split16(ldexpf((float)v[u][e], shift), a, b);
+                        split16(ldexpf((float)v[u][e], shift[u]), a, b);
                         h[e] = a;
                         l[e] = b;
                     } else {
@@ -291,12 +316,20 @@ __global__ __launch_bounds__(256) void stage_kernel(Source s0, Source s1, int D,
                 if (SPLIT == 3) *reinterpret_cast<typename Vec<T, VEC>::type*>(q + s.lo) = l;
             }
         }
+    }
+    if (SPLIT == 3 && s.reach) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) reach = max(reach, __shfl_xor(reach, o, 64));
+        __shared__ int top[4];
+        if (lane == 0) top[threadIdx.x >> 6] = reach;
+        __syncthreads();
+        reach = max(max(top[0], top[1]), max(top[2], top[3]));
+        if (threadIdx.x == 0 && reach > kNone) atomicMax(&s.reach->reach[blockIdx.x % kReach].most, reach);
+    }
 }
 
-// exponent of accumulated products of planes -> logits
-__device__ __forceinline__ int logit_shift(const HeadState* st) {
-    return -shift_for(from_bits(st->amax_h)) - shift_for(from_bits(st->amax_w));
-}
+// exponent of the weight's planes
+__device__ __forceinline__ int weight_shift(const HeadState* st) { return shift_for(from_bits(st->amax_w)); }
 
 // ------------------------------------------------------------------------------------------------------------ forward
 // Statistics of one tile of l^T: classes along m, rows along n, so that a lane holds 4 FM classes of FN rows and most of the
@@ -304,6 +337,7 @@ __device__ __forceinline__ int logit_shift(const HeadState* st) {
 // and on return.
 struct StatsArgs {
     int V;
+    const int* shifts;   // exponents of the rows' planes
     const int* tgt;
     const float* centers;
     float* tlogit;
@@ -321,17 +355,16 @@ __device__ __forceinline__ void stats_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0
                                               const StatsArgs& a, float* red) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / S::WN, wn = wave % S::WN, v0 = m0 + wm * S::FM * 16 + (lane >> 4) * 4;
-    if (SPLIT == 3) {
-        const int shift = logit_shift(st);
-#pragma unroll
-        for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-            for (int j = 0; j < S::FN; ++j) acc[i][j] = scaled(acc[i][j], shift);
-    }
+    const int ws = SPLIT == 3 ? weight_shift(st) : 0;
     const bool edge = m0 + S::BM > a.V;      // only the last class tile has classes that do not exist
 #pragma unroll
     for (int j = 0; j < S::FN; ++j) {
         const int nl = (wn * S::FN + j) * 16 + (lane & 15), n = n0 + nl;
+        if (SPLIT == 3) {
+            const int shift = -ws - (n < cnt ? a.shifts[n] : 0);
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i) acc[i][j] = scaled(acc[i][j], shift);
+        }
         if (edge) {
 #pragma unroll
             for (int i = 0; i < S::FM; ++i)
@@ -567,26 +600,42 @@ template <class T>
 __device__ __forceinline__ int dl_exp(const BackState* bs, int mode) {
     return std::is_same<T, bf16>::value ? 0 : (mode == kExpect ? center_exp(bs) : 0) - kDlTop;
 }
-// exponent of a row's weight in dW, at most 0: rows without a gradient weigh nothing either way, and are left as they are
-__device__ __forceinline__ int weight_exp(const BackState* bs, float g) {
-    return g != 0.f && __builtin_isfinite(g) ? exp_above(fabsf(g)) - bs->most : 0;
+// What a row weighs in dW.  A product there is dl_r h_r; dl is stored under the row's upstream exponent e, features of fp32
+// under the row's own shift, so that a row takes part with 2^(e + 15 - shift), and that is brought to 2^most by the weight, at
+// most 1 (most: the largest of the sums e + 15 - shift, or of e where features have one size for all, `reach` false).  Rows
+// without a gradient are left as they are.
+__device__ __forceinline__ int weight_exp(float g, int reach, int most) {
+    return g != 0.f && __builtin_isfinite(g) && most > kNone ? exp_above(fabsf(g)) + reach - most : 0;
 }
-// exponent of sums over rows -> dW, beside the inputs' own
-template <class T>
-__device__ __forceinline__ int dw_exp(const BackState* bs, const Upstream& u, int mode, int cnt) {
+// the largest exponent that a row takes part with.  SPLIT 3: always with its features' reach
+template <class T, int SPLIT>
+__device__ __forceinline__ int most_of(const HeadState* st, const BackState* bs, const Upstream& u, int cnt) {
     if (std::is_same<T, bf16>::value) return 0;
-    return dl_exp<T>(bs, mode) + (u.each ? bs->most == kNone ? 0 : bs->most : row_exp<T>(upstream(u, 0, cnt)));
+    if (u.each) return bs->most;
+    int r = SPLIT == 3 ? kNone : 0;
+    if (SPLIT == 3)
+        for (int i = 0; i < kReach; ++i) r = max(r, st->reach[i].most);
+    return r == kNone ? kNone : r + row_exp<T>(upstream(u, 0, cnt));
+}
+constexpr int kReachTop = 15;      // features that take part with 2^most are below 2^15 as stored, or as weighted
+// exponent of sums over rows -> dW
+template <class T, int SPLIT>
+__device__ __forceinline__ int dw_exp(const HeadState* st, const BackState* bs, const Upstream& u, int mode, int cnt, bool reach) {
+    if (std::is_same<T, bf16>::value) return 0;
+    const int most = most_of<T, SPLIT>(st, bs, u, cnt);
+    return dl_exp<T>(bs, mode) + (most == kNone ? 0 : most) - (reach ? kReachTop : 0);
 }
 
-// bs->most (with `h`, the features of float16 rows that fold_rows_kernel will weigh: as far as they reach, too) and the largest
-// |centre|, for upstreams that differ; *bs set by back_init_kernel before, unless one workgroup does it all (a launch less)
+// bs->most (with the rows' shifts, or of float16 rows that lie as the caller left them the features themselves, where rows weigh
+// with their reach) and the largest |centre|, for upstreams that differ; *bs set by back_init_kernel before, unless one workgroup does it all (a launch less)
 constexpr int kScaleT = 512, kScaleAlone = 16 * kScaleT;
 __global__ void back_init_kernel(BackState* bs) {
     bs->most = kNone;
     bs->cmax = 0;
 }
 struct Features {
-    const f16* h;        // NULL: not asked for
+    const int* shifts;   // of staged rows
+    const f16* h;        // both NULL: not asked for
     long long ld;
     const int* rows;     // listed rows (NULL: in order)
     int D, L;
@@ -619,7 +668,7 @@ __global__ __launch_bounds__(kScaleT) void back_scale_kernel(Upstream u, const H
         }
     } else {
 #pragma unroll 4
-        for (int n = i0; n < cnt; n += step) take(upstream(u, n, cnt), 0);
+        for (int n = i0; n < cnt; n += step) take(upstream(u, n, cnt), f.shifts ? kReachTop - f.shifts[n] : 0);
     }
     if (centers)
 #pragma unroll 4
@@ -646,19 +695,18 @@ __global__ __launch_bounds__(kScaleT) void back_scale_kernel(Upstream u, const H
     }
 }
 
-// The features of kept rows times 2^weight_exp, for dW (whose other operand holds every row of dl at full size): float32's
-// planes as they are scaled already; float16 to 2^14, where its rows reach at most.  Eight elements a thread.
+// The features of kept rows times 2^weight_exp, for dW, whose other operand holds every row of dl at full size (float16: from
+// their own size to that of fp32's planes).  Eight elements a thread.
 template <int SPLIT>
-__global__ __launch_bounds__(256) void fold_rows_kernel(Operand H, const HeadState* __restrict__ st, Upstream u,
+__global__ __launch_bounds__(256) void fold_rows_kernel(Operand H, const int* __restrict__ shifts,
+                                                        const HeadState* __restrict__ st, Upstream u,
                                                         const BackState* __restrict__ bs, f16* __restrict__ y, int Dp,
                                                         long long lo) {
-    const int cnt = st->count, q = Dp / 8;
+    const int cnt = st->count, q = Dp / 8, most = most_of<f16, SPLIT>(st, bs, u, cnt);
     const long long all = (long long)cnt * q;
     for (long long i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
         const int n = (int)(i / q), d = (int)(i - (long long)n * q) * 8;
-        const float g = upstream(u, n, cnt);
-        const bool weighs = g != 0.f && __builtin_isfinite(g) && bs->most != kNone;
-        const int e = weighs ? weight_exp(bs, g) + (SPLIT == 3 ? 0 : 14) : 0;
+        const int e = weight_exp(upstream(u, n, cnt), kReachTop - (SPLIT == 3 ? shifts[n] : 0), most);
 #pragma unroll
         for (int p = 0; p < (SPLIT == 3 ? 2 : 1); ++p) {
             f16x8 x = *reinterpret_cast<const f16x8*>(static_cast<const f16*>(H.p) + n * H.ld + d + p * H.lo);
@@ -674,6 +722,7 @@ __global__ __launch_bounds__(256) void fold_rows_kernel(Operand H, const HeadSta
 // with the two planes of fp32 inputs; p - 1 and c - E are formed in fp32 before it.
 struct DlArgs {
     int v0, cols;
+    const int* shifts;
     const int* tgt;
     const float* centers;
     const float* top;
@@ -687,7 +736,7 @@ struct DlArgs {
 template <class T, class S, int SPLIT, int MODE>
 __device__ __forceinline__ void dl_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int cnt, const HeadState* st,
                                            const BackState* bs, const DlArgs& a) {
-    const int shift = SPLIT == 3 ? logit_shift(st) : 0;
+    const int ws = SPLIT == 3 ? weight_shift(st) : 0;
     const float cs = MODE == kExpect && !std::is_same<T, bf16>::value ? ldexpf(1.f, -center_exp(bs)) : 1.f;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / S::WN, wn = wave % S::WN, c0 = m0 + wm * S::FM * 16 + (lane >> 4) * 4;
@@ -698,6 +747,7 @@ __device__ __forceinline__ void dl_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, i
         const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
         if (n >= cnt) continue;
         const float tp = a.top[n], rs = a.inv_sum[n];
+        const int shift = SPLIT == 3 ? -ws - a.shifts[n] : 0;
         float g = upstream(a.up, n, cnt);
         if (!std::is_same<T, bf16>::value) g = ldexpf(g, kDlTop - row_exp<T>(g));
         if (MODE == kCE) {
@@ -800,14 +850,15 @@ struct GradArgs {
     float* part;
     long long part_split;
     Upstream up;
-    int folded;                  // dW: exponent that fold_rows_kernel gave the features
+    bool reach;                  // dW: rows weigh with their reach
 };
 // which: 0 = dH, 1 = dW.  Writes the tile of row / class n and features m.
 template <class T, class S, int SPLIT, class O, bool ACC, int WHICH>
 __device__ __forceinline__ void grad_of_tile(const f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int sp, int bound,
                                              const HeadState* st, const BackState* bs, const GradArgs& a) {
-    const int cnt = st->count, inputs = SPLIT == 3 ? shift_for(from_bits(WHICH == 0 ? st->amax_w : st->amax_h)) : 0;
-    const int all = (WHICH == 0 ? dl_exp<T>(bs, a.mode) : dw_exp<T>(bs, a.up, a.mode, cnt) - a.folded) - inputs;
+    const int cnt = st->count;
+    const int all = WHICH == 0 ? dl_exp<T>(bs, a.mode) - (SPLIT == 3 ? weight_shift(st) : 0)
+                               : dw_exp<T, SPLIT>(st, bs, a.up, a.mode, cnt, a.reach);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / S::WN, wn = wave % S::WN, Dp = (a.D + 3) & ~3;
 #pragma unroll
@@ -890,13 +941,13 @@ constexpr long long kShareOuts = 1 << 17;
 template <class T, int SPLIT, class O, int PAR>
 __global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__ part, long long part_split, int splits,
                                                        const HeadState* __restrict__ st, const BackState* __restrict__ bs, int n,
-                                                       int D, int mode, int which, Upstream up, int folded,
+                                                       int D, int mode, int which, Upstream up, bool reach,
                                                        const int* __restrict__ rows, O* __restrict__ out) {
     constexpr int kOuts = 256 / PAR;
     __shared__ f32x4 red[PAR][kOuts + 1];
     const int cnt = which == 0 ? st->count : n, Dp = (D + 3) & ~3, q = Dp / 4;
-    const int inputs = SPLIT == 3 ? shift_for(from_bits(which == 0 ? st->amax_w : st->amax_h)) : 0;
-    const int same = (which == 0 ? dl_exp<T>(bs, mode) : dw_exp<T>(bs, up, mode, st->count) - folded) - inputs;
+    const int same = which == 0 ? dl_exp<T>(bs, mode) - (SPLIT == 3 ? weight_shift(st) : 0)
+                                : dw_exp<T, SPLIT>(st, bs, up, mode, st->count, reach);
     const long long all = (long long)cnt * q;
     const int x = threadIdx.x % kOuts, y = threadIdx.x / kOuts, per = (splits + PAR - 1) / PAR;
     for (long long i0 = (long long)blockIdx.x * kOuts; i0 < all; i0 += (long long)gridDim.x * kOuts) {
@@ -980,6 +1031,7 @@ struct SlimArgs {
     int set_count;
     int n, D, V, Vp;           // Vp: V rounded up to 32
     Operand W;
+    const int* shifts;         // exponents of the rows' planes
     const int* tgt;
     const float* centers;
     float *top, *inv_sum, *mean;
@@ -1085,7 +1137,7 @@ __global__ __launch_bounds__(kSlimT) void slim_fwd_kernel(SlimArgs a, SlimFwd o)
     SlimRows<P, ND> next;
     if (b < blocks) next.load(a, b * 16 + (lane & 15), cnt, lane);
     slim_load_w<P, ND>(a, lds);
-    const int shift = P == 2 ? logit_shift(a.st) : 0;
+    const int ws = P == 2 ? weight_shift(a.st) : 0;
     const int base = lds_chunk<kK, 16>(lane & 15, lane >> 4), frags = a.Vp / 16, q4 = (lane >> 4) * 4;
     const float* centers = reinterpret_cast<const float*>(lds + P * a.Vp * ND * 64);
     double total = 0.0;
@@ -1094,6 +1146,7 @@ __global__ __launch_bounds__(kSlimT) void slim_fwd_kernel(SlimArgs a, SlimFwd o)
         const int n = b * 16 + (lane & 15);
         if (b + step < blocks) next.load(a, (b + step) * 16 + (lane & 15), cnt, lane);
         const int target = MODE == kCE ? a.tgt[n < cnt ? n : cnt - 1] : -1, t = target - q4;      // t: from the lane's first class
+        const int shift = P == 2 ? -ws - a.shifts[n < cnt ? n : cnt - 1] : 0;
         float mx = -INFINITY, s = 0.f, sc = 0.f, tl = 0.f;
         for (int f = 0; f < frags; f += 2) {
             f32x4 l[2];
@@ -1171,8 +1224,8 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
     SlimRows<P, ND> next;
     if (b < blocks) next.load(a, b * 16 + (lane & 15), cnt, lane);
     slim_load_w<P, ND>(a, lds);
-    const int shift = P == 2 ? logit_shift(a.st) : 0;
-    const int same = dl_exp<T>(o.bs, MODE) - (P == 2 ? shift_for(from_bits(a.st->amax_w)) : 0);
+    const int ws = P == 2 ? weight_shift(a.st) : 0, same = dl_exp<T>(o.bs, MODE) - ws;
+    const int most = most_of<T, P == 2 ? 3 : 1>(a.st, o.bs, o.up, cnt);
     const float cs = MODE == kExpect && !std::is_same<T, bf16>::value ? ldexpf(1.f, -center_exp(o.bs)) : 1.f;
     const int base = lds_chunk<kK, 16>(lane & 15, lane >> 4), frags = a.Vp / 16, q4 = (lane >> 4) * 4;
     const float* centers = reinterpret_cast<const float*>(lds + P * a.Vp * ND * 64);
@@ -1188,7 +1241,8 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
         const float tp = a.top[m], rs = a.inv_sum[m], e0 = MODE == kExpect ? a.mean[m] * cs : 0.f;
         const int target = MODE == kCE ? a.tgt[m] : -1, t = target - q4;
         float g = upstream(o.up, m, cnt);
-        const int ge = row_exp<T>(g), we = !std::is_same<T, bf16>::value && o.up.each ? weight_exp(o.bs, g) : 0;
+        const int own = P == 2 ? a.shifts[m] : 0, shift = -ws - own;
+        const int ge = row_exp<T>(g), we = std::is_same<T, bf16>::value ? 0 : weight_exp(g, P == 2 ? kReachTop - own : 0, most);
         g = ldexpf(g, std::is_same<T, bf16>::value ? 0 : kDlTop - ge);
         if (MODE == kCE && target < 0) g = __builtin_nanf("");
         const float gr = g * rs;
@@ -1301,7 +1355,7 @@ __global__ __launch_bounds__(kFewT) void few_kernel(const IT* __restrict__ h, lo
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, Dq = (a.D + 7) & ~7;
     if (a.set_count && blockIdx.x == 0 && threadIdx.x == 0) {
         a.st->count = a.n;
-        a.st->amax_h = a.st->amax_w = 0;
+        a.st->amax_w = 0;
     }
     const int cnt = a.set_count ? a.n : a.st->count;
     for (int r = 0; r < NR; ++r)
@@ -1448,8 +1502,9 @@ struct Saved {
     float* mean;
     int* rows;
     int* tgt;
+    int* shifts;       // exponents of staged rows (fp32, fp16)
 };
-size_t saved_bytes(long long N) { return align256(sizeof(HeadState)) + 5 * align256((size_t)N * 4); }
+size_t saved_bytes(long long N) { return align256(sizeof(HeadState)) + 6 * align256((size_t)N * 4); }
 Saved saved_of(void* p, long long N) {
     char* c = static_cast<char*>(p);
     Saved s;
@@ -1461,6 +1516,7 @@ Saved saved_of(void* p, long long N) {
     s.mean = reinterpret_cast<float*>(c + 2 * a);
     s.rows = reinterpret_cast<int*>(c + 3 * a);
     s.tgt = reinterpret_cast<int*>(c + 4 * a);
+    s.shifts = reinterpret_cast<int*>(c + 5 * a);
     return s;
 }
 
@@ -1567,23 +1623,21 @@ int launched() {
     return e == hipSuccess ? DS_OK : (int)e;
 }
 
-// scales of fp32 inputs (st->amax_h, amax_w); `clear`: all N rows, and *st is not cleared yet
+// the scale of an fp32 weight; `clear`: *st is not set yet, all N rows
 template <class IT>
-void scales(const IT* hidden, long long ldh, const int* rows, const IT* weight, long long N, int D, int V, HeadState* st,
-            bool clear, hipStream_t q) {
+void scale_weight(const IT* weight, long long N, int D, int V, HeadState* st, bool clear, hipStream_t q) {
     constexpr int VEC = 16 / sizeof(IT);
-    const int L = lanes_for(cdiv(D, VEC)), per = 4 * 64 / L * 4;
-    const bool alone = cdiv(N, per) <= 4 && cdiv(V, per) <= 4;      // a pass of loads takes less than a launch
-    const int bx = alone ? 1 : cdiv(N, per) < 512 ? cdiv(N, per) : 512, bw = alone ? 1 : cdiv(V, per) < 512 ? cdiv(V, per) : 512;
-    if (clear && bx + bw > 2) head_init_kernel<<<1, 1, 0, q>>>(st, (int)N);
-    amax_kernel<IT, VEC><<<bx + bw, 256, 0, q>>>(hidden, ldh, rows, st, weight, V, D, L, bx, clear ? (int)N : 0);
+    const int L = lanes_for(cdiv(D, VEC)), per = 4 * 64 / L * 4, b = cdiv(V, per);
+    const int blocks = b <= 4 ? 1 : b < 512 ? b : 512;       // four passes of loads take less than a launch
+    if (clear && blocks > 1) head_init_kernel<<<1, 1, 0, q>>>(st, (int)N);
+    amax_kernel<IT, VEC><<<blocks, 256, 0, q>>>(weight, st, V, D, L, clear ? (int)N : 0);
 }
 // inputs as matrix operands: in place, or staged at wh and ww (stage: now; clear: *s.st is not set yet)
 template <class IT, class T, int SPLIT>
-void operands(const Plan& p, const IT* hidden, long long ldh, const IT* weight, long long N, int D, int V, const Saved& s,
+void operands(const Plan& p, int mode, const IT* hidden, long long ldh, const IT* weight, long long N, int D, int V, const Saved& s,
               const int* rows, bool stage, bool clear, char* wh, char* ww, Operand& H, Operand& W, hipStream_t q) {
     if constexpr (SPLIT == 3)
-        if (stage) scales(hidden, ldh, rows, weight, N, D, V, s.st, clear, q);
+        if (stage) scale_weight(weight, N, D, V, s.st, clear, q);
     H = Operand{hidden, ldh, 0, (int)N, D};
     W = Operand{weight, D, 0, V, D};
     constexpr int VEC = 16 / sizeof(IT);
@@ -1595,12 +1649,12 @@ void operands(const Plan& p, const IT* hidden, long long ldh, const IT* weight, 
     Source a{}, b{};
     if (p.stage_h) {
         const long long lo = N * p.Dp;
-        a = Source{hidden, ldh, rows, &s.st->count, (int)N, &s.st->amax_h, wh, lo, 0, blocks(N)};
+        a = Source{hidden, ldh, rows, &s.st->count, (int)N, nullptr, s.shifts, mode == kCE ? s.st : nullptr, wh, lo, 0, blocks(N)};
         H = Operand{wh, p.Dp, lo, (int)N, p.Dp};
     }
     if (p.stage_w) {
         const long long lo = (long long)V * p.Dp;
-        b = Source{weight, D, nullptr, nullptr, V, &s.st->amax_w, ww, lo, a.blocks, blocks(V)};
+        b = Source{weight, D, nullptr, nullptr, V, &s.st->amax_w, nullptr, nullptr, ww, lo, a.blocks, blocks(V)};
         W = Operand{ww, p.Dp, lo, V, p.Dp};
     }
     if (stage && a.blocks + b.blocks > 0)
@@ -1616,7 +1670,7 @@ int with_lds(K kernel, int bytes) {    // what a kernel may use beyond 64 KB it 
 SlimArgs slim_args(const Plan& p, const Operand& H, const Operand& W, const Saved& s, const int* rows, long long N, int D, int V,
                    const float* centers) {
     return SlimArgs{H.p, H.ld, H.lo, p.stage_h ? nullptr : rows, rows, s.st, 0, (int)N, D, V, (V + 31) & ~31, W,
-                    s.tgt, centers, s.top, s.inv_sum, s.mean};
+                    s.shifts, s.tgt, centers, s.top, s.inv_sum, s.mean};
 }
 template <class T, int P, int ND, int MODE>
 int slim_fwd_launch(const Plan& p, const SlimArgs& a, const SlimFwd& o, hipStream_t q) {
@@ -1714,7 +1768,7 @@ int head_fwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
     }
     Operand H, W;
     char* keep = static_cast<char*>(saved);
-    operands<IT, T, SPLIT>(p, hidden, ldh, weight, N, D, V, s, rows, true, clear, keep + p.sh, keep + p.sw, H, W, q);
+    operands<IT, T, SPLIT>(p, mode, hidden, ldh, weight, N, D, V, s, rows, true, clear, keep + p.sh, keep + p.sw, H, W, q);
     double* sums = mode == kCE && reduction != DS_REDUCE_NONE ? reinterpret_cast<double*>(ws + p.sums) : nullptr;
     if (p.slim) {
         SlimArgs a = slim_args(p, H, W, s, rows, N, D, V, centers);
@@ -1725,7 +1779,7 @@ int head_fwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
         if (sums) loss_total_kernel<<<1, 256, 0, q>>>(sums, s.st, reduction == DS_REDUCE_MEAN, p.slim_grid, out);
         return launched();
     }
-    const StatsArgs sa{V, s.tgt, centers, tlogit, part, (long long)(align256((size_t)p.vt_fwd * N * 4) / 4), (int)N,
+    const StatsArgs sa{V, s.shifts, s.tgt, centers, tlogit, part, (long long)(align256((size_t)p.vt_fwd * N * 4) / 4), (int)N,
                        set_count ? (int)N : 0};
     if (mode == kCE)
         stats_launch<T, SPLIT, kCE>(p, W, H, s, N, D, sa, q);
@@ -1796,22 +1850,25 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
     const int* rows = mode == kCE ? s.rows : nullptr;
     BackState* bs = reinterpret_cast<BackState*>(ws + p.bs);
     Upstream up{g, reduction == DS_REDUCE_NONE, reduction == DS_REDUCE_MEAN, rows};
-    const bool weigh = !std::is_same<T, bf16>::value && up.each, fold = weigh && g_weight && !p.slim_back;
-    if (weigh) {
+    // the forward of few rows stages nothing and leaves no scales; what a second backward of the same forward, maybe at the
+    // same time, finds there is what it forms itself
+    Operand H, W;
+    char* staged = p.few ? ws : static_cast<char*>(saved);
+    operands<IT, T, SPLIT>(p, mode, hidden, ldh, weight, N, D, V, s, rows, p.few != 0, false, staged + (p.few ? p.bh : p.sh),
+                           staged + (p.few ? p.bw : p.sw), H, W, q);
+    // dW weighs rows where their upstream differs, and fp32's always; heads on chip weigh dl as they store it
+    const bool fold = std::is_same<T, f16>::value && (up.each || SPLIT == 3) && g_weight && !p.slim_back;
+    const bool reach = SPLIT == 3 || fold;
+    if (!std::is_same<T, bf16>::value && up.each) {
         Features f{};
+        if (reach && p.stage_h) f.shifts = s.shifts;
         if constexpr (std::is_same<IT, f16>::value)
-            if (fold) f = Features{hidden, ldh, rows, D, lanes_for(cdiv(D, 8))};
+            if (fold && !p.stage_h) f = Features{nullptr, hidden, ldh, rows, D, lanes_for(cdiv(D, 8))};
         const long long most = std::max<long long>(centers ? V : 0, f.h ? N * f.L : N);      // threads
         const int blocks = most <= kScaleAlone ? 1 : cdiv(most, 4 * kScaleT) < 256 ? cdiv(most, 4 * kScaleT) : 256;
         if (blocks > 1) back_init_kernel<<<1, 1, 0, q>>>(bs);
         back_scale_kernel<<<blocks, kScaleT, 0, q>>>(up, s.st, centers, V, f, bs);
     }
-    // the forward of few rows stages nothing and leaves zero scales; the maximum that a second backward of the same forward,
-    // maybe at the same time, finds there is the one that it forms itself
-    Operand H, W;
-    char* staged = p.few ? ws : static_cast<char*>(saved);
-    operands<IT, T, SPLIT>(p, hidden, ldh, weight, N, D, V, s, rows, p.few != 0, false, staged + (p.few ? p.bh : p.sh),
-                           staged + (p.few ? p.bw : p.sw), H, W, q);
     Ignored ignored{};
     if (mode == kCE && g_hidden) {
         constexpr int VEC = 16 / sizeof(IT);
@@ -1826,10 +1883,9 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
         if (fold) {
             Hw = Operand{ws + p.hw, p.Dp, N * p.Dp, (int)N, p.Dp};
             const int blocks = cdiv(N * p.Dp, 8 * 256 * 2);
-            fold_rows_kernel<SPLIT><<<blocks < 4096 ? blocks : 4096, 256, 0, q>>>(H, s.st, up, bs, reinterpret_cast<f16*>(ws + p.hw),
-                                                                                  p.Dp, N * p.Dp);
+            fold_rows_kernel<SPLIT><<<blocks < 4096 ? blocks : 4096, 256, 0, q>>>(H, s.shifts, s.st, up, bs,
+                                                                                  reinterpret_cast<f16*>(ws + p.hw), p.Dp, N * p.Dp);
         }
-    const int folded = fold && SPLIT != 3 ? 14 : 0;
     T* dl = reinterpret_cast<T*>(ws + p.dl);
     float* dhp = reinterpret_cast<float*>(ws + p.dhp);
     float* dwp = reinterpret_cast<float*>(ws + p.dwp);
@@ -1848,7 +1904,7 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
             if (rc) return rc;
             if (p.pack) Hw = Operand{ws + p.bh, p.Dp, 0, (int)N, p.Dp};
         } else {
-            const DlArgs da{v0, cols, s.tgt, centers, s.top, s.inv_sum, s.mean, up, dl, ld, lo};
+            const DlArgs da{v0, cols, s.shifts, s.tgt, centers, s.top, s.inv_sum, s.mean, up, dl, ld, lo};
             if (mode == kCE)
                 dl_launch<T, SPLIT, kCE>(p, Wp, H, s, bs, N, D, da, q);
             else
@@ -1856,29 +1912,29 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
         }
         const Operand G{dl, ld, lo, (int)N, ld};
         if (g_hidden && !p.slim_back) {
-            const GradArgs ga{D, cols, p.dh_splits, mode, cols, v0 == 0, rows, g_hidden, dhp, N * D4, up, 0};
+            const GradArgs ga{D, cols, p.dh_splits, mode, cols, v0 == 0, rows, g_hidden, dhp, N * D4, up, false};
             grad_launch<IT, T, SPLIT, 0>(p.dh, p.dh_part, Wp, G, s, bs, N, ga, q);
         }
         if (g_weight) {
             IT* gw = g_weight + (long long)v0 * D;
-            const GradArgs ga{D, cols, p.dw_splits, mode, cols, 1, nullptr, gw, dwp, (long long)p.piece * D4, up, folded};
+            const GradArgs ga{D, cols, p.dw_splits, mode, cols, 1, nullptr, gw, dwp, (long long)p.piece * D4, up, reach};
             grad_launch<IT, T, SPLIT, 1>(p.dw, p.dw_splits > 1, Hw, G, s, bs, cols, ga, q);
             if (p.dw_splits > 8 && (long long)cols * D4 <= kShareOuts)
                 head_sum_kernel<T, SPLIT, IT, 16><<<cdiv((long long)cols * D4 / 4, 16), 256, 0, q>>>(
-                    dwp, (long long)p.piece * D4, p.dw_splits, s.st, bs, cols, D, mode, 1, up, folded, nullptr, gw);
+                    dwp, (long long)p.piece * D4, p.dw_splits, s.st, bs, cols, D, mode, 1, up, reach, nullptr, gw);
             else if (p.dw_splits > 1)
                 head_sum_kernel<T, SPLIT, IT, 1><<<cdiv((long long)cols * D4 / 4, 256), 256, 0, q>>>(
-                    dwp, (long long)p.piece * D4, p.dw_splits, s.st, bs, cols, D, mode, 1, up, folded, nullptr, gw);
+                    dwp, (long long)p.piece * D4, p.dw_splits, s.st, bs, cols, D, mode, 1, up, reach, nullptr, gw);
         }
     }
     if (g_hidden && p.dh_part && !p.slim_back) {
         const bool many = p.dh_splits > 8 && N * D4 <= kShareOuts;
         const int blocks = cdiv(N * (D4 / 4), many ? 16 : 256), grid = blocks < 16384 ? blocks : 16384;
         if (many)
-            head_sum_kernel<T, SPLIT, IT, 16><<<grid, 256, 0, q>>>(dhp, N * D4, p.dh_splits, s.st, bs, (int)N, D, mode, 0, up, 0, rows,
+            head_sum_kernel<T, SPLIT, IT, 16><<<grid, 256, 0, q>>>(dhp, N * D4, p.dh_splits, s.st, bs, (int)N, D, mode, 0, up, false, rows,
                                                                    g_hidden);
         else
-            head_sum_kernel<T, SPLIT, IT, 1><<<grid, 256, 0, q>>>(dhp, N * D4, p.dh_splits, s.st, bs, (int)N, D, mode, 0, up, 0, rows,
+            head_sum_kernel<T, SPLIT, IT, 1><<<grid, 256, 0, q>>>(dhp, N * D4, p.dh_splits, s.st, bs, (int)N, D, mode, 0, up, false, rows,
                                                                   g_hidden);
     }
     return launched();

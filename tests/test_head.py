@@ -365,6 +365,65 @@ def test_weighted_out_rows_leave_no_trace(n, d, v, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+@pytest.mark.parametrize("n,d,v", [(20, 70, 500), (60, 40, 50), (200, 64, 900), (300, 515, 70), (9000, 24, 40), (3000, 136, 1500)])
+def test_float32_rows_do_not_see_each_other(n, d, v, reduction):
+    """Features of 1e-12, 1 and 1e12 in the rows of one batch: a row's loss, depth and gradient have the bits that they have in a
+    batch of its like (the same sizes, so the same kernels), and dW what follows from the largest."""
+    h, w, t, up, c = _data(n, d, v, torch.float32, seed=n + d)
+    size = torch.ones(n, device=DEV)
+    size[0::4], size[1::4], size[2::4] = 1e12, 1e-12, 1e30
+    if reduction == "mean":          # a count that every batch has
+        up = torch.full_like(up, 0.5)
+    mixed = h * size[:, None]
+    for f in (1.0, 1e12, 1e-12, 1e30):
+        rows = size == f
+        if not bool(rows.any()):
+            continue
+        alike = h * f
+        a, b = _ce(mixed, w, t, "none", up), _ce(alike, w, t, "none", up)
+        assert torch.equal(a[0][rows], b[0][rows]) and torch.equal(a[1][rows], b[1][rows])
+        a, b = _ex(mixed, w, c, up), _ex(alike, w, c, up)
+        assert torch.equal(a[0][rows], b[0][rows]) and torch.equal(a[1][rows], b[1][rows])
+    size[2::4] = 1e-6
+    mixed = h * size[:, None]
+    scale = torch.tensor(0.5 * n, device=DEV)
+    got = _ce(mixed, w, t, reduction, up if reduction == "none" else scale)
+    out, gh, gw, tol, th, tw = _oracle(mixed, w, t=t, up=up if reduction == "none" else torch.full_like(up, 0.5))
+    row = (2.0 ** -21 + (d + 4) * 2.0 ** -24) * (mixed.double().abs() @ w.double().abs().T)
+    row = row.max(dim=1).values + 2.0 ** -39 * d * mixed.double().abs().max(dim=1).values * w.double().abs().max()
+    own = 2 * row + (v + 32) * 2.0 ** -24 + 4 * 2.0 ** -24 * ((mixed.double() @ w.double().T).abs().max(dim=1).values + out.abs() + 1)
+    if reduction == "none":
+        _close(got[0], out, own, "loss")
+    _close(got[1], gh, th, "g_hidden")
+    _close(got[2], gw, tw + (2.0 ** -22 * gw.abs() if reduction == "mean" else 0.0), "g_weight")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+@pytest.mark.parametrize("n,d,v", [(4, 40, 500), (60, 40, 50), (200, 64, 900)])
+def test_float32_rows_of_zeros_and_of_masked_size(n, d, v, reduction):
+    """Rows of zeros, and rows of 1e35 with zero upstream or ignored: the gradient of the weight is that without them."""
+    h, w, t, up, c = _data(n, d, v, torch.float32, seed=n)
+    h = h * 1e-3
+    h[0], h[n // 2] = 0, 0
+    loud = h.clone()
+    loud[1::3] = 1e32 * h[1::3]
+    if reduction == "none":
+        up[1::3] = 0
+        pairs = [(_ce(loud, w, t, "none", up), _oracle(torch.where((up == 0)[:, None], 0.0, h), w, t=t, up=up)),
+                 (_ex(loud, w, c, up), _oracle(torch.where((up == 0)[:, None], 0.0, h), w, c=c, up=up))]
+    else:
+        t[1::3] = -100
+        f = 1.0 / int((t != -100).sum()) if reduction == "mean" else 1.0
+        pairs = [(_ce(loud, w, t, reduction), _oracle(h, w, t=t, up=torch.full((n,), f, dtype=torch.float64, device=DEV)))]
+    for got, (_, gh, gw, _, th, tw) in pairs:
+        _close(got[2], gw, tw + 2.0 ** -22 * gw.abs(), "g_weight")
+        quiet = torch.arange(n, device=DEV) % 3 != 1
+        _close(got[1][quiet], gh[quiet], (th + 2.0 ** -22 * gh.abs())[quiet], "g_hidden")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_confident_rows(dtype):
     """Rows that are all but certain of their class: p - 1 keeps its digits, nothing overflows."""
