@@ -249,63 +249,39 @@ struct Source {
     long long lo;
     int first, blocks;         // blocks 0: not there
 };
+constexpr int kReachTop = 15;      // a row with that shift has features below 2^15 as stored
 constexpr int kZeroShift = 163;    // of a row without finite elements but zeros: it reaches nowhere
-template <class IT, class T, int SPLIT, int VEC>
-__global__ __launch_bounds__(256) void stage_kernel(Source s0, Source s1, int D, int Dp, int L) {
-    const bool second = s1.blocks > 0 && (int)blockIdx.x >= s1.first;
-    const Source& s = second ? s1 : s0;
+// Own: rows find their own shifts; kept: and one load brings a whole row
+enum StageHow { kSame, kOwn, kOwnKept };
+template <class IT, class T, int SPLIT, int VEC, StageHow HOW>
+__device__ __forceinline__ int stage_rows(const Source& s, int D, int Dp, int L) {
     const IT* x = static_cast<const IT*>(s.x);
     const int c = s.cnt ? *s.cnt : s.n;
     const int lane = threadIdx.x & 63, sub = lane & (L - 1), R = 64 / L;
     constexpr int U = 4;
-    constexpr bool kShifts = !std::is_same<T, bf16>::value;      // (fp16 rows are left as they are, but dW wants to know)
     int shift[U], reach = kNone;
-#pragma unroll
-    for (int u = 0; u < U; ++u) shift[u] = SPLIT == 3 && s.amax ? shift_for(from_bits(*s.amax)) : 0;
+    const int same = SPLIT == 3 && HOW == kSame ? shift_for(from_bits(*s.amax)) : 0;
     const int hop = s.blocks * 4 * R;
     for (int r0 = (((int)blockIdx.x - s.first) * 4 + (threadIdx.x >> 6)) * R + lane / L; r0 < c; r0 += hop * U) {
-        IT v[U][VEC];
-        auto load = [&](int d) {
+        auto load = [&](int d, IT (&v)[U][VEC]) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int r = min(r0 + u * hop, c - 1);
                 load_vec<IT, VEC>(x + (s.rows ? s.rows[r] : r) * s.ld, d, D, v[u]);
             }
         };
-        const bool kept = kShifts && s.shifts && Dp <= L * VEC;      // one load brings the whole row
-        if (kShifts && s.shifts) {
-            float m[U] = {};
-            for (int d = sub * VEC; d < Dp; d += L * VEC) {
-                load(d);
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) m[u] = fmaxf(m[u], finite_abs((float)v[u][e]));
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                for (int o = 1; o < L; o <<= 1) m[u] = fmaxf(m[u], __shfl_xor(m[u], o, 64));
-                const int own = m[u] > 0.f ? shift_for(m[u]) : kZeroShift;
-                if (SPLIT == 3) shift[u] = own;
-                if (sub == 0 && r0 + u * hop < c) {
-                    s.shifts[r0 + u * hop] = own;
-                    reach = max(reach, 15 - own);
-                }
-            }
-        }
-        for (int d = sub * VEC; d < Dp; d += L * VEC) {
-            if (!kept) load(d);
+        auto store = [&](int d, const IT (&v)[U][VEC]) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int r = r0 + u * hop;
-                if (r >= c) break;
+                if (r >= c) continue;
                 T* q = static_cast<T*>(s.y) + (long long)r * Dp + d;
                 typename Vec<T, VEC>::type h, l;
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     if constexpr (SPLIT == 3) {
                         f16 a, b;
-                        split16(ldexpf((float)v[u][e], shift[u]), a, b);
+                        split16(ldexpf((float)v[u][e], HOW == kSame ? same : shift[u]), a, b);
                         h[e] = a;
                         l[e] = b;
                     } else {
@@ -315,13 +291,68 @@ __global__ __launch_bounds__(256) void stage_kernel(Source s0, Source s1, int D,
                 *reinterpret_cast<typename Vec<T, VEC>::type*>(q) = h;
                 if (SPLIT == 3) *reinterpret_cast<typename Vec<T, VEC>::type*>(q + s.lo) = l;
             }
+        };
+        float m[U] = {};
+        auto largest = [&](const IT (&v)[U][VEC]) {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) m[u] = fmaxf(m[u], finite_abs((float)v[u][e]));
+        };
+        auto settle = [&] {
+            // (all lanes of a row are here: L divides 64 and r0 is the row's)
+            for (int o = 1; o < L; o <<= 1)
+#pragma unroll
+                for (int u = 0; u < U; ++u) m[u] = fmaxf(m[u], __shfl_xor(m[u], o, 64));
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                shift[u] = m[u] > 0.f ? shift_for(m[u]) : kZeroShift;
+                if (sub == 0 && r0 + u * hop < c) {
+                    s.shifts[r0 + u * hop] = shift[u];
+                    reach = max(reach, kReachTop - shift[u]);
+                }
+            }
+        };
+        const int d0 = sub * VEC;
+        if constexpr (HOW == kOwnKept) {
+            IT v[U][VEC] = {};
+            if (d0 < Dp) load(d0, v);
+            largest(v);
+            settle();
+            if (d0 < Dp) store(d0, v);
+        } else {
+            if (HOW == kOwn) {
+                for (int d = d0; d < Dp; d += L * VEC) {
+                    IT v[U][VEC];
+                    load(d, v);
+                    largest(v);
+                }
+                settle();
+            }
+            for (int d = d0; d < Dp; d += L * VEC) {
+                IT v[U][VEC];
+                load(d, v);
+                store(d, v);
+            }
         }
     }
+    return reach;
+}
+template <class IT, class T, int SPLIT, int VEC>
+__global__ __launch_bounds__(256) void stage_kernel(Source s0, Source s1, int D, int Dp, int L) {
+    const bool second = s1.blocks > 0 && (int)blockIdx.x >= s1.first;
+    const Source s = second ? s1 : s0;
+    // (bf16 rows need no shifts; fp16 rows are left as they are, but dW wants to know)
+    if (std::is_same<T, bf16>::value || !s.shifts) {
+        stage_rows<IT, T, SPLIT, VEC, kSame>(s, D, Dp, L);
+        return;
+    }
+    int reach = Dp <= L * VEC ? stage_rows<IT, T, SPLIT, VEC, kOwnKept>(s, D, Dp, L) : stage_rows<IT, T, SPLIT, VEC, kOwn>(s, D, Dp, L);
     if (SPLIT == 3 && s.reach) {
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) reach = max(reach, __shfl_xor(reach, o, 64));
         __shared__ int top[4];
-        if (lane == 0) top[threadIdx.x >> 6] = reach;
+        if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = reach;
         __syncthreads();
         reach = max(max(top[0], top[1]), max(top[2], top[3]));
         if (threadIdx.x == 0 && reach > kNone) atomicMax(&s.reach->reach[blockIdx.x % kReach].most, reach);
@@ -617,7 +648,6 @@ __device__ __forceinline__ int most_of(const HeadState* st, const BackState* bs,
         for (int i = 0; i < kReach; ++i) r = max(r, st->reach[i].most);
     return r == kNone ? kNone : r + row_exp<T>(upstream(u, 0, cnt));
 }
-constexpr int kReachTop = 15;      // features that take part with 2^most are below 2^15 as stored, or as weighted
 // exponent of sums over rows -> dW
 template <class T, int SPLIT>
 __device__ __forceinline__ int dw_exp(const HeadState* st, const BackState* bs, const Upstream& u, int mode, int cnt, bool reach) {
