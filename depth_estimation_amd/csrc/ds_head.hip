@@ -1559,8 +1559,13 @@ struct Plan {
     bool slim_back, pack;
     size_t sh, sw, saved_total;                                            // staged operands behind Saved (not of few rows)
     size_t counts, tlogit, part, sums, fwd_total;                          // offsets of the forward's workspace
-    size_t bh, bw, bs, hw, dl, dhp, dwp, bwd_total;                            // offsets of the backward's
+    size_t bh, bw, bs, hw, dl, dhp, dwp, own, bwd_total;                   // offsets of the backward's
 };
+// statistics that a backward of few rows forms itself: three planes of class tiles, then as Saved, the targets' logits, and the
+// outputs that nobody reads
+size_t few_stats_bytes(const Plan& p, long long N) {
+    return 3 * align256((size_t)p.vt_fwd * N * 4) + 5 * align256((size_t)N * 4);
+}
 
 int splits_for(long long tiles, long long steps) {
     // enough workgroups for two a CU, no split shorter than four steps of 64
@@ -1621,6 +1626,10 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     p.piece = pieces == 1 ? V : (cdiv((long long)V, pieces) + 63) / 64 * 64;
     p.piece_ld = pad8(p.piece);
     p.dl_shape = thin ? kThin : cut_of(p.piece, N, D, p.planes, false).shape;
+    // The backward's logits must have the forward's bits: probabilities are exp(l - top), and where logits are large their
+    // rounding is too.  All shapes add up in the same order, but the large one takes planes pair by pair.
+    if (p.planes == 2 && (p.slim || (p.fwd == kBig) != (p.dl_shape == kBig)))
+        p.dl_shape = !p.slim ? p.fwd : p.dl_shape == kBig ? kSq : p.dl_shape;
     const Cut dh = cut_of(D, N, p.piece, p.planes, true), dw = cut_of(D, p.piece, N, p.planes, true);
     p.dh = thin ? kThin : dh.shape;
     p.dh_splits = thin ? splits_for(cdiv(D, 128), cdiv(p.piece, kBK)) : dh.splits;
@@ -1636,6 +1645,7 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     p.dl = o; o += align256((size_t)N * p.piece_ld * el);
     p.dhp = o; o += p.dh_part ? align256((size_t)p.dh_splits * N * D4 * 4) : 0;
     p.dwp = o; o += p.dw_splits > 1 ? align256((size_t)p.dw_splits * p.piece * D4 * 4) : 0;
+    p.own = o; o += p.few ? few_stats_bytes(p, N) : 0;
     p.bwd_total = o;
     return p;
 }
@@ -1752,6 +1762,12 @@ void stats_launch(const Plan& p, const Operand& W, const Operand& H, const Saved
         head_stats_kernel<T, Sq, SPLIT, MODE><<<tiles, Sq::T, 0, q>>>(W, H, s.st, D, a);
 }
 
+// of stats_launch, up to 32 rows
+JoinArgs join_tiles(const Plan& p, int mode, const Saved& s, const StatsArgs& a, long long N, float* out, int total) {
+    return JoinArgs{a.part, a.part + a.plane, a.part + 2 * a.plane, a.tlogit, N, 1, 0, p.vt_fwd, mode, s.st, s.rows, s.tgt,
+                    s.top, s.inv_sum, s.mean, out, total};
+}
+
 template <class IT, class T, int SPLIT>
 int head_fwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT* weight, const long long* target, const float* centers,
              long long N, int D, int V, long long ignore, int reduction, float* out, void* saved, char* ws, hipStream_t q) {
@@ -1771,29 +1787,14 @@ int head_fwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
     if (clear && SPLIT != 3) head_init_kernel<<<1, 1, 0, q>>>(s.st, (int)N);
     float* part = reinterpret_cast<float*>(ws + p.part);
     float* tlogit = reinterpret_cast<float*>(ws + p.tlogit);
-    JoinArgs ja{};
-    ja.mode = mode;
-    ja.st = s.st;
-    ja.rows = s.rows;
-    ja.tgt = s.tgt;
-    ja.top = s.top;
-    ja.inv_sum = s.inv_sum;
-    ja.mean = s.mean;
-    ja.out = out;
-    ja.total = mode == kCE ? reduction : 0;
     if (p.few) {
         const FewArgs fa{rows, s.st, set_count, (int)N, D, V, 0, mode == kCE ? s.tgt : nullptr, centers, part};
         p.few == 1   ? few_launch<IT, 1>(p, hidden, ldh, weight, fa, q)
         : p.few == 2 ? few_launch<IT, 2>(p, hidden, ldh, weight, fa, q)
                      : few_launch<IT, 4>(p, hidden, ldh, weight, fa, q);
-        ja.mx = part;
-        ja.s = part + 1;
-        ja.sc = part + 2;
-        ja.tl = part + 3;
-        ja.step = ja.tl_step = p.few * 4;
-        ja.pitch = 4;
-        ja.entries = p.few_grid;
-        join_few_kernel<<<1, 1024, 0, q>>>(ja);
+        const int step = p.few * 4;
+        join_few_kernel<<<1, 1024, 0, q>>>(JoinArgs{part, part + 1, part + 2, part + 3, step, 4, step, p.few_grid, mode, s.st, s.rows, s.tgt,
+                                                    s.top, s.inv_sum, s.mean, out, mode == kCE ? reduction : DS_REDUCE_NONE});
         return launched();
     }
     Operand H, W;
@@ -1816,14 +1817,7 @@ int head_fwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
     else
         stats_launch<T, SPLIT, kExpect>(p, W, H, s, N, D, sa, q);
     if (N <= 32) {
-        ja.mx = part;
-        ja.s = part + sa.plane;
-        ja.sc = part + 2 * sa.plane;
-        ja.tl = tlogit;
-        ja.step = N;
-        ja.pitch = 1;
-        ja.entries = p.vt_fwd;
-        join_few_kernel<<<1, 1024, 0, q>>>(ja);
+        join_few_kernel<<<1, 1024, 0, q>>>(join_tiles(p, mode, s, sa, N, out, mode == kCE ? reduction : DS_REDUCE_NONE));
         return launched();
     }
     head_join_kernel<<<cdiv(N, 32), 256, 0, q>>>(part, sa.plane, (int)N, p.vt_fwd, s.st, mode, s.rows, s.tgt, tlogit, s.top,
@@ -1876,7 +1870,7 @@ template <class IT, class T, int SPLIT>
 int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT* weight, const long long* target, const float* centers,
              const float* g, long long N, int D, int V, long long ignore, int reduction, void* saved, IT* g_hidden,
              IT* g_weight, char* ws, hipStream_t q) {
-    const Saved s = saved_of(saved, N);
+    Saved s = saved_of(saved, N);
     const int* rows = mode == kCE ? s.rows : nullptr;
     BackState* bs = reinterpret_cast<BackState*>(ws + p.bs);
     Upstream up{g, reduction == DS_REDUCE_NONE, reduction == DS_REDUCE_MEAN, rows};
@@ -1898,6 +1892,20 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
         const int blocks = most <= kScaleAlone ? 1 : cdiv(most, 4 * kScaleT) < 256 ? cdiv(most, 4 * kScaleT) : 256;
         if (blocks > 1) back_init_kernel<<<1, 1, 0, q>>>(bs);
         back_scale_kernel<<<blocks, kScaleT, 0, q>>>(up, s.st, centers, V, f, bs);
+    }
+    if (p.few) {      // the forward formed its logits without the matrix instructions: these have other bits
+        float* part = reinterpret_cast<float*>(ws + p.own);
+        const long long plane = align256((size_t)p.vt_fwd * N * 4) / 4, n4 = align256((size_t)N * 4) / 4;
+        float* tlogit = part + 3 * plane;
+        s.top = tlogit + n4;
+        s.inv_sum = tlogit + 2 * n4;
+        s.mean = tlogit + 3 * n4;
+        const StatsArgs sa{V, s.shifts, s.tgt, centers, tlogit, part, plane, (int)N, 0};
+        if (mode == kCE)
+            stats_launch<T, SPLIT, kCE>(p, W, H, s, N, D, sa, q);
+        else
+            stats_launch<T, SPLIT, kExpect>(p, W, H, s, N, D, sa, q);
+        join_few_kernel<<<1, 1024, 0, q>>>(join_tiles(p, mode, s, sa, N, tlogit + 4 * n4, DS_REDUCE_NONE));
     }
     Ignored ignored{};
     if (mode == kCE && g_hidden) {

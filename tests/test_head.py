@@ -301,6 +301,37 @@ def test_large_logits_and_upstreams(dtype):
         _close(a[inside], b[inside], tol_[inside], "gradient")
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,d,v", [(1, 37, 1001), (3, 40, 500), (4, 250, 60), (20, 70, 500), (60, 40, 50), (200, 64, 900),
+                                   (2500, 301, 4100), (1500, 96, 20000)])
+def test_huge_logits_give_whole_probabilities(n, d, v, dtype):
+    """Logits of 1e9 (float16: 1e5): the backward's are the forward's bit by bit, so a probability is 1 or 0 however large their
+    rounding is.  Rows whose two largest logits lie within what that may be are left out (their upstream is 0), and so is dl's
+    error: dl is 0 or +-upstream, rounded to its stored type."""
+    h, w, t, up, c = _data(n, d, v, dtype, seed=n + v)
+    h = (h.float() * (2.0 ** 11 if dtype == torch.float16 else 2.0 ** 28)).to(dtype)
+    l = h.double() @ w.double().T
+    two = l.topk(2, dim=1).values
+    far = two[:, 0] - two[:, 1] > 40 + 2.0 ** -20 * d * (h.double().abs() @ w.double().abs().T).max(dim=1).values / d ** 0.5
+    assert bool(far.any())
+    up = torch.where(far, up, torch.zeros_like(up))
+    p = torch.nn.functional.one_hot(l.argmax(1), v).double()
+    u = 2.0 ** -21 if dtype == torch.float32 else U[dtype]
+    pairs = [(_ce(h, w, t, "none", up), (p - torch.nn.functional.one_hot(t, v)) * up.double()[:, None]),
+             (_ex(h, w, c, up), torch.zeros_like(p))]
+    for got, dl in pairs:
+        gh, gw = dl @ w.double(), dl.T @ h.double()
+        # a probability of exp(-40) and less beside: 4e-18 of the upstream (times the largest centre)
+        err = (u + (n + v + 8) * 2.0 ** -24) * dl.abs() + 1e-15 * up.double()[:, None] * (1.0 + 80.0)
+        split = 2.0 ** -21 if dtype == torch.float32 else 0.0
+        _close(got[1], gh, (err + split * dl.abs()) @ w.double().abs() + U[dtype] * gh.abs() + 2.0 ** -24, "g_hidden")
+        inside = gw.abs() < torch.finfo(dtype).max / 2
+        tw = (err + split * dl.abs()).T @ h.double().abs() + U[dtype] * gw.abs() + 2.0 ** -24
+        _close(got[2][inside], gw[inside], tw[inside], "g_weight")
+    assert torch.equal(pairs[1][0][0][far], c[l.argmax(1)][far])
+
+
 def _row_oracle(h, w, up, t=None, c=None):
     """g_hidden and its tolerance row by row: a row's gradient is its upstream value times what it is for 1, and so is what it may be
     off by, whatever the other rows' upstream"""
