@@ -647,6 +647,39 @@ def test_pieces_with_a_row_of_nan(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_several_pieces_with_rows_left_out(dtype):
+    """70001 classes of 4000 rows: two pieces (four in float32), a smaller last one, rows left out, targets at the pieces' ends.  Cross
+    entropy and the expectation, whose centres belong to the piece; every row and every class checked."""
+    n, d, v = 4000, 40, 70001
+    h, w, t, up, c = _data(n, d, v, dtype, seed=41, keep=0.8)
+    for k, cls in enumerate((v - 1, 0, 17535, 17536, 35007, 35008, 52608, 70000)):
+        t[10 + k] = cls
+    for got, k in ((_ce(h, w, t, "none", up), dict(t=t)), (_ex(h, w, c, up), dict(c=c))):
+        out, gh, gw, tol, th, tw = _oracle(h, w, up=up, **k)
+        _close(got[0], out, tol, "output")
+        _close(got[1], gh, th, "g_hidden")
+        _close(got[2], gw, tw, "g_weight")
+        del out, gh, gw, tol, th, tw
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,d,v,keep", [(515, 96, 15593, 0.9), (914, 131, 43010, 0.9), (227, 131, 3165, 0.9), (121, 96, 3187, 1.0),
+                                        (16961, 96, 753, 0.9), (1706, 131, 38516, 0.9), (16593, 96, 791, 0.05),
+                                        (60000, 504, 520, 0.02), (60000, 504, 520, 0.0)])
+def test_sums_with_splits_that_get_nothing(n, d, v, keep, dtype):
+    """Sums over classes whose steps of 64 are no multiple of the splits (the last ones, up to nine of 128, are empty), in tiles of
+    every size, and sums over rows most of which are left out, so that most splits are."""
+    h, w, t, up, _ = _data(n, d, v, dtype, seed=n + v, keep=keep)
+    out, gh, gw, tol, th, tw = _oracle(h, w, t=t, up=up)
+    got = _ce(h, w, t, "none", up)
+    _close(got[0], out, tol, "loss")
+    _close(got[1], gh, th, "g_hidden")
+    _close(got[2], gw, tw, "g_weight")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("n,d,v", [(777, 250, 128), (600, 120, 288), (900, 64, 576), (500, 33, 289), (400, 256, 64), (300, 128, 144)])
 def test_small_heads_up_to_what_fits(n, d, v, dtype):
     """Heads around the largest weights that are held on chip; the loss of another forward replayed from a captured graph."""
