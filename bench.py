@@ -528,6 +528,8 @@ def main():
     ap.add_argument("--no-also", action="store_true",
                     help="default workload at N=1: skip the short joined runs of the other workloads (the `also` object)")
     args = ap.parse_args()
+    if args.optimizer != "adam" and args.workload != "full_step":
+        ap.error(f"--optimizer {args.optimizer} belongs to --workload full_step: no other workload has an optimizer")
 
     if "WORLD_SIZE" not in os.environ and args.gpus > 1:
         raise SystemExit(self_launch(args.gpus))   # before anything here touches the GPU

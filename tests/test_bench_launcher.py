@@ -33,6 +33,11 @@ def test_single_rank_needs_no_launcher():
     assert line["n_gpus"] == 1 and line["world_size"] == 1
 
 
+def test_optimizer_of_a_workload_without_one_is_an_error():
+    p = _run("--gpus", "1", "--optimizer", "muon")
+    assert p.returncode == 2 and "full_step" in p.stderr and not p.stdout
+
+
 def test_world_size_mismatch_is_an_error():
     p = _run("--gpus", "2", env_extra={"WORLD_SIZE": "1", "RANK": "0"})
     assert p.returncode != 0 and "WORLD_SIZE" in p.stderr
