@@ -574,6 +574,34 @@ def test_streams_and_captured_graphs():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,d,v", [(3, 40, 500), (60, 40, 50), (200, 64, 900), (9000, 72, 600)])
+def test_captured_with_upstreams_that_change(n, d, v, dtype):
+    """Row scales are found anew in every replay: features and upstream values of another size, other rows left out, eager calls
+    between."""
+    h, w, t, up, c = _data(n, d, v, dtype, seed=n, keep=0.8 if n > 3 else 1.0)
+    h2, t2, up2 = h.clone(), t.clone(), up.clone()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        _ce(h2, w, t2, "none", up2), _ex(h2, w, c, up2), _ce(h2, w, t2, "mean")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        out = _ce(h2, w, t2, "none", up2) + _ex(h2, w, c, up2) + _ce(h2, w, t2, "mean")
+    for k in range(4):
+        spread = 10.0 ** (torch.arange(n, device=DEV) % (2 + k) - 1.0)
+        h2.copy_(h * (1.0, 0.25, 1.0, 2.0 ** -6)[k])
+        up2.copy_(up * spread * (1.0, 1e-2, 1.0, 30.0)[k])
+        t2.copy_(t if k % 2 == 0 else t.flip(0))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        eager = _ce(h2, w, t2, "none", up2) + _ex(h2, w, c, up2) + _ce(h2, w, t2, "mean")
+        assert all(torch.equal(a, b) for a, b in zip(out, eager))
+
+
+@pytest.mark.gpu
 def test_head_into_the_photometric_loss():
     """The operators together, as a trainer uses them: features -> expected depth -> warp and photometric loss, plus the cross
     entropy of the same head where a depth was measured; one backward, one orthogonalised step.  Checked: the head's gradient
