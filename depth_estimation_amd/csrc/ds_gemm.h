@@ -451,12 +451,24 @@ __device__ __forceinline__ void put4(f16* p, long long lo, const float (&v)[4]) 
     *reinterpret_cast<f16x4*>(p) = h;
     if (SPLIT == 3) *reinterpret_cast<f16x4*>(p + lo) = l;
 }
+// as split16, to 8 bits each
+__device__ __forceinline__ void split16(float x, bf16& hi, bf16& lo) {
+    hi = (bf16)x;
+    const float h = (float)hi;
+    lo = __builtin_isfinite(h) ? (bf16)(x - h) : (bf16)0.f;
+}
 template <int SPLIT>
-__device__ __forceinline__ void put4(bf16* p, long long, const float (&v)[4]) {
-    bf16x4 h;
+__device__ __forceinline__ void put4(bf16* p, long long lo, const float (&v)[4]) {
+    bf16x4 h, l;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) h[e] = (bf16)v[e];
+    for (int e = 0; e < 4; ++e) {
+        bf16 a, b;
+        split16(v[e], a, b);
+        h[e] = a;
+        l[e] = b;
+    }
     *reinterpret_cast<bf16x4*>(p) = h;
+    if (SPLIT == 3) *reinterpret_cast<bf16x4*>(p + lo) = l;
 }
 
 // Fragments i and i + 1 of a row in 16 bits: lane group q holds four elements from 4 q of either (x, y) and gets eight
@@ -486,11 +498,13 @@ __device__ __forceinline__ s16x4 round4(const f32x4& v) {
 }
 
 // the low plane of four values
+template <class T = f16>
 __device__ __forceinline__ s16x4 rest4(const f32x4& v) {
-    f16x4 r;
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    t4 r;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        f16 h, l;
+        T h, l;
         split16(v[e], h, l);
         r[e] = l;
     }

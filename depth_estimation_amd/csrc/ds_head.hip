@@ -23,9 +23,11 @@
 namespace ds {
 namespace {
 
-// planes of an operand; SPLIT: products a step, 1 (16-bit inputs) or 3 (fp32)
+// planes of an operand; SPLIT: products a step, 1 (16-bit inputs) or 3 (fp32), or 2 (16-bit inputs, but dl in two planes)
 template <int SPLIT>
 constexpr int kP = SPLIT == 3 ? 2 : 1;
+template <int SPLIT>
+constexpr int kPdl = SPLIT > 1 ? 2 : 1;
 
 enum Mode { kCE = 0, kExpect = 1 };
 constexpr int kNone = -(1 << 30);   // no exponent
@@ -748,8 +750,8 @@ __global__ __launch_bounds__(256) void fold_rows_kernel(Operand H, const int* __
 }
 
 // dl of classes [v0, v0 + cols) in 16 bits: [row][class - v0], pitch ld (cols rounded up to 8; zeros behind the last class).
-// The rounding to 16 bits is the products' operand rounding: half a step of the gradients' own type for 16-bit inputs, 2^-22
-// with the two planes of fp32 inputs; p - 1 and c - E are formed in fp32 before it.
+// p - 1 and c - E are formed in fp32, and what is dropped is 2^-22 of dl in two planes of fp16, 2^-16 of bf16, or half a step of
+// the gradients' own type where 16-bit inputs take one plane: Plan::dl_planes.
 struct DlArgs {
     int v0, cols;
     const int* shifts;
@@ -812,7 +814,7 @@ __device__ __forceinline__ void dl_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, i
         }
         if constexpr (S::FM == 1) {
             const float d[4] = {acc[0][j][0], acc[0][j][1], acc[0][j][2], acc[0][j][3]};
-            if (!(edge && c0 >= a.ld)) put4<SPLIT>(dl + (long long)n * a.ld + c0, a.lo, d);
+            if (!(edge && c0 >= a.ld)) put4<SPLIT == 1 ? 1 : 3>(dl + (long long)n * a.ld + c0, a.lo, d);
             continue;
         }
         const int c8 = m0 + wm * S::FM * 16 + (lane >> 4) * 8;
@@ -821,11 +823,11 @@ __device__ __forceinline__ void dl_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, i
             const int c = c8 + i * 16;
             s16x8 hi, lo;
             eight_of(round4<T>(acc[i][j]), round4<T>(acc[i + 1][j]), hi);
-            if constexpr (SPLIT == 3) eight_of(rest4(acc[i][j]), rest4(acc[i + 1][j]), lo);
+            if constexpr (SPLIT > 1) eight_of(rest4<T>(acc[i][j]), rest4<T>(acc[i + 1][j]), lo);
             if (edge && c >= a.ld) continue;
             T* q = dl + (long long)n * a.ld + c;
             *reinterpret_cast<s16x8*>(q) = hi;
-            if constexpr (SPLIT == 3) *reinterpret_cast<s16x8*>(q + a.lo) = lo;
+            if constexpr (SPLIT > 1) *reinterpret_cast<s16x8*>(q + a.lo) = lo;
         }
     }
 }
@@ -923,7 +925,7 @@ __device__ __forceinline__ void grad_of_tile(const f32x4 (&acc)[S::FM][S::FN], i
 template <class T, class S, int SPLIT, class O, bool ACC, int WHICH>
 __global__ __launch_bounds__(S::T) void head_grad_kernel(Operand A, Operand B, const HeadState* __restrict__ st,
                                                          const BackState* __restrict__ bs, GradArgs a) {
-    __shared__ __align__(16) char lds[std::is_same<S, Big>::value ? Big::kLds : lds_bytes<S, kP<SPLIT>, kP<SPLIT>>()];
+    __shared__ __align__(16) char lds[std::is_same<S, Big>::value ? Big::kLds : lds_bytes<S, kP<SPLIT>, kPdl<SPLIT>>()];
     const int cnt = st->count, mt = cdiv(a.D, S::BM), bound = WHICH == 0 ? cnt : a.cols;
     const int k = WHICH == 0 ? a.k : cnt, per = cdiv(cdiv(k, kBK), a.splits) * kBK;
     B.outer = cnt;
@@ -943,7 +945,7 @@ __global__ __launch_bounds__(S::T) void head_grad_kernel(Operand A, Operand B, c
     int sp;
     if constexpr (std::is_same<S, Big>::value) {
         int next_sp = 0;
-        TileStream<T, kM, LB, kP<SPLIT>, kP<SPLIT>> stream(lds, job(t, sp));
+        TileStream<T, kM, LB, kP<SPLIT>, kPdl<SPLIT>> stream(lds, job(t, sp));
         for (; t < units; t += gridDim.x) {
             const int m0 = stream.job.m0, n0 = stream.job.n0;
             f32x4 acc[S::FM][S::FN];
@@ -958,7 +960,7 @@ __global__ __launch_bounds__(S::T) void head_grad_kernel(Operand A, Operand B, c
     } else {
         const Job j = job(t, sp);
         f32x4 acc[S::FM][S::FN];
-        gemm_tile<T, S, kM, LB, kP<SPLIT>, kP<SPLIT>>(A, B, j.m0, j.n0, j.kbeg, j.kend, lds, acc);
+        gemm_tile<T, S, kM, LB, kP<SPLIT>, kPdl<SPLIT>>(A, B, j.m0, j.n0, j.kbeg, j.kend, lds, acc);
         grad_of_tile<T, S, SPLIT, O, ACC, WHICH>(acc, j.m0, j.n0, sp, bound, st, bs, a);
     }
 }
@@ -1049,7 +1051,8 @@ __global__ __launch_bounds__(256) void zero_ignored_kernel(Ignored g, int D, con
 // their features in registers, meets all classes in LDS and has the whole softmax of its rows to itself -- no partial
 // statistics, no barrier.  Backward the same: dl of 32 classes, as the matrix instruction leaves it, is the operand of
 // dH = dl W as it stands (its lanes hold rows, its registers classes, taken as k in the order 4 q + e of two fragments; the
-// transposing LDS reads of W follow that order), so dH needs no second pass; dl itself is written once for dW.
+// transposing LDS reads of W follow that order), so dH needs no second pass; dl itself is written once for dW.  dH takes two
+// planes of dl, straight from registers, whatever the inputs' type.
 //   12 x 96 x 320 rows, 64 features, 80 bins, bf16, forward 20 us (47 MB of features; the tiles above: 48)
 constexpr int kSlimT = 512;
 struct SlimArgs {
@@ -1075,7 +1078,7 @@ struct SlimBwd {
     Upstream up;
     void* g_hidden;            // NULL: not wanted
     void* dl;                  // NULL: dW not wanted
-    int ld;
+    int ld, planes;
     long long lo;
     Ignored ignored;           // the caller's rows that were left out (with g_hidden)
     void* packed;              // kept rows' features written densely for dW (NULL: they lie so already), pitch Dp
@@ -1303,7 +1306,10 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
                 if (dl && n < cnt && v < o.ld) {
                     const f32x4 w = std::is_same<T, bf16>::value ? d[u] : scaled(d[u], we);      // weighted for dW
                     const float y[4] = {w[0], w[1], w[2], w[3]};
-                    put4<P == 2 ? 3 : 1>(dl + (long long)n * o.ld + v, o.lo, y);
+                    if (P == 2 || o.planes == 2)
+                        put4<3>(dl + (long long)n * o.ld + v, o.lo, y);
+                    else
+                        put4<1>(dl + (long long)n * o.ld + v, o.lo, y);
                 }
             }
             if (o.g_hidden) {
@@ -1311,15 +1317,10 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
                 t8 hi, lw;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float y = d[e >> 2][e & 3];
-                    if constexpr (P == 2) {
-                        f16 p, q;
-                        split16(y, p, q);
-                        hi[e] = p;
-                        lw[e] = q;
-                    } else {
-                        hi[e] = (T)y;
-                    }
+                    T p, q;
+                    split16(d[e >> 2][e & 3], p, q);
+                    hi[e] = p;
+                    lw[e] = q;
                 }
                 const s16x8 bh = __builtin_bit_cast(s16x8, hi);
 #pragma unroll
@@ -1331,10 +1332,8 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
                         return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
                     };
                     const s16x8 w = get(p);
-                    if constexpr (P == 2) {
-                        acc[i] = mfma(get(p + a.Vp * ND * 64), bh, acc[i], T());
-                        acc[i] = mfma(w, __builtin_bit_cast(s16x8, lw), acc[i], T());
-                    }
+                    if constexpr (P == 2) acc[i] = mfma(get(p + a.Vp * ND * 64), bh, acc[i], T());
+                    acc[i] = mfma(w, __builtin_bit_cast(s16x8, lw), acc[i], T());
                     acc[i] = mfma(w, bh, acc[i], T());
                 }
             }
@@ -1518,9 +1517,9 @@ __global__ __launch_bounds__(1024) void join_few_kernel(JoinArgs a) {
 // own, most of whose work would otherwise be dropped (a training step of 16 rows: 65536 classes of 1024 features, bf16, 127
 // us against 142; 1000 of 256, float32, 48 against 54).
 typedef Shape<128, 32, 4, 1> Thin;    // 32 along n
-Cut cut_of(long long M, long long N, long long K, int planes, bool grad) {      // grad: operands kM, sums may be split
-    return ds::cut_of([&](long long b) { return ((M + b - 1) / b) * ((N + b - 1) / b); }, (double)M * N, K,
-                      planes == 2 ? 3 : 1, grad, grad, cu_count());
+Cut cut_of(long long M, long long N, long long K, int pairs, bool grad) {      // grad: operands kM, sums may be split
+    return ds::cut_of([&](long long b) { return ((M + b - 1) / b) * ((N + b - 1) / b); }, (double)M * N, K, pairs, grad, grad,
+                      cu_count());
 }
 
 bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
@@ -1551,7 +1550,7 @@ Saved saved_of(void* p, long long N) {
 }
 
 struct Plan {
-    int planes, Dp, vt_fwd, piece, piece_ld, dh_splits, dw_splits;
+    int planes, dl_planes, Dp, vt_fwd, piece, piece_ld, dh_splits, dw_splits;
     bool stage_w, stage_h, dh_part;
     ShapeId fwd, dl_shape, dh, dw;
     int few, few_grid;                 // forward of few rows: rows a workgroup holds (0: not that path)
@@ -1599,6 +1598,13 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     p.slim_bytes = (int)bytes + Vp * 4;
     p.slim_grid = cdiv(N, 16 * (kSlimT / 64)) < 2 * cu_count() ? cdiv(N, 16 * (kSlimT / 64)) : 2 * cu_count();
     p.slim_back = p.slim && (long long)N * pad8(V) * (long long)el <= (1ll << 30);
+    // 16-bit inputs: one plane of dl makes the gradients' error against 64 bits 1.2 .. 1.5 times that of rounding them, and up to 2.2
+    // times for a few rows or classes (a row of 56, 3784 classes, bf16, 1.8; 483 rows of 56, 19229 classes, fp16, a twentieth kept,
+    // 1.5); two planes make it 1.0.  They are taken where the products are not the bound: up to 2^31 products of numbers (a second
+    // plane of 8192 x 65536 x 1024 would take six products for four, 5.8 ms for 4.0).  On chip dl is stored for dW alone, whose sums
+    // over 64 rows a class and more average its rounding out (1.0 .. 1.15; 368640 x 64, 512 classes, bf16 403 us, 626 with two).
+    p.dl_planes = p.planes == 2 ? 2 : (p.slim_back ? N < 64ll * V : (double)N * V * D <= 2147483648.0) ? 2 : 1;
+    const size_t el_dl = 2 * p.dl_planes;
     // rows of the caller's can be read as they are (a tile's byte offsets have 31 bits: 256 rows)
     const bool whole = D % 8 == 0 && ldh % 8 == 0 && dtype != DS_F32 && ldh <= (1 << 21);
     p.stage_h = !whole || (mode == kCE && !p.slim_back);
@@ -1606,7 +1612,8 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     const size_t h = align256((size_t)N * p.Dp * el), w = p.stage_w ? align256((size_t)V * p.Dp * el) : 0;
     // what the forward stages is kept for the backward (staging 50021 classes of 771 features once more: 35 of 490 us); few
     // rows are read as they are
-    p.fwd = thin ? kThin : cut_of(V, N, D, p.planes, false).shape;
+    const int pairs = p.planes == 2 ? 3 : 1;
+    p.fwd = thin ? kThin : cut_of(V, N, D, pairs, false).shape;
     p.vt_fwd = cdiv(V, side_of(p.fwd));
     size_t o = saved_bytes(N);
     p.sh = o; o += p.stage_h && !p.few ? h : 0;
@@ -1621,16 +1628,17 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     // a piece of the classes: about 256 MB of dl (64 MB: 16 % slower at 8192 x 65536 x 1024, 128 MB: 4 %, 512 MB: the same), at
     // least 1024 classes; pieces of one size, up to half larger where that saves one (6872 x 19619 x 496, bf16, in pieces of
     // 19456 and 163 classes 959 us, in two of 9856 761, in one 749)
-    const long long room = (256ll << 20) / ((long long)el * N), fit = room < 1024 ? 1024 : room;
+    const long long room = (256ll << 20) / ((long long)el_dl * N), fit = room < 1024 ? 1024 : room;
     const long long pieces = p.slim_back || V <= fit ? 1 : (V + fit / 2) / fit;
     p.piece = pieces == 1 ? V : (cdiv((long long)V, pieces) + 63) / 64 * 64;
     p.piece_ld = pad8(p.piece);
-    p.dl_shape = thin ? kThin : cut_of(p.piece, N, D, p.planes, false).shape;
+    p.dl_shape = thin ? kThin : cut_of(p.piece, N, D, pairs, false).shape;
     // The backward's logits must have the forward's bits: probabilities are exp(l - top), and where logits are large their
     // rounding is too.  All shapes add up in the same order, but the large one takes planes pair by pair.
     if (p.planes == 2 && (p.slim || (p.fwd == kBig) != (p.dl_shape == kBig)))
         p.dl_shape = !p.slim ? p.fwd : p.dl_shape == kBig ? kSq : p.dl_shape;
-    const Cut dh = cut_of(D, N, p.piece, p.planes, true), dw = cut_of(D, p.piece, N, p.planes, true);
+    const int gp = p.planes + p.dl_planes - 1;
+    const Cut dh = cut_of(D, N, p.piece, gp, true), dw = cut_of(D, p.piece, N, gp, true);
     p.dh = thin ? kThin : dh.shape;
     p.dh_splits = thin ? splits_for(cdiv(D, 128), cdiv(p.piece, kBK)) : dh.splits;
     p.dw = dw.shape;
@@ -1642,7 +1650,7 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     p.bw = o; o += p.few ? w : 0;
     p.bs = o; o += 256;
     p.hw = o; o += dtype == DS_BF16 || p.slim_back ? 0 : h;      // weighted rows for dW
-    p.dl = o; o += align256((size_t)N * p.piece_ld * el);
+    p.dl = o; o += align256((size_t)N * p.piece_ld * el_dl);
     p.dhp = o; o += p.dh_part ? align256((size_t)p.dh_splits * N * D4 * 4) : 0;
     p.dwp = o; o += p.dw_splits > 1 ? align256((size_t)p.dw_splits * p.piece * D4 * 4) : 0;
     p.own = o; o += p.few ? few_stats_bytes(p, N) : 0;
@@ -1928,6 +1936,8 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
     float* dhp = reinterpret_cast<float*>(ws + p.dhp);
     float* dwp = reinterpret_cast<float*>(ws + p.dwp);
     const long long lo = N * p.piece_ld;
+    constexpr int kTwo = SPLIT == 1 ? 2 : SPLIT;
+    const bool two = SPLIT == 1 && p.dl_planes == 2;
     const int D4 = (D + 3) & ~3;
     for (int v0 = 0; v0 < V; v0 += p.piece) {
         const int cols = V - v0 < p.piece ? V - v0 : p.piece, ld = pad8(cols);
@@ -1936,27 +1946,33 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
         Wp.outer = cols;
         if (p.slim_back) {
             const SlimArgs a = slim_args(p, H, W, s, rows, N, D, V, centers);
-            const SlimBwd o{bs, up, g_hidden, g_weight ? dl : nullptr, ld, lo, ignored, g_weight && p.pack ? ws + p.bh : nullptr, p.Dp};
+            const SlimBwd o{bs, up, g_hidden, g_weight ? dl : nullptr, ld, p.dl_planes, lo, ignored, g_weight && p.pack ? ws + p.bh : nullptr, p.Dp};
             const int rc = mode == kCE ? slim_bwd<T, SPLIT == 3 ? 2 : 1, kCE, IT>(p, a, o, q)
                                        : slim_bwd<T, SPLIT == 3 ? 2 : 1, kExpect, IT>(p, a, o, q);
             if (rc) return rc;
             if (p.pack) Hw = Operand{ws + p.bh, p.Dp, 0, (int)N, p.Dp};
         } else {
             const DlArgs da{v0, cols, s.shifts, s.tgt, centers, s.top, s.inv_sum, s.mean, up, dl, ld, lo};
-            if (mode == kCE)
-                dl_launch<T, SPLIT, kCE>(p, Wp, H, s, bs, N, D, da, q);
+            if (two)
+                mode == kCE ? dl_launch<T, kTwo, kCE>(p, Wp, H, s, bs, N, D, da, q) : dl_launch<T, kTwo, kExpect>(p, Wp, H, s, bs, N, D, da, q);
             else
-                dl_launch<T, SPLIT, kExpect>(p, Wp, H, s, bs, N, D, da, q);
+                mode == kCE ? dl_launch<T, SPLIT, kCE>(p, Wp, H, s, bs, N, D, da, q) : dl_launch<T, SPLIT, kExpect>(p, Wp, H, s, bs, N, D, da, q);
         }
         const Operand G{dl, ld, lo, (int)N, ld};
         if (g_hidden && !p.slim_back) {
             const GradArgs ga{D, cols, p.dh_splits, mode, cols, v0 == 0, rows, g_hidden, dhp, N * D4, up, false};
-            grad_launch<IT, T, SPLIT, 0>(p.dh, p.dh_part, Wp, G, s, bs, N, ga, q);
+            if (two)
+                grad_launch<IT, T, kTwo, 0>(p.dh, p.dh_part, Wp, G, s, bs, N, ga, q);
+            else
+                grad_launch<IT, T, SPLIT, 0>(p.dh, p.dh_part, Wp, G, s, bs, N, ga, q);
         }
         if (g_weight) {
             IT* gw = g_weight + (long long)v0 * D;
             const GradArgs ga{D, cols, p.dw_splits, mode, cols, 1, nullptr, gw, dwp, (long long)p.piece * D4, up, reach};
-            grad_launch<IT, T, SPLIT, 1>(p.dw, p.dw_splits > 1, Hw, G, s, bs, cols, ga, q);
+            if (two)
+                grad_launch<IT, T, kTwo, 1>(p.dw, p.dw_splits > 1, Hw, G, s, bs, cols, ga, q);
+            else
+                grad_launch<IT, T, SPLIT, 1>(p.dw, p.dw_splits > 1, Hw, G, s, bs, cols, ga, q);
             if (p.dw_splits > 8 && (long long)cols * D4 <= kShareOuts)
                 head_sum_kernel<T, SPLIT, IT, 16><<<cdiv((long long)cols * D4 / 4, 16), 256, 0, q>>>(
                     dwp, (long long)p.piece * D4, p.dw_splits, s.st, bs, cols, D, mode, 1, up, reach, nullptr, gw);

@@ -674,6 +674,29 @@ def test_pieces_with_a_row_of_nan(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("n,d,v", [(400, 64, 8), (777, 250, 128), (600, 120, 288), (3000, 64, 80), (500, 33, 289), (1, 56, 3784),
+                                   (2, 40, 500), (4, 250, 2000), (25, 1744, 1001), (483, 56, 19229), (5719, 64, 1232), (300, 515, 700),
+                                   (3000, 96, 7000)])
+def test_smaller_heads_round_once(n, d, v, dtype):
+    """16-bit heads of up to 2^31 products, on chip those of few rows a class: as float32 heads of the same values, and rounded once.
+    The logits' gradient is held in two planes, 2^-16 (bfloat16) of it or less is dropped."""
+    h, w, t, up, c = _data(n, d, v, dtype, seed=n + d + v, keep=0.8)
+    for got, k in ((_ce(h, w, t, "none", up), dict(t=t)), (_ex(h, w, c, up), dict(c=c))):
+        _, gh, gw, _, th, tw = _oracle(h.float(), w.float(), up=up, **k)
+        p = torch.softmax(h.double() @ w.double().T, 1)
+        if "t" in k:
+            dl = (p + torch.nn.functional.one_hot(t.clamp(min=0), v)) * (up * (t != -100)).double()[:, None]
+        else:
+            dl = p * (c.double()[None] - (p @ c.double())[:, None]).abs() * up.double()[:, None]
+        sub = 2.0 ** -24 if dtype == torch.float16 else 2.0 ** -133
+        _close(got[1], gh, th + 2.0 ** -16 * dl @ w.double().abs() + U[dtype] * gh.abs() + sub, "g_hidden")
+        live = torch.ones(n, dtype=torch.bool, device=DEV) if "c" in k else t != -100
+        _close(got[2], gw, tw + 2.0 ** -16 * dl.T @ torch.where(live[:, None], h, 0).double().abs() + U[dtype] * gw.abs() + sub,
+               "g_weight")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_several_pieces_with_rows_left_out(dtype):
     """70001 classes of 4000 rows: two pieces (four in float32), a smaller last one, rows left out, targets at the pieces' ends.  Cross
