@@ -79,9 +79,13 @@ _SIGNATURES = {
     "ds_linear_ce_workspace_bytes": (_sz, [_i, _ll, _i, _i, _ll, _i]),
     "ds_linear_ce_fwd": (_i, [_fp, _ll, _fp, _fp, _i, _ll, _i, _i, _ll, _i, _fp, _fp, _fp, _sz, _fp]),
     "ds_linear_ce_bwd": (_i, [_fp, _ll, _fp, _fp, _fp, _i, _ll, _i, _i, _ll, _i, _fp, _fp, _fp, _fp, _sz, _fp]),
+    "ds_linear_ce_eval_workspace_bytes": (_sz, [_i, _ll, _i, _i, _ll]),
+    "ds_linear_ce_eval": (_i, [_fp, _ll, _fp, _fp, _i, _ll, _i, _i, _ll, _i, _fp, _fp, _sz, _fp]),
     "ds_bin_expect_saved_bytes": (_sz, [_i, _ll, _i, _i, _ll]),
     "ds_bin_expect_workspace_bytes": (_sz, [_i, _ll, _i, _i, _ll, _i]),
     "ds_bin_expect_fwd": (_i, [_fp, _ll, _fp, _fp, _i, _ll, _i, _i, _fp, _fp, _fp, _sz, _fp]),
+    "ds_bin_expect_eval_workspace_bytes": (_sz, [_i, _ll, _i, _i, _ll]),
+    "ds_bin_expect_eval": (_i, [_fp, _ll, _fp, _fp, _i, _ll, _i, _i, _fp, _fp, _sz, _fp]),
     "ds_bin_expect_bwd": (_i, [_fp, _ll, _fp, _fp, _fp, _i, _ll, _i, _i, _fp, _fp, _fp, _fp, _sz, _fp]),
     "ds_orthogonalize_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "ds_orthogonalize_check": (_i, [_i, _i, _i, _i, _i, C.POINTER(C.c_double), C.c_double]),

@@ -1557,14 +1557,9 @@ struct Plan {
     int slim, slim_bytes, slim_grid;   // small head: k steps of 32 a row (0: not that path); backward: slim_back
     bool slim_back, pack;
     size_t sh, sw, saved_total;                                            // staged operands behind Saved (not of few rows)
-    size_t counts, tlogit, part, sums, fwd_total;                          // offsets of the forward's workspace
-    size_t bh, bw, bs, hw, dl, dhp, dwp, own, bwd_total;                   // offsets of the backward's
+    size_t counts, tlogit, part, sums, alone, fwd_total;                   // offsets of the forward's workspace
+    size_t bh, bs, hw, dl, dhp, dwp, bwd_total;                            // offsets of the backward's
 };
-// statistics that a backward of few rows forms itself: three planes of class tiles, then as Saved, the targets' logits, and the
-// outputs that nobody reads
-size_t few_stats_bytes(const Plan& p, long long N) {
-    return 3 * align256((size_t)p.vt_fwd * N * 4) + 5 * align256((size_t)N * 4);
-}
 
 int splits_for(long long tiles, long long steps) {
     // enough workgroups for two a CU, no split shorter than four steps of 64
@@ -1573,18 +1568,20 @@ int splits_for(long long tiles, long long steps) {
     return (int)(s < 1 ? 1 : (s > 256 ? 256 : s));
 }
 
-Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
+// alone: a forward that no backward follows
+Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh, bool alone = false) {
     Plan p;
     p.planes = dtype == DS_F32 ? 2 : 1;
     p.Dp = pad8(D);
     p.stage_w = dtype == DS_F32 || D % 8 != 0;
     const size_t el = 2 * p.planes;
     const bool thin = N <= 32;
-    // few rows of a weight that would have to be packed first (20000 classes of 256 features, float32, 1 / 4 / 8 rows: 18 / 30
-    // / 76 us here, 39 / 39 / 40 packed and multiplied); a 16-bit weight is read as it is by the matrix instructions as well
-    // (65536 of 1024, bf16: 39 / 70 / 177 us here, 36 / 36 / 39 there).  Their features have to fit LDS in fp32 beside three
-    // more workgroups.
-    p.few = N > kFewMax || !p.stage_w ? 0 : N <= 1 ? 1 : N <= 2 ? 2 : 4;
+    // Few rows of a weight that would have to be packed first (20000 classes of 256 features, float32, 1 / 2 / 4 rows: 18 / 22 / 31
+    // us here, 40 packed and multiplied; a 16-bit weight is read as it is by the matrix instructions as well: 65536 of 1024, bf16,
+    // 39 / 49 / 70 us here, 36 there).  Not where a backward follows: it needs the packed weight, and logits with the forward's
+    // bits, which these are not (the training step 92 us here with its statistics formed again, 77 all packed).  Their features
+    // have to fit LDS in fp32 beside three more workgroups.
+    p.few = !alone || N > kFewMax || !p.stage_w ? 0 : N <= 1 ? 1 : N <= 2 ? 2 : 4;
     if (p.few && (size_t)p.few * pad8(D) * 4 > 40 * 1024) p.few = 0;
     const int vec = dtype == DS_F32 ? 4 : 8, lanes = lanes_for(cdiv(D, vec));
     p.few_grid = cdiv(V, kFewT / lanes * 4) < 2 * cu_count() ? cdiv(V, kFewT / lanes * 4) : 2 * cu_count();
@@ -1610,8 +1607,7 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     p.stage_h = !whole || (mode == kCE && !p.slim_back);
     p.pack = whole && mode == kCE && p.slim_back;
     const size_t h = align256((size_t)N * p.Dp * el), w = p.stage_w ? align256((size_t)V * p.Dp * el) : 0;
-    // what the forward stages is kept for the backward (staging 50021 classes of 771 features once more: 35 of 490 us); few
-    // rows are read as they are
+    // what the forward stages is kept for the backward (staging 50021 classes of 771 features once more: 35 of 490 us)
     const int pairs = p.planes == 2 ? 3 : 1;
     p.fwd = thin ? kThin : cut_of(V, N, D, pairs, false).shape;
     p.vt_fwd = cdiv(V, side_of(p.fwd));
@@ -1624,6 +1620,7 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     p.tlogit = o; o += align256((size_t)N * 4);
     p.part = o; o += p.few ? align256((size_t)p.few_grid * p.few * 16) : p.slim ? 0 : 3 * align256((size_t)p.vt_fwd * N * 4);
     p.sums = o; o += align256((size_t)(cdiv(N, 32) > p.slim_grid ? cdiv(N, 32) : p.slim_grid) * 8);
+    p.alone = o; o += alone ? p.saved_total : 0;        // what would be saved
     p.fwd_total = o;
     // a piece of the classes: about 256 MB of dl (64 MB: 16 % slower at 8192 x 65536 x 1024, 128 MB: 4 %, 512 MB: the same), at
     // least 1024 classes; pieces of one size, up to half larger where that saves one (6872 x 19619 x 496, bf16, in pieces of
@@ -1646,14 +1643,12 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh) {
     p.dh_part = p.dh_splits > 1 || p.piece < V;
     const size_t D4 = (D + 3) & ~3;
     o = 0;
-    p.bh = o; o += (p.stage_h && p.few) || p.pack ? h : 0;
-    p.bw = o; o += p.few ? w : 0;
+    p.bh = o; o += p.pack ? h : 0;
     p.bs = o; o += 256;
     p.hw = o; o += dtype == DS_BF16 || p.slim_back ? 0 : h;      // weighted rows for dW
     p.dl = o; o += align256((size_t)N * p.piece_ld * el_dl);
     p.dhp = o; o += p.dh_part ? align256((size_t)p.dh_splits * N * D4 * 4) : 0;
     p.dwp = o; o += p.dw_splits > 1 ? align256((size_t)p.dw_splits * p.piece * D4 * 4) : 0;
-    p.own = o; o += p.few ? few_stats_bytes(p, N) : 0;
     p.bwd_total = o;
     return p;
 }
@@ -1878,16 +1873,13 @@ template <class IT, class T, int SPLIT>
 int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT* weight, const long long* target, const float* centers,
              const float* g, long long N, int D, int V, long long ignore, int reduction, void* saved, IT* g_hidden,
              IT* g_weight, char* ws, hipStream_t q) {
-    Saved s = saved_of(saved, N);
+    const Saved s = saved_of(saved, N);
     const int* rows = mode == kCE ? s.rows : nullptr;
     BackState* bs = reinterpret_cast<BackState*>(ws + p.bs);
     Upstream up{g, reduction == DS_REDUCE_NONE, reduction == DS_REDUCE_MEAN, rows};
-    // the forward of few rows stages nothing and leaves no scales; what a second backward of the same forward, maybe at the
-    // same time, finds there is what it forms itself
     Operand H, W;
-    char* staged = p.few ? ws : static_cast<char*>(saved);
-    operands<IT, T, SPLIT>(p, mode, hidden, ldh, weight, N, D, V, s, rows, p.few != 0, false, staged + (p.few ? p.bh : p.sh),
-                           staged + (p.few ? p.bw : p.sw), H, W, q);
+    char* keep = static_cast<char*>(saved);
+    operands<IT, T, SPLIT>(p, mode, hidden, ldh, weight, N, D, V, s, rows, false, false, keep + p.sh, keep + p.sw, H, W, q);
     // dW weighs rows where their upstream differs, and fp32's always; heads on chip weigh dl as they store it
     const bool fold = std::is_same<T, f16>::value && (up.each || SPLIT == 3) && g_weight && !p.slim_back;
     const bool reach = SPLIT == 3 || fold;
@@ -1900,20 +1892,6 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
         const int blocks = most <= kScaleAlone ? 1 : cdiv(most, 4 * kScaleT) < 256 ? cdiv(most, 4 * kScaleT) : 256;
         if (blocks > 1) back_init_kernel<<<1, 1, 0, q>>>(bs);
         back_scale_kernel<<<blocks, kScaleT, 0, q>>>(up, s.st, centers, V, f, bs);
-    }
-    if (p.few) {      // the forward formed its logits without the matrix instructions: these have other bits
-        float* part = reinterpret_cast<float*>(ws + p.own);
-        const long long plane = align256((size_t)p.vt_fwd * N * 4) / 4, n4 = align256((size_t)N * 4) / 4;
-        float* tlogit = part + 3 * plane;
-        s.top = tlogit + n4;
-        s.inv_sum = tlogit + 2 * n4;
-        s.mean = tlogit + 3 * n4;
-        const StatsArgs sa{V, s.shifts, s.tgt, centers, tlogit, part, plane, (int)N, 0};
-        if (mode == kCE)
-            stats_launch<T, SPLIT, kCE>(p, W, H, s, N, D, sa, q);
-        else
-            stats_launch<T, SPLIT, kExpect>(p, W, H, s, N, D, sa, q);
-        join_few_kernel<<<1, 1024, 0, q>>>(join_tiles(p, mode, s, sa, N, tlogit + 4 * n4, DS_REDUCE_NONE));
     }
     Ignored ignored{};
     if (mode == kCE && g_hidden) {
@@ -1999,16 +1977,18 @@ int by_type(int dtype, F32 f32, F16 h, BF16 b) {
     return dtype == DS_F32 ? f32() : dtype == DS_F16 ? h() : b();
 }
 
+// saved NULL: no backward follows
 int fwd_any(int mode, const void* hidden, long long ldh, const void* weight, const long long* target, const float* centers,
             int dtype, long long N, int D, int V, long long ignore, int reduction, float* out, void* saved, void* ws,
             size_t bytes, void* stream) {
-    if (!hidden || !weight || !saved || !out) return DS_ERR_INVALID_ARG;
+    if (!hidden || !weight || !out) return DS_ERR_INVALID_ARG;
     const int rc = check_sizes(dtype, N, D, V, ldh);
     if (rc) return rc;
-    const Plan p = plan_of(mode, dtype, N, D, V, ldh);
+    const Plan p = plan_of(mode, dtype, N, D, V, ldh, !saved);
     if (!ws || bytes < p.fwd_total || misaligned(ws) || misaligned(saved)) return DS_ERR_WORKSPACE;
     if ((!p.stage_w && misaligned(weight)) || (!p.stage_h && misaligned(hidden))) return DS_ERR_INVALID_ARG;
     char* w = static_cast<char*>(ws);
+    if (!saved) saved = w + p.alone;
     hipStream_t q = static_cast<hipStream_t>(stream);
 #define DS_GO(IT, T, SP)                                                                                                     \
     [&] {                                                                                                                    \
@@ -2057,8 +2037,18 @@ size_t ds_linear_ce_workspace_bytes(int dtype, long long N, int D, int V, long l
 int ds_linear_ce_fwd(const void* hidden, long long ldh, const void* weight, const long long* target, int dtype, long long N,
                      int D, int V, long long ignore_index, int reduction, float* loss, void* saved, void* workspace,
                      size_t workspace_bytes, void* stream) {
-    if (!target || reduction < DS_REDUCE_NONE || reduction > DS_REDUCE_MEAN) return DS_ERR_INVALID_ARG;
+    if (!target || !saved || reduction < DS_REDUCE_NONE || reduction > DS_REDUCE_MEAN) return DS_ERR_INVALID_ARG;
     return ds::fwd_any(ds::kCE, hidden, ldh, weight, target, nullptr, dtype, N, D, V, ignore_index, reduction, loss, saved,
+                       workspace, workspace_bytes, stream);
+}
+size_t ds_linear_ce_eval_workspace_bytes(int dtype, long long N, int D, int V, long long ldh) {
+    return ds::check_sizes(dtype, N, D, V, ldh) ? 0 : ds::plan_of(ds::kCE, dtype, N, D, V, ldh, true).fwd_total;
+}
+int ds_linear_ce_eval(const void* hidden, long long ldh, const void* weight, const long long* target, int dtype, long long N,
+                      int D, int V, long long ignore_index, int reduction, float* loss, void* workspace, size_t workspace_bytes,
+                      void* stream) {
+    if (!target || reduction < DS_REDUCE_NONE || reduction > DS_REDUCE_MEAN) return DS_ERR_INVALID_ARG;
+    return ds::fwd_any(ds::kCE, hidden, ldh, weight, target, nullptr, dtype, N, D, V, ignore_index, reduction, loss, nullptr,
                        workspace, workspace_bytes, stream);
 }
 int ds_linear_ce_bwd(const void* hidden, long long ldh, const void* weight, const long long* target, const float* g_loss,
@@ -2079,8 +2069,17 @@ size_t ds_bin_expect_workspace_bytes(int dtype, long long N, int D, int V, long 
 }
 int ds_bin_expect_fwd(const void* hidden, long long ldh, const void* weight, const float* centers, int dtype, long long N, int D,
                       int V, float* out, void* saved, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!centers) return DS_ERR_INVALID_ARG;
+    if (!centers || !saved) return DS_ERR_INVALID_ARG;
     return ds::fwd_any(ds::kExpect, hidden, ldh, weight, nullptr, centers, dtype, N, D, V, 0, DS_REDUCE_NONE, out, saved,
+                       workspace, workspace_bytes, stream);
+}
+size_t ds_bin_expect_eval_workspace_bytes(int dtype, long long N, int D, int V, long long ldh) {
+    return ds::check_sizes(dtype, N, D, V, ldh) ? 0 : ds::plan_of(ds::kExpect, dtype, N, D, V, ldh, true).fwd_total;
+}
+int ds_bin_expect_eval(const void* hidden, long long ldh, const void* weight, const float* centers, int dtype, long long N, int D,
+                       int V, float* out, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!centers) return DS_ERR_INVALID_ARG;
+    return ds::fwd_any(ds::kExpect, hidden, ldh, weight, nullptr, centers, dtype, N, D, V, 0, DS_REDUCE_NONE, out, nullptr,
                        workspace, workspace_bytes, stream);
 }
 int ds_bin_expect_bwd(const void* hidden, long long ldh, const void* weight, const float* centers, const float* g_out, int dtype,

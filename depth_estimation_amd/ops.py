@@ -646,9 +646,16 @@ def _scratch(nbytes: int, device) -> torch.Tensor:
 # what a call needs depends on sizes alone; asked for once per size (a small training step is bound by the host)
 @functools.lru_cache(maxsize=1024)
 def _head_bytes(op: str, code: int, n: int, d: int, v: int, ldh: int):
-    """bytes to save, of the forward's workspace and of the backward's"""
+    """bytes to save, of the workspaces of a forward, of its backward, and of a forward alone"""
     saved, ws = getattr(L.lib(), f"ds_{op}_saved_bytes"), getattr(L.lib(), f"ds_{op}_workspace_bytes")
-    return int(saved(code, n, d, v, ldh)), int(ws(code, n, d, v, ldh, 0)), int(ws(code, n, d, v, ldh, 1))
+    alone = getattr(L.lib(), f"ds_{op}_eval_workspace_bytes")
+    return (int(saved(code, n, d, v, ldh)), int(ws(code, n, d, v, ldh, 0)), int(ws(code, n, d, v, ldh, 1)),
+            int(alone(code, n, d, v, ldh)))
+
+
+def _trains(*ts):
+    """whether a backward may follow (what a Function's context knows does not say)"""
+    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in ts)
 
 
 _INT = 2 ** 31 - 1      # sizes and counts cross the C interface as int
@@ -696,7 +703,7 @@ _INTEGERS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 
 class _LinearCE(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, targets, ignore_index, reduction):
+    def forward(ctx, hidden, weight, targets, ignore_index, reduction, train):
         h, n, d, ldh, w = _head_args(hidden, weight)
         if not isinstance(targets, torch.Tensor) or targets.dtype not in _INTEGERS:
             raise RuntimeError("targets must be a tensor of integers")
@@ -708,17 +715,22 @@ class _LinearCE(torch.autograd.Function):
         v, lib, dev = w.shape[0], L.lib(), h.device
         code, red = L.DTYPES[h.dtype], _REDUCTIONS[reduction]
         out = torch.empty(targets.shape if red == 0 else (), dtype=torch.float32, device=dev)
-        keep, nb, _ = _head_bytes("linear_ce", code, n, d, v, ldh)
-        saved = _scratch(keep, dev)
+        keep, nb, _, alone = _head_bytes("linear_ce", code, n, d, v, ldh)
+        saved = _scratch(keep, dev) if train else None
         if n == 0:
             if red:
                 out.fill_(0.0 if red == 1 else float("nan"))
-        else:
+        elif train:
             ws = _scratch(nb, dev)
             L.check(lib.ds_linear_ce_fwd(h.data_ptr(), ldh, w.data_ptr(), t.data_ptr(), code, n, d, v, ignore_index, red,
                                          out.data_ptr(), saved.data_ptr(), ws.data_ptr(), nb, L.stream()), "ds_linear_ce_fwd")
-        ctx.save_for_backward(h, w, t, saved)
-        ctx.args = ldh, ignore_index, red, hidden.shape
+        else:
+            ws = _scratch(alone, dev)
+            L.check(lib.ds_linear_ce_eval(h.data_ptr(), ldh, w.data_ptr(), t.data_ptr(), code, n, d, v, ignore_index, red,
+                                          out.data_ptr(), ws.data_ptr(), alone, L.stream()), "ds_linear_ce_eval")
+        if train:
+            ctx.save_for_backward(h, w, t, saved)
+            ctx.args = ldh, ignore_index, red, hidden.shape
         return out
 
     @staticmethod
@@ -739,7 +751,7 @@ class _LinearCE(torch.autograd.Function):
             L.check(lib.ds_linear_ce_bwd(h.data_ptr(), ldh, w.data_ptr(), t.data_ptr(), g.data_ptr(), code, n, d, v,
                                          ignore_index, red, saved.data_ptr(), L.ptr(gh), L.ptr(gw), ws.data_ptr(), nb,
                                          L.stream()), "ds_linear_ce_bwd")
-        return gh if gh is None or len(shape) == 2 else gh.reshape(shape), gw, None, None, None
+        return gh if gh is None or len(shape) == 2 else gh.reshape(shape), gw, None, None, None, None
 
 
 def linear_cross_entropy(hidden, weight, targets, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
@@ -749,12 +761,12 @@ def linear_cross_entropy(hidden, weight, targets, ignore_index: int = -100, redu
         raise RuntimeError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
     if not -2 ** 63 <= int(ignore_index) < 2 ** 63:
         raise RuntimeError(f"ignore_index must be a 64-bit integer, got {ignore_index}")
-    return _LinearCE.apply(hidden, weight, targets, int(ignore_index), reduction)
+    return _LinearCE.apply(hidden, weight, targets, int(ignore_index), reduction, _trains(hidden, weight))
 
 
 class _BinExpect(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, centers):
+    def forward(ctx, hidden, weight, centers, train):
         h, n, d, ldh, w = _head_args(hidden, weight)
         c = L.dev_f32(centers, "centers")
         v, lib, dev, code = w.shape[0], L.lib(), h.device, L.DTYPES[h.dtype]
@@ -762,14 +774,19 @@ class _BinExpect(torch.autograd.Function):
             raise RuntimeError(f"centers must be ({v},), got {tuple(c.shape)}")
         L.same_device(h, c)
         out = torch.empty(hidden.shape[:-1], dtype=torch.float32, device=dev)
-        keep, nb, _ = _head_bytes("bin_expect", code, n, d, v, ldh)
-        saved = _scratch(keep, dev)
-        if n:
+        keep, nb, _, alone = _head_bytes("bin_expect", code, n, d, v, ldh)
+        saved = _scratch(keep, dev) if train else None
+        if n and train:
             ws = _scratch(nb, dev)
             L.check(lib.ds_bin_expect_fwd(h.data_ptr(), ldh, w.data_ptr(), c.data_ptr(), code, n, d, v, out.data_ptr(),
                                           saved.data_ptr(), ws.data_ptr(), nb, L.stream()), "ds_bin_expect_fwd")
-        ctx.save_for_backward(h, w, c, saved)
-        ctx.args = ldh, hidden.shape
+        elif n:
+            ws = _scratch(alone, dev)
+            L.check(lib.ds_bin_expect_eval(h.data_ptr(), ldh, w.data_ptr(), c.data_ptr(), code, n, d, v, out.data_ptr(),
+                                           ws.data_ptr(), alone, L.stream()), "ds_bin_expect_eval")
+        if train:
+            ctx.save_for_backward(h, w, c, saved)
+            ctx.args = ldh, hidden.shape
         return out
 
     @staticmethod
@@ -790,7 +807,7 @@ class _BinExpect(torch.autograd.Function):
             L.check(lib.ds_bin_expect_bwd(h.data_ptr(), ldh, w.data_ptr(), c.data_ptr(), g.data_ptr(), code, n, d, v,
                                           saved.data_ptr(), L.ptr(gh), L.ptr(gw), ws.data_ptr(), nb, L.stream()),
                     "ds_bin_expect_bwd")
-        return gh if gh is None or len(shape) == 2 else gh.reshape(shape), gw, None
+        return gh if gh is None or len(shape) == 2 else gh.reshape(shape), gw, None, None
 
 
 def bin_expectation(hidden, weight, centers) -> torch.Tensor:
@@ -798,7 +815,7 @@ def bin_expectation(hidden, weight, centers) -> torch.Tensor:
     differentiable w.r.t. hidden and weight."""
     if isinstance(centers, torch.Tensor) and centers.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("bin_expectation: gradient w.r.t. centers is not implemented (detach them)")
-    return _BinExpect.apply(hidden, weight, centers)
+    return _BinExpect.apply(hidden, weight, centers, _trains(hidden, weight))
 
 
 # ----------------------------------------------------------------------------------------------------

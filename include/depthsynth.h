@@ -312,6 +312,8 @@ int ds_ingest_depth_u16(const uint16_t* depth, int N, int H, int W, float* out, 
  * no multiple of 8, selected rows), which any number of backward passes read.  g_hidden (N,D) and g_weight (V,D),
  * contiguous, of type `dtype`; either may be NULL.  fp32 inputs: every product in three fp16 products of two planes (22
  * bits).  Results do not depend on scheduling: the same inputs give the same bits.
+ * ds_*_eval: a forward that no backward follows; nothing is saved, and up to four rows read the weight as it is (in fp32: the
+ * last bits may differ from ds_*_fwd's).
  * saved and workspace (ds_*_workspace_bytes(..., backward)) are 16-byte aligned; 0 bytes = sizes outside the limits above.
  * With D a multiple of 8 and 16-bit types, weight (and for ds_bin_expect_*, with ldh a multiple of 8, hidden) must be
  * 16-byte aligned; g_hidden and g_weight always. */
@@ -323,10 +325,17 @@ int ds_linear_ce_fwd(const void* hidden, long long ldh, const void* weight, cons
 int ds_linear_ce_bwd(const void* hidden, long long ldh, const void* weight, const long long* target, const float* g_loss,
                      int dtype, long long N, int D, int V, long long ignore_index, int reduction, const void* saved,
                      void* g_hidden, void* g_weight, void* workspace, size_t workspace_bytes, void* stream);
+size_t ds_linear_ce_eval_workspace_bytes(int dtype, long long N, int D, int V, long long ldh);
+int ds_linear_ce_eval(const void* hidden, long long ldh, const void* weight, const long long* target, int dtype, long long N,
+                      int D, int V, long long ignore_index, int reduction, float* loss, void* workspace, size_t workspace_bytes,
+                      void* stream);
 size_t ds_bin_expect_saved_bytes(int dtype, long long N, int D, int V, long long ldh);
 size_t ds_bin_expect_workspace_bytes(int dtype, long long N, int D, int V, long long ldh, int backward);
 int ds_bin_expect_fwd(const void* hidden, long long ldh, const void* weight, const float* centers, int dtype, long long N, int D,
                       int V, float* out, void* saved, void* workspace, size_t workspace_bytes, void* stream);
+size_t ds_bin_expect_eval_workspace_bytes(int dtype, long long N, int D, int V, long long ldh);
+int ds_bin_expect_eval(const void* hidden, long long ldh, const void* weight, const float* centers, int dtype, long long N, int D,
+                       int V, float* out, void* workspace, size_t workspace_bytes, void* stream);
 int ds_bin_expect_bwd(const void* hidden, long long ldh, const void* weight, const float* centers, const float* g_out, int dtype,
                       long long N, int D, int V, const void* saved, void* g_hidden, void* g_weight, void* workspace,
                       size_t workspace_bytes, void* stream);

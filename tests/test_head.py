@@ -780,6 +780,29 @@ def test_few_rows(n, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5, 33, 300])
+def test_answers_without_gradients(n, dtype):
+    """What a program that only answers gets: few rows of a weight that would have to be packed have kernels of their own."""
+    from depth_estimation_amd import metrics, synthesis
+    for d, v in ((37, 1001), (256, 700), (1300, 80), (10300, 33)):
+        h, w, t, up, c = _data(n, d, v, dtype, seed=n + d)
+        if n > 2:
+            t[1] = -100
+        out, _, _, tol, _, _ = _oracle(h, w, t=t, up=up)
+        _close(metrics.linear_cross_entropy(h, w, t, reduction="none"), out, tol, "loss")
+        total = out.sum()
+        _close(metrics.linear_cross_entropy(h, w, t, reduction="sum"), total, tol.sum() + 2.0 ** -23 * total.abs(), "sum")
+        exp, _, _, etol, _, _ = _oracle(h, w, c=c, up=up)
+        depth = synthesis.depth_from_bins(h, w, c)
+        _close(depth, exp, etol, "depth")
+        assert not depth.requires_grad
+        with torch.no_grad():
+            assert torch.equal(synthesis.depth_from_bins(h.clone().requires_grad_(True), w, c), depth)
+        _close(synthesis.depth_from_bins(h.clone().requires_grad_(True), w, c).detach(), exp, etol, "depth, with a gradient")
+
+
+@pytest.mark.gpu
 def test_rows_far_apart():
     """A row pitch of ten million bytes: 250 rows lie across more than 2^31 bytes."""
     from depth_estimation_amd import synthesis
@@ -810,6 +833,29 @@ def test_two_calls_at_once():
     for k in (0, 1):
         for ce, ex in got[k]:
             assert all(torch.equal(x, y) for x, y in zip(ce + ex, want[k][0] + want[k][1]))
+
+
+def test_refusals_of_answers_on_the_host():
+    """Every wrong argument of the C entries of a forward alone, before any launch."""
+    from depth_estimation_amd import _lib as L
+    if not os.path.exists(L.LIB_PATH):
+        pytest.skip("libdepthsynth.so not built (run __graft_entry__.build())")
+    lib, fake, big = L.lib(), 0x1000, 1 << 40
+
+    def ce(h=fake, ldh=64, w=fake, t=fake, dt=2, n=8, d=64, v=16, red=2, out=fake, ws=fake, nb=big):
+        return lib.ds_linear_ce_eval(h, ldh, w, t, dt, n, d, v, -100, red, out, ws, nb, None)
+
+    def ex(h=fake, w=fake, c=fake, dt=2, n=8, out=fake, ws=fake, nb=big):
+        return lib.ds_bin_expect_eval(h, 64, w, c, dt, n, 64, 16, out, ws, nb, None)
+
+    for rc, want in [(ce(h=None), -1), (ce(w=None), -1), (ce(t=None), -1), (ce(out=None), -1), (ce(n=0), -1), (ce(ldh=63), -1),
+                     (ce(red=3), -1), (ce(dt=3), -2), (ce(n=(1 << 24) + 1), -2), (ce(ws=None), -3), (ce(nb=64), -3),
+                     (ce(ws=fake + 4), -3), (ce(w=fake + 2), -1), (ex(h=None), -1), (ex(c=None), -1), (ex(out=None), -1), (ex(n=0), -1),
+                     (ex(dt=9), -2), (ex(nb=64), -3), (ex(h=fake + 2), -1)]:
+        assert rc == want
+    assert lib.ds_linear_ce_eval_workspace_bytes(2, 0, 64, 16, 64) == 0
+    assert lib.ds_bin_expect_eval_workspace_bytes(9, 8, 64, 16, 64) == 0
+    assert lib.ds_bin_expect_fwd(fake, 64, fake, fake, 2, 8, 64, 16, fake, None, fake, big, None) == -1
 
 
 def test_refusals_on_the_host():
