@@ -1513,9 +1513,10 @@ __global__ __launch_bounds__(1024) void join_few_kernel(JoinArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
-// Shapes: 256x256 outputs a workgroup (TileStream) for large products; 128x128, 64x64 and 32x32 below that; up to 32 rows have a shape of their
-// own, most of whose work would otherwise be dropped (a training step of 16 rows: 65536 classes of 1024 features, bf16, 127
-// us against 142; 1000 of 256, float32, 48 against 54).
+// Shapes: 256x256 outputs a workgroup (TileStream) for large products; 128x128, 64x64 and 32x32 below that.  Up to 32 rows of many
+// classes have a shape of their own: long tiles read the weight in long runs (training steps of 16 rows, 65536 classes of 1024
+// features, bf16, 137 us against 152 in the others; of 32 rows, 65536 of 256, float32, 141 / 183, 16000 of 64, bf16, 43 / 50, but
+// 4000 of 256 43 / 40 and 1000 of 256, float32, 54 / 47).
 typedef Shape<128, 32, 4, 1> Thin;    // 32 along n
 Cut cut_of(long long M, long long N, long long K, int pairs, bool grad) {      // grad: operands kM, sums may be split
     return ds::cut_of([&](long long b) { return ((M + b - 1) / b) * ((N + b - 1) / b); }, (double)M * N, K, pairs, grad, grad,
@@ -1575,7 +1576,7 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh, bool
     p.Dp = pad8(D);
     p.stage_w = dtype == DS_F32 || D % 8 != 0;
     const size_t el = 2 * p.planes;
-    const bool thin = N <= 32;
+    const bool thin = N <= 32 && V >= 16000;
     // Few rows of a weight that would have to be packed first (20000 classes of 256 features, float32, 1 / 2 / 4 rows: 18 / 22 / 31
     // us here, 40 packed and multiplied; a 16-bit weight is read as it is by the matrix instructions as well: 65536 of 1024, bf16,
     // 39 / 49 / 70 us here, 36 there).  Not where a backward follows: it needs the packed weight, and logits with the forward's
@@ -1586,12 +1587,14 @@ Plan plan_of(int mode, int dtype, long long N, int D, int V, long long ldh, bool
     const int vec = dtype == DS_F32 ? 4 : 8, lanes = lanes_for(cdiv(D, vec));
     p.few_grid = cdiv(V, kFewT / lanes * 4) < 2 * cu_count() ? cdiv(V, kFewT / lanes * 4) : 2 * cu_count();
     // small head: the weight in LDS, two workgroups a CU (training steps of 100000 rows, here / in tiles: 80 classes of 64
-    // features, bf16, 62 / 90 us; 576 of 64 133 / 190; 256 of 128 109 / 134; 128 of 250 142 / 139, forward 49 / 51; 288 of 64,
-    // float32, 170 / 224)
+    // features, bf16, 65 / 101 us; 576 of 64 141 / 188; 256 of 128 120 / 135; 128 of 250 144 / 141, forward 48 / 52; 288 of 64,
+    // float32, 150 / 219).  Every workgroup brings the whole weight, which does not pay for a few rows of a large one (576 of 64,
+    // bf16: 300 rows 49 / 39, 3000 57 / 51, 8000 67 / 68, 20000 72 / 85; 288 of 64, float32: 1000 51 / 47, 8000 64 / 74; but 80 of 64,
+    // bf16: 300 30 / 35)
     const int Vp = (V + 31) & ~31;
     p.slim = D <= 64 ? 2 : D <= 128 ? 4 : D <= 256 ? 8 : 0;
     const long long bytes = (long long)Vp * p.slim * 64 * p.planes;
-    if (bytes + Vp * 4 > 78 * 1024) p.slim = 0;
+    if (bytes + Vp * 4 > 78 * 1024 || (bytes > 40 * 1024 && N < 6144)) p.slim = 0;
     p.slim_bytes = (int)bytes + Vp * 4;
     p.slim_grid = cdiv(N, 16 * (kSlimT / 64)) < 2 * cu_count() ? cdiv(N, 16 * (kSlimT / 64)) : 2 * cu_count();
     p.slim_back = p.slim && (long long)N * pad8(V) * (long long)el <= (1ll << 30);

@@ -781,6 +781,32 @@ def test_few_rows(n, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,d,v", [(1, 64, 16384), (8, 37, 16000), (32, 72, 16001), (16, 40, 15999), (32, 200, 17000)])
+def test_few_rows_of_many_classes(n, d, v, dtype):
+    """Around where up to 32 rows take a shape of their own."""
+    h, w, t, up, c = _data(n, d, v, dtype, seed=n + v, keep=0.8 if n > 1 else 1.0)
+    for got, (out, gh, gw, tol, th, tw) in ((_ce(h, w, t, "none", up), _oracle(h, w, t=t, up=up)),
+                                            (_ex(h, w, c, up), _oracle(h, w, c=c, up=up))):
+        _close(got[0], out, tol, "output")
+        _close(got[1], gh, th, "g_hidden")
+        _close(got[2], gw, tw, "g_weight")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,d,v", [(6143, 64, 560), (6144, 64, 560), (6500, 120, 288), (6500, 250, 128), (6200, 33, 289)])
+def test_heads_on_chip_with_large_weights(n, d, v, dtype):
+    """Around where a head whose weight takes more than 40 KB is held on chip."""
+    h, w, t, up, c = _data(n, d, v, dtype, seed=n + v, keep=0.7)
+    for got, (out, gh, gw, tol, th, tw) in ((_ce(h, w, t, "none", up), _oracle(h, w, t=t, up=up)),
+                                            (_ex(h, w, c, up), _oracle(h, w, c=c, up=up))):
+        _close(got[0], out, tol, "output")
+        _close(got[1], gh, th, "g_hidden")
+        _close(got[2], gw, tw, "g_weight")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("n", [1, 2, 3, 4, 5, 33, 300])
 def test_answers_without_gradients(n, dtype):
     """What a program that only answers gets: few rows of a weight that would have to be packed have kernels of their own."""
