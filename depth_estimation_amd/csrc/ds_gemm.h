@@ -132,8 +132,8 @@ struct Fragments {
 // `lds`.  A step brings all planes of both operands and adds its products from them, so that each plane is moved once and a
 // step's latency is covered by up to three products.  128 x 128 tiles then keep one step in LDS (the next one
 // waits in registers), which leaves room for two workgroups a CU.  Eight waves a 128 x 128 tile, two a SIMD, so that one's
-// LDS reads run beside the other's products: 512 x 4608 x 512 of two planes 15.1 us, 17.5 with four waves; two buffers or
-// loads two steps ahead gained nothing.
+// LDS reads run beside the other's products: 512 x 4608 x 512 of two planes, within an update, 18.6 us, 21.2 with four waves;
+// two buffers or loads two steps ahead gained nothing.
 template <class S, int PA, int PB>
 constexpr int lds_buffers() { return PA + PB > 2 && S::BM * S::BN > 64 * 128 ? 1 : 2; }
 template <class S, int PA, int PB>

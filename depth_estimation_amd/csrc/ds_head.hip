@@ -10,7 +10,7 @@
 // Forward: a workgroup forms a tile of l in registers and leaves three numbers per row and class tile (maximum, sum of
 // exponentials, sum of exponentials times centres); a second launch joins the tiles of a row.  Backward: per piece of the
 // classes, the tile is formed again, turned into dl with the saved maximum and sum and written once in 16 bits (two planes for fp32
-// inputs); the two products read it in place, one as kK, one as kM operand.
+// inputs and for smaller 16-bit heads); the two products read it in place, one as kK, one as kM operand.
 //
 // Rows whose target is ignore_index take no part: the kept rows are listed first (in order, so results do not depend on
 // scheduling), everything after works on that list, and how long it is stays on the device.
@@ -71,7 +71,7 @@ __global__ void head_init_kernel(HeadState* st, int rows) {
 }
 
 // Up to four workgroups count what comes before them themselves: a launch (3 us of the host's time) less, and no slower (61440
-// rows: 13.9 us, against 7.0 and 6.4 in two launches; every further workgroup waits for 2 us more).
+// rows: 15 us, against 7.3 and 7.7 in two launches; every further workgroup waits for 2 us more).
 constexpr int kListAlone = 4;
 
 // rows kept per 16384 (only launched for more workgroups than that)
@@ -967,8 +967,8 @@ __global__ __launch_bounds__(S::T) void head_grad_kernel(Operand A, Operand B, c
 
 // sums the splits of a product in order, scales, and writes rows of the caller.  which: 0 = dH, 1 = dW.  PAR lanes share the
 // splits of an output (each a contiguous share, joined in order), for products of few outputs and many splits.
-// (16 of them: 80 x 64 outputs of 100000 rows 62 us a step against 83, 256 x 128 of 20000 56 against 61, 600 x 256 200 against
-// 196.)
+// (16 of them: 80 x 64 outputs of 100000 rows 66 us a step against 84, 256 x 128 of 20000 57 against 60, 600 x 256 199 against
+// 198.)
 constexpr long long kShareOuts = 1 << 17;
 template <class T, int SPLIT, class O, int PAR>
 __global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__ part, long long part_split, int splits,
@@ -1053,7 +1053,8 @@ __global__ __launch_bounds__(256) void zero_ignored_kernel(Ignored g, int D, con
 // dH = dl W as it stands (its lanes hold rows, its registers classes, taken as k in the order 4 q + e of two fragments; the
 // transposing LDS reads of W follow that order), so dH needs no second pass; dl itself is written once for dW.  dH takes two
 // planes of dl, straight from registers, whatever the inputs' type.
-//   12 x 96 x 320 rows, 64 features, 80 bins, bf16, forward 20 us (47 MB of features; the tiles above: 48)
+//   12 x 96 x 320 rows, 64 features, 80 bins, bf16, forward 18 us (47 MB of features; the tiles above: 48).  By its counters the
+//   vector instructions are what it takes: 88 % of a busy CU's time, LDS 24 %, matrix instructions 12 %.
 constexpr int kSlimT = 512;
 struct SlimArgs {
     const void* h;             // features: the caller's rows, or staged ones

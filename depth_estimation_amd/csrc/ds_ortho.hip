@@ -416,7 +416,7 @@ __global__ __launch_bounds__(S::T) void ortho_finish_kernel(ProductArgs p, UseAr
 // X (small side s first, so a tall matrix is held transposed) and A, later B in its place, stay in LDS as two planes each;
 // rows are padded to a multiple of 32 with zeros and by 8 elements more, which spreads the fragment reads over the banks.
 // A wave forms fragments (16 x 16) of the products in registers; a result replaces its operand behind a barrier.  What bounds
-// it is the latency of the chain norm -> 3 products a step -> store: 64 x 147 in 5 steps 32 us (71 as 17 launches).
+// it is the latency of the chain norm -> 3 products a step -> store: 64 x 147 in 5 steps 33 us (71 as 17 launches).
 constexpr int kSmallT = 512;
 
 struct SmallPlan {
@@ -751,8 +751,9 @@ OrthoPlan ortho_plan(int dtype, int batch, int m, int n, bool light) {      // l
     p.sp = pad8(p.s);
     p.np = pad8(n);
     p.blocks = norm_blocks((long long)m * n);
-    // on smaller sides launches and latency are what a step takes, not products (five steps of 256 x 1024: 149 us so, 145
-    // with all planes; 512 x 512 150 and 166, 1024 x 1024 229 and 254, 2048 x 2048 505 and 759)
+    // on smaller sides launches and latency are what a step takes, more than products (five steps of 256 x 1024: 116 us so, 105
+    // with all planes; 128 x 4608 121 and 120, 300 x 1100 130 and 122, 384 x 4608 174 and 186; 512 x 512 119 and 126, 512 x 4608
+    // 215 and 230, 1024 x 1024 205 and 252, 2048 x 2048 498 and 735)
     p.light = light && dtype == DS_BF16 && p.s >= 512;
     auto cut = [&](int M, int N, int K, int pairs, bool tri, bool strided) {
         return cut_of(

@@ -2,7 +2,8 @@
 
 A weight matrix (a linear layer; a convolution as (out, in*kh*kw)) is stepped along its momentum with the singular values
 taken out by Newton-Schulz products (HIP kernels, ds_orthogonalize); biases and other vectors stay with torch.optim.Adam, as
-the reference steps everything (train.py:140).  Not in the reference.
+the reference steps everything (train.py:140).  Not in the reference.  The method and the coefficients are published: Muon, K.
+Jordan and others, 2024.
 """
 from __future__ import annotations
 
