@@ -42,10 +42,14 @@ struct HeadState {
         int most, pad[31];          // max over staged rows of the exponent above their largest feature (cross entropy)
     } reach[kReach];
 };
+struct Centers {
+    unsigned most;       // bits of max |centre|
+    int signs;           // 1: some are positive, 2: some are negative
+};
 struct BackState {
     int most;            // the largest exponent that a kept row takes part in dW with (kNone: no row does)
-    unsigned cmax;       // bits of max |centre|
-    int pad[14];
+    Centers centers;
+    int pad[13];
 };
 
 
@@ -603,7 +607,7 @@ __global__ __launch_bounds__(256) void loss_total_kernel(const double* __restric
 
 // ----------------------------------------------------------------------------------------------------------- backward
 // How dl is scaled: fp16 storage wants values of a fixed size, so a row of dl is kept as 2^14 dl / 2^e, where 2^e is above the
-// row's upstream value, times the largest |c - E| for the expectation; dH's rows are scaled back one by one, so that a row keeps
+// row's upstream value, times the row's p |c - E| for the expectation; dH's rows are scaled back one by one, so that a row keeps
 // its digits whatever the others' upstream is.  dW adds rows up, weighted with 2^e, and what is lost there is 2^-39 of the largest
 // row's part.  bf16 has fp32's range and takes dl as it is.  All powers of two are exponents, for ldexpf: upstreams of 1e38 or
 // 1e-38 are in range.
@@ -615,30 +619,36 @@ struct Upstream {
     const float* g;      // one value, or one per row of the caller
     int each, mean;
     const int* rows;     // caller's row of a kept row (NULL: the same)
+    const float* expect; // E of a kept row (NULL: cross entropy)
 };
 __device__ __forceinline__ float upstream(const Upstream& u, int n, int cnt) {
     if (u.each) return u.g[u.rows ? u.rows[n] : n];
     return u.mean ? u.g[0] / cnt : u.g[0];
 }
-// |c - E| < 2^e; as a factor 2^-e of the centres (in float32's normal range)
-__device__ __forceinline__ int center_exp(const BackState* bs) {
-    const int e = exp_above(from_bits(bs->cmax)) + 1;
-    return e < -125 ? -125 : (e > 126 ? 126 : e);
+// p |c - E| < 2^e.  Centres of one sign: it is at most |E|, however far the largest centre is (a bin of 1e9 for "no depth" takes no
+// digits from rows that are sure of another); else twice the largest.  As a factor 2^-e of the centres in float32's normal range,
+// which leaves them below 2^100.
+__device__ __forceinline__ int center_exp(const Centers& c, float E) {
+    const int top = exp_above(from_bits(c.most)) + 1, own = c.signs == 3 ? top : max(exp_above(fabsf(E)) + 1, top - 100);
+    return own < -125 ? -125 : (own > 126 ? 126 : own);
 }
-// exponent e of a row's upstream value, 0 where T needs none
+__device__ __forceinline__ int row_exp_of(const Upstream& u, const Centers& c, int n, float g) {
+    return exp_above(fabsf(g)) + (u.expect ? center_exp(c, u.expect[n]) : 0);
+}
+// exponent e of a row: its upstream value's (g) and its centres', 0 where T needs none
 template <class T>
-__device__ __forceinline__ int row_exp(float g) { return std::is_same<T, bf16>::value ? 0 : exp_above(fabsf(g)); }
+__device__ __forceinline__ int row_exp(const Upstream& u, const BackState* bs, int n, float g) {
+    return std::is_same<T, bf16>::value ? 0 : row_exp_of(u, u.expect ? bs->centers : Centers{0, 0}, n, g);
+}
 // exponent of a row of stored dl -> dl: this and the row's
 template <class T>
-__device__ __forceinline__ int dl_exp(const BackState* bs, int mode) {
-    return std::is_same<T, bf16>::value ? 0 : (mode == kExpect ? center_exp(bs) : 0) - kDlTop;
-}
-// What a row weighs in dW.  A product there is dl_r h_r; dl is stored under the row's upstream exponent e, features of fp32
+constexpr int kDlExp = std::is_same<T, bf16>::value ? 0 : -kDlTop;
+// What a row weighs in dW.  A product there is dl_r h_r; dl is stored under the row's exponent e, features of fp32
 // under the row's own shift, so that a row takes part with 2^(e + 15 - shift), and that is brought to 2^most by the weight, at
-// most 1 (most: the largest of the sums e + 15 - shift, or of e where features have one size for all, `reach` false).  Rows
+// most 1 (most: the largest of the sums e + 15 - shift, or of e where features have one size for all, `reach` 0).  Rows
 // without a gradient are left as they are.
-__device__ __forceinline__ int weight_exp(float g, int reach, int most) {
-    return g != 0.f && __builtin_isfinite(g) && most > kNone ? exp_above(fabsf(g)) + reach - most : 0;
+__device__ __forceinline__ int weight_exp(float g, int e, int reach, int most) {
+    return g != 0.f && __builtin_isfinite(g) && most > kNone ? e + reach - most : 0;
 }
 // the largest exponent that a row takes part with.  SPLIT 3: always with its features' reach
 template <class T, int SPLIT>
@@ -648,23 +658,21 @@ __device__ __forceinline__ int most_of(const HeadState* st, const BackState* bs,
     int r = SPLIT == 3 ? kNone : 0;
     if (SPLIT == 3)
         for (int i = 0; i < kReach; ++i) r = max(r, st->reach[i].most);
-    return r == kNone ? kNone : r + row_exp<T>(upstream(u, 0, cnt));
+    return r == kNone ? kNone : r + exp_above(fabsf(upstream(u, 0, cnt)));
 }
 // exponent of sums over rows -> dW
 template <class T, int SPLIT>
-__device__ __forceinline__ int dw_exp(const HeadState* st, const BackState* bs, const Upstream& u, int mode, int cnt, bool reach) {
+__device__ __forceinline__ int dw_exp(const HeadState* st, const BackState* bs, const Upstream& u, int cnt, bool reach) {
     if (std::is_same<T, bf16>::value) return 0;
     const int most = most_of<T, SPLIT>(st, bs, u, cnt);
-    return dl_exp<T>(bs, mode) + (most == kNone ? 0 : most) - (reach ? kReachTop : 0);
+    return kDlExp<T> + (most == kNone ? 0 : most) - (reach ? kReachTop : 0);
 }
 
 // bs->most (with the rows' shifts, or of float16 rows that lie as the caller left them the features themselves, where rows weigh
-// with their reach) and the largest |centre|, for upstreams that differ; *bs set by back_init_kernel before, unless one workgroup does it all (a launch less)
+// with their reach) and the centres' size and signs, which every workgroup finds for itself; for upstreams that differ.  *bs is
+// set by back_init_kernel before, unless one workgroup does it all (a launch less).
 constexpr int kScaleT = 512, kScaleAlone = 16 * kScaleT;
-__global__ void back_init_kernel(BackState* bs) {
-    bs->most = kNone;
-    bs->cmax = 0;
-}
+__global__ void back_init_kernel(BackState* bs) { bs->most = kNone; }
 struct Features {
     const int* shifts;   // of staged rows
     const f16* h;        // both NULL: not asked for
@@ -676,13 +684,37 @@ __global__ __launch_bounds__(kScaleT) void back_scale_kernel(Upstream u, const H
                                                              const float* __restrict__ centers, int V, Features f,
                                                              BackState* __restrict__ bs) {
     __shared__ float red[kScaleT / 64];
-    __shared__ int top[kScaleT / 64];
+    __shared__ int top[kScaleT / 64], sign[kScaleT / 64];
     const int cnt = st->count, step = gridDim.x * kScaleT, i0 = blockIdx.x * kScaleT + threadIdx.x;
     const int lane = threadIdx.x & 63;
-    float c = 0.f;
+    Centers all{0, 0};
+    if (centers) {
+        float c = 0.f;
+        int signs = 0;
+#pragma unroll 4
+        for (int v = threadIdx.x; v < V; v += kScaleT) {
+            const float x = centers[v];
+            c = fmaxf(c, finite_abs(x));
+            signs |= x > 0.f ? 1 : x < 0.f ? 2 : 0;
+        }
+        c = wave_max(c);
+        signs = (__ballot(signs & 1) ? 1 : 0) | (__ballot(signs & 2) ? 2 : 0);
+        if (lane == 0) {
+            red[threadIdx.x >> 6] = c;
+            sign[threadIdx.x >> 6] = signs;
+        }
+        __syncthreads();
+        for (int i = 0; i < kScaleT / 64; ++i) {
+            c = fmaxf(c, red[i]);
+            signs |= sign[i];
+        }
+        all = Centers{__builtin_bit_cast(unsigned, c), signs};
+        if (blockIdx.x == 0 && threadIdx.x == 0) bs->centers = all;
+    }
     int most = kNone;
-    auto take = [&](float g, int more) {
-        if (g != 0.f && __builtin_isfinite(g)) most = max(most, exp_above(fabsf(g)) + more);
+    auto take = [&](int n, int more) {
+        const float g = upstream(u, n, cnt);
+        if (g != 0.f && __builtin_isfinite(g)) most = max(most, row_exp_of(u, all, n, g) + more);
     };
     if (f.h) {
         const int sub = lane & (f.L - 1), R = 64 / f.L;
@@ -696,35 +728,22 @@ __global__ __launch_bounds__(kScaleT) void back_scale_kernel(Upstream u, const H
                 for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_abs((float)x[e]));
             }
             for (int o = 1; o < f.L; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-            if (m > 0.f) take(upstream(u, n, cnt), exp_above(m));
+            if (m > 0.f) take(n, exp_above(m));
         }
     } else {
 #pragma unroll 4
-        for (int n = i0; n < cnt; n += step) take(upstream(u, n, cnt), f.shifts ? kReachTop - f.shifts[n] : 0);
+        for (int n = i0; n < cnt; n += step) take(n, f.shifts ? kReachTop - f.shifts[n] : 0);
     }
-    if (centers)
-#pragma unroll 4
-        for (int v = i0; v < V; v += step) c = fmaxf(c, finite_abs(centers[v]));
-    c = wave_max(c);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
-    if (lane == 0) {
-        red[threadIdx.x >> 6] = c;
-        top[threadIdx.x >> 6] = most;
-    }
+    if (lane == 0) top[threadIdx.x >> 6] = most;
     __syncthreads();
     if (threadIdx.x != 0) return;
-    for (int i = 1; i < kScaleT / 64; ++i) {
-        c = fmaxf(c, red[i]);
-        most = max(most, top[i]);
-    }
-    if (gridDim.x == 1) {
+    for (int i = 1; i < kScaleT / 64; ++i) most = max(most, top[i]);
+    if (gridDim.x == 1)
         bs->most = most;
-        bs->cmax = __builtin_bit_cast(unsigned, c);
-    } else {
-        if (most > kNone) atomicMax(&bs->most, most);
-        if (c > 0.f) atomicMax(&bs->cmax, __builtin_bit_cast(unsigned, c));
-    }
+    else if (most > kNone)
+        atomicMax(&bs->most, most);
 }
 
 // The features of kept rows times 2^weight_exp, for dW, whose other operand holds every row of dl at full size (float16: from
@@ -738,7 +757,8 @@ __global__ __launch_bounds__(256) void fold_rows_kernel(Operand H, const int* __
     const long long all = (long long)cnt * q;
     for (long long i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
         const int n = (int)(i / q), d = (int)(i - (long long)n * q) * 8;
-        const int e = weight_exp(upstream(u, n, cnt), kReachTop - (SPLIT == 3 ? shifts[n] : 0), most);
+        const float g = upstream(u, n, cnt);
+        const int e = weight_exp(g, row_exp<f16>(u, bs, n, g), kReachTop - (SPLIT == 3 ? shifts[n] : 0), most);
 #pragma unroll
         for (int p = 0; p < (SPLIT == 3 ? 2 : 1); ++p) {
             f16x8 x = *reinterpret_cast<const f16x8*>(static_cast<const f16*>(H.p) + n * H.ld + d + p * H.lo);
@@ -769,7 +789,8 @@ template <class T, class S, int SPLIT, int MODE>
 __device__ __forceinline__ void dl_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int cnt, const HeadState* st,
                                            const BackState* bs, const DlArgs& a) {
     const int ws = SPLIT == 3 ? weight_shift(st) : 0;
-    const float cs = MODE == kExpect && !std::is_same<T, bf16>::value ? ldexpf(1.f, -center_exp(bs)) : 1.f;
+    constexpr bool kScaled = !std::is_same<T, bf16>::value;
+    const Centers all = MODE == kExpect && kScaled ? bs->centers : Centers{0, 0};
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / S::WN, wn = wave % S::WN, c0 = m0 + wm * S::FM * 16 + (lane >> 4) * 4;
     T* dl = static_cast<T*>(a.dl);
@@ -781,7 +802,7 @@ __device__ __forceinline__ void dl_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, i
         const float tp = a.top[n], rs = a.inv_sum[n];
         const int shift = SPLIT == 3 ? -ws - a.shifts[n] : 0;
         float g = upstream(a.up, n, cnt);
-        if (!std::is_same<T, bf16>::value) g = ldexpf(g, kDlTop - row_exp<T>(g));
+        if (kScaled) g = ldexpf(g, kDlTop - exp_above(fabsf(g)));
         if (MODE == kCE) {
             const int t = a.tgt[n] - a.v0 - c0;
             if (a.tgt[n] < 0) g = __builtin_nanf("");
@@ -795,7 +816,8 @@ __device__ __forceinline__ void dl_of_tile(f32x4 (&acc)[S::FM][S::FN], int m0, i
                     acc[i][j][e] = fmaf(x, gr, t == i * 16 + e ? -g : 0.f);
                 }
         } else {
-            const float e0 = a.mean[n] * cs, gr = g * rs;      // (cs: a power of two, exact)
+            const float cs = kScaled ? ldexpf(1.f, -center_exp(all, a.mean[n])) : 1.f;      // (a power of two: exact)
+            const float e0 = a.mean[n] * cs, gr = g * rs;
 #pragma unroll
             for (int i = 0; i < S::FM; ++i)
 #pragma unroll
@@ -875,7 +897,7 @@ __global__ __launch_bounds__(Big::T) void head_dl_big_kernel(Operand W, Operand 
 // what earlier pieces of the classes left; otherwise straight into the caller's rows.
 // dW of one piece = dl^T H: features along m, classes along n, k = rows (both kM operands).
 struct GradArgs {
-    int D, k, splits, mode;      // k: classes of the piece (dH); cols: classes of the piece (dW, whose k is the row count)
+    int D, k, splits;            // k: classes of the piece (dH); cols: classes of the piece (dW, whose k is the row count)
     int cols, first;
     const int* rows;
     void* out;
@@ -889,8 +911,7 @@ template <class T, class S, int SPLIT, class O, bool ACC, int WHICH>
 __device__ __forceinline__ void grad_of_tile(const f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int sp, int bound,
                                              const HeadState* st, const BackState* bs, const GradArgs& a) {
     const int cnt = st->count;
-    const int all = WHICH == 0 ? dl_exp<T>(bs, a.mode) - (SPLIT == 3 ? weight_shift(st) : 0)
-                               : dw_exp<T, SPLIT>(st, bs, a.up, a.mode, cnt, a.reach);
+    const int all = WHICH == 0 ? kDlExp<T> - (SPLIT == 3 ? weight_shift(st) : 0) : dw_exp<T, SPLIT>(st, bs, a.up, cnt, a.reach);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / S::WN, wn = wave % S::WN, Dp = (a.D + 3) & ~3;
 #pragma unroll
@@ -898,7 +919,7 @@ __device__ __forceinline__ void grad_of_tile(const f32x4 (&acc)[S::FM][S::FN], i
         const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
         if (n >= bound) continue;
         const long long row = !ACC && WHICH == 0 && a.rows ? a.rows[n] : n;
-        const int back = !ACC && WHICH == 0 ? all + row_exp<T>(upstream(a.up, n, cnt)) : all;
+        const int back = !ACC && WHICH == 0 ? all + row_exp<T>(a.up, bs, n, upstream(a.up, n, cnt)) : all;
         if (ACC) {
 #pragma unroll
             for (int i = 0; i < S::FM; ++i) {
@@ -973,13 +994,12 @@ constexpr long long kShareOuts = 1 << 17;
 template <class T, int SPLIT, class O, int PAR>
 __global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__ part, long long part_split, int splits,
                                                        const HeadState* __restrict__ st, const BackState* __restrict__ bs, int n,
-                                                       int D, int mode, int which, Upstream up, bool reach,
+                                                       int D, int which, Upstream up, bool reach,
                                                        const int* __restrict__ rows, O* __restrict__ out) {
     constexpr int kOuts = 256 / PAR;
     __shared__ f32x4 red[PAR][kOuts + 1];
     const int cnt = which == 0 ? st->count : n, Dp = (D + 3) & ~3, q = Dp / 4;
-    const int same = which == 0 ? dl_exp<T>(bs, mode) - (SPLIT == 3 ? weight_shift(st) : 0)
-                                : dw_exp<T, SPLIT>(st, bs, up, mode, st->count, reach);
+    const int same = which == 0 ? kDlExp<T> - (SPLIT == 3 ? weight_shift(st) : 0) : dw_exp<T, SPLIT>(st, bs, up, st->count, reach);
     const long long all = (long long)cnt * q;
     const int x = threadIdx.x % kOuts, y = threadIdx.x / kOuts, per = (splits + PAR - 1) / PAR;
     for (long long i0 = (long long)blockIdx.x * kOuts; i0 < all; i0 += (long long)gridDim.x * kOuts) {
@@ -1002,7 +1022,7 @@ __global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__
         if (i < all && y == 0) {
             const long long r = i / q;
             const int d = (int)(i - r * q) * 4;
-            a = scaled(a, which == 0 ? same + row_exp<T>(upstream(up, (int)r, cnt)) : same);
+            a = scaled(a, which == 0 ? same + row_exp<T>(up, bs, (int)r, upstream(up, (int)r, cnt)) : same);
             const float v[4] = {a[0], a[1], a[2], a[3]};
             put_row4(out + (rows && which == 0 ? (long long)rows[r] : r) * D, d, D, v);
         }
@@ -1258,9 +1278,10 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
     SlimRows<P, ND> next;
     if (b < blocks) next.load(a, b * 16 + (lane & 15), cnt, lane);
     slim_load_w<P, ND>(a, lds);
-    const int ws = P == 2 ? weight_shift(a.st) : 0, same = dl_exp<T>(o.bs, MODE) - ws;
+    const int ws = P == 2 ? weight_shift(a.st) : 0, same = kDlExp<T> - ws;
     const int most = most_of<T, P == 2 ? 3 : 1>(a.st, o.bs, o.up, cnt);
-    const float cs = MODE == kExpect && !std::is_same<T, bf16>::value ? ldexpf(1.f, -center_exp(o.bs)) : 1.f;
+    constexpr bool kScaled = !std::is_same<T, bf16>::value;
+    const Centers all = MODE == kExpect && kScaled ? o.bs->centers : Centers{0, 0};
     const int base = lds_chunk<kK, 16>(lane & 15, lane >> 4), frags = a.Vp / 16, q4 = (lane >> 4) * 4;
     const float* centers = reinterpret_cast<const float*>(lds + P * a.Vp * ND * 64);
     // transposing reads: lane i of a 16-lane group q starts at class 4 q + i / 4, feature 4 (i % 4)
@@ -1272,12 +1293,15 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
         const SlimRows<P, ND> r = next;
         const int n = b * 16 + (lane & 15), m = n < cnt ? n : cnt - 1;
         if (b + step < blocks) next.load(a, (b + step) * 16 + (lane & 15), cnt, lane);
-        const float tp = a.top[m], rs = a.inv_sum[m], e0 = MODE == kExpect ? a.mean[m] * cs : 0.f;
+        const float tp = a.top[m], rs = a.inv_sum[m], mean = MODE == kExpect ? a.mean[m] : 0.f;
+        const int ce = MODE == kExpect && kScaled ? center_exp(all, mean) : 0;
+        const float cs = ldexpf(1.f, -ce), e0 = mean * cs;
         const int target = MODE == kCE ? a.tgt[m] : -1, t = target - q4;
         float g = upstream(o.up, m, cnt);
         const int own = P == 2 ? a.shifts[m] : 0, shift = -ws - own;
-        const int ge = row_exp<T>(g), we = std::is_same<T, bf16>::value ? 0 : weight_exp(g, P == 2 ? kReachTop - own : 0, most);
-        g = ldexpf(g, std::is_same<T, bf16>::value ? 0 : kDlTop - ge);
+        const int ge = kScaled ? exp_above(fabsf(g)) : 0, re = ge + ce;
+        const int we = kScaled ? weight_exp(g, re, P == 2 ? kReachTop - own : 0, most) : 0;
+        if (kScaled) g = ldexpf(g, kDlTop - ge);
         if (MODE == kCE && target < 0) g = __builtin_nanf("");
         const float gr = g * rs;
         f32x4 acc[2 * ND];
@@ -1345,7 +1369,7 @@ __global__ __launch_bounds__(kSlimT) void slim_bwd_kernel(SlimArgs a, SlimBwd o)
 #pragma unroll
                 for (int i = 0; i < 2 * ND; ++i) {
                     const int c = i * 16 + (lane >> 4) * 4;
-                    const f32x4 x = scaled(acc[i], same + ge);
+                    const f32x4 x = scaled(acc[i], same + re);
                     const float y[4] = {x[0], x[1], x[2], x[3]};
                     if (c < a.D) put_row4(row, c, a.D, y);
                 }
@@ -1880,7 +1904,7 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
     const Saved s = saved_of(saved, N);
     const int* rows = mode == kCE ? s.rows : nullptr;
     BackState* bs = reinterpret_cast<BackState*>(ws + p.bs);
-    Upstream up{g, reduction == DS_REDUCE_NONE, reduction == DS_REDUCE_MEAN, rows};
+    Upstream up{g, reduction == DS_REDUCE_NONE, reduction == DS_REDUCE_MEAN, rows, mode == kExpect ? s.mean : nullptr};
     Operand H, W;
     char* keep = static_cast<char*>(saved);
     operands<IT, T, SPLIT>(p, mode, hidden, ldh, weight, N, D, V, s, rows, false, false, keep + p.sh, keep + p.sw, H, W, q);
@@ -1942,7 +1966,7 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
         }
         const Operand G{dl, ld, lo, (int)N, ld};
         if (g_hidden && !p.slim_back) {
-            const GradArgs ga{D, cols, p.dh_splits, mode, cols, v0 == 0, rows, g_hidden, dhp, N * D4, up, false};
+            const GradArgs ga{D, cols, p.dh_splits, cols, v0 == 0, rows, g_hidden, dhp, N * D4, up, false};
             if (two)
                 grad_launch<IT, T, kTwo, 0>(p.dh, p.dh_part, Wp, G, s, bs, N, ga, q);
             else
@@ -1950,27 +1974,27 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
         }
         if (g_weight) {
             IT* gw = g_weight + (long long)v0 * D;
-            const GradArgs ga{D, cols, p.dw_splits, mode, cols, 1, nullptr, gw, dwp, (long long)p.piece * D4, up, reach};
+            const GradArgs ga{D, cols, p.dw_splits, cols, 1, nullptr, gw, dwp, (long long)p.piece * D4, up, reach};
             if (two)
                 grad_launch<IT, T, kTwo, 1>(p.dw, p.dw_splits > 1, Hw, G, s, bs, cols, ga, q);
             else
                 grad_launch<IT, T, SPLIT, 1>(p.dw, p.dw_splits > 1, Hw, G, s, bs, cols, ga, q);
             if (p.dw_splits > 8 && (long long)cols * D4 <= kShareOuts)
                 head_sum_kernel<T, SPLIT, IT, 16><<<cdiv((long long)cols * D4 / 4, 16), 256, 0, q>>>(
-                    dwp, (long long)p.piece * D4, p.dw_splits, s.st, bs, cols, D, mode, 1, up, reach, nullptr, gw);
+                    dwp, (long long)p.piece * D4, p.dw_splits, s.st, bs, cols, D, 1, up, reach, nullptr, gw);
             else if (p.dw_splits > 1)
                 head_sum_kernel<T, SPLIT, IT, 1><<<cdiv((long long)cols * D4 / 4, 256), 256, 0, q>>>(
-                    dwp, (long long)p.piece * D4, p.dw_splits, s.st, bs, cols, D, mode, 1, up, reach, nullptr, gw);
+                    dwp, (long long)p.piece * D4, p.dw_splits, s.st, bs, cols, D, 1, up, reach, nullptr, gw);
         }
     }
     if (g_hidden && p.dh_part && !p.slim_back) {
         const bool many = p.dh_splits > 8 && N * D4 <= kShareOuts;
         const int blocks = cdiv(N * (D4 / 4), many ? 16 : 256), grid = blocks < 16384 ? blocks : 16384;
         if (many)
-            head_sum_kernel<T, SPLIT, IT, 16><<<grid, 256, 0, q>>>(dhp, N * D4, p.dh_splits, s.st, bs, (int)N, D, mode, 0, up, false, rows,
+            head_sum_kernel<T, SPLIT, IT, 16><<<grid, 256, 0, q>>>(dhp, N * D4, p.dh_splits, s.st, bs, (int)N, D, 0, up, false, rows,
                                                                    g_hidden);
         else
-            head_sum_kernel<T, SPLIT, IT, 1><<<grid, 256, 0, q>>>(dhp, N * D4, p.dh_splits, s.st, bs, (int)N, D, mode, 0, up, false, rows,
+            head_sum_kernel<T, SPLIT, IT, 1><<<grid, 256, 0, q>>>(dhp, N * D4, p.dh_splits, s.st, bs, (int)N, D, 0, up, false, rows,
                                                                   g_hidden);
     }
     return launched();

@@ -313,8 +313,9 @@ int ds_ingest_depth_u16(const uint16_t* depth, int N, int H, int W, float* out, 
  * contiguous, of type `dtype`; either may be NULL.  Results do not depend on scheduling: the same inputs give the same bits.
  * Numbers: fp32 inputs go through every product as two fp16 planes (22 bits; three products).  Rows of hidden have a power of two
  * each, so that a row's result does not depend on the others; the weight has one, and what is below 2^-16 of its largest
- * element loses bits, below 2^-40 all.  The logits' gradient has a power of two per row from the upstream value; in g_weight
- * a row counts relative to the one that reaches farthest (2^-39 of its part is lost).  16-bit inputs: the logits' gradient goes
+ * element loses bits, below 2^-40 all.  The logits' gradient has a power of two per row from the upstream value and, for the
+ * expectation, from |out| where the centres have one sign (from the largest centre where they do not); in g_weight a row counts
+ * relative to the one that reaches farthest (2^-39 of its part is lost).  16-bit inputs: the logits' gradient goes
  * into its products in two 16-bit planes up to N V D = 2^31 and on chip (g_weight: below 64 rows a class), in one beyond, which
  * leaves the gradients 1.2 to 1.5 times as far from exact as their rounding.
  * ds_*_eval: a forward that no backward follows; nothing is saved, and up to four rows read the weight as it is (in fp32: the

@@ -396,6 +396,59 @@ def test_weighted_out_rows_leave_no_trace(n, d, v, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("kind", ["log", "far", "negative", "mixed"])
+@pytest.mark.parametrize("n,d,v", [(4, 40, 500), (60, 40, 50), (200, 64, 900), (9000, 24, 40), (3000, 136, 1500)])
+def test_small_depths_beside_large_centers(n, d, v, kind, dtype):
+    """Centres over nine decades, or a last one of 1e12: rows that are sure of small ones keep their gradient's digits.  p (c - E) is
+    rounded relative to sum p |c| (centres of one sign) or, where signs differ, to the largest centre."""
+    g = torch.Generator().manual_seed(n + v)
+    w = (torch.randn(v, d, generator=g) / math.sqrt(d)).to(dtype).to(DEV)
+    cls = torch.randint(0, v - 1, (n,), generator=g)
+    h = (torch.randn(n, d, generator=g) + 8.0 * w.float().cpu()[cls] * math.sqrt(d / 8)).to(dtype).to(DEV)
+    c = torch.logspace(-6, 3, v).to(DEV)
+    if kind == "far":
+        w[-1] = -8 * h.float().mean(0).to(dtype) - 4 * w.abs().amax()
+        c = torch.linspace(1.0, 2.0, v).to(DEV)
+        c[-1] = 1e12
+        h = torch.cat([h[:, :-1].abs(), h[:, -1:].abs()], 1)       # the far class is out of reach: features and weight disagree
+        w[-1] = -(60.0 / h.float().sum(1).min()).clamp(min=1.0).to(dtype) * 2
+    if kind == "negative":
+        c = -c
+    if kind == "mixed":
+        c = c - 1e-4
+    up = (torch.rand(n, generator=g) + 0.5).to(DEV)
+    got = _ex(h, w, c, up)
+    H, W, C, U64 = h.double(), w.double(), c.double(), up.double()[:, None]
+    p = torch.softmax(H @ W.T, 1)
+    E = (p @ C)[:, None]
+    size = p @ C.abs()
+    split = 2.0 ** -21 if dtype == torch.float32 else 0.0
+    el = (split + (d + 4) * 2.0 ** -24) * (H.abs() @ W.abs().T)
+    ep = 2 * el.max(dim=1, keepdim=True).values + (v + 32) * 2.0 ** -24
+    tol = (ep[:, 0] * size) + 4 * 2.0 ** -24 * size
+    dl = p * (C[None] - E) * U64
+    ref = C.abs().max() if kind == "mixed" else size[:, None]
+    u = {torch.float32: 2.0 ** -21, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[dtype]
+    err = (p * (ep * (C[None] - E).abs() + tol[:, None] + 2.0 ** -23 * C.abs()[None])) * U64 + u * dl.abs()
+    if dtype != torch.bfloat16:
+        err = err + 2.0 ** -37 * ref * U64
+    out = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[dtype]
+    sub = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -24, torch.bfloat16: 2.0 ** -133}[dtype]
+    _close(got[0], E[:, 0], tol, "depth")
+    gh = dl @ W
+    fits = gh.abs() < torch.finfo(dtype).max / 2
+    th = (err + (split + (v + 8) * 2.0 ** -24) * dl.abs()) @ W.abs() + out * gh.abs() + sub
+    _close(torch.where(fits, got[1].double(), 0), torch.where(fits, gh, 0), th, "g_hidden")
+    gw = dl.T @ H
+    if dtype != torch.bfloat16 and kind != "mixed":      # dW is relative to the row that reaches farthest
+        err = err + 2.0 ** -37 * (size[:, None] * U64).max()
+    tw = (err + (split + (n + 8) * 2.0 ** -24) * dl.abs()).T @ H.abs() + out * gw.abs() + sub
+    fits = gw.abs() < torch.finfo(dtype).max / 2
+    _close(torch.where(fits, got[2].double(), 0), torch.where(fits, gw, 0), tw, "g_weight")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("reduction", ["none", "mean"])
 @pytest.mark.parametrize("n,d,v", [(20, 70, 500), (60, 40, 50), (200, 64, 900), (300, 515, 70), (9000, 24, 40), (3000, 136, 1500)])
 def test_float32_rows_do_not_see_each_other(n, d, v, reduction):
