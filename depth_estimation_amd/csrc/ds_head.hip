@@ -353,7 +353,8 @@ __global__ __launch_bounds__(256) void stage_kernel(Source s0, Source s1, int D,
         stage_rows<IT, T, SPLIT, VEC, kSame>(s, D, Dp, L);
         return;
     }
-    int reach = Dp <= L * VEC ? stage_rows<IT, T, SPLIT, VEC, kOwnKept>(s, D, Dp, L) : stage_rows<IT, T, SPLIT, VEC, kOwn>(s, D, Dp, L);
+    int reach = Dp <= L * VEC ? stage_rows<IT, T, SPLIT, VEC, kOwnKept>(s, D, Dp, L)
+                              : stage_rows<IT, T, SPLIT, VEC, kOwn>(s, D, Dp, L);
     if (SPLIT == 3 && s.reach) {
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) reach = max(reach, __shfl_xor(reach, o, 64));
@@ -1824,8 +1825,8 @@ int head_fwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
         : p.few == 2 ? few_launch<IT, 2>(p, hidden, ldh, weight, fa, q)
                      : few_launch<IT, 4>(p, hidden, ldh, weight, fa, q);
         const int step = p.few * 4;
-        join_few_kernel<<<1, 1024, 0, q>>>(JoinArgs{part, part + 1, part + 2, part + 3, step, 4, step, p.few_grid, mode, s.st, s.rows, s.tgt,
-                                                    s.top, s.inv_sum, s.mean, out, mode == kCE ? reduction : DS_REDUCE_NONE});
+        join_few_kernel<<<1, 1024, 0, q>>>(JoinArgs{part, part + 1, part + 2, part + 3, step, 4, step, p.few_grid, mode, s.st, s.rows,
+                                                    s.tgt, s.top, s.inv_sum, s.mean, out, mode == kCE ? reduction : DS_REDUCE_NONE});
         return launched();
     }
     Operand H, W;
@@ -1952,7 +1953,8 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
         Wp.outer = cols;
         if (p.slim_back) {
             const SlimArgs a = slim_args(p, H, W, s, rows, N, D, V, centers);
-            const SlimBwd o{bs, up, g_hidden, g_weight ? dl : nullptr, ld, p.dl_planes, lo, ignored, g_weight && p.pack ? ws + p.bh : nullptr, p.Dp};
+            const SlimBwd o{bs, up, g_hidden, g_weight ? dl : nullptr, ld, p.dl_planes, lo, ignored,
+                            g_weight && p.pack ? ws + p.bh : nullptr, p.Dp};
             const int rc = mode == kCE ? slim_bwd<T, SPLIT == 3 ? 2 : 1, kCE, IT>(p, a, o, q)
                                        : slim_bwd<T, SPLIT == 3 ? 2 : 1, kExpect, IT>(p, a, o, q);
             if (rc) return rc;
@@ -1960,9 +1962,11 @@ int head_bwd(const Plan& p, int mode, const IT* hidden, long long ldh, const IT*
         } else {
             const DlArgs da{v0, cols, s.shifts, s.tgt, centers, s.top, s.inv_sum, s.mean, up, dl, ld, lo};
             if (two)
-                mode == kCE ? dl_launch<T, kTwo, kCE>(p, Wp, H, s, bs, N, D, da, q) : dl_launch<T, kTwo, kExpect>(p, Wp, H, s, bs, N, D, da, q);
+                mode == kCE ? dl_launch<T, kTwo, kCE>(p, Wp, H, s, bs, N, D, da, q)
+                            : dl_launch<T, kTwo, kExpect>(p, Wp, H, s, bs, N, D, da, q);
             else
-                mode == kCE ? dl_launch<T, SPLIT, kCE>(p, Wp, H, s, bs, N, D, da, q) : dl_launch<T, SPLIT, kExpect>(p, Wp, H, s, bs, N, D, da, q);
+                mode == kCE ? dl_launch<T, SPLIT, kCE>(p, Wp, H, s, bs, N, D, da, q)
+                            : dl_launch<T, SPLIT, kExpect>(p, Wp, H, s, bs, N, D, da, q);
         }
         const Operand G{dl, ld, lo, (int)N, ld};
         if (g_hidden && !p.slim_back) {

@@ -9,8 +9,8 @@
 // follow from the coefficients alone: singular values begin in [0, 1], so how far each step can take them is known before it
 // (steps_of), and entries are at most as large as the largest singular value.
 //
-// bf16 results of larger matrices after few steps need less, and take half the products (Light): A keeps one plane (11 bits) off the diagonal,
-// where its entries are small, and its diagonal in fp32 beside it.  B keeps one plane; what its diagonal, which carries most of
+// bf16 results of larger matrices after few steps need less, and take half the products (Light): A keeps one plane (11 bits) off
+// the diagonal, where its entries are small, and its diagonal in fp32 beside it.  B keeps one plane; what its diagonal, which carries most of
 // X, lost by that is made up for as a factor of the result's row: diag(d) X (1 + rounding) off the diagonal is the smaller part.
 // X keeps two planes where it is multiplied by B.  What that costs after five steps is 4e-4 .. 9e-4 of the result's norm (sides
 // of 256 and more; Gaussian, decaying and nearly low-rank matrices, written out in float64), under the 1.7e-3 that rounding the
@@ -32,7 +32,7 @@ constexpr float kXs = 8192.f;    // stored X = 2^13 X where singular values are 
 // stored; B with its bound |a| + |b| A + |c| A^2 in (2^14, 2^15].
 struct Step {
     float gram;          // accumulated X X^T -> stored A
-    float ca, cb, cc;    // accumulated A A, stored A, and the identity -> stored B
+    float ca, cb, cc;    // the identity, stored A and accumulated A A -> stored B
     float next;          // accumulated B X -> the next stored X, or after the last step X itself
 };
 struct Steps {
